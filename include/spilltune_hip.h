@@ -313,6 +313,34 @@ int st_rope_qkv_norm_bwd(const uint16_t* dq, const uint16_t* dk, const uint16_t*
                          const uint16_t* wq, const uint16_t* wk, const float* rstd, int64_t B,
                          int64_t S, int64_t heads, int64_t kv_heads, int64_t D, uint16_t* dx,
                          int64_t lddx, st_stream_t stream);
+/*
+ * Rotary embedding of a fused q|k|v projection output by per-token positions,
+ * with the relayout to heads, for packed rows and long contexts.  No
+ * counterpart in the reference, whose positions are 0..S-1 in fp32 and bf16
+ * tables (dense.py:232-248).  x rows (stride ldx) hold heads*D query, kv_heads*D
+ * key and kv_heads*D value columns; q [B,heads,S,D], k and v [B,kv_heads,S,D].
+ * positions [B,S] int32 (pos64 = 0) or int64; inv_freq [rotary_dim/2] fp64 on
+ * the device; cos and sin are amplitude * cos/sin(position * inv_freq), the
+ * angle formed and reduced in fp64.  The first rotary_dim columns of each head
+ * turn (even, at most D and 256), as pairs (i, i + rotary_dim/2) or, with
+ * interleave, (2i, 2i+1).  wq, wk: NULL, or [D] weights of an RMS norm of each
+ * query and key head before the rotation (D = 64, 128 or 256; rstd
+ * [B*S, heads+kv_heads] is then written for the backward).  fp32 arithmetic,
+ * one rounding.  D a multiple of 8 up to 512, 16-byte aligned operands.
+ */
+int st_rope_pos_fwd(const uint16_t* x, int64_t ldx, const void* positions, int32_t pos64,
+                    const double* inv_freq, double amplitude, int64_t B, int64_t S, int64_t heads,
+                    int64_t kv_heads, int64_t D, int64_t rotary_dim, int32_t interleave,
+                    const uint16_t* wq, const uint16_t* wk, float eps, uint16_t* q, uint16_t* k,
+                    uint16_t* v, float* rstd, st_stream_t stream);
+/* VJP: head-major dq, dk, dv -> dx rows of stride lddx.  x (the forward's rows)
+ * and rstd are read with norms only. */
+int st_rope_pos_bwd(const uint16_t* dq, const uint16_t* dk, const uint16_t* dv, const uint16_t* x,
+                    int64_t ldx, const void* positions, int32_t pos64, const double* inv_freq,
+                    double amplitude, int64_t B, int64_t S, int64_t heads, int64_t kv_heads,
+                    int64_t D, int64_t rotary_dim, int32_t interleave, const uint16_t* wq,
+                    const uint16_t* wk, const float* rstd, uint16_t* dx, int64_t lddx,
+                    st_stream_t stream);
 /* [B,heads,S,D] -> [B,S,heads*D] copy (attention output relayout). */
 int st_heads_to_tokens(const uint16_t* x, int64_t B, int64_t S, int64_t heads, int64_t D,
                        uint16_t* out, st_stream_t stream);
@@ -404,6 +432,40 @@ int st_mla_attn_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v,
                     int64_t S, int64_t H, int64_t DQ, int64_t DV, float scale,
                     const int32_t* kv_len, uint16_t* dq, uint16_t* dk, uint16_t* dv,
                     void* workspace, int64_t workspace_bytes, st_stream_t stream);
+
+/* ---------------------------------------------------------------------
+ * Attention over runs of keys: query i of row b sees the keys
+ * [key_start[b,i], key_end[b,i]) (int32 [B,S], clamped to [0,S]; an empty run
+ * sees nothing): packed documents, bidirectional runs, sliding windows and
+ * padding.  No counterpart in the reference, whose mask is causal with right
+ * padding (dense.py:236-247).  cap > 0 replaces each score s = scale * q.k by
+ * cap * tanh(s / cap); slopes (NULL or fp32 [H]) then subtracts
+ * slopes[h] * |i - j|.  Layouts as st_flash_attn_*: q [B,H,S,DQ], k
+ * [B,Hkv,S,DQ], v [B,Hkv,S,DV], out and dout token-major [B,S,H*DV], lse
+ * [B,H,S] base-2 log-sum-exp; (DQ, DV) = (64, 64), (128, 128) or (192, 128).
+ * A query with an empty run has out = 0, lse = +inf and a zero dq, whatever its
+ * rows hold; infinities and NaN in rows that a query does not see do not reach
+ * it.  scale > 0.  Deterministic: no atomics.
+ * `plan`: st_span_plan's tables of the same key_start and key_end, made once
+ * per mask and read by every call (st_span_plan_bytes(B, S), 16-byte aligned);
+ * it belongs to that mask alone.
+ * --------------------------------------------------------------------- */
+int64_t st_span_plan_bytes(int64_t B, int64_t S);
+int st_span_plan(const int32_t* key_start, const int32_t* key_end, int64_t B, int64_t S, void* plan,
+                 int64_t plan_bytes, st_stream_t stream);
+int64_t st_span_attn_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t DQ,
+                                     int64_t DV, int32_t backward);
+int st_span_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B, int64_t S,
+                     int64_t H, int64_t Hkv, int64_t DQ, int64_t DV, float scale, float cap,
+                     const float* slopes, const int32_t* key_start, const int32_t* key_end,
+                     const void* plan, uint16_t* out, float* lse, void* workspace,
+                     int64_t workspace_bytes, st_stream_t stream);
+int st_span_attn_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* out,
+                     const float* lse, const uint16_t* dout, int64_t B, int64_t S, int64_t H,
+                     int64_t Hkv, int64_t DQ, int64_t DV, float scale, float cap,
+                     const float* slopes, const int32_t* key_start, const int32_t* key_end,
+                     const void* plan, uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace,
+                     int64_t workspace_bytes, st_stream_t stream);
 
 /* ---------------------------------------------------------------------
  * Plain bf16 linear (router logits and their input gradient).

@@ -28,6 +28,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -101,6 +102,17 @@ _SIGNATURES = {
                                _P]),
     "st_mla_attn_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P, _P,
                                _P, _P, _P, _I64, _P]),
+    "st_rope_pos_fwd": (_I32, [_P, _I64, _P, _I32, _P, _D, _I64, _I64, _I64, _I64, _I64, _I64, _I32,
+                               _P, _P, _F, _P, _P, _P, _P, _P]),
+    "st_rope_pos_bwd": (_I32, [_P, _P, _P, _P, _I64, _P, _I32, _P, _D, _I64, _I64, _I64, _I64, _I64,
+                               _I64, _I32, _P, _P, _P, _P, _I64, _P]),
+    "st_span_plan_bytes": (_I64, [_I64, _I64]),
+    "st_span_plan": (_I32, [_P, _P, _I64, _I64, _P, _I64, _P]),
+    "st_span_attn_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I32]),
+    "st_span_attn_fwd": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _F, _P, _P, _P,
+                                _P, _P, _P, _P, _I64, _P]),
+    "st_span_attn_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _F,
+                                _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "st_cross_entropy_rows": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _F, _P, _P]),
     "st_moe_lora_grads": (_I32, [_I64, _I32, _I64, _I32, _P, _I64, _I64, _P, _P, _I64, _I64, _P,
                                  _I32, _F, _P, _I64, _I64, _I64, _I32, _P]),

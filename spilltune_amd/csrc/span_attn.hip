@@ -1,0 +1,1228 @@
+// Attention in which query i of a row sees the keys [key_start[i], key_end[i]):
+// packed documents, bidirectional runs inside them, sliding windows, padding
+// (an empty run) -- and, optionally, scores capped by a tanh and a bias that
+// falls with the distance.  Forward and deterministic backward.
+//
+//   x[i,j] = cap * tanh(scale * q_i.k_j / cap) - slope[h] * |i - j|
+//   P[i,:] = softmax of x[i,:] over the seen keys,   o_i = sum_j P[i,j] v_j
+//   dP = dO V^T,  delta_i = dO_i . o_i,  dx = P (dP - delta)
+//   dS = dx * (1 - tanh^2),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
+//
+// Layout as the causal kernels (attention.hip): q [B,H,S,DQ], k [B,Hkv,S,DQ],
+// v [B,Hkv,S,DV] head-major bf16, out and dout token-major [B,S,H*DV], lse
+// [B,H,S] fp32 the base-2 log-sum-exp (+inf for a query that sees no key, so
+// every probability recomputed from it is 0).  Scores, statistics and sums are
+// fp32; probabilities and dS are rounded to bf16 for their MFMA products.
+//
+// A plan (span_plan below, made once per mask) holds for each 32-query block
+// the extremes of its runs, for each 128-key tile the query blocks that see it,
+// and the tiles by falling work, so a workgroup walks only the tiles that some
+// of its queries see and the long ones start first.
+//
+// Masked places never reach a result: a masked score is replaced, not added to,
+// but an infinity or NaN in a key, value or gradient row that a 32-row block
+// partly sees does meet a zero probability inside an MFMA product.  A wave that
+// ends with a sum that is not finite says so in a flag, and `span_fix_*` redoes
+// those rows over the seen pairs alone.
+#include <algorithm>
+#include <cmath>
+
+#include "attn_tile.h"
+
+namespace {
+
+using namespace attn;
+
+constexpr int NT = 256;
+constexpr int TILE = 128;  // queries (dQ, forward) or keys (dK, dV) per workgroup
+constexpr int BKT = 64;    // keys per step of the forward and dQ passes
+constexpr int QT = 64;     // queries per step of the dK/dV pass
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_LOG2 = 8.0f;  // the running maximum may lag by up to 2^8
+
+// ---------------------------------------------------------------- plan
+// Int32 regions, in order: blocks int4 [B, nb] (least and greatest run start,
+// least and greatest run end of 32 queries; an empty run makes the greatest
+// start INT_MAX and the least end 0, so the block is never taken for wholly
+// visible), key tiles int2 [B, nt] (first query block that sees the tile, end),
+// query and key tiles by falling work [B*nt] each, and their work [B*nt] each.
+struct Plan {
+  const int4* blk;
+  const int2* keys;
+  const int32_t *qorder, *korder;
+  int32_t *qwork, *kwork;
+  int nb, nt;
+  int64_t bytes;
+};
+Plan plan_of(const void* base, int64_t B, int64_t S) {
+  Plan p;
+  const int64_t nb = st::cdiv(S, 32), nt = st::cdiv(S, TILE);
+  int32_t* w = (int32_t*)base;
+  p.nb = (int)nb;
+  p.nt = (int)nt;
+  p.blk = (const int4*)w;
+  w += 4 * B * nb;
+  p.keys = (const int2*)w;
+  w += 2 * B * nt;
+  p.qorder = w;
+  w += B * nt;
+  p.korder = w;
+  w += B * nt;
+  p.qwork = w;
+  w += B * nt;
+  p.kwork = w;
+  w += B * nt;
+  p.bytes = (char*)w - (char*)base;
+  return p;
+}
+
+__device__ __forceinline__ int2 run_of(const int32_t* __restrict__ lo, const int32_t* __restrict__ hi,
+                                       int64_t at, int S) {
+  const int a = min(max(lo[at], 0), S), z = min(max(hi[at], 0), S);
+  return a < z ? make_int2(a, z) : make_int2(0, 0);
+}
+
+// one 32-lane half per block of 32 queries
+__global__ __launch_bounds__(NT) void span_blocks(const int32_t* __restrict__ lo,
+                                                  const int32_t* __restrict__ hi, int S, int nb,
+                                                  int64_t total, int4* __restrict__ blk) {
+  const int64_t id = ((int64_t)blockIdx.x * NT + threadIdx.x) >> 5;
+  if (id >= total) return;
+  const int64_t b = id / nb;
+  const int i = (int)(id % nb) * 32 + (threadIdx.x & 31);
+  int2 r = i < S ? run_of(lo, hi, b * S + i, S) : make_int2(0, 0);
+  const bool some = r.x < r.y;
+  int4 x = some ? make_int4(r.x, r.x, r.y, r.y) : make_int4(INT_MAX, INT_MAX, 0, 0);
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) {
+    x.x = min(x.x, __shfl_xor(x.x, d));
+    x.y = max(x.y, __shfl_xor(x.y, d));
+    x.z = min(x.z, __shfl_xor(x.z, d));
+    x.w = max(x.w, __shfl_xor(x.w, d));
+  }
+  if ((threadIdx.x & 31) == 0) blk[id] = x;
+}
+
+// per 128-row tile: the work of its queries, and the query blocks that see it as keys
+__global__ __launch_bounds__(64) void span_tiles(const int4* __restrict__ blk, int nb, int nt,
+                                                 int2* __restrict__ keys, int32_t* __restrict__ qwork,
+                                                 int32_t* __restrict__ kwork) {
+  const int64_t t = blockIdx.x;
+  const int64_t b = t / nt;
+  const int k0 = (int)(t % nt) * TILE, lane = threadIdx.x;
+  const int4* row = blk + b * nb;
+  int first = INT_MAX, end = 0;
+  for (int i = lane; i < nb; i += 64) {
+    const int4 x = row[i];
+    if (x.x < k0 + TILE && x.w > k0) {
+      first = min(first, i);
+      end = max(end, i + 1);
+    }
+  }
+  const int q = (int)(t % nt) * 4 + lane;
+  int a = INT_MAX, z = 0;
+  if (lane < 4 && q < nb) {
+    a = row[q].x;
+    z = row[q].w;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    first = min(first, __shfl_xor(first, d));
+    end = max(end, __shfl_xor(end, d));
+    a = min(a, __shfl_xor(a, d));
+    z = max(z, __shfl_xor(z, d));
+  }
+  if (lane == 0) {
+    keys[t] = first < end ? make_int2(first, end) : make_int2(0, 0);
+    kwork[t] = first < end ? end - first : 0;
+    qwork[t] = a < z ? z - a : 0;
+  }
+}
+
+// tiles by falling work (ties by index): each counts those before it; more
+// tiles than `sorted` keep their own order (the count is quadratic)
+__global__ __launch_bounds__(NT) void span_order(const int32_t* __restrict__ qwork,
+                                                 const int32_t* __restrict__ kwork, int64_t n,
+                                                 int sorted, int32_t* __restrict__ qorder,
+                                                 int32_t* __restrict__ korder) {
+  const int32_t* w = blockIdx.y ? kwork : qwork;
+  int32_t* o = blockIdx.y ? korder : qorder;
+  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+  if (i >= n) return;
+  if (!sorted) {
+    o[i] = (int32_t)i;
+    return;
+  }
+  const int mine = w[i];
+  int64_t rank = 0;
+  for (int64_t j = 0; j < n; ++j) rank += w[j] > mine || (w[j] == mine && j < i);
+  o[rank] = (int32_t)i;
+}
+constexpr int64_t SORT_LIMIT = 16384;
+
+// ---------------------------------------------------------------- shared
+struct Args {
+  const uint16_t *q, *k, *v;
+  const int32_t *lo, *hi;
+  const float* slopes;  // [H] or NULL
+  Plan plan;
+  int S, H, Hkv;
+  float scale, sl2;          // scale, scale * log2(e)
+  float cap_in, cap_out;     // MODE 1 with a cap: 2 log2(e) scale / cap, cap * log2(e); else 0
+};
+
+// Workgroup head index -> head, so that the query heads of a KV head share an
+// XCD (blocks go to the 8 XCDs in turn) and its L2 holds that KV head's rows.
+__device__ __forceinline__ int head_of(int x, int H, int Hkv) {
+  if (Hkv % 8) return x;
+  const int group = H / Hkv, y = x / 8;
+  return (x % 8 + 8 * (y / group)) * group + y % group;
+}
+
+// Base-2 score of a raw product s at distance `far` (>= 0); `grad`: d x / d (scale s).
+__device__ __forceinline__ float score(const Args& a, float slope2, float s, float far, float& grad) {
+  grad = 1.0f;
+  float x = s * a.sl2;
+  if (a.cap_in != 0.0f) {
+    // tanh(y) = 1 - 2 r, r = 1 / (1 + e^2y); absolute error of a few 2^-24
+    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.cap_in));
+    x = __builtin_fmaf(-2.0f * a.cap_out, r, a.cap_out);
+    grad = 4.0f * r * (1.0f - r);
+  }
+  return __builtin_fmaf(-slope2, far, x);
+}
+
+__device__ __forceinline__ bool finite(float x) { return x - x == 0.0f; }
+
+// copies of the K and V tiles of a step, as RowCopy lays them out
+template <int D, int NTHR, int ROWS>
+struct TileCopy {
+  using C = RowCopy<D, NTHR>;
+  static constexpr int PER = ROWS * D / 8 / NTHR;
+  static_assert(PER * NTHR * 8 == ROWS * D, "tiles are whole thread copies");
+  uint32_t off[C::uniform ? 1 : PER];
+  __device__ __forceinline__ TileCopy(int tid, int64_t ld) {
+#pragma unroll
+    for (int i = 0; i < (C::uniform ? 1 : PER); ++i) {
+      const int P = i * NTHR + tid, row = P / (D / 8);
+      off[i] = (uint32_t)(row * ld + ((P % (D / 8)) ^ swz<D>(row)) * 8) * 2;
+    }
+  }
+  // rows [r0, r0 + ROWS) of a [n][ld] matrix at `base` (rows past n read zeros)
+  __device__ __forceinline__ void operator()(const uint16_t* base, int64_t ld, int r0, int n,
+                                             uint16_t* tile, int wave) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = r0 + (C::uniform ? i * C::rows : 0);
+      const int left = min(max(n - r, 0), C::uniform ? C::rows : ROWS);
+      const int64_t bytes = left > 0 ? ((left - 1) * ld + D) * 2 : 0;
+      b2lds16(st::make_rsrc(base + (int64_t)r * ld, bytes), off[C::uniform ? 0 : i],
+              tile + (i * NTHR + wave * 64) * 8);
+    }
+  }
+};
+
+// O^T or dQ^T accumulators of a wave's 32 queries -> rows of `out` (row stride
+// ld) through the wave's own LDS space; rows for which `keep` is false get zeros
+template <int D>
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float mul, bool keep,
+                                           uint16_t* os, int lane, int rows, uint16_t* out,
+                                           int64_t ld) {
+  constexpr int LDO = D + 8;
+  const int g = lane >> 5, c = lane & 31;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int v4 = 0; v4 < 4; ++v4) {
+      const int d = db * 32 + v4 * 8 + g * 4;
+      u32x2 w = {st::pack_bf16x2(acc[db][4 * v4] * mul, acc[db][4 * v4 + 1] * mul),
+                 st::pack_bf16x2(acc[db][4 * v4 + 2] * mul, acc[db][4 * v4 + 3] * mul)};
+      if (!keep) w = u32x2{0, 0};
+      *(u32x2*)(os + c * LDO + d) = w;
+    }
+  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_wave_barrier();  // each wave reads back only its own rows
+  for (int i = lane; i < 32 * (D / 8); i += 64) {
+    const int r = i / (D / 8), ch = i % (D / 8);
+    if (r < rows) {
+      const u32x2 a = *(const u32x2*)(os + r * LDO + ch * 8);
+      const u32x2 b = *(const u32x2*)(os + r * LDO + ch * 8 + 4);
+      *(uint4*)(out + r * ld + ch * 8) = make_uint4(a.x, a.y, b.x, b.y);
+    }
+  }
+}
+
+// a value that every lane of the wave holds alike, in scalar registers
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int4 uniform(int4 x) {
+  return make_int4(uniform(x.x), uniform(x.y), uniform(x.z), uniform(x.w));
+}
+
+// Key range of a 128-query tile and the wave's own block of extremes.
+struct Walk {
+  int4 mine;       // of this wave's 32 queries
+  int first, end;  // keys that some query of the tile sees
+};
+__device__ __forceinline__ Walk walk_of(const Plan& p, int b, int qt, int wave) {
+  Walk w{make_int4(INT_MAX, INT_MAX, 0, 0), INT_MAX, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = qt * 4 + i;
+    if (n >= p.nb) break;
+    const int4 x = uniform(p.blk[(int64_t)b * p.nb + n]);
+    w.first = min(w.first, x.x);
+    w.end = max(w.end, x.w);
+    if (i == wave) w.mine = x;
+  }
+  return w;
+}
+
+// ---------------------------------------------------------------- forward
+// 4 waves of 32 queries over steps of 64 keys from the first key that the tile
+// sees; K and V tiles [key][D] in LDS, two buffers, one barrier a step.  Every
+// MFMA tile is S^T = K Q^T (a lane owns a query column), O^T += V^T P^T with
+// V^T read by the transposing LDS loads.
+template <int DQ, int DV, int MODE>
+__global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__ out,
+                                                  float* __restrict__ lse,
+                                                  int32_t* __restrict__ flags) {
+  constexpr int DS = DQ / 16, DB = DV / 32, LK = BKT * DQ, LV = BKT * DV;
+  static_assert(4 * 32 * (DV + 8) <= 2 * (LK + LV), "output staging fits");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * (LK + LV)];
+  const int S = a.S, H = a.H;
+  const int id = uniform(a.plan.qorder[blockIdx.x / H]), h = head_of(blockIdx.x % H, H, a.Hkv);
+  const int b = id / a.plan.nt, qt = id % a.plan.nt;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, c = lane & 31, hk = h / (H / a.Hkv);
+  const uint16_t* qb = a.q + (int64_t)(b * H + h) * S * DQ;
+  const uint16_t* kb = a.k + (int64_t)(b * a.Hkv + hk) * S * DQ;
+  const uint16_t* vb = a.v + (int64_t)(b * a.Hkv + hk) * S * DV;
+  const int q0 = qt * TILE + wave * 32, myq = q0 + c;
+  const Walk w = walk_of(a.plan, b, qt, wave);
+  const int2 run = myq < S ? run_of(a.lo, a.hi, (int64_t)b * S + myq, S) : make_int2(0, 0);
+  const float slope2 = MODE && a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+
+  bf16x8 qf[DS];
+#pragma unroll
+  for (int s = 0; s < DS; ++s)
+    qf[s] = as_bf16x8(myq < S ? ld_global16(qb + (int64_t)myq * DQ + 16 * s + 8 * g)
+                              : make_uint4(0, 0, 0, 0));
+  f32x16 oacc[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) oacc[i][v] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  const TileCopy<DQ, NT, BKT> ck(tid, DQ);
+  const TileCopy<DV, NT, BKT> cv(tid, DV);
+  auto issue = [&](int k0, int buf) {
+    uint16_t* ks = lds + buf * (LK + LV);
+    ck(kb, DQ, k0, S, ks, wave);
+    cv(vb, DV, k0, S, ks + LK, wave);
+  };
+  if (w.first < w.end) issue(w.first, 0);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = w.first; k0 < w.end; k0 += BKT, buf ^= 1) {
+    if (k0 + BKT < w.end) issue(k0 + BKT, buf ^ 1);
+    const uint16_t* ks = lds + buf * (LK + LV);
+    const uint16_t* vs = ks + LK;
+    if (k0 < w.mine.w && k0 + BKT > w.mine.x) {  // some query of the wave sees some key
+      const bool edge = k0 < w.mine.y || k0 + BKT > w.mine.z;  // wave-uniform
+      f32x16 sacc[2];
+#pragma unroll
+      for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sacc[jb][v] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+          sacc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_row<DQ>(ks, jb * 32 + c, s, g),
+                                                             qf[s], sacc[jb], 0, 0, 0);
+      if constexpr (MODE == 1) {
+        const float far0 = (float)(myq - k0 - 4 * g);
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            float grad;
+            sacc[jb][v] = score(a, slope2, sacc[jb][v],
+                                fabsf(far0 - (float)(jb * 32 + (v >> 2) * 8 + (v & 3))), grad);
+          }
+      }
+      if (edge) {
+        const int base = run.x - k0 - 4 * g;
+        const unsigned width = (unsigned)(run.y - run.x);
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            sacc[jb][v] = (unsigned)(jb * 32 + (v >> 2) * 8 + (v & 3) - base) < width
+                              ? sacc[jb][v] : -INFINITY;
+      }
+      const float mul = MODE == 1 ? 1.0f : a.sl2;
+      float mt = sacc[0][0];
+#pragma unroll
+      for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mt = fmaxf(mt, sacc[jb][v]);
+      mt = fmaxf(mt, __shfl_xor(mt, 32)) * mul;
+      if (__ballot(mt > m_run + RESCALE_LOG2)) {
+        const float m_new = fmaxf(m_run, mt);
+        // a row with no key yet: -inf - -inf is not a number, its sums are 0
+        const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) oacc[i][v] *= alpha;
+        l_run *= alpha;
+        m_run = m_new;
+      }
+      const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+      bf16x8 pf[4];
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(
+              __builtin_fmaf(sacc[cc >> 1][8 * (cc & 1) + e], mul, -m_use));
+          l_run += p[e];
+        }
+        pf[cc] = as_bf16x8(make_uint4(st::pack_bf16x2(p[0], p[1]), st::pack_bf16x2(p[2], p[3]),
+                                      st::pack_bf16x2(p[4], p[5]), st::pack_bf16x2(p[6], p[7])));
+      }
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_tr<DV>(vs, cc * 16, db * 32, lane),
+                                                             pf[cc], oacc[db], 0, 0, 0);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+
+  const float l_tot = l_run + __shfl_xor(l_run, 32);
+  const bool some = run.x < run.y;
+  if (g == 0 && myq < S)
+    lse[(int64_t)(b * H + h) * S + myq] = some ? m_run + log2f(l_tot) : INFINITY;
+  float probe = 0.0f;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) probe = __builtin_fmaf(oacc[i][v], 0.0f, probe);
+  const bool bad = __ballot(some && !(probe == 0.0f && finite(l_tot) && l_tot > 0.0f)) != 0;
+  if (lane == 0 && q0 < S)
+    flags[(int64_t)(b * H + h) * a.plan.nb + (q0 >> 5)] = bad;
+  store_rows<DV>(oacc, 1.0f / l_tot, some, lds + wave * 32 * (DV + 8), lane, S - q0,
+                 out + ((int64_t)b * S + q0) * H * DV + (int64_t)h * DV, (int64_t)H * DV);
+}
+
+// ---------------------------------------------------------------- backward
+// dQ (and delta) of a 128-query tile: S^T and dP^T = V dO^T as in the forward,
+// dQ^T += K^T dS^T.
+template <int DQ, int DV, int MODE>
+__global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __restrict__ o,
+                                                     const uint16_t* __restrict__ dout,
+                                                     const float* __restrict__ lse,
+                                                     float* __restrict__ delta,
+                                                     uint16_t* __restrict__ dq,
+                                                     int32_t* __restrict__ flags) {
+  constexpr int DSQ = DQ / 16, DSV = DV / 16, DB = DQ / 32, LK = BKT * DQ, LV = BKT * DV;
+  static_assert(4 * 32 * (DQ + 8) <= 2 * (LK + LV), "output staging fits");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * (LK + LV)];
+  const int S = a.S, H = a.H;
+  const int id = uniform(a.plan.qorder[blockIdx.x / H]), h = head_of(blockIdx.x % H, H, a.Hkv);
+  const int b = id / a.plan.nt, qt = id % a.plan.nt;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, c = lane & 31, hk = h / (H / a.Hkv);
+  const int64_t ldt = (int64_t)H * DV;
+  const uint16_t* qb = a.q + (int64_t)(b * H + h) * S * DQ;
+  const uint16_t* kb = a.k + (int64_t)(b * a.Hkv + hk) * S * DQ;
+  const uint16_t* vb = a.v + (int64_t)(b * a.Hkv + hk) * S * DV;
+  const int q0 = qt * TILE + wave * 32, myq = q0 + c;
+  const bool qok = myq < S;
+  const Walk w = walk_of(a.plan, b, qt, wave);
+  const int2 run = qok ? run_of(a.lo, a.hi, (int64_t)b * S + myq, S) : make_int2(0, 0);
+  const float slope2 = MODE && a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+  const int64_t srow = (int64_t)(b * H + h) * S;
+  const int64_t trow = ((int64_t)b * S + myq) * ldt + (int64_t)h * DV;
+
+  bf16x8 qf[DSQ], dof[DSV];
+  float dl = 0.0f;
+  const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int s = 0; s < DSQ; ++s)
+    qf[s] = as_bf16x8(qok ? ld_global16(qb + (int64_t)myq * DQ + 16 * s + 8 * g) : z);
+#pragma unroll
+  for (int s = 0; s < DSV; ++s) {
+    const int d = 16 * s + 8 * g;
+    const uint4 gv = qok ? ld_global16(dout + trow + d) : z;
+    const uint4 ov = qok ? ld_global16(o + trow + d) : z;
+    dof[s] = as_bf16x8(gv);
+    const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, ow[4] = {ov.x, ov.y, ov.z, ov.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      dl += st::bf16_to_f32((uint16_t)(gw[e >> 1] >> (16 * (e & 1)))) *
+            st::bf16_to_f32((uint16_t)(ow[e >> 1] >> (16 * (e & 1))));
+  }
+  dl += __shfl_xor(dl, 32);
+  if (g == 0 && qok) delta[srow + myq] = dl;
+  const float lq = qok ? lse[srow + myq] : INFINITY;
+
+  f32x16 dqacc[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dqacc[i][e] = 0.0f;
+
+  const TileCopy<DQ, NT, BKT> ck(tid, DQ);
+  const TileCopy<DV, NT, BKT> cv(tid, DV);
+  auto issue = [&](int k0, int buf) {
+    uint16_t* ks = lds + buf * (LK + LV);
+    ck(kb, DQ, k0, S, ks, wave);
+    cv(vb, DV, k0, S, ks + LK, wave);
+  };
+  if (w.first < w.end) issue(w.first, 0);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = w.first; k0 < w.end; k0 += BKT, buf ^= 1) {
+    if (k0 + BKT < w.end) issue(k0 + BKT, buf ^ 1);
+    const uint16_t* ks = lds + buf * (LK + LV);
+    const uint16_t* vs = ks + LK;
+#pragma unroll
+    for (int jb = 0; jb < 2; ++jb) {
+      const int kb0 = k0 + jb * 32;
+      if (kb0 >= w.mine.w || kb0 + 32 <= w.mine.x) continue;  // wave-uniform
+      const bool edge = kb0 < w.mine.y || kb0 + 32 > w.mine.z;
+      // an edge keeps the offsets of the lane's run, other blocks keep all
+      const int base = edge ? run.x - kb0 - 4 * g : 0;
+      const unsigned width = edge ? (unsigned)(run.y - run.x) : 32u;
+      const float far0 = (float)(myq - kb0 - 4 * g);
+      f32x16 sacc, pacc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) { sacc[e] = 0.0f; pacc[e] = 0.0f; }
+#pragma unroll
+      for (int s = 0; s < DSQ; ++s) {
+        sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_row<DQ>(ks, jb * 32 + c, s, g), qf[s],
+                                                       sacc, 0, 0, 0);
+        if (s < DSV)
+          pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_row<DV>(vs, jb * 32 + c, s, g),
+                                                         dof[s < DSV ? s : 0], pacc, 0, 0, 0);
+      }
+      bf16x8 dsf[2];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        float ds[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int vv = 8 * hh + e, ro = (vv >> 2) * 8 + (vv & 3);
+          float d;
+          if constexpr (MODE == 1) {
+            float grad;
+            const float x = score(a, slope2, sacc[vv], fabsf(far0 - (float)ro), grad);
+            d = __builtin_amdgcn_exp2f(x - lq) * (pacc[vv] - dl) * grad;
+          } else {
+            d = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[vv], a.sl2, -lq)) * (pacc[vv] - dl);
+          }
+          ds[e] = (unsigned)(ro - base) < width ? d : 0.0f;
+        }
+        dsf[hh] = as_bf16x8(make_uint4(st::pack_bf16x2(ds[0], ds[1]), st::pack_bf16x2(ds[2], ds[3]),
+                                       st::pack_bf16x2(ds[4], ds[5]), st::pack_bf16x2(ds[6], ds[7])));
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          dqacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              tile_tr<DQ>(ks, jb * 32 + 16 * hh, db * 32, lane), dsf[hh], dqacc[db], 0, 0, 0);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+  const bool some = run.x < run.y;
+  float probe = 0.0f;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) probe = __builtin_fmaf(dqacc[i][e], 0.0f, probe);
+  const bool bad = __ballot(some && probe != 0.0f) != 0;
+  if (lane == 0 && q0 < S) flags[(int64_t)(b * H + h) * a.plan.nb + (q0 >> 5)] = bad;
+  store_rows<DQ>(dqacc, a.scale, some, lds + wave * 32 * (DQ + 8), lane, S - q0,
+                 dq + (srow + q0) * DQ, DQ);
+}
+
+// dK, dV of a 128-key tile of one KV head over the query heads of one part of
+// its group: steps of 64 queries of each head in turn, from the first query
+// block that sees the tile.  S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T +=
+// Q^T dS.  The whole group in one workgroup needs no partial sums in memory;
+// `parts` > 1 splits the group where that leaves CUs idle, and the parts' fp32
+// sums are added in order by span_reduce.
+// DQ <= 128: 8 waves (4 key quarters x 2 query halves, two waves a SIMD), K and
+// V tiles in LDS; the halves' sums meet in LDS at the end.  DQ = 192: 4 waves,
+// one a key quarter, each taking both query halves in turn, its K and V
+// fragments in registers.
+template <int DQ>
+constexpr int dkdv_waves() {
+  return DQ <= 128 ? 8 : 4;
+}
+template <int DQ, int DV>
+constexpr int dkdv_lds() {
+  return (dkdv_waves<DQ>() == 8 ? TILE + 2 * QT : 2 * QT) * (DQ + DV);
+}
+
+template <int DQ, int DV, int MODE>
+__global__ __launch_bounds__(64 * dkdv_waves<DQ>(), dkdv_waves<DQ>() == 8 ? 2 : 1)
+void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __restrict__ lse,
+                   const float* __restrict__ delta, int parts, float* __restrict__ dk_part,
+                   float* __restrict__ dv_part, uint16_t* __restrict__ dk,
+                   uint16_t* __restrict__ dv, int32_t* __restrict__ flags) {
+  constexpr int DSQ = DQ / 16, DSV = DV / 16, DBQ = DQ / 32, DBV = DV / 32;
+  constexpr int LK = TILE * DQ, LV = TILE * DV, LQ = QT * DQ, LG = QT * DV;
+  constexpr int NW = dkdv_waves<DQ>(), NTH = 64 * NW, QH = 8 / NW;
+  constexpr bool KREG = NW == 4;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[dkdv_lds<DQ, DV>()];
+  __shared__ __attribute__((aligned(16))) float lse_s[2][QT], dl_s[2][QT];
+  __shared__ __attribute__((aligned(16))) int lo_s[2][QT], wd_s[2][QT];
+  const int S = a.S, H = a.H, nb = a.plan.nb;
+  const int per = a.Hkv * parts;
+  const int id = uniform(a.plan.korder[blockIdx.x / per]), rest = blockIdx.x % per;
+  const int hk = rest % a.Hkv, part = rest / a.Hkv;
+  const int b = id / a.plan.nt, kt = id % a.plan.nt;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, c = lane & 31;
+  const int kq = wave & 3, qh0 = NW == 8 ? wave >> 2 : 0;
+  const int heads = H / a.Hkv / parts, h0 = hk * (H / a.Hkv) + part * heads;
+  const int64_t ldt = (int64_t)H * DV;
+  const uint16_t* kb = a.k + (int64_t)(b * a.Hkv + hk) * S * DQ;
+  const uint16_t* vb = a.v + (int64_t)(b * a.Hkv + hk) * S * DV;
+  uint16_t* Ks = lds;
+  uint16_t* Vs = lds + LK;
+  uint16_t* qg = KREG ? lds : lds + LK + LV;
+  const int k0 = kt * TILE, kw0 = k0 + kq * 32, mykey = kw0 + c;
+  const int2 seen = make_int2(uniform(a.plan.keys[id].x), uniform(a.plan.keys[id].y));
+  const int4* blk = a.plan.blk + (int64_t)b * nb;
+  bf16x8 kfr[KREG ? DSQ : 1], vfr[KREG ? DSV : 1];
+  if constexpr (KREG) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int s = 0; s < DSQ; ++s)
+      kfr[s] = as_bf16x8(mykey < S ? ld_global16(kb + (int64_t)mykey * DQ + 16 * s + 8 * g) : z);
+#pragma unroll
+    for (int s = 0; s < DSV; ++s)
+      vfr[s] = as_bf16x8(mykey < S ? ld_global16(vb + (int64_t)mykey * DV + 16 * s + 8 * g) : z);
+  } else {
+    const TileCopy<DQ, NTH, TILE> ck(tid, DQ);
+    const TileCopy<DV, NTH, TILE> cv(tid, DV);
+    ck(kb, DQ, k0, S, Ks, wave);
+    cv(vb, DV, k0, S, Vs, wave);
+  }
+  f32x16 dvacc[DBV], dkacc[DBQ];
+#pragma unroll
+  for (int i = 0; i < DBV; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dvacc[i][e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < DBQ; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dkacc[i][e] = 0.0f;
+
+  const int qfirst = seen.x * 32, nq = (seen.y - seen.x + 1) / 2;  // 64-query steps of a head
+  const int steps = nq * heads;
+  const TileCopy<DQ, NTH, QT> cq(tid, DQ);
+  const TileCopy<DV, NTH, QT> cg(tid, ldt);
+  float lr = 0.0f, dr = 0.0f;
+  int2 rr = make_int2(0, 0);
+  auto issue = [&](int h, int q0, int buf) {
+    uint16_t* qs = qg + buf * (LQ + LG);
+    cq(a.q + (int64_t)(b * H + h) * S * DQ, DQ, q0, S, qs, wave);
+    cg(dout + (int64_t)b * S * ldt + (int64_t)h * DV, ldt, q0, S, qs + LQ, wave);
+    if (tid < QT) {
+      const int i = q0 + tid;
+      const int64_t at = (int64_t)(b * H + h) * S + i;
+      lr = i < S ? lse[at] : INFINITY;
+      dr = i < S ? delta[at] : 0.0f;
+      rr = i < S ? run_of(a.lo, a.hi, (int64_t)b * S + i, S) : make_int2(0, 0);
+    }
+  };
+  auto stats = [&](int buf) {
+    if (tid < QT) {
+      lse_s[buf][tid] = lr;
+      dl_s[buf][tid] = dr;
+      lo_s[buf][tid] = rr.x;
+      wd_s[buf][tid] = rr.y - rr.x;
+    }
+  };
+  if (steps > 0) {
+    issue(h0, qfirst, 0);
+    stats(0);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  int j = 0, u = 0;  // head of the part, step of the head
+  for (int n = 0; n < steps; ++n) {
+    const int buf = n & 1, q0 = qfirst + u * QT;
+    const float slope2 = MODE && a.slopes ? a.slopes[h0 + j] * LOG2E : 0.0f;
+    if (++u == nq) {
+      u = 0;
+      ++j;
+    }
+    if (n + 1 < steps) issue(h0 + j, qfirst + u * QT, buf ^ 1);
+    const uint16_t* qs = qg + buf * (LQ + LG);
+    const uint16_t* gs = qs + LQ;
+#pragma unroll
+    for (int hq = 0; hq < QH; ++hq) {
+      const int qh = NW == 8 ? qh0 : hq;
+      const int qw0 = q0 + qh * 32;
+      const int4 x = qw0 < S ? uniform(blk[qw0 >> 5]) : make_int4(INT_MAX, INT_MAX, 0, 0);
+      if (kw0 < x.w && kw0 + 32 > x.x) {  // some query sees some key
+        const bool edge = kw0 < x.y || kw0 + 32 > x.z;
+        const float far0 = (float)(qw0 + 4 * g - mykey);
+        f32x16 sacc, pacc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { sacc[e] = 0.0f; pacc[e] = 0.0f; }
+#pragma unroll
+        for (int s = 0; s < DSQ; ++s) {
+          sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              tile_row<DQ>(qs, qh * 32 + c, s, g),
+              KREG ? kfr[KREG ? s : 0] : tile_row<DQ>(Ks, kq * 32 + c, s, g), sacc, 0, 0, 0);
+          if (s < DSV)
+            pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                tile_row<DV>(gs, qh * 32 + c, s, g),
+                KREG ? vfr[KREG && s < DSV ? s : 0] : tile_row<DV>(Vs, kq * 32 + c, s, g), pacc,
+                0, 0, 0);
+        }
+        bf16x8 pf[2], dsf[2];
+        const int r0 = qh * 32 + g * 4;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          float p8[8], d8[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int vv = 8 * hh + e, ro = (vv >> 2) * 8 + (vv & 3);
+            const float l = lse_s[buf][r0 + ro], dl = dl_s[buf][r0 + ro];
+            if constexpr (MODE == 1) {
+              float grad;
+              const float y = score(a, slope2, sacc[vv], fabsf(far0 + (float)ro), grad);
+              p8[e] = __builtin_amdgcn_exp2f(y - l);
+              d8[e] = p8[e] * (pacc[vv] - dl) * grad;
+            } else {
+              p8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[vv], a.sl2, -l));
+              d8[e] = p8[e] * (pacc[vv] - dl);
+            }
+          }
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int vv = 8 * hh + e, r = r0 + (vv >> 2) * 8 + (vv & 3);
+              const bool keep = (unsigned)(mykey - lo_s[buf][r]) < (unsigned)wd_s[buf][r];
+              p8[e] = keep ? p8[e] : 0.0f;
+              d8[e] = keep ? d8[e] : 0.0f;
+            }
+          }
+          pf[hh] = as_bf16x8(make_uint4(st::pack_bf16x2(p8[0], p8[1]), st::pack_bf16x2(p8[2], p8[3]),
+                                        st::pack_bf16x2(p8[4], p8[5]), st::pack_bf16x2(p8[6], p8[7])));
+          dsf[hh] = as_bf16x8(make_uint4(st::pack_bf16x2(d8[0], d8[1]), st::pack_bf16x2(d8[2], d8[3]),
+                                         st::pack_bf16x2(d8[4], d8[5]), st::pack_bf16x2(d8[6], d8[7])));
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int db = 0; db < DBQ; ++db) {
+            if (db < DBV)
+              dvacc[db < DBV ? db : 0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  tile_tr<DV>(gs, qh * 32 + 16 * hh, db * 32, lane), pf[hh],
+                  dvacc[db < DBV ? db : 0], 0, 0, 0);
+            dkacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                tile_tr<DQ>(qs, qh * 32 + 16 * hh, db * 32, lane), dsf[hh], dkacc[db], 0, 0, 0);
+          }
+      }
+    }
+    if (n + 1 < steps) stats(buf ^ 1);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+  // 8 waves: query half 1 parks its sums in LDS, half 0 adds them and writes
+  // [key][d] rows; dV first, then dK
+  float* red = (float*)lds;
+  constexpr int PARTV = DBV * 16 * 64, PARTK = DBQ * 16 * 64;
+  static_assert(NW == 4 || 4 * PARTK * 4 <= dkdv_lds<DQ, DV>() * 2, "sums fit in LDS");
+  const int64_t krow = (int64_t)(b * a.Hkv + hk) * S + mykey;            // of dk, dv
+  const int64_t prow = ((int64_t)(b * a.Hkv + hk) * parts + part) * S + mykey;  // of the partials
+  float probe = 0.0f;
+  auto write = [&](auto& acc, auto dims, int stride, float mul, float* part_out, uint16_t* direct) {
+    constexpr int D = decltype(dims)::value;
+    if (NW == 8 && qh0 == 1) {
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) red[kq * stride + (db * 16 + e) * 64 + lane] = acc[db][e];
+    }
+    __syncthreads();
+    if (qh0 == 0 && mykey < S) {
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int v4 = 0; v4 < 4; ++v4) {
+          float4 r;
+          float* pr = &r.x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int vv = 4 * v4 + e;
+            pr[e] = (NW == 8 ? acc[db][vv] + red[kq * stride + (db * 16 + vv) * 64 + lane]
+                             : acc[db][vv]) * mul;
+            probe = __builtin_fmaf(pr[e], 0.0f, probe);
+          }
+          const int col = db * 32 + v4 * 8 + g * 4;
+          if (direct)
+            *(u32x2*)(direct + krow * D + col) =
+                u32x2{st::pack_bf16x2(r.x, r.y), st::pack_bf16x2(r.z, r.w)};
+          else
+            *(float4*)(part_out + prow * D + col) = r;
+        }
+    }
+    __syncthreads();
+  };
+  write(dvacc, std::integral_constant<int, DV>{}, PARTV, 1.0f, dv_part, parts == 1 ? dv : nullptr);
+  write(dkacc, std::integral_constant<int, DQ>{}, PARTK, a.scale, dk_part,
+        parts == 1 ? dk : nullptr);
+  const bool bad = __ballot(probe != 0.0f) != 0;
+  if (qh0 == 0 && lane == 0 && kw0 < S)
+    flags[((int64_t)(b * a.Hkv + hk) * parts + part) * nb + (kw0 >> 5)] = bad;
+}
+
+// dk = bf16(sum over the parts, in order), same for dv
+__global__ __launch_bounds__(NT) void span_reduce(const float* __restrict__ dk_part,
+                                                  const float* __restrict__ dv_part, int64_t rows,
+                                                  int parts, int64_t S, int DQ, int DV,
+                                                  uint16_t* __restrict__ dk,
+                                                  uint16_t* __restrict__ dv) {
+  // rows = B * Hkv
+  const int64_t nk = rows * S * DQ / 4, n = nk + rows * S * DV / 4;
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
+    const bool isk = i < nk;
+    const int64_t per = S * (isk ? DQ : DV), e = (isk ? i : i - nk) * 4;
+    const float* part = (isk ? dk_part : dv_part) + e / per * parts * per + e % per;
+    float4 s = make_float4(0, 0, 0, 0);
+    for (int j = 0; j < parts; ++j) {
+      const float4 x = *(const float4*)(part + j * per);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+    *(u32x2*)((isk ? dk : dv) + e) = u32x2{st::pack_bf16x2(s.x, s.y), st::pack_bf16x2(s.z, s.w)};
+  }
+}
+
+// ---------------------------------------------------------------- flagged blocks
+// The rows of a 32-row block whose sums are not finite, over the seen pairs
+// alone.  Correct, not fast: none is flagged while operands are finite.
+template <int D>
+__device__ __forceinline__ float dot(const uint16_t* __restrict__ x, const uint16_t* __restrict__ y) {
+  float s = 0.0f;
+  for (int d = 0; d < D; d += 8) {
+    const uint4 u = ld_global16(x + d), w = ld_global16(y + d);
+    const uint32_t p[4] = {u.x, u.y, u.z, u.w}, r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = __builtin_fmaf(__uint_as_float(p[e] << 16), __uint_as_float(r[e] << 16), s);
+      s = __builtin_fmaf(__uint_as_float(p[e] & 0xffff0000u), __uint_as_float(r[e] & 0xffff0000u), s);
+    }
+  }
+  return s;
+}
+template <bool MAX>
+__device__ __forceinline__ float block_reduce(float x, float* red) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    const float y = __shfl_xor(x, d);
+    x = MAX ? fmaxf(x, y) : x + y;
+  }
+  __syncthreads();
+  if ((tid & 63) == 0) red[tid >> 6] = x;
+  __syncthreads();
+  x = red[0];
+  for (int i = 1; i < NT / 64; ++i) x = MAX ? fmaxf(x, red[i]) : x + red[i];
+  return x;
+}
+
+// calls fn(block) for each set flag among the workgroup's 256
+template <typename F>
+__device__ __forceinline__ void each_flag(const int32_t* __restrict__ flags, int64_t n, F&& fn) {
+  __shared__ unsigned long long sets[NT / 64];
+  const int64_t i0 = (int64_t)blockIdx.x * NT, i = i0 + threadIdx.x;
+  const unsigned long long m = __ballot(i < n && flags[i] != 0);
+  if ((threadIdx.x & 63) == 0) sets[threadIdx.x >> 6] = m;
+  __syncthreads();
+  for (int w = 0; w < NT / 64; ++w)
+    for (unsigned long long s = sets[w]; s; s &= s - 1)
+      fn(i0 + w * 64 + __ffsll((long long)s) - 1);
+}
+
+template <int DQ, int DV>
+__global__ __launch_bounds__(NT) void span_fix_fwd(Args a, const int32_t* __restrict__ flags,
+                                                   int64_t n, uint16_t* __restrict__ out,
+                                                   float* __restrict__ lse) {
+  __shared__ float red[NT / 64], ps[NT];
+  const int tid = threadIdx.x, S = a.S, H = a.H;
+  each_flag(flags, n, [&](int64_t f) {
+    const int64_t bh = f / a.plan.nb;
+    const int b = (int)(bh / H), h = (int)(bh % H);
+    const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
+    const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
+    const float slope2 = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+    const int i0 = (int)(f % a.plan.nb) * 32;
+    for (int i = i0; i < min(i0 + 32, S); ++i) {
+      const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
+      if (run.x >= run.y) continue;
+      const uint16_t* qi = a.q + (bh * S + i) * DQ;
+      auto x_of = [&](int j) {
+        float grad;
+        return score(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ), fabsf((float)(i - j)), grad);
+      };
+      float m = -INFINITY;
+      for (int j = run.x + tid; j < run.y; j += NT) m = fmaxf(m, x_of(j));
+      m = block_reduce<true>(m, red);
+      float l = 0.0f, o = 0.0f;
+      for (int c0 = run.x; c0 < run.y; c0 += NT) {
+        const float p = c0 + tid < run.y ? __builtin_amdgcn_exp2f(x_of(c0 + tid) - m) : 0.0f;
+        l += p;
+        __syncthreads();
+        ps[tid] = p;
+        __syncthreads();
+        if (tid < DV)
+          for (int j = c0; j < min(c0 + NT, run.y); ++j)
+            o = __builtin_fmaf(ps[j - c0], st::bf16_to_f32(vb[(int64_t)j * DV + tid]), o);
+      }
+      l = block_reduce<false>(l, red);
+      if (tid < DV) out[((int64_t)b * S + i) * H * DV + (int64_t)h * DV + tid] = st::f32_to_bf16(o / l);
+      if (tid == 0) lse[bh * S + i] = m + log2f(l);
+    }
+  });
+}
+
+template <int DQ, int DV>
+__global__ __launch_bounds__(NT) void span_fix_dq(Args a, const int32_t* __restrict__ flags, int64_t n,
+                                                  const uint16_t* __restrict__ dout,
+                                                  const float* __restrict__ lse,
+                                                  const float* __restrict__ delta,
+                                                  uint16_t* __restrict__ dq) {
+  __shared__ float ps[NT];
+  const int tid = threadIdx.x, S = a.S, H = a.H;
+  each_flag(flags, n, [&](int64_t f) {
+    const int64_t bh = f / a.plan.nb;
+    const int b = (int)(bh / H), h = (int)(bh % H);
+    const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
+    const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
+    const float slope2 = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+    const int i0 = (int)(f % a.plan.nb) * 32;
+    for (int i = i0; i < min(i0 + 32, S); ++i) {
+      const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
+      if (run.x >= run.y) continue;
+      const uint16_t* qi = a.q + (bh * S + i) * DQ;
+      const uint16_t* gi = dout + ((int64_t)b * S + i) * H * DV + (int64_t)h * DV;
+      const float li = lse[bh * S + i], di = delta[bh * S + i];
+      float o = 0.0f;
+      for (int c0 = run.x; c0 < run.y; c0 += NT) {
+        const int j = c0 + tid;
+        float ds = 0.0f;
+        if (j < run.y) {
+          float grad;
+          const float x = score(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ), fabsf((float)(i - j)), grad);
+          ds = __builtin_amdgcn_exp2f(x - li) * (dot<DV>(gi, vb + (int64_t)j * DV) - di) * grad;
+        }
+        __syncthreads();
+        ps[tid] = ds;
+        __syncthreads();
+        if (tid < DQ)
+          for (int jj = c0; jj < min(c0 + NT, run.y); ++jj)
+            o = __builtin_fmaf(ps[jj - c0], st::bf16_to_f32(kb[(int64_t)jj * DQ + tid]), o);
+      }
+      if (tid < DQ) dq[(bh * S + i) * DQ + tid] = st::f32_to_bf16(o * a.scale);
+    }
+  });
+}
+
+// flags [B*Hkv, parts, nb]: a block is redone by its first flagged part
+template <int DQ, int DV>
+__global__ __launch_bounds__(NT) void span_fix_dkdv(Args a, const int32_t* __restrict__ flags,
+                                                    int64_t n, int parts,
+                                                    const uint16_t* __restrict__ dout,
+                                                    const float* __restrict__ lse,
+                                                    const float* __restrict__ delta,
+                                                    uint16_t* __restrict__ dk,
+                                                    uint16_t* __restrict__ dv) {
+  __shared__ float ps[NT], ds[NT];
+  __shared__ int vis[NT];
+  const int tid = threadIdx.x, S = a.S, H = a.H, group = H / a.Hkv, nb = a.plan.nb;
+  each_flag(flags, n, [&](int64_t f) {
+    const int64_t bhk = f / nb / parts;
+    const int part = (int)(f / nb % parts);
+    for (int p = 0; p < part; ++p)
+      if (flags[(bhk * parts + p) * nb + f % nb]) return;
+    const int b = (int)(bhk / a.Hkv), hk = (int)(bhk % a.Hkv);
+    const int j0 = (int)(f % nb) * 32;
+    const int2 seen = a.plan.keys[(int64_t)b * a.plan.nt + j0 / TILE];
+    const int qa = seen.x * 32, qz = min(seen.y * 32, S);
+    for (int j = j0; j < min(j0 + 32, S); ++j) {
+      const uint16_t* kj = a.k + (bhk * S + j) * DQ;
+      const uint16_t* vj = a.v + (bhk * S + j) * DV;
+      float sk = 0.0f, sv = 0.0f;  // this thread's column of dK, of dV
+      for (int hh = 0; hh < group; ++hh) {
+        const int h = hk * group + hh;
+        const float slope2 = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+        const int64_t bh = (int64_t)b * H + h;
+        const uint16_t* gb = dout + (int64_t)b * S * H * DV + (int64_t)h * DV;
+        for (int c0 = qa; c0 < qz; c0 += NT) {
+          const int i = c0 + tid;
+          bool sees = false;
+          float p = 0.0f, d = 0.0f;
+          if (i < qz) {
+            const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
+            sees = run.x <= j && j < run.y;
+          }
+          if (sees) {
+            float grad;
+            const float x = score(a, slope2, dot<DQ>(a.q + (bh * S + i) * DQ, kj),
+                                  fabsf((float)(i - j)), grad);
+            p = __builtin_amdgcn_exp2f(x - lse[bh * S + i]);
+            d = p * (dot<DV>(gb + (int64_t)i * H * DV, vj) - delta[bh * S + i]) * grad;
+          }
+          __syncthreads();
+          ps[tid] = p;
+          ds[tid] = d;
+          vis[tid] = sees;
+          __syncthreads();
+          for (int q = c0; q < min(c0 + NT, qz); ++q) {
+            if (!vis[q - c0]) continue;
+            if (tid < DQ)
+              sk = __builtin_fmaf(ds[q - c0], st::bf16_to_f32(a.q[(bh * S + q) * DQ + tid]), sk);
+            if (tid < DV)
+              sv = __builtin_fmaf(ps[q - c0], st::bf16_to_f32(gb[(int64_t)q * H * DV + tid]), sv);
+          }
+        }
+      }
+      if (tid < DQ) dk[(bhk * S + j) * DQ + tid] = st::f32_to_bf16(sk * a.scale);
+      if (tid < DV) dv[(bhk * S + j) * DV + tid] = st::f32_to_bf16(sv);
+    }
+  });
+}
+
+// ---------------------------------------------------------------- host
+bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Parts of a KV head's group in the dK/dV pass: the fewest that give every CU
+// a workgroup (one runs per CU).
+int parts_of(int64_t B, int64_t S, int64_t H, int64_t Hkv) {
+  const int64_t group = H / Hkv, wgs = B * st::cdiv(S, TILE) * Hkv;
+  for (int64_t p = 1; p < group; ++p)
+    if (group % p == 0 && wgs * p >= 256) return (int)p;
+  return (int)group;
+}
+
+struct Space {
+  int64_t flags, flags2, delta, dkp, dvp, bytes;  // byte offsets
+  int parts;
+};
+Space space_of(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t DQ, int64_t DV, bool backward) {
+  Space s{};
+  const int64_t nb = st::cdiv(S, 32);
+  int64_t at = 0;
+  s.flags = at;
+  at += up256(B * H * nb * 4);
+  if (backward) {
+    s.parts = parts_of(B, S, H, Hkv);
+    s.flags2 = at;
+    at += up256(B * Hkv * s.parts * nb * 4);
+    s.delta = at;
+    at += up256(B * H * S * 4);
+    if (s.parts > 1) {
+      s.dkp = at;
+      at += up256(B * Hkv * s.parts * S * DQ * 4);
+      s.dvp = at;
+      at += up256(B * Hkv * s.parts * S * DV * 4);
+    }
+  }
+  s.bytes = at + 256;
+  return s;
+}
+
+bool dims_ok(int64_t DQ, int64_t DV) {
+  return (DQ == 64 && DV == 64) || (DQ == 128 && DV == 128) || (DQ == 192 && DV == 128);
+}
+
+int check_common(const char* name, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t DQ,
+                 int64_t DV, float scale, float cap) {
+  ST_CHECK_ARG(B >= 0 && S >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0, "%s: bad head counts", name);
+  if (!dims_ok(DQ, DV))
+    return st::fail(ST_EUNSUPPORTED, "%s: head dims %lld/%lld (64/64, 128/128 or 192/128 only)",
+                    name, (long long)DQ, (long long)DV);
+  ST_CHECK_ARG(std::isfinite(scale) && scale > 0, "%s: scale must be positive and finite", name);
+  ST_CHECK_ARG(std::isfinite(cap) && cap >= 0, "%s: cap must be finite, 0 for none", name);
+  // tiles by 32-bit ids, one grid of tiles x heads, and 64 token-major rows
+  // within a 32-bit byte offset
+  const int64_t lim = (int64_t)1 << 31;
+  if (S >= (1 << 30) || H >= (1 << 16) || B >= (1 << 24) || B * st::cdiv(S, 32) * H >= lim ||
+      64 * H * DV * 2 >= lim)
+    return st::fail(ST_EUNSUPPORTED, "%s: B=%lld S=%lld H=%lld is too large", name, (long long)B,
+                    (long long)S, (long long)H);
+  return ST_OK;
+}
+
+Args args_of(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B, int64_t S,
+             int64_t H, int64_t Hkv, float scale, float cap, const float* slopes,
+             const int32_t* lo, const int32_t* hi, const void* plan) {
+  Args a{};
+  a.q = q; a.k = k; a.v = v;
+  a.lo = lo; a.hi = hi;
+  a.slopes = slopes;
+  a.plan = plan_of(plan, B, S);
+  a.S = (int)S; a.H = (int)H; a.Hkv = (int)Hkv;
+  a.scale = scale;
+  a.sl2 = scale * LOG2E;
+  if (cap > 0) {
+    a.cap_in = 2.0f * LOG2E * scale / cap;
+    a.cap_out = cap * LOG2E;
+  }
+  return a;
+}
+
+template <int DQ, int DV, int MODE>
+int run_fwd(const Args& a, int64_t B, uint16_t* out, float* lse, char* ws, hipStream_t s) {
+  int32_t* flags = (int32_t*)ws;
+  const int64_t n = B * a.H * a.plan.nb;
+  span_fwd<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, lse, flags);
+  if (int rc = st::check_launch("span_fwd")) return rc;
+  span_fix_fwd<DQ, DV><<<(unsigned)st::cdiv(n, NT), NT, 0, s>>>(a, flags, n, out, lse);
+  return st::check_launch("span_fix_fwd");
+}
+
+template <int DQ, int DV, int MODE>
+int run_bwd(const Args& a, int64_t B, const uint16_t* out, const float* lse, const uint16_t* dout,
+            uint16_t* dq, uint16_t* dk, uint16_t* dv, char* ws, hipStream_t s) {
+  const Space sp = space_of(B, a.S, a.H, a.Hkv, DQ, DV, true);
+  int32_t *f1 = (int32_t*)(ws + sp.flags), *f2 = (int32_t*)(ws + sp.flags2);
+  float* delta = (float*)(ws + sp.delta);
+  float *dkp = (float*)(ws + sp.dkp), *dvp = (float*)(ws + sp.dvp);
+  span_bwd_dq<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, dout, lse, delta,
+                                                                          dq, f1);
+  if (int rc = st::check_launch("span_bwd_dq")) return rc;
+  span_bwd_dkdv<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.Hkv * sp.parts), 64 * dkdv_waves<DQ>(), 0, s>>>(
+      a, dout, lse, delta, sp.parts, dkp, dvp, dk, dv, f2);
+  if (int rc = st::check_launch("span_bwd_dkdv")) return rc;
+  if (sp.parts > 1) {
+    const int64_t n4 = B * a.Hkv * a.S * (DQ + DV) / 4;
+    span_reduce<<<(unsigned)std::min<int64_t>(st::cdiv(n4, NT), 4096), NT, 0, s>>>(
+        dkp, dvp, B * a.Hkv, sp.parts, a.S, DQ, DV, dk, dv);
+    if (int rc = st::check_launch("span_reduce")) return rc;
+  }
+  const int64_t n1 = B * a.H * a.plan.nb, n2 = B * a.Hkv * sp.parts * a.plan.nb;
+  span_fix_dq<DQ, DV><<<(unsigned)st::cdiv(n1, NT), NT, 0, s>>>(a, f1, n1, dout, lse, delta, dq);
+  if (int rc = st::check_launch("span_fix_dq")) return rc;
+  span_fix_dkdv<DQ, DV><<<(unsigned)st::cdiv(n2, NT), NT, 0, s>>>(a, f2, n2, sp.parts, dout, lse,
+                                                                  delta, dk, dv);
+  return st::check_launch("span_fix_dkdv");
+}
+
+}  // namespace
+
+extern "C" int64_t st_span_plan_bytes(int64_t B, int64_t S) {
+  if (B <= 0 || S <= 0) return 0;
+  return plan_of(nullptr, B, S).bytes;
+}
+
+extern "C" int st_span_plan(const int32_t* key_start, const int32_t* key_end, int64_t B, int64_t S,
+                            void* plan, int64_t plan_bytes, st_stream_t stream) {
+  ST_CHECK_ARG(B >= 0 && S >= 0 && S < (1 << 30), "st_span_plan: bad shape");
+  if (B == 0 || S == 0) return ST_OK;
+  if (B >= (1 << 24) || B * st::cdiv(S, 32) >= (int64_t)1 << 31)
+    return st::fail(ST_EUNSUPPORTED, "st_span_plan: too many rows");
+  ST_CHECK_ARG(key_start && key_end && plan && al16(plan), "st_span_plan: NULL or unaligned pointer");
+  const Plan p = plan_of(plan, B, S);
+  if (plan_bytes < p.bytes)
+    return st::fail(ST_EWORKSPACE, "st_span_plan: needs %lld bytes", (long long)p.bytes);
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t blocks = B * p.nb, tiles = B * p.nt;
+  span_blocks<<<(unsigned)st::cdiv(blocks * 32, NT), NT, 0, s>>>(key_start, key_end, (int)S, p.nb,
+                                                                 blocks, (int4*)p.blk);
+  if (int rc = st::check_launch("span_blocks")) return rc;
+  span_tiles<<<(unsigned)tiles, 64, 0, s>>>(p.blk, p.nb, p.nt, (int2*)p.keys, p.qwork, p.kwork);
+  if (int rc = st::check_launch("span_tiles")) return rc;
+  span_order<<<dim3((unsigned)st::cdiv(tiles, NT), 2), NT, 0, s>>>(
+      p.qwork, p.kwork, tiles, tiles <= SORT_LIMIT, (int32_t*)p.qorder, (int32_t*)p.korder);
+  return st::check_launch("span_order");
+}
+
+extern "C" int64_t st_span_attn_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv,
+                                                int64_t DQ, int64_t DV, int32_t backward) {
+  if (B <= 0 || S <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || !dims_ok(DQ, DV)) return 0;
+  return space_of(B, S, H, Hkv, DQ, DV, backward != 0).bytes;
+}
+
+extern "C" int st_span_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B,
+                                int64_t S, int64_t H, int64_t Hkv, int64_t DQ, int64_t DV,
+                                float scale, float cap, const float* slopes,
+                                const int32_t* key_start, const int32_t* key_end, const void* plan,
+                                uint16_t* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                st_stream_t stream) {
+  const char* name = "st_span_attn_fwd";
+  if (int rc = check_common(name, B, S, H, Hkv, DQ, DV, scale, cap)) return rc;
+  if (B == 0 || S == 0) return ST_OK;
+  ST_CHECK_ARG(q && k && v && out && lse && key_start && key_end && plan && al16(q) && al16(k) &&
+                   al16(v) && al16(out) && al16(plan), "%s: NULL or unaligned pointer", name);
+  const int64_t need = space_of(B, S, H, Hkv, DQ, DV, false).bytes;
+  if (!workspace || workspace_bytes < need)
+    return st::fail(ST_EWORKSPACE, "%s: needs %lld workspace bytes", name, (long long)need);
+  const Args a = args_of(q, k, v, B, S, H, Hkv, scale, cap, slopes, key_start, key_end, plan);
+  char* ws = (char*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  hipStream_t s = (hipStream_t)stream;
+  const bool mod = cap > 0 || slopes;
+#define ST_SPAN(DQ_, DV_)                                          \
+  if (DQ == DQ_)                                                   \
+    return mod ? run_fwd<DQ_, DV_, 1>(a, B, out, lse, ws, s)       \
+               : run_fwd<DQ_, DV_, 0>(a, B, out, lse, ws, s)
+  ST_SPAN(64, 64);
+  ST_SPAN(128, 128);
+  ST_SPAN(192, 128);
+#undef ST_SPAN
+  return ST_OK;
+}
+
+extern "C" int st_span_attn_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                                const uint16_t* out, const float* lse, const uint16_t* dout,
+                                int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t DQ,
+                                int64_t DV, float scale, float cap, const float* slopes,
+                                const int32_t* key_start, const int32_t* key_end, const void* plan,
+                                uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace,
+                                int64_t workspace_bytes, st_stream_t stream) {
+  const char* name = "st_span_attn_bwd";
+  if (int rc = check_common(name, B, S, H, Hkv, DQ, DV, scale, cap)) return rc;
+  if (B == 0 || S == 0) return ST_OK;
+  ST_CHECK_ARG(q && k && v && out && lse && dout && dq && dk && dv && key_start && key_end && plan &&
+                   al16(q) && al16(k) && al16(v) && al16(out) && al16(dout) && al16(dq) &&
+                   al16(dk) && al16(dv) && al16(plan), "%s: NULL or unaligned pointer", name);
+  const int64_t need = space_of(B, S, H, Hkv, DQ, DV, true).bytes;
+  if (!workspace || workspace_bytes < need)
+    return st::fail(ST_EWORKSPACE, "%s: needs %lld workspace bytes", name, (long long)need);
+  const Args a = args_of(q, k, v, B, S, H, Hkv, scale, cap, slopes, key_start, key_end, plan);
+  char* ws = (char*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  hipStream_t s = (hipStream_t)stream;
+  const bool mod = cap > 0 || slopes;
+#define ST_SPAN(DQ_, DV_)                                                             \
+  if (DQ == DQ_)                                                                      \
+    return mod ? run_bwd<DQ_, DV_, 1>(a, B, out, lse, dout, dq, dk, dv, ws, s)        \
+               : run_bwd<DQ_, DV_, 0>(a, B, out, lse, dout, dq, dk, dv, ws, s)
+  ST_SPAN(64, 64);
+  ST_SPAN(128, 128);
+  ST_SPAN(192, 128);
+#undef ST_SPAN
+  return ST_OK;
+}
