@@ -494,6 +494,41 @@ int st_cross_entropy_rows(uint16_t* logits, int64_t rows, int64_t vocab, int64_t
                           float* loss_rows, st_stream_t stream);
 
 /* ---------------------------------------------------------------------
+ * Log probabilities of given tokens under the frozen vocabulary head, with
+ * entropy and top alternatives; no logits of all rows are kept.  The reference
+ * has the summed cross-entropy only (native_terminal.py:11-47).
+ *   l = hidden head^T (bf16 products, fp32 sums),
+ *   x = (cap > 0 ? cap * tanh(l / cap) : l) / temperature,
+ *   logprobs[r] = x[tokens[r]] - lse[r] (0 where tokens[r] == ignore_index, NaN
+ *   for another token outside [0, V)), entropy[r], lse[r] = log sum e^x, all
+ *   natural; top_logprobs and top_tokens [rows, top] (top <= 64, V <= 2^20):
+ *   the greatest l, ties to the lowest index, in falling order (-1 and NaN where
+ *   fewer logits are numbers).
+ * hidden [rows, H] (stride ldh), head [V, H] (stride ldw): bf16, 16-byte rows.
+ * The backward takes the forward's outputs and the gradients of logprobs,
+ * entropy and top_logprobs (fp32, each may be NULL) and writes dhidden (stride
+ * ldd, bf16); rows whose gradients are all 0 get 0.  dl of each row is rounded to
+ * bf16 in the workspace (2 bytes a logit); the forward's holds 4 bytes a logit
+ * with top > 0 and 16 per 256 logits without.
+ * --------------------------------------------------------------------- */
+int64_t st_token_logprobs_workspace_bytes(int64_t rows, int64_t H, int64_t V, int64_t ldw,
+                                          int64_t top, int32_t backward);
+int st_token_logprobs_fwd(const uint16_t* hidden, int64_t rows, int64_t H, int64_t ldh,
+                          const uint16_t* head, int64_t V, int64_t ldw, const int64_t* tokens,
+                          int64_t ignore_index, float temperature, float cap, int64_t top,
+                          float* logprobs, float* entropy, float* lse, float* top_logprobs,
+                          int64_t* top_tokens, void* workspace, int64_t workspace_bytes,
+                          st_stream_t stream);
+int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64_t H, int64_t ldh,
+                          const uint16_t* head, int64_t V, int64_t ldw, const int64_t* tokens,
+                          int64_t ignore_index, float temperature, float cap, int64_t top,
+                          const float* logprobs, const float* entropy, const float* lse,
+                          const float* top_logprobs, const int64_t* top_tokens,
+                          const float* g_logprobs, const float* g_entropy, const float* g_top,
+                          uint16_t* dhidden, int64_t ldd, void* workspace, int64_t workspace_bytes,
+                          st_stream_t stream);
+
+/* ---------------------------------------------------------------------
  * Mixture of experts (adapters/qwen3_moe.py:95-113; adapters/deepseek.py:
  * 115-176).  Tokens T, picks per token k, experts E; a "pick" is (token t,
  * slot j) at flat index t*k + j; permuted rows list the picks grouped by

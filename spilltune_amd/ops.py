@@ -26,6 +26,7 @@ from contextlib import contextmanager
 from dataclasses import dataclass, field
 from functools import lru_cache
 from itertools import accumulate
+from typing import NamedTuple
 
 import torch
 
@@ -207,6 +208,12 @@ def _scratch(device, nbytes: int) -> torch.Tensor | None:
     that captured an earlier one, never share it (one torch.empty is ~2 us of
     host time)."""
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous from a 16-byte boundary (a copy where it is not)."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _gemm_scratch(weight: Q4Weight, form: int, M: int, rank: int, cols: int):
@@ -753,6 +760,117 @@ def chunked_causal_loss(normalized, head, labels, *, normalization, token_chunk,
                             tuple(supervised_chunks))
 
 
+class TokenLogProbs(NamedTuple):
+    """What :func:`token_logprobs` gives for each token."""
+    logprobs: torch.Tensor      # fp32 [...]
+    entropy: torch.Tensor       # fp32 [...], natural
+    top_logprobs: torch.Tensor  # fp32 [..., top], falling
+    top_tokens: torch.Tensor    # int64 [..., top]
+
+
+LOGPROB_SCRATCH = 2 << 30  # bytes of scratch a token_logprobs call aims to stay within
+
+
+class _TokenLogProbs(torch.autograd.Function):
+    @staticmethod
+    def _row_chunks(hidden, head, top, backward):
+        """Row ranges whose scratch stays within LOGPROB_SCRATCH (256 rows at
+        least): 4 bytes a logit with alternatives, 2 in the backward."""
+        rows, (V, H) = hidden.shape[0], head.shape
+        per = 2 * V if backward else 4 * V if top else V // 16 + 20
+        step = max(256, LOGPROB_SCRATCH // per // 256 * 256)
+        return [(r, min(r + step, rows)) for r in range(0, rows, step)]
+
+    @staticmethod
+    def forward(ctx, hidden, head, tokens, ignore_index, temperature, cap, top):
+        rows, H = hidden.shape
+        V, dev = head.shape[0], hidden.device
+        lp, ent, lse = (torch.empty(rows, dtype=_F32, device=dev) for _ in range(3))
+        top_lp = torch.empty((rows, top), dtype=_F32, device=dev)
+        top_tok = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        with torch.cuda.device(dev):
+            for a, z in _TokenLogProbs._row_chunks(hidden, head, top, False):
+                ws = _scratch(dev, _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V,
+                                              head.stride(0), top, 0))
+                _lib.call("st_token_logprobs_fwd", _lib.ptr(hidden[a:z]), z - a, H, hidden.stride(0),
+                          _lib.ptr(head), V, head.stride(0), _lib.ptr(tokens[a:z]), ignore_index,
+                          temperature, cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]),
+                          _lib.ptr(lse[a:z]), _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]),
+                          _lib.ptr(ws), ws.numel(), _lib.stream_handle(dev))
+        ctx.save_for_backward(hidden, head, tokens, lp, ent, lse, top_lp, top_tok)
+        ctx.meta = (ignore_index, temperature, cap, top)
+        ctx.mark_non_differentiable(top_tok)
+        ctx.set_materialize_grads(False)
+        return lp, ent, top_lp, top_tok
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _):
+        hidden, head, tokens, lp, ent, lse, top_lp, top_tok = ctx.saved_tensors
+        ignore_index, temperature, cap, top = ctx.meta
+        H, V, dev = hidden.shape[1], head.shape[0], hidden.device
+        g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
+        part = lambda g, a, z: None if g is None else _lib.ptr(g[a:z])  # noqa: E731
+        dh = torch.empty(hidden.shape, dtype=_BF16, device=dev)
+        with torch.cuda.device(dev):
+            for a, z in _TokenLogProbs._row_chunks(hidden, head, top, True):
+                ws = _scratch(dev, _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V,
+                                              head.stride(0), top, 1))
+                _lib.call("st_token_logprobs_bwd", _lib.ptr(hidden[a:z]), z - a, H, hidden.stride(0),
+                          _lib.ptr(head), V, head.stride(0), _lib.ptr(tokens[a:z]), ignore_index,
+                          temperature, cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]),
+                          _lib.ptr(lse[a:z]), _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]),
+                          part(g_lp, a, z), part(g_ent, a, z), part(g_top, a, z), _lib.ptr(dh[a:z]),
+                          dh.stride(0), _lib.ptr(ws), ws.numel(), _lib.stream_handle(dev))
+        return dh, None, None, None, None, None, None
+
+
+def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ignore_index=-100):
+    """Log probability of ``tokens`` (int64 [...]; no shift) after the hidden
+    states ``hidden`` (bf16 [..., H]) under the frozen ``head`` (bf16 [V, H]),
+    with the entropy of each distribution and its ``top`` (at most 64) most
+    probable tokens, as :class:`TokenLogProbs`.
+
+    Logits are ``hidden head^T``, with ``cap`` ``cap * tanh(logits / cap)``, over
+    ``temperature``; they are summed in fp32 and not kept, the backward forms them
+    again.  Differentiable in ``hidden`` through all three fp32 results.  A token
+    equal to ``ignore_index`` has log probability 0 and no gradient from it (its
+    entropy and alternatives are those of its hidden state); any other token
+    outside [0, V) gives NaN when it comes on the device and is refused when it
+    comes from the host."""
+    if hidden.dtype != _BF16 or head.dtype != _BF16 or head.dim() != 2 or hidden.dim() < 1 \
+            or hidden.shape[-1] != head.shape[1]:
+        raise ValueError("unsupported_capability: token_logprobs expects bf16 hidden [..., H] and "
+                         "head [V, H]")
+    if head.requires_grad:
+        raise ValueError("unsupported_capability: token_logprobs takes a frozen head")
+    V, H = head.shape
+    if H % 8 or H == 0 or V == 0:
+        raise ValueError("unsupported_capability: token_logprobs needs a hidden size of whole "
+                         "multiples of 8")
+    if tokens.dtype != torch.int64 or tokens.shape != hidden.shape[:-1]:
+        raise ValueError(f"unsupported_capability: tokens must be int64 {tuple(hidden.shape[:-1])}")
+    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(64, V):
+        raise ValueError(f"unsupported_capability: top must be 0..{min(64, V)}")
+    temperature, cap = float(temperature), 0.0 if cap is None else float(cap)
+    if not (math.isfinite(temperature) and temperature > 0 and math.isfinite(cap) and cap >= 0):
+        raise ValueError("unsupported_capability: temperature must be positive, cap None or positive")
+    if not hidden.is_cuda:
+        raise ValueError("unsupported_capability: token_logprobs runs on the GPU")
+    if tokens.device.type == "cpu":
+        if bool((((tokens < 0) | (tokens >= V)) & (tokens != ignore_index)).any()):
+            raise ValueError("unsupported_capability: tokens must be ignore_index or in [0, vocab)")
+        tokens = tokens.to(hidden.device)
+    if head.device != hidden.device or tokens.device != hidden.device:
+        raise ValueError("unsupported_capability: hidden, head and tokens on one device")
+    shape = tuple(tokens.shape)
+    lp, ent, top_lp, top_tok = _TokenLogProbs.apply(
+        _operand(hidden.reshape(-1, H)), _operand(head), tokens.reshape(-1).contiguous(),
+        int(ignore_index), temperature, cap, top)
+    return TokenLogProbs(lp.view(shape), ent.view(shape), top_lp.view(*shape, top),
+                         top_tok.view(*shape, top))
+
+
 # ----------------------------------------------------------------- RoPE
 class _RopeHeads(torch.autograd.Function):
     """Token-major projection output columns -> [B, heads, S, D] (rotated)."""
@@ -1086,4 +1204,4 @@ __all__ = ["Q4Weight", "concat_rows", "lora_fusable", "q4_lora_linear", "rms_nor
            "mla_rope", "mla_attention",
            "rms_norm_residual",
            "linear_bf16", "linear_bf16_dgrad", "supervised_chunk_intervals",
-           "chunked_causal_loss"]
+           "chunked_causal_loss", "TokenLogProbs", "token_logprobs"]

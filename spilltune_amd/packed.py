@@ -24,16 +24,10 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib
-from .ops import _scratch
+from .ops import _operand, _scratch
 
 _BF16 = torch.bfloat16
 _F32 = torch.float32
-
-
-def _operand(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous from a 16-byte boundary (a copy where it is not)."""
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
 
 
 # ----------------------------------------------------------------- masks
@@ -64,6 +58,8 @@ def span_mask(key_start: torch.Tensor, key_end: torch.Tensor, positions=None) ->
     B, S = key_start.shape
     if B < 1 or S < 1:
         raise ValueError("unsupported_capability: a mask needs at least one token")
+    if not key_start.is_cuda:
+        raise ValueError("unsupported_capability: a mask lives on the GPU")
     dev = key_start.device
     if positions is None:
         positions = torch.arange(S, dtype=torch.int32, device=dev).expand(B, S)
@@ -188,6 +184,8 @@ def span_attention(q, k, v, scale, mask: SpanMask, *, cap=None, slopes=None):
             raise ValueError("unsupported_capability: slopes must be constant fp32 [heads] on the "
                              "attention's device")
         slopes = slopes.contiguous()
+    if not q.is_cuda:
+        raise ValueError("unsupported_capability: span_attention runs on the GPU")
     return _SpanAttention.apply(_operand(q), _operand(k), _operand(v), scale, mask, cap, slopes)
 
 
@@ -339,6 +337,8 @@ def rope_positions(y, positions, rotary: Rotary, heads: int, kv_heads: int, *, n
         wq, wk = (_operand(w.detach()) for w in norms)
         if any(w.dtype != _BF16 or tuple(w.shape) != (D,) or w.device != y.device for w in (wq, wk)):
             raise ValueError("unsupported_capability: norm weights must be bf16 [head_dim]")
+    if not y.is_cuda:
+        raise ValueError("unsupported_capability: rope_positions runs on the GPU")
     if y.stride(1) != 1 or y.stride(0) % 8 or y.stride(0) < y.shape[1] or y.data_ptr() % 16:
         y = y.clone(memory_format=torch.contiguous_format)
     return _RopePositions.apply(y, positions.contiguous(), rotary, int(heads), int(kv_heads), wq, wk,

@@ -1,0 +1,65 @@
+"""Token log probabilities on the CPU: refusals before any device work."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from spilltune_amd import _lib, ops
+
+BF = torch.bfloat16
+
+
+def test_token_logprobs_refuses():
+    h, w, t = torch.zeros(2, 3, 16, dtype=BF), torch.zeros(40, 16, dtype=BF), torch.zeros(2, 3).long()
+    f = ops.token_logprobs
+    for a, b in ((h.float(), w), (h, w.float()), (h, w[0]), (h[..., :8], w)):
+        with pytest.raises(ValueError, match="expects bf16"):
+            f(a, b, t)
+    with pytest.raises(ValueError, match="frozen"):
+        f(h, w.clone().requires_grad_(True), t)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        f(h[..., :12].contiguous(), w[:, :12].contiguous(), t)
+    for bad in (t.int(), t[:1], t[0]):
+        with pytest.raises(ValueError, match="tokens must be int64"):
+            f(h, w, bad)
+    for top in (-1, 65, 2.0, True):
+        with pytest.raises(ValueError, match="top must be"):
+            f(h, w, t, top=top)
+    with pytest.raises(ValueError, match="top must be 0..5"):
+        f(h, w[:5], t, top=6)
+    for kw in ({"temperature": 0.0}, {"temperature": -1.0}, {"temperature": math.nan}, {"cap": -1.0},
+               {"cap": math.inf}):
+        with pytest.raises(ValueError, match="temperature must be positive"):
+            f(h, w, t, **kw)
+    with pytest.raises(ValueError, match="GPU"):
+        f(h, w, t)
+
+
+def test_abi_refuses_before_the_device():
+    p, n = ctypes.c_void_p(16), ctypes.c_void_p(None)
+
+    def fwd(rows=4, H=16, V=40, ldh=16, ldw=16, T=1.0, cap=0.0, top=0, hidden=p, ws=p, wb=1 << 40,
+            lp=p, tt=p):
+        _lib.call("st_token_logprobs_fwd", hidden, rows, H, ldh, p, V, ldw, p, -100, T, cap, top, lp, p,
+                  p, p, tt, ws, wb, None)
+    for kw, msg in (({"H": 12}, "16-byte"), ({"ldw": 8}, "16-byte"), ({"ldh": 20}, "16-byte"),
+                    ({"T": 0.0}, "temperature"), ({"cap": -1.0}, "cap"), ({"top": 41}, "within"),
+                    ({"V": 400, "top": 65}, "too large"), ({"V": 1 << 23}, "too large"),
+                    ({"V": (1 << 20) + 1, "top": 1}, "too large"), ({"hidden": n}, "NULL"),
+                    ({"hidden": ctypes.c_void_p(8)}, "unaligned"), ({"lp": n}, "NULL"),
+                    ({"tt": n, "top": 2}, "NULL"), ({"wb": 10}, "workspace"), ({"ws": n}, "workspace")):
+        with pytest.raises(ValueError, match=msg):
+            fwd(**kw)
+    fwd(rows=0)
+
+    def bwd(ldd=16, dh=p, wb=1 << 40):
+        _lib.call("st_token_logprobs_bwd", p, 4, 16, 16, p, 40, 16, p, -100, 1.0, 0.0, 0, p, p, p, n, n,
+                  p, n, n, dh, ldd, p, wb, None)
+    for kw, msg in (({"ldd": 8}, "NULL or"), ({"dh": n}, "NULL"), ({"wb": 10}, "workspace")):
+        with pytest.raises(ValueError, match=msg):
+            bwd(**kw)
+    q = lambda *a: _lib.query("st_token_logprobs_workspace_bytes", *a)  # noqa: E731
+    assert q(0, 16, 40, 16, 0, 0) == 0 and q(4, 16, 40, 8, 0, 0) == 0
+    assert q(1000, 64, 5000, 64, 5, 0) - q(1000, 64, 5000, 64, 0, 0) == 1000 * 5000 * 4
+    assert q(1000, 64, 5000, 64, 0, 1) >= 1000 * 5000 * 2

@@ -55,6 +55,8 @@ def test_document_runs_refuse():
         packed.span_mask(d, d[:, :2])
     with pytest.raises(ValueError, match="at least one token"):
         packed.span_mask(d[:0], d[:0])
+    with pytest.raises(ValueError, match="GPU"):
+        packed.span_mask(d, d)
 
 
 def test_span_attention_refuses():
@@ -80,6 +82,8 @@ def test_span_attention_refuses():
                    torch.zeros(2, requires_grad=True)):
         with pytest.raises(ValueError, match="slopes"):
             f(q, q, q, 1.0, mask, slopes=slopes)
+    with pytest.raises(ValueError, match="GPU"):
+        f(q, q, q, 1.0, mask)
 
 
 def test_abi_refuses_before_the_device():
@@ -129,6 +133,8 @@ def test_rope_positions_refuses():
             f(bad, pos, r, 2, 1)
     with pytest.raises(ValueError, match="norm weights"):
         f(y, pos, r, 2, 1, norms=(y[0, :64], y[0, :32]))
+    with pytest.raises(ValueError, match="GPU"):
+        f(y, pos, r, 2, 1)
     for head, kw in ((60, {}), (64, {"rotary_dim": 63}), (64, {"rotary_dim": 80}),
                      (64, {"rotary_dim": 0})):
         with pytest.raises(ValueError, match="rotary part"):
