@@ -40,7 +40,7 @@ from pathlib import Path
 
 import torch
 
-from . import ops, slots
+from . import ops, packed, slots
 from .archive import MARKER, ArchiveReader
 from .codecs import FORMATS
 from .dense import positions_and_masks
@@ -101,6 +101,7 @@ class ArchiveDenseAdapter:
         if quantization not in FORMATS:
             raise ValueError(f"unsupported_quantization: explicit format required; supported={FORMATS}")
         self.device = torch.device(device)
+        self._rotary = None  # of packed rows, made on their first use
         if self.device.type != "cuda":
             raise ValueError("unsupported_capability: the 4-bit HIP path runs on a GPU device")
         if not torch.cuda.is_available():
@@ -165,6 +166,16 @@ class ArchiveDenseAdapter:
         rot, mask = positions_and_masks(valid, head_dim=self.config["head_dim"],
                                         theta=self.config["theta"], device=self.device)
         return rot, {"full_attention": mask}
+
+    def packed_positions_and_masks(self, documents, **kw):
+        """Positions and masks of packed rows (packed.positions_and_masks)."""
+        if documents.ndim != 2 or documents.shape[1] > self.config["max_positions"]:
+            raise ValueError("unsupported_capability: sequence beyond configured context")
+        if self._rotary is None:
+            self._rotary = packed.Rotary(self.config["head_dim"], self.config["theta"],
+                                         device=self.device)
+        positions, mask = packed.positions_and_masks(documents, self._rotary, **kw)
+        return positions, {"full_attention": mask}
 
     def terminal_norm(self, hidden):
         B, S, H = hidden.shape

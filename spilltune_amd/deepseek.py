@@ -29,7 +29,7 @@ import math
 
 import torch
 
-from . import moe, ops
+from . import moe, ops, packed
 from .dense import CausalMask, key_lengths
 
 ATTENTION_TARGETS_Q_LORA = ("self_attn.q_a_proj", "self_attn.q_b_proj",
@@ -102,12 +102,24 @@ def positions_and_masks(valid: torch.Tensor, *, rope: dict, rope_dim: int, devic
         raise ValueError("unsupported_deepseek: invalid mask/context")
     lengths = key_lengths(valid, device, "unsupported_deepseek: all-valid/right padding only")
     batch, length = valid.shape
-    inverse, amplitude = rope_parameters(rope, rope_dim, device)
     pos = torch.arange(length, device=device).expand(batch, -1)
-    phase = (inverse[None, :, None].expand(batch, -1, 1) @ pos[:, None].float()).transpose(1, 2)
+    return _tables(pos, rope, rope_dim, dtype), CausalMask(batch, length, lengths)
+
+
+def _tables(pos, rope, rope_dim, dtype):
+    inverse, amplitude = rope_parameters(rope, rope_dim, pos.device)
+    phase = (inverse[None, :, None].expand(len(pos), -1, 1) @ pos[:, None].float()).transpose(1, 2)
     phase = torch.cat((phase, phase), -1)
-    return ((phase.cos() * amplitude).to(dtype), (phase.sin() * amplitude).to(dtype)), \
-        CausalMask(batch, length, lengths)
+    return (phase.cos() * amplitude).to(dtype), (phase.sin() * amplitude).to(dtype)
+
+
+def packed_positions_and_masks(documents: torch.Tensor, *, rope: dict, rope_dim: int, device,
+                               bidirectional=None, window=None, dtype=torch.bfloat16):
+    """(cos, sin) by the positions within each document, and the span mask, of
+    packed rows (:func:`spilltune_amd.packed.document_mask`)."""
+    move = lambda t: None if t is None else t.to(device)  # noqa: E731
+    mask = packed.document_mask(move(documents), bidirectional=move(bidirectional), window=window)
+    return _tables(mask.positions, rope, rope_dim, dtype), mask
 
 
 def _weight(weights, name):
@@ -131,8 +143,9 @@ def deepseek_block(hidden_states, position_embeddings, attention_mask, *, parame
                    lora_q=None, lora_qa=None, lora_qb=None, lora_kva=None, lora_kvb=None,
                    lora_o=None, lora_shared_gate=None, lora_shared_up=None,
                    lora_shared_down=None, **w):
-    if attention_mask is not None and not isinstance(attention_mask, CausalMask):
-        raise ValueError("unsupported_capability: only the causal mask marker is supported")
+    if attention_mask is not None and not isinstance(attention_mask, (CausalMask, packed.SpanMask)):
+        raise ValueError("unsupported_capability: only the causal mask marker and span masks are "
+                         "supported")
     c = parameters
     B, S, Hd = hidden_states.shape
     cos, sin = position_embeddings
@@ -157,8 +170,12 @@ def deepseek_block(hidden_states, position_embeddings, attention_mask, *, parame
     kv = ops.q4_lora_linear(kvn, _weight(w, "self_attn.kv_b_proj"), [lora_kvb])
     Q, K, V = ops.mla_rope(q, kv, comp, cos, sin, batch=B, seq=S, heads=heads, nope=nope,
                            rope=rope, v_dim=vdim, kv_rank=kv_rank, interleave=c["interleave"])
-    kv_len = attention_mask.lengths if attention_mask is not None else None
-    attended = ops.mla_attention(Q, K, V, c["attention_scale"], kv_len).reshape(B * S, heads * vdim)
+    if isinstance(attention_mask, packed.SpanMask):
+        attended = packed.span_attention(Q, K, V, c["attention_scale"], attention_mask)
+    else:
+        kv_len = attention_mask.lengths if attention_mask is not None else None
+        attended = ops.mla_attention(Q, K, V, c["attention_scale"], kv_len)
+    attended = attended.reshape(B * S, heads * vdim)
     h1 = ops.q4_lora_linear(attended, _weight(w, "self_attn.o_proj"), [lora_o], residual=residual)
     h1, xn2 = ops.rms_norm_residual(h1, w["post_attention_layernorm.weight"], c["eps"])
     if not c["moe"]:  # dense layer: residual + down(silu(gate) * up)
@@ -231,5 +248,5 @@ def lora_kwargs(adapters: dict) -> dict:
 
 
 __all__ = ["deepseek_block", "rope_parameters", "attention_scale", "positions_and_masks",
-           "lora_kwargs", "make_deepseek_block", "ATTENTION_TARGETS_Q_LORA", "ATTENTION_TARGETS_Q",
+           "packed_positions_and_masks", "lora_kwargs", "make_deepseek_block", "ATTENTION_TARGETS_Q_LORA", "ATTENTION_TARGETS_Q",
            "SHARED_EXPERT_TARGETS"]

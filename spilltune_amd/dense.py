@@ -16,7 +16,10 @@ no reference to slot memory.  Differences in *how*, not *what*:
 * ``attention_mask`` is a :class:`CausalMask` marker: causal attention with
   each row's keys past its valid prefix masked (right padding; none for the
   all-valid rows the engine builds) -- applied structurally by the softmax
-  kernel, exactly as adding ``finfo(bf16).min`` does (exp underflows to 0).
+  kernel, exactly as adding ``finfo(bf16).min`` does (exp underflows to 0);
+* packed rows (no counterpart in the reference) come as a
+  :class:`~spilltune_amd.packed.SpanMask` and as
+  :class:`~spilltune_amd.packed.Positions` in the place of (cos, sin).
 """
 from __future__ import annotations
 
@@ -24,7 +27,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from . import ops
+from . import ops, packed
 
 
 @dataclass(frozen=True)
@@ -80,8 +83,9 @@ def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv
     feed-forward the Qwen3-MoE block of qwen3_moe.py:95-113 over the slot's
     ``mlp.experts.*`` stacks, with the optional per-expert LoRA objects
     ``lora_experts_gate_up`` / ``lora_experts_down``."""
-    if attention_mask is not None and not isinstance(attention_mask, CausalMask):
-        raise ValueError("unsupported_capability: only the causal mask marker is supported")
+    if attention_mask is not None and not isinstance(attention_mask, (CausalMask, packed.SpanMask)):
+        raise ValueError("unsupported_capability: only the causal mask marker and span masks are "
+                         "supported")
     if moe is not None and feed_forward is None:
         from . import moe as moe_ops
 
@@ -89,7 +93,12 @@ def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv
             return moe_ops.moe_feed_forward(x, w, lora_gate_up=lora_experts_gate_up,
                                             lora_down=lora_experts_down, **moe)
     B, S, Hd = hidden_states.shape
-    cos, sin = position_embeddings
+    by_position = isinstance(position_embeddings, packed.Positions)
+    if by_position and (position_embeddings.rotary.head_dim != head_dim
+                        or tuple(position_embeddings.positions.shape) != (B, S)):
+        raise ValueError(f"unsupported_capability: positions of other heads or rows than {B} x {S} "
+                         f"with heads of {head_dim}")
+    cos, sin = (None, None) if by_position else position_embeddings
     x2d = hidden_states.reshape(B * S, Hd)
     residual, xn = ops.rms_norm_residual(x2d, weights["input_layernorm.weight"], eps)
 
@@ -106,8 +115,17 @@ def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv
     # one after the other, k and v alone are too narrow to fill the GPU (2103
     # rows, 4096 wide: 99 + 74 + 74 us a pass against 95 in one, besides the
     # separate head norms, rotations and gradient adds: a step of 3.81 -> 3.38 ms)
-    if qkv is not None and ops.lora_fusable(loras_qkv, partial=True):
+    fused = qkv is not None and ops.lora_fusable(loras_qkv, partial=True)
+    if fused:
         y = ops.q4_lora_linear(xn, qkv, loras_qkv, partial=True)
+    elif by_position:
+        y = torch.cat([ops.q4_lora_linear(xn, w, [l]) for w, l in zip((wq, wk, wv), loras_qkv)], 1)
+    if by_position:
+        norms = (weights["self_attn.q_norm.weight"], weights["self_attn.k_norm.weight"]) if qk_norm \
+            else None
+        q, k, v = packed.rope_positions(y, position_embeddings.positions, position_embeddings.rotary,
+                                        heads, kv_heads, norms=norms, eps=eps)
+    elif fused:
         if qk_norm:
             # per-head q/k RMSNorm and the rotation in one kernel each way
             q, k, v = ops.rope_qkv_norm(y, B, S, heads, kv_heads, head_dim, cos, sin,
@@ -123,9 +141,12 @@ def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv
         v = ops.rope_heads(ops.q4_lora_linear(xn, wv, [lora_v]), 0, B, S, kv_heads, head_dim, cos,
                            sin, rotate=False)
 
-    kv_len = attention_mask.lengths if attention_mask is not None else None
-    attended = ops.causal_attention(q, k, v, ops.attention_scale(head_dim),
-                                    kv_len).reshape(B * S, heads * head_dim)
+    if isinstance(attention_mask, packed.SpanMask):
+        attended = packed.span_attention(q, k, v, ops.attention_scale(head_dim), attention_mask)
+    else:
+        kv_len = attention_mask.lengths if attention_mask is not None else None
+        attended = ops.causal_attention(q, k, v, ops.attention_scale(head_dim), kv_len)
+    attended = attended.reshape(B * S, heads * head_dim)
     h1 = ops.q4_lora_linear(attended, _weight(weights, "self_attn.o_proj"), [lora_o], residual=residual)
 
     h1, xn2 = ops.rms_norm_residual(h1, weights["post_attention_layernorm.weight"], eps)

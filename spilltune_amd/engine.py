@@ -18,6 +18,10 @@ I/O around it).
   cyclic rows (engine.py:162-182), microbatch-major as the reference or
   layer-major (:func:`window_layer_major`: one layer load per phase per
   accumulation window instead of one per microbatch, same results).
+* Packed rows (``documents``: several documents in a row, see
+  :mod:`spilltune_amd.packed`) in all of the above, an ``objective`` on token log
+  probabilities in the place of the cross-entropy, and :func:`score`, the log
+  probabilities of given rows; these have no counterpart in the reference.
 * :class:`DenseModel` -- the adapter surface the engine uses
   (adapters/protocol.py:23-34) for a Llama-family model whose decoder
   matrices are stored 4-bit.
@@ -29,7 +33,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import ops, slots
+from . import ops, packed, slots
 from .dense import positions_and_masks
 from .recompute import (_borrow_weights, _call_functional_block, block_adapter_backward,
                         streaming_block)
@@ -58,19 +62,43 @@ def forward(model, session, hidden, positions, masks, *, accumulate=False):
     return hidden
 
 
-def microbatch(model, session, input_ids, labels, *, normalization, token_chunk, accumulate=False):
-    """Exact shifted summed CE / window token count; one decoder backward."""
+def _row_inputs(model, input_ids, documents):
+    """Positions and masks of a batch: all-valid rows, or packed documents."""
+    if documents is None:
+        return model.positions_and_masks(torch.ones_like(input_ids, dtype=torch.bool))
+    if documents.shape != input_ids.shape:
+        raise ValueError("unsupported_capability: documents must be shaped like the token rows")
+    return model.packed_positions_and_masks(documents)
+
+
+def _terminal(model, normalized, labels, *, normalization, token_chunk, objective):
+    """The summed cross-entropy over ``normalization``, or the scalar that
+    ``objective`` makes of the labels' log probabilities (row ``t`` of the
+    :class:`~spilltune_amd.ops.TokenLogProbs` is label ``t + 1``; 0 at -100)."""
+    if objective is not None:
+        return objective(ops.token_logprobs(normalized[:, :-1], model.head,
+                                            labels[:, 1:].to(torch.int64)))
+    chunks = ops.supervised_chunk_intervals(labels, token_chunk)
+    return ops.chunked_causal_loss(normalized, model.head, labels,
+                                   normalization=normalization, token_chunk=token_chunk,
+                                   supervised_chunks=chunks)
+
+
+def microbatch(model, session, input_ids, labels, *, normalization, token_chunk, accumulate=False,
+               documents=None, objective=None):
+    """Exact shifted summed CE / window token count; one decoder backward.
+    ``documents``: packed rows (labels across a document's start are dropped);
+    ``objective``: see :func:`_terminal`."""
     device = model.device
-    valid = torch.ones_like(input_ids, dtype=torch.bool)
-    positions, masks = model.positions_and_masks(valid)
+    positions, masks = _row_inputs(model, input_ids, documents)
+    if documents is not None:
+        labels = packed.document_labels(labels, documents)
     embedded = F.embedding(input_ids.cpu(), model.embedding).to(device).detach().requires_grad_(True)
     hidden = forward(model, session, embedded, positions, masks, accumulate=accumulate)
     terminal_input = hidden.detach().requires_grad_(True)
     normalized = model.terminal_norm(terminal_input)
-    chunks = ops.supervised_chunk_intervals(labels, token_chunk)
-    loss = ops.chunked_causal_loss(normalized, model.head, labels,
-                                   normalization=normalization, token_chunk=token_chunk,
-                                   supervised_chunks=chunks)
+    loss = _terminal(model, normalized, labels, normalization=normalization,
+                     token_chunk=token_chunk, objective=objective)
     (gradient,) = torch.autograd.grad(loss, terminal_input)
     if not torch.isfinite(loss) or not torch.isfinite(gradient).all():
         raise FloatingPointError("non-finite causal loss/gradient")
@@ -78,7 +106,22 @@ def microbatch(model, session, input_ids, labels, *, normalization, token_chunk,
     return float(loss.detach()), embedded.grad.detach().clone()
 
 
-def window_layer_major(model, session, items, *, normalization, token_chunk):
+def score(model, session, input_ids, *, documents=None, top=0, temperature=1.0):
+    """Log probabilities of given rows under the model, no gradients: a
+    :class:`~spilltune_amd.ops.TokenLogProbs` of [batch, length - 1], whose entry
+    ``t`` is token ``t + 1`` after the tokens up to ``t`` (0 where ``documents``
+    starts another document or padding there), with the entropy and the ``top``
+    alternatives of that place."""
+    with torch.no_grad():
+        positions, masks = _row_inputs(model, input_ids, documents)
+        tokens = input_ids if documents is None else packed.document_labels(input_ids, documents)
+        embedded = F.embedding(input_ids.cpu(), model.embedding).to(model.device)
+        normalized = model.terminal_norm(forward(model, session, embedded, positions, masks))
+        return ops.token_logprobs(normalized[:, :-1], model.head, tokens[:, 1:].to(torch.int64),
+                                  top=top, temperature=temperature)
+
+
+def window_layer_major(model, session, items, *, normalization, token_chunk, objective=None):
     """One gradient-accumulation window processed layer by layer, so each
     layer's 4-bit image crosses PCIe once per phase instead of once per
     microbatch (the reference streams every layer for every microbatch,
@@ -96,9 +139,10 @@ def window_layer_major(model, session, items, *, normalization, token_chunk):
     the same bits.  Returns the per-microbatch losses."""
     device = model.device
     mbs = []
-    for ids, labels in items:
-        valid = torch.ones_like(ids, dtype=torch.bool)
-        positions, masks = model.positions_and_masks(valid)
+    for ids, labels, *documents in items:
+        positions, masks = _row_inputs(model, ids, *documents or [None])
+        if documents and documents[0] is not None:
+            labels = packed.document_labels(labels, documents[0])
         embedded = F.embedding(ids.cpu(), model.embedding).to(device)
         mbs.append({"pos": positions, "masks": masks, "h": [embedded], "labels": labels})
     for block in model.blocks:
@@ -111,10 +155,8 @@ def window_layer_major(model, session, items, *, normalization, token_chunk):
     for mb in mbs:
         terminal_input = mb["h"].pop().detach().requires_grad_(True)
         normalized = model.terminal_norm(terminal_input)
-        loss = ops.chunked_causal_loss(
-            normalized, model.head, mb["labels"], normalization=normalization,
-            token_chunk=token_chunk,
-            supervised_chunks=ops.supervised_chunk_intervals(mb["labels"], token_chunk))
+        loss = _terminal(model, normalized, mb["labels"], normalization=normalization,
+                         token_chunk=token_chunk, objective=objective)
         (mb["g"],) = torch.autograd.grad(loss, terminal_input)
         if not torch.isfinite(loss) or not torch.isfinite(mb["g"]).all():
             raise FloatingPointError("non-finite causal loss/gradient")
@@ -164,29 +206,34 @@ class AdamW:
 
 
 def train(model, session, rows, *, steps, accumulation=1, lr=1e-4, weight_decay=0.0,
-          token_chunk=64, layer_major=False):
+          token_chunk=64, layer_major=False, objective=None):
     """Optimizer-step loop with cyclic rows (engine.py:162-182); returns losses.
+    Rows are ``(ids, labels)`` or, packed, ``(ids, labels, documents)``.
     ``layer_major`` runs each accumulation window with ``window_layer_major``
-    (same results, one layer load per phase per window)."""
+    (same results, one layer load per phase per window).  ``objective``: in the
+    place of the cross-entropy, see :func:`microbatch`."""
     projections = flatten(model)
     optimizer = AdamW(lr=lr, weight_decay=weight_decay)
     cursor, losses = 0, []
     for _ in range(steps):
         items = [rows[(cursor + i) % len(rows)] for i in range(accumulation)]
-        normalization = sum(int((labels[:, 1:] != -100).sum()) for _, labels in items)
+        normalization = sum(
+            int(((labels if not docs or docs[0] is None else packed.document_labels(labels, docs[0]))
+                 [:, 1:] != -100).sum()) for _, labels, *docs in items)
         optimizer.zero_grad(projections)
         loss = 0.0
         with session.run():
             if layer_major:
                 for micro in window_layer_major(model, session, items,
                                                 normalization=normalization,
-                                                token_chunk=token_chunk):
+                                                token_chunk=token_chunk, objective=objective):
                     loss += micro
             else:
-                for i, (ids, labels) in enumerate(items):
+                for i, (ids, labels, *docs) in enumerate(items):
                     micro, _ = microbatch(model, session, ids, labels,
                                           normalization=normalization, token_chunk=token_chunk,
-                                          accumulate=i > 0)
+                                          accumulate=i > 0, documents=docs[0] if docs else None,
+                                          objective=objective)
                     loss += micro
             optimizer.step(projections)
         cursor += accumulation
@@ -200,14 +247,17 @@ class DenseModel:
 
     def __init__(self, *, embedding, norm, head, layers=None, heads, kv_heads, head_dim, eps,
                  theta, rank, alpha, targets, device, codec="nf4-g128", generator=None,
-                 blocks=None, qk_norm=False):
+                 blocks=None, qk_norm=False, rotary=None):
         """``layers``: per-layer weight dicts, encoded here; or ``blocks``:
-        prebuilt BlockPlans (e.g. ``slots.make_archive_block``)."""
+        prebuilt BlockPlans (e.g. ``slots.make_archive_block``).  ``rotary``: the
+        :class:`~spilltune_amd.packed.Rotary` of packed rows (default: whole
+        heads, ``theta``, no scaling)."""
         self.device = torch.device(device)
         self.embedding = embedding.to(torch.bfloat16).contiguous()      # stays on the host
         self.norm = norm.to(torch.bfloat16).to(self.device)
         self.head = head.to(torch.bfloat16).to(self.device)
         self.eps, self.theta, self.head_dim = eps, theta, head_dim
+        self.rotary = rotary
         if (layers is None) == (blocks is None):
             raise ValueError("DenseModel needs exactly one of layers / blocks")
         self.blocks = list(blocks) if blocks is not None else [
@@ -221,6 +271,13 @@ class DenseModel:
         rot, mask = positions_and_masks(valid, head_dim=self.head_dim, theta=self.theta,
                                         device=self.device)
         return rot, {"full_attention": mask}
+
+    def packed_positions_and_masks(self, documents, **kw):
+        """Positions and masks of packed rows (packed.positions_and_masks)."""
+        if self.rotary is None:
+            self.rotary = packed.Rotary(self.head_dim, self.theta, device=self.device)
+        positions, mask = packed.positions_and_masks(documents, self.rotary, **kw)
+        return positions, {"full_attention": mask}
 
     def terminal_norm(self, hidden):
         B, S, H = hidden.shape

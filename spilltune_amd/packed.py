@@ -9,6 +9,8 @@ adapters/dense.py:232-248); these have no counterpart there.
   the kernels' tile plan.  Made once for a batch and read by every layer.
 * :func:`span_attention` -- attention over those runs, optionally with scores
   capped by a tanh and a bias that falls with the distance, differentiable.
+* :func:`positions_and_masks` and :func:`document_labels` -- what a model's
+  blocks and its loss take for a batch of packed rows.
 * :class:`Rotary` and :func:`rope_positions` -- rotation of query and key heads
   by per-token positions: whole heads or a part of them, half or interleaved
   pairs, the scalings for long contexts, optionally after Qwen3's per-head norms.
@@ -345,5 +347,37 @@ def rope_positions(y, positions, rotary: Rotary, heads: int, kv_heads: int, *, n
                                 float(eps))
 
 
+# ----------------------------------------------------------------- a model's packed rows
+@dataclass(frozen=True)
+class Positions:
+    """Position embeddings of packed rows for a decoder block: per-token
+    positions (int32 [batch, length]) and the rotary embedding they turn by, in
+    the place of (cos, sin) tables."""
+    positions: torch.Tensor = field(compare=False)
+    rotary: Rotary = field(compare=False)
+
+
+def positions_and_masks(documents: torch.Tensor, rotary: Rotary, *, bidirectional=None, window=None):
+    """``(Positions, SpanMask)`` of packed rows, in the place of
+    ``dense.positions_and_masks``; ``documents`` and ``bidirectional`` as for
+    :func:`document_mask`, from the host or the device."""
+    move = lambda t: None if t is None else t.to(rotary.device)  # noqa: E731
+    mask = document_mask(move(documents), bidirectional=move(bidirectional), window=window)
+    return Positions(mask.positions, rotary), mask
+
+
+def document_labels(labels: torch.Tensor, documents: torch.Tensor) -> torch.Tensor:
+    """``labels`` with -100 where no token of the same document comes before: a
+    document's first token is not predicted from another document's last, and
+    padding is not predicted at all."""
+    if labels.shape != documents.shape or labels.dim() != 2:
+        raise ValueError("unsupported_capability: labels and documents must be [batch, length]")
+    documents = documents.to(labels.device)
+    follows = torch.zeros(labels.shape, dtype=torch.bool, device=labels.device)
+    follows[:, 1:] = (documents[:, 1:] == documents[:, :-1]) & (documents[:, 1:] >= 0)
+    return torch.where(follows, labels, -100)
+
+
 __all__ = ["SpanMask", "span_mask", "document_runs", "document_mask", "span_attention",
-           "rotary_frequencies", "Rotary", "rope_positions"]
+           "rotary_frequencies", "Rotary", "rope_positions", "Positions", "positions_and_masks",
+           "document_labels"]

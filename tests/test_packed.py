@@ -7,7 +7,7 @@ import random
 import pytest
 import torch
 
-from spilltune_amd import _lib, deepseek, packed
+from spilltune_amd import _lib, deepseek, dense, engine, packed
 from tests._packed_ref import rope_ref, runs_brute, span_forward, span_ref
 
 
@@ -216,3 +216,25 @@ def test_rope_reference_gradients_against_differences(interleaved):
     assert torch.autograd.gradcheck(
         lambda t: rope_ref(t, pos, inv, 1.3, heads, kv, D, rot, interleaved, w), (y,), eps=1e-6,
         atol=1e-7, rtol=1e-6)
+
+
+def test_block_refuses_positions_of_other_rows():
+    z = torch.zeros(1, 4, 256, dtype=torch.bfloat16)
+    pos = packed.Positions(torch.zeros(1, 4, dtype=torch.int32), packed.Rotary(64, 1e4, device="cpu"))
+    for head_dim, h in ((128, z), (64, z[:, :3])):
+        with pytest.raises(ValueError, match="positions of other"):
+            dense.dense_block(h, pos, None, heads=4, kv_heads=4, head_dim=head_dim, eps=1e-5)
+    with pytest.raises(ValueError, match="causal mask marker and span masks"):
+        dense.dense_block(z, pos, "mask", heads=4, kv_heads=4, head_dim=64, eps=1e-5)
+
+
+def test_engine_refuses():
+    model, session = object(), object()
+    ids = torch.zeros(1, 4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="shaped like"):
+        engine.score(model, session, ids, documents=ids[:, :3])
+    with pytest.raises(ValueError, match="labels and documents"):
+        packed.document_labels(ids, ids[0])
+    assert packed.document_labels(torch.arange(6).view(1, 6),
+                                  torch.tensor([[0, 0, 1, 1, -1, -1]])).tolist() \
+        == [[-100, 1, -100, 3, -100, -100]]
