@@ -454,12 +454,11 @@ int64_t st_span_plan_bytes(int64_t B, int64_t S);
 int st_span_plan(const int32_t* key_start, const int32_t* key_end, int64_t B, int64_t S, void* plan,
                  int64_t plan_bytes, st_stream_t stream);
 int64_t st_span_attn_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t DQ,
-                                     int64_t DV, int32_t backward);
+                                     int64_t DV); /* of the backward */
 int st_span_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B, int64_t S,
                      int64_t H, int64_t Hkv, int64_t DQ, int64_t DV, float scale, float cap,
                      const float* slopes, const int32_t* key_start, const int32_t* key_end,
-                     const void* plan, uint16_t* out, float* lse, void* workspace,
-                     int64_t workspace_bytes, st_stream_t stream);
+                     const void* plan, uint16_t* out, float* lse, st_stream_t stream);
 int st_span_attn_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* out,
                      const float* lse, const uint16_t* dout, int64_t B, int64_t S, int64_t H,
                      int64_t Hkv, int64_t DQ, int64_t DV, float scale, float cap,

@@ -108,9 +108,9 @@ _SIGNATURES = {
                                _I64, _I32, _P, _P, _P, _P, _I64, _P]),
     "st_span_plan_bytes": (_I64, [_I64, _I64]),
     "st_span_plan": (_I32, [_P, _P, _I64, _I64, _P, _I64, _P]),
-    "st_span_attn_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I32]),
+    "st_span_attn_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "st_span_attn_fwd": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _F, _P, _P, _P,
-                                _P, _P, _P, _P, _I64, _P]),
+                                _P, _P, _P, _P]),
     "st_span_attn_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _F,
                                 _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "st_token_logprobs_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I32]),

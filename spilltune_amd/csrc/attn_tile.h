@@ -32,20 +32,23 @@ struct RowCopy {
   static constexpr int rows = NT / (D / 8);
 };
 
-// Row-major [rows][D] LDS tile, 16-byte chunks XOR-swizzled by row.  For
-// D = 128 (rows of 256 bytes, each starting at bank 0) the XOR value
-// ((row & 3) << 2) | ((row >> 2) & 3) is a permutation of row & 15, so the
-// 16 rows of a quarter-wave 16-byte read (tile_row) land on 16 distinct chunk
-// positions, and the 4 rows x 4 chunks of a half-wave transposing 8-byte read
-// (tile_tr: rows 4 apart in bits 2-3 of the XOR value, chunks in bits 0-1)
-// land on 16 distinct chunks: both are free of bank conflicts.  Other widths
-// keep the XOR value ((row & 7) << 1), which stays inside the row's chunks.
+// Row-major [rows][D] LDS tile, 16-byte chunks XOR-swizzled by row.  A
+// quarter-wave 16-byte read (tile_row: one chunk of 16 rows) and a half-wave
+// transposing 8-byte read (tile_tr: 4 chunks of 4 rows, both aligned) must each
+// land on 16 distinct positions of the 64 banks.  D = 128: a row is 256 bytes
+// and starts at bank 0, so the XOR value ((row & 3) << 2) | ((row >> 2) & 3), a
+// permutation of row & 15, serves both (rows apart in bits 2-3, chunks in bits
+// 0-1).  D = 64 and 192: rows start at bank 0 and 32 in turn, the XOR value must
+// stay below 8 and differ among the 8 rows of one parity, in bit 2 among
+// neighbours of one parity: ((row & 2) << 1) | ((row >> 2) & 3).  Measured
+// without bank conflicts (SQ_LDS_BANK_CONFLICT).
 template <int D>
 __device__ __forceinline__ int swz(int row) {
+  static_assert(D == 64 || D == 128 || D == 192, "row lengths");
   if constexpr (D == 128)
     return ((row & 3) << 2) | ((row >> 2) & 3);
   else
-    return ((row & 7) << 1) & (D / 8 - 1);
+    return ((row & 2) << 1) | ((row >> 2) & 3);
 }
 template <int D>
 __device__ __forceinline__ int tswz(int row, int chunk) {
@@ -71,6 +74,40 @@ __device__ __forceinline__ bf16x8 tile_tr(const uint16_t* t, int kb, int nb, int
     const int row = kb + 8 * h + 4 * g + (i >> 2);
     const uint16_t* p = t + tswz<D>(row, col >> 3) + (col & 7);
     r[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) v4bf*)p);
+  }
+  return __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// The same two operands by a lane's own address: `lane_row` / `lane_tr` once,
+// then one exclusive-or with a constant per read, the rest in the instruction's
+// offset (the row's chunks stay within aligned bits of the byte address).
+template <int D>
+__device__ __forceinline__ uint32_t lane_row(int row, int g) {
+  return (uint32_t)(row * D * 2 + ((g ^ swz<D>(row)) << 4));
+}
+template <int D>  // chunk 2 s + g of row `row0` + the lane's, row0 a multiple of 16
+__device__ __forceinline__ bf16x8 read_row(const uint16_t* t, uint32_t lane, int row0, int s) {
+  constexpr int IN = D == 128 ? 15 : 7;  // chunks that the swizzle permutes
+  const uint32_t at = (lane ^ (uint32_t)((2 * s & IN) << 4)) + (2 * s & ~IN) * 16 + row0 * D * 2;
+  return as_bf16x8(*(const uint4*)((const char*)t + at));
+}
+template <int D>
+__device__ __forceinline__ uint32_t lane_tr(int lane) {
+  const int G = lane >> 4, i = lane & 15, g = lane >> 5, row = 4 * g + (i >> 2);
+  const int chunk = 2 * (G & 1) + ((i & 3) >> 1);
+  return (uint32_t)(row * D * 2 + ((chunk ^ swz<D>(row)) << 4) + (i & 1) * 8);
+}
+template <int D>  // tile_tr(t, kb, 32 db), kb a multiple of 16
+__device__ __forceinline__ bf16x8 read_tr(const uint16_t* t, uint32_t lane, int kb, int db) {
+  constexpr int IN = D == 128 ? 15 : 7;
+  typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+  v4bf r[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // 8 rows on, swz flips bit 1
+    const uint32_t at = (lane ^ (uint32_t)(((4 * db & IN) ^ (2 * h)) << 4)) + (4 * db & ~IN) * 16 +
+                        (kb + 8 * h) * D * 2;
+    r[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+        (__attribute__((address_space(3))) v4bf*)((const char*)t + at));
   }
   return __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }

@@ -5,14 +5,19 @@
 //
 //   x[i,j] = cap * tanh(scale * q_i.k_j / cap) - slope[h] * |i - j|
 //   P[i,:] = softmax of x[i,:] over the seen keys,   o_i = sum_j P[i,j] v_j
-//   dP = dO V^T,  delta_i = dO_i . o_i,  dx = P (dP - delta)
+//   dP = dO V^T,  delta_i = sum_j P dP = dO_i . o_i,  dx = P (dP - delta)
 //   dS = dx * (1 - tanh^2),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
 //
 // Layout as the causal kernels (attention.hip): q [B,H,S,DQ], k [B,Hkv,S,DQ],
 // v [B,Hkv,S,DV] head-major bf16, out and dout token-major [B,S,H*DV], lse
 // [B,H,S] fp32 the base-2 log-sum-exp (+inf for a query that sees no key, so
 // every probability recomputed from it is 0).  Scores, statistics and sums are
-// fp32; probabilities and dS are rounded to bf16 for their MFMA products.
+// fp32.  Probabilities are rounded to bf16 for their MFMA products, dS is split
+// into two bf16 parts (2^-17): the second product reads no operand of its own
+// and cost 3-7% of a pass.  delta from the rounded output is off by 2^-9 of
+// |dO||o|, which counts where few keys share the weight, so a tile whose queries
+// see at most SHORT keys in all sums P dP itself, in a sweep of its own before
+// dQ's.  A query that sees one key has dS = 0, and gets exactly that.
 //
 // A plan (span_plan below, made once per mask) holds for each 32-query block
 // the extremes of its runs, for each 128-key tile the query blocks that see it,
@@ -22,10 +27,11 @@
 // Masked places never reach a result: a masked score is replaced, not added to,
 // but an infinity or NaN in a key, value or gradient row that a 32-row block
 // partly sees does meet a zero probability inside an MFMA product.  A wave that
-// ends with a sum that is not finite says so in a flag, and `span_fix_*` redoes
-// those rows over the seen pairs alone.
+// ends with a sum that is not finite has its rows redone over the seen pairs
+// alone, by its whole workgroup, before the kernel ends (redo_*).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attn_tile.h"
 
@@ -37,6 +43,7 @@ constexpr int NT = 256;
 constexpr int TILE = 128;  // queries (dQ, forward) or keys (dK, dV) per workgroup
 constexpr int BKT = 64;    // keys per step of the forward and dQ passes
 constexpr int QT = 64;     // queries per step of the dK/dV pass
+constexpr int SHORT = 256;   // keys of a tile whose delta is summed from P dP
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_LOG2 = 8.0f;  // the running maximum may lag by up to 2^8
 
@@ -45,12 +52,14 @@ constexpr float RESCALE_LOG2 = 8.0f;  // the running maximum may lag by up to 2^
 // least and greatest run end of 32 queries; an empty run makes the greatest
 // start INT_MAX and the least end 0, so the block is never taken for wholly
 // visible), key tiles int2 [B, nt] (first query block that sees the tile, end),
-// query and key tiles by falling work [B*nt] each, and their work [B*nt] each.
+// query and key tiles [B*nt] by falling work, their work (keys of the tile's
+// queries; query blocks of the tile's keys), the key tiles' sum (0 where the
+// tiles were not sorted).
 struct Plan {
   const int4* blk;
   const int2* keys;
   const int32_t *qorder, *korder;
-  int32_t *qwork, *kwork;
+  int32_t *qwork, *kwork, *ktotal;
   int nb, nt;
   int64_t bytes;
 };
@@ -72,6 +81,8 @@ Plan plan_of(const void* base, int64_t B, int64_t S) {
   w += B * nt;
   p.kwork = w;
   w += B * nt;
+  p.ktotal = w;
+  w += 1;
   p.bytes = (char*)w - (char*)base;
   return p;
 }
@@ -103,7 +114,7 @@ __global__ __launch_bounds__(NT) void span_blocks(const int32_t* __restrict__ lo
   if ((threadIdx.x & 31) == 0) blk[id] = x;
 }
 
-// per 128-row tile: the work of its queries, and the query blocks that see it as keys
+// per 128-row tile: the query blocks that see it as keys, and the work of both kinds
 __global__ __launch_bounds__(64) void span_tiles(const int4* __restrict__ blk, int nb, int nt,
                                                  int2* __restrict__ keys, int32_t* __restrict__ qwork,
                                                  int32_t* __restrict__ kwork) {
@@ -140,25 +151,32 @@ __global__ __launch_bounds__(64) void span_tiles(const int4* __restrict__ blk, i
 }
 
 // tiles by falling work (ties by index): each counts those before it; more
-// tiles than `sorted` keep their own order (the count is quadratic)
+// tiles than SORT_LIMIT keep their own order (the count is quadratic)
+constexpr int64_t SORT_LIMIT = 16384;
 __global__ __launch_bounds__(NT) void span_order(const int32_t* __restrict__ qwork,
                                                  const int32_t* __restrict__ kwork, int64_t n,
-                                                 int sorted, int32_t* __restrict__ qorder,
-                                                 int32_t* __restrict__ korder) {
-  const int32_t* w = blockIdx.y ? kwork : qwork;
-  int32_t* o = blockIdx.y ? korder : qorder;
+                                                 int32_t* __restrict__ qorder,
+                                                 int32_t* __restrict__ korder,
+                                                 int32_t* __restrict__ ktotal) {
+  const bool keys = blockIdx.y != 0;
+  const int32_t* w = keys ? kwork : qwork;
+  int32_t* o = keys ? korder : qorder;
   const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
   if (i >= n) return;
-  if (!sorted) {
+  if (n > SORT_LIMIT) {
     o[i] = (int32_t)i;
+    if (keys && i == 0) *ktotal = 0;
     return;
   }
   const int mine = w[i];
-  int64_t rank = 0;
-  for (int64_t j = 0; j < n; ++j) rank += w[j] > mine || (w[j] == mine && j < i);
+  int64_t rank = 0, sum = 0;
+  for (int64_t j = 0; j < n; ++j) {
+    rank += w[j] > mine || (w[j] == mine && j < i);
+    sum += w[j];
+  }
   o[rank] = (int32_t)i;
+  if (keys && i == 0) *ktotal = (int32_t)min(sum, (int64_t)INT_MAX);
 }
-constexpr int64_t SORT_LIMIT = 16384;
 
 // ---------------------------------------------------------------- shared
 struct Args {
@@ -168,7 +186,8 @@ struct Args {
   Plan plan;
   int S, H, Hkv;
   float scale, sl2;          // scale, scale * log2(e)
-  float cap_in, cap_out;     // MODE 1 with a cap: 2 log2(e) scale / cap, cap * log2(e); else 0
+  float cap_in, cap_out;     // with a cap: 2 log2(e) scale / cap, cap * log2(e)
+  float cap_small, cap_p[3]; // |s| up to which score_small holds, its coefficients
 };
 
 // Workgroup head index -> head, so that the query heads of a KV head share an
@@ -179,20 +198,60 @@ __device__ __forceinline__ int head_of(int x, int H, int Hkv) {
   return (x % 8 + 8 * (y / group)) * group + y % group;
 }
 
+// MODE: what is done to a score, CAP and BIAS
+constexpr int CAP = 1, BIAS = 2;
 // Base-2 score of a raw product s at distance `far` (>= 0); `grad`: d x / d (scale s).
+template <int MODE>
 __device__ __forceinline__ float score(const Args& a, float slope2, float s, float far, float& grad) {
   grad = 1.0f;
   float x = s * a.sl2;
-  if (a.cap_in != 0.0f) {
+  if constexpr ((MODE & CAP) != 0) {
     // tanh(y) = 1 - 2 r, r = 1 / (1 + e^2y); absolute error of a few 2^-24
     const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.cap_in));
     x = __builtin_fmaf(-2.0f * a.cap_out, r, a.cap_out);
     grad = 4.0f * r * (1.0f - r);
   }
-  return __builtin_fmaf(-slope2, far, x);
+  if constexpr ((MODE & BIAS) != 0) x = __builtin_fmaf(-slope2, far, x);
+  return x;
+}
+// tanh(y) = y + y z P(z), z = y^2, for |y| <= 0.35: P by least squares on
+// Chebyshev points, reweighted to level the relative error (4e-8).  Most capped
+// scores are there, and the polynomial takes half of the time of the exponential
+// and the reciprocal.  Callers choose it for a whole wave (Args::cap_small).
+__device__ __forceinline__ float score_small(const Args& a, float s) {
+  const float z = s * s;
+  float p = __builtin_fmaf(a.cap_p[2], z, a.cap_p[1]);
+  p = __builtin_fmaf(p, z, a.cap_p[0]);
+  return s * __builtin_fmaf(p, z, a.sl2);
 }
 
 __device__ __forceinline__ bool finite(float x) { return x - x == 0.0f; }
+// 0 if every value is finite
+template <int N>
+__device__ __forceinline__ float probe_of(const f32x16 (&acc)[N]) {
+  float p = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) p = __builtin_fmaf(acc[i][v], 0.0f, p);
+  return p;
+}
+// eight fp32 values as bf16 `hi` and what the rounding left as bf16 `lo`
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8& hi, bf16x8& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = st::pack_bf16x2(x[2 * e], x[2 * e + 1]);
+    l[e] = st::pack_bf16x2(x[2 * e] - __uint_as_float(h[e] << 16),
+                           x[2 * e + 1] - __uint_as_float(h[e] & 0xffff0000u));
+  }
+  hi = as_bf16x8(make_uint4(h[0], h[1], h[2], h[3]));
+  lo = as_bf16x8(make_uint4(l[0], l[1], l[2], l[3]));
+}
+__device__ __forceinline__ bf16x8 pack8(const float (&x)[8]) {
+  return as_bf16x8(make_uint4(st::pack_bf16x2(x[0], x[1]), st::pack_bf16x2(x[2], x[3]),
+                              st::pack_bf16x2(x[4], x[5]), st::pack_bf16x2(x[6], x[7])));
+}
 
 // copies of the K and V tiles of a step, as RowCopy lays them out
 template <int D, int NTHR, int ROWS>
@@ -258,6 +317,29 @@ __device__ __forceinline__ int4 uniform(int4 x) {
   return make_int4(uniform(x.x), uniform(x.y), uniform(x.z), uniform(x.w));
 }
 
+// the same in fp32 (`os`: 32 rows of D + 4 floats)
+template <int D>
+__device__ __forceinline__ void store_rows_f32(const f32x16 (&acc)[D / 32], float mul, float* os,
+                                               int lane, int rows, float* out) {
+  constexpr int LDO = D + 4;
+  const int g = lane >> 5, c = lane & 31;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int v4 = 0; v4 < 4; ++v4)
+      *(float4*)(os + c * LDO + db * 32 + v4 * 8 + g * 4) =
+          make_float4(acc[db][4 * v4] * mul, acc[db][4 * v4 + 1] * mul, acc[db][4 * v4 + 2] * mul,
+                      acc[db][4 * v4 + 3] * mul);
+  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_wave_barrier();
+  for (int i = lane; i < 32 * (D / 4); i += 64) {
+    const int r = i / (D / 4), ch = i % (D / 4);
+    if (r < rows) *(float4*)(out + r * D + ch * 4) = *(const float4*)(os + r * LDO + ch * 4);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Key range of a 128-query tile and the wave's own block of extremes.
 struct Walk {
   int4 mine;       // of this wave's 32 queries
@@ -277,6 +359,195 @@ __device__ __forceinline__ Walk walk_of(const Plan& p, int b, int qt, int wave) 
   return w;
 }
 
+// ---------------------------------------------------------------- redone rows
+// A 32-row block whose sums are not finite, over the seen pairs alone, by the
+// whole workgroup (NTH threads).  Correct, not fast: no block comes here while
+// the operands are finite.  `mem`: LDS that the tiles no longer need.
+template <int D>
+__device__ float dot(const uint16_t* __restrict__ x, const uint16_t* __restrict__ y) {
+  float s = 0.0f;
+#pragma unroll 1
+  for (int d = 0; d < D; d += 8) {
+    const uint4 u = ld_global16(x + d), w = ld_global16(y + d);
+    const uint32_t p[4] = {u.x, u.y, u.z, u.w}, r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = __builtin_fmaf(__uint_as_float(p[e] << 16), __uint_as_float(r[e] << 16), s);
+      s = __builtin_fmaf(__uint_as_float(p[e] & 0xffff0000u), __uint_as_float(r[e] & 0xffff0000u), s);
+    }
+  }
+  return s;
+}
+template <bool MAX, int NTH>
+__device__ __forceinline__ float block_reduce(float x, float* red) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    const float y = __shfl_xor(x, d);
+    x = MAX ? fmaxf(x, y) : x + y;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = red[0];
+  for (int i = 1; i < NTH / 64; ++i) x = MAX ? fmaxf(x, red[i]) : x + red[i];
+  return x;
+}
+// calls fn(wave, mem) for each wave that is bad; every thread of the workgroup
+// comes here, its tiles and staging no longer needed
+template <int NTH, typename F>
+__device__ __forceinline__ void redo(bool bad, int wave, int lane, float* lds, F&& fn) {
+  __syncthreads();
+  if (lane == 0) lds[wave] = bad ? 1.0f : 0.0f;
+  __syncthreads();
+  unsigned set = 0;
+#pragma unroll
+  for (int w = 0; w < NTH / 64; ++w) set |= lds[w] != 0.0f ? 1u << w : 0u;
+  if (set == 0) return;
+  __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < NTH / 64; ++w)
+    if (set >> w & 1) fn(w, lds);
+}
+
+template <int DQ, int DV, int MODE>
+__device__ void redo_fwd(const Args& a, int b, int h, int i0, uint16_t* __restrict__ out,
+                         float* __restrict__ lse, float* mem) {
+  const int tid = threadIdx.x, S = a.S, H = a.H;
+  float *red = mem, *ps = mem + 64;
+  const int64_t bh = (int64_t)b * H + h;
+  const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
+  const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
+  const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
+#pragma unroll 1
+  for (int i = i0; i < min(i0 + 32, S); ++i) {
+    const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
+    uint16_t* o_row = out + ((int64_t)b * S + i) * H * DV + (int64_t)h * DV;
+    if (run.x >= run.y) {
+      if (tid < DV) o_row[tid] = 0;
+      if (tid == 0) lse[bh * S + i] = INFINITY;
+      continue;
+    }
+    const uint16_t* qi = a.q + (bh * S + i) * DQ;
+    auto x_of = [&](int j) {
+      float grad;
+      return score<MODE>(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ), fabsf((float)(i - j)), grad);
+    };
+    float m = -INFINITY;
+#pragma unroll 1
+    for (int j = run.x + tid; j < run.y; j += NT) m = fmaxf(m, x_of(j));
+    m = block_reduce<true, NT>(m, red);
+    float l = 0.0f, o = 0.0f;
+#pragma unroll 1
+    for (int c0 = run.x; c0 < run.y; c0 += NT) {
+      const float p = c0 + tid < run.y ? __builtin_amdgcn_exp2f(x_of(c0 + tid) - m) : 0.0f;
+      l += p;
+      __syncthreads();
+      ps[tid] = p;
+      __syncthreads();
+      if (tid < DV)
+#pragma unroll 1
+        for (int j = c0; j < min(c0 + NT, run.y); ++j)
+          o = __builtin_fmaf(ps[j - c0], st::bf16_to_f32(vb[(int64_t)j * DV + tid]), o);
+    }
+    l = block_reduce<false, NT>(l, red);
+    if (tid < DV) o_row[tid] = st::f32_to_bf16(o / l);
+    if (tid == 0) lse[bh * S + i] = m + log2f(l);
+  }
+}
+
+template <int DQ, int DV, int MODE>
+__device__ void redo_dq(const Args& a, int b, int h, int i0, const uint16_t* __restrict__ dout,
+                        const float* __restrict__ lse, const float* delta,
+                        uint16_t* __restrict__ dq, float* mem) {
+  const int tid = threadIdx.x, S = a.S, H = a.H;
+  const int64_t bh = (int64_t)b * H + h;
+  const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
+  const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
+  const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
+#pragma unroll 1
+  for (int i = i0; i < min(i0 + 32, S); ++i) {
+    const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
+    const uint16_t* qi = a.q + (bh * S + i) * DQ;
+    const uint16_t* gi = dout + ((int64_t)b * S + i) * H * DV + (int64_t)h * DV;
+    const float li = lse[bh * S + i], di = delta[bh * S + i];
+    float o = 0.0f;
+#pragma unroll 1
+    for (int c0 = run.x; c0 < run.y; c0 += NT) {
+      const int j = c0 + tid;
+      float ds = 0.0f;
+      if (j < run.y) {
+        float grad;
+        const float x = score<MODE>(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ),
+                                    fabsf((float)(i - j)), grad);
+        ds = __builtin_amdgcn_exp2f(x - li) * (dot<DV>(gi, vb + (int64_t)j * DV) - di) * grad;
+        if (run.y - run.x == 1) ds = 0.0f;
+      }
+      __syncthreads();
+      mem[tid] = ds;
+      __syncthreads();
+      if (tid < DQ)
+#pragma unroll 1
+        for (int jj = c0; jj < min(c0 + NT, run.y); ++jj)
+          o = __builtin_fmaf(mem[jj - c0], st::bf16_to_f32(kb[(int64_t)jj * DQ + tid]), o);
+    }
+    if (tid < DQ) dq[(bh * S + i) * DQ + tid] = st::f32_to_bf16(o * a.scale);
+  }
+}
+
+// keys [j0, j0 + 32) over the query heads [h0, h0 + heads) of KV head hk
+template <int DQ, int DV, int MODE, int NTH, typename W>
+__device__ void redo_dkdv(const Args& a, int b, int hk, int h0, int heads, int j0, int2 seen,
+                          const uint16_t* __restrict__ dout, const float* __restrict__ lse,
+                          const float* __restrict__ delta, float* mem, W&& write) {
+  const int tid = threadIdx.x, S = a.S, H = a.H;
+  float *ps = mem, *ds = mem + NTH, *vis = mem + 2 * NTH;
+  const int qa = seen.x * 32, qz = min(seen.y * 32, S);
+#pragma unroll 1
+  for (int j = j0; j < min(j0 + 32, S); ++j) {
+    const uint16_t* kj = a.k + (((int64_t)b * a.Hkv + hk) * S + j) * DQ;
+    const uint16_t* vj = a.v + (((int64_t)b * a.Hkv + hk) * S + j) * DV;
+    float sk = 0.0f, sv = 0.0f;  // this thread's column of dK, of dV
+#pragma unroll 1
+    for (int h = h0; h < h0 + heads; ++h) {
+      const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
+      const int64_t bh = (int64_t)b * H + h;
+      const uint16_t* gb = dout + (int64_t)b * S * H * DV + (int64_t)h * DV;
+#pragma unroll 1
+      for (int c0 = qa; c0 < qz; c0 += NTH) {
+        const int i = c0 + tid;
+        bool sees = false, one = false;
+        float p = 0.0f, d = 0.0f;
+        if (i < qz) {
+          const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
+          sees = run.x <= j && j < run.y;
+          one = run.y - run.x == 1;
+        }
+        if (sees) {
+          float grad;
+          const float x = score<MODE>(a, slope2, dot<DQ>(a.q + (bh * S + i) * DQ, kj),
+                                      fabsf((float)(i - j)), grad);
+          p = __builtin_amdgcn_exp2f(x - lse[bh * S + i]);
+          d = one ? 0.0f : p * (dot<DV>(gb + (int64_t)i * H * DV, vj) - delta[bh * S + i]) * grad;
+        }
+        __syncthreads();
+        ps[tid] = p;
+        ds[tid] = d;
+        vis[tid] = sees ? 1.0f : 0.0f;
+        __syncthreads();
+#pragma unroll 1
+        for (int q = c0; q < min(c0 + NTH, qz); ++q) {
+          if (vis[q - c0] == 0.0f) continue;
+          if (tid < DQ)
+            sk = __builtin_fmaf(ds[q - c0], st::bf16_to_f32(a.q[(bh * S + q) * DQ + tid]), sk);
+          if (tid < DV)
+            sv = __builtin_fmaf(ps[q - c0], st::bf16_to_f32(gb[(int64_t)q * H * DV + tid]), sv);
+        }
+      }
+    }
+    write(j, tid, sk * a.scale, sv);
+  }
+}
+
 // ---------------------------------------------------------------- forward
 // 4 waves of 32 queries over steps of 64 keys from the first key that the tile
 // sees; K and V tiles [key][D] in LDS, two buffers, one barrier a step.  Every
@@ -284,8 +555,7 @@ __device__ __forceinline__ Walk walk_of(const Plan& p, int b, int qt, int wave) 
 // V^T read by the transposing LDS loads.
 template <int DQ, int DV, int MODE>
 __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__ out,
-                                                  float* __restrict__ lse,
-                                                  int32_t* __restrict__ flags) {
+                                                  float* __restrict__ lse) {
   constexpr int DS = DQ / 16, DB = DV / 32, LK = BKT * DQ, LV = BKT * DV;
   static_assert(4 * 32 * (DV + 8) <= 2 * (LK + LV), "output staging fits");
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * (LK + LV)];
@@ -301,7 +571,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
   const int q0 = qt * TILE + wave * 32, myq = q0 + c;
   const Walk w = walk_of(a.plan, b, qt, wave);
   const int2 run = myq < S ? run_of(a.lo, a.hi, (int64_t)b * S + myq, S) : make_int2(0, 0);
-  const float slope2 = MODE && a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+  const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
 
   bf16x8 qf[DS];
 #pragma unroll
@@ -314,6 +584,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
 #pragma unroll
     for (int v = 0; v < 16; ++v) oacc[i][v] = 0.0f;
   float m_run = -INFINITY, l_run = 0.0f;
+  const uint32_t lr = lane_row<DQ>(c, g), lt = lane_tr<DV>(lane);
 
   const TileCopy<DQ, NT, BKT> ck(tid, DQ);
   const TileCopy<DV, NT, BKT> cv(tid, DV);
@@ -341,17 +612,39 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
       for (int s = 0; s < DS; ++s)
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
-          sacc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_row<DQ>(ks, jb * 32 + c, s, g),
+          sacc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DQ>(ks, lr, jb * 32, s),
                                                              qf[s], sacc[jb], 0, 0, 0);
-      if constexpr (MODE == 1) {
+      if constexpr ((MODE & CAP) != 0) {
+        float top = 0.0f;
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) top = fmaxf(top, fabsf(sacc[jb][v]));
+        // (a NaN product passes either way: both forms keep it)
+        if (__ballot(top > a.cap_small) == 0) {
+#pragma unroll
+          for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sacc[jb][v] = score_small(a, sacc[jb][v]);
+        } else {
+#pragma unroll
+          for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              float grad;
+              sacc[jb][v] = score<CAP>(a, 0.0f, sacc[jb][v], 0.0f, grad);
+            }
+        }
+      }
+      if constexpr ((MODE & BIAS) != 0) {
         const float far0 = (float)(myq - k0 - 4 * g);
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            float grad;
-            sacc[jb][v] = score(a, slope2, sacc[jb][v],
-                                fabsf(far0 - (float)(jb * 32 + (v >> 2) * 8 + (v & 3))), grad);
+            const float x = (MODE & CAP) ? sacc[jb][v] : sacc[jb][v] * a.sl2;
+            sacc[jb][v] = __builtin_fmaf(
+                -slope2, fabsf(far0 - (float)(jb * 32 + (v >> 2) * 8 + (v & 3))), x);
           }
       }
       if (edge) {
@@ -364,7 +657,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
             sacc[jb][v] = (unsigned)(jb * 32 + (v >> 2) * 8 + (v & 3) - base) < width
                               ? sacc[jb][v] : -INFINITY;
       }
-      const float mul = MODE == 1 ? 1.0f : a.sl2;
+      const float mul = MODE ? 1.0f : a.sl2;
       float mt = sacc[0][0];
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
@@ -400,7 +693,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
       for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-          oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_tr<DV>(vs, cc * 16, db * 32, lane),
+          oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_tr<DV>(vs, lt, cc * 16, db),
                                                              pf[cc], oacc[db], 0, 0, 0);
     }
     __builtin_amdgcn_s_waitcnt(0);
@@ -409,18 +702,16 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
 
   const float l_tot = l_run + __shfl_xor(l_run, 32);
   const bool some = run.x < run.y;
-  if (g == 0 && myq < S)
-    lse[(int64_t)(b * H + h) * S + myq] = some ? m_run + log2f(l_tot) : INFINITY;
-  float probe = 0.0f;
-#pragma unroll
-  for (int i = 0; i < DB; ++i)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) probe = __builtin_fmaf(oacc[i][v], 0.0f, probe);
-  const bool bad = __ballot(some && !(probe == 0.0f && finite(l_tot) && l_tot > 0.0f)) != 0;
-  if (lane == 0 && q0 < S)
-    flags[(int64_t)(b * H + h) * a.plan.nb + (q0 >> 5)] = bad;
-  store_rows<DV>(oacc, 1.0f / l_tot, some, lds + wave * 32 * (DV + 8), lane, S - q0,
-                 out + ((int64_t)b * S + q0) * H * DV + (int64_t)h * DV, (int64_t)H * DV);
+  const bool bad = __ballot(some && !(probe_of(oacc) == 0.0f && finite(l_tot) && l_tot > 0.0f)) != 0;
+  if (!bad) {
+    if (g == 0 && myq < S)
+      lse[(int64_t)(b * H + h) * S + myq] = some ? m_run + log2f(l_tot) : INFINITY;
+    store_rows<DV>(oacc, 1.0f / l_tot, some, lds + wave * 32 * (DV + 8), lane, S - q0,
+                   out + ((int64_t)b * S + q0) * H * DV + (int64_t)h * DV, (int64_t)H * DV);
+  }
+  redo<NT>(bad, wave, lane, (float*)lds, [&](int w, float* mem) {
+    redo_fwd<DQ, DV, MODE>(a, b, h, qt * TILE + w * 32, out, lse, mem);
+  });
 }
 
 // ---------------------------------------------------------------- backward
@@ -431,8 +722,7 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
                                                      const uint16_t* __restrict__ dout,
                                                      const float* __restrict__ lse,
                                                      float* __restrict__ delta,
-                                                     uint16_t* __restrict__ dq,
-                                                     int32_t* __restrict__ flags) {
+                                                     uint16_t* __restrict__ dq) {
   constexpr int DSQ = DQ / 16, DSV = DV / 16, DB = DQ / 32, LK = BKT * DQ, LV = BKT * DV;
   static_assert(4 * 32 * (DQ + 8) <= 2 * (LK + LV), "output staging fits");
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * (LK + LV)];
@@ -450,11 +740,12 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
   const bool qok = myq < S;
   const Walk w = walk_of(a.plan, b, qt, wave);
   const int2 run = qok ? run_of(a.lo, a.hi, (int64_t)b * S + myq, S) : make_int2(0, 0);
-  const float slope2 = MODE && a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+  const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
   const int64_t srow = (int64_t)(b * H + h) * S;
   const int64_t trow = ((int64_t)b * S + myq) * ldt + (int64_t)h * DV;
 
   bf16x8 qf[DSQ], dof[DSV];
+  const bool shortrow = w.end - w.first <= SHORT;  // uniform over the workgroup
   float dl = 0.0f;
   const uint4 z = make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -464,8 +755,9 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
   for (int s = 0; s < DSV; ++s) {
     const int d = 16 * s + 8 * g;
     const uint4 gv = qok ? ld_global16(dout + trow + d) : z;
-    const uint4 ov = qok ? ld_global16(o + trow + d) : z;
     dof[s] = as_bf16x8(gv);
+    if (shortrow) continue;
+    const uint4 ov = qok ? ld_global16(o + trow + d) : z;
     const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, ow[4] = {ov.x, ov.y, ov.z, ov.w};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -473,8 +765,8 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
             st::bf16_to_f32((uint16_t)(ow[e >> 1] >> (16 * (e & 1))));
   }
   dl += __shfl_xor(dl, 32);
-  if (g == 0 && qok) delta[srow + myq] = dl;
   const float lq = qok ? lse[srow + myq] : INFINITY;
+  const uint32_t lrq = lane_row<DQ>(c, g), lrv = lane_row<DV>(c, g), lt = lane_tr<DQ>(lane);
 
   f32x16 dqacc[DB];
 #pragma unroll
@@ -493,8 +785,15 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   int buf = 0;
+#pragma unroll 1
+  for (int sweep = shortrow ? 0 : 1; sweep < 2; ++sweep) {
+  const bool only_delta = sweep == 0;
+#pragma unroll 1
   for (int k0 = w.first; k0 < w.end; k0 += BKT, buf ^= 1) {
-    if (k0 + BKT < w.end) issue(k0 + BKT, buf ^ 1);
+    if (k0 + BKT < w.end)
+      issue(k0 + BKT, buf ^ 1);
+    else if (only_delta)
+      issue(w.first, buf ^ 1);
     const uint16_t* ks = lds + buf * (LK + LV);
     const uint16_t* vs = ks + LK;
 #pragma unroll
@@ -502,73 +801,93 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
       const int kb0 = k0 + jb * 32;
       if (kb0 >= w.mine.w || kb0 + 32 <= w.mine.x) continue;  // wave-uniform
       const bool edge = kb0 < w.mine.y || kb0 + 32 > w.mine.z;
-      // an edge keeps the offsets of the lane's run, other blocks keep all
+      // an edge keeps the offsets of the lane's run (of more than one key, or
+      // dS is 0), other blocks keep all
       const int base = edge ? run.x - kb0 - 4 * g : 0;
-      const unsigned width = edge ? (unsigned)(run.y - run.x) : 32u;
+      const unsigned width = edge ? (run.y - run.x > 1 ? (unsigned)(run.y - run.x) : 0u) : 32u;
       const float far0 = (float)(myq - kb0 - 4 * g);
       f32x16 sacc, pacc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) { sacc[e] = 0.0f; pacc[e] = 0.0f; }
 #pragma unroll
       for (int s = 0; s < DSQ; ++s) {
-        sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_row<DQ>(ks, jb * 32 + c, s, g), qf[s],
+        sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DQ>(ks, lrq, jb * 32, s), qf[s],
                                                        sacc, 0, 0, 0);
         if (s < DSV)
-          pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_row<DV>(vs, jb * 32 + c, s, g),
+          pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DV>(vs, lrv, jb * 32, s),
                                                          dof[s < DSV ? s : 0], pacc, 0, 0, 0);
       }
-      bf16x8 dsf[2];
+      bf16x8 dsf[2], dsl[2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         float ds[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int vv = 8 * hh + e, ro = (vv >> 2) * 8 + (vv & 3);
-          float d;
-          if constexpr (MODE == 1) {
-            float grad;
-            const float x = score(a, slope2, sacc[vv], fabsf(far0 - (float)ro), grad);
-            d = __builtin_amdgcn_exp2f(x - lq) * (pacc[vv] - dl) * grad;
-          } else {
-            d = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[vv], a.sl2, -lq)) * (pacc[vv] - dl);
-          }
-          ds[e] = (unsigned)(ro - base) < width ? d : 0.0f;
+          float p, grad = 1.0f;
+          if constexpr (MODE != 0)
+            p = __builtin_amdgcn_exp2f(
+                score<MODE>(a, slope2, sacc[vv], fabsf(far0 - (float)ro), grad) - lq);
+          else
+            p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[vv], a.sl2, -lq));
+          // in the first sweep dl is 0 and P dP is what is summed
+          const float d = p * (pacc[vv] - (only_delta ? 0.0f : dl));
+          const float kept = (unsigned)(ro - base) < width ? d : 0.0f;
+          if (only_delta) dl += kept;
+          ds[e] = MODE ? kept * grad : kept;
         }
-        dsf[hh] = as_bf16x8(make_uint4(st::pack_bf16x2(ds[0], ds[1]), st::pack_bf16x2(ds[2], ds[3]),
-                                       st::pack_bf16x2(ds[4], ds[5]), st::pack_bf16x2(ds[6], ds[7])));
+        split8(ds, dsf[hh], dsl[hh]);
       }
+      if (only_delta) continue;
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-          dqacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              tile_tr<DQ>(ks, jb * 32 + 16 * hh, db * 32, lane), dsf[hh], dqacc[db], 0, 0, 0);
+        for (int db = 0; db < DB; ++db) {
+          const bf16x8 kt = read_tr<DQ>(ks, lt, jb * 32 + 16 * hh, db);
+          dqacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, dsf[hh], dqacc[db], 0, 0, 0);
+          dqacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, dsl[hh], dqacc[db], 0, 0, 0);
+        }
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }
+  if (only_delta) dl += __shfl_xor(dl, 32);
+  }
+  if (g == 0 && qok) delta[srow + myq] = dl;
   const bool some = run.x < run.y;
-  float probe = 0.0f;
-#pragma unroll
-  for (int i = 0; i < DB; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) probe = __builtin_fmaf(dqacc[i][e], 0.0f, probe);
-  const bool bad = __ballot(some && probe != 0.0f) != 0;
-  if (lane == 0 && q0 < S) flags[(int64_t)(b * H + h) * a.plan.nb + (q0 >> 5)] = bad;
-  store_rows<DQ>(dqacc, a.scale, some, lds + wave * 32 * (DQ + 8), lane, S - q0,
-                 dq + (srow + q0) * DQ, DQ);
+  const bool bad = __ballot(some && probe_of(dqacc) != 0.0f) != 0;
+  if (!bad)
+    store_rows<DQ>(dqacc, a.scale, some, lds + wave * 32 * (DQ + 8), lane, S - q0,
+                   dq + (srow + q0) * DQ, DQ);
+  redo<NT>(bad, wave, lane, (float*)lds, [&](int w, float* mem) {
+    redo_dq<DQ, DV, MODE>(a, b, h, qt * TILE + w * 32, dout, lse, delta, dq, mem);
+  });
 }
 
 // dK, dV of a 128-key tile of one KV head over the query heads of one part of
 // its group: steps of 64 queries of each head in turn, from the first query
 // block that sees the tile.  S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T +=
-// Q^T dS.  The whole group in one workgroup needs no partial sums in memory;
-// `parts` > 1 splits the group where that leaves CUs idle, and the parts' fp32
-// sums are added in order by span_reduce.
-// DQ <= 128: 8 waves (4 key quarters x 2 query halves, two waves a SIMD), K and
-// V tiles in LDS; the halves' sums meet in LDS at the end.  DQ = 192: 4 waves,
-// one a key quarter, each taking both query halves in turn, its K and V
-// fragments in registers.
+// Q^T dS.  DQ <= 128: 8 waves (4 key quarters x 2 query halves, two waves a
+// SIMD), K and V tiles in LDS, the halves' sums meet in LDS at the end.  (4 waves
+// with their K and V rows in registers and two workgroups a CU spilled 37 of 256
+// registers: 857 us against 306 for 8192 packed tokens, 32/8 heads of 128.)
+// DQ = 192: 4 waves, one a key quarter, each taking both query halves in turn,
+// its K and V rows in registers.
+// The whole group in one workgroup needs no partial sums in memory; a tile with
+// much more work than a CU's share has its group split over several workgroups
+// (parts_of), and span_reduce adds their fp32 sums in order.
+constexpr int SHARE = 2;
+__device__ __forceinline__ int parts_of(const Plan& p, int id, int group, int Hkv, int most) {
+  // work of this tile over SHARE quarters of a CU's share of all tiles, as a
+  // divisor of the group; tiles of at most 16 steps (2 blocks each) stay whole
+  if (most == 1) return 1;
+  const int64_t w = (int64_t)uniform(p.kwork[id]) * group, all = uniform(*p.ktotal);
+  const int64_t share = max(all * group * Hkv * SHARE / 1024, (int64_t)32);
+  int n = 1;
+  while (n < most && (group % n || w > share * n)) ++n;
+  return n;
+}
+
 template <int DQ>
 constexpr int dkdv_waves() {
   return DQ <= 128 ? 8 : 4;
@@ -581,9 +900,9 @@ constexpr int dkdv_lds() {
 template <int DQ, int DV, int MODE>
 __global__ __launch_bounds__(64 * dkdv_waves<DQ>(), dkdv_waves<DQ>() == 8 ? 2 : 1)
 void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __restrict__ lse,
-                   const float* __restrict__ delta, int parts, float* __restrict__ dk_part,
+                   const float* __restrict__ delta, int most, float* __restrict__ dk_part,
                    float* __restrict__ dv_part, uint16_t* __restrict__ dk,
-                   uint16_t* __restrict__ dv, int32_t* __restrict__ flags) {
+                   uint16_t* __restrict__ dv) {
   constexpr int DSQ = DQ / 16, DSV = DV / 16, DBQ = DQ / 32, DBV = DV / 32;
   constexpr int LK = TILE * DQ, LV = TILE * DV, LQ = QT * DQ, LG = QT * DV;
   constexpr int NW = dkdv_waves<DQ>(), NTH = 64 * NW, QH = 8 / NW;
@@ -591,16 +910,20 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   __shared__ __attribute__((aligned(16))) uint16_t lds[dkdv_lds<DQ, DV>()];
   __shared__ __attribute__((aligned(16))) float lse_s[2][QT], dl_s[2][QT];
   __shared__ __attribute__((aligned(16))) int lo_s[2][QT], wd_s[2][QT];
-  const int S = a.S, H = a.H, nb = a.plan.nb;
-  const int per = a.Hkv * parts;
-  const int id = uniform(a.plan.korder[blockIdx.x / per]), rest = blockIdx.x % per;
-  const int hk = rest % a.Hkv, part = rest / a.Hkv;
+  const int S = a.S, H = a.H, nb = a.plan.nb, group = H / a.Hkv;
+  // an XCD's shader engines take its workgroups in turn: the parts that a tile
+  // does not have are rotated from tile to tile, or one engine got all the work
+  const int slot = blockIdx.x / (a.Hkv * most), rest = blockIdx.x % (a.Hkv * most);
+  const int id = uniform(a.plan.korder[slot]), hk = rest % a.Hkv;
+  const int part = (rest / a.Hkv + slot) % most;
+  const int parts = parts_of(a.plan, id, group, a.Hkv, most);
+  if (part >= parts) return;
   const int b = id / a.plan.nt, kt = id % a.plan.nt;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c = lane & 31;
   const int kq = wave & 3, qh0 = NW == 8 ? wave >> 2 : 0;
-  const int heads = H / a.Hkv / parts, h0 = hk * (H / a.Hkv) + part * heads;
+  const int heads = group / parts, h0 = hk * group + part * heads;
   const int64_t ldt = (int64_t)H * DV;
   const uint16_t* kb = a.k + (int64_t)(b * a.Hkv + hk) * S * DQ;
   const uint16_t* vb = a.v + (int64_t)(b * a.Hkv + hk) * S * DV;
@@ -610,6 +933,8 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   const int k0 = kt * TILE, kw0 = k0 + kq * 32, mykey = kw0 + c;
   const int2 seen = make_int2(uniform(a.plan.keys[id].x), uniform(a.plan.keys[id].y));
   const int4* blk = a.plan.blk + (int64_t)b * nb;
+  const uint32_t lrq = lane_row<DQ>(c, g), lrv = lane_row<DV>(c, g);
+  const uint32_t ltq = lane_tr<DQ>(lane), ltv = lane_tr<DV>(lane);
   bf16x8 kfr[KREG ? DSQ : 1], vfr[KREG ? DSV : 1];
   if constexpr (KREG) {
     const uint4 z = make_uint4(0, 0, 0, 0);
@@ -668,9 +993,10 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   int j = 0, u = 0;  // head of the part, step of the head
+#pragma unroll 1
   for (int n = 0; n < steps; ++n) {
     const int buf = n & 1, q0 = qfirst + u * QT;
-    const float slope2 = MODE && a.slopes ? a.slopes[h0 + j] * LOG2E : 0.0f;
+    const float slope2 = (MODE & BIAS) ? a.slopes[h0 + j] * LOG2E : 0.0f;
     if (++u == nq) {
       u = 0;
       ++j;
@@ -681,26 +1007,27 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
 #pragma unroll
     for (int hq = 0; hq < QH; ++hq) {
       const int qh = NW == 8 ? qh0 : hq;
-      const int qw0 = q0 + qh * 32;
+      const int qw0 = q0 + qh * 32;  // this wave's queries
       const int4 x = qw0 < S ? uniform(blk[qw0 >> 5]) : make_int4(INT_MAX, INT_MAX, 0, 0);
       if (kw0 < x.w && kw0 + 32 > x.x) {  // some query sees some key
         const bool edge = kw0 < x.y || kw0 + 32 > x.z;
         const float far0 = (float)(qw0 + 4 * g - mykey);
+        const uint16_t *qt = qs + qh * 32 * DQ, *gt = gs + qh * 32 * DV;  // the wave's rows
         f32x16 sacc, pacc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) { sacc[e] = 0.0f; pacc[e] = 0.0f; }
 #pragma unroll
         for (int s = 0; s < DSQ; ++s) {
           sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              tile_row<DQ>(qs, qh * 32 + c, s, g),
-              KREG ? kfr[KREG ? s : 0] : tile_row<DQ>(Ks, kq * 32 + c, s, g), sacc, 0, 0, 0);
+              read_row<DQ>(qt, lrq, 0, s),
+              KREG ? kfr[KREG ? s : 0] : read_row<DQ>(Ks + kq * 32 * DQ, lrq, 0, s), sacc, 0, 0, 0);
           if (s < DSV)
             pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                tile_row<DV>(gs, qh * 32 + c, s, g),
-                KREG ? vfr[KREG && s < DSV ? s : 0] : tile_row<DV>(Vs, kq * 32 + c, s, g), pacc,
-                0, 0, 0);
+                read_row<DV>(gt, lrv, 0, s),
+                KREG ? vfr[KREG && s < DSV ? s : 0] : read_row<DV>(Vs + kq * 32 * DV, lrv, 0, s),
+                pacc, 0, 0, 0);
         }
-        bf16x8 pf[2], dsf[2];
+        bf16x8 pf[2], dsf[2], dsl[2];
         const int r0 = qh * 32 + g * 4;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -709,9 +1036,9 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
           for (int e = 0; e < 8; ++e) {
             const int vv = 8 * hh + e, ro = (vv >> 2) * 8 + (vv & 3);
             const float l = lse_s[buf][r0 + ro], dl = dl_s[buf][r0 + ro];
-            if constexpr (MODE == 1) {
+            if constexpr (MODE != 0) {
               float grad;
-              const float y = score(a, slope2, sacc[vv], fabsf(far0 + (float)ro), grad);
+              const float y = score<MODE>(a, slope2, sacc[vv], fabsf(far0 + (float)ro), grad);
               p8[e] = __builtin_amdgcn_exp2f(y - l);
               d8[e] = p8[e] * (pacc[vv] - dl) * grad;
             } else {
@@ -725,13 +1052,11 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
               const int vv = 8 * hh + e, r = r0 + (vv >> 2) * 8 + (vv & 3);
               const bool keep = (unsigned)(mykey - lo_s[buf][r]) < (unsigned)wd_s[buf][r];
               p8[e] = keep ? p8[e] : 0.0f;
-              d8[e] = keep ? d8[e] : 0.0f;
+              d8[e] = keep && wd_s[buf][r] > 1 ? d8[e] : 0.0f;
             }
           }
-          pf[hh] = as_bf16x8(make_uint4(st::pack_bf16x2(p8[0], p8[1]), st::pack_bf16x2(p8[2], p8[3]),
-                                        st::pack_bf16x2(p8[4], p8[5]), st::pack_bf16x2(p8[6], p8[7])));
-          dsf[hh] = as_bf16x8(make_uint4(st::pack_bf16x2(d8[0], d8[1]), st::pack_bf16x2(d8[2], d8[3]),
-                                         st::pack_bf16x2(d8[4], d8[5]), st::pack_bf16x2(d8[6], d8[7])));
+          pf[hh] = pack8(p8);
+          split8(d8, dsf[hh], dsl[hh]);
         }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
@@ -739,10 +1064,10 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
           for (int db = 0; db < DBQ; ++db) {
             if (db < DBV)
               dvacc[db < DBV ? db : 0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  tile_tr<DV>(gs, qh * 32 + 16 * hh, db * 32, lane), pf[hh],
-                  dvacc[db < DBV ? db : 0], 0, 0, 0);
-            dkacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                tile_tr<DQ>(qs, qh * 32 + 16 * hh, db * 32, lane), dsf[hh], dkacc[db], 0, 0, 0);
+                  read_tr<DV>(gt, ltv, 16 * hh, db), pf[hh], dvacc[db < DBV ? db : 0], 0, 0, 0);
+            const bf16x8 qtr = read_tr<DQ>(qt, ltq, 16 * hh, db);
+            dkacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtr, dsf[hh], dkacc[db], 0, 0, 0);
+            dkacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtr, dsl[hh], dkacc[db], 0, 0, 0);
           }
       }
     }
@@ -750,306 +1075,130 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }
-  // 8 waves: query half 1 parks its sums in LDS, half 0 adds them and writes
-  // [key][d] rows; dV first, then dK
+  // 8 waves: query half 1 parks its sums in LDS, half 0 adds them; dV first, then dK
   float* red = (float*)lds;
-  constexpr int PARTV = DBV * 16 * 64, PARTK = DBQ * 16 * 64;
-  static_assert(NW == 4 || 4 * PARTK * 4 <= dkdv_lds<DQ, DV>() * 2, "sums fit in LDS");
-  const int64_t krow = (int64_t)(b * a.Hkv + hk) * S + mykey;            // of dk, dv
-  const int64_t prow = ((int64_t)(b * a.Hkv + hk) * parts + part) * S + mykey;  // of the partials
-  float probe = 0.0f;
-  auto write = [&](auto& acc, auto dims, int stride, float mul, float* part_out, uint16_t* direct) {
-    constexpr int D = decltype(dims)::value;
-    if (NW == 8 && qh0 == 1) {
+  auto meet = [&](auto& acc, auto blocks) {
+    constexpr int DB = decltype(blocks)::value;
+    static_assert(NW == 4 || 4 * DB * 16 * 64 * 4 <= dkdv_lds<DQ, DV>() * 2, "sums fit in LDS");
+    if (qh0 == 1) {
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) red[kq * stride + (db * 16 + e) * 64 + lane] = acc[db][e];
+        for (int e = 0; e < 16; ++e) red[(kq * DB * 16 + db * 16 + e) * 64 + lane] = acc[db][e];
     }
     __syncthreads();
-    if (qh0 == 0 && mykey < S) {
+    if (qh0 == 0) {
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int v4 = 0; v4 < 4; ++v4) {
-          float4 r;
-          float* pr = &r.x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int vv = 4 * v4 + e;
-            pr[e] = (NW == 8 ? acc[db][vv] + red[kq * stride + (db * 16 + vv) * 64 + lane]
-                             : acc[db][vv]) * mul;
-            probe = __builtin_fmaf(pr[e], 0.0f, probe);
-          }
-          const int col = db * 32 + v4 * 8 + g * 4;
-          if (direct)
-            *(u32x2*)(direct + krow * D + col) =
-                u32x2{st::pack_bf16x2(r.x, r.y), st::pack_bf16x2(r.z, r.w)};
-          else
-            *(float4*)(part_out + prow * D + col) = r;
-        }
+        for (int e = 0; e < 16; ++e) acc[db][e] += red[(kq * DB * 16 + db * 16 + e) * 64 + lane];
     }
     __syncthreads();
   };
-  write(dvacc, std::integral_constant<int, DV>{}, PARTV, 1.0f, dv_part, parts == 1 ? dv : nullptr);
-  write(dkacc, std::integral_constant<int, DQ>{}, PARTK, a.scale, dk_part,
-        parts == 1 ? dk : nullptr);
-  const bool bad = __ballot(probe != 0.0f) != 0;
-  if (qh0 == 0 && lane == 0 && kw0 < S)
-    flags[((int64_t)(b * a.Hkv + hk) * parts + part) * nb + (kw0 >> 5)] = bad;
+  if constexpr (NW == 8) {
+    meet(dvacc, std::integral_constant<int, DBV>{});
+    meet(dkacc, std::integral_constant<int, DBQ>{});
+  }
+  const bool bad =
+      __ballot(qh0 == 0 && mykey < S && probe_of(dvacc) + probe_of(dkacc) != 0.0f) != 0;
+  const int64_t krow = (int64_t)(b * a.Hkv + hk) * S;                  // of dk, dv
+  const int64_t prow = ((int64_t)(b * a.Hkv + hk) * most + part) * S;  // of the partials
+  if (qh0 == 0 && !bad && kw0 < S) {
+    // staged by each wave in its own LDS space
+    uint16_t* os = lds + kq * (dkdv_lds<DQ, DV>() / 4);
+    static_assert(32 * (DQ + 8) <= dkdv_lds<DQ, DV>() / 4 && 32 * (DV + 8) <= dkdv_lds<DQ, DV>() / 4,
+                  "bf16 staging fits");
+    if (parts == 1) {
+      store_rows<DV>(dvacc, 1.0f, true, os, lane, S - kw0, dv + (krow + kw0) * DV, DV);
+      __builtin_amdgcn_s_waitcnt(0);
+      __builtin_amdgcn_wave_barrier();
+      store_rows<DQ>(dkacc, a.scale, true, os, lane, S - kw0, dk + (krow + kw0) * DQ, DQ);
+    } else {
+      static_assert(32 * (DQ + 4) * 2 <= dkdv_lds<DQ, DV>() / 2, "fp32 staging of two waves fits");
+      constexpr bool whole = 32 * (DQ + 4) * 2 <= dkdv_lds<DQ, DV>() / 4;
+      if constexpr (whole) {
+        store_rows_f32<DV>(dvacc, 1.0f, (float*)os, lane, S - kw0, dv_part + (prow + kw0) * DV);
+        store_rows_f32<DQ>(dkacc, a.scale, (float*)os, lane, S - kw0, dk_part + (prow + kw0) * DQ);
+      } else if (mykey < S) {  // heads of 192: the tile's LDS does not hold fp32 rows
+#pragma unroll
+        for (int v = 0; v < DBV * 4; ++v)
+          *(float4*)(dv_part + (prow + mykey) * DV + v / 4 * 32 + v % 4 * 8 + g * 4) =
+              make_float4(dvacc[v / 4][v % 4 * 4], dvacc[v / 4][v % 4 * 4 + 1],
+                          dvacc[v / 4][v % 4 * 4 + 2], dvacc[v / 4][v % 4 * 4 + 3]);
+#pragma unroll
+        for (int v = 0; v < DBQ * 4; ++v)
+          *(float4*)(dk_part + (prow + mykey) * DQ + v / 4 * 32 + v % 4 * 8 + g * 4) =
+              make_float4(dkacc[v / 4][v % 4 * 4] * a.scale, dkacc[v / 4][v % 4 * 4 + 1] * a.scale,
+                          dkacc[v / 4][v % 4 * 4 + 2] * a.scale, dkacc[v / 4][v % 4 * 4 + 3] * a.scale);
+      }
+    }
+  }
+  redo<NTH>(bad, wave, lane, (float*)lds, [&](int w, float* mem) {
+    redo_dkdv<DQ, DV, MODE, NTH>(a, b, hk, h0, heads, k0 + (w & 3) * 32, seen, dout, lse, delta, mem,
+                                 [&](int key, int d, float sk, float sv) {
+      if (parts == 1) {
+        if (d < DQ) dk[(krow + key) * DQ + d] = st::f32_to_bf16(sk);
+        if (d < DV) dv[(krow + key) * DV + d] = st::f32_to_bf16(sv);
+      } else {
+        if (d < DQ) dk_part[(prow + key) * DQ + d] = sk;
+        if (d < DV) dv_part[(prow + key) * DV + d] = sv;
+      }
+    });
+  });
 }
 
-// dk = bf16(sum over the parts, in order), same for dv
-__global__ __launch_bounds__(NT) void span_reduce(const float* __restrict__ dk_part,
-                                                  const float* __restrict__ dv_part, int64_t rows,
-                                                  int parts, int64_t S, int DQ, int DV,
+// dk = bf16(sum over the parts, in order), same for dv, of the tiles in parts
+__global__ __launch_bounds__(NT) void span_reduce(Plan plan, const float* __restrict__ dk_part,
+                                                  const float* __restrict__ dv_part, int group,
+                                                  int Hkv, int most, int S, int DQ, int DV,
                                                   uint16_t* __restrict__ dk,
                                                   uint16_t* __restrict__ dv) {
-  // rows = B * Hkv
-  const int64_t nk = rows * S * DQ / 4, n = nk + rows * S * DV / 4;
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
-    const bool isk = i < nk;
-    const int64_t per = S * (isk ? DQ : DV), e = (isk ? i : i - nk) * 4;
-    const float* part = (isk ? dk_part : dv_part) + e / per * parts * per + e % per;
-    float4 s = make_float4(0, 0, 0, 0);
-    for (int j = 0; j < parts; ++j) {
-      const float4 x = *(const float4*)(part + j * per);
-      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
-    }
-    *(u32x2*)((isk ? dk : dv) + e) = u32x2{st::pack_bf16x2(s.x, s.y), st::pack_bf16x2(s.z, s.w)};
-  }
-}
-
-// ---------------------------------------------------------------- flagged blocks
-// The rows of a 32-row block whose sums are not finite, over the seen pairs
-// alone.  Correct, not fast: none is flagged while operands are finite.
-template <int D>
-__device__ __forceinline__ float dot(const uint16_t* __restrict__ x, const uint16_t* __restrict__ y) {
-  float s = 0.0f;
-  for (int d = 0; d < D; d += 8) {
-    const uint4 u = ld_global16(x + d), w = ld_global16(y + d);
-    const uint32_t p[4] = {u.x, u.y, u.z, u.w}, r[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s = __builtin_fmaf(__uint_as_float(p[e] << 16), __uint_as_float(r[e] << 16), s);
-      s = __builtin_fmaf(__uint_as_float(p[e] & 0xffff0000u), __uint_as_float(r[e] & 0xffff0000u), s);
-    }
-  }
-  return s;
-}
-template <bool MAX>
-__device__ __forceinline__ float block_reduce(float x, float* red) {
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    const float y = __shfl_xor(x, d);
-    x = MAX ? fmaxf(x, y) : x + y;
-  }
-  __syncthreads();
-  if ((tid & 63) == 0) red[tid >> 6] = x;
-  __syncthreads();
-  x = red[0];
-  for (int i = 1; i < NT / 64; ++i) x = MAX ? fmaxf(x, red[i]) : x + red[i];
-  return x;
-}
-
-// calls fn(block) for each set flag among the workgroup's 256
-template <typename F>
-__device__ __forceinline__ void each_flag(const int32_t* __restrict__ flags, int64_t n, F&& fn) {
-  __shared__ unsigned long long sets[NT / 64];
-  const int64_t i0 = (int64_t)blockIdx.x * NT, i = i0 + threadIdx.x;
-  const unsigned long long m = __ballot(i < n && flags[i] != 0);
-  if ((threadIdx.x & 63) == 0) sets[threadIdx.x >> 6] = m;
-  __syncthreads();
-  for (int w = 0; w < NT / 64; ++w)
-    for (unsigned long long s = sets[w]; s; s &= s - 1)
-      fn(i0 + w * 64 + __ffsll((long long)s) - 1);
-}
-
-template <int DQ, int DV>
-__global__ __launch_bounds__(NT) void span_fix_fwd(Args a, const int32_t* __restrict__ flags,
-                                                   int64_t n, uint16_t* __restrict__ out,
-                                                   float* __restrict__ lse) {
-  __shared__ float red[NT / 64], ps[NT];
-  const int tid = threadIdx.x, S = a.S, H = a.H;
-  each_flag(flags, n, [&](int64_t f) {
-    const int64_t bh = f / a.plan.nb;
-    const int b = (int)(bh / H), h = (int)(bh % H);
-    const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
-    const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
-    const float slope2 = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
-    const int i0 = (int)(f % a.plan.nb) * 32;
-    for (int i = i0; i < min(i0 + 32, S); ++i) {
-      const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
-      if (run.x >= run.y) continue;
-      const uint16_t* qi = a.q + (bh * S + i) * DQ;
-      auto x_of = [&](int j) {
-        float grad;
-        return score(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ), fabsf((float)(i - j)), grad);
-      };
-      float m = -INFINITY;
-      for (int j = run.x + tid; j < run.y; j += NT) m = fmaxf(m, x_of(j));
-      m = block_reduce<true>(m, red);
-      float l = 0.0f, o = 0.0f;
-      for (int c0 = run.x; c0 < run.y; c0 += NT) {
-        const float p = c0 + tid < run.y ? __builtin_amdgcn_exp2f(x_of(c0 + tid) - m) : 0.0f;
-        l += p;
-        __syncthreads();
-        ps[tid] = p;
-        __syncthreads();
-        if (tid < DV)
-          for (int j = c0; j < min(c0 + NT, run.y); ++j)
-            o = __builtin_fmaf(ps[j - c0], st::bf16_to_f32(vb[(int64_t)j * DV + tid]), o);
+  const int id = uniform(plan.korder[blockIdx.x / Hkv]), hk = blockIdx.x % Hkv;
+  const int parts = parts_of(plan, id, group, Hkv, most);
+  if (parts == 1) return;
+  constexpr int ROWS = TILE / 8;  // few tiles are in parts: 8 workgroups each
+  const int k0 = id % plan.nt * TILE + blockIdx.y * ROWS, rows = min(ROWS, S - k0);
+  const int64_t bhk = (int64_t)(id / plan.nt) * Hkv + hk;
+  auto add = [&](const float* part, uint16_t* out, int D) {
+    for (int i = threadIdx.x; i < rows * D / 4; i += NT) {
+      float4 s = make_float4(0, 0, 0, 0);
+      for (int j = 0; j < parts; ++j) {
+        const float4 x = *(const float4*)(part + ((bhk * most + j) * S + k0) * D + i * 4);
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
       }
-      l = block_reduce<false>(l, red);
-      if (tid < DV) out[((int64_t)b * S + i) * H * DV + (int64_t)h * DV + tid] = st::f32_to_bf16(o / l);
-      if (tid == 0) lse[bh * S + i] = m + log2f(l);
+      *(u32x2*)(out + (bhk * S + k0) * D + i * 4) =
+          u32x2{st::pack_bf16x2(s.x, s.y), st::pack_bf16x2(s.z, s.w)};
     }
-  });
-}
-
-template <int DQ, int DV>
-__global__ __launch_bounds__(NT) void span_fix_dq(Args a, const int32_t* __restrict__ flags, int64_t n,
-                                                  const uint16_t* __restrict__ dout,
-                                                  const float* __restrict__ lse,
-                                                  const float* __restrict__ delta,
-                                                  uint16_t* __restrict__ dq) {
-  __shared__ float ps[NT];
-  const int tid = threadIdx.x, S = a.S, H = a.H;
-  each_flag(flags, n, [&](int64_t f) {
-    const int64_t bh = f / a.plan.nb;
-    const int b = (int)(bh / H), h = (int)(bh % H);
-    const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
-    const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
-    const float slope2 = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
-    const int i0 = (int)(f % a.plan.nb) * 32;
-    for (int i = i0; i < min(i0 + 32, S); ++i) {
-      const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
-      if (run.x >= run.y) continue;
-      const uint16_t* qi = a.q + (bh * S + i) * DQ;
-      const uint16_t* gi = dout + ((int64_t)b * S + i) * H * DV + (int64_t)h * DV;
-      const float li = lse[bh * S + i], di = delta[bh * S + i];
-      float o = 0.0f;
-      for (int c0 = run.x; c0 < run.y; c0 += NT) {
-        const int j = c0 + tid;
-        float ds = 0.0f;
-        if (j < run.y) {
-          float grad;
-          const float x = score(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ), fabsf((float)(i - j)), grad);
-          ds = __builtin_amdgcn_exp2f(x - li) * (dot<DV>(gi, vb + (int64_t)j * DV) - di) * grad;
-        }
-        __syncthreads();
-        ps[tid] = ds;
-        __syncthreads();
-        if (tid < DQ)
-          for (int jj = c0; jj < min(c0 + NT, run.y); ++jj)
-            o = __builtin_fmaf(ps[jj - c0], st::bf16_to_f32(kb[(int64_t)jj * DQ + tid]), o);
-      }
-      if (tid < DQ) dq[(bh * S + i) * DQ + tid] = st::f32_to_bf16(o * a.scale);
-    }
-  });
-}
-
-// flags [B*Hkv, parts, nb]: a block is redone by its first flagged part
-template <int DQ, int DV>
-__global__ __launch_bounds__(NT) void span_fix_dkdv(Args a, const int32_t* __restrict__ flags,
-                                                    int64_t n, int parts,
-                                                    const uint16_t* __restrict__ dout,
-                                                    const float* __restrict__ lse,
-                                                    const float* __restrict__ delta,
-                                                    uint16_t* __restrict__ dk,
-                                                    uint16_t* __restrict__ dv) {
-  __shared__ float ps[NT], ds[NT];
-  __shared__ int vis[NT];
-  const int tid = threadIdx.x, S = a.S, H = a.H, group = H / a.Hkv, nb = a.plan.nb;
-  each_flag(flags, n, [&](int64_t f) {
-    const int64_t bhk = f / nb / parts;
-    const int part = (int)(f / nb % parts);
-    for (int p = 0; p < part; ++p)
-      if (flags[(bhk * parts + p) * nb + f % nb]) return;
-    const int b = (int)(bhk / a.Hkv), hk = (int)(bhk % a.Hkv);
-    const int j0 = (int)(f % nb) * 32;
-    const int2 seen = a.plan.keys[(int64_t)b * a.plan.nt + j0 / TILE];
-    const int qa = seen.x * 32, qz = min(seen.y * 32, S);
-    for (int j = j0; j < min(j0 + 32, S); ++j) {
-      const uint16_t* kj = a.k + (bhk * S + j) * DQ;
-      const uint16_t* vj = a.v + (bhk * S + j) * DV;
-      float sk = 0.0f, sv = 0.0f;  // this thread's column of dK, of dV
-      for (int hh = 0; hh < group; ++hh) {
-        const int h = hk * group + hh;
-        const float slope2 = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
-        const int64_t bh = (int64_t)b * H + h;
-        const uint16_t* gb = dout + (int64_t)b * S * H * DV + (int64_t)h * DV;
-        for (int c0 = qa; c0 < qz; c0 += NT) {
-          const int i = c0 + tid;
-          bool sees = false;
-          float p = 0.0f, d = 0.0f;
-          if (i < qz) {
-            const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
-            sees = run.x <= j && j < run.y;
-          }
-          if (sees) {
-            float grad;
-            const float x = score(a, slope2, dot<DQ>(a.q + (bh * S + i) * DQ, kj),
-                                  fabsf((float)(i - j)), grad);
-            p = __builtin_amdgcn_exp2f(x - lse[bh * S + i]);
-            d = p * (dot<DV>(gb + (int64_t)i * H * DV, vj) - delta[bh * S + i]) * grad;
-          }
-          __syncthreads();
-          ps[tid] = p;
-          ds[tid] = d;
-          vis[tid] = sees;
-          __syncthreads();
-          for (int q = c0; q < min(c0 + NT, qz); ++q) {
-            if (!vis[q - c0]) continue;
-            if (tid < DQ)
-              sk = __builtin_fmaf(ds[q - c0], st::bf16_to_f32(a.q[(bh * S + q) * DQ + tid]), sk);
-            if (tid < DV)
-              sv = __builtin_fmaf(ps[q - c0], st::bf16_to_f32(gb[(int64_t)q * H * DV + tid]), sv);
-          }
-        }
-      }
-      if (tid < DQ) dk[(bhk * S + j) * DQ + tid] = st::f32_to_bf16(sk * a.scale);
-      if (tid < DV) dv[(bhk * S + j) * DV + tid] = st::f32_to_bf16(sv);
-    }
-  });
+  };
+  add(dk_part, dk, DQ);
+  add(dv_part, dv, DV);
 }
 
 // ---------------------------------------------------------------- host
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Parts of a KV head's group in the dK/dV pass: the fewest that give every CU
-// a workgroup (one runs per CU).
-int parts_of(int64_t B, int64_t S, int64_t H, int64_t Hkv) {
-  const int64_t group = H / Hkv, wgs = B * st::cdiv(S, TILE) * Hkv;
-  for (int64_t p = 1; p < group; ++p)
-    if (group % p == 0 && wgs * p >= 256) return (int)p;
-  return (int)group;
+// Most parts that a KV head's group may be split into: none where a tile has at
+// most 16 steps anyway or the tiles are many.
+int most_parts(int64_t B, int64_t S, int64_t H, int64_t Hkv) {
+  const int64_t group = H / Hkv;
+  return st::cdiv(S, QT) * group <= 16 || B * st::cdiv(S, TILE) * Hkv > 8192 ? 1 : (int)group;
 }
 
 struct Space {
-  int64_t flags, flags2, delta, dkp, dvp, bytes;  // byte offsets
-  int parts;
+  int64_t delta, dkp, dvp, bytes;  // byte offsets
+  int most;
 };
-Space space_of(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t DQ, int64_t DV, bool backward) {
+Space space_of(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t DQ, int64_t DV) {
   Space s{};
-  const int64_t nb = st::cdiv(S, 32);
-  int64_t at = 0;
-  s.flags = at;
-  at += up256(B * H * nb * 4);
-  if (backward) {
-    s.parts = parts_of(B, S, H, Hkv);
-    s.flags2 = at;
-    at += up256(B * Hkv * s.parts * nb * 4);
-    s.delta = at;
-    at += up256(B * H * S * 4);
-    if (s.parts > 1) {
-      s.dkp = at;
-      at += up256(B * Hkv * s.parts * S * DQ * 4);
-      s.dvp = at;
-      at += up256(B * Hkv * s.parts * S * DV * 4);
-    }
+  s.most = most_parts(B, S, H, Hkv);
+  s.delta = 0;
+  int64_t at = up256(B * H * S * 4);
+  if (s.most > 1) {
+    s.dkp = at;
+    at += up256(B * Hkv * s.most * S * DQ * 4);
+    s.dvp = at;
+    at += up256(B * Hkv * s.most * S * DV * 4);
   }
   s.bytes = at + 256;
   return s;
@@ -1091,45 +1240,55 @@ Args args_of(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B,
   if (cap > 0) {
     a.cap_in = 2.0f * LOG2E * scale / cap;
     a.cap_out = cap * LOG2E;
+    const float r = scale / cap;
+    a.cap_small = 0.35f / r;
+    const float c[3] = {-0.33332663774490356f, 0.1329982578754425f, -0.049148499965667725f};
+    for (int i = 0; i < 3; ++i) a.cap_p[i] = a.sl2 * c[i] * powf(r, 2.0f * (float)(i + 1));
   }
   return a;
 }
 
 template <int DQ, int DV, int MODE>
-int run_fwd(const Args& a, int64_t B, uint16_t* out, float* lse, char* ws, hipStream_t s) {
-  int32_t* flags = (int32_t*)ws;
-  const int64_t n = B * a.H * a.plan.nb;
-  span_fwd<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, lse, flags);
-  if (int rc = st::check_launch("span_fwd")) return rc;
-  span_fix_fwd<DQ, DV><<<(unsigned)st::cdiv(n, NT), NT, 0, s>>>(a, flags, n, out, lse);
-  return st::check_launch("span_fix_fwd");
+int run_fwd(const Args& a, int64_t B, uint16_t* out, float* lse, hipStream_t s) {
+  span_fwd<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, lse);
+  return st::check_launch("span_fwd");
 }
 
 template <int DQ, int DV, int MODE>
 int run_bwd(const Args& a, int64_t B, const uint16_t* out, const float* lse, const uint16_t* dout,
             uint16_t* dq, uint16_t* dk, uint16_t* dv, char* ws, hipStream_t s) {
-  const Space sp = space_of(B, a.S, a.H, a.Hkv, DQ, DV, true);
-  int32_t *f1 = (int32_t*)(ws + sp.flags), *f2 = (int32_t*)(ws + sp.flags2);
+  const Space sp = space_of(B, a.S, a.H, a.Hkv, DQ, DV);
   float* delta = (float*)(ws + sp.delta);
   float *dkp = (float*)(ws + sp.dkp), *dvp = (float*)(ws + sp.dvp);
   span_bwd_dq<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, dout, lse, delta,
-                                                                          dq, f1);
+                                                                          dq);
   if (int rc = st::check_launch("span_bwd_dq")) return rc;
-  span_bwd_dkdv<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.Hkv * sp.parts), 64 * dkdv_waves<DQ>(), 0, s>>>(
-      a, dout, lse, delta, sp.parts, dkp, dvp, dk, dv, f2);
-  if (int rc = st::check_launch("span_bwd_dkdv")) return rc;
-  if (sp.parts > 1) {
-    const int64_t n4 = B * a.Hkv * a.S * (DQ + DV) / 4;
-    span_reduce<<<(unsigned)std::min<int64_t>(st::cdiv(n4, NT), 4096), NT, 0, s>>>(
-        dkp, dvp, B * a.Hkv, sp.parts, a.S, DQ, DV, dk, dv);
-    if (int rc = st::check_launch("span_reduce")) return rc;
-  }
-  const int64_t n1 = B * a.H * a.plan.nb, n2 = B * a.Hkv * sp.parts * a.plan.nb;
-  span_fix_dq<DQ, DV><<<(unsigned)st::cdiv(n1, NT), NT, 0, s>>>(a, f1, n1, dout, lse, delta, dq);
-  if (int rc = st::check_launch("span_fix_dq")) return rc;
-  span_fix_dkdv<DQ, DV><<<(unsigned)st::cdiv(n2, NT), NT, 0, s>>>(a, f2, n2, sp.parts, dout, lse,
-                                                                  delta, dk, dv);
-  return st::check_launch("span_fix_dkdv");
+  const unsigned tiles = (unsigned)(B * a.plan.nt * a.Hkv);
+  span_bwd_dkdv<DQ, DV, MODE><<<tiles * sp.most, 64 * dkdv_waves<DQ>(), 0, s>>>(
+      a, dout, lse, delta, sp.most, dkp, dvp, dk, dv);
+  int rc = st::check_launch("span_bwd_dkdv");
+  if (rc || sp.most == 1) return rc;
+  span_reduce<<<dim3(tiles, 8), NT, 0, s>>>(a.plan, dkp, dvp, a.H / a.Hkv, a.Hkv, sp.most, a.S, DQ, DV, dk, dv);
+  return st::check_launch("span_reduce");
+}
+
+// fn(DQ, DV, MODE) of a call as compile-time values
+template <typename F>
+int by_kind(int64_t DQ, float cap, const float* slopes, F&& fn) {
+  auto with = [&](auto dq, auto dv) {
+    const int mode = (cap > 0 ? CAP : 0) | (slopes ? BIAS : 0);
+    switch (mode) {
+      case 0: return fn(dq, dv, std::integral_constant<int, 0>{});
+      case CAP: return fn(dq, dv, std::integral_constant<int, CAP>{});
+      case BIAS: return fn(dq, dv, std::integral_constant<int, BIAS>{});
+      default: return fn(dq, dv, std::integral_constant<int, CAP | BIAS>{});
+    }
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (DQ == 64) return with(D64{}, D64{});
+  if (DQ == 128) return with(D128{}, D128{});
+  return with(std::integral_constant<int, 192>{}, D128{});
 }
 
 }  // namespace
@@ -1157,43 +1316,31 @@ extern "C" int st_span_plan(const int32_t* key_start, const int32_t* key_end, in
   span_tiles<<<(unsigned)tiles, 64, 0, s>>>(p.blk, p.nb, p.nt, (int2*)p.keys, p.qwork, p.kwork);
   if (int rc = st::check_launch("span_tiles")) return rc;
   span_order<<<dim3((unsigned)st::cdiv(tiles, NT), 2), NT, 0, s>>>(
-      p.qwork, p.kwork, tiles, tiles <= SORT_LIMIT, (int32_t*)p.qorder, (int32_t*)p.korder);
+      p.qwork, p.kwork, tiles, (int32_t*)p.qorder, (int32_t*)p.korder, p.ktotal);
   return st::check_launch("span_order");
 }
 
 extern "C" int64_t st_span_attn_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv,
-                                                int64_t DQ, int64_t DV, int32_t backward) {
+                                                int64_t DQ, int64_t DV) {
   if (B <= 0 || S <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || !dims_ok(DQ, DV)) return 0;
-  return space_of(B, S, H, Hkv, DQ, DV, backward != 0).bytes;
+  return space_of(B, S, H, Hkv, DQ, DV).bytes;
 }
 
 extern "C" int st_span_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B,
                                 int64_t S, int64_t H, int64_t Hkv, int64_t DQ, int64_t DV,
                                 float scale, float cap, const float* slopes,
                                 const int32_t* key_start, const int32_t* key_end, const void* plan,
-                                uint16_t* out, float* lse, void* workspace, int64_t workspace_bytes,
-                                st_stream_t stream) {
+                                uint16_t* out, float* lse, st_stream_t stream) {
   const char* name = "st_span_attn_fwd";
   if (int rc = check_common(name, B, S, H, Hkv, DQ, DV, scale, cap)) return rc;
   if (B == 0 || S == 0) return ST_OK;
   ST_CHECK_ARG(q && k && v && out && lse && key_start && key_end && plan && al16(q) && al16(k) &&
                    al16(v) && al16(out) && al16(plan), "%s: NULL or unaligned pointer", name);
-  const int64_t need = space_of(B, S, H, Hkv, DQ, DV, false).bytes;
-  if (!workspace || workspace_bytes < need)
-    return st::fail(ST_EWORKSPACE, "%s: needs %lld workspace bytes", name, (long long)need);
   const Args a = args_of(q, k, v, B, S, H, Hkv, scale, cap, slopes, key_start, key_end, plan);
-  char* ws = (char*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
-  hipStream_t s = (hipStream_t)stream;
-  const bool mod = cap > 0 || slopes;
-#define ST_SPAN(DQ_, DV_)                                          \
-  if (DQ == DQ_)                                                   \
-    return mod ? run_fwd<DQ_, DV_, 1>(a, B, out, lse, ws, s)       \
-               : run_fwd<DQ_, DV_, 0>(a, B, out, lse, ws, s)
-  ST_SPAN(64, 64);
-  ST_SPAN(128, 128);
-  ST_SPAN(192, 128);
-#undef ST_SPAN
-  return ST_OK;
+  return by_kind(DQ, cap, slopes, [&](auto dq, auto dv, auto mode) {
+    return run_fwd<decltype(dq)::value, decltype(dv)::value, decltype(mode)::value>(
+        a, B, out, lse, (hipStream_t)stream);
+  });
 }
 
 extern "C" int st_span_attn_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v,
@@ -1209,20 +1356,13 @@ extern "C" int st_span_attn_bwd(const uint16_t* q, const uint16_t* k, const uint
   ST_CHECK_ARG(q && k && v && out && lse && dout && dq && dk && dv && key_start && key_end && plan &&
                    al16(q) && al16(k) && al16(v) && al16(out) && al16(dout) && al16(dq) &&
                    al16(dk) && al16(dv) && al16(plan), "%s: NULL or unaligned pointer", name);
-  const int64_t need = space_of(B, S, H, Hkv, DQ, DV, true).bytes;
+  const int64_t need = space_of(B, S, H, Hkv, DQ, DV).bytes;
   if (!workspace || workspace_bytes < need)
     return st::fail(ST_EWORKSPACE, "%s: needs %lld workspace bytes", name, (long long)need);
   const Args a = args_of(q, k, v, B, S, H, Hkv, scale, cap, slopes, key_start, key_end, plan);
   char* ws = (char*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
-  hipStream_t s = (hipStream_t)stream;
-  const bool mod = cap > 0 || slopes;
-#define ST_SPAN(DQ_, DV_)                                                             \
-  if (DQ == DQ_)                                                                      \
-    return mod ? run_bwd<DQ_, DV_, 1>(a, B, out, lse, dout, dq, dk, dv, ws, s)        \
-               : run_bwd<DQ_, DV_, 0>(a, B, out, lse, dout, dq, dk, dv, ws, s)
-  ST_SPAN(64, 64);
-  ST_SPAN(128, 128);
-  ST_SPAN(192, 128);
-#undef ST_SPAN
-  return ST_OK;
+  return by_kind(DQ, cap, slopes, [&](auto dq_, auto dv_, auto mode) {
+    return run_bwd<decltype(dq_)::value, decltype(dv_)::value, decltype(mode)::value>(
+        a, B, out, lse, dout, dq, dk, dv, ws, (hipStream_t)stream);
+  });
 }

@@ -131,11 +131,9 @@ class _SpanAttention(torch.autograd.Function):
         out = torch.empty((B, S, H * DV), dtype=_BF16, device=dev)
         lse = torch.empty((B, H, S), dtype=_F32, device=dev)
         with torch.cuda.device(dev):
-            ws = _scratch(dev, _lib.query("st_span_attn_workspace_bytes", B, S, H, Hkv, DQ, DV, 0))
             _lib.call("st_span_attn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), B, S, H, Hkv, DQ, DV,
                       scale, cap, _lib.ptr(slopes), _lib.ptr(mask.key_start), _lib.ptr(mask.key_end),
-                      _lib.ptr(mask.plan), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws),
-                      0 if ws is None else ws.numel(), _lib.stream_handle(dev))
+                      _lib.ptr(mask.plan), _lib.ptr(out), _lib.ptr(lse), _lib.stream_handle(dev))
         ctx.save_for_backward(q, k, v, out, lse, slopes)
         ctx.scale, ctx.mask, ctx.cap = scale, mask, cap
         return out
@@ -150,7 +148,7 @@ class _SpanAttention(torch.autograd.Function):
         dout = _operand(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         with torch.cuda.device(dev):
-            ws = _scratch(dev, _lib.query("st_span_attn_workspace_bytes", B, S, H, Hkv, DQ, DV, 1))
+            ws = _scratch(dev, _lib.query("st_span_attn_workspace_bytes", B, S, H, Hkv, DQ, DV))
             _lib.call("st_span_attn_bwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out),
                       _lib.ptr(lse), _lib.ptr(dout), B, S, H, Hkv, DQ, DV, ctx.scale, ctx.cap,
                       _lib.ptr(slopes), _lib.ptr(mask.key_start), _lib.ptr(mask.key_end),

@@ -54,12 +54,16 @@ def span_forward(q, k, v, scale, lo, hi, cap=None, slopes=None):
     return (e / torch.where(n > 0, n, 1.0)) @ v
 
 
-def span_ref(q, k, v, scale, lo, hi, cap=None, slopes=None, dout=None):
+def span_ref(q, k, v, scale, lo, hi, cap=None, slopes=None, dout=None, rounded_ds=False):
     """(values, bounds) of out [B,S,H*DV] and, with dout, dq, dk, dv, by the formulas.
 
-    Bounds: probabilities and dS are rounded to bf16 (U of each value), delta is
-    summed from the rounded output, each result is rounded once; a tenth on top
-    covers the fp32 scores, exponentials and sums (each relative 2^-12 at most)."""
+    Bounds: probabilities are rounded to bf16 (U of each value), dS is not; each
+    result is rounded once.  delta is summed from the rounded output where a tile's
+    queries see more than 256 keys in all (rows longer than that may), from the
+    fp32 products otherwise.  fp32 scores of D products, exponentials and sums are
+    off by 2^-12 at most, dP by D products of |dO||V|; a tenth covers the first in
+    the terms that bf16 rules.  ``rounded_ds``: the bounds of a kernel that rounds
+    dS to bf16 and always sums delta from the rounded output."""
     B, H, S, DQ = q.shape
     KV, DV = k.shape[1], v.shape[-1]
     G = H // KV
@@ -77,7 +81,13 @@ def span_ref(q, k, v, scale, lo, hi, cap=None, slopes=None, dout=None):
     do = dout.double().view(B, S, H, DV).transpose(1, 2).contiguous()
     dp = do @ v.transpose(-1, -2).contiguous()
     ds = p * (dp - (do * o).sum(-1, keepdim=True)) * grad
-    ds_err = U * ds.abs() + p * grad * (do.abs() * o_err).sum(-1, keepdim=True)
+    size = do.abs() @ v.abs().transpose(-1, -2).contiguous()
+    delta_err = (do.abs() * o_err).sum(-1, keepdim=True) \
+        if S > 256 or rounded_ds else 0.0
+    one = sees.sum(-1, keepdim=True) == 1
+    ds_err = p * grad * (2.0 ** -12 * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True))
+                         + 2.0 ** -17 * (size + (p * size).sum(-1, keepdim=True)) + delta_err)
+    ds_err = ds_err + U * ds.abs() if rounded_ds else torch.where(one, 0.0, ds_err)
     T = lambda t: t.transpose(-1, -2).contiguous()  # noqa: E731
     fold = lambda t: t.view(B, KV, G, S, -1).sum(2)  # noqa: E731
     dq, dk, dv = ds @ k * scale, fold(T(ds) @ q) * scale, fold(T(p) @ do)

@@ -91,21 +91,28 @@ def test_abi_refuses_before_the_device():
     reach a kernel)."""
     p, n = ctypes.c_void_p(16), ctypes.c_void_p(None)
 
-    def fwd(B=1, S=4, H=2, KV=1, DQ=64, DV=64, scale=1.0, cap=0.0, q=p, plan=p, ws=p, wb=1 << 40):
+    def fwd(B=1, S=4, H=2, KV=1, DQ=64, DV=64, scale=1.0, cap=0.0, q=p, plan=p):
         _lib.call("st_span_attn_fwd", q, p, p, B, S, H, KV, DQ, DV, scale, cap, None, p, p, plan, p,
-                  p, ws, wb, None)
+                  p, None)
     for kw, msg in (({"H": 3, "KV": 2}, "head counts"), ({"DQ": 96, "DV": 96}, "head dims"),
                     ({"scale": 0.0}, "scale"), ({"cap": -1.0}, "cap"), ({"q": n}, "NULL"),
-                    ({"plan": ctypes.c_void_p(8)}, "unaligned"), ({"wb": 10}, "workspace"),
-                    ({"ws": n}, "workspace"), ({"S": 1 << 30}, "too large"),
+                    ({"plan": ctypes.c_void_p(8)}, "unaligned"), ({"S": 1 << 30}, "too large"),
                     ({"H": 1 << 17}, "too large")):
         with pytest.raises(ValueError, match=msg):
             fwd(**kw)
     fwd(B=0)  # nothing to do
+
+    def bwd(dq=p, ws=p, wb=1 << 40):
+        _lib.call("st_span_attn_bwd", p, p, p, p, p, p, 1, 4, 2, 1, 64, 64, 1.0, 0.0, None, p, p, p, dq,
+                  p, p, ws, wb, None)
+    for kw, msg in (({"dq": n}, "NULL"), ({"wb": 10}, "workspace"), ({"ws": n}, "workspace")):
+        with pytest.raises(ValueError, match=msg):
+            bwd(**kw)
     with pytest.raises(ValueError, match="needs"):
         _lib.call("st_span_plan", p, p, 2, 100, p, 16, None)
-    assert _lib.query("st_span_plan_bytes", 2, 100) == 4 * (2 * 4 * 4 + 2 * (2 + 4))
-    assert _lib.query("st_span_attn_workspace_bytes", 1, 8, 3, 2, 64, 64, 0) == 0
+    # blocks, key tiles, two orders, two works, the sum
+    assert _lib.query("st_span_plan_bytes", 2, 100) == 4 * (2 * 4 * 4 + 2 * 2 * 1 + 4 * 2 * 1 + 1)
+    assert _lib.query("st_span_attn_workspace_bytes", 1, 8, 3, 2, 64, 64) == 0
 
     def rope(D=64, rot=64, ldx=256, wq=None, wk=None, x=p, B=1, S=4):
         _lib.call("st_rope_pos_fwd", x, ldx, p, 0, p, 1.0, B, S, 2, 1, D, rot, 0, wq, wk, 1e-6, p, p,
