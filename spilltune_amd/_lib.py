@@ -8,6 +8,7 @@ for argument/capability errors, ``RuntimeError`` for device failures.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import threading
@@ -198,6 +199,15 @@ def stream_handle(device: torch.device | str | int | None = None) -> int:
         index = device
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None
                                               else index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one: kernels are launched on
+    the current device, whatever the stream's (nothing to do where it is already)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 class RkProduct(ctypes.Structure):

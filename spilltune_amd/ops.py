@@ -216,6 +216,12 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def _once() -> None:
+    """Refuses a backward that is to be differentiated itself."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("unsupported_capability: this operator has no second derivative")
+
+
 def _gemm_scratch(weight: Q4Weight, form: int, M: int, rank: int, cols: int):
     """Scratch of one fused GEMM call (decoded weights within the weight's
     ``decode_limit``, or split-K partials), from the caching allocator, so that
@@ -788,7 +794,7 @@ class _TokenLogProbs(torch.autograd.Function):
         lp, ent, lse = (torch.empty(rows, dtype=_F32, device=dev) for _ in range(3))
         top_lp = torch.empty((rows, top), dtype=_F32, device=dev)
         top_tok = torch.empty((rows, top), dtype=torch.int64, device=dev)
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             for a, z in _TokenLogProbs._row_chunks(hidden, head, top, False):
                 ws = _scratch(dev, _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V,
                                               head.stride(0), top, 0))
@@ -804,15 +810,15 @@ class _TokenLogProbs(torch.autograd.Function):
         return lp, ent, top_lp, top_tok
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_ent, g_top, _):
+        _once()
         hidden, head, tokens, lp, ent, lse, top_lp, top_tok = ctx.saved_tensors
         ignore_index, temperature, cap, top = ctx.meta
         H, V, dev = hidden.shape[1], head.shape[0], hidden.device
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
         part = lambda g, a, z: None if g is None else _lib.ptr(g[a:z])  # noqa: E731
         dh = torch.empty(hidden.shape, dtype=_BF16, device=dev)
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             for a, z in _TokenLogProbs._row_chunks(hidden, head, top, True):
                 ws = _scratch(dev, _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V,
                                               head.stride(0), top, 1))

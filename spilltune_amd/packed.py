@@ -26,7 +26,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib
-from .ops import _operand, _scratch
+from .ops import _once, _operand, _scratch
 
 _BF16 = torch.bfloat16
 _F32 = torch.float32
@@ -68,7 +68,7 @@ def span_mask(key_start: torch.Tensor, key_end: torch.Tensor, positions=None) ->
     # own copies: the plan below is of these values
     key_start, key_end, positions = (t.detach().clone(memory_format=torch.contiguous_format)
                                      for t in (key_start, key_end, positions))
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         nbytes = _lib.query("st_span_plan_bytes", B, S)
         plan = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call("st_span_plan", _lib.ptr(key_start), _lib.ptr(key_end), B, S, _lib.ptr(plan), nbytes,
@@ -130,30 +130,33 @@ class _SpanAttention(torch.autograd.Function):
         dev = q.device
         out = torch.empty((B, S, H * DV), dtype=_BF16, device=dev)
         lse = torch.empty((B, H, S), dtype=_F32, device=dev)
-        with torch.cuda.device(dev):
-            _lib.call("st_span_attn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), B, S, H, Hkv, DQ, DV,
-                      scale, cap, _lib.ptr(slopes), _lib.ptr(mask.key_start), _lib.ptr(mask.key_end),
-                      _lib.ptr(mask.plan), _lib.ptr(out), _lib.ptr(lse), _lib.stream_handle(dev))
+        operands = (q.data_ptr(), k.data_ptr(), v.data_ptr())
+        shape = (B, S, H, Hkv, DQ, DV)
+        mode = (scale, cap, _lib.ptr(slopes), mask.key_start.data_ptr(), mask.key_end.data_ptr(),
+                mask.plan.data_ptr())
+        with _lib.on_device(dev):
+            _lib.call("st_span_attn_fwd", *operands, *shape, *mode, out.data_ptr(), lse.data_ptr(),
+                      _lib.stream_handle(dev))
         ctx.save_for_backward(q, k, v, out, lse, slopes)
-        ctx.scale, ctx.mask, ctx.cap = scale, mask, cap
+        # the backward's arguments as far as they are known (the tensors above and
+        # the mask keep their memory): it runs in a thread that is woken for it
+        ctx.args, ctx.shape, ctx.keep = (operands, mode), shape, mask
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, slopes = ctx.saved_tensors
-        B, H, S, DQ = q.shape
-        Hkv, DV = k.shape[1], v.shape[-1]
-        dev, mask = q.device, ctx.mask
+        _once()
+        q, k, v, out, lse, _ = ctx.saved_tensors
+        operands, mode = ctx.args
+        dev = dout.device
         dout = _operand(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        with torch.cuda.device(dev):
-            ws = _scratch(dev, _lib.query("st_span_attn_workspace_bytes", B, S, H, Hkv, DQ, DV))
-            _lib.call("st_span_attn_bwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out),
-                      _lib.ptr(lse), _lib.ptr(dout), B, S, H, Hkv, DQ, DV, ctx.scale, ctx.cap,
-                      _lib.ptr(slopes), _lib.ptr(mask.key_start), _lib.ptr(mask.key_end),
-                      _lib.ptr(mask.plan), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(ws),
-                      0 if ws is None else ws.numel(), _lib.stream_handle(dev))
+        with _lib.on_device(dev):
+            nbytes = _lib.query("st_span_attn_workspace_bytes", *ctx.shape)
+            ws = _scratch(dev, nbytes)
+            _lib.call("st_span_attn_bwd", *operands, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                      *ctx.shape, *mode, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws),
+                      nbytes, _lib.stream_handle(dev))
         return dq, dk, dv, None, None, None, None
 
 
@@ -283,34 +286,34 @@ class _RopePositions(torch.autograd.Function):
         k = torch.empty((B, kv_heads, S, D), dtype=_BF16, device=dev)
         v = torch.empty_like(k)
         rstd = None if wq is None else torch.empty((B * S, heads + kv_heads), dtype=_F32, device=dev)
-        with torch.cuda.device(dev):
-            _lib.call("st_rope_pos_fwd", _lib.ptr(y), y.stride(0), _lib.ptr(positions),
-                      int(positions.dtype == torch.int64), _lib.ptr(rotary.inv_freq),
-                      rotary.amplitude, B, S, heads, kv_heads, D, rotary.rotary_dim,
-                      int(rotary.interleaved), _lib.ptr(wq), _lib.ptr(wk), eps, _lib.ptr(q),
-                      _lib.ptr(k), _lib.ptr(v), _lib.ptr(rstd), _lib.stream_handle(dev))
-        ctx.save_for_backward(None if wq is None else y, positions, wq, wk, rstd, rotary.inv_freq)
-        ctx.meta = (tuple(y.shape), rotary, heads, kv_heads)
+        rows = (y.data_ptr(), y.stride(0))
+        turn = (positions.data_ptr(), int(positions.dtype == torch.int64), rotary.inv_freq.data_ptr(),
+                rotary.amplitude, B, S, heads, kv_heads, D, rotary.rotary_dim,
+                int(rotary.interleaved), _lib.ptr(wq), _lib.ptr(wk))
+        with _lib.on_device(dev):
+            _lib.call("st_rope_pos_fwd", *rows, *turn, eps, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                      _lib.ptr(rstd), _lib.stream_handle(dev))
+        if wq is None:  # the rotation's gradient does not read its input
+            ctx.save_for_backward(positions)
+        else:
+            ctx.save_for_backward(positions, y, wq, wk)
+        # the backward's arguments but for the gradients, and what they point to
+        ctx.args = (*rows, *turn, _lib.ptr(rstd))
+        ctx.shape, ctx.keep = (tuple(y.shape), tuple(q.shape), tuple(k.shape)), (rotary.inv_freq, rstd)
         ctx.set_materialize_grads(False)
         return q, k, v
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk, dv):
-        y, positions, wq, wk, rstd, inv_freq = ctx.saved_tensors
-        shape, rotary, heads, kv_heads = ctx.meta
-        B, S = positions.shape
-        D, dev = rotary.head_dim, inv_freq.device
+        _once()
+        dev = ctx.saved_tensors[0].device
+        shape, qs, ks = ctx.shape
         dy = torch.empty(shape, dtype=_BF16, device=dev)
-        gs = [torch.zeros((B, h, S, D), dtype=_BF16, device=dev) if g is None else _operand(g)
-              for g, h in ((dq, heads), (dk, kv_heads), (dv, kv_heads))]
-        with torch.cuda.device(dev):
-            _lib.call("st_rope_pos_bwd", *(_lib.ptr(g) for g in gs), _lib.ptr(y),
-                      0 if y is None else y.stride(0), _lib.ptr(positions),
-                      int(positions.dtype == torch.int64), _lib.ptr(inv_freq), rotary.amplitude, B,
-                      S, heads, kv_heads, D, rotary.rotary_dim, int(rotary.interleaved),
-                      _lib.ptr(wq), _lib.ptr(wk), _lib.ptr(rstd), _lib.ptr(dy), dy.stride(0),
-                      _lib.stream_handle(dev))
+        dq, dk, dv = (torch.zeros(s, dtype=_BF16, device=dev) if g is None else _operand(g)
+                      for g, s in ((dq, qs), (dk, ks), (dv, ks)))
+        with _lib.on_device(dev):
+            _lib.call("st_rope_pos_bwd", dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ctx.args,
+                      dy.data_ptr(), shape[1], _lib.stream_handle(dev))
         return dy, None, None, None, None, None, None, None
 
 

@@ -255,6 +255,20 @@ def test_operands_of_any_layout_and_repeatable():
         assert torch.equal(x, y)
 
 
+def test_no_second_derivative():
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = _randn(g, 1, 1, 8, 64).to(BF).requires_grad_(True)
+    mask = packed.document_mask(torch.zeros(1, 8, dtype=torch.int32, device="cuda"))
+    out = packed.span_attention(q, q.detach(), q.detach(), 0.125, mask)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.sum(), q, create_graph=True)
+    y = _randn(g, 8, 3 * 64).to(BF).requires_grad_(True)
+    pos = torch.arange(8, device="cuda").view(1, 8)
+    out = packed.rope_positions(y, pos, packed.Rotary(64, 1e4, device="cuda"), 1, 1)[0]
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.sum(), y, create_graph=True)
+
+
 def test_graph_replays():
     """Forward and backward captured; replays after eager work with new operands."""
     B, S, H, KV, D = 1, 260, 4, 2, 64
