@@ -506,24 +506,26 @@ int st_cross_entropy_rows(uint16_t* logits, int64_t rows, int64_t vocab, int64_t
  * hidden [rows, H] (stride ldh), head [V, H] (stride ldw): bf16, 16-byte rows.
  * The backward takes the forward's outputs and the gradients of logprobs,
  * entropy and top_logprobs (fp32, each may be NULL) and writes dhidden (stride
- * ldd, bf16); rows whose gradients are all 0 get 0.  dl of each row is rounded to
- * bf16 in the workspace (2 bytes a logit); the forward's holds 4 bytes a logit
- * with top > 0 and 16 per 256 logits without.
+ * ldd, bf16); rows whose gradients are all 0 get 0.  logits: NULL, or fp32 [rows,
+ * V rounded up to 4] that the forward writes l to and the backward reads instead
+ * of forming it again (kept = 1 in the query).  dl of each row is rounded to
+ * bf16 in the backward's workspace (2 bytes a logit); the forward's holds 4 bytes
+ * a logit with top > 0 and no logits, and 16 per 128 or 256 logits.
  * --------------------------------------------------------------------- */
 int64_t st_token_logprobs_workspace_bytes(int64_t rows, int64_t H, int64_t V, int64_t ldw,
-                                          int64_t top, int32_t backward);
+                                          int64_t top, int32_t kept, int32_t backward);
 int st_token_logprobs_fwd(const uint16_t* hidden, int64_t rows, int64_t H, int64_t ldh,
                           const uint16_t* head, int64_t V, int64_t ldw, const int64_t* tokens,
                           int64_t ignore_index, float temperature, float cap, int64_t top,
                           float* logprobs, float* entropy, float* lse, float* top_logprobs,
-                          int64_t* top_tokens, void* workspace, int64_t workspace_bytes,
-                          st_stream_t stream);
+                          int64_t* top_tokens, float* logits, void* workspace,
+                          int64_t workspace_bytes, st_stream_t stream);
 int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64_t H, int64_t ldh,
                           const uint16_t* head, int64_t V, int64_t ldw, const int64_t* tokens,
                           int64_t ignore_index, float temperature, float cap, int64_t top,
                           const float* logprobs, const float* entropy, const float* lse,
                           const float* top_logprobs, const int64_t* top_tokens,
-                          const float* g_logprobs, const float* g_entropy, const float* g_top,
+                          const float* logits, const float* g_logprobs, const float* g_entropy, const float* g_top,
                           uint16_t* dhidden, int64_t ldd, void* workspace, int64_t workspace_bytes,
                           st_stream_t stream);
 

@@ -114,11 +114,11 @@ _SIGNATURES = {
                                 _P, _P, _P, _P]),
     "st_span_attn_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _F,
                                 _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
-    "st_token_logprobs_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I32]),
+    "st_token_logprobs_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I32, _I32]),
     "st_token_logprobs_fwd": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _F, _F, _I64,
-                                     _P, _P, _P, _P, _P, _P, _I64, _P]),
+                                     _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "st_token_logprobs_bwd": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _F, _F, _I64,
-                                     _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P]),
+                                     _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P]),
     "st_cross_entropy_rows": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _F, _P, _P]),
     "st_moe_lora_grads": (_I32, [_I64, _I32, _I64, _I32, _P, _I64, _I64, _P, _P, _I64, _I64, _P,
                                  _I32, _F, _P, _I64, _I64, _I64, _I32, _P]),

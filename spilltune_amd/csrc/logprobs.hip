@@ -16,14 +16,17 @@
 // reductions run down its own accumulators (two exchanges between lanes per
 // token; the other way round took four for each of its 32 rows).
 // Top alternatives are chosen on l before cap and temperature (ties to the
-// lowest index): only then the tiles also write l (fp32), and the join reads
-// back just the tiles that hold the largest maxima.
+// lowest index): only then, or for a caller that keeps them for the backward, the
+// tiles also write l (fp32); the join reads back just the tiles that hold the
+// largest maxima.
 //
-// Backward: the same GEMM again, its epilogue turning l into dl (bf16: a choice,
-// half a step of 2^-8 on values that are then summed over the vocabulary), the
-// given token's and the alternatives' entries redone by a small kernel from the
-// saved log probabilities, and dl head as a GEMM split over the vocabulary so
-// that few rows fill the GPU; fp32 partials are summed in order.
+// Backward: l read back, or formed again by the same GEMM, becomes dl (bf16: a
+// choice, half a step of 2^-8 on values that are then summed over the
+// vocabulary); the given token's and the alternatives' entries, the large ones,
+// are redone by a small kernel from the saved log probabilities, which keeps what
+// their rounding leaves in fp32.  dl head is a GEMM split over the vocabulary so
+// that few rows fill the GPU; its fp32 partials are summed in order and the
+// picked entries' remainders times their rows of the head added.
 #include <algorithm>
 #include <cmath>
 
@@ -32,7 +35,6 @@
 namespace {
 
 constexpr int NT = 256;
-constexpr int VT = 256;  // vocabulary columns of a tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Transform {
@@ -83,7 +85,7 @@ struct Head {
   const uint16_t *hidden, *head;
   const int64_t* tokens;
   int64_t ldh, ldw, rows, V;
-  int H, vtiles, rtiles;
+  int H, vt, vtiles, rtiles;  // vt: vocabulary columns of a tile
   Transform tf;
 };
 
@@ -98,8 +100,8 @@ __device__ __forceinline__ bool tile_of(const Head& h, int64_t& vt, int64_t& rt)
 template <class LP>
 __device__ __forceinline__ void products(const Head& h, int64_t vt, int64_t rt, uint4* lds, int wave,
                                          int lane, int& vn, int& rn, f32x4 (&acc)[LP::FM][LP::FN]) {
-  const int64_t v0 = vt * VT, r0 = rt * LP::BN;
-  vn = (int)min((int64_t)VT, h.V - v0);
+  const int64_t v0 = vt * LP::BM, r0 = rt * LP::BN;
+  vn = (int)min((int64_t)LP::BM, h.V - v0);
   rn = (int)min((int64_t)LP::BN, h.rows - r0);
   const st::DmaOperands o{h.head + v0 * h.ldw, h.hidden + r0 * h.ldh, h.ldw, h.ldh,
                           ((vn - 1) * h.ldw + h.H) * 2, ((rn - 1) * h.ldh + h.H) * 2};
@@ -111,8 +113,7 @@ template <class LP>
 __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_tiles(Head h, float4* __restrict__ part,
                                                                      float* __restrict__ xy,
                                                                      float* __restrict__ logits,
-                                                                     int64_t ldl) {
-  static_assert(LP::BM == VT, "vocabulary tile");
+                                                                     int64_t ldl, int top) {
   constexpr int WMS = LP::WAVES / LP::WAVES_N;
   __shared__ uint4 lds[LP::LDS16];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_tiles(Head h, flo
   products<LP>(h, vt, rt, lds, wave, lane, vn, rn, acc);
 
   const int wm = wave / LP::WAVES_N, wn = wave % LP::WAVES_N, lr = lane & 15, lh = lane >> 4;
-  const int64_t v0 = vt * VT, r0 = rt * LP::BN;
+  const int64_t v0 = vt * LP::BM, r0 = rt * LP::BN;
   const int vw = wm * LP::WM + lh * 4;  // this lane's first column of the tile
   float4* red = (float4*)lds;           // [WMS][BN]
 #pragma unroll
@@ -144,8 +145,8 @@ __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_tiles(Head h, flo
     for (int i = 0; i < LP::FM; ++i)
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const bool ok = vn == VT || vw + i * 16 + v < vn;
-        if (logits) raw = fmaxf(raw, ok ? acc[i][j][v] : -INFINITY);
+        const bool ok = vn == LP::BM || vw + i * 16 + v < vn;
+        if (top) raw = fmaxf(raw, ok ? acc[i][j][v] : -INFINITY);
         const float x = value(h.tf, acc[i][j][v]);
         acc[i][j][v] = ok ? x : -INFINITY;
         m = fmaxf(m, acc[i][j][v]);
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_tiles(Head h, flo
       ties += __shfl_xor(ties, 32);
       if (s < 1.0078125f) rest = less + (ties - 1.0f);
     }
-    if (logits) {
+    if (top) {
       raw = fmaxf(raw, __shfl_xor(raw, 16));
       raw = fmaxf(raw, __shfl_xor(raw, 32));
     }
@@ -228,6 +229,7 @@ __device__ __forceinline__ void wave_best(float& v, int& i) {
 
 // One wave a row: joins the tiles, then picks `top` alternatives one by one
 // from the tile with the greatest value left.
+template <int VT>
 __global__ __launch_bounds__(NT) void lp_join(Head h, int64_t ignore, const float4* __restrict__ part,
                                               const float* __restrict__ xy,
                                               const float* __restrict__ logits, int64_t ldl, int top,
@@ -274,19 +276,22 @@ __global__ __launch_bounds__(NT) void lp_join(Head h, int64_t ignore, const floa
       }
       continue;
     }
-    const int c0 = bt * VT + lane * 4;
-    float f[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if (c0 < h.V) {
-      const float4 x = *(const float4*)(logits + row * ldl + c0);
-      const float g[4] = {x.x, x.y, x.z, x.w};
+    constexpr int PER = VT / 64;
+    const int c0 = bt * VT + lane * PER;
+    float f[PER];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c0 + e < h.V && (g[e] < lv || (g[e] == lv && c0 + e > li))) f[e] = g[e];
+    for (int e = 0; e < PER; ++e) f[e] = -INFINITY;
+    if (c0 < h.V) {  // rows of `logits` are padded to whole float4
+      typedef float fv __attribute__((ext_vector_type(PER)));
+      const fv x = *(const fv*)(logits + row * ldl + c0);
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (c0 + e < h.V && (x[e] < lv || (x[e] == lv && c0 + e > li))) f[e] = x[e];
     }
     float v = -INFINITY;
     int i = INT_MAX;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < PER; ++e)
       if (f[e] > v) {
         v = f[e];
         i = c0 + e;
@@ -296,7 +301,7 @@ __global__ __launch_bounds__(NT) void lp_join(Head h, int64_t ignore, const floa
     li = i;
     float next = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < PER; ++e)
       if (c0 + e != i) next = fmaxf(next, f[e]);
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) next = fmaxf(next, __shfl_xor(next, d));
@@ -319,7 +324,24 @@ __device__ __forceinline__ float given(const Head& h, const Upstream& g, int64_t
   return g.lp && h.tokens[row] != ignore ? g.lp[row] : 0.0f;
 }
 
-// dl of every column but for the picked tokens' own terms
+// (sum over the picked, of the entropy, lse, entropy) of a row
+__device__ __forceinline__ float4 upstream(const Head& h, const Upstream& g, int64_t row, int64_t ignore,
+                                           const int64_t* top_idx, const float* lse, const float* ent) {
+  float sum = given(h, g, row, ignore);
+  if (g.top)
+    for (int k = 0; k < g.ntop; ++k)
+      sum += top_idx[row * g.ntop + k] >= 0 ? g.top[row * g.ntop + k] : 0.0f;
+  return make_float4(sum, g.ent ? g.ent[row] : 0.0f, lse[row], ent[row]);
+}
+// dl of a logit but for a picked token's own term; a row without an upstream
+// gradient has none, whatever it holds
+__device__ __forceinline__ float dlogit(const Transform& t, float4 c, float l) {
+  const float lp = value(t, l) - c.z, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+  const float d = -p * __builtin_fmaf(c.y, lp + c.w, c.x) * slope(t, l);
+  return c.x == 0.0f && c.y == 0.0f ? 0.0f : d;
+}
+
+// dl from logits formed again
 template <class LP>
 __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_dlogits(Head h, Upstream g,
                                                                        int64_t ignore,
@@ -338,56 +360,71 @@ __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_dlogits(Head h, U
   products<LP>(h, vt, rt, lds, wave, lane, vn, rn, acc);
 
   const int wm = wave / LP::WAVES_N, wn = wave % LP::WAVES_N, lr = lane & 15, lh = lane >> 4;
-  const int64_t v0 = vt * VT, r0 = rt * LP::BN;
-  float4* up = (float4*)lds;  // (sum over the picked, of the entropy, lse, entropy) per row
-  for (int r = tid; r < rn; r += LP::NT) {
-    const int64_t row = r0 + r;
-    float sum = given(h, g, row, ignore);
-    if (g.top)
-      for (int k = 0; k < g.ntop; ++k)
-        sum += top_idx[row * g.ntop + k] >= 0 ? g.top[row * g.ntop + k] : 0.0f;
-    up[r] = make_float4(sum, g.ent ? g.ent[row] : 0.0f, lse[row], ent[row]);
-  }
+  const int64_t v0 = vt * LP::BM, r0 = rt * LP::BN;
+  float4* up = (float4*)lds;
+  for (int r = tid; r < rn; r += LP::NT) up[r] = upstream(h, g, r0 + r, ignore, top_idx, lse, ent);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < LP::FN; ++j) {
     const int r = wn * LP::WN + j * 16 + lr;
     if (r >= rn) continue;
     const float4 c = up[r];
-    // a row without an upstream gradient has none, whatever it holds
-    const bool dead = c.x == 0.0f && c.y == 0.0f;
     uint16_t* out = dl + (r0 + r) * ldd + v0 + wm * LP::WM + lh * 4;
 #pragma unroll
     for (int i = 0; i < LP::FM; ++i) {
       const int col = wm * LP::WM + lh * 4 + i * 16;
       float d[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float l = acc[i][j][v], lp = value(h.tf, l) - c.z;
-        const float p = __builtin_amdgcn_exp2f(lp * LOG2E);
-        // a column past the vocabulary (up to the row's padding) gets 0
-        d[v] = col + v < vn && !dead ? -p * __builtin_fmaf(c.y, lp + c.w, c.x) * slope(h.tf, l) : 0.0f;
-      }
+      for (int v = 0; v < 4; ++v)  // a column past the vocabulary (up to the row's padding) gets 0
+        d[v] = col + v < vn ? dlogit(h.tf, c, acc[i][j][v]) : 0.0f;
       if (v0 + col < ldd)
         *(uint2*)(out + i * 16) = make_uint2(st::pack_bf16x2(d[0], d[1]), st::pack_bf16x2(d[2], d[3]));
     }
   }
 }
+// dl from kept logits: 4 + 2 bytes a logit, bound by HBM
+constexpr int KEPT = 8;  // logits of a thread
+__global__ __launch_bounds__(NT) void lp_dlogits_kept(Head h, Upstream g, int64_t ignore,
+                                                      const int64_t* __restrict__ top_idx,
+                                                      const float* __restrict__ lse,
+                                                      const float* __restrict__ ent,
+                                                      const float* __restrict__ logits, int64_t ldl,
+                                                      uint16_t* __restrict__ dl, int64_t ldd) {
+  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  if (row >= h.rows) return;
+  const float4 c = upstream(h, g, row, ignore, top_idx, lse, ent);
+  const int64_t c0 = ((int64_t)blockIdx.x * NT + threadIdx.x) * KEPT;
+  if (c0 >= ldd) return;
+  float l[KEPT], d[KEPT];
+#pragma unroll
+  for (int e = 0; e < KEPT; e += 4) {
+    float4 x = make_float4(0, 0, 0, 0);
+    if (c0 + e < ldl) x = *(const float4*)(logits + row * ldl + c0 + e);
+    l[e] = x.x; l[e + 1] = x.y; l[e + 2] = x.z; l[e + 3] = x.w;
+  }
+#pragma unroll
+  for (int e = 0; e < KEPT; ++e) d[e] = c0 + e < h.V ? dlogit(h.tf, c, l[e]) : 0.0f;
+  *(uint4*)(dl + row * ldd + c0) = make_uint4(st::pack_bf16x2(d[0], d[1]), st::pack_bf16x2(d[2], d[3]),
+                                              st::pack_bf16x2(d[4], d[5]), st::pack_bf16x2(d[6], d[7]));
+}
 
 // the picked tokens' entries whole: thread k of a row takes alternative k, or
-// the given token (k = ntop); a token picked twice gets one value from both
+// the given token (k = ntop); a token picked twice gets one value from both.
+// left[row][k]: what the entry's rounding leaves, once for each entry.
 __global__ __launch_bounds__(NT) void lp_picked(Head h, Upstream g, int64_t ignore,
                                                 const int64_t* __restrict__ top_idx,
                                                 const float* __restrict__ top_lp,
                                                 const float* __restrict__ logprobs,
                                                 const float* __restrict__ lse,
                                                 const float* __restrict__ ent,
-                                                uint16_t* __restrict__ dl, int64_t ldd) {
+                                                uint16_t* __restrict__ dl, int64_t ldd,
+                                                float* __restrict__ left) {
   const int64_t n = (int64_t)blockIdx.x * NT + threadIdx.x;
   const int per = g.ntop + 1;
   const int64_t row = n / per;
   const int k = (int)(n % per);
   if (row >= h.rows) return;
+  left[n] = 0.0f;
   const int64_t y = h.tokens[row];
   const bool has = y != ignore && y >= 0 && y < h.V;
   const int64_t c = k < g.ntop ? top_idx[row * g.ntop + k] : has ? y : -1;
@@ -395,13 +432,14 @@ __global__ __launch_bounds__(NT) void lp_picked(Head h, Upstream g, int64_t igno
   const float lp = k < g.ntop ? top_lp[row * g.ntop + k] : logprobs[row];
   const float own_lp = given(h, g, row, ignore);
   float sum = own_lp, own = has && c == y ? own_lp : 0.0f;
-  if (g.top)
-    for (int j = 0; j < g.ntop; ++j) {
-      const int64_t t = top_idx[row * g.ntop + j];
-      const float w = g.top[row * g.ntop + j];
-      if (t >= 0) sum += w;
-      if (t == c) own += w;
-    }
+  bool again = false;  // the given token among the alternatives
+  for (int j = 0; j < g.ntop; ++j) {
+    const int64_t t = top_idx[row * g.ntop + j];
+    const float w = g.top ? g.top[row * g.ntop + j] : 0.0f;
+    if (t >= 0) sum += w;
+    if (t == c) own += w;
+    again |= k == g.ntop && t == c;
+  }
   const float p = __builtin_amdgcn_exp2f(lp * LOG2E), ge = g.ent ? g.ent[row] : 0.0f;
   if (own == 0.0f && sum == 0.0f && ge == 0.0f) return;  // as the other columns left it
   float d = own - p * __builtin_fmaf(ge, lp + ent[row], sum);
@@ -409,7 +447,10 @@ __global__ __launch_bounds__(NT) void lp_picked(Head h, Upstream g, int64_t igno
     const float t = (lp + lse[row]) / h.tf.inv_t * h.tf.inv_cap;  // tanh of the raw logit
     d *= (1.0f - t) * (1.0f + t);
   }
-  dl[row * ldd + c] = st::f32_to_bf16(d * h.tf.inv_t);
+  d *= h.tf.inv_t;
+  const uint16_t b = st::f32_to_bf16(d);
+  dl[row * ldd + c] = b;
+  if (!again) left[n] = d - st::bf16_to_f32(b);
 }
 
 // dhidden partials: part[split][row][h] = sum over the split's columns of dl head
@@ -451,17 +492,30 @@ __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_dhidden(Dgrad g, 
       }
     }
 }
-__global__ __launch_bounds__(NT) void lp_reduce(const float* __restrict__ part, int64_t rows, int H,
-                                                int splits, uint16_t* __restrict__ out, int64_t ldo) {
-  const int64_t n = rows * H / 4;
+// dhidden = the splits' sums in order, and the picked entries' remainders
+__global__ __launch_bounds__(NT) void lp_reduce(Head h, const float* __restrict__ part, int splits,
+                                                const float* __restrict__ left, int ntop,
+                                                const int64_t* __restrict__ top_idx,
+                                                uint16_t* __restrict__ out, int64_t ldo) {
+  const int64_t per = h.rows * h.H, n = per / 4;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
+    const int64_t row = i * 4 / h.H, col = i * 4 % h.H;
     float4 s = make_float4(0, 0, 0, 0);
     for (int k = 0; k < splits; ++k) {
-      const float4 x = *(const float4*)(part + k * rows * H + i * 4);
+      const float4 x = *(const float4*)(part + k * per + i * 4);
       s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
-    *(uint2*)(out + i * 4 / H * ldo + i * 4 % H) =
-        make_uint2(st::pack_bf16x2(s.x, s.y), st::pack_bf16x2(s.z, s.w));
+    for (int k = 0; k <= ntop; ++k) {
+      const float w = left[row * (ntop + 1) + k];
+      if (w == 0.0f) continue;
+      const int64_t c = k < ntop ? top_idx[row * ntop + k] : h.tokens[row];
+      const uint2 x = *(const uint2*)(h.head + c * h.ldw + col);
+      s.x = __builtin_fmaf(w, __uint_as_float(x.x << 16), s.x);
+      s.y = __builtin_fmaf(w, __uint_as_float(x.x & 0xffff0000u), s.y);
+      s.z = __builtin_fmaf(w, __uint_as_float(x.y << 16), s.z);
+      s.w = __builtin_fmaf(w, __uint_as_float(x.y & 0xffff0000u), s.w);
+    }
+    *(uint2*)(out + row * ldo + col) = make_uint2(st::pack_bf16x2(s.x, s.y), st::pack_bf16x2(s.z, s.w));
   }
 }
 
@@ -471,11 +525,16 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // Row tile of the vocabulary GEMM: cost of a k-step of its 256-column tile
 // relative to 256 rows (a 256x128 tile takes 0.57 of it; a 256x64 one is bound
-// by the head's rows, 0.4).
+// by the head's rows, 0.4).  64 rows whose 256-column tiles leave CUs idle take
+// 128 columns and a deeper ring (col_tile).
 int row_tile(int64_t rows) {
   const double c256 = (double)st::cdiv(rows, 256), c128 = 0.57 * (double)st::cdiv(rows, 128),
                c64 = 0.4 * (double)st::cdiv(rows, 64);
   return c64 <= c128 && c64 <= c256 ? 64 : c128 <= c256 ? 128 : 256;
+}
+
+int col_tile(int64_t rows, int64_t V) {
+  return rows <= 64 && st::cdiv(V, 256) < 256 ? 128 : 256;
 }
 
 // Tile and split of dl head: rounds of 256 workgroups, each a split's k-steps
@@ -515,25 +574,26 @@ Split split_of(int64_t rows, int64_t H, int64_t ldw, int64_t V) {
 struct Space {
   int64_t part, xy, logits, bytes, ldl;
 };
-Space fwd_space(int64_t rows, int64_t V, int64_t top) {
+Space fwd_space(int64_t rows, int64_t V, int64_t top, bool kept) {
   Space s{};
   s.part = 0;
-  s.xy = up(rows * st::cdiv(V, VT) * 16, 256);
+  s.xy = up(rows * st::cdiv(V, col_tile(rows, V)) * 16, 256);
   s.logits = s.xy + up(rows * 4, 256);
   s.ldl = up(V, 4);
-  s.bytes = s.logits + (top > 0 ? rows * s.ldl * 4 : 0) + 256;
+  s.bytes = s.logits + (top > 0 && !kept ? rows * s.ldl * 4 : 0) + 256;
   return s;
 }
 // dl rows padded to 64 columns: whole k-steps start on 128-byte lines
 struct BwdSpace {
-  int64_t part, bytes, ldd;
+  int64_t left, part, bytes, ldd;
   Split split;
 };
-BwdSpace bwd_space(int64_t rows, int64_t H, int64_t ldw, int64_t V) {
+BwdSpace bwd_space(int64_t rows, int64_t H, int64_t ldw, int64_t V, int64_t top) {
   BwdSpace s{};
   s.ldd = up(V, 64);
   s.split = split_of(rows, H, ldw, V);
-  s.part = up(rows * s.ldd * 2, 256);
+  s.left = up(rows * s.ldd * 2, 256);
+  s.part = s.left + up(rows * (top + 1) * 4, 256);
   s.bytes = s.part + s.split.splits * rows * H * 4 + 256;
   return s;
 }
@@ -556,7 +616,8 @@ int check(const char* name, Head& h, const uint16_t* hidden, int64_t rows, int64
   h.hidden = hidden; h.head = head; h.tokens = tokens;
   h.ldh = ldh; h.ldw = ldw; h.rows = rows; h.V = V;
   h.H = (int)H;
-  h.vtiles = (int)st::cdiv(V, VT);
+  h.vt = col_tile(rows, V);
+  h.vtiles = (int)st::cdiv(V, h.vt);
   h.tf = {cap, cap > 0 ? 1.0f / cap : 0.0f, 1.0f / temperature};
   return ST_OK;
 }
@@ -571,16 +632,17 @@ int by_rows(Head& h, F&& fn) {
   const dim3 grid((unsigned)tiles);
   if (bn == 256) fn(st::DmaLoop256<false, false>{}, grid);
   else if (bn == 128) fn(st::DmaLoop64<false, false, 4, 2, 3>{}, grid);
-  else fn(st::DmaLoop64<false, false, 4, 1, 4>{}, grid);
+  else if (h.vt == 256) fn(st::DmaLoop64<false, false, 4, 1, 4>{}, grid);
+  else fn(st::DmaLoop64<false, false, 2, 1, 6>{}, grid);
   return ST_OK;
 }
 
 }  // namespace
 
 extern "C" int64_t st_token_logprobs_workspace_bytes(int64_t rows, int64_t H, int64_t V, int64_t ldw,
-                                                     int64_t top, int32_t backward) {
-  if (rows <= 0 || H <= 0 || V <= 0 || ldw < H || ldw > (1 << 20)) return 0;
-  return backward ? bwd_space(rows, H, ldw, V).bytes : fwd_space(rows, V, top).bytes;
+                                                     int64_t top, int32_t kept, int32_t backward) {
+  if (rows <= 0 || H <= 0 || V <= 0 || ldw < H || ldw > (1 << 20) || top < 0) return 0;
+  return backward ? bwd_space(rows, H, ldw, V, top).bytes : fwd_space(rows, V, top, kept != 0).bytes;
 }
 
 extern "C" int st_token_logprobs_fwd(const uint16_t* hidden, int64_t rows, int64_t H, int64_t ldh,
@@ -588,29 +650,35 @@ extern "C" int st_token_logprobs_fwd(const uint16_t* hidden, int64_t rows, int64
                                      const int64_t* tokens, int64_t ignore_index, float temperature,
                                      float cap, int64_t top, float* logprobs, float* entropy,
                                      float* lse, float* top_logprobs, int64_t* top_tokens,
-                                     void* workspace, int64_t workspace_bytes, st_stream_t stream) {
+                                     float* logits, void* workspace, int64_t workspace_bytes,
+                                     st_stream_t stream) {
   const char* name = "st_token_logprobs_fwd";
   Head h{};
   if (int rc = check(name, h, hidden, rows, H, ldh, head, V, ldw, tokens, temperature, cap, top)) return rc;
   if (rows == 0) return ST_OK;
-  ST_CHECK_ARG(logprobs && entropy && lse && (!top || (top_logprobs && top_tokens)),
+  ST_CHECK_ARG(logprobs && entropy && lse && (!top || (top_logprobs && top_tokens)) && al16(logits),
                "%s: NULL or unaligned pointer", name);
-  const Space sp = fwd_space(rows, V, top);
+  const Space sp = fwd_space(rows, V, top, logits != nullptr);
   if (!workspace || workspace_bytes < sp.bytes)
     return st::fail(ST_EWORKSPACE, "%s: needs %lld workspace bytes", name, (long long)sp.bytes);
   char* ws = (char*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
   float4* part = (float4*)(ws + sp.part);
   float* xy = (float*)(ws + sp.xy);
-  float* logits = top ? (float*)(ws + sp.logits) : nullptr;
+  if (top && !logits) logits = (float*)(ws + sp.logits);
   hipStream_t s = (hipStream_t)stream;
   if (int rc = by_rows(h, [&](auto lp, dim3 grid) {
         using LP = decltype(lp);
-        lp_tiles<LP><<<grid, LP::NT, 0, s>>>(h, part, xy, logits, sp.ldl);
+        lp_tiles<LP><<<grid, LP::NT, 0, s>>>(h, part, xy, logits, sp.ldl, top > 0);
       })) return rc;
   if (int rc = st::check_launch(name)) return rc;
-  lp_join<<<(unsigned)st::cdiv(rows, NT / 64), NT, top ? (NT / 64) * h.vtiles * 4 : 0, s>>>(
-      h, ignore_index, part, xy, logits, sp.ldl, (int)top, logprobs, entropy, lse, top_logprobs,
-      top_tokens);
+  const dim3 grid((unsigned)st::cdiv(rows, NT / 64));
+  const size_t lds = top ? (NT / 64) * h.vtiles * 4 : 0;
+  auto join = [&](auto kernel) {
+    kernel<<<grid, NT, lds, s>>>(h, ignore_index, part, xy, logits, sp.ldl, (int)top, logprobs, entropy,
+                                 lse, top_logprobs, top_tokens);
+  };
+  if (h.vt == 256) join(lp_join<256>);
+  else join(lp_join<128>);
   return st::check_launch("lp_join");
 }
 
@@ -620,32 +688,41 @@ extern "C" int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64
                                      float cap, int64_t top, const float* logprobs,
                                      const float* entropy, const float* lse,
                                      const float* top_logprobs, const int64_t* top_tokens,
-                                     const float* g_logprobs, const float* g_entropy,
-                                     const float* g_top, uint16_t* dhidden, int64_t ldd,
-                                     void* workspace, int64_t workspace_bytes, st_stream_t stream) {
+                                     const float* logits, const float* g_logprobs,
+                                     const float* g_entropy, const float* g_top, uint16_t* dhidden,
+                                     int64_t ldd, void* workspace, int64_t workspace_bytes,
+                                     st_stream_t stream) {
   const char* name = "st_token_logprobs_bwd";
   Head h{};
   if (int rc = check(name, h, hidden, rows, H, ldh, head, V, ldw, tokens, temperature, cap, top)) return rc;
   if (rows == 0) return ST_OK;
   ST_CHECK_ARG(logprobs && entropy && lse && (!top || (top_logprobs && top_tokens)) && dhidden &&
-                   al16(dhidden) && ldd % 8 == 0 && ldd >= H, "%s: NULL or unaligned pointer", name);
-  const BwdSpace sp = bwd_space(rows, H, ldw, V);
+                   al16(dhidden) && al16(logits) && ldd % 8 == 0 && ldd >= H,
+               "%s: NULL or unaligned pointer", name);
+  const BwdSpace sp = bwd_space(rows, H, ldw, V, top);
   if (!workspace || workspace_bytes < sp.bytes)
     return st::fail(ST_EWORKSPACE, "%s: needs %lld workspace bytes", name, (long long)sp.bytes);
   if (sp.split.splits == 0)
     return st::fail(ST_EUNSUPPORTED, "%s: 64 columns of the head span 2 GiB", name);
   char* ws = (char*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
   uint16_t* dl = (uint16_t*)ws;
-  float* part = (float*)(ws + sp.part);
+  float *left = (float*)(ws + sp.left), *part = (float*)(ws + sp.part);
   hipStream_t s = (hipStream_t)stream;
   const Upstream g{g_logprobs, g_entropy, top ? g_top : nullptr, (int)top};
-  if (int rc = by_rows(h, [&](auto lp, dim3 grid) {
-        using LP = decltype(lp);
-        lp_dlogits<LP><<<grid, LP::NT, 0, s>>>(h, g, ignore_index, top_tokens, lse, entropy, dl, sp.ldd);
-      })) return rc;
+  if (logits) {
+    const unsigned y = (unsigned)std::min<int64_t>(rows, 32768);
+    lp_dlogits_kept<<<dim3((unsigned)st::cdiv(sp.ldd, NT * KEPT), y, (unsigned)st::cdiv(rows, y)), NT, 0,
+                      s>>>(h, g, ignore_index, top_tokens, lse, entropy, logits, up(V, 4), dl, sp.ldd);
+  } else if (int rc = by_rows(h, [&](auto lp, dim3 grid) {
+               using LP = decltype(lp);
+               lp_dlogits<LP><<<grid, LP::NT, 0, s>>>(h, g, ignore_index, top_tokens, lse, entropy, dl,
+                                                     sp.ldd);
+             })) {
+    return rc;
+  }
   if (int rc = st::check_launch(name)) return rc;
   lp_picked<<<(unsigned)st::cdiv(rows * (top + 1), NT), NT, 0, s>>>(
-      h, g, ignore_index, top_tokens, top_logprobs, logprobs, lse, entropy, dl, sp.ldd);
+      h, g, ignore_index, top_tokens, top_logprobs, logprobs, lse, entropy, dl, sp.ldd, left);
   if (int rc = st::check_launch("lp_picked")) return rc;
   const Split& k = sp.split;
   const Dgrad d{dl, head, sp.ldd, ldw, rows, V, (int)H, (int)st::cdiv(rows, k.bm),
@@ -659,6 +736,6 @@ extern "C" int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64
     lp_dhidden<st::DmaLoop256<true, false>><<<grid, 512, 0, s>>>(d, part);
   if (int rc = st::check_launch("lp_dhidden")) return rc;
   lp_reduce<<<(unsigned)std::min<int64_t>(st::cdiv(rows * H / 4, NT), 4096), NT, 0, s>>>(
-      part, rows, (int)H, k.splits, dhidden, ldd);
+      h, part, k.splits, left, (int)top, top_tokens, dhidden, ldd);
   return st::check_launch("lp_reduce");
 }

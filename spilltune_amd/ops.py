@@ -775,35 +775,46 @@ class TokenLogProbs(NamedTuple):
 
 
 LOGPROB_SCRATCH = 2 << 30  # bytes of scratch a token_logprobs call aims to stay within
+# bytes of fp32 logits that a call keeps for its backward, which then does not form
+# them again (2048 rows of 151936 tokens, hidden 4096: 1.2 GB, a quarter of the pass)
+LOGPROB_KEEP = 2 << 30
 
 
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def _row_chunks(hidden, head, top, backward):
-        """Row ranges whose scratch stays within LOGPROB_SCRATCH (256 rows at
-        least): 4 bytes a logit with alternatives, 2 in the backward."""
-        rows, (V, H) = hidden.shape[0], head.shape
-        per = 2 * V if backward else 4 * V if top else V // 16 + 20
+    def _row_chunks(rows, per):
+        """Row ranges whose scratch of ``per`` bytes a row stays within
+        LOGPROB_SCRATCH (256 rows at least)."""
         step = max(256, LOGPROB_SCRATCH // per // 256 * 256)
         return [(r, min(r + step, rows)) for r in range(0, rows, step)]
 
     @staticmethod
-    def forward(ctx, hidden, head, tokens, ignore_index, temperature, cap, top):
+    def forward(ctx, hidden, head, tokens, ignore_index, temperature, cap, top, grad):
         rows, H = hidden.shape
         V, dev = head.shape[0], hidden.device
+        ldw, ldl = head.stride(0), (V + 3) // 4 * 4
         lp, ent, lse = (torch.empty(rows, dtype=_F32, device=dev) for _ in range(3))
         top_lp = torch.empty((rows, top), dtype=_F32, device=dev)
         top_tok = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        logits = None
+        if grad and rows and rows * ldl * 4 <= LOGPROB_KEEP:
+            try:
+                logits = torch.empty((rows, ldl), dtype=_F32, device=dev)
+            except torch.OutOfMemoryError:
+                pass
+        kept = int(logits is not None)
         with _lib.on_device(dev):
-            for a, z in _TokenLogProbs._row_chunks(hidden, head, top, False):
-                ws = _scratch(dev, _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V,
-                                              head.stride(0), top, 0))
+            for a, z in _TokenLogProbs._row_chunks(rows, 4 * V if top and not kept else V // 8 + 20):
+                nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, ldw, top, kept, 0)
+                ws = _scratch(dev, nbytes)
                 _lib.call("st_token_logprobs_fwd", _lib.ptr(hidden[a:z]), z - a, H, hidden.stride(0),
-                          _lib.ptr(head), V, head.stride(0), _lib.ptr(tokens[a:z]), ignore_index,
-                          temperature, cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]),
-                          _lib.ptr(lse[a:z]), _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]),
-                          _lib.ptr(ws), ws.numel(), _lib.stream_handle(dev))
-        ctx.save_for_backward(hidden, head, tokens, lp, ent, lse, top_lp, top_tok)
+                          _lib.ptr(head), V, ldw, _lib.ptr(tokens[a:z]), ignore_index, temperature,
+                          cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]), _lib.ptr(lse[a:z]),
+                          _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]),
+                          _lib.ptr(logits[a:z]) if kept else None, _lib.ptr(ws), nbytes,
+                          _lib.stream_handle(dev))
+        if grad:
+            ctx.save_for_backward(hidden, head, tokens, lp, ent, lse, top_lp, top_tok, logits)
         ctx.meta = (ignore_index, temperature, cap, top)
         ctx.mark_non_differentiable(top_tok)
         ctx.set_materialize_grads(False)
@@ -812,23 +823,23 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g_lp, g_ent, g_top, _):
         _once()
-        hidden, head, tokens, lp, ent, lse, top_lp, top_tok = ctx.saved_tensors
+        hidden, head, tokens, lp, ent, lse, top_lp, top_tok, logits = ctx.saved_tensors
         ignore_index, temperature, cap, top = ctx.meta
-        H, V, dev = hidden.shape[1], head.shape[0], hidden.device
+        (rows, H), V, ldw, dev = hidden.shape, head.shape[0], head.stride(0), hidden.device
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
         part = lambda g, a, z: None if g is None else _lib.ptr(g[a:z])  # noqa: E731
-        dh = torch.empty(hidden.shape, dtype=_BF16, device=dev)
+        dh = torch.empty((rows, H), dtype=_BF16, device=dev)
         with _lib.on_device(dev):
-            for a, z in _TokenLogProbs._row_chunks(hidden, head, top, True):
-                ws = _scratch(dev, _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V,
-                                              head.stride(0), top, 1))
+            for a, z in _TokenLogProbs._row_chunks(rows, 2 * V):
+                nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, ldw, top, 0, 1)
+                ws = _scratch(dev, nbytes)
                 _lib.call("st_token_logprobs_bwd", _lib.ptr(hidden[a:z]), z - a, H, hidden.stride(0),
-                          _lib.ptr(head), V, head.stride(0), _lib.ptr(tokens[a:z]), ignore_index,
-                          temperature, cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]),
-                          _lib.ptr(lse[a:z]), _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]),
+                          _lib.ptr(head), V, ldw, _lib.ptr(tokens[a:z]), ignore_index, temperature,
+                          cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]), _lib.ptr(lse[a:z]),
+                          _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]), part(logits, a, z),
                           part(g_lp, a, z), part(g_ent, a, z), part(g_top, a, z), _lib.ptr(dh[a:z]),
-                          dh.stride(0), _lib.ptr(ws), ws.numel(), _lib.stream_handle(dev))
-        return dh, None, None, None, None, None, None
+                          H, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+        return dh, None, None, None, None, None, None, None
 
 
 def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ignore_index=-100):
@@ -838,8 +849,8 @@ def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ig
     probable tokens, as :class:`TokenLogProbs`.
 
     Logits are ``hidden head^T``, with ``cap`` ``cap * tanh(logits / cap)``, over
-    ``temperature``; they are summed in fp32 and not kept, the backward forms them
-    again.  Differentiable in ``hidden`` through all three fp32 results.  A token
+    ``temperature``, summed in fp32.  They are kept for a backward where they take
+    at most ``LOGPROB_KEEP`` bytes; otherwise it forms them again.  Differentiable in ``hidden`` through all three fp32 results.  A token
     equal to ``ignore_index`` has log probability 0 and no gradient from it (its
     entropy and alternatives are those of its hidden state); any other token
     outside [0, V) gives NaN when it comes on the device and is refused when it
@@ -872,7 +883,7 @@ def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ig
     shape = tuple(tokens.shape)
     lp, ent, top_lp, top_tok = _TokenLogProbs.apply(
         _operand(hidden.reshape(-1, H)), _operand(head), tokens.reshape(-1).contiguous(),
-        int(ignore_index), temperature, cap, top)
+        int(ignore_index), temperature, cap, top, torch.is_grad_enabled() and hidden.requires_grad)
     return TokenLogProbs(lp.view(shape), ent.view(shape), top_lp.view(*shape, top),
                          top_tok.view(*shape, top))
 

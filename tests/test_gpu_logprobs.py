@@ -78,7 +78,10 @@ SIZES = [(1, 8, 1), (1, 64, 7), (5, 72, 255), (61, 264, 257), (64, 128, 1000), (
 
 @pytest.mark.parametrize("rows,H,V", SIZES)
 @pytest.mark.parametrize("temperature,cap", [(1.0, None), (0.7, 5.0), (2.0, None)])
-def test_values_and_gradient(rows, H, V, temperature, cap):
+@pytest.mark.parametrize("kept", [True, False])
+def test_values_and_gradient(monkeypatch, rows, H, V, temperature, cap, kept):
+    if not kept:  # the backward forms the logits again
+        monkeypatch.setattr(ops, "LOGPROB_KEEP", 0)
     h, w, t, g = _inputs(rows, H, V, seed=rows)
     t[::7] = -100
     g_lp, g_ent = (torch.randn(rows, generator=g, device="cuda") for _ in range(2))
@@ -94,8 +97,11 @@ def test_values_and_gradient(rows, H, V, temperature, cap):
 
 @pytest.mark.parametrize("rows,V,top", [(1, 64, 64), (5, 300, 1), (70, 5000, 20), (260, 2049, 5),
                                         (3, 2, 2), (130, 1000, 8)])
-def test_alternatives(rows, V, top):
+@pytest.mark.parametrize("kept", [True, False])
+def test_alternatives(monkeypatch, rows, V, top, kept):
     """Falling values, ties to the lowest index, and their gradient."""
+    if not kept:
+        monkeypatch.setattr(ops, "LOGPROB_KEEP", 0)
     h, w, t, g = _inputs(rows, 64, V, seed=V, grid=True)
     w[V // 2:] = w[:V - V // 2].clone()  # every logit of the second half ties with one of the first
     t[1::5] = -100
@@ -151,6 +157,31 @@ def test_rows_of_garbage():
     assert bool((r.top_tokens < 700).all())
 
 
+def test_the_same_token_given_and_among_the_alternatives():
+    """An entry picked twice counts once; gradients of the alternatives alone."""
+    h, w, _, g = _inputs(40, 64, 900, seed=5, grid=True)
+    l = h.double() @ w.double().T
+    idx = torch.sort(l, dim=1, descending=True, stable=True).indices[:, :3]
+    t = idx[:, 1].contiguous()
+    g_lp, g_top = torch.randn(40, generator=g, device="cuda"), torch.randn(40, 3, generator=g,
+                                                                           device="cuda")
+    h.requires_grad_(True)
+    r = ops.token_logprobs(h, w, t, top=3)
+    assert torch.equal(r.logprobs, r.top_logprobs[:, 1])
+    for grads in ((g_lp, g_top), (None, g_top), (g_lp, None)):
+        outs = [o for o, x in zip((r.logprobs, r.top_logprobs), grads) if x is not None]
+        (dh,) = torch.autograd.grad(outs, h, [x for x in grads if x is not None], retain_graph=True)
+        want, err, _, _ = _reference(h.detach(), w, t, grads=(grads[0], None, grads[1]), top_idx=idx)
+        _close("dh", dh, want[2], err[2])
+
+
+def test_no_second_derivative():
+    h, w, t, _ = _inputs(4, 64, 300)
+    h.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(ops.token_logprobs(h, w, t).logprobs.sum(), h, create_graph=True)
+
+
 def test_host_tokens_and_shapes():
     h, w, t, _ = _inputs(12, 64, 300)
     a = ops.token_logprobs(h.view(3, 4, 64), w, t.cpu().view(3, 4), top=2)
@@ -166,12 +197,14 @@ def test_host_tokens_and_shapes():
         h[:1], w, t[:1]).logprobs[0])
 
 
-def test_row_chunks(monkeypatch):
+@pytest.mark.parametrize("keep", [0, 1 << 30])
+def test_row_chunks(monkeypatch, keep):
     h, w, t, g = _inputs(600, 64, 3000, grid=True)
     g_lp = torch.randn(600, generator=g, device="cuda")
     h.requires_grad_(True)
     want, err, l, _ = _reference(h.detach(), w, t, grads=(g_lp, None, None))
     monkeypatch.setattr(ops, "LOGPROB_SCRATCH", 1 << 20)
+    monkeypatch.setattr(ops, "LOGPROB_KEEP", keep)
     r = ops.token_logprobs(h, w, t, top=4)
     (dh,) = torch.autograd.grad(r.logprobs, h, g_lp)
     _close("logprobs", r.logprobs, want[0], err[0])

@@ -42,7 +42,7 @@ def test_abi_refuses_before_the_device():
     def fwd(rows=4, H=16, V=40, ldh=16, ldw=16, T=1.0, cap=0.0, top=0, hidden=p, ws=p, wb=1 << 40,
             lp=p, tt=p):
         _lib.call("st_token_logprobs_fwd", hidden, rows, H, ldh, p, V, ldw, p, -100, T, cap, top, lp, p,
-                  p, p, tt, ws, wb, None)
+                  p, p, tt, None, ws, wb, None)
     for kw, msg in (({"H": 12}, "16-byte"), ({"ldw": 8}, "16-byte"), ({"ldh": 20}, "16-byte"),
                     ({"T": 0.0}, "temperature"), ({"cap": -1.0}, "cap"), ({"top": 41}, "within"),
                     ({"V": 400, "top": 65}, "too large"), ({"V": 1 << 23}, "too large"),
@@ -55,11 +55,12 @@ def test_abi_refuses_before_the_device():
 
     def bwd(ldd=16, dh=p, wb=1 << 40):
         _lib.call("st_token_logprobs_bwd", p, 4, 16, 16, p, 40, 16, p, -100, 1.0, 0.0, 0, p, p, p, n, n,
-                  p, n, n, dh, ldd, p, wb, None)
+                  n, p, n, n, dh, ldd, p, wb, None)
     for kw, msg in (({"ldd": 8}, "NULL or"), ({"dh": n}, "NULL"), ({"wb": 10}, "workspace")):
         with pytest.raises(ValueError, match=msg):
             bwd(**kw)
     q = lambda *a: _lib.query("st_token_logprobs_workspace_bytes", *a)  # noqa: E731
-    assert q(0, 16, 40, 16, 0, 0) == 0 and q(4, 16, 40, 8, 0, 0) == 0
-    assert q(1000, 64, 5000, 64, 5, 0) - q(1000, 64, 5000, 64, 0, 0) == 1000 * 5000 * 4
-    assert q(1000, 64, 5000, 64, 0, 1) >= 1000 * 5000 * 2
+    assert q(0, 16, 40, 16, 0, 0, 0) == 0 and q(4, 16, 40, 8, 0, 0, 0) == 0
+    assert q(1000, 64, 5000, 64, 5, 0, 0) - q(1000, 64, 5000, 64, 0, 0, 0) == 1000 * 5000 * 4
+    assert q(1000, 64, 5000, 64, 5, 1, 0) == q(1000, 64, 5000, 64, 0, 0, 0)
+    assert q(1000, 64, 5000, 64, 0, 0, 1) >= 1000 * 5000 * 2
