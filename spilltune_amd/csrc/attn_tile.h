@@ -80,13 +80,16 @@ __device__ __forceinline__ bf16x8 tile_tr(const uint16_t* t, int kb, int nb, int
 
 // The same two operands by a lane's own address: `lane_row` / `lane_tr` once,
 // then one exclusive-or with a constant per read, the rest in the instruction's
-// offset (the row's chunks stay within aligned bits of the byte address).
+// offset (the row's chunks stay within aligned bits of the byte address).  The
+// tile comes through a __restrict__ pointer: the caller has waited for its DMAs
+// and passed the barrier, and without it the compiler waits for every DMA in
+// flight before the first read.
 template <int D>
 __device__ __forceinline__ uint32_t lane_row(int row, int g) {
   return (uint32_t)(row * D * 2 + ((g ^ swz<D>(row)) << 4));
 }
 template <int D>  // chunk 2 s + g of row `row0` + the lane's, row0 a multiple of 16
-__device__ __forceinline__ bf16x8 read_row(const uint16_t* t, uint32_t lane, int row0, int s) {
+__device__ __forceinline__ bf16x8 read_row(const uint16_t* __restrict__ t, uint32_t lane, int row0, int s) {
   constexpr int IN = D == 128 ? 15 : 7;  // chunks that the swizzle permutes
   const uint32_t at = (lane ^ (uint32_t)((2 * s & IN) << 4)) + (2 * s & ~IN) * 16 + row0 * D * 2;
   return as_bf16x8(*(const uint4*)((const char*)t + at));
@@ -98,7 +101,7 @@ __device__ __forceinline__ uint32_t lane_tr(int lane) {
   return (uint32_t)(row * D * 2 + ((chunk ^ swz<D>(row)) << 4) + (i & 1) * 8);
 }
 template <int D>  // tile_tr(t, kb, 32 db), kb a multiple of 16
-__device__ __forceinline__ bf16x8 read_tr(const uint16_t* t, uint32_t lane, int kb, int db) {
+__device__ __forceinline__ bf16x8 read_tr(const uint16_t* __restrict__ t, uint32_t lane, int kb, int db) {
   constexpr int IN = D == 128 ? 15 : 7;
   typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
   v4bf r[2];

@@ -43,6 +43,7 @@ constexpr int NT = 256;
 constexpr int TILE = 128;  // queries (dQ, forward) or keys (dK, dV) per workgroup
 constexpr int BKT = 64;    // keys per step of the forward and dQ passes
 constexpr int QT = 64;     // queries per step of the dK/dV pass
+constexpr int LEAD = 6;  // LDS reads ahead of the MFMAs (see fed)
 constexpr int SHORT = 256;   // keys of a tile whose delta is summed from P dP
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_LOG2 = 8.0f;  // the running maximum may lag by up to 2^8
@@ -87,10 +88,13 @@ Plan plan_of(const void* base, int64_t B, int64_t S) {
   return p;
 }
 
+__device__ __forceinline__ int2 clamp_run(int2 r, int S) {
+  const int a = min(max(r.x, 0), S), z = min(max(r.y, 0), S);
+  return a < z ? make_int2(a, z) : make_int2(0, 0);
+}
 __device__ __forceinline__ int2 run_of(const int32_t* __restrict__ lo, const int32_t* __restrict__ hi,
                                        int64_t at, int S) {
-  const int a = min(max(lo[at], 0), S), z = min(max(hi[at], 0), S);
-  return a < z ? make_int2(a, z) : make_int2(0, 0);
+  return clamp_run(make_int2(lo[at], hi[at]), S);
 }
 
 // one 32-lane half per block of 32 queries
@@ -225,7 +229,26 @@ __device__ __forceinline__ float score_small(const Args& a, float s) {
   return s * __builtin_fmaf(p, z, a.sl2);
 }
 
+// Instruction order of a run of MFMAs fed from LDS: LEAD reads ahead, then PER
+// after each MFMA.  Left alone the compiler reads an operand just before its use
+// and every pair of MFMAs waits for the LDS.
+template <int READS, int MFMAS, int LEAD, int PER>
+__device__ __forceinline__ void fed() {
+  __builtin_amdgcn_sched_group_barrier(0x100, LEAD, 0);
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (LEAD + i * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+  }
+}
+
 __device__ __forceinline__ bool finite(float x) { return x - x == 0.0f; }
+// the greater of this lane's value and of the lane's 32 on or back
+__device__ __forceinline__ float half_max(float x) {
+  // the swap leaves the lower half's values in both halves of r[0], the upper's in r[1]
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 // 0 if every value is finite
 template <int N>
 __device__ __forceinline__ float probe_of(const f32x16 (&acc)[N]) {
@@ -313,8 +336,20 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float mu
 
 // a value that every lane of the wave holds alike, in scalar registers
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int4 uniform(int4 x) {
-  return make_int4(uniform(x.x), uniform(x.y), uniform(x.z), uniform(x.w));
+
+// A value at a wave-uniform address that no one writes during the kernel, by a
+// scalar load: a vector load behind the tile copies would wait for all of them.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+  typedef const __attribute__((address_space(4))) T* sp;
+  return *(sp)(uintptr_t)p;
+}
+
+// LDS values that no copy in flight writes (as read_row's tiles)
+__device__ __forceinline__ float4 lds4(const float* __restrict__ p) { return *(const float4*)p; }
+template <typename T>
+__device__ __forceinline__ T lds1(const T* __restrict__ p) {
+  return *p;
 }
 
 // the same in fp32 (`os`: 32 rows of D + 4 floats)
@@ -340,6 +375,12 @@ __device__ __forceinline__ void store_rows_f32(const f32x16 (&acc)[D / 32], floa
   __builtin_amdgcn_wave_barrier();
 }
 
+__device__ __forceinline__ int4 extremes(const int4* p) {
+  typedef int i4 __attribute__((ext_vector_type(4)));
+  const i4 x = scalar_load((const i4*)p);
+  return make_int4(x.x, x.y, x.z, x.w);
+}
+
 // Key range of a 128-query tile and the wave's own block of extremes.
 struct Walk {
   int4 mine;       // of this wave's 32 queries
@@ -351,7 +392,7 @@ __device__ __forceinline__ Walk walk_of(const Plan& p, int b, int qt, int wave) 
   for (int i = 0; i < 4; ++i) {
     const int n = qt * 4 + i;
     if (n >= p.nb) break;
-    const int4 x = uniform(p.blk[(int64_t)b * p.nb + n]);
+    const int4 x = extremes(p.blk + (int64_t)b * p.nb + n);
     w.first = min(w.first, x.x);
     w.end = max(w.end, x.w);
     if (i == wave) w.mine = x;
@@ -596,8 +637,10 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
   if (w.first < w.end) issue(w.first, 0);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  int buf = 0;
-  for (int k0 = w.first; k0 < w.end; k0 += BKT, buf ^= 1) {
+  // the buffer is a constant of each half of the unrolled loop: LDS addresses
+  // are then a lane's own and an offset within the instruction
+  auto step = [&](int k0, auto which) {
+    constexpr int buf = decltype(which)::value;
     if (k0 + BKT < w.end) issue(k0 + BKT, buf ^ 1);
     const uint16_t* ks = lds + buf * (LK + LV);
     const uint16_t* vs = ks + LK;
@@ -614,6 +657,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
         for (int jb = 0; jb < 2; ++jb)
           sacc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DQ>(ks, lr, jb * 32, s),
                                                              qf[s], sacc[jb], 0, 0, 0);
+      fed<2 * DS, 2 * DS, LEAD, 1>();
       if constexpr ((MODE & CAP) != 0) {
         float top = 0.0f;
 #pragma unroll
@@ -663,7 +707,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
       for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) mt = fmaxf(mt, sacc[jb][v]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32)) * mul;
+      mt = half_max(mt) * mul;
       if (__ballot(mt > m_run + RESCALE_LOG2)) {
         const float m_new = fmaxf(m_run, mt);
         // a row with no key yet: -inf - -inf is not a number, its sums are 0
@@ -695,9 +739,15 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
         for (int db = 0; db < DB; ++db)
           oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_tr<DV>(vs, lt, cc * 16, db),
                                                              pf[cc], oacc[db], 0, 0, 0);
+      fed<8 * DB, 4 * DB, 2 * LEAD, 2>();
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
+  };
+#pragma unroll 1
+  for (int k0 = w.first; k0 < w.end; k0 += 2 * BKT) {
+    step(k0, std::integral_constant<int, 0>{});
+    if (k0 + BKT < w.end) step(k0 + BKT, std::integral_constant<int, 1>{});
   }
 
   const float l_tot = l_run + __shfl_xor(l_run, 32);
@@ -817,6 +867,7 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
           pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DV>(vs, lrv, jb * 32, s),
                                                          dof[s < DSV ? s : 0], pacc, 0, 0, 0);
       }
+      if constexpr (DQ != 192) fed<DSQ + DSV, DSQ + DSV, LEAD, 1>();
       bf16x8 dsf[2], dsl[2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
@@ -840,13 +891,27 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
       }
       if (only_delta) continue;
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
+      for (int hh = 0; hh < 2; ++hh) {
+        // operands in registers at once; at DQ = 192 all six, or reads ordered
+        // ahead of the MFMAs, spilled (the pass 561 us against 540 at one
+        // sequence of 2048 tokens and 128 heads)
+        constexpr int GRP = DQ == 192 ? 2 : DB;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const bf16x8 kt = read_tr<DQ>(ks, lt, jb * 32 + 16 * hh, db);
-          dqacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, dsf[hh], dqacc[db], 0, 0, 0);
-          dqacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, dsl[hh], dqacc[db], 0, 0, 0);
+        for (int d0 = 0; d0 < DB; d0 += GRP) {
+          bf16x8 ktr[GRP];
+#pragma unroll
+          for (int e = 0; e < GRP; ++e) ktr[e] = read_tr<DQ>(ks, lt, jb * 32 + 16 * hh, d0 + e);
+#pragma unroll
+          for (int e = 0; e < GRP; ++e)
+            dqacc[d0 + e] =
+                __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktr[e], dsf[hh], dqacc[d0 + e], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < GRP; ++e)
+            dqacc[d0 + e] =
+                __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktr[e], dsl[hh], dqacc[d0 + e], 0, 0, 0);
         }
+      }
+      if constexpr (DQ != 192) fed<4 * DB, 4 * DB, 6, 2>();
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -876,15 +941,20 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
 // The whole group in one workgroup needs no partial sums in memory; a tile with
 // much more work than a CU's share has its group split over several workgroups
 // (parts_of), and span_reduce adds their fp32 sums in order.
-constexpr int SHARE = 2;
+// A tile stays whole up to a CU's share of all work (256 CUs) or 16 steps (of 2
+// blocks each); a heavier one is split, by a divisor of the group, into parts of
+// at most three quarters of a share.  Training pass in us, against parts of at
+// most half a share whatever the tile: 8192 tokens, 32/8 heads of 128, 16 equal
+// documents 283 : 316, documents of 60 to 2500 tokens 463 : 479; one document 2718
+// : 2800; 16384 tokens of 2 documents, 16/2 heads, 3282 : 3036.
 __device__ __forceinline__ int parts_of(const Plan& p, int id, int group, int Hkv, int most) {
-  // work of this tile over SHARE quarters of a CU's share of all tiles, as a
-  // divisor of the group; tiles of at most 16 steps (2 blocks each) stay whole
   if (most == 1) return 1;
-  const int64_t w = (int64_t)uniform(p.kwork[id]) * group, all = uniform(*p.ktotal);
-  const int64_t share = max(all * group * Hkv * SHARE / 1024, (int64_t)32);
+  const int64_t w = (int64_t)uniform(p.kwork[id]) * group;
+  const int64_t share = (int64_t)uniform(*p.ktotal) * group * Hkv;  // of 256 CUs
+  if (w * 256 <= share || w <= 32) return 1;
+  const int64_t piece = max(share * 3 / 1024, (int64_t)32);
   int n = 1;
-  while (n < most && (group % n || w > share * n)) ++n;
+  while (n < most && (group % n || w > piece * n)) ++n;
   return n;
 }
 
@@ -892,9 +962,12 @@ template <int DQ>
 constexpr int dkdv_waves() {
   return DQ <= 128 ? 8 : 4;
 }
+// elements of the LDS array that holds the K and V tiles, later the sums' meeting
+// place and each wave's rows on their way out (fp32 rows of 192 do not fit)
 template <int DQ, int DV>
 constexpr int dkdv_lds() {
-  return (dkdv_waves<DQ>() == 8 ? TILE + 2 * QT : 2 * QT) * (DQ + DV);
+  constexpr int tiles = TILE * (DQ + DV), sums = 4 * 32 * (DQ + 4) * 2, rows = 4 * 32 * (DQ + 8);
+  return dkdv_waves<DQ>() == 4 ? rows : tiles > sums ? tiles : sums;
 }
 
 template <int DQ, int DV, int MODE>
@@ -908,6 +981,9 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   constexpr int NW = dkdv_waves<DQ>(), NTH = 64 * NW, QH = 8 / NW;
   constexpr bool KREG = NW == 4;
   __shared__ __attribute__((aligned(16))) uint16_t lds[dkdv_lds<DQ, DV>()];
+  // arrays of their own: a read of one is not taken for a read of what the copies
+  // into another still write, and does not wait for them
+  __shared__ __attribute__((aligned(16))) uint16_t q_a[LQ], q_b[LQ], g_a[LG], g_b[LG];
   __shared__ __attribute__((aligned(16))) float lse_s[2][QT], dl_s[2][QT];
   __shared__ __attribute__((aligned(16))) int lo_s[2][QT], wd_s[2][QT];
   const int S = a.S, H = a.H, nb = a.plan.nb, group = H / a.Hkv;
@@ -929,7 +1005,6 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   const uint16_t* vb = a.v + (int64_t)(b * a.Hkv + hk) * S * DV;
   uint16_t* Ks = lds;
   uint16_t* Vs = lds + LK;
-  uint16_t* qg = KREG ? lds : lds + LK + LV;
   const int k0 = kt * TILE, kw0 = k0 + kq * 32, mykey = kw0 + c;
   const int2 seen = make_int2(uniform(a.plan.keys[id].x), uniform(a.plan.keys[id].y));
   const int4* blk = a.plan.blk + (int64_t)b * nb;
@@ -964,116 +1039,153 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   const int steps = nq * heads;
   const TileCopy<DQ, NTH, QT> cq(tid, DQ);
   const TileCopy<DV, NTH, QT> cg(tid, ldt);
-  float lr = 0.0f, dr = 0.0f;
+  float lr = INFINITY, dr = 0.0f;
   int2 rr = make_int2(0, 0);
-  auto issue = [&](int h, int q0, int buf) {
-    uint16_t* qs = qg + buf * (LQ + LG);
-    cq(a.q + (int64_t)(b * H + h) * S * DQ, DQ, q0, S, qs, wave);
-    cg(dout + (int64_t)b * S * ldt + (int64_t)h * DV, ldt, q0, S, qs + LQ, wave);
-    if (tid < QT) {
+  auto issue = [&](int h, int q0, auto which) {
+    constexpr int buf = decltype(which)::value;
+    cq(a.q + (int64_t)(b * H + h) * S * DQ, DQ, q0, S, buf ? q_b : q_a, wave);
+    cg(dout + (int64_t)b * S * ldt + (int64_t)h * DV, ldt, q0, S, buf ? g_b : g_a, wave);
+    if (tid < QT) {  // used at the end of the step, when the copies have landed too
       const int i = q0 + tid;
-      const int64_t at = (int64_t)(b * H + h) * S + i;
-      lr = i < S ? lse[at] : INFINITY;
-      dr = i < S ? delta[at] : 0.0f;
-      rr = i < S ? run_of(a.lo, a.hi, (int64_t)b * S + i, S) : make_int2(0, 0);
+      const bool in = i < S;
+      const int64_t at = (int64_t)(b * H + h) * S + i, row = (int64_t)b * S + i;
+      lr = in ? lse[at] : INFINITY;
+      dr = in ? delta[at] : 0.0f;
+      rr = in ? make_int2(a.lo[row], a.hi[row]) : make_int2(0, 0);
     }
   };
+  // FOLD: the accumulators of S and dP start from -lse / sl2 and -delta of their
+  // rows, read from LDS as they lie, so the statistics take no registers of their
+  // own and no instruction (a cap needs the bare product)
+  constexpr bool FOLD = (MODE & CAP) == 0;
+  const float over = 1.0f / a.sl2;
   auto stats = [&](int buf) {
     if (tid < QT) {
-      lse_s[buf][tid] = lr;
-      dl_s[buf][tid] = dr;
-      lo_s[buf][tid] = rr.x;
-      wd_s[buf][tid] = rr.y - rr.x;
+      const int2 r = clamp_run(rr, S);
+      lse_s[buf][tid] = FOLD ? -lr * over : -lr;
+      dl_s[buf][tid] = -dr;
+      lo_s[buf][tid] = r.x;
+      wd_s[buf][tid] = r.y - r.x;
     }
   };
   if (steps > 0) {
-    issue(h0, qfirst, 0);
+    issue(h0, qfirst, std::integral_constant<int, 0>{});
     stats(0);
   }
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   int j = 0, u = 0;  // head of the part, step of the head
-#pragma unroll 1
-  for (int n = 0; n < steps; ++n) {
-    const int buf = n & 1, q0 = qfirst + u * QT;
-    const float slope2 = (MODE & BIAS) ? a.slopes[h0 + j] * LOG2E : 0.0f;
+  auto step = [&](int n, auto which) {
+    constexpr int buf = decltype(which)::value;
+    const int q0 = qfirst + u * QT;
+    const float slope2 = (MODE & BIAS) ? scalar_load(a.slopes + h0 + j) * LOG2E : 0.0f;
     if (++u == nq) {
       u = 0;
       ++j;
     }
-    if (n + 1 < steps) issue(h0 + j, qfirst + u * QT, buf ^ 1);
-    const uint16_t* qs = qg + buf * (LQ + LG);
-    const uint16_t* gs = qs + LQ;
+    if (n + 1 < steps) issue(h0 + j, qfirst + u * QT, std::integral_constant<int, buf ^ 1>{});
+    const uint16_t* qs = buf ? q_b : q_a;
+    const uint16_t* gs = buf ? g_b : g_a;
 #pragma unroll
     for (int hq = 0; hq < QH; ++hq) {
       const int qh = NW == 8 ? qh0 : hq;
       const int qw0 = q0 + qh * 32;  // this wave's queries
-      const int4 x = qw0 < S ? uniform(blk[qw0 >> 5]) : make_int4(INT_MAX, INT_MAX, 0, 0);
+      const int4 x = qw0 < S ? extremes(blk + (qw0 >> 5)) : make_int4(INT_MAX, INT_MAX, 0, 0);
       if (kw0 < x.w && kw0 + 32 > x.x) {  // some query sees some key
         const bool edge = kw0 < x.y || kw0 + 32 > x.z;
         const float far0 = (float)(qw0 + 4 * g - mykey);
-        const uint16_t *qt = qs + qh * 32 * DQ, *gt = gs + qh * 32 * DV;  // the wave's rows
+        // this wave's rows of the tiles, through its lane addresses
+        const uint32_t q_row = lrq + qh * 32 * DQ * 2, g_row = lrv + qh * 32 * DV * 2;
+        const uint32_t q_tr = ltq + qh * 32 * DQ * 2, g_tr = ltv + qh * 32 * DV * 2;
+        const uint32_t k_row = lrq + kq * 32 * DQ * 2, v_row = lrv + kq * 32 * DV * 2;
+        const int r0 = qh * 32 + g * 4;
         f32x16 sacc, pacc;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) { sacc[e] = 0.0f; pacc[e] = 0.0f; }
+        for (int v4 = 0; v4 < 4; ++v4) {
+          const float4 l = lds4(&lse_s[buf][r0 + 8 * v4]);
+          const float4 d = lds4(&dl_s[buf][r0 + 8 * v4]);
+          const float lv[4] = {l.x, l.y, l.z, l.w}, dv4[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sacc[4 * v4 + e] = FOLD ? lv[e] : 0.0f;
+            pacc[4 * v4 + e] = dv4[e];
+          }
+        }
 #pragma unroll
         for (int s = 0; s < DSQ; ++s) {
           sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              read_row<DQ>(qt, lrq, 0, s),
-              KREG ? kfr[KREG ? s : 0] : read_row<DQ>(Ks + kq * 32 * DQ, lrq, 0, s), sacc, 0, 0, 0);
+              read_row<DQ>(qs, q_row, 0, s),
+              KREG ? kfr[KREG ? s : 0] : read_row<DQ>(Ks, k_row, 0, s), sacc, 0, 0, 0);
           if (s < DSV)
             pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                read_row<DV>(gt, lrv, 0, s),
-                KREG ? vfr[KREG && s < DSV ? s : 0] : read_row<DV>(Vs + kq * 32 * DV, lrv, 0, s),
-                pacc, 0, 0, 0);
+                read_row<DV>(gs, g_row, 0, s),
+                KREG ? vfr[KREG && s < DSV ? s : 0] : read_row<DV>(Vs, v_row, 0, s), pacc, 0, 0, 0);
         }
+        fed<8 + (KREG ? 1 : 2) * (DSQ + DSV), DSQ + DSV, 8 + (KREG ? 4 : 6), KREG ? 1 : 2>();
         bf16x8 pf[2], dsf[2], dsl[2];
-        const int r0 = qh * 32 + g * 4;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           float p8[8], d8[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int vv = 8 * hh + e, ro = (vv >> 2) * 8 + (vv & 3);
-            const float l = lse_s[buf][r0 + ro], dl = dl_s[buf][r0 + ro];
-            if constexpr (MODE != 0) {
+            if constexpr (FOLD) {
+              float y = sacc[vv] * a.sl2;
+              if constexpr ((MODE & BIAS) != 0) y = __builtin_fmaf(-slope2, fabsf(far0 + (float)ro), y);
+              p8[e] = __builtin_amdgcn_exp2f(y);
+              d8[e] = p8[e] * pacc[vv];
+            } else {
               float grad;
               const float y = score<MODE>(a, slope2, sacc[vv], fabsf(far0 + (float)ro), grad);
-              p8[e] = __builtin_amdgcn_exp2f(y - l);
-              d8[e] = p8[e] * (pacc[vv] - dl) * grad;
-            } else {
-              p8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[vv], a.sl2, -l));
-              d8[e] = p8[e] * (pacc[vv] - dl);
+              p8[e] = __builtin_amdgcn_exp2f(y + lds1(&lse_s[buf][r0 + ro]));
+              d8[e] = p8[e] * pacc[vv] * grad;
             }
           }
           if (edge) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int vv = 8 * hh + e, r = r0 + (vv >> 2) * 8 + (vv & 3);
-              const bool keep = (unsigned)(mykey - lo_s[buf][r]) < (unsigned)wd_s[buf][r];
+              const int width = lds1(&wd_s[buf][r]);
+              const bool keep = (unsigned)(mykey - lds1(&lo_s[buf][r])) < (unsigned)width;
               p8[e] = keep ? p8[e] : 0.0f;
-              d8[e] = keep && wd_s[buf][r] > 1 ? d8[e] : 0.0f;
+              d8[e] = keep && width > 1 ? d8[e] : 0.0f;
             }
           }
           pf[hh] = pack8(p8);
           split8(d8, dsf[hh], dsl[hh]);
         }
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
+        for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
-          for (int db = 0; db < DBQ; ++db) {
-            if (db < DBV)
-              dvacc[db < DBV ? db : 0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  read_tr<DV>(gt, ltv, 16 * hh, db), pf[hh], dvacc[db < DBV ? db : 0], 0, 0, 0);
-            const bf16x8 qtr = read_tr<DQ>(qt, ltq, 16 * hh, db);
-            dkacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtr, dsf[hh], dkacc[db], 0, 0, 0);
-            dkacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtr, dsl[hh], dkacc[db], 0, 0, 0);
+          for (int db = 0; db < DBV; ++db)
+            dvacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_tr<DV>(gs, g_tr, 16 * hh, db),
+                                                                pf[hh], dvacc[db], 0, 0, 0);
+#pragma unroll
+          for (int db = 0; db < DBQ; db += 2) {
+            bf16x8 qtr[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qtr[e] = read_tr<DQ>(qs, q_tr, 16 * hh, db + e);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              dkacc[db + e] =
+                  __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtr[e], dsf[hh], dkacc[db + e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              dkacc[db + e] =
+                  __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtr[e], dsl[hh], dkacc[db + e], 0, 0, 0);
           }
+        }
+        fed<4 * (DBV + DBQ), 2 * DBV + 4 * DBQ, 6, 2>();
       }
     }
     if (n + 1 < steps) stats(buf ^ 1);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
+  };
+#pragma unroll 1
+  for (int n = 0; n < steps; n += 2) {
+    step(n, std::integral_constant<int, 0>{});
+    if (n + 1 < steps) step(n + 1, std::integral_constant<int, 1>{});
   }
   // 8 waves: query half 1 parks its sums in LDS, half 0 adds them; dV first, then dK
   float* red = (float*)lds;
@@ -1114,7 +1226,6 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
       __builtin_amdgcn_wave_barrier();
       store_rows<DQ>(dkacc, a.scale, true, os, lane, S - kw0, dk + (krow + kw0) * DQ, DQ);
     } else {
-      static_assert(32 * (DQ + 4) * 2 <= dkdv_lds<DQ, DV>() / 2, "fp32 staging of two waves fits");
       constexpr bool whole = 32 * (DQ + 4) * 2 <= dkdv_lds<DQ, DV>() / 4;
       if constexpr (whole) {
         store_rows_f32<DV>(dvacc, 1.0f, (float*)os, lane, S - kw0, dv_part + (prow + kw0) * DV);
