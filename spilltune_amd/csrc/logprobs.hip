@@ -35,6 +35,7 @@
 namespace {
 
 constexpr int NT = 256;
+constexpr int VT = 256;  // vocabulary columns of a tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Transform {
@@ -85,7 +86,7 @@ struct Head {
   const uint16_t *hidden, *head;
   const int64_t* tokens;
   int64_t ldh, ldw, rows, V;
-  int H, vt, vtiles, rtiles;  // vt: vocabulary columns of a tile
+  int H, vtiles, rtiles;
   Transform tf;
 };
 
@@ -214,22 +215,29 @@ __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_tiles(Head h, flo
   }
 }
 
-// the greater value, the lower index among equals, over the wave
-__device__ __forceinline__ void wave_best(float& v, int& i) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    const float w = __shfl_xor(v, d);
-    const int k = __shfl_xor(i, d);
-    if (w > v || (w == v && k < i)) {
-      v = w;
-      i = k;
-    }
-  }
+// Maximum over the wave without LDS: within rows of 16 lanes, then across them;
+// the last lane holds it.  (No NaN comes here.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_from(float x) {
+  const int v = __float_as_int(x);
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(v, v, CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_from<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8
+  x = max_from<0x112, 0xf>(x);
+  x = max_from<0x114, 0xf>(x);
+  x = max_from<0x118, 0xf>(x);
+  x = max_from<0x142, 0xa>(x);  // row_bcast:15, 31
+  x = max_from<0x143, 0xc>(x);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+// the first lane that holds the greatest value
+__device__ __forceinline__ int first_of(float x, float most) {
+  return __ffsll((unsigned long long)__ballot(x == most)) - 1;
 }
 
 // One wave a row: joins the tiles, then picks `top` alternatives one by one
 // from the tile with the greatest value left.
-template <int VT>
 __global__ __launch_bounds__(NT) void lp_join(Head h, int64_t ignore, const float4* __restrict__ part,
                                               const float* __restrict__ xy,
                                               const float* __restrict__ logits, int64_t ldl, int top,
@@ -258,24 +266,30 @@ __global__ __launch_bounds__(NT) void lp_join(Head h, int64_t ignore, const floa
     entropy[row] = logs - a.u / (1.0f + a.rest);
     lse[row] = a.m + logs;
   }
+  // a lane's tiles are neighbours: the first lane with a maximum has the lowest
+  // index, of tiles as of columns
+  const int per = (h.vtiles + 63) / 64, t0 = lane * per, t1 = min(t0 + per, h.vtiles);
+  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_wave_barrier();
   float lv = INFINITY;  // the last pick: what is left comes after it
   int li = -1;
   for (int k = 0; k < top; ++k) {
     float bv = -INFINITY;
-    int bt = INT_MAX;
-    for (int t = lane; t < h.vtiles; t += 64)
+    int bt = 0;
+    for (int t = t0; t < t1; ++t)
       if (tm[t] > bv) {
         bv = tm[t];
         bt = t;
       }
-    wave_best(bv, bt);
-    if (!(bv > -INFINITY)) {  // nothing left that is a number
+    const float best = wave_max(bv);
+    if (!(best > -INFINITY)) {  // nothing left that is a number
       if (lane == 0) {
         top_lp[row * top + k] = nan;
         top_idx[row * top + k] = -1;
       }
       continue;
     }
+    bt = __builtin_amdgcn_readlane(bt, first_of(bv, best));
     constexpr int PER = VT / 64;
     const int c0 = bt * VT + lane * PER;
     float f[PER];
@@ -289,26 +303,24 @@ __global__ __launch_bounds__(NT) void lp_join(Head h, int64_t ignore, const floa
         if (c0 + e < h.V && (x[e] < lv || (x[e] == lv && c0 + e > li))) f[e] = x[e];
     }
     float v = -INFINITY;
-    int i = INT_MAX;
+    int i = 0;
 #pragma unroll
     for (int e = 0; e < PER; ++e)
       if (f[e] > v) {
         v = f[e];
         i = c0 + e;
       }
-    wave_best(v, i);
-    lv = v;
-    li = i;
+    li = __builtin_amdgcn_readlane(i, first_of(v, best));
+    lv = best;  // the tile's maximum is one of its columns
     float next = -INFINITY;
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-      if (c0 + e != i) next = fmaxf(next, f[e]);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) next = fmaxf(next, __shfl_xor(next, d));
+      if (c0 + e != li) next = fmaxf(next, f[e]);
+    next = wave_max(next);
     if (lane == 0) {
       tm[bt] = next;
-      top_lp[row * top + k] = (value(h.tf, v) - a.m) - logs;
-      top_idx[row * top + k] = i;
+      top_lp[row * top + k] = (value(h.tf, lv) - a.m) - logs;
+      top_idx[row * top + k] = li;
     }
     __builtin_amdgcn_s_waitcnt(0);
     __builtin_amdgcn_wave_barrier();
@@ -525,16 +537,13 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // Row tile of the vocabulary GEMM: cost of a k-step of its 256-column tile
 // relative to 256 rows (a 256x128 tile takes 0.57 of it; a 256x64 one is bound
-// by the head's rows, 0.4).  64 rows whose 256-column tiles leave CUs idle take
-// 128 columns and a deeper ring (col_tile).
+// by the head's rows, 0.4). 
+// (64 rows with 128 columns and a deeper ring, so that a vocabulary of 32000
+// fills the CUs, took as long: 20.5 against 20.4 us for 5 x 1024.)
 int row_tile(int64_t rows) {
   const double c256 = (double)st::cdiv(rows, 256), c128 = 0.57 * (double)st::cdiv(rows, 128),
                c64 = 0.4 * (double)st::cdiv(rows, 64);
   return c64 <= c128 && c64 <= c256 ? 64 : c128 <= c256 ? 128 : 256;
-}
-
-int col_tile(int64_t rows, int64_t V) {
-  return rows <= 64 && st::cdiv(V, 256) < 256 ? 128 : 256;
 }
 
 // Tile and split of dl head: rounds of 256 workgroups, each a split's k-steps
@@ -577,7 +586,7 @@ struct Space {
 Space fwd_space(int64_t rows, int64_t V, int64_t top, bool kept) {
   Space s{};
   s.part = 0;
-  s.xy = up(rows * st::cdiv(V, col_tile(rows, V)) * 16, 256);
+  s.xy = up(rows * st::cdiv(V, VT) * 16, 256);
   s.logits = s.xy + up(rows * 4, 256);
   s.ldl = up(V, 4);
   s.bytes = s.logits + (top > 0 && !kept ? rows * s.ldl * 4 : 0) + 256;
@@ -616,8 +625,7 @@ int check(const char* name, Head& h, const uint16_t* hidden, int64_t rows, int64
   h.hidden = hidden; h.head = head; h.tokens = tokens;
   h.ldh = ldh; h.ldw = ldw; h.rows = rows; h.V = V;
   h.H = (int)H;
-  h.vt = col_tile(rows, V);
-  h.vtiles = (int)st::cdiv(V, h.vt);
+  h.vtiles = (int)st::cdiv(V, VT);
   h.tf = {cap, cap > 0 ? 1.0f / cap : 0.0f, 1.0f / temperature};
   return ST_OK;
 }
@@ -632,8 +640,7 @@ int by_rows(Head& h, F&& fn) {
   const dim3 grid((unsigned)tiles);
   if (bn == 256) fn(st::DmaLoop256<false, false>{}, grid);
   else if (bn == 128) fn(st::DmaLoop64<false, false, 4, 2, 3>{}, grid);
-  else if (h.vt == 256) fn(st::DmaLoop64<false, false, 4, 1, 4>{}, grid);
-  else fn(st::DmaLoop64<false, false, 2, 1, 6>{}, grid);
+  else fn(st::DmaLoop64<false, false, 4, 1, 4>{}, grid);
   return ST_OK;
 }
 
@@ -673,12 +680,8 @@ extern "C" int st_token_logprobs_fwd(const uint16_t* hidden, int64_t rows, int64
   if (int rc = st::check_launch(name)) return rc;
   const dim3 grid((unsigned)st::cdiv(rows, NT / 64));
   const size_t lds = top ? (NT / 64) * h.vtiles * 4 : 0;
-  auto join = [&](auto kernel) {
-    kernel<<<grid, NT, lds, s>>>(h, ignore_index, part, xy, logits, sp.ldl, (int)top, logprobs, entropy,
-                                 lse, top_logprobs, top_tokens);
-  };
-  if (h.vt == 256) join(lp_join<256>);
-  else join(lp_join<128>);
+  lp_join<<<grid, NT, lds, s>>>(h, ignore_index, part, xy, logits, sp.ldl, (int)top, logprobs, entropy,
+                                lse, top_logprobs, top_tokens);
   return st::check_launch("lp_join");
 }
 
