@@ -780,41 +780,52 @@ LOGPROB_SCRATCH = 2 << 30  # bytes of scratch a token_logprobs call aims to stay
 LOGPROB_KEEP = 2 << 30
 
 
+def _row_chunks(rows, per):
+    """Row ranges whose scratch of ``per`` bytes a row stays within
+    LOGPROB_SCRATCH (256 rows at least)."""
+    step = max(256, LOGPROB_SCRATCH // per // 256 * 256)
+    return [(r, min(r + step, rows)) for r in range(0, rows, step)]
+
+
+def _row_ptr(t, row):
+    """Address of ``t[row]`` without a view of it; None for None."""
+    return None if t is None else t.data_ptr() + row * t.stride(0) * t.element_size()
+
+
+def _logprobs(hidden, head, tokens, ignore_index, temperature, cap, top, keep):
+    """(logprobs, entropy, lse, top logprobs, top tokens, logits or None): the
+    logits where ``keep`` asks for them and LOGPROB_KEEP and the memory allow."""
+    rows, H = hidden.shape
+    V, dev = head.shape[0], hidden.device
+    ldw, ldl = head.stride(0), (V + 3) // 4 * 4
+    lp, ent, lse = (torch.empty(rows, dtype=_F32, device=dev) for _ in range(3))
+    top_lp = torch.empty((rows, top), dtype=_F32, device=dev)
+    top_tok = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    logits = None
+    if keep and rows and rows * ldl * 4 <= LOGPROB_KEEP:
+        try:
+            logits = torch.empty((rows, ldl), dtype=_F32, device=dev)
+        except torch.OutOfMemoryError:
+            pass
+    kept = int(logits is not None)
+    with _lib.on_device(dev):
+        for a, z in _row_chunks(rows, 4 * V if top and not kept else V // 8 + 20):
+            nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, ldw, top, kept, 0)
+            ws = _scratch(dev, nbytes)
+            _lib.call("st_token_logprobs_fwd", _row_ptr(hidden, a), z - a, H, hidden.stride(0),
+                      _lib.ptr(head), V, ldw, _row_ptr(tokens, a), ignore_index, temperature, cap,
+                      top, _row_ptr(lp, a), _row_ptr(ent, a), _row_ptr(lse, a), _row_ptr(top_lp, a),
+                      _row_ptr(top_tok, a), _row_ptr(logits, a), _lib.ptr(ws), nbytes,
+                      _lib.stream_handle(dev))
+    return lp, ent, lse, top_lp, top_tok, logits
+
+
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def _row_chunks(rows, per):
-        """Row ranges whose scratch of ``per`` bytes a row stays within
-        LOGPROB_SCRATCH (256 rows at least)."""
-        step = max(256, LOGPROB_SCRATCH // per // 256 * 256)
-        return [(r, min(r + step, rows)) for r in range(0, rows, step)]
-
-    @staticmethod
-    def forward(ctx, hidden, head, tokens, ignore_index, temperature, cap, top, grad):
-        rows, H = hidden.shape
-        V, dev = head.shape[0], hidden.device
-        ldw, ldl = head.stride(0), (V + 3) // 4 * 4
-        lp, ent, lse = (torch.empty(rows, dtype=_F32, device=dev) for _ in range(3))
-        top_lp = torch.empty((rows, top), dtype=_F32, device=dev)
-        top_tok = torch.empty((rows, top), dtype=torch.int64, device=dev)
-        logits = None
-        if grad and rows and rows * ldl * 4 <= LOGPROB_KEEP:
-            try:
-                logits = torch.empty((rows, ldl), dtype=_F32, device=dev)
-            except torch.OutOfMemoryError:
-                pass
-        kept = int(logits is not None)
-        with _lib.on_device(dev):
-            for a, z in _TokenLogProbs._row_chunks(rows, 4 * V if top and not kept else V // 8 + 20):
-                nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, ldw, top, kept, 0)
-                ws = _scratch(dev, nbytes)
-                _lib.call("st_token_logprobs_fwd", _lib.ptr(hidden[a:z]), z - a, H, hidden.stride(0),
-                          _lib.ptr(head), V, ldw, _lib.ptr(tokens[a:z]), ignore_index, temperature,
-                          cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]), _lib.ptr(lse[a:z]),
-                          _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]),
-                          _lib.ptr(logits[a:z]) if kept else None, _lib.ptr(ws), nbytes,
-                          _lib.stream_handle(dev))
-        if grad:
-            ctx.save_for_backward(hidden, head, tokens, lp, ent, lse, top_lp, top_tok, logits)
+    def forward(ctx, hidden, head, tokens, ignore_index, temperature, cap, top):
+        lp, ent, lse, top_lp, top_tok, logits = _logprobs(hidden, head, tokens, ignore_index,
+                                                          temperature, cap, top, True)
+        ctx.save_for_backward(hidden, head, tokens, lp, ent, lse, top_lp, top_tok, logits)
         ctx.meta = (ignore_index, temperature, cap, top)
         ctx.mark_non_differentiable(top_tok)
         ctx.set_materialize_grads(False)
@@ -827,19 +838,18 @@ class _TokenLogProbs(torch.autograd.Function):
         ignore_index, temperature, cap, top = ctx.meta
         (rows, H), V, ldw, dev = hidden.shape, head.shape[0], head.stride(0), hidden.device
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
-        part = lambda g, a, z: None if g is None else _lib.ptr(g[a:z])  # noqa: E731
         dh = torch.empty((rows, H), dtype=_BF16, device=dev)
         with _lib.on_device(dev):
-            for a, z in _TokenLogProbs._row_chunks(rows, 2 * V):
+            for a, z in _row_chunks(rows, 2 * V):
                 nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, ldw, top, 0, 1)
                 ws = _scratch(dev, nbytes)
-                _lib.call("st_token_logprobs_bwd", _lib.ptr(hidden[a:z]), z - a, H, hidden.stride(0),
-                          _lib.ptr(head), V, ldw, _lib.ptr(tokens[a:z]), ignore_index, temperature,
-                          cap, top, _lib.ptr(lp[a:z]), _lib.ptr(ent[a:z]), _lib.ptr(lse[a:z]),
-                          _lib.ptr(top_lp[a:z]), _lib.ptr(top_tok[a:z]), part(logits, a, z),
-                          part(g_lp, a, z), part(g_ent, a, z), part(g_top, a, z), _lib.ptr(dh[a:z]),
-                          H, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
-        return dh, None, None, None, None, None, None, None
+                _lib.call("st_token_logprobs_bwd", _row_ptr(hidden, a), z - a, H, hidden.stride(0),
+                          _lib.ptr(head), V, ldw, _row_ptr(tokens, a), ignore_index, temperature,
+                          cap, top, _row_ptr(lp, a), _row_ptr(ent, a), _row_ptr(lse, a),
+                          _row_ptr(top_lp, a), _row_ptr(top_tok, a), _row_ptr(logits, a),
+                          _row_ptr(g_lp, a), _row_ptr(g_ent, a), _row_ptr(g_top, a),
+                          _row_ptr(dh, a), H, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+        return dh, None, None, None, None, None, None
 
 
 def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ignore_index=-100):
@@ -850,11 +860,12 @@ def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ig
 
     Logits are ``hidden head^T``, with ``cap`` ``cap * tanh(logits / cap)``, over
     ``temperature``, summed in fp32.  They are kept for a backward where they take
-    at most ``LOGPROB_KEEP`` bytes; otherwise it forms them again.  Differentiable in ``hidden`` through all three fp32 results.  A token
-    equal to ``ignore_index`` has log probability 0 and no gradient from it (its
-    entropy and alternatives are those of its hidden state); any other token
-    outside [0, V) gives NaN when it comes on the device and is refused when it
-    comes from the host."""
+    at most ``LOGPROB_KEEP`` bytes; otherwise it forms them again.  Differentiable
+    in ``hidden`` through all three fp32 results.  A token equal to
+    ``ignore_index`` has log probability 0 and no gradient from it (its entropy
+    and alternatives are those of its hidden state); any other token outside
+    [0, V) gives NaN when it comes on the device and is refused when it comes
+    from the host."""
     if hidden.dtype != _BF16 or head.dtype != _BF16 or head.dim() != 2 or hidden.dim() < 1 \
             or hidden.shape[-1] != head.shape[1]:
         raise ValueError("unsupported_capability: token_logprobs expects bf16 hidden [..., H] and "
@@ -881,9 +892,12 @@ def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ig
     if head.device != hidden.device or tokens.device != hidden.device:
         raise ValueError("unsupported_capability: hidden, head and tokens on one device")
     shape = tuple(tokens.shape)
-    lp, ent, top_lp, top_tok = _TokenLogProbs.apply(
-        _operand(hidden.reshape(-1, H)), _operand(head), tokens.reshape(-1).contiguous(),
-        int(ignore_index), temperature, cap, top, torch.is_grad_enabled() and hidden.requires_grad)
+    args = (_operand(hidden.reshape(-1, H)), _operand(head), tokens.reshape(-1).contiguous(),
+            int(ignore_index), temperature, cap, top)
+    if torch.is_grad_enabled() and hidden.requires_grad:
+        lp, ent, top_lp, top_tok = _TokenLogProbs.apply(*args)
+    else:
+        lp, ent, _, top_lp, top_tok, _ = _logprobs(*args, False)
     return TokenLogProbs(lp.view(shape), ent.view(shape), top_lp.view(*shape, top),
                          top_tok.view(*shape, top))
 
