@@ -122,41 +122,48 @@ def document_mask(documents: torch.Tensor, *, bidirectional=None, window=None) -
 
 
 # ----------------------------------------------------------------- attention
+def _span_forward(q, k, v, scale, mask, cap, slopes):
+    """(output, log-sum-exp)"""
+    B, H, S, DQ = q.shape
+    Hkv, DV = k.shape[1], v.shape[-1]
+    dev = q.device
+    out = torch.empty((B, S, H * DV), dtype=_BF16, device=dev)
+    lse = torch.empty((B, H, S), dtype=_F32, device=dev)
+    with _lib.on_device(dev):
+        _lib.call("st_span_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), B, S, H, Hkv, DQ, DV,
+                  scale, cap, _lib.ptr(slopes), mask.key_start.data_ptr(), mask.key_end.data_ptr(),
+                  mask.plan.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.stream_handle(dev))
+    return out, lse
+
+
 class _SpanAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, mask, cap, slopes):
-        B, H, S, DQ = q.shape
-        Hkv, DV = k.shape[1], v.shape[-1]
-        dev = q.device
-        out = torch.empty((B, S, H * DV), dtype=_BF16, device=dev)
-        lse = torch.empty((B, H, S), dtype=_F32, device=dev)
-        operands = (q.data_ptr(), k.data_ptr(), v.data_ptr())
-        shape = (B, S, H, Hkv, DQ, DV)
-        mode = (scale, cap, _lib.ptr(slopes), mask.key_start.data_ptr(), mask.key_end.data_ptr(),
-                mask.plan.data_ptr())
-        with _lib.on_device(dev):
-            _lib.call("st_span_attn_fwd", *operands, *shape, *mode, out.data_ptr(), lse.data_ptr(),
-                      _lib.stream_handle(dev))
+        out, lse = _span_forward(q, k, v, scale, mask, cap, slopes)
         ctx.save_for_backward(q, k, v, out, lse, slopes)
-        # the backward's arguments as far as they are known (the tensors above and
-        # the mask keep their memory): it runs in a thread that is woken for it
-        ctx.args, ctx.shape, ctx.keep = (operands, mode), shape, mask
+        ctx.meta = (scale, mask, cap)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _once()
-        q, k, v, out, lse, _ = ctx.saved_tensors
-        operands, mode = ctx.args
+        # addresses come from the saved tensors as they are now: a hook may have
+        # moved them
+        q, k, v, out, lse, slopes = ctx.saved_tensors
+        scale, mask, cap = ctx.meta
+        B, H, S, DQ = q.shape
+        shape = (B, S, H, k.shape[1], DQ, v.shape[3])
         dev = dout.device
         dout = _operand(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         with _lib.on_device(dev):
-            nbytes = _lib.query("st_span_attn_workspace_bytes", *ctx.shape)
+            nbytes = _lib.query("st_span_attn_workspace_bytes", *shape)
             ws = _scratch(dev, nbytes)
-            _lib.call("st_span_attn_bwd", *operands, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                      *ctx.shape, *mode, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws),
-                      nbytes, _lib.stream_handle(dev))
+            _lib.call("st_span_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                      lse.data_ptr(), dout.data_ptr(), *shape, scale, cap, _lib.ptr(slopes),
+                      mask.key_start.data_ptr(), mask.key_end.data_ptr(), mask.plan.data_ptr(),
+                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws), nbytes,
+                      _lib.stream_handle(dev))
         return dq, dk, dv, None, None, None, None
 
 
@@ -189,7 +196,10 @@ def span_attention(q, k, v, scale, mask: SpanMask, *, cap=None, slopes=None):
         slopes = slopes.contiguous()
     if not q.is_cuda:
         raise ValueError("unsupported_capability: span_attention runs on the GPU")
-    return _SpanAttention.apply(_operand(q), _operand(k), _operand(v), scale, mask, cap, slopes)
+    args = (_operand(q), _operand(k), _operand(v), scale, mask, cap, slopes)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _SpanAttention.apply(*args)
+    return _span_forward(*args)[0]
 
 
 # ----------------------------------------------------------------- rotation
@@ -277,42 +287,55 @@ class Rotary:
         return self.inv_freq.device
 
 
+def _turn(positions, rotary, heads, kv_heads, wq, wk):
+    """The arguments that both directions of the rotation share."""
+    return (positions.data_ptr(), int(positions.dtype == torch.int64), rotary.inv_freq.data_ptr(),
+            rotary.amplitude, *positions.shape, heads, kv_heads, rotary.head_dim, rotary.rotary_dim,
+            int(rotary.interleaved), _lib.ptr(wq), _lib.ptr(wk))
+
+
+def _rope_forward(y, positions, rotary, heads, kv_heads, wq, wk, eps):
+    """(q, k, v, reciprocal norms or None)"""
+    B, S = positions.shape
+    D, dev = rotary.head_dim, y.device
+    q = torch.empty((B, heads, S, D), dtype=_BF16, device=dev)
+    k = torch.empty((B, kv_heads, S, D), dtype=_BF16, device=dev)
+    v = torch.empty_like(k)
+    rstd = None if wq is None else torch.empty((B * S, heads + kv_heads), dtype=_F32, device=dev)
+    with _lib.on_device(dev):
+        _lib.call("st_rope_pos_fwd", y.data_ptr(), y.stride(0),
+                  *_turn(positions, rotary, heads, kv_heads, wq, wk), eps, q.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), _lib.ptr(rstd), _lib.stream_handle(dev))
+    return q, k, v, rstd
+
+
 class _RopePositions(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, positions, rotary, heads, kv_heads, wq, wk, eps):
-        B, S = positions.shape
-        D, dev = rotary.head_dim, y.device
-        q = torch.empty((B, heads, S, D), dtype=_BF16, device=dev)
-        k = torch.empty((B, kv_heads, S, D), dtype=_BF16, device=dev)
-        v = torch.empty_like(k)
-        rstd = None if wq is None else torch.empty((B * S, heads + kv_heads), dtype=_F32, device=dev)
-        rows = (y.data_ptr(), y.stride(0))
-        turn = (positions.data_ptr(), int(positions.dtype == torch.int64), rotary.inv_freq.data_ptr(),
-                rotary.amplitude, B, S, heads, kv_heads, D, rotary.rotary_dim,
-                int(rotary.interleaved), _lib.ptr(wq), _lib.ptr(wk))
-        with _lib.on_device(dev):
-            _lib.call("st_rope_pos_fwd", *rows, *turn, eps, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                      _lib.ptr(rstd), _lib.stream_handle(dev))
+        q, k, v, rstd = _rope_forward(y, positions, rotary, heads, kv_heads, wq, wk, eps)
         if wq is None:  # the rotation's gradient does not read its input
             ctx.save_for_backward(positions)
         else:
-            ctx.save_for_backward(positions, y, wq, wk)
-        # the backward's arguments but for the gradients, and what they point to
-        ctx.args = (*rows, *turn, _lib.ptr(rstd))
-        ctx.shape, ctx.keep = (tuple(y.shape), tuple(q.shape), tuple(k.shape)), (rotary.inv_freq, rstd)
+            ctx.save_for_backward(positions, y, wq, wk, rstd)
+        ctx.meta = (rotary, heads, kv_heads, tuple(y.shape))
         ctx.set_materialize_grads(False)
         return q, k, v
 
     @staticmethod
     def backward(ctx, dq, dk, dv):
         _once()
-        dev = ctx.saved_tensors[0].device
-        shape, qs, ks = ctx.shape
+        # addresses come from the saved tensors as they are now: a hook may have
+        # moved them
+        positions, y, wq, wk, rstd = (*ctx.saved_tensors, None, None, None, None)[:5]
+        rotary, heads, kv_heads, shape = ctx.meta
+        (B, S), D, dev = positions.shape, rotary.head_dim, positions.device
         dy = torch.empty(shape, dtype=_BF16, device=dev)
-        dq, dk, dv = (torch.zeros(s, dtype=_BF16, device=dev) if g is None else _operand(g)
-                      for g, s in ((dq, qs), (dk, ks), (dv, ks)))
+        dq, dk, dv = (torch.zeros((B, n, S, D), dtype=_BF16, device=dev) if g is None else _operand(g)
+                      for g, n in ((dq, heads), (dk, kv_heads), (dv, kv_heads)))
         with _lib.on_device(dev):
-            _lib.call("st_rope_pos_bwd", dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ctx.args,
+            _lib.call("st_rope_pos_bwd", dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(y),
+                      shape[1] if y is None else y.stride(0),
+                      *_turn(positions, rotary, heads, kv_heads, wq, wk), _lib.ptr(rstd),
                       dy.data_ptr(), shape[1], _lib.stream_handle(dev))
         return dy, None, None, None, None, None, None, None
 
@@ -344,8 +367,10 @@ def rope_positions(y, positions, rotary: Rotary, heads: int, kv_heads: int, *, n
         raise ValueError("unsupported_capability: rope_positions runs on the GPU")
     if y.stride(1) != 1 or y.stride(0) % 8 or y.stride(0) < y.shape[1] or y.data_ptr() % 16:
         y = y.clone(memory_format=torch.contiguous_format)
-    return _RopePositions.apply(y, positions.contiguous(), rotary, int(heads), int(kv_heads), wq, wk,
-                                float(eps))
+    args = (y, positions.contiguous(), rotary, int(heads), int(kv_heads), wq, wk, float(eps))
+    if torch.is_grad_enabled() and y.requires_grad:
+        return _RopePositions.apply(*args)
+    return _rope_forward(*args)[:3]
 
 
 # ----------------------------------------------------------------- a model's packed rows

@@ -397,3 +397,62 @@ def test_rope_graph_and_stream():
         graph.replay()
         for a, b in zip(held, eager):
             assert torch.equal(a, b)
+
+
+def _moved(f, inputs):
+    """Gradients of ``f`` over copies of ``inputs`` whose saved tensors are kept
+    on the host and come back elsewhere, the places they had overwritten."""
+    leaves = [t.detach().clone().requires_grad_() for t in inputs]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        out = f(*(t * 1 for t in leaves))
+    junk = [torch.full_like(t, float("nan")) for t in leaves for _ in range(8)]
+    outs = out if isinstance(out, tuple) else (out,)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ups = [torch.randn(o.shape, generator=g, device="cuda").to(o.dtype) for o in outs]
+    grads = torch.autograd.grad(outs, leaves, ups)
+    del junk
+    return grads, ups
+
+
+@pytest.mark.parametrize("kind", ["spans", "turned", "normed"])
+def test_saved_tensors_that_a_hook_moved(kind):
+    g = torch.Generator(device="cuda").manual_seed(11)
+    B, S, H, KV, D = 2, 150, 4, 2, 64
+    documents = torch.zeros(B, S, dtype=torch.int64).cuda()
+    mask = packed.document_mask(documents)
+    if kind == "spans":
+        inputs = [_randn(g, B, h, S, D).to(BF) for h in (H, KV, KV)]
+        slopes = torch.rand(H, generator=g, device="cuda")
+        f = lambda q, k, v: packed.span_attention(q, k, v, 0.125, mask, slopes=slopes)  # noqa: E731
+    else:
+        inputs = [_randn(g, B * S, (H + 2 * KV) * D).to(BF)]
+        norms = (_randn(g, D).to(BF), _randn(g, D).to(BF)) if kind == "normed" else None
+        rotary = packed.Rotary(D, 1e4, device="cuda")
+        f = lambda y: packed.rope_positions(y, mask.positions.clone(), rotary, H, KV,  # noqa: E731
+                                            norms=norms)
+    got, ups = _moved(f, inputs)
+    leaves = [t.detach().clone().requires_grad_() for t in inputs]
+    outs = f(*leaves)
+    want = torch.autograd.grad(outs if isinstance(outs, tuple) else (outs,), leaves, ups)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_checkpointed_attention():
+    """Recomputed operands take the place of the saved ones."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator(device="cuda").manual_seed(12)
+    B, S, H, KV, D = 1, 200, 4, 2, 128
+    mask = packed.document_mask((torch.arange(S)[None] // 70).cuda())
+    rotary = packed.Rotary(D, 1e4, device="cuda")
+    x, up = _randn(g, B * S, (H + 2 * KV) * D).to(BF), _randn(g, B, S, H * D).to(BF)
+
+    def layer(y):
+        q, k, v = packed.rope_positions(y * 1, mask.positions, rotary, H, KV)
+        return packed.span_attention(q, k, v, D ** -0.5, mask)
+
+    grads = []
+    for run in (layer, lambda y: checkpoint(layer, y, use_reentrant=False)):
+        y = x.clone().requires_grad_()
+        grads += torch.autograd.grad(run(y), [y], up)
+    assert torch.equal(*grads)
