@@ -615,7 +615,10 @@ int check(const char* name, Head& h, const uint16_t* hidden, int64_t rows, int64
   ST_CHECK_ARG(std::isfinite(temperature) && temperature > 0 && std::isfinite(cap) && cap >= 0,
                "%s: temperature must be positive, cap 0 (none) or positive", name);
   ST_CHECK_ARG(top >= 0 && top <= V, "%s: top must be within the vocabulary", name);
-  if (top > 64 || V > (1 << 22) || (top && V > (1 << 20)) || H > (1 << 20) || ldw > (1 << 20) ||
+  if (temperature < 1e-30f || temperature > 1e30f || (cap > 0 && (cap < 1e-30f || cap > 1e30f)))
+    return st::fail(ST_EUNSUPPORTED, "%s: temperature %g or cap %g out of range (1e-30 to 1e30)", name,
+                    temperature, cap);
+  if (top > 64 || V > (1 << 21) || (top && V > (1 << 20)) || H > (1 << 20) || ldw > (1 << 20) ||
       ldh > (1 << 20) || rows > (1 << 22))
     return st::fail(ST_EUNSUPPORTED, "%s: rows=%lld H=%lld V=%lld top=%lld is too large (top <= 64)",
                     name, (long long)rows, (long long)H, (long long)V, (long long)top);

@@ -782,8 +782,8 @@ LOGPROB_KEEP = 2 << 30
 
 def _row_chunks(rows, per):
     """Row ranges whose scratch of ``per`` bytes a row stays within
-    LOGPROB_SCRATCH (256 rows at least)."""
-    step = max(256, LOGPROB_SCRATCH // per // 256 * 256)
+    LOGPROB_SCRATCH (256 rows at least, 2^22 at most, a call's limit)."""
+    step = min(max(256, LOGPROB_SCRATCH // per // 256 * 256), 1 << 22)
     return [(r, min(r + step, rows)) for r in range(0, rows, step)]
 
 

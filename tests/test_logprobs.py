@@ -64,3 +64,26 @@ def test_abi_refuses_before_the_device():
     assert q(1000, 64, 5000, 64, 5, 0, 0) - q(1000, 64, 5000, 64, 0, 0, 0) == 1000 * 5000 * 4
     assert q(1000, 64, 5000, 64, 5, 1, 0) == q(1000, 64, 5000, 64, 0, 0, 0)
     assert q(1000, 64, 5000, 64, 0, 0, 1) >= 1000 * 5000 * 2
+
+
+def test_abi_refuses_numbers_and_sizes_out_of_range():
+    """Temperatures and caps whose reciprocals leave fp32; a vocabulary whose
+    gradient rows leave 32-bit offsets."""
+    p = ctypes.c_void_p(16)
+
+    def fwd(V=40, T=1.0, cap=0.0):
+        _lib.call("st_token_logprobs_fwd", p, 4, 16, 16, p, V, 16, p, -100, T, cap, 0, p, p, p, p, p,
+                  None, p, 1 << 40, None)
+    for kw in ({"T": 1e-31}, {"T": 1e31}, {"cap": 1e-31}, {"cap": 1e31}):
+        with pytest.raises(ValueError, match="out of range"):
+            fwd(**kw)
+    with pytest.raises(ValueError, match="too large"):
+        fwd(V=(1 << 21) + 1)
+
+
+def test_row_chunks_stay_within_a_call():
+    for rows, per in ((5, 1 << 40), (1 << 24, 21), (100000, 1 << 20)):
+        chunks = ops._row_chunks(rows, per)
+        assert chunks[0][0] == 0 and chunks[-1][1] == rows
+        assert all(0 < z - a <= 1 << 22 for a, z in chunks)
+        assert all(z == a for (_, z), (a, _) in zip(chunks, chunks[1:]))
