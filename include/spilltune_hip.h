@@ -445,7 +445,8 @@ int st_mla_attn_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v,
  * [B,H,S] base-2 log-sum-exp; (DQ, DV) = (64, 64), (128, 128) or (192, 128).
  * A query with an empty run has out = 0, lse = +inf and a zero dq, whatever its
  * rows hold; infinities and NaN in rows that a query does not see do not reach
- * it.  scale > 0.  Deterministic: no atomics.
+ * it.  scale within 1e-30 .. 1e30, cap up to 1e30 and at least scale / 1e4.
+ * Deterministic: no atomics.
  * `plan`: st_span_plan's tables of the same key_start and key_end, made once
  * per mask and read by every call (st_span_plan_bytes(B, S), 16-byte aligned);
  * it belongs to that mask alone.
@@ -510,7 +511,8 @@ int st_cross_entropy_rows(uint16_t* logits, int64_t rows, int64_t vocab, int64_t
  * V rounded up to 4] that the forward writes l to and the backward reads instead
  * of forming it again (kept = 1 in the query).  dl of each row is rounded to
  * bf16 in the backward's workspace (2 bytes a logit); the forward's holds 4 bytes
- * a logit with top > 0 and no logits, and 16 per 128 or 256 logits.
+ * a logit with top > 0 and no logits, and 16 per 256 logits.  temperature, and a
+ * cap, within 1e-30 .. 1e30; V up to 2^21 (2^20 with top), rows up to 2^22.
  * --------------------------------------------------------------------- */
 int64_t st_token_logprobs_workspace_bytes(int64_t rows, int64_t H, int64_t V, int64_t ldw,
                                           int64_t top, int32_t kept, int32_t backward);

@@ -204,24 +204,10 @@ __device__ __forceinline__ int head_of(int x, int H, int Hkv) {
 
 // MODE: what is done to a score, CAP and BIAS
 constexpr int CAP = 1, BIAS = 2;
-// Base-2 score of a raw product s at distance `far` (>= 0); `grad`: d x / d (scale s).
-template <int MODE>
-__device__ __forceinline__ float score(const Args& a, float slope2, float s, float far, float& grad) {
-  grad = 1.0f;
-  float x = s * a.sl2;
-  if constexpr ((MODE & CAP) != 0) {
-    // tanh(y) = 1 - 2 r, r = 1 / (1 + e^2y); absolute error of a few 2^-24
-    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.cap_in));
-    x = __builtin_fmaf(-2.0f * a.cap_out, r, a.cap_out);
-    grad = 4.0f * r * (1.0f - r);
-  }
-  if constexpr ((MODE & BIAS) != 0) x = __builtin_fmaf(-slope2, far, x);
-  return x;
-}
 // tanh(y) = y + y z P(z), z = y^2, for |y| <= 0.35: P by least squares on
 // Chebyshev points, reweighted to level the relative error (4e-8).  Most capped
 // scores are there, and the polynomial takes half of the time of the exponential
-// and the reciprocal.  Callers choose it for a whole wave (Args::cap_small).
+// and the reciprocal: the forward chooses it alone where a whole wave's are.
 __device__ __forceinline__ float score_small(const Args& a, float s) {
   const float z = s * s;
   float p = __builtin_fmaf(a.cap_p[2], z, a.cap_p[1]);
@@ -229,6 +215,22 @@ __device__ __forceinline__ float score_small(const Args& a, float s) {
   return s * __builtin_fmaf(p, z, a.sl2);
 }
 
+// Base-2 score of a raw product s at distance `far` (>= 0); `grad`: d x / d (scale s).
+template <int MODE>
+__device__ __forceinline__ float score(const Args& a, float slope2, float s, float far, float& grad) {
+  grad = 1.0f;
+  float x = s * a.sl2;
+  if constexpr ((MODE & CAP) != 0) {
+    // tanh(y) = 1 - 2 r, r = 1 / (1 + e^2y); absolute error of a few 2^-24, which a
+    // large cap would multiply: small scores take the polynomial
+    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.cap_in));
+    const float far_out = __builtin_fmaf(-2.0f * a.cap_out, r, a.cap_out);
+    x = fabsf(s) <= a.cap_small ? score_small(a, s) : far_out;
+    grad = 4.0f * r * (1.0f - r);
+  }
+  if constexpr ((MODE & BIAS) != 0) x = __builtin_fmaf(-slope2, far, x);
+  return x;
+}
 // Instruction order of a run of MFMAs fed from LDS: LEAD reads ahead, then PER
 // after each MFMA.  Left alone the compiler reads an operand just before its use
 // and every pair of MFMAs waits for the LDS.
@@ -1327,11 +1329,15 @@ int check_common(const char* name, int64_t B, int64_t S, int64_t H, int64_t Hkv,
                     name, (long long)DQ, (long long)DV);
   ST_CHECK_ARG(std::isfinite(scale) && scale > 0, "%s: scale must be positive and finite", name);
   ST_CHECK_ARG(std::isfinite(cap) && cap >= 0, "%s: cap must be finite, 0 for none", name);
+  // the kernels divide by the scale and form the sixth power of scale / cap
+  if (scale < 1e-30f || scale > 1e30f || (cap > 0 && (cap > 1e30f || scale / cap > 1e4f)))
+    return st::fail(ST_EUNSUPPORTED, "%s: scale %g or cap %g out of range (scale 1e-30 to 1e30, cap up "
+                    "to 1e30 and at least scale / 1e4)", name, scale, cap);
   // tiles by 32-bit ids, one grid of tiles x heads, and 64 token-major rows
   // within a 32-bit byte offset
   const int64_t lim = (int64_t)1 << 31;
-  if (S >= (1 << 30) || H >= (1 << 16) || B >= (1 << 24) || B * st::cdiv(S, 32) * H >= lim ||
-      64 * H * DV * 2 >= lim)
+  if (S >= (1 << 30) || H >= (1 << 16) || B >= (1 << 24) || B * st::cdiv(S, 32) >= lim ||
+      B * st::cdiv(S, 32) * H >= lim || 64 * H * DV * 2 >= lim)
     return st::fail(ST_EUNSUPPORTED, "%s: B=%lld S=%lld H=%lld is too large", name, (long long)B,
                     (long long)S, (long long)H);
   return ST_OK;

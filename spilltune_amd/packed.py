@@ -172,6 +172,7 @@ def span_attention(q, k, v, scale, mask: SpanMask, *, cap=None, slopes=None):
     128/128 or 192/128) -> token-major [B,S,H*DV]: each query over its run of keys
     in ``mask``.  Scores are ``scale * q.k``, with ``cap`` ``cap * tanh(scale * q.k
     / cap)``; ``slopes`` (fp32 [H], constants) subtracts ``slopes[h] * |i - j|``.
+    (``scale`` 1e-30 to 1e30, ``cap`` up to 1e30 and at least ``scale / 1e4``.)
     A query that sees nothing gets zeros and passes no gradient on."""
     if not isinstance(mask, SpanMask):
         raise ValueError("unsupported_capability: span_attention needs a SpanMask")
@@ -360,7 +361,9 @@ def rope_positions(y, positions, rotary: Rotary, heads: int, kv_heads: int, *, n
         raise ValueError("unsupported_capability: y, positions and the Rotary on one device")
     wq = wk = None
     if norms is not None:
-        wq, wk = (_operand(w.detach()) for w in norms)
+        if any(w.requires_grad for w in norms):
+            raise ValueError("unsupported_capability: norm weights are frozen")
+        wq, wk = (_operand(w) for w in norms)
         if any(w.dtype != _BF16 or tuple(w.shape) != (D,) or w.device != y.device for w in (wq, wk)):
             raise ValueError("unsupported_capability: norm weights must be bf16 [head_dim]")
     if not y.is_cuda:

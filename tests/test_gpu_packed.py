@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from spilltune_amd import _lib, ops, packed
-from tests._packed_ref import U, rope_ref, runs_brute, span_ref
+from tests._packed_ref import U, rope_ref, runs_brute, span_ref, span_scores
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -456,3 +456,35 @@ def test_checkpointed_attention():
         y = x.clone().requires_grad_()
         grads += torch.autograd.grad(run(y), [y], up)
     assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128), (192, 128)])
+@pytest.mark.parametrize("cap", [1e3, 1e6, 1e20])
+def test_caps_far_above_the_scores(dims, cap):
+    """As good as no cap: what a tanh near 1 is off by must not be multiplied."""
+    B, S, H = 1, 150, 2
+    mask = packed.document_mask(torch.zeros(B, S, dtype=torch.int32, device="cuda"))
+    _check(*_run(B, S, H, 2, *dims, mask, cap=cap, seed=7))
+
+
+def test_scores_on_both_sides_of_a_cap():
+    """Blocks whose scores lie in the linear part and well beyond the cap."""
+    B, S, H, D, cap, scale = 1, 180, 2, 128, 2.0, 1.5 * 128 ** -0.5
+    mask = packed.document_mask(torch.zeros(B, S, dtype=torch.int32, device="cuda"))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, k, v = (_randn(g, B, H, S, D) for _ in range(3))
+    q[:, :, ::3] *= 3.0
+    k[:, :, 64:] *= 0.05
+    q, k, v, dout = q.to(BF), k.to(BF), v.to(BF), _randn(g, B, S, H * D).to(BF)
+    want, bound = span_ref(q, k, v, scale, mask.key_start, mask.key_end, cap, None, dout)
+    # 1 - tanh^2 is off by up to 2^-21 (four rounded fp32 steps around 1), whatever it is
+    x, _, sees = span_scores(q.double(), k.double(), scale, mask.key_start, mask.key_end, cap, None)
+    p = torch.softmax(torch.where(sees, x, -1e300), -1)
+    do = dout.double().view(B, S, H, D).transpose(1, 2)
+    dp = (do @ v.double().transpose(-1, -2)).abs()
+    err = 2.0 ** -21 * p * (dp + (p * dp).sum(-1, keepdim=True)) * scale
+    bound[1] = bound[1] + err @ k.double().abs()
+    bound[2] = bound[2] + err.transpose(-1, -2) @ q.double().abs()
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = packed.span_attention(*leaves, scale, mask, cap=cap)
+    _check((out, *torch.autograd.grad(out, leaves, dout)), want, bound)

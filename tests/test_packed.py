@@ -245,3 +245,26 @@ def test_engine_refuses():
     assert packed.document_labels(torch.arange(6).view(1, 6),
                                   torch.tensor([[0, 0, 1, 1, -1, -1]])).tolist() \
         == [[-100, 1, -100, 3, -100, -100]]
+
+
+def test_abi_refuses_scales_out_of_range():
+    """Numbers whose reciprocals or powers leave fp32, and row counts whose
+    product leaves 64 bits."""
+    p = ctypes.c_void_p(16)
+
+    def fwd(B=1, S=4, H=2, scale=1.0, cap=0.0):
+        _lib.call("st_span_attn_fwd", p, p, p, B, S, H, 1, 64, 64, scale, cap, None, p, p, p, p, p,
+                  None)
+    for kw in ({"scale": 1e-31}, {"scale": 1e31}, {"cap": 1e31}, {"cap": 9e-5}, {"scale": 1e4, "cap": 0.5}):
+        with pytest.raises(ValueError, match="out of range"):
+            fwd(**kw)
+    with pytest.raises(ValueError, match="too large"):
+        fwd(B=(1 << 24) - 1, S=(1 << 30) - 1, H=(1 << 16) - 1)
+
+
+def test_rope_positions_refuses_norms_that_train():
+    y, w = torch.zeros(2, 4 * 64, dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16)
+    rotary = packed.Rotary(64, 1e4, device="cpu")
+    with pytest.raises(ValueError, match="frozen"):
+        packed.rope_positions(y, torch.zeros(1, 2, dtype=torch.int32), rotary, 2, 1,
+                              norms=(w, w.clone().requires_grad_(True)))
