@@ -15,8 +15,9 @@
 // A workgroup takes one token and makes its table in LDS once for all heads;
 // then each thread turns 8 elements at a time, its pair partners read beside them
 // (from L1: the neighbouring thread's elements).  Four tokens a workgroup, for
-// longer runs of memory in each head's output, took 15.1 us against 11.1 for 2048
-// tokens of 48 heads of 128 and 32.6 against 32.4 for 8192 (202 MB).
+// longer runs of memory in each head's rows, took 15.1 us against 10.7 for 2048
+// tokens of 48 heads of 128, and for 8192 (202 MB; in a trace, cold) 46 against 41
+// forward, 41 against 47 back.
 #include "common.h"
 
 namespace {

@@ -602,7 +602,12 @@ __device__ void redo_dkdv(const Args& a, int b, int hk, int h0, int heads, int j
 // 4 waves of 32 queries over steps of 64 keys from the first key that the tile
 // sees; K and V tiles [key][D] in LDS, two buffers, one barrier a step.  Every
 // MFMA tile is S^T = K Q^T (a lane owns a query column), O^T += V^T P^T with
-// V^T read by the transposing LDS loads.
+// V^T read by the transposing LDS loads.  Two waves a SIMD: one's exponentials run
+// under the other's MFMAs.  Bound by that overlap: the MFMA pipes are busy 38% of
+// the time, the vector units 43%, LDS without conflicts in the loop.  8192 packed
+// tokens (7 documents, 32/8 heads of 128): 88 us, 0.73 PFLOP/s of what the runs
+// need; 16384 tokens, window 4096, capped: 1068 us, 0.90 PFLOP/s; 2048 tokens and
+// 128 heads of 192/128: 98 us, 0.50 PFLOP/s.
 template <int DQ, int DV, int MODE>
 __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__ out,
                                                   float* __restrict__ lse) {
@@ -775,7 +780,10 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
 
 // ---------------------------------------------------------------- backward
 // dQ (and delta) of a 128-query tile: S^T and dP^T = V dO^T as in the forward,
-// dQ^T += K^T dS^T.
+// dQ^T += K^T dS^T.  Bound as the forward (MFMA pipes 43% busy): 176 us in a
+// trace, 0.55 PFLOP/s, at its 8192 packed tokens, 193 us at its heads of 192/128.
+// Unrolled by two steps as the forward is, it spilled (495 us a training pass
+// against 467).
 template <int DQ, int DV, int MODE>
 __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __restrict__ o,
                                                      const uint16_t* __restrict__ dout,
@@ -950,6 +958,10 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
 // The whole group in one workgroup needs no partial sums in memory; a tile with
 // much more work than a CU's share has its group split over several workgroups
 // (parts_of), and span_reduce adds their fp32 sums in order.
+// Bound as the forward for DQ <= 128 (MFMA pipes 43% busy): 226 us in a trace,
+// 0.57 PFLOP/s, at its 8192 packed tokens.  DQ = 192 has one wave a SIMD and one
+// workgroup a CU, so nothing covers a tile's start and end (MFMA pipes 23% busy):
+// 280 us, 0.35 PFLOP/s (both query halves in one run of instructions took as long).
 // A tile stays whole up to a CU's share of all work (256 CUs) or 16 steps (of 2
 // blocks each); a heavier one is split, by a divisor of the group, into parts of
 // at most three quarters of a share.  Training pass in us, against parts of at
