@@ -488,3 +488,76 @@ def test_scores_on_both_sides_of_a_cap():
     leaves = [t.requires_grad_(True) for t in (q, k, v)]
     out = packed.span_attention(*leaves, scale, mask, cap=cap)
     _check((out, *torch.autograd.grad(out, leaves, dout)), want, bound)
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last document of the last heads."""
+    S, H, KV, D, n, scale = 257 * 256, 264, 8, 128, 256, 128 ** -0.5
+    G = H // KV
+    assert S * H * D > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(21)
+    mask = packed.document_mask((torch.arange(S, device="cuda")[None] // n).int())
+    q, k, v, dout = (torch.zeros(s, dtype=BF, device="cuda")
+                     for s in ((1, H, S, D), (1, KV, S, D), (1, KV, S, D), (1, S, H * D)))
+    ends = [q[:, -G:, -n:], k[:, -1:, -n:], v[:, -1:, -n:], dout[:, -n:, -G * D:]]
+    for t in ends:
+        t.copy_(_randn(g, *t.shape))
+    lo, hi = (t[:, -n:] - (S - n) for t in (mask.key_start, mask.key_end))
+    want, bound = span_ref(*(t.contiguous() for t in ends[:3]), scale, lo, hi, None, None,
+                           ends[3].contiguous())
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = packed.span_attention(*leaves, scale, mask)
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    _check((out[:, -n:, -G * D:], dq[:, -G:, -n:], dk[:, -1:, -n:], dv[:, -1:, -n:]), want, bound)
+    # everything else is made of zeros
+    assert not bool(out[:, :-n].any()) and not bool(dq[:, :, :-n].any())
+
+
+def test_rope_offsets_past_32_bits():
+    """The last tokens of more than 2^31 elements, against those tokens alone."""
+    T, H, KV, D, n = 360001, 32, 8, 128, 5
+    W = (H + 2 * KV) * D
+    assert T * W > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(22)
+    rotary = packed.Rotary(D, 1e4, device="cuda")
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")[None]
+    y = torch.zeros(T, W, dtype=BF, device="cuda")
+    y[-n:] = _randn(g, n, W).to(BF)
+    last = y[-n:].clone().requires_grad_(True)
+    outs = packed.rope_positions(last, pos[:, -n:].contiguous(), rotary, H, KV)
+    ups = [_randn(g, *o.shape).to(BF) for o in outs]
+    (want,) = torch.autograd.grad(outs, last, ups)
+    y.requires_grad_(True)
+    got = packed.rope_positions(y, pos, rotary, H, KV)
+    for a, b in zip(got, outs):
+        assert torch.equal(a[:, :, -n:], b)
+    full = [torch.zeros_like(o) for o in got]
+    for f, u in zip(full, ups):
+        f[:, :, -n:] = u
+    (dy,) = torch.autograd.grad(got, y, full)
+    assert torch.equal(dy[-n:], want) and not bool(dy[:-n].any())
+
+
+def test_one_mask_on_two_streams_at_once():
+    """Passes on two streams over one mask, interleaved, against one after the other."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    B, S, H, KV, D = 2, 700, 8, 2, 128
+    mask = packed.document_mask(_documents(random.Random(5), B, S, 20, 300, 7).cuda())
+    sets = [[_randn(g, *s).to(BF) for s in ((B, H, S, D), (B, KV, S, D), (B, KV, S, D), (B, S, H * D))]
+            for _ in range(2)]
+
+    def one(q, k, v, dout):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = packed.span_attention(*leaves, 0.1, mask, cap=5.0)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    want = [one(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                got.append(one(*s))
+    torch.cuda.synchronize()
+    for i, res in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i % 2]))
