@@ -23,8 +23,8 @@
 // Backward: l read back, or formed again by the same GEMM, becomes dl (bf16: a
 // choice, half a step of 2^-8 on values that are then summed over the
 // vocabulary); the given token's and the alternatives' entries, the large ones,
-// are redone by a small kernel from the saved log probabilities, which keeps what
-// their rounding leaves in fp32.  dl head is a GEMM split over the vocabulary so
+// come from the saved log probabilities, and what their rounding leaves is kept in
+// fp32.  dl head is a GEMM split over the vocabulary so
 // that few rows fill the GPU; its fp32 partials are summed in order and the
 // picked entries' remainders times their rows of the head added.
 #include <algorithm>
@@ -359,6 +359,49 @@ __device__ __forceinline__ float dlogit(const Transform& t, float4 c, float l) {
   return c.x == 0.0f && c.y == 0.0f ? 0.0f : d;
 }
 
+// Column of pick k of a row (alternative k, or the given token for k = ntop), -1
+// for none.
+struct Picks {
+  const int64_t* top_idx;
+  const float *top_lp, *logprobs, *lse, *ent;
+};
+__device__ __forceinline__ int64_t column_of(const Head& h, const Upstream& g, int64_t ignore,
+                                             const Picks& p, int64_t row, int k) {
+  if (k < g.ntop) return p.top_idx[row * g.ntop + k];
+  const int64_t y = h.tokens[row];
+  return y != ignore && y >= 0 && y < h.V ? y : -1;
+}
+// dl of pick k, in column c, from the saved log probability; a token picked twice
+// gets one value from both.  Returns whether the entry is to be replaced; `left`:
+// what its rounding leaves, once for each entry.
+__device__ __forceinline__ bool picked(const Head& h, const Upstream& g, int64_t ignore, const Picks& p,
+                                       int64_t row, int k, int64_t c, uint16_t& value, float& left) {
+  left = 0.0f;
+  const int64_t y = column_of(h, g, ignore, p, row, g.ntop);
+  const float lp = k < g.ntop ? p.top_lp[row * g.ntop + k] : p.logprobs[row];
+  const float own_lp = given(h, g, row, ignore);
+  float sum = own_lp, own = c == y ? own_lp : 0.0f;
+  bool again = false;  // the given token among the alternatives
+  for (int j = 0; j < g.ntop; ++j) {
+    const int64_t t = p.top_idx[row * g.ntop + j];
+    const float w = g.top ? g.top[row * g.ntop + j] : 0.0f;
+    if (t >= 0) sum += w;
+    if (t == c) own += w;
+    again |= k == g.ntop && t == c;
+  }
+  const float pr = __builtin_amdgcn_exp2f(lp * LOG2E), ge = g.ent ? g.ent[row] : 0.0f;
+  if (own == 0.0f && sum == 0.0f && ge == 0.0f) return false;  // as the other columns
+  float d = own - pr * __builtin_fmaf(ge, lp + p.ent[row], sum);
+  if (h.tf.cap != 0.0f) {
+    const float t = (lp + p.lse[row]) / h.tf.inv_t * h.tf.inv_cap;  // tanh of the raw logit
+    d *= (1.0f - t) * (1.0f + t);
+  }
+  d *= h.tf.inv_t;
+  value = st::f32_to_bf16(d);
+  if (!again) left = d - st::bf16_to_f32(value);
+  return true;
+}
+
 // dl from logits formed again
 template <class LP>
 __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_dlogits(Head h, Upstream g,
@@ -400,18 +443,17 @@ __global__ __launch_bounds__(LP::NT, LP::MIN_WG_WAVES) void lp_dlogits(Head h, U
     }
   }
 }
-// dl from kept logits: 4 + 2 bytes a logit, bound by HBM (2048 x 151936: 297 us,
+// dl from kept logits, the picked entries in the same pass (by the thread that
+// holds the column): 4 + 2 bytes a logit, bound by HBM (2048 x 151936: 297 us,
 // 6.3 TB/s)
 constexpr int KEPT = 8;  // logits of a thread
-__global__ __launch_bounds__(NT) void lp_dlogits_kept(Head h, Upstream g, int64_t ignore,
-                                                      const int64_t* __restrict__ top_idx,
-                                                      const float* __restrict__ lse,
-                                                      const float* __restrict__ ent,
+__global__ __launch_bounds__(NT) void lp_dlogits_kept(Head h, Upstream g, int64_t ignore, Picks p,
                                                       const float* __restrict__ logits, int64_t ldl,
-                                                      uint16_t* __restrict__ dl, int64_t ldd) {
+                                                      uint16_t* __restrict__ dl, int64_t ldd,
+                                                      float* __restrict__ left) {
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
   if (row >= h.rows) return;
-  const float4 c = upstream(h, g, row, ignore, top_idx, lse, ent);
+  const float4 c = upstream(h, g, row, ignore, p.top_idx, p.lse, p.ent);
   const int64_t c0 = ((int64_t)blockIdx.x * NT + threadIdx.x) * KEPT;
   if (c0 >= ldd) return;
   float l[KEPT], d[KEPT];
@@ -423,19 +465,25 @@ __global__ __launch_bounds__(NT) void lp_dlogits_kept(Head h, Upstream g, int64_
   }
 #pragma unroll
   for (int e = 0; e < KEPT; ++e) d[e] = c0 + e < h.V ? dlogit(h.tf, c, l[e]) : 0.0f;
+  for (int k = 0; k <= g.ntop; ++k) {
+    const int64_t at = column_of(h, g, ignore, p, row, k);
+    if (at < 0 ? c0 != 0 : at < c0 || at >= c0 + KEPT) continue;
+    uint16_t value;
+    float rest = 0.0f;
+    if (at >= 0 && picked(h, g, ignore, p, row, k, at, value, rest)) {
+#pragma unroll
+      for (int e = 0; e < KEPT; ++e)
+        if (at == c0 + e) d[e] = st::bf16_to_f32(value);
+    }
+    left[row * (g.ntop + 1) + k] = rest;
+  }
   *(uint4*)(dl + row * ldd + c0) = make_uint4(st::pack_bf16x2(d[0], d[1]), st::pack_bf16x2(d[2], d[3]),
                                               st::pack_bf16x2(d[4], d[5]), st::pack_bf16x2(d[6], d[7]));
 }
 
-// the picked tokens' entries whole: thread k of a row takes alternative k, or
-// the given token (k = ntop); a token picked twice gets one value from both.
-// left[row][k]: what the entry's rounding leaves, once for each entry.
-__global__ __launch_bounds__(NT) void lp_picked(Head h, Upstream g, int64_t ignore,
-                                                const int64_t* __restrict__ top_idx,
-                                                const float* __restrict__ top_lp,
-                                                const float* __restrict__ logprobs,
-                                                const float* __restrict__ lse,
-                                                const float* __restrict__ ent,
+// the picked tokens' entries whole, over what lp_dlogits wrote: thread k of a row
+// takes pick k.  left[row][k]: see picked
+__global__ __launch_bounds__(NT) void lp_picked(Head h, Upstream g, int64_t ignore, Picks p,
                                                 uint16_t* __restrict__ dl, int64_t ldd,
                                                 float* __restrict__ left) {
   const int64_t n = (int64_t)blockIdx.x * NT + threadIdx.x;
@@ -443,33 +491,11 @@ __global__ __launch_bounds__(NT) void lp_picked(Head h, Upstream g, int64_t igno
   const int64_t row = n / per;
   const int k = (int)(n % per);
   if (row >= h.rows) return;
-  left[n] = 0.0f;
-  const int64_t y = h.tokens[row];
-  const bool has = y != ignore && y >= 0 && y < h.V;
-  const int64_t c = k < g.ntop ? top_idx[row * g.ntop + k] : has ? y : -1;
-  if (c < 0) return;
-  const float lp = k < g.ntop ? top_lp[row * g.ntop + k] : logprobs[row];
-  const float own_lp = given(h, g, row, ignore);
-  float sum = own_lp, own = has && c == y ? own_lp : 0.0f;
-  bool again = false;  // the given token among the alternatives
-  for (int j = 0; j < g.ntop; ++j) {
-    const int64_t t = top_idx[row * g.ntop + j];
-    const float w = g.top ? g.top[row * g.ntop + j] : 0.0f;
-    if (t >= 0) sum += w;
-    if (t == c) own += w;
-    again |= k == g.ntop && t == c;
-  }
-  const float p = __builtin_amdgcn_exp2f(lp * LOG2E), ge = g.ent ? g.ent[row] : 0.0f;
-  if (own == 0.0f && sum == 0.0f && ge == 0.0f) return;  // as the other columns left it
-  float d = own - p * __builtin_fmaf(ge, lp + ent[row], sum);
-  if (h.tf.cap != 0.0f) {
-    const float t = (lp + lse[row]) / h.tf.inv_t * h.tf.inv_cap;  // tanh of the raw logit
-    d *= (1.0f - t) * (1.0f + t);
-  }
-  d *= h.tf.inv_t;
-  const uint16_t b = st::f32_to_bf16(d);
-  dl[row * ldd + c] = b;
-  if (!again) left[n] = d - st::bf16_to_f32(b);
+  const int64_t c = column_of(h, g, ignore, p, row, k);
+  uint16_t value;
+  float rest = 0.0f;
+  if (c >= 0 && picked(h, g, ignore, p, row, k, c, value, rest)) dl[row * ldd + c] = value;
+  left[n] = rest;
 }
 
 // dhidden partials: part[split][row][h] = sum over the split's columns of dl head.
@@ -522,9 +548,13 @@ __global__ __launch_bounds__(NT) void lp_reduce(Head h, const float* __restrict_
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
     const int64_t row = i * 4 / h.H, col = i * 4 % h.H;
     float4 s = make_float4(0, 0, 0, 0);
-    for (int k = 0; k < splits; ++k) {
-      const float4 x = *(const float4*)(part + k * per + i * 4);
-      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    for (int k = 0; k < splits; k += 8) {  // eight reads in flight, added in order
+      float4 x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = *(const float4*)(part + min(k + e, splits - 1) * per + i * 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k + e < splits) { s.x += x[e].x; s.y += x[e].y; s.z += x[e].z; s.w += x[e].w; }
     }
     for (int k = 0; k <= ntop; ++k) {
       const float w = left[row * (ntop + 1) + k];
@@ -724,21 +754,22 @@ extern "C" int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64
   float *left = (float*)(ws + sp.left), *part = (float*)(ws + sp.part);
   hipStream_t s = (hipStream_t)stream;
   const Upstream g{g_logprobs, g_entropy, top ? g_top : nullptr, (int)top};
+  const Picks p{top_tokens, top_logprobs, logprobs, lse, entropy};
   if (logits) {
     const unsigned y = (unsigned)std::min<int64_t>(rows, 32768);
     lp_dlogits_kept<<<dim3((unsigned)st::cdiv(sp.ldd, NT * KEPT), y, (unsigned)st::cdiv(rows, y)), NT, 0,
-                      s>>>(h, g, ignore_index, top_tokens, lse, entropy, logits, up(V, 4), dl, sp.ldd);
-  } else if (int rc = by_rows(h, [&](auto lp, dim3 grid) {
-               using LP = decltype(lp);
-               lp_dlogits<LP><<<grid, LP::NT, 0, s>>>(h, g, ignore_index, top_tokens, lse, entropy, dl,
-                                                     sp.ldd);
-             })) {
-    return rc;
+                      s>>>(h, g, ignore_index, p, logits, up(V, 4), dl, sp.ldd, left);
+    if (int rc = st::check_launch("lp_dlogits_kept")) return rc;
+  } else {
+    if (int rc = by_rows(h, [&](auto lp, dim3 grid) {
+          using LP = decltype(lp);
+          lp_dlogits<LP><<<grid, LP::NT, 0, s>>>(h, g, ignore_index, top_tokens, lse, entropy, dl, sp.ldd);
+        })) return rc;
+    if (int rc = st::check_launch("lp_dlogits")) return rc;
+    lp_picked<<<(unsigned)st::cdiv(rows * (top + 1), NT), NT, 0, s>>>(h, g, ignore_index, p, dl, sp.ldd,
+                                                                     left);
+    if (int rc = st::check_launch("lp_picked")) return rc;
   }
-  if (int rc = st::check_launch(name)) return rc;
-  lp_picked<<<(unsigned)st::cdiv(rows * (top + 1), NT), NT, 0, s>>>(
-      h, g, ignore_index, top_tokens, top_logprobs, logprobs, lse, entropy, dl, sp.ldd, left);
-  if (int rc = st::check_launch("lp_picked")) return rc;
   const Split& k = sp.split;
   const Dgrad d{dl, head, sp.ldd, ldw, rows, V, (int)H, (int)st::cdiv(rows, k.bm),
                 (int)st::cdiv(H, k.bn), k.splits, k.per};

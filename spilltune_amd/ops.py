@@ -788,20 +788,21 @@ def _row_chunks(rows, per):
     return [(r, min(r + step, rows)) for r in range(0, rows, step)]
 
 
-def _row_ptr(t, row):
-    """Address of ``t[row]`` without a view of it; None for None."""
-    return None if t is None else t.data_ptr() + row * t.stride(0) * t.element_size()
+def _row_ptr(t, row, width=1):
+    """Address of row ``row`` of a contiguous ``t`` in rows of ``width``, without
+    a view of it; None for None."""
+    return None if t is None else t.data_ptr() + row * width * t.element_size()
 
 
 def _logprobs(hidden, head, tokens, ignore_index, temperature, cap, top, keep):
     """(logprobs, entropy, lse, top logprobs, top tokens, logits or None): the
     logits where ``keep`` asks for them and LOGPROB_KEEP and the memory allow."""
-    rows, H = hidden.shape
-    V, dev = head.shape[0], hidden.device
-    ldw, ldl = head.stride(0), (V + 3) // 4 * 4
-    lp, ent, lse = (torch.empty(rows, dtype=_F32, device=dev) for _ in range(3))
-    top_lp = torch.empty((rows, top), dtype=_F32, device=dev)
-    top_tok = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    shape, dev = tokens.shape, hidden.device
+    rows, (V, H) = tokens.numel(), head.shape
+    ldl = (V + 3) // 4 * 4
+    lp, ent, lse = (torch.empty(shape, dtype=_F32, device=dev) for _ in range(3))
+    top_lp = torch.empty((*shape, top), dtype=_F32, device=dev)
+    top_tok = torch.empty((*shape, top), dtype=torch.int64, device=dev)
     logits = None
     if keep and rows and rows * ldl * 4 <= LOGPROB_KEEP:
         try:
@@ -811,12 +812,12 @@ def _logprobs(hidden, head, tokens, ignore_index, temperature, cap, top, keep):
     kept = int(logits is not None)
     with _lib.on_device(dev):
         for a, z in _row_chunks(rows, 4 * V if top and not kept else V // 8 + 20):
-            nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, ldw, top, kept, 0)
+            nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, H, top, kept, 0)
             ws = _scratch(dev, nbytes)
-            _lib.call("st_token_logprobs_fwd", _row_ptr(hidden, a), z - a, H, hidden.stride(0),
-                      _lib.ptr(head), V, ldw, _row_ptr(tokens, a), ignore_index, temperature, cap,
-                      top, _row_ptr(lp, a), _row_ptr(ent, a), _row_ptr(lse, a), _row_ptr(top_lp, a),
-                      _row_ptr(top_tok, a), _row_ptr(logits, a), _lib.ptr(ws), nbytes,
+            _lib.call("st_token_logprobs_fwd", _row_ptr(hidden, a, H), z - a, H, H, head.data_ptr(),
+                      V, H, _row_ptr(tokens, a), ignore_index, temperature, cap, top, _row_ptr(lp, a),
+                      _row_ptr(ent, a), _row_ptr(lse, a), _row_ptr(top_lp, a, top),
+                      _row_ptr(top_tok, a, top), _row_ptr(logits, a, ldl), _lib.ptr(ws), nbytes,
                       _lib.stream_handle(dev))
     return lp, ent, lse, top_lp, top_tok, logits
 
@@ -837,19 +838,21 @@ class _TokenLogProbs(torch.autograd.Function):
         _once()
         hidden, head, tokens, lp, ent, lse, top_lp, top_tok, logits = ctx.saved_tensors
         ignore_index, temperature, cap, top = ctx.meta
-        (rows, H), V, ldw, dev = hidden.shape, head.shape[0], head.stride(0), hidden.device
+        rows, (V, H), dev = tokens.numel(), head.shape, hidden.device
+        ldl = (V + 3) // 4 * 4
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
-        dh = torch.empty((rows, H), dtype=_BF16, device=dev)
+        dh = torch.empty(hidden.shape, dtype=_BF16, device=dev)
         with _lib.on_device(dev):
             for a, z in _row_chunks(rows, 2 * V):
-                nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, ldw, top, 0, 1)
+                nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, H, top, 0, 1)
                 ws = _scratch(dev, nbytes)
-                _lib.call("st_token_logprobs_bwd", _row_ptr(hidden, a), z - a, H, hidden.stride(0),
-                          _lib.ptr(head), V, ldw, _row_ptr(tokens, a), ignore_index, temperature,
-                          cap, top, _row_ptr(lp, a), _row_ptr(ent, a), _row_ptr(lse, a),
-                          _row_ptr(top_lp, a), _row_ptr(top_tok, a), _row_ptr(logits, a),
-                          _row_ptr(g_lp, a), _row_ptr(g_ent, a), _row_ptr(g_top, a),
-                          _row_ptr(dh, a), H, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+                _lib.call("st_token_logprobs_bwd", _row_ptr(hidden, a, H), z - a, H, H,
+                          head.data_ptr(), V, H, _row_ptr(tokens, a), ignore_index, temperature, cap,
+                          top, _row_ptr(lp, a), _row_ptr(ent, a), _row_ptr(lse, a),
+                          _row_ptr(top_lp, a, top), _row_ptr(top_tok, a, top),
+                          _row_ptr(logits, a, ldl), _row_ptr(g_lp, a), _row_ptr(g_ent, a),
+                          _row_ptr(g_top, a, top), _row_ptr(dh, a, H), H, _lib.ptr(ws), nbytes,
+                          _lib.stream_handle(dev))
         return dh, None, None, None, None, None, None
 
 
@@ -892,15 +895,12 @@ def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ig
         tokens = tokens.to(hidden.device)
     if head.device != hidden.device or tokens.device != hidden.device:
         raise ValueError("unsupported_capability: hidden, head and tokens on one device")
-    shape = tuple(tokens.shape)
-    args = (_operand(hidden.reshape(-1, H)), _operand(head), tokens.reshape(-1).contiguous(),
-            int(ignore_index), temperature, cap, top)
+    args = (_operand(hidden), _operand(head), tokens.contiguous(), int(ignore_index), temperature, cap,
+            top)
     if torch.is_grad_enabled() and hidden.requires_grad:
-        lp, ent, top_lp, top_tok = _TokenLogProbs.apply(*args)
-    else:
-        lp, ent, _, top_lp, top_tok, _ = _logprobs(*args, False)
-    return TokenLogProbs(lp.view(shape), ent.view(shape), top_lp.view(*shape, top),
-                         top_tok.view(*shape, top))
+        return TokenLogProbs(*_TokenLogProbs.apply(*args))
+    lp, ent, _, top_lp, top_tok, _ = _logprobs(*args, False)
+    return TokenLogProbs(lp, ent, top_lp, top_tok)
 
 
 # ----------------------------------------------------------------- RoPE

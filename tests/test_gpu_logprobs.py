@@ -267,3 +267,24 @@ def test_operands_of_any_layout_streams_and_graphs():
         graph.replay()
         for x, y in zip(held, eager):
             assert torch.equal(x, y)
+
+
+def test_saved_tensors_that_a_hook_moved_and_any_shape():
+    """Saved tensors kept on the host come back elsewhere; one token, no token and
+    rows of tokens."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    w = torch.randn(500, 64, generator=g, device="cuda").bfloat16()
+    for shape in ((), (0,), (2, 3)):
+        h = torch.randn(*shape, 64, generator=g, device="cuda").bfloat16().requires_grad_(True)
+        t = torch.randint(500, shape, generator=g, device="cuda")
+        grads = []
+        for moved in (False, True):
+            pack = (lambda x: x.cpu()) if moved else (lambda x: x)
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda x: x.cuda()):
+                r = ops.token_logprobs(h * 1, w, t, top=3)
+            junk = [torch.full((4, 64), float("nan"), device="cuda") for _ in range(8)]
+            assert r.logprobs.shape == r.entropy.shape == shape
+            assert r.top_logprobs.shape == r.top_tokens.shape == (*shape, 3)
+            grads += torch.autograd.grad(r.logprobs.sum() + r.entropy.sum() + r.top_logprobs.sum(), h)
+            del junk
+        assert grads[0].shape == h.shape and torch.equal(*grads)
