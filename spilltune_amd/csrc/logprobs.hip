@@ -548,14 +548,16 @@ __global__ __launch_bounds__(NT) void lp_reduce(Head h, const float* __restrict_
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
     const int64_t row = i * 4 / h.H, col = i * 4 % h.H;
     float4 s = make_float4(0, 0, 0, 0);
-    for (int k = 0; k < splits; k += 8) {  // eight reads in flight, added in order
+    auto add = [&](const float4& x) { s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w; };
+    int k = 0;
+    for (; k + 8 <= splits; k += 8) {  // eight reads in flight, added in order
       float4 x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = *(const float4*)(part + min(k + e, splits - 1) * per + i * 4);
+      for (int e = 0; e < 8; ++e) x[e] = *(const float4*)(part + (k + e) * per + i * 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (k + e < splits) { s.x += x[e].x; s.y += x[e].y; s.z += x[e].z; s.w += x[e].w; }
+      for (int e = 0; e < 8; ++e) add(x[e]);
     }
+    for (; k < splits; ++k) add(*(const float4*)(part + k * per + i * 4));
     for (int k = 0; k <= ntop; ++k) {
       const float w = left[row * (ntop + 1) + k];
       if (w == 0.0f) continue;
