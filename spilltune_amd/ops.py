@@ -29,6 +29,7 @@ from itertools import accumulate
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .codecs import GROUP, codebook
@@ -220,6 +221,16 @@ def _once() -> None:
     """Refuses a backward that is to be differentiated itself."""
     if torch.is_grad_enabled():
         raise RuntimeError("unsupported_capability: this operator has no second derivative")
+
+
+def _no_tangents(*tensors) -> None:
+    """Refuses dual tensors of forward-mode differentiation: they do not require a
+    gradient, and an operator called without its autograd node would drop their
+    tangents."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("unsupported_capability: this operator has no forward-mode "
+                                  "derivative")
 
 
 def _gemm_scratch(weight: Q4Weight, form: int, M: int, rank: int, cols: int):
@@ -876,6 +887,7 @@ def token_logprobs(hidden, head, tokens, *, top=0, temperature=1.0, cap=None, ig
                          "head [V, H]")
     if head.requires_grad:
         raise ValueError("unsupported_capability: token_logprobs takes a frozen head")
+    _no_tangents(hidden, head)
     V, H = head.shape
     if H % 8 or H == 0 or V == 0:
         raise ValueError("unsupported_capability: token_logprobs needs a hidden size of whole "

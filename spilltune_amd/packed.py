@@ -26,7 +26,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib
-from .ops import _once, _operand, _scratch
+from .ops import _no_tangents, _once, _operand, _scratch
 
 _BF16 = torch.bfloat16
 _F32 = torch.float32
@@ -195,6 +195,7 @@ def span_attention(q, k, v, scale, mask: SpanMask, *, cap=None, slopes=None):
             raise ValueError("unsupported_capability: slopes must be constant fp32 [heads] on the "
                              "attention's device")
         slopes = slopes.contiguous()
+    _no_tangents(q, k, v, slopes)
     if not q.is_cuda:
         raise ValueError("unsupported_capability: span_attention runs on the GPU")
     args = (_operand(q), _operand(k), _operand(v), scale, mask, cap, slopes)
@@ -366,6 +367,7 @@ def rope_positions(y, positions, rotary: Rotary, heads: int, kv_heads: int, *, n
         wq, wk = (_operand(w) for w in norms)
         if any(w.dtype != _BF16 or tuple(w.shape) != (D,) or w.device != y.device for w in (wq, wk)):
             raise ValueError("unsupported_capability: norm weights must be bf16 [head_dim]")
+    _no_tangents(y, wq, wk)
     if not y.is_cuda:
         raise ValueError("unsupported_capability: rope_positions runs on the GPU")
     if y.stride(1) != 1 or y.stride(0) % 8 or y.stride(0) < y.shape[1] or y.data_ptr() % 16:
