@@ -54,13 +54,18 @@ def key_lengths(valid: torch.Tensor, device, what: str = "unsupported_capability
 
 
 def positions_and_masks(valid: torch.Tensor, *, head_dim: int, theta: float, device,
-                        dtype=torch.bfloat16):
+                        dtype=torch.bfloat16, rotary=None):
     """Rotary tables (bf16 cos/sin [B,S,D]) and the causal mask marker
-    (dense.py:232-248), with the valid prefix lengths of right-padded rows."""
+    (dense.py:232-248), with the valid prefix lengths of right-padded rows.  With
+    ``rotary`` (:class:`~spilltune_amd.packed.Rotary`) in the place of ``theta``,
+    :class:`~spilltune_amd.packed.Positions` instead of tables."""
     if valid.dtype != torch.bool or valid.ndim != 2 or valid.shape[1] < 1:
         raise ValueError("unsupported_capability: mask must be 2D bool")
     lengths = key_lengths(valid, device)
     batch, length = valid.shape
+    if rotary is not None:
+        at = torch.arange(length, dtype=torch.int32, device=device).repeat(batch, 1)
+        return packed.Positions(at, rotary), CausalMask(batch, length, lengths)
     positions = torch.arange(length, device=device).expand(batch, -1)
     inv = 1.0 / theta ** (torch.arange(0, head_dim, 2, device=device).float() / head_dim)
     freq = (inv[None, :, None].expand(batch, -1, 1) @ positions[:, None].float()).transpose(1, 2)

@@ -250,14 +250,16 @@ class DenseModel:
                  blocks=None, qk_norm=False, rotary=None):
         """``layers``: per-layer weight dicts, encoded here; or ``blocks``:
         prebuilt BlockPlans (e.g. ``slots.make_archive_block``).  ``rotary``: the
-        :class:`~spilltune_amd.packed.Rotary` of packed rows (default: whole
-        heads, ``theta``, no scaling)."""
+        model's :class:`~spilltune_amd.packed.Rotary`, of plain and of packed rows
+        (default: whole heads, ``theta``, no scaling; plain rows then by bf16
+        tables)."""
         self.device = torch.device(device)
         self.embedding = embedding.to(torch.bfloat16).contiguous()      # stays on the host
         self.norm = norm.to(torch.bfloat16).to(self.device)
         self.head = head.to(torch.bfloat16).to(self.device)
         self.eps, self.theta, self.head_dim = eps, theta, head_dim
         self.rotary = rotary
+        self._packed_rotary = rotary  # without one: made on the first packed rows
         if (layers is None) == (blocks is None):
             raise ValueError("DenseModel needs exactly one of layers / blocks")
         self.blocks = list(blocks) if blocks is not None else [
@@ -269,14 +271,14 @@ class DenseModel:
 
     def positions_and_masks(self, valid):
         rot, mask = positions_and_masks(valid, head_dim=self.head_dim, theta=self.theta,
-                                        device=self.device)
+                                        device=self.device, rotary=self.rotary)
         return rot, {"full_attention": mask}
 
     def packed_positions_and_masks(self, documents, **kw):
         """Positions and masks of packed rows (packed.positions_and_masks)."""
-        if self.rotary is None:
-            self.rotary = packed.Rotary(self.head_dim, self.theta, device=self.device)
-        positions, mask = packed.positions_and_masks(documents, self.rotary, **kw)
+        if self._packed_rotary is None:
+            self._packed_rotary = packed.Rotary(self.head_dim, self.theta, device=self.device)
+        positions, mask = packed.positions_and_masks(documents, self._packed_rotary, **kw)
         return positions, {"full_attention": mask}
 
     def terminal_norm(self, hidden):

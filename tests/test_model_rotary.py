@@ -1,0 +1,69 @@
+"""A model turns plain and packed rows by one rotary embedding."""
+import pytest
+import torch
+
+from spilltune_amd import dense, engine, packed, slots
+
+BF = torch.bfloat16
+
+
+def _plain(rotary, device="cpu"):
+    z = torch.zeros(8, 16, dtype=BF)
+    return engine.DenseModel(embedding=z, norm=z[0], head=z, blocks=[], heads=2, kv_heads=1,
+                             head_dim=64, eps=1e-6, theta=1e4, rank=1, alpha=1.0, targets=(),
+                             device=device, rotary=rotary)
+
+
+def test_plain_rows_take_the_models_rotary():
+    valid = torch.ones(2, 5, dtype=torch.bool)
+    valid[1, 3:] = False
+    rotary = packed.Rotary(64, 1e4, rotary_dim=32, device="cpu")
+    positions, masks = _plain(rotary).positions_and_masks(valid)
+    assert isinstance(positions, packed.Positions) and positions.rotary is rotary
+    assert positions.positions.is_contiguous()
+    assert positions.positions.tolist() == [[0, 1, 2, 3, 4]] * 2
+    assert masks["full_attention"].lengths.tolist() == [5, 3]
+    (cos, sin), _ = _plain(None).positions_and_masks(valid)
+    want, _ = dense.positions_and_masks(valid, head_dim=64, theta=1e4, device="cpu")
+    assert torch.equal(cos, want[0]) and torch.equal(sin, want[1])
+
+
+SCALED = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+          "original_max_position_embeddings": 64}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [{"rotary_dim": 16}, {"scaling": SCALED}, {"interleaved": True}])
+def test_a_plain_row_scores_as_one_document(kw):
+    """The same row without documents and as one document.  The two attention
+    kernels round their bf16 outputs apart: half a step, 2^-8, of logits below 8,
+    in the logit and in the log-sum-exp; on the average 1e-2, as in training."""
+    from tests.test_gpu_packed_train import _model
+    from tests.test_gpu_train import CFG
+    dev = torch.device("cuda:0")
+    model, _, _ = _model(dev, packed.Rotary(CFG["D"], CFG["theta"], device=dev, **kw))
+    ids = torch.randint(0, CFG["vocab"], (2, 90), generator=torch.Generator().manual_seed(4))
+    session = slots.ResidentSession(model.blocks, dev)
+    with session.run():
+        plain = engine.score(model, session, ids).logprobs.double()
+        packed_row = engine.score(model, session, ids,
+                                  documents=torch.zeros_like(ids)).logprobs.double()
+        loss, _ = engine.microbatch(model, session, ids, ids, normalization=178, token_chunk=64)
+    session.close()
+    print("mean difference", float((plain - packed_row).mean()),
+          "rms", float((plain - packed_row).square().mean().sqrt()))
+    assert abs(float((plain - packed_row).mean())) <= 1e-2
+    assert float((plain - packed_row).square().mean().sqrt()) <= 2 * 8 * 2.0 ** -8
+    assert abs(loss + float(packed_row.mean())) <= 2 * 8 * 2.0 ** -8
+
+
+@pytest.mark.gpu
+def test_packed_rows_leave_a_plain_models_tables():
+    """A model without a rotary of its own turns plain rows by its bf16 tables,
+    also after it has seen packed rows."""
+    from tests.test_gpu_packed_train import _model
+    dev = torch.device("cuda:0")
+    model, _, _ = _model(dev)
+    model.packed_positions_and_masks(torch.zeros(1, 8, dtype=torch.int64))
+    rot, _ = model.positions_and_masks(torch.ones(1, 8, dtype=torch.bool))
+    assert isinstance(rot, tuple)
