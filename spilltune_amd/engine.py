@@ -71,13 +71,32 @@ def _row_inputs(model, input_ids, documents):
     return model.packed_positions_and_masks(documents)
 
 
-def _terminal(model, normalized, labels, *, normalization, token_chunk, objective):
+class LabelLogProbs(ops.TokenLogProbs):
+    """What an objective is given: the :class:`~spilltune_amd.ops.TokenLogProbs`
+    of a microbatch's labels, entry ``t`` of a row that of label ``t + 1``, with
+
+    * ``labels`` (int64 [batch, length - 1], on the device): those labels, -100
+      where none is to be learnt (dropped by the caller, a document's first token,
+      padding).  Log probabilities are 0 there, entropies are real: a term on
+      them is to be masked with ``labels != -100``;
+    * ``normalization``: the labels of the whole accumulation window, so that the
+      microbatches' terms, divided by it, add up to an average;
+    * ``item``: which row this is -- its index in ``train``'s rows, or what the
+      caller of ``microbatch`` names it."""
+    labels: torch.Tensor
+    normalization: int
+    item: object
+
+
+def _terminal(model, normalized, labels, *, normalization, token_chunk, objective, item=None):
     """The summed cross-entropy over ``normalization``, or the scalar that
-    ``objective`` makes of the labels' log probabilities (row ``t`` of the
-    :class:`~spilltune_amd.ops.TokenLogProbs` is label ``t + 1``; 0 at -100)."""
+    ``objective`` makes of the :class:`LabelLogProbs`."""
     if objective is not None:
-        return objective(ops.token_logprobs(normalized[:, :-1], model.head,
-                                            labels[:, 1:].to(torch.int64)))
+        labels = labels[:, 1:].to(torch.int64)
+        given = LabelLogProbs(*ops.token_logprobs(normalized[:, :-1], model.head, labels))
+        given.labels = labels.to(normalized.device)
+        given.normalization, given.item = normalization, item
+        return objective(given)
     chunks = ops.supervised_chunk_intervals(labels, token_chunk)
     return ops.chunked_causal_loss(normalized, model.head, labels,
                                    normalization=normalization, token_chunk=token_chunk,
@@ -85,10 +104,11 @@ def _terminal(model, normalized, labels, *, normalization, token_chunk, objectiv
 
 
 def microbatch(model, session, input_ids, labels, *, normalization, token_chunk, accumulate=False,
-               documents=None, objective=None):
+               documents=None, objective=None, item=None):
     """Exact shifted summed CE / window token count; one decoder backward.
     ``documents``: packed rows (labels across a document's start are dropped);
-    ``objective``: see :func:`_terminal`."""
+    ``objective``: a function of :class:`LabelLogProbs` (which tells it ``item``)
+    to a scalar, in the place of the cross-entropy."""
     device = model.device
     positions, masks = _row_inputs(model, input_ids, documents)
     if documents is not None:
@@ -98,7 +118,7 @@ def microbatch(model, session, input_ids, labels, *, normalization, token_chunk,
     terminal_input = hidden.detach().requires_grad_(True)
     normalized = model.terminal_norm(terminal_input)
     loss = _terminal(model, normalized, labels, normalization=normalization,
-                     token_chunk=token_chunk, objective=objective)
+                     token_chunk=token_chunk, objective=objective, item=item)
     (gradient,) = torch.autograd.grad(loss, terminal_input)
     if not torch.isfinite(loss) or not torch.isfinite(gradient).all():
         raise FloatingPointError("non-finite causal loss/gradient")
@@ -121,7 +141,8 @@ def score(model, session, input_ids, *, documents=None, top=0, temperature=1.0):
                                   top=top, temperature=temperature)
 
 
-def window_layer_major(model, session, items, *, normalization, token_chunk, objective=None):
+def window_layer_major(model, session, items, *, normalization, token_chunk, objective=None,
+                       names=None):
     """One gradient-accumulation window processed layer by layer, so each
     layer's 4-bit image crosses PCIe once per phase instead of once per
     microbatch (the reference streams every layer for every microbatch,
@@ -136,8 +157,12 @@ def window_layer_major(model, session, items, *, normalization, token_chunk, obj
 
     For each layer the fp32 adapter-gradient sums take the microbatches in the
     same order as the microbatch-major loop, so the gradients and losses are
-    the same bits.  Returns the per-microbatch losses."""
+    the same bits.  ``objective`` as for :func:`microbatch`; ``names`` its ``item`` of
+    each microbatch (default 0, 1, ...).  Returns the per-microbatch losses."""
     device = model.device
+    names = range(len(items)) if names is None else names
+    if len(names) != len(items):
+        raise ValueError(f"unsupported_capability: {len(names)} names for {len(items)} microbatches")
     mbs = []
     for ids, labels, *documents in items:
         positions, masks = _row_inputs(model, ids, *documents or [None])
@@ -152,11 +177,11 @@ def window_layer_major(model, session, items, *, normalization, token_chunk, obj
                                                       mb["masks"][block.kind], weights,
                                                       block.kwargs))
     losses = []
-    for mb in mbs:
+    for mb, name in zip(mbs, names):
         terminal_input = mb["h"].pop().detach().requires_grad_(True)
         normalized = model.terminal_norm(terminal_input)
         loss = _terminal(model, normalized, mb["labels"], normalization=normalization,
-                         token_chunk=token_chunk, objective=objective)
+                         token_chunk=token_chunk, objective=objective, item=name)
         (mb["g"],) = torch.autograd.grad(loss, terminal_input)
         if not torch.isfinite(loss) or not torch.isfinite(mb["g"]).all():
             raise FloatingPointError("non-finite causal loss/gradient")
@@ -216,7 +241,8 @@ def train(model, session, rows, *, steps, accumulation=1, lr=1e-4, weight_decay=
     optimizer = AdamW(lr=lr, weight_decay=weight_decay)
     cursor, losses = 0, []
     for _ in range(steps):
-        items = [rows[(cursor + i) % len(rows)] for i in range(accumulation)]
+        names = [(cursor + i) % len(rows) for i in range(accumulation)]
+        items = [rows[i] for i in names]
         normalization = sum(
             int(((labels if not docs or docs[0] is None else packed.document_labels(labels, docs[0]))
                  [:, 1:] != -100).sum()) for _, labels, *docs in items)
@@ -226,14 +252,15 @@ def train(model, session, rows, *, steps, accumulation=1, lr=1e-4, weight_decay=
             if layer_major:
                 for micro in window_layer_major(model, session, items,
                                                 normalization=normalization,
-                                                token_chunk=token_chunk, objective=objective):
+                                                token_chunk=token_chunk, objective=objective,
+                                                names=names):
                     loss += micro
             else:
                 for i, (ids, labels, *docs) in enumerate(items):
                     micro, _ = microbatch(model, session, ids, labels,
                                           normalization=normalization, token_chunk=token_chunk,
                                           accumulate=i > 0, documents=docs[0] if docs else None,
-                                          objective=objective)
+                                          objective=objective, item=names[i])
                     loss += micro
             optimizer.step(projections)
         cursor += accumulation
