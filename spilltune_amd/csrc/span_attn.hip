@@ -196,7 +196,9 @@ struct Args {
   int S, H, Hkv;
   float scale, sl2;          // scale, scale * log2(e)
   float cap_in, cap_out;     // with a cap: 2 log2(e) scale / cap, cap * log2(e)
-  float cap_small, cap_p[3]; // |s| up to which score_small holds, its coefficients
+  float cap_small, cap_r;    // |s| up to which score_small holds, scale / cap
+  float cap_p[3];            // score_small's coefficients, in powers of y^2
+  float cap_s[3];            // in powers of s^2; 0 where those leave fp32
 };
 
 // Workgroup head index -> head, so that the query heads of a KV head share an
@@ -214,10 +216,15 @@ constexpr int CAP = 1, BIAS = 2;
 // Chebyshev points, reweighted to level the relative error (4e-8).  Most capped
 // scores are there, and the polynomial takes half of the time of the exponential
 // and the reciprocal: the forward chooses it alone where a whole wave's are.
+// In powers of s^2 it is one product shorter (SQUARES; 16384 tokens, window 4096:
+// 1070 us against 1118), but s^2 and the coefficients can leave fp32 where the
+// score does not (scale / cap below 1e-19 or far from 1 with an extreme scale).
+template <bool SQUARES>
 __device__ __forceinline__ float score_small(const Args& a, float s) {
-  const float z = s * s;
-  float p = __builtin_fmaf(a.cap_p[2], z, a.cap_p[1]);
-  p = __builtin_fmaf(p, z, a.cap_p[0]);
+  const float y = SQUARES ? s : s * a.cap_r, z = y * y;
+  const float* c = SQUARES ? a.cap_s : a.cap_p;
+  float p = __builtin_fmaf(c[2], z, c[1]);
+  p = __builtin_fmaf(p, z, c[0]);
   return s * __builtin_fmaf(p, z, a.sl2);
 }
 
@@ -231,7 +238,7 @@ __device__ __forceinline__ float score(const Args& a, float slope2, float s, flo
     // large cap would multiply: small scores take the polynomial
     const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.cap_in));
     const float far_out = __builtin_fmaf(-2.0f * a.cap_out, r, a.cap_out);
-    x = fabsf(s) <= a.cap_small ? score_small(a, s) : far_out;
+    x = fabsf(s) <= a.cap_small ? score_small<false>(a, s) : far_out;
     grad = 4.0f * r * (1.0f - r);
   }
   if constexpr ((MODE & BIAS) != 0) x = __builtin_fmaf(-slope2, far, x);
@@ -679,11 +686,18 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
 #pragma unroll
           for (int v = 0; v < 16; ++v) top = fmaxf(top, fabsf(sacc[jb][v]));
         // (a NaN product passes either way: both forms keep it)
-        if (__ballot(top > a.cap_small) == 0) {
+        auto all = [&](auto squares) {
 #pragma unroll
           for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) sacc[jb][v] = score_small(a, sacc[jb][v]);
+            for (int v = 0; v < 16; ++v)
+              sacc[jb][v] = score_small<decltype(squares)::value>(a, sacc[jb][v]);
+        };
+        if (__ballot(top > a.cap_small) == 0) {
+          if (a.cap_s[2] != 0.0f)
+            all(std::true_type{});
+          else
+            all(std::false_type{});
         } else {
 #pragma unroll
           for (int jb = 0; jb < 2; ++jb)
@@ -1349,7 +1363,7 @@ int check_common(const char* name, int64_t B, int64_t S, int64_t H, int64_t Hkv,
                     name, (long long)DQ, (long long)DV);
   ST_CHECK_ARG(std::isfinite(scale) && scale > 0, "%s: scale must be positive and finite", name);
   ST_CHECK_ARG(std::isfinite(cap) && cap >= 0, "%s: cap must be finite, 0 for none", name);
-  // the kernels divide by the scale and form the sixth power of scale / cap
+  // the kernels divide by the scale, and multiply the cap and the scale by constants
   if (scale < 1e-30f || scale > 1e30f || (cap > 0 && (cap > 1e30f || scale / cap > 1e4f)))
     return st::fail(ST_EUNSUPPORTED, "%s: scale %g or cap %g out of range (scale 1e-30 to 1e30, cap up "
                     "to 1e30 and at least scale / 1e4)", name, scale, cap);
@@ -1379,8 +1393,13 @@ Args args_of(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B,
     a.cap_out = cap * LOG2E;
     const float r = scale / cap;
     a.cap_small = 0.35f / r;
+    a.cap_r = r;
     const float c[3] = {-0.33332663774490356f, 0.1329982578754425f, -0.049148499965667725f};
-    for (int i = 0; i < 3; ++i) a.cap_p[i] = a.sl2 * c[i] * powf(r, 2.0f * (float)(i + 1));
+    for (int i = 0; i < 3; ++i) a.cap_p[i] = a.sl2 * c[i];
+    // (the greatest s^2 used is 0.35^2 / r^2; the smallest and greatest coefficient)
+    const double last = (double)a.cap_p[2] * pow((double)r, 6.0), first = (double)a.cap_p[0] * r * r;
+    if (r > 1e-19f && std::min(fabs(first), fabs(last)) > 1e-36 && std::max(fabs(first), fabs(last)) < 1e36)
+      for (int i = 0; i < 3; ++i) a.cap_s[i] = (float)(a.cap_p[i] * pow((double)r, 2.0 * (i + 1)));
   }
   return a;
 }
