@@ -18,6 +18,8 @@
 // longer runs of memory in each head's rows, took 15.1 us against 10.7 for 2048
 // tokens of 48 heads of 128, and for 8192 (202 MB; in a trace, cold) 46 against 41
 // forward, 41 against 47 back.
+#include <algorithm>
+
 #include "common.h"
 
 namespace {
@@ -29,7 +31,7 @@ struct Rot {
   const uint16_t *x, *wq, *wk;   // token rows (fwd: input; bwd: the forward's, with norms)
   const void* pos;
   const double* inv;
-  int64_t ldx, S;
+  int64_t ldx, S, total;  // total: tokens
   int heads, kv, D, rot, pos64, inter;
   float amplitude, eps;
 };
@@ -103,13 +105,21 @@ __device__ __forceinline__ void turn(const Rot& a, const float2* cs, int d0, flo
   }
 }
 
+// A launch of 2^32 threads or more in one dimension is refused by the runtime:
+// tokens past 2^23 continue in the grid's third.
+constexpr int64_t MAX_X = (int64_t)1 << 23;
+__device__ __forceinline__ int64_t token_of() {
+  return (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
+}
+
 // CH: chunks of a head when known (0: a.D / 8)
 template <int CH, bool NORM>
 __global__ __launch_bounds__(NT) void rope_pos_fwd(Rot a, uint16_t* __restrict__ q,
                                                    uint16_t* __restrict__ k, uint16_t* __restrict__ v,
                                                    float* __restrict__ rstd) {
   __shared__ float2 cs[MAX_ROT / 2];
-  const int64_t t = blockIdx.x;
+  const int64_t t = token_of();
+  if (t >= a.total) return;  // the whole workgroup
   table(a, t, cs);
   __syncthreads();
   const int ch = CH ? CH : a.D / 8;
@@ -169,7 +179,8 @@ __global__ __launch_bounds__(NT) void rope_pos_bwd(Rot a, const uint16_t* __rest
                                                    const float* __restrict__ rstd,
                                                    uint16_t* __restrict__ dx, int64_t lddx) {
   __shared__ float2 cs[MAX_ROT / 2];
-  const int64_t t = blockIdx.x;
+  const int64_t t = token_of();
+  if (t >= a.total) return;  // the whole workgroup
   table(a, t, cs);
   __syncthreads();
   const int ch = CH ? CH : a.D / 8;
@@ -235,6 +246,7 @@ int check_rot(const char* name, Rot& a, const void* positions, int32_t pos64, co
   a.pos = positions; a.pos64 = pos64;
   a.inv = inv_freq;
   a.S = S;
+  a.total = B * S;
   a.heads = (int)heads; a.kv = (int)kv; a.D = (int)D; a.rot = (int)rot; a.inter = inter;
   a.amplitude = (float)amplitude;
   a.eps = eps;
@@ -244,9 +256,10 @@ int check_rot(const char* name, Rot& a, const void* positions, int32_t pos64, co
 // a token's workgroups: one, or as many as its chunks fill where few tokens
 // leave CUs without work (16 tokens of 48 heads of 128: 3.2 us against 4.1; 400:
 // 4.7 against 5.0; 600: 5.6 either way)
-dim3 grid_of(const Rot& a, int64_t total) {
-  const int64_t chunks = (int64_t)(a.heads + 2 * a.kv) * (a.D / 8);
-  return dim3((unsigned)total, (unsigned)(total >= 512 ? 1 : st::cdiv(chunks, NT)));
+dim3 grid_of(const Rot& a) {
+  const int64_t chunks = (int64_t)(a.heads + 2 * a.kv) * (a.D / 8), x = std::min(a.total, MAX_X);
+  return dim3((unsigned)x, (unsigned)(a.total >= 512 ? 1 : st::cdiv(chunks, NT)),
+              (unsigned)st::cdiv(a.total, x));
 }
 template <typename F>
 void by_head(const Rot& a, F&& go) {
@@ -282,7 +295,7 @@ extern "C" int st_rope_pos_fwd(const uint16_t* x, int64_t ldx, const void* posit
   a.ldx = ldx;
   by_head(a, [&](auto ch, auto norm) {
     rope_pos_fwd<decltype(ch)::value, decltype(norm)::value>
-        <<<grid_of(a, B * S), NT, 0, (hipStream_t)stream>>>(a, q, k, v, rstd);
+        <<<grid_of(a), NT, 0, (hipStream_t)stream>>>(a, q, k, v, rstd);
   });
   return st::check_launch(name);
 }
@@ -308,7 +321,7 @@ extern "C" int st_rope_pos_bwd(const uint16_t* dq, const uint16_t* dk, const uin
   a.ldx = ldx;
   by_head(a, [&](auto ch, auto norm) {
     rope_pos_bwd<decltype(ch)::value, decltype(norm)::value>
-        <<<grid_of(a, B * S), NT, 0, (hipStream_t)stream>>>(a, dq, dk, dv, rstd, dx, lddx);
+        <<<grid_of(a), NT, 0, (hipStream_t)stream>>>(a, dq, dk, dv, rstd, dx, lddx);
   });
   return st::check_launch(name);
 }

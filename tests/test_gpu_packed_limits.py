@@ -31,3 +31,22 @@ def test_scales_and_caps_at_their_limits(dims, scale, cap):
     leaves = [t.requires_grad_(True) for t in (q, k, v)]
     out = packed.span_attention(*leaves, scale, mask, cap=cap)
     _check((out, *torch.autograd.grad(out, leaves, dout)), want, bound)
+
+
+def test_rotation_of_more_tokens_than_one_grid_dimension():
+    """2^24 and more tokens (2^32 threads) in one call, against slices of it."""
+    T, D = (1 << 24) + 11, 8
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rotary = packed.Rotary(D, 1e4, device="cuda")
+    y = _randn(g, T, 3 * D).to(BF).requires_grad_(True)
+    pos = (torch.arange(T, device="cuda") % 4099)[None]
+    ups = [_randn(g, 1, 1, T, D).to(BF) for _ in range(3)]
+    got = packed.rope_positions(y, pos, rotary, 1, 1)
+    (dy,) = torch.autograd.grad(got, y, ups)
+    for a in (0, (1 << 22) - 5, (1 << 23) - 5, (1 << 23) + 7000, (1 << 24) - 5):
+        part = slice(a, a + 16)
+        x = y.detach()[part].clone().requires_grad_(True)
+        want = packed.rope_positions(x, pos[:, part].contiguous(), rotary, 1, 1)
+        (dx,) = torch.autograd.grad(want, x, [u[:, :, part] for u in ups])
+        assert all(torch.equal(o[:, :, part], w) for o, w in zip(got, want))
+        assert torch.equal(dy[part], dx)
