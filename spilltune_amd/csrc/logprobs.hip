@@ -674,13 +674,16 @@ int check(const char* name, Head& h, const uint16_t* hidden, int64_t rows, int64
   return ST_OK;
 }
 
+// a dimension of a launch holds less than 2^32 threads
+bool fits(int64_t groups, int threads) { return groups * threads < (int64_t)1 << 32; }
+
 // fn(loop type, grid) with the row tile that suits the rows
 template <typename F>
 int by_rows(Head& h, F&& fn) {
   const int bn = row_tile(h.rows);
   h.rtiles = (int)st::cdiv(h.rows, bn);
   const int64_t tiles = up((int64_t)h.rtiles * h.vtiles, 8);
-  if (tiles > 0x7fffffff) return st::fail(ST_EUNSUPPORTED, "token_logprobs: too many tiles");
+  if (!fits(tiles, 512)) return st::fail(ST_EUNSUPPORTED, "token_logprobs: too many tiles");
   const dim3 grid((unsigned)tiles);
   if (bn == 256) fn(st::DmaLoop256<false, false>{}, grid);
   else if (bn == 128) fn(st::DmaLoop64<false, false, 4, 2, 3>{}, grid);
@@ -755,6 +758,11 @@ extern "C" int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64
   uint16_t* dl = (uint16_t*)ws;
   float *left = (float*)(ws + sp.left), *part = (float*)(ws + sp.part);
   hipStream_t s = (hipStream_t)stream;
+  const Split& k = sp.split;
+  const Dgrad d{dl, head, sp.ldd, ldw, rows, V, (int)H, (int)st::cdiv(rows, k.bm),
+                (int)st::cdiv(H, k.bn), k.splits, k.per};
+  const int64_t parts = up((int64_t)d.rtiles * d.htiles * d.splits, 8);
+  if (!fits(parts, 512)) return st::fail(ST_EUNSUPPORTED, "%s: too many tiles", name);
   const Upstream g{g_logprobs, g_entropy, top ? g_top : nullptr, (int)top};
   const Picks p{top_tokens, top_logprobs, logprobs, lse, entropy};
   if (logits) {
@@ -772,10 +780,7 @@ extern "C" int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64
                                                                      left);
     if (int rc = st::check_launch("lp_picked")) return rc;
   }
-  const Split& k = sp.split;
-  const Dgrad d{dl, head, sp.ldd, ldw, rows, V, (int)H, (int)st::cdiv(rows, k.bm),
-                (int)st::cdiv(H, k.bn), k.splits, k.per};
-  const dim3 grid((unsigned)up((int64_t)d.rtiles * d.htiles * d.splits, 8));
+  const dim3 grid((unsigned)parts);
   if (k.bm == 64)
     lp_dhidden<st::DmaLoop64<true, false, 1, 4, 4>><<<grid, 256, 0, s>>>(d, part);
   else if (k.bn == 128)

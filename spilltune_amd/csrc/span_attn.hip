@@ -1404,8 +1404,17 @@ Args args_of(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t B,
   return a;
 }
 
+// a dimension of a launch holds less than 2^32 threads
+int fits(const char* name, int64_t groups, int64_t threads) {
+  if (groups * threads >= (int64_t)1 << 32)
+    return st::fail(ST_EUNSUPPORTED, "%s: %lld workgroups of %lld threads are too large a launch", name,
+                    (long long)groups, (long long)threads);
+  return ST_OK;
+}
+
 template <int DQ, int DV, int MODE>
 int run_fwd(const Args& a, int64_t B, uint16_t* out, float* lse, hipStream_t s) {
+  if (int rc = fits("st_span_attn_fwd", B * a.plan.nt * a.H, NT)) return rc;
   span_fwd<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, lse);
   return st::check_launch("span_fwd");
 }
@@ -1416,15 +1425,20 @@ int run_bwd(const Args& a, int64_t B, const uint16_t* out, const float* lse, con
   const Space sp = space_of(B, a.S, a.H, a.Hkv, DQ, DV);
   float* delta = (float*)(ws + sp.delta);
   float *dkp = (float*)(ws + sp.dkp), *dvp = (float*)(ws + sp.dvp);
+  constexpr int NTH = 64 * dkdv_waves<DQ>();
+  const int64_t tiles = B * a.plan.nt * a.Hkv;
+  if (int rc = fits("st_span_attn_bwd", B * a.plan.nt * a.H, NT)) return rc;
+  if (int rc = fits("st_span_attn_bwd", tiles * sp.most, NTH)) return rc;
+  if (int rc = fits("st_span_attn_bwd", sp.most > 1 ? tiles : 0, NT)) return rc;
   span_bwd_dq<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, dout, lse, delta,
                                                                           dq);
   if (int rc = st::check_launch("span_bwd_dq")) return rc;
-  const unsigned tiles = (unsigned)(B * a.plan.nt * a.Hkv);
-  span_bwd_dkdv<DQ, DV, MODE><<<tiles * sp.most, 64 * dkdv_waves<DQ>(), 0, s>>>(
+  span_bwd_dkdv<DQ, DV, MODE><<<(unsigned)(tiles * sp.most), NTH, 0, s>>>(
       a, dout, lse, delta, sp.most, dkp, dvp, dk, dv);
   int rc = st::check_launch("span_bwd_dkdv");
   if (rc || sp.most == 1) return rc;
-  span_reduce<<<dim3(tiles, 8), NT, 0, s>>>(a.plan, dkp, dvp, a.H / a.Hkv, a.Hkv, sp.most, a.S, DQ, DV, dk, dv);
+  span_reduce<<<dim3((unsigned)tiles, 8), NT, 0, s>>>(a.plan, dkp, dvp, a.H / a.Hkv, a.Hkv, sp.most, a.S,
+                                                     DQ, DV, dk, dv);
   return st::check_launch("span_reduce");
 }
 
@@ -1466,6 +1480,8 @@ extern "C" int st_span_plan(const int32_t* key_start, const int32_t* key_end, in
     return st::fail(ST_EWORKSPACE, "st_span_plan: needs %lld bytes", (long long)p.bytes);
   hipStream_t s = (hipStream_t)stream;
   const int64_t blocks = B * p.nb, tiles = B * p.nt;
+  if (int rc = fits("st_span_plan", st::cdiv(blocks * 32, NT), NT)) return rc;
+  if (int rc = fits("st_span_plan", tiles, 64)) return rc;
   span_blocks<<<(unsigned)st::cdiv(blocks * 32, NT), NT, 0, s>>>(key_start, key_end, (int)S, p.nb,
                                                                  blocks, (int4*)p.blk);
   if (int rc = st::check_launch("span_blocks")) return rc;
