@@ -799,6 +799,21 @@ def _row_chunks(rows, per):
     return [(r, min(r + step, rows)) for r in range(0, rows, step)]
 
 
+def _scratch_chunks(rows, per, bytes_of):
+    """(first row, end, scratch bytes) of row ranges of ``per`` bytes a row and more:
+    ``bytes_of(n)`` is the scratch of n rows, which shrinks the ranges until it
+    stays within LOGPROB_SCRATCH (or they are down to 256 rows)."""
+    chunks = _row_chunks(rows, per)
+    while chunks:
+        size = chunks[0][1]
+        need = bytes_of(size)
+        if need <= LOGPROB_SCRATCH or size <= 256:
+            return [(a, z, need if z - a == size else bytes_of(z - a)) for a, z in chunks]
+        per *= 2
+        chunks = _row_chunks(rows, per)
+    return []
+
+
 def _row_ptr(t, row, width=1):
     """Address of row ``row`` of a contiguous ``t`` in rows of ``width``, without
     a view of it; None for None."""
@@ -854,8 +869,10 @@ class _TokenLogProbs(torch.autograd.Function):
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
         dh = torch.empty(hidden.shape, dtype=_BF16, device=dev)
         with _lib.on_device(dev):
-            for a, z in _row_chunks(rows, 2 * V):
-                nbytes = _lib.query("st_token_logprobs_workspace_bytes", z - a, H, V, H, top, 0, 1)
+            # dl of a row, and besides it the partial sums of its hidden gradient: more than
+            # dl where the vocabulary is small
+            for a, z, nbytes in _scratch_chunks(rows, 2 * V, lambda n: _lib.query(
+                    "st_token_logprobs_workspace_bytes", n, H, V, H, top, 0, 1)):
                 ws = _scratch(dev, nbytes)
                 _lib.call("st_token_logprobs_bwd", _row_ptr(hidden, a, H), z - a, H, H,
                           head.data_ptr(), V, H, _row_ptr(tokens, a), ignore_index, temperature, cap,

@@ -87,3 +87,20 @@ def test_row_chunks_stay_within_a_call():
         assert chunks[0][0] == 0 and chunks[-1][1] == rows
         assert all(0 < z - a <= 1 << 22 for a, z in chunks)
         assert all(z == a for (_, z), (a, _) in zip(chunks, chunks[1:]))
+
+
+@pytest.mark.parametrize("rows,H,V", [(100000, 8192, 512), (1 << 20, 16384, 32), (3000, 4096, 151936), (7, 64, 40),
+                                      (200, 16384, 200000)])
+def test_backward_scratch_counts_the_partial_sums(rows, H, V):
+    """A small vocabulary under a wide model: the fp32 partial sums are the larger
+    part of the backward's scratch."""
+    def need(n):
+        return _lib.query("st_token_logprobs_workspace_bytes", n, H, V, H, 0, 0, 1)
+    chunks = ops._scratch_chunks(rows, 2 * V, need)
+    assert chunks[0][0] == 0 and chunks[-1][1] == rows
+    assert all(z == a for (_, z, _), (a, _, _) in zip(chunks, chunks[1:]))
+    for a, z, nbytes in chunks:
+        assert nbytes == need(z - a) and (nbytes <= ops.LOGPROB_SCRATCH or z - a <= 256)
+    assert not ops._scratch_chunks(0, 2 * V, need)
+    # no more ranges than they take
+    assert len(chunks) == 1 or need(2 * (chunks[0][1] + 256)) > ops.LOGPROB_SCRATCH
