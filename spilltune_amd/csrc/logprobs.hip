@@ -371,11 +371,14 @@ __device__ __forceinline__ int64_t column_of(const Head& h, const Upstream& g, i
   const int64_t y = h.tokens[row];
   return y != ignore && y >= 0 && y < h.V ? y : -1;
 }
-// dl of pick k, in column c, from the saved log probability; a token picked twice
-// gets one value from both.  Returns whether the entry is to be replaced; `left`:
-// what its rounding leaves, once for each entry.
+// dl of pick k, in column c of logit l (read with a cap only), from the saved log
+// probability; a token picked twice gets one value from both.  Returns whether the
+// entry is to be replaced; `left`: what its rounding leaves, once for each entry.
+// (The tanh is not taken back from lp + lse: those are of the size of log V, and a
+// temperature far above the cap would multiply their rounding.)
 __device__ __forceinline__ bool picked(const Head& h, const Upstream& g, int64_t ignore, const Picks& p,
-                                       int64_t row, int k, int64_t c, uint16_t& value, float& left) {
+                                       int64_t row, int k, int64_t c, float l, uint16_t& value,
+                                       float& left) {
   left = 0.0f;
   const int64_t y = column_of(h, g, ignore, p, row, g.ntop);
   const float lp = k < g.ntop ? p.top_lp[row * g.ntop + k] : p.logprobs[row];
@@ -391,12 +394,7 @@ __device__ __forceinline__ bool picked(const Head& h, const Upstream& g, int64_t
   }
   const float pr = __builtin_amdgcn_exp2f(lp * LOG2E), ge = g.ent ? g.ent[row] : 0.0f;
   if (own == 0.0f && sum == 0.0f && ge == 0.0f) return false;  // as the other columns
-  float d = own - pr * __builtin_fmaf(ge, lp + p.ent[row], sum);
-  if (h.tf.cap != 0.0f) {
-    const float t = (lp + p.lse[row]) / h.tf.inv_t * h.tf.inv_cap;  // tanh of the raw logit
-    d *= (1.0f - t) * (1.0f + t);
-  }
-  d *= h.tf.inv_t;
+  const float d = (own - pr * __builtin_fmaf(ge, lp + p.ent[row], sum)) * slope(h.tf, l);
   value = st::f32_to_bf16(d);
   if (!again) left = d - st::bf16_to_f32(value);
   return true;
@@ -470,7 +468,11 @@ __global__ __launch_bounds__(NT) void lp_dlogits_kept(Head h, Upstream g, int64_
     if (at < 0 ? c0 != 0 : at < c0 || at >= c0 + KEPT) continue;
     uint16_t value;
     float rest = 0.0f;
-    if (at >= 0 && picked(h, g, ignore, p, row, k, at, value, rest)) {
+    float raw = 0.0f;
+#pragma unroll
+    for (int e = 0; e < KEPT; ++e)
+      if (at == c0 + e) raw = l[e];
+    if (at >= 0 && picked(h, g, ignore, p, row, k, at, raw, value, rest)) {
 #pragma unroll
       for (int e = 0; e < KEPT; ++e)
         if (at == c0 + e) d[e] = st::bf16_to_f32(value);
@@ -482,20 +484,40 @@ __global__ __launch_bounds__(NT) void lp_dlogits_kept(Head h, Upstream g, int64_
 }
 
 // the picked tokens' entries whole, over what lp_dlogits wrote: thread k of a row
-// takes pick k.  left[row][k]: see picked
+// takes pick k; with a cap wave k does, and forms the logit again.  left[row][k]:
+// see picked
+template <bool CAP>
 __global__ __launch_bounds__(NT) void lp_picked(Head h, Upstream g, int64_t ignore, Picks p,
                                                 uint16_t* __restrict__ dl, int64_t ldd,
                                                 float* __restrict__ left) {
-  const int64_t n = (int64_t)blockIdx.x * NT + threadIdx.x;
-  const int per = g.ntop + 1;
-  const int64_t row = n / per;
-  const int k = (int)(n % per);
-  if (row >= h.rows) return;
-  const int64_t c = column_of(h, g, ignore, p, row, k);
-  uint16_t value;
-  float rest = 0.0f;
-  if (c >= 0 && picked(h, g, ignore, p, row, k, c, value, rest)) dl[row * ldd + c] = value;
-  left[n] = rest;
+  constexpr int OF = CAP ? 64 : 1;  // threads of a pick
+  const int per = g.ntop + 1, lane = threadIdx.x & 63;
+  for (int64_t n = ((int64_t)blockIdx.x * NT + threadIdx.x) / OF; n < h.rows * per;
+       n += (int64_t)gridDim.x * NT / OF) {
+    const int64_t row = n / per;
+    const int k = (int)(n % per);
+    const int64_t c = column_of(h, g, ignore, p, row, k);
+    float l = 0.0f;
+    if (CAP && c >= 0) {
+      for (int i = lane * 8; i < h.H; i += 64 * 8) {
+        const uint4 a = *(const uint4*)(h.hidden + row * h.ldh + i);
+        const uint4 b = *(const uint4*)(h.head + c * h.ldw + i);
+        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          l = __builtin_fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), l);
+          l = __builtin_fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), l);
+        }
+      }
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
+    }
+    if (CAP && lane != 0) continue;
+    uint16_t value;
+    float rest = 0.0f;
+    if (c >= 0 && picked(h, g, ignore, p, row, k, c, l, value, rest)) dl[row * ldd + c] = value;
+    left[n] = rest;
+  }
 }
 
 // dhidden partials: part[split][row][h] = sum over the split's columns of dl head.
@@ -776,8 +798,12 @@ extern "C" int st_token_logprobs_bwd(const uint16_t* hidden, int64_t rows, int64
           lp_dlogits<LP><<<grid, LP::NT, 0, s>>>(h, g, ignore_index, top_tokens, lse, entropy, dl, sp.ldd);
         })) return rc;
     if (int rc = st::check_launch("lp_dlogits")) return rc;
-    lp_picked<<<(unsigned)st::cdiv(rows * (top + 1), NT), NT, 0, s>>>(h, g, ignore_index, p, dl, sp.ldd,
-                                                                     left);
+    const int64_t picks = rows * (top + 1);
+    const unsigned groups = (unsigned)std::min<int64_t>(st::cdiv(picks, h.tf.cap != 0.0f ? NT / 64 : NT), 1 << 20);
+    if (h.tf.cap != 0.0f)
+      lp_picked<true><<<groups, NT, 0, s>>>(h, g, ignore_index, p, dl, sp.ldd, left);
+    else
+      lp_picked<false><<<groups, NT, 0, s>>>(h, g, ignore_index, p, dl, sp.ldd, left);
     if (int rc = st::check_launch("lp_picked")) return rc;
   }
   const dim3 grid((unsigned)parts);
