@@ -28,9 +28,13 @@
 //
 // Masked places never reach a result: a masked score is replaced, not added to,
 // but an infinity or NaN in a key, value or gradient row that a 32-row block
-// partly sees does meet a zero probability inside an MFMA product.  A wave that
-// ends with a sum that is not finite has its rows redone over the seen pairs
-// alone, by its whole workgroup, before the kernel ends (redo_*).
+// partly sees does meet a zero probability inside an MFMA product.  A workgroup
+// in which a wave's sums are not finite therefore walks its tile once more
+// (CAREFUL), with products in which a masked pair adds nothing whatever its rows
+// hold (add_seen), and those waves' rows are taken from there.  What is not finite
+// then is the answer.  A training pass of 4096 tokens in one document whose values
+// are all NaN, 8/2 heads of 128: 2.5 ms, of finite ones 0.38 (rows summed pair by
+// pair instead took 62 ms at 1024 tokens, 0.2 finite, and grew with their square).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -416,193 +420,130 @@ __device__ __forceinline__ Walk walk_of(const Plan& p, int b, int qt, int wave) 
   return w;
 }
 
-// ---------------------------------------------------------------- redone rows
-// A 32-row block whose sums are not finite, over the seen pairs alone, by the
-// whole workgroup (NTH threads).  Correct, not fast: no block comes here while
-// the operands are finite.  `mem`: LDS that the tiles no longer need.
-template <int D>
-__device__ float dot(const uint16_t* __restrict__ x, const uint16_t* __restrict__ y) {
-  float s = 0.0f;
-#pragma unroll 1
-  for (int d = 0; d < D; d += 8) {
-    const uint4 u = ld_global16(x + d), w = ld_global16(y + d);
-    const uint32_t p[4] = {u.x, u.y, u.z, u.w}, r[4] = {w.x, w.y, w.z, w.w};
+// ---------------------------------------------------------------- careful pass
+// whether any wave of the workgroup says so; `flags`: LDS that no wave needs
+template <int NTH>
+__device__ __forceinline__ bool any_wave(bool x, int* flags) {
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) flags[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int any = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s = __builtin_fmaf(__uint_as_float(p[e] << 16), __uint_as_float(r[e] << 16), s);
-      s = __builtin_fmaf(__uint_as_float(p[e] & 0xffff0000u), __uint_as_float(r[e] & 0xffff0000u), s);
-    }
-  }
-  return s;
+  for (int w = 0; w < NTH / 64; ++w) any |= flags[w];
+  __syncthreads();
+  return uniform(any) != 0;
 }
-template <bool MAX, int NTH>
-__device__ __forceinline__ float block_reduce(float x, float* red) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    const float y = __shfl_xor(x, d);
-    x = MAX ? fmaxf(x, y) : x + y;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = red[0];
-  for (int i = 1; i < NTH / 64; ++i) x = MAX ? fmaxf(x, red[i]) : x + red[i];
+// The careful pass reads its arguments and forms its indexes again: kept from the
+// first one they would take registers through its loop (a training pass of 8192
+// packed tokens 514 us against 477).
+template <typename T>  // T: the kernel's only argument
+__device__ __forceinline__ T arguments_again() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const T*)p;
+}
+template <bool AGAIN>
+__device__ __forceinline__ int block_index() {
+  int x = blockIdx.x;
+  if constexpr (AGAIN) asm volatile("" : "+s"(x));
   return x;
 }
-// calls fn(wave, mem) for each wave that is bad; every thread of the workgroup
-// comes here, its tiles and staging no longer needed
-template <int NTH, typename F>
-__device__ __forceinline__ void redo(bool bad, int wave, int lane, float* lds, F&& fn) {
-  __syncthreads();
-  if (lane == 0) lds[wave] = bad ? 1.0f : 0.0f;
-  __syncthreads();
-  unsigned set = 0;
+template <bool AGAIN>
+__device__ __forceinline__ int thread_index() {
+  int x = threadIdx.x;
+  if constexpr (AGAIN) asm volatile("" : "+v"(x));
+  return x;
+}
+// a lane's rows of an operand in registers, or read again at each use
+template <int N, bool AGAIN>
+struct Rows {
+  bf16x8 held[AGAIN || N == 0 ? 1 : N];
+  const uint16_t* at;  // NULL: zeros
+  __device__ __forceinline__ bf16x8 read(int s) const {
+    return as_bf16x8(at ? ld_global16(at + 16 * s) : make_uint4(0, 0, 0, 0));
+  }
+  __device__ __forceinline__ explicit Rows(const uint16_t* p) : at(p) {
+    if constexpr (!AGAIN)
 #pragma unroll
-  for (int w = 0; w < NTH / 64; ++w) set |= lds[w] != 0.0f ? 1u << w : 0u;
-  if (set == 0) return;
-  __syncthreads();
-#pragma unroll 1
-  for (int w = 0; w < NTH / 64; ++w)
-    if (set >> w & 1) fn(w, lds);
-}
+      for (int s = 0; s < N; ++s) held[s] = read(s);
+  }
+  __device__ __forceinline__ void forget() {  // or the reads would leave the loop
+    if constexpr (AGAIN) asm volatile("" : "+v"(at));
+  }
+  __device__ __forceinline__ bf16x8 operator[](int s) const {
+    if constexpr (AGAIN) return read(s);
+    else return held[s];
+  }
+};
 
-template <int DQ, int DV, int MODE>
-__device__ void redo_fwd(const Args& a, int b, int h, int i0, uint16_t* __restrict__ out,
-                         float* __restrict__ lse, float* mem) {
-  const int tid = threadIdx.x, S = a.S, H = a.H;
-  float *red = mem, *ps = mem + 64;
-  const int64_t bh = (int64_t)b * H + h;
-  const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
-  const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
-  const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
-#pragma unroll 1
-  for (int i = i0; i < min(i0 + 32, S); ++i) {
-    const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
-    uint16_t* o_row = out + ((int64_t)b * S + i) * H * DV + (int64_t)h * DV;
-    if (run.x >= run.y) {
-      if (tid < DV) o_row[tid] = 0;
-      if (tid == 0) lse[bh * S + i] = INFINITY;
-      continue;
-    }
-    const uint16_t* qi = a.q + (bh * S + i) * DQ;
-    auto x_of = [&](int j) {
-      float grad;
-      return score<MODE>(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ), fabsf((float)(i - j)), grad);
+// acc += A B over the seen pairs of a block, where A's rows may hold infinities and
+// NaN, B's weights of masked pairs are 0.  Those are taken out of A, which leaves every pair's
+// product finite, and what they make of a sum is found by a second product: of
+// their kind (+inf 1, -inf 2^10, NaN 2^20) with 1 for a seen pair, 2^20 for one of
+// weight 0 (0 * inf), 0 for a masked one.  At most 64 pairs meet, so the kinds do
+// not run into each other.
+constexpr uint32_t ONE = 0x3f80, NEG = 0x4480, NAN20 = 0x4980;  // bf16 1, 2^10, 2^20
+__device__ __forceinline__ void part_kinds(bf16x8 x, bf16x8& rest, bf16x8& kind) {
+  uint4 w = __builtin_bit_cast(uint4, x), k;
+  auto one = [](uint32_t& v, uint32_t& to) {
+    auto half = [](uint32_t h) {
+      return (h & 0x7f80) != 0x7f80 ? 0u : (h & 0x7f) ? NAN20 : (h & 0x8000) ? NEG : ONE;
     };
-    float m = -INFINITY;
-#pragma unroll 1
-    for (int j = run.x + tid; j < run.y; j += NT) m = fmaxf(m, x_of(j));
-    m = block_reduce<true, NT>(m, red);
-    float l = 0.0f, o = 0.0f;
-#pragma unroll 1
-    for (int c0 = run.x; c0 < run.y; c0 += NT) {
-      const float p = c0 + tid < run.y ? __builtin_amdgcn_exp2f(x_of(c0 + tid) - m) : 0.0f;
-      l += p;
-      __syncthreads();
-      ps[tid] = p;
-      __syncthreads();
-      if (tid < DV)
-#pragma unroll 1
-        for (int j = c0; j < min(c0 + NT, run.y); ++j)
-          o = __builtin_fmaf(ps[j - c0], st::bf16_to_f32(vb[(int64_t)j * DV + tid]), o);
-    }
-    l = block_reduce<false, NT>(l, red);
-    if (tid < DV) o_row[tid] = st::f32_to_bf16(o / l);
-    if (tid == 0) lse[bh * S + i] = m + log2f(l);
-  }
+    const uint32_t lo = half(v & 0xffff), hi = half(v >> 16);
+    to = lo | hi << 16;
+    v &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+  };
+  one(w.x, k.x);
+  one(w.y, k.y);
+  one(w.z, k.z);
+  one(w.w, k.w);
+  rest = as_bf16x8(w);
+  kind = as_bf16x8(k);
 }
-
-template <int DQ, int DV, int MODE>
-__device__ void redo_dq(const Args& a, int b, int h, int i0, const uint16_t* __restrict__ dout,
-                        const float* __restrict__ lse, const float* delta,
-                        uint16_t* __restrict__ dq, float* mem) {
-  const int tid = threadIdx.x, S = a.S, H = a.H;
-  const int64_t bh = (int64_t)b * H + h;
-  const uint16_t* kb = a.k + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DQ;
-  const uint16_t* vb = a.v + ((int64_t)b * a.Hkv + h / (H / a.Hkv)) * S * DV;
-  const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
-#pragma unroll 1
-  for (int i = i0; i < min(i0 + 32, S); ++i) {
-    const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
-    const uint16_t* qi = a.q + (bh * S + i) * DQ;
-    const uint16_t* gi = dout + ((int64_t)b * S + i) * H * DV + (int64_t)h * DV;
-    const float li = lse[bh * S + i], di = delta[bh * S + i];
-    float o = 0.0f;
-#pragma unroll 1
-    for (int c0 = run.x; c0 < run.y; c0 += NT) {
-      const int j = c0 + tid;
-      float ds = 0.0f;
-      if (j < run.y) {
-        float grad;
-        const float x = score<MODE>(a, slope2, dot<DQ>(qi, kb + (int64_t)j * DQ),
-                                    fabsf((float)(i - j)), grad);
-        ds = __builtin_amdgcn_exp2f(x - li) * (dot<DV>(gi, vb + (int64_t)j * DV) - di) * grad;
-        if (run.y - run.x == 1) ds = 0.0f;
-      }
-      __syncthreads();
-      mem[tid] = ds;
-      __syncthreads();
-      if (tid < DQ)
-#pragma unroll 1
-        for (int jj = c0; jj < min(c0 + NT, run.y); ++jj)
-          o = __builtin_fmaf(mem[jj - c0], st::bf16_to_f32(kb[(int64_t)jj * DQ + tid]), o);
-    }
-    if (tid < DQ) dq[(bh * S + i) * DQ + tid] = st::f32_to_bf16(o * a.scale);
+// The pairs of a lane: bit i of `seen`, and of `none` where the weight is 0.
+struct Pairs {
+  uint32_t seen = 0, none = 0;
+  __device__ __forceinline__ void put(int i, bool sees, float weight) {
+    seen |= sees ? 1u << i : 0u;
+    none |= weight == 0.0f ? 1u << i : 0u;
+    asm volatile("" : "+v"(seen), "+v"(none));  // or every pair keeps two lane masks
   }
+  // what pairs 8 i .. 8 i + 7 say to the second product
+  __device__ __forceinline__ bf16x8 kinds(int i) const {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      auto half = [&](int bit) { return !(seen >> bit & 1) ? 0u : none >> bit & 1 ? NAN20 : ONE; };
+      w[e] = half(8 * i + 2 * e) | half(8 * i + 2 * e + 1) << 16;
+    }
+    return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+  }
+};
+__device__ __forceinline__ float of_kinds(float c) {
+  const float nan = __uint_as_float(0x7fc00000u);
+  const bool neg = c >= 1024.0f, pos = c - 1024.0f * floorf(c * (1.0f / 1024.0f)) > 0.0f;
+  return c >= 1048576.0f || (neg && pos) ? nan : neg ? -INFINITY : pos ? INFINITY : 0.0f;
 }
-
-// keys [j0, j0 + 32) over the query heads [h0, h0 + heads) of KV head hk
-template <int DQ, int DV, int MODE, int NTH, typename W>
-__device__ void redo_dkdv(const Args& a, int b, int hk, int h0, int heads, int j0, int2 seen,
-                          const uint16_t* __restrict__ dout, const float* __restrict__ lse,
-                          const float* __restrict__ delta, float* mem, W&& write) {
-  const int tid = threadIdx.x, S = a.S, H = a.H;
-  float *ps = mem, *ds = mem + NTH, *vis = mem + 2 * NTH;
-  const int qa = seen.x * 32, qz = min(seen.y * 32, S);
-#pragma unroll 1
-  for (int j = j0; j < min(j0 + 32, S); ++j) {
-    const uint16_t* kj = a.k + (((int64_t)b * a.Hkv + hk) * S + j) * DQ;
-    const uint16_t* vj = a.v + (((int64_t)b * a.Hkv + hk) * S + j) * DV;
-    float sk = 0.0f, sv = 0.0f;  // this thread's column of dK, of dV
-#pragma unroll 1
-    for (int h = h0; h < h0 + heads; ++h) {
-      const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
-      const int64_t bh = (int64_t)b * H + h;
-      const uint16_t* gb = dout + (int64_t)b * S * H * DV + (int64_t)h * DV;
-#pragma unroll 1
-      for (int c0 = qa; c0 < qz; c0 += NTH) {
-        const int i = c0 + tid;
-        bool sees = false, one = false;
-        float p = 0.0f, d = 0.0f;
-        if (i < qz) {
-          const int2 run = run_of(a.lo, a.hi, (int64_t)b * S + i, S);
-          sees = run.x <= j && j < run.y;
-          one = run.y - run.x == 1;
-        }
-        if (sees) {
-          float grad;
-          const float x = score<MODE>(a, slope2, dot<DQ>(a.q + (bh * S + i) * DQ, kj),
-                                      fabsf((float)(i - j)), grad);
-          p = __builtin_amdgcn_exp2f(x - lse[bh * S + i]);
-          d = one ? 0.0f : p * (dot<DV>(gb + (int64_t)i * H * DV, vj) - delta[bh * S + i]) * grad;
-        }
-        __syncthreads();
-        ps[tid] = p;
-        ds[tid] = d;
-        vis[tid] = sees ? 1.0f : 0.0f;
-        __syncthreads();
-#pragma unroll 1
-        for (int q = c0; q < min(c0 + NTH, qz); ++q) {
-          if (vis[q - c0] == 0.0f) continue;
-          if (tid < DQ)
-            sk = __builtin_fmaf(ds[q - c0], st::bf16_to_f32(a.q[(bh * S + q) * DQ + tid]), sk);
-          if (tid < DV)
-            sv = __builtin_fmaf(ps[q - c0], st::bf16_to_f32(gb[(int64_t)q * H * DV + tid]), sv);
-        }
-      }
-    }
-    write(j, tid, sk * a.scale, sv);
+// N steps of 16 rows: a(i) the A operand of step i, b and lo its weights in one or
+// two parts
+template <int N, bool TWO, typename F>
+__device__ __forceinline__ void add_seen(f32x16& acc, F&& a, const bf16x8 (&b)[N], const bf16x8 (&lo)[N],
+                                         const Pairs& pairs) {
+  f32x16 count;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) count[e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    bf16x8 rest, kind;
+    part_kinds(a(i), rest, kind);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rest, b[i], acc, 0, 0, 0);
+    if constexpr (TWO) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rest, lo[i], acc, 0, 0, 0);
+    count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kind, pairs.kinds(i), count, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);  // one at a time: the first pass needs the registers
   }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] += of_kinds(count[e]);
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // ---------------------------------------------------------------- forward
@@ -615,16 +556,17 @@ __device__ void redo_dkdv(const Args& a, int b, int hk, int h0, int heads, int j
 // tokens (7 documents, 32/8 heads of 128): 88 us, 0.73 PFLOP/s of what the runs
 // need; 16384 tokens, window 4096, capped: 1068 us, 0.90 PFLOP/s; 2048 tokens and
 // 128 heads of 192/128: 98 us, 0.50 PFLOP/s.
-template <int DQ, int DV, int MODE>
-__global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__ out,
-                                                  float* __restrict__ lse) {
+// Returns whether the wave's sums are not finite (its rows are then not stored);
+// the careful pass stores the rows of waves with `again`.
+template <int DQ, int DV, int MODE, bool CAREFUL>
+__device__ __forceinline__ bool fwd_pass(const Args& a, uint16_t* lds, bool again,
+                                         uint16_t* __restrict__ out, float* __restrict__ lse) {
   constexpr int DS = DQ / 16, DB = DV / 32, LK = BKT * DQ, LV = BKT * DV;
   static_assert(4 * 32 * (DV + 8) <= 2 * (LK + LV), "output staging fits");
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * (LK + LV)];
-  const int S = a.S, H = a.H;
-  const int id = uniform(a.plan.qorder[blockIdx.x / H]), h = head_of(blockIdx.x % H, H, a.Hkv);
+  const int S = a.S, H = a.H, block = block_index<CAREFUL>();
+  const int id = uniform(a.plan.qorder[block / H]), h = head_of(block % H, H, a.Hkv);
   const int b = id / a.plan.nt, qt = id % a.plan.nt;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = thread_index<CAREFUL>(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c = lane & 31, hk = h / (H / a.Hkv);
   const uint16_t* qb = a.q + (int64_t)(b * H + h) * S * DQ;
@@ -635,11 +577,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
   const int2 run = myq < S ? run_of(a.lo, a.hi, (int64_t)b * S + myq, S) : make_int2(0, 0);
   const float slope2 = (MODE & BIAS) ? a.slopes[h] * LOG2E : 0.0f;
 
-  bf16x8 qf[DS];
-#pragma unroll
-  for (int s = 0; s < DS; ++s)
-    qf[s] = as_bf16x8(myq < S ? ld_global16(qb + (int64_t)myq * DQ + 16 * s + 8 * g)
-                              : make_uint4(0, 0, 0, 0));
+  Rows<DS, CAREFUL> qf(myq < S ? qb + (int64_t)myq * DQ + 8 * g : nullptr);
   f32x16 oacc[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i)
@@ -661,12 +599,13 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
   // the buffer is a constant of each half of the unrolled loop: LDS addresses
   // are then a lane's own and an offset within the instruction
   auto step = [&](int k0, auto which) {
-    constexpr int buf = decltype(which)::value;
+    const int buf = which;
     if (k0 + BKT < w.end) issue(k0 + BKT, buf ^ 1);
     const uint16_t* ks = lds + buf * (LK + LV);
     const uint16_t* vs = ks + LK;
     if (k0 < w.mine.w && k0 + BKT > w.mine.x) {  // some query of the wave sees some key
-      const bool edge = k0 < w.mine.y || k0 + BKT > w.mine.z;  // wave-uniform
+      const bool edge = CAREFUL || k0 < w.mine.y || k0 + BKT > w.mine.z;  // wave-uniform
+      qf.forget();
       f32x16 sacc[2];
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
@@ -678,7 +617,15 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
         for (int jb = 0; jb < 2; ++jb)
           sacc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DQ>(ks, lr, jb * 32, s),
                                                              qf[s], sacc[jb], 0, 0, 0);
-      fed<2 * DS, 2 * DS, LEAD, 1>();
+      if constexpr (!CAREFUL) fed<2 * DS, 2 * DS, LEAD, 1>();
+      if constexpr (CAREFUL && MODE == 0) {
+        // rounded before the maximum is taken off: of scores beyond 2^31 a fused
+        // product would leave more than an exponent holds
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sacc[jb][v] *= a.sl2;
+      }
       if constexpr ((MODE & CAP) != 0) {
         float top = 0.0f;
 #pragma unroll
@@ -729,7 +676,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
             sacc[jb][v] = (unsigned)(jb * 32 + (v >> 2) * 8 + (v & 3) - base) < width
                               ? sacc[jb][v] : -INFINITY;
       }
-      const float mul = MODE ? 1.0f : a.sl2;
+      const float mul = MODE || CAREFUL ? 1.0f : a.sl2;
       float mt = sacc[0][0];
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
@@ -749,6 +696,7 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
       }
       const float m_use = m_run == -INFINITY ? 0.0f : m_run;
       bf16x8 pf[4];
+      Pairs pairs;  // of the careful pass
 #pragma unroll
       for (int cc = 0; cc < 4; ++cc) {
         float p[8];
@@ -757,39 +705,73 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
           p[e] = __builtin_amdgcn_exp2f(
               __builtin_fmaf(sacc[cc >> 1][8 * (cc & 1) + e], mul, -m_use));
           l_run += p[e];
+          if constexpr (CAREFUL) {
+            const int v = 8 * (cc & 1) + e, key = k0 + (cc >> 1) * 32 + (v >> 2) * 8 + (v & 3) + 4 * g;
+            pairs.put(8 * cc + e, key >= run.x && key < run.y, p[e]);
+          }
         }
         pf[cc] = as_bf16x8(make_uint4(st::pack_bf16x2(p[0], p[1]), st::pack_bf16x2(p[2], p[3]),
                                       st::pack_bf16x2(p[4], p[5]), st::pack_bf16x2(p[6], p[7])));
       }
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc)
+      if constexpr (CAREFUL) {
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-          oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_tr<DV>(vs, lt, cc * 16, db),
-                                                             pf[cc], oacc[db], 0, 0, 0);
-      fed<8 * DB, 4 * DB, 2 * LEAD, 2>();
+          add_seen<4, false>(oacc[db], [&](int cc) { return read_tr<DV>(vs, lt, cc * 16, db); }, pf, pf,
+                             pairs);
+      } else {
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_tr<DV>(vs, lt, cc * 16, db), pf[cc],
+                                                               oacc[db], 0, 0, 0);
+        fed<8 * DB, 4 * DB, 2 * LEAD, 2>();
+      }
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   };
+  if constexpr (CAREFUL) {
+    int buf = 0;
 #pragma unroll 1
-  for (int k0 = w.first; k0 < w.end; k0 += 2 * BKT) {
-    step(k0, std::integral_constant<int, 0>{});
-    if (k0 + BKT < w.end) step(k0 + BKT, std::integral_constant<int, 1>{});
+    for (int k0 = w.first; k0 < w.end; k0 += BKT, buf ^= 1) step(k0, buf);
+  } else {
+#pragma unroll 1
+    for (int k0 = w.first; k0 < w.end; k0 += 2 * BKT) {
+      step(k0, std::integral_constant<int, 0>{});
+      if (k0 + BKT < w.end) step(k0 + BKT, std::integral_constant<int, 1>{});
+    }
   }
 
   const float l_tot = l_run + __shfl_xor(l_run, 32);
   const bool some = run.x < run.y;
-  const bool bad = __ballot(some && !(probe_of(oacc) == 0.0f && finite(l_tot) && l_tot > 0.0f)) != 0;
-  if (!bad) {
+  bool bad = false;
+  if constexpr (!CAREFUL)
+    bad = __ballot(some && !(probe_of(oacc) == 0.0f && finite(l_tot) && l_tot > 0.0f)) != 0;
+  if (CAREFUL ? again : !bad) {
     if (g == 0 && myq < S)
       lse[(int64_t)(b * H + h) * S + myq] = some ? m_run + log2f(l_tot) : INFINITY;
     store_rows<DV>(oacc, 1.0f / l_tot, some, lds + wave * 32 * (DV + 8), lane, S - q0,
                    out + ((int64_t)b * S + q0) * H * DV + (int64_t)h * DV, (int64_t)H * DV);
   }
-  redo<NT>(bad, wave, lane, (float*)lds, [&](int w, float* mem) {
-    redo_fwd<DQ, DV, MODE>(a, b, h, qt * TILE + w * 32, out, lse, mem);
-  });
+  return bad;
+}
+
+// (heads of 64 without a cap: the first pass runs four waves a SIMD, 72 us for 8192
+// packed tokens of 32/8 heads; with the registers that the careful one would like,
+// three and 77.)
+struct FwdCall {
+  Args a;
+  uint16_t* out;
+  float* lse;
+};
+template <int DQ, int DV, int MODE>
+__global__ __launch_bounds__(NT, DQ == 64 && !(MODE & CAP) ? 4 : 2) void span_fwd(FwdCall c) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * BKT * (DQ + DV)];
+  const bool bad = fwd_pass<DQ, DV, MODE, false>(c.a, lds, false, c.out, c.lse);
+  if (!any_wave<NT>(bad, (int*)lds)) return;
+  const FwdCall d = arguments_again<FwdCall>();
+  fwd_pass<DQ, DV, MODE, true>(d.a, lds, bad, d.out, d.lse);
 }
 
 // ---------------------------------------------------------------- backward
@@ -798,19 +780,18 @@ __global__ __launch_bounds__(NT, 2) void span_fwd(Args a, uint16_t* __restrict__
 // trace, 0.55 PFLOP/s, at its 8192 packed tokens, 193 us at its heads of 192/128.
 // Unrolled by two steps as the forward is, it spilled (495 us a training pass
 // against 467).
-template <int DQ, int DV, int MODE>
-__global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __restrict__ o,
-                                                     const uint16_t* __restrict__ dout,
-                                                     const float* __restrict__ lse,
-                                                     float* __restrict__ delta,
-                                                     uint16_t* __restrict__ dq) {
+template <int DQ, int DV, int MODE, bool CAREFUL>
+__device__ __forceinline__ bool dq_pass(const Args& a, uint16_t* lds, bool again,
+                                        const uint16_t* __restrict__ o,
+                                        const uint16_t* __restrict__ dout,
+                                        const float* __restrict__ lse, float* __restrict__ delta,
+                                        uint16_t* __restrict__ dq) {
   constexpr int DSQ = DQ / 16, DSV = DV / 16, DB = DQ / 32, LK = BKT * DQ, LV = BKT * DV;
   static_assert(4 * 32 * (DQ + 8) <= 2 * (LK + LV), "output staging fits");
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * (LK + LV)];
-  const int S = a.S, H = a.H;
-  const int id = uniform(a.plan.qorder[blockIdx.x / H]), h = head_of(blockIdx.x % H, H, a.Hkv);
+  const int S = a.S, H = a.H, block = block_index<CAREFUL>();
+  const int id = uniform(a.plan.qorder[block / H]), h = head_of(block % H, H, a.Hkv);
   const int b = id / a.plan.nt, qt = id % a.plan.nt;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = thread_index<CAREFUL>(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c = lane & 31, hk = h / (H / a.Hkv);
   const int64_t ldt = (int64_t)H * DV;
@@ -825,20 +806,15 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
   const int64_t srow = (int64_t)(b * H + h) * S;
   const int64_t trow = ((int64_t)b * S + myq) * ldt + (int64_t)h * DV;
 
-  bf16x8 qf[DSQ], dof[DSV];
+  Rows<DSQ, CAREFUL> qf(qok ? qb + (int64_t)myq * DQ + 8 * g : nullptr);
+  Rows<DSV, CAREFUL> dof(qok ? dout + trow + 8 * g : nullptr);
   const bool shortrow = w.end - w.first <= SHORT;  // uniform over the workgroup
   float dl = 0.0f;
-  const uint4 z = make_uint4(0, 0, 0, 0);
-#pragma unroll
-  for (int s = 0; s < DSQ; ++s)
-    qf[s] = as_bf16x8(qok ? ld_global16(qb + (int64_t)myq * DQ + 16 * s + 8 * g) : z);
 #pragma unroll
   for (int s = 0; s < DSV; ++s) {
-    const int d = 16 * s + 8 * g;
-    const uint4 gv = qok ? ld_global16(dout + trow + d) : z;
-    dof[s] = as_bf16x8(gv);
     if (shortrow) continue;
-    const uint4 ov = qok ? ld_global16(o + trow + d) : z;
+    const uint4 gv = __builtin_bit_cast(uint4, dof[s]);
+    const uint4 ov = qok ? ld_global16(o + trow + 16 * s + 8 * g) : make_uint4(0, 0, 0, 0);
     const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, ow[4] = {ov.x, ov.y, ov.z, ov.w};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -881,7 +857,7 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
     for (int jb = 0; jb < 2; ++jb) {
       const int kb0 = k0 + jb * 32;
       if (kb0 >= w.mine.w || kb0 + 32 <= w.mine.x) continue;  // wave-uniform
-      const bool edge = kb0 < w.mine.y || kb0 + 32 > w.mine.z;
+      const bool edge = CAREFUL || kb0 < w.mine.y || kb0 + 32 > w.mine.z;
       // an edge keeps the offsets of the lane's run (of more than one key, or
       // dS is 0), other blocks keep all
       const int base = edge ? run.x - kb0 - 4 * g : 0;
@@ -890,16 +866,19 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
       f32x16 sacc, pacc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) { sacc[e] = 0.0f; pacc[e] = 0.0f; }
+      qf.forget();
+      dof.forget();
 #pragma unroll
       for (int s = 0; s < DSQ; ++s) {
         sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DQ>(ks, lrq, jb * 32, s), qf[s],
                                                        sacc, 0, 0, 0);
         if (s < DSV)
           pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_row<DV>(vs, lrv, jb * 32, s),
-                                                         dof[s < DSV ? s : 0], pacc, 0, 0, 0);
+                                                         dof[s], pacc, 0, 0, 0);
       }
-      if constexpr (DQ != 192) fed<DSQ + DSV, DSQ + DSV, LEAD, 1>();
+      if constexpr (DQ != 192 && !CAREFUL) fed<DSQ + DSV, DSQ + DSV, LEAD, 1>();
       bf16x8 dsf[2], dsl[2];
+      Pairs pairs;  // of the careful pass
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         float ds[8];
@@ -907,7 +886,7 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
         for (int e = 0; e < 8; ++e) {
           const int vv = 8 * hh + e, ro = (vv >> 2) * 8 + (vv & 3);
           float p, grad = 1.0f;
-          if constexpr (MODE != 0)
+          if constexpr (MODE != 0 || CAREFUL)
             p = __builtin_amdgcn_exp2f(
                 score<MODE>(a, slope2, sacc[vv], fabsf(far0 - (float)ro), grad) - lq);
           else
@@ -917,10 +896,22 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
           const float kept = (unsigned)(ro - base) < width ? d : 0.0f;
           if (only_delta) dl += kept;
           ds[e] = MODE ? kept * grad : kept;
+          if constexpr (CAREFUL) {
+            const bool sees = (unsigned)(ro - base) < width;
+            if (!sees) ds[e] = 0.0f;  // not 0 times a masked pair's slope
+            pairs.put(vv, sees, ds[e]);
+          }
         }
         split8(ds, dsf[hh], dsl[hh]);
       }
       if (only_delta) continue;
+      if constexpr (CAREFUL) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          add_seen<2, true>(dqacc[db], [&](int hh) { return read_tr<DQ>(ks, lt, jb * 32 + 16 * hh, db); },
+                            dsf, dsl, pairs);
+        continue;
+      }
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         // operands in registers at once; at DQ = 192 all six, or reads ordered
@@ -942,22 +933,37 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(Args a, const uint16_t* __r
                 __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktr[e], dsl[hh], dqacc[d0 + e], 0, 0, 0);
         }
       }
-      if constexpr (DQ != 192) fed<4 * DB, 4 * DB, 6, 2>();
+      if constexpr (DQ != 192 && !CAREFUL) fed<4 * DB, 4 * DB, 6, 2>();
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }
   if (only_delta) dl += __shfl_xor(dl, 32);
   }
-  if (g == 0 && qok) delta[srow + myq] = dl;
+  if (g == 0 && qok && (!CAREFUL || again)) delta[srow + myq] = dl;
   const bool some = run.x < run.y;
-  const bool bad = __ballot(some && probe_of(dqacc) != 0.0f) != 0;
-  if (!bad)
+  bool bad = false;
+  if constexpr (!CAREFUL) bad = __ballot(some && probe_of(dqacc) != 0.0f) != 0;
+  if (CAREFUL ? again : !bad)
     store_rows<DQ>(dqacc, a.scale, some, lds + wave * 32 * (DQ + 8), lane, S - q0,
                    dq + (srow + q0) * DQ, DQ);
-  redo<NT>(bad, wave, lane, (float*)lds, [&](int w, float* mem) {
-    redo_dq<DQ, DV, MODE>(a, b, h, qt * TILE + w * 32, dout, lse, delta, dq, mem);
-  });
+  return bad;
+}
+
+struct DqCall {
+  Args a;
+  const uint16_t *o, *dout;
+  const float* lse;
+  float* delta;
+  uint16_t* dq;
+};
+template <int DQ, int DV, int MODE>
+__global__ __launch_bounds__(NT, 2) void span_bwd_dq(DqCall c) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * BKT * (DQ + DV)];
+  const bool bad = dq_pass<DQ, DV, MODE, false>(c.a, lds, false, c.o, c.dout, c.lse, c.delta, c.dq);
+  if (!any_wave<NT>(bad, (int*)lds)) return;
+  const DqCall d = arguments_again<DqCall>();
+  dq_pass<DQ, DV, MODE, true>(d.a, lds, bad, d.o, d.dout, d.lse, d.delta, d.dq);
 }
 
 // dK, dV of a 128-key tile of one KV head over the query heads of one part of
@@ -1005,32 +1011,40 @@ constexpr int dkdv_lds() {
   return dkdv_waves<DQ>() == 4 ? rows : tiles > sums ? tiles : sums;
 }
 
-template <int DQ, int DV, int MODE>
-__global__ __launch_bounds__(64 * dkdv_waves<DQ>(), dkdv_waves<DQ>() == 8 ? 2 : 1)
-void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __restrict__ lse,
-                   const float* __restrict__ delta, int most, float* __restrict__ dk_part,
-                   float* __restrict__ dv_part, uint16_t* __restrict__ dk,
-                   uint16_t* __restrict__ dv) {
+// (arrays of their own: a read of one is not taken for a read of what the copies
+// into another still write, and does not wait for them)
+template <int DQ, int DV>
+struct DkdvTiles {
+  uint16_t *lds, *q_a, *q_b, *g_a, *g_b;
+  float (*lse)[QT], (*dl)[QT];
+  int (*lo)[QT], (*wd)[QT];
+};
+
+template <int DQ, int DV, int MODE, bool CAREFUL>
+__device__ __forceinline__ bool dkdv_pass(const Args& a, const DkdvTiles<DQ, DV>& tiles, bool again,
+                                          const uint16_t* __restrict__ dout,
+                                          const float* __restrict__ lse,
+                                          const float* __restrict__ delta, int most,
+                                          float* __restrict__ dk_part, float* __restrict__ dv_part,
+                                          uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
   constexpr int DSQ = DQ / 16, DSV = DV / 16, DBQ = DQ / 32, DBV = DV / 32;
-  constexpr int LK = TILE * DQ, LV = TILE * DV, LQ = QT * DQ, LG = QT * DV;
+  constexpr int LK = TILE * DQ, LQ = QT * DQ, LG = QT * DV;
   constexpr int NW = dkdv_waves<DQ>(), NTH = 64 * NW, QH = 8 / NW;
   constexpr bool KREG = NW == 4;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[dkdv_lds<DQ, DV>()];
-  // arrays of their own: a read of one is not taken for a read of what the copies
-  // into another still write, and does not wait for them
-  __shared__ __attribute__((aligned(16))) uint16_t q_a[LQ], q_b[LQ], g_a[LG], g_b[LG];
-  __shared__ __attribute__((aligned(16))) float lse_s[2][QT], dl_s[2][QT];
-  __shared__ __attribute__((aligned(16))) int lo_s[2][QT], wd_s[2][QT];
+  uint16_t *lds = tiles.lds, *q_a = tiles.q_a, *q_b = tiles.q_b, *g_a = tiles.g_a, *g_b = tiles.g_b;
+  float (*lse_s)[QT] = tiles.lse, (*dl_s)[QT] = tiles.dl;
+  int (*lo_s)[QT] = tiles.lo, (*wd_s)[QT] = tiles.wd;
   const int S = a.S, H = a.H, nb = a.plan.nb, group = H / a.Hkv;
   // an XCD's shader engines take its workgroups in turn: the parts that a tile
   // does not have are rotated from tile to tile, or one engine got all the work
-  const int slot = blockIdx.x / (a.Hkv * most), rest = blockIdx.x % (a.Hkv * most);
+  const int block = block_index<CAREFUL>();
+  const int slot = block / (a.Hkv * most), rest = block % (a.Hkv * most);
   const int id = uniform(a.plan.korder[slot]), hk = rest % a.Hkv;
   const int part = (rest / a.Hkv + slot) % most;
   const int parts = parts_of(a.plan, id, group, a.Hkv, most);
-  if (part >= parts) return;
+  if (part >= parts) return false;
   const int b = id / a.plan.nt, kt = id % a.plan.nt;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = thread_index<CAREFUL>(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c = lane & 31;
   const int kq = wave & 3, qh0 = NW == 8 ? wave >> 2 : 0;
@@ -1045,16 +1059,9 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   const int4* blk = a.plan.blk + (int64_t)b * nb;
   const uint32_t lrq = lane_row<DQ>(c, g), lrv = lane_row<DV>(c, g);
   const uint32_t ltq = lane_tr<DQ>(lane), ltv = lane_tr<DV>(lane);
-  bf16x8 kfr[KREG ? DSQ : 1], vfr[KREG ? DSV : 1];
-  if constexpr (KREG) {
-    const uint4 z = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int s = 0; s < DSQ; ++s)
-      kfr[s] = as_bf16x8(mykey < S ? ld_global16(kb + (int64_t)mykey * DQ + 16 * s + 8 * g) : z);
-#pragma unroll
-    for (int s = 0; s < DSV; ++s)
-      vfr[s] = as_bf16x8(mykey < S ? ld_global16(vb + (int64_t)mykey * DV + 16 * s + 8 * g) : z);
-  } else {
+  Rows<KREG ? DSQ : 0, CAREFUL> kfr(KREG && mykey < S ? kb + (int64_t)mykey * DQ + 8 * g : nullptr);
+  Rows<KREG ? DSV : 0, CAREFUL> vfr(KREG && mykey < S ? vb + (int64_t)mykey * DV + 8 * g : nullptr);
+  if constexpr (!KREG) {
     const TileCopy<DQ, NTH, TILE> ck(tid, DQ);
     const TileCopy<DV, NTH, TILE> cv(tid, DV);
     ck(kb, DQ, k0, S, Ks, wave);
@@ -1092,7 +1099,7 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
   // FOLD: the accumulators of S and dP start from -lse / sl2 and -delta of their
   // rows, read from LDS as they lie, so the statistics take no registers of their
   // own and no instruction (a cap needs the bare product)
-  constexpr bool FOLD = (MODE & CAP) == 0;
+  constexpr bool FOLD = (MODE & CAP) == 0 && !CAREFUL;
   const float over = 1.0f / a.sl2;
   auto stats = [&](int buf) {
     if (tid < QT) {
@@ -1127,7 +1134,7 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
       const int qw0 = q0 + qh * 32;  // this wave's queries
       const int4 x = qw0 < S ? extremes(blk + (qw0 >> 5)) : make_int4(INT_MAX, INT_MAX, 0, 0);
       if (kw0 < x.w && kw0 + 32 > x.x) {  // some query sees some key
-        const bool edge = kw0 < x.y || kw0 + 32 > x.z;
+        const bool edge = CAREFUL || kw0 < x.y || kw0 + 32 > x.z;
         const float far0 = (float)(qw0 + 4 * g - mykey);
         // this wave's rows of the tiles, through its lane addresses
         const uint32_t q_row = lrq + qh * 32 * DQ * 2, g_row = lrv + qh * 32 * DV * 2;
@@ -1135,6 +1142,8 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
         const uint32_t k_row = lrq + kq * 32 * DQ * 2, v_row = lrv + kq * 32 * DV * 2;
         const int r0 = qh * 32 + g * 4;
         f32x16 sacc, pacc;
+        kfr.forget();
+        vfr.forget();
 #pragma unroll
         for (int v4 = 0; v4 < 4; ++v4) {
           const float4 l = lds4(&lse_s[buf][r0 + 8 * v4]);
@@ -1150,14 +1159,16 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
         for (int s = 0; s < DSQ; ++s) {
           sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               read_row<DQ>(qs, q_row, 0, s),
-              KREG ? kfr[KREG ? s : 0] : read_row<DQ>(Ks, k_row, 0, s), sacc, 0, 0, 0);
+              KREG ? kfr[s] : read_row<DQ>(Ks, k_row, 0, s), sacc, 0, 0, 0);
           if (s < DSV)
             pacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 read_row<DV>(gs, g_row, 0, s),
-                KREG ? vfr[KREG && s < DSV ? s : 0] : read_row<DV>(Vs, v_row, 0, s), pacc, 0, 0, 0);
+                KREG ? vfr[s] : read_row<DV>(Vs, v_row, 0, s), pacc, 0, 0, 0);
         }
-        fed<8 + (KREG ? 1 : 2) * (DSQ + DSV), DSQ + DSV, 8 + (KREG ? 4 : 6), KREG ? 1 : 2>();
+        if constexpr (!CAREFUL)
+          fed<8 + (KREG ? 1 : 2) * (DSQ + DSV), DSQ + DSV, 8 + (KREG ? 4 : 6), KREG ? 1 : 2>();
         bf16x8 pf[2], dsf[2], dsl[2];
+        Pairs pairs_p, pairs_d;  // of the careful pass
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           float p8[8], d8[8];
@@ -1184,10 +1195,25 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
               const bool keep = (unsigned)(mykey - lds1(&lo_s[buf][r])) < (unsigned)width;
               p8[e] = keep ? p8[e] : 0.0f;
               d8[e] = keep && width > 1 ? d8[e] : 0.0f;
+              if constexpr (CAREFUL) {
+                pairs_p.put(vv, keep, p8[e]);
+                pairs_d.put(vv, keep && width > 1, d8[e]);
+              }
             }
           }
           pf[hh] = pack8(p8);
           split8(d8, dsf[hh], dsl[hh]);
+        }
+        if constexpr (CAREFUL) {
+#pragma unroll
+          for (int db = 0; db < DBV; ++db)
+            add_seen<2, false>(dvacc[db], [&](int hh) { return read_tr<DV>(gs, g_tr, 16 * hh, db); }, pf, pf,
+                               pairs_p);
+#pragma unroll
+          for (int db = 0; db < DBQ; ++db)
+            add_seen<2, true>(dkacc[db], [&](int hh) { return read_tr<DQ>(qs, q_tr, 16 * hh, db); }, dsf, dsl,
+                              pairs_d);
+          continue;
         }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -1210,7 +1236,7 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
                   __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtr[e], dsl[hh], dkacc[db + e], 0, 0, 0);
           }
         }
-        fed<4 * (DBV + DBQ), 2 * DBV + 4 * DBQ, 6, 2>();
+        if constexpr (!CAREFUL) fed<4 * (DBV + DBQ), 2 * DBV + 4 * DBQ, 6, 2>();
       }
     }
     if (n + 1 < steps) stats(buf ^ 1);
@@ -1246,11 +1272,12 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
     meet(dvacc, std::integral_constant<int, DBV>{});
     meet(dkacc, std::integral_constant<int, DBQ>{});
   }
-  const bool bad =
-      __ballot(qh0 == 0 && mykey < S && probe_of(dvacc) + probe_of(dkacc) != 0.0f) != 0;
+  bool bad = false;
+  if constexpr (!CAREFUL)
+    bad = __ballot(qh0 == 0 && mykey < S && probe_of(dvacc) + probe_of(dkacc) != 0.0f) != 0;
   const int64_t krow = (int64_t)(b * a.Hkv + hk) * S;                  // of dk, dv
   const int64_t prow = ((int64_t)(b * a.Hkv + hk) * most + part) * S;  // of the partials
-  if (qh0 == 0 && !bad && kw0 < S) {
+  if (qh0 == 0 && (CAREFUL ? again : !bad) && kw0 < S) {
     // staged by each wave in its own LDS space
     uint16_t* os = lds + kq * (dkdv_lds<DQ, DV>() / 4);
     static_assert(32 * (DQ + 8) <= dkdv_lds<DQ, DV>() / 4 && 32 * (DV + 8) <= dkdv_lds<DQ, DV>() / 4,
@@ -1279,18 +1306,31 @@ void span_bwd_dkdv(Args a, const uint16_t* __restrict__ dout, const float* __res
       }
     }
   }
-  redo<NTH>(bad, wave, lane, (float*)lds, [&](int w, float* mem) {
-    redo_dkdv<DQ, DV, MODE, NTH>(a, b, hk, h0, heads, k0 + (w & 3) * 32, seen, dout, lse, delta, mem,
-                                 [&](int key, int d, float sk, float sv) {
-      if (parts == 1) {
-        if (d < DQ) dk[(krow + key) * DQ + d] = st::f32_to_bf16(sk);
-        if (d < DV) dv[(krow + key) * DV + d] = st::f32_to_bf16(sv);
-      } else {
-        if (d < DQ) dk_part[(prow + key) * DQ + d] = sk;
-        if (d < DV) dv_part[(prow + key) * DV + d] = sv;
-      }
-    });
-  });
+  return bad;
+}
+
+struct DkdvCall {
+  Args a;
+  const uint16_t* dout;
+  const float *lse, *delta;
+  int most;
+  float *dk_part, *dv_part;
+  uint16_t *dk, *dv;
+};
+template <int DQ, int DV, int MODE>
+__global__ __launch_bounds__(64 * dkdv_waves<DQ>(), dkdv_waves<DQ>() == 8 ? 2 : 1)
+void span_bwd_dkdv(DkdvCall c) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[dkdv_lds<DQ, DV>()];
+  __shared__ __attribute__((aligned(16))) uint16_t q_a[QT * DQ], q_b[QT * DQ], g_a[QT * DV], g_b[QT * DV];
+  __shared__ __attribute__((aligned(16))) float lse_s[2][QT], dl_s[2][QT];
+  __shared__ __attribute__((aligned(16))) int lo_s[2][QT], wd_s[2][QT];
+  const DkdvTiles<DQ, DV> tiles{lds, q_a, q_b, g_a, g_b, lse_s, dl_s, lo_s, wd_s};
+  const bool bad = dkdv_pass<DQ, DV, MODE, false>(c.a, tiles, false, c.dout, c.lse, c.delta, c.most,
+                                                  c.dk_part, c.dv_part, c.dk, c.dv);
+  if (!any_wave<64 * dkdv_waves<DQ>()>(bad, (int*)lds)) return;
+  const DkdvCall d = arguments_again<DkdvCall>();
+  dkdv_pass<DQ, DV, MODE, true>(d.a, tiles, bad, d.dout, d.lse, d.delta, d.most, d.dk_part, d.dv_part, d.dk,
+                                d.dv);
 }
 
 // dk = bf16(sum over the parts, in order), same for dv, of the tiles in parts
@@ -1415,7 +1455,7 @@ int fits(const char* name, int64_t groups, int64_t threads) {
 template <int DQ, int DV, int MODE>
 int run_fwd(const Args& a, int64_t B, uint16_t* out, float* lse, hipStream_t s) {
   if (int rc = fits("st_span_attn_fwd", B * a.plan.nt * a.H, NT)) return rc;
-  span_fwd<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, lse);
+  span_fwd<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>({a, out, lse});
   return st::check_launch("span_fwd");
 }
 
@@ -1430,11 +1470,11 @@ int run_bwd(const Args& a, int64_t B, const uint16_t* out, const float* lse, con
   if (int rc = fits("st_span_attn_bwd", B * a.plan.nt * a.H, NT)) return rc;
   if (int rc = fits("st_span_attn_bwd", tiles * sp.most, NTH)) return rc;
   if (int rc = fits("st_span_attn_bwd", sp.most > 1 ? tiles : 0, NT)) return rc;
-  span_bwd_dq<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(a, out, dout, lse, delta,
-                                                                          dq);
+  span_bwd_dq<DQ, DV, MODE><<<(unsigned)(B * a.plan.nt * a.H), NT, 0, s>>>(
+      {a, out, dout, lse, delta, dq});
   if (int rc = st::check_launch("span_bwd_dq")) return rc;
   span_bwd_dkdv<DQ, DV, MODE><<<(unsigned)(tiles * sp.most), NTH, 0, s>>>(
-      a, dout, lse, delta, sp.most, dkp, dvp, dk, dv);
+      {a, dout, lse, delta, sp.most, dkp, dvp, dk, dv});
   int rc = st::check_launch("span_bwd_dkdv");
   if (rc || sp.most == 1) return rc;
   span_reduce<<<dim3((unsigned)tiles, 8), NT, 0, s>>>(a.plan, dkp, dvp, a.H / a.Hkv, a.Hkv, sp.most, a.S,
