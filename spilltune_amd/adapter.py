@@ -168,8 +168,11 @@ class ArchiveDenseAdapter:
         return rot, {"full_attention": mask}
 
     def packed_positions_and_masks(self, documents, **kw):
-        """Positions and masks of packed rows (packed.positions_and_masks)."""
-        if documents.ndim != 2 or documents.shape[1] > self.config["max_positions"]:
+        """Positions and masks of packed rows (packed.positions_and_masks); the
+        configured context bounds each document, not the row."""
+        if documents.ndim != 2 or (
+                documents.shape[1] > self.config["max_positions"]
+                and int(packed.document_runs(documents)[2].max()) >= self.config["max_positions"]):
             raise ValueError("unsupported_capability: sequence beyond configured context")
         if self._rotary is None:
             self._rotary = packed.Rotary(self.config["head_dim"], self.config["theta"],

@@ -67,3 +67,16 @@ def test_packed_rows_leave_a_plain_models_tables():
     model.packed_positions_and_masks(torch.zeros(1, 8, dtype=torch.int64))
     rot, _ = model.positions_and_masks(torch.ones(1, 8, dtype=torch.bool))
     assert isinstance(rot, tuple)
+
+
+def test_an_adapters_context_bounds_documents_not_rows():
+    from spilltune_amd.adapter import ArchiveDenseAdapter
+    adapter = object.__new__(ArchiveDenseAdapter)  # nothing below needs an archive or a GPU
+    adapter.config = {"max_positions": 8, "head_dim": 64, "theta": 1e4}
+    adapter.device, adapter._rotary = torch.device("cpu"), None
+    docs = torch.tensor([[0] * 8 + [1] * 5 + [-1] * 4])
+    with pytest.raises(ValueError, match="must be on the GPU"):  # past the context check
+        adapter.packed_positions_and_masks(docs)
+    for bad in (torch.tensor([[0] * 9 + [1] * 3]), torch.zeros(9, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="beyond configured context"):
+            adapter.packed_positions_and_masks(bad)
