@@ -21,7 +21,7 @@ another implementation.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 
@@ -33,7 +33,7 @@ _F32 = torch.float32
 
 
 # ----------------------------------------------------------------- masks
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)  # equal to itself alone: sizes do not make a mask
 class SpanMask:
     """Query ``i`` of row ``b`` sees the keys ``[key_start[b, i], key_end[b, i])``
     (int32 [batch, length]); an empty run sees nothing.  ``positions`` (int32) is
@@ -41,10 +41,10 @@ class SpanMask:
     runs: the tensors belong together and are not to be changed."""
     batch: int
     length: int
-    key_start: torch.Tensor = field(compare=False)
-    key_end: torch.Tensor = field(compare=False)
-    positions: torch.Tensor = field(compare=False)
-    plan: torch.Tensor = field(compare=False)
+    key_start: torch.Tensor
+    key_end: torch.Tensor
+    positions: torch.Tensor
+    plan: torch.Tensor
 
 
 def span_mask(key_start: torch.Tensor, key_end: torch.Tensor, positions=None) -> SpanMask:
@@ -379,13 +379,13 @@ def rope_positions(y, positions, rotary: Rotary, heads: int, kv_heads: int, *, n
 
 
 # ----------------------------------------------------------------- a model's packed rows
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Positions:
     """Position embeddings of packed rows for a decoder block: per-token
     positions (int32 [batch, length]) and the rotary embedding they turn by, in
     the place of (cos, sin) tables."""
-    positions: torch.Tensor = field(compare=False)
-    rotary: Rotary = field(compare=False)
+    positions: torch.Tensor
+    rotary: Rotary
 
 
 def positions_and_masks(documents: torch.Tensor, rotary: Rotary, *, bidirectional=None, window=None):
