@@ -446,7 +446,8 @@ int st_mla_attn_bwd(const uint16_t* q, const uint16_t* k, const uint16_t* v,
  * A query with an empty run has out = 0, lse = +inf and a zero dq, whatever its
  * rows hold; infinities and NaN in rows that a query does not see do not reach
  * it.  scale within 1e-30 .. 1e30, cap up to 1e30 and at least scale / 1e4.
- * Deterministic: no atomics.
+ * Deterministic: no atomics.  The backward's workspace holds 4 bytes a query and
+ * head, and where key tiles can be split 4 B H S (DQ + DV) bytes of partial sums.
  * `plan`: st_span_plan's tables of the same key_start and key_end, made once
  * per mask and read by every call (st_span_plan_bytes(B, S), 16-byte aligned);
  * it belongs to that mask alone.
@@ -495,8 +496,9 @@ int st_cross_entropy_rows(uint16_t* logits, int64_t rows, int64_t vocab, int64_t
 
 /* ---------------------------------------------------------------------
  * Log probabilities of given tokens under the frozen vocabulary head, with
- * entropy and top alternatives; no logits of all rows are kept.  The reference
- * has the summed cross-entropy only (native_terminal.py:11-47).
+ * entropy and top alternatives.  Without alternatives and without `logits` no
+ * logit is written.  The reference has the summed cross-entropy only
+ * (native_terminal.py:11-47).
  *   l = hidden head^T (bf16 products, fp32 sums),
  *   x = (cap > 0 ? cap * tanh(l / cap) : l) / temperature,
  *   logprobs[r] = x[tokens[r]] - lse[r] (0 where tokens[r] == ignore_index, NaN

@@ -8,7 +8,7 @@
 //   dl = dx (1 - tanh^2) / temperature,  dhidden = dl head
 //
 // Forward: one pass over the head.  The GEMM's tiles (bf16 products, fp32 sums)
-// never leave registers: each tile of 256 vocabulary columns reduces its x to
+// are reduced in registers: each tile of 256 vocabulary columns reduces its x to
 // (max, sum of e^(x - max), sum of e^(x - max) (x - max)) per row, and a second
 // kernel joins the tiles.  All three are kept relative to the maximum, so
 // nothing cancels: the entropy is log(sum) less a sum of terms below zero.

@@ -776,8 +776,8 @@ __global__ __launch_bounds__(NT, DQ == 64 && !(MODE & CAP) ? 4 : 2) void span_fw
 
 // ---------------------------------------------------------------- backward
 // dQ (and delta) of a 128-query tile: S^T and dP^T = V dO^T as in the forward,
-// dQ^T += K^T dS^T.  Bound as the forward (MFMA pipes 43% busy): 176 us in a
-// trace, 0.55 PFLOP/s, at its 8192 packed tokens, 193 us at its heads of 192/128.
+// dQ^T += K^T dS^T.  Bound as the forward (MFMA pipes 44% busy): 174 us in a
+// trace, 0.55 PFLOP/s, at its 8192 packed tokens, 191 us at its heads of 192/128.
 // Unrolled by two steps as the forward is, it spilled (495 us a training pass
 // against 467).
 template <int DQ, int DV, int MODE, bool CAREFUL>
@@ -980,8 +980,8 @@ __global__ __launch_bounds__(NT, 2) void span_bwd_dq(DqCall c) {
 // (parts_of), and span_reduce adds their fp32 sums in order.
 // Bound as the forward for DQ <= 128 (MFMA pipes 43% busy): 226 us in a trace,
 // 0.57 PFLOP/s, at its 8192 packed tokens.  DQ = 192 has one wave a SIMD and one
-// workgroup a CU, so nothing covers a tile's start and end (MFMA pipes 23% busy):
-// 280 us, 0.35 PFLOP/s (both query halves in one run of instructions took as long).
+// workgroup a CU, so nothing covers a tile's start and end (MFMA pipes 24% busy):
+// 273 us, 0.36 PFLOP/s (both query halves in one run of instructions took as long).
 // A tile stays whole up to a CU's share of all work (256 CUs) or 16 steps (of 2
 // blocks each); a heavier one is split, by a divisor of the group, into parts of
 // at most three quarters of a share.  Training pass in us, against parts of at

@@ -173,7 +173,10 @@ def span_attention(q, k, v, scale, mask: SpanMask, *, cap=None, slopes=None):
     in ``mask``.  Scores are ``scale * q.k``, with ``cap`` ``cap * tanh(scale * q.k
     / cap)``; ``slopes`` (fp32 [H], constants) subtracts ``slopes[h] * |i - j|``.
     (``scale`` 1e-30 to 1e30, ``cap`` up to 1e30 and at least ``scale / 1e4``.)
-    A query that sees nothing gets zeros and passes no gradient on."""
+    A query that sees nothing gets zeros and passes no gradient on.  Infinities and
+    NaN reach what sees them and nothing else.  The gradients form the
+    probabilities again from scores and their log-sum-exp in fp32: off by 2^-24 of
+    the scores' size."""
     if not isinstance(mask, SpanMask):
         raise ValueError("unsupported_capability: span_attention needs a SpanMask")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or any(t.dtype != _BF16 for t in (q, k, v)):
