@@ -286,7 +286,7 @@ class DenseModel:
         self.head = head.to(torch.bfloat16).to(self.device)
         self.eps, self.theta, self.head_dim = eps, theta, head_dim
         self.rotary = rotary
-        self._packed_rotary = rotary  # without one: made on the first packed rows
+        self._plain = None  # of packed rows without one, made on their first use
         if (layers is None) == (blocks is None):
             raise ValueError("DenseModel needs exactly one of layers / blocks")
         self.blocks = list(blocks) if blocks is not None else [
@@ -303,9 +303,12 @@ class DenseModel:
 
     def packed_positions_and_masks(self, documents, **kw):
         """Positions and masks of packed rows (packed.positions_and_masks)."""
-        if self._packed_rotary is None:
-            self._packed_rotary = packed.Rotary(self.head_dim, self.theta, device=self.device)
-        positions, mask = packed.positions_and_masks(documents, self._packed_rotary, **kw)
+        rotary = self.rotary
+        if rotary is None:
+            if self._plain is None:
+                self._plain = packed.Rotary(self.head_dim, self.theta, device=self.device)
+            rotary = self._plain
+        positions, mask = packed.positions_and_masks(documents, rotary, **kw)
         return positions, {"full_attention": mask}
 
     def terminal_norm(self, hidden):

@@ -80,3 +80,15 @@ def test_an_adapters_context_bounds_documents_not_rows():
     for bad in (torch.tensor([[0] * 9 + [1] * 3]), torch.zeros(9, dtype=torch.int64)):
         with pytest.raises(ValueError, match="beyond configured context"):
             adapter.packed_positions_and_masks(bad)
+
+
+def test_a_rotary_given_later_turns_both(monkeypatch):
+    model = _plain(None)
+    monkeypatch.setattr(packed, "positions_and_masks", lambda documents, rotary, **kw: (rotary, None))
+    docs, valid = torch.zeros(1, 4, dtype=torch.int64), torch.ones(1, 4, dtype=torch.bool)
+    first, _ = model.packed_positions_and_masks(docs)
+    assert first.rotary_dim == 64 and model.packed_positions_and_masks(docs)[0] is first
+    assert isinstance(model.positions_and_masks(valid)[0], tuple)
+    model.rotary = packed.Rotary(64, 1e4, rotary_dim=32, device="cpu")
+    assert model.packed_positions_and_masks(docs)[0] is model.rotary
+    assert model.positions_and_masks(valid)[0].rotary is model.rotary
