@@ -477,11 +477,11 @@ struct Rows {
 };
 
 // acc += A B over the seen pairs of a block, where A's rows may hold infinities and
-// NaN, B's weights of masked pairs are 0.  Those are taken out of A, which leaves every pair's
-// product finite, and what they make of a sum is found by a second product: of
-// their kind (+inf 1, -inf 2^10, NaN 2^20) with 1 for a seen pair, 2^20 for one of
-// weight 0 (0 * inf), 0 for a masked one.  At most 64 pairs meet, so the kinds do
-// not run into each other.
+// NaN; B's weights of masked pairs are 0.  The infinities and NaN are taken out of
+// A, so a masked pair adds 0, and what they make of a sum is found by a second
+// product: of their kind (+inf 1, -inf 2^10, NaN 2^20) with 1 for a seen pair,
+// 2^20 for one of weight 0 (0 * inf), 0 for a masked one.  At most 64 pairs meet,
+// so the kinds do not run into each other.
 constexpr uint32_t ONE = 0x3f80, NEG = 0x4480, NAN20 = 0x4980;  // bf16 1, 2^10, 2^20
 __device__ __forceinline__ void part_kinds(bf16x8 x, bf16x8& rest, bf16x8& kind) {
   uint4 w = __builtin_bit_cast(uint4, x), k;
