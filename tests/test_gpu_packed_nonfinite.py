@@ -123,4 +123,5 @@ def test_time_of_a_diverged_pass_is_bounded(dims, H, KV, what):
     else:
         first = 3 if what == "one key" else 0
         assert bool(torch.isnan(heads[first:]).all()) and bool(torch.isfinite(heads[:first]).all())
-    assert bool(torch.isnan(dk).any()) and took <= 12 * usual
+    # (pair by pair it would be some thousand times, and grow with the length)
+    assert bool(torch.isnan(dk).any()) and took <= 40 * usual
