@@ -636,6 +636,26 @@ int st_moe_lora_grads(int64_t rows, int32_t R, int64_t seg_len, int32_t nseg,
                       int32_t groups, float alpha, float* out, int64_t o_gstride, int64_t so_m,
                       int64_t so_j, int32_t accumulate, st_stream_t stream);
 
+/* ---------------------------------------------------------------- updates */
+/*
+ * Orthogonalised updates (no counterpart in the reference): for every matrix U of
+ * `count` row-major [rows, cols] ones back to back at `x`, X = U / (|U|_F + eps)
+ * and `steps` times X <- aX + (b XX' + c (XX')^2) X on its shorter side (at most
+ * 1024), written to `out` in the same layout.  x and out bf16 or fp32 (`dtype`),
+ * all sums in 64 bits; out may not overlap any x.  |a|^(2 steps) <= 1e13, which
+ * bounds the growth of what 64 bits round.  A matrix with a value that is not
+ * finite gives NaN throughout.  `table` is a host array read during the call.
+ */
+typedef struct st_matrix_batch {
+  const void* x;
+  void* out;
+  int64_t count, rows, cols;
+} st_matrix_batch;
+int64_t st_orthogonalize_workspace_bytes(int32_t n, const st_matrix_batch* table);
+int st_orthogonalize(int32_t n, const st_matrix_batch* table, int32_t dtype, int32_t steps,
+                     double a, double b, double c, double eps, void* workspace,
+                     int64_t workspace_bytes, st_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,6 +119,8 @@ _SIGNATURES = {
                                      _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "st_token_logprobs_bwd": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _F, _F, _I64,
                                      _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P]),
+    "st_orthogonalize_workspace_bytes": (_I64, [_I32, _P]),
+    "st_orthogonalize": (_I32, [_I32, _P, _I32, _I32, _D, _D, _D, _D, _P, _I64, _P]),
     "st_cross_entropy_rows": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _F, _P, _P]),
     "st_moe_lora_grads": (_I32, [_I64, _I32, _I64, _I32, _P, _I64, _I64, _P, _P, _I64, _I64, _P,
                                  _I32, _F, _P, _I64, _I64, _I64, _I32, _P]),
@@ -217,6 +219,12 @@ class RkProduct(ctypes.Structure):
                 ("big", ctypes.c_int64), ("r", ctypes.c_int64), ("Kc", ctypes.c_int64),
                 ("alpha", ctypes.c_float), ("out", ctypes.c_void_p), ("so_m", ctypes.c_int64),
                 ("so_j", ctypes.c_int64), ("accumulate", ctypes.c_int32)]
+
+
+class MatrixBatch(ctypes.Structure):
+    """``st_matrix_batch`` (include/spilltune_hip.h): equal matrices back to back."""
+    _fields_ = [("x", ctypes.c_void_p), ("out", ctypes.c_void_p), ("count", ctypes.c_int64),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
 
 
 @functools.lru_cache(maxsize=16)

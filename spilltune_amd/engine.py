@@ -231,14 +231,17 @@ class AdamW:
 
 
 def train(model, session, rows, *, steps, accumulation=1, lr=1e-4, weight_decay=0.0,
-          token_chunk=64, layer_major=False, objective=None):
+          token_chunk=64, layer_major=False, objective=None, optimizer=None):
     """Optimizer-step loop with cyclic rows (engine.py:162-182); returns losses.
     Rows are ``(ids, labels)`` or, packed, ``(ids, labels, documents)``.
     ``layer_major`` runs each accumulation window with ``window_layer_major``
     (same results, one layer load per phase per window).  ``objective``: in the
-    place of the cross-entropy, see :func:`microbatch`."""
+    place of the cross-entropy, see :func:`microbatch`.  ``optimizer`` (an
+    :class:`AdamW` or :class:`~spilltune_amd.muon.Muon`, with its own rates) in the
+    place of the AdamW of ``lr`` and ``weight_decay``."""
     projections = flatten(model)
-    optimizer = AdamW(lr=lr, weight_decay=weight_decay)
+    if optimizer is None:
+        optimizer = AdamW(lr=lr, weight_decay=weight_decay)
     cursor, losses = 0, []
     for _ in range(steps):
         names = [(cursor + i) % len(rows) for i in range(accumulation)]
