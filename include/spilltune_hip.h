@@ -636,6 +636,88 @@ int st_moe_lora_grads(int64_t rows, int32_t R, int64_t seg_len, int32_t nseg,
                       int32_t groups, float alpha, float* out, int64_t o_gstride, int64_t so_m,
                       int64_t so_j, int32_t accumulate, st_stream_t stream);
 
+/* ------------------------------------------------- norms around a block part */
+/*
+ * Norms after and before a part of a block with its gate and residual scale (no
+ * counterpart in the reference); y, residual, h, normed and their gradients bf16
+ * [rows, hidden], contiguous, hidden at most 16384, every tensor on a 16-byte
+ * boundary (a gate of ST_GATE_TOKENS on its element's):
+ *   z = post ? y * rsqrt(mean(y^2) + eps) * post : y
+ *   h = residual + scale * gate * z
+ *   normed = h * rsqrt(mean(h^2) + eps) * pre     (of the unrounded h; pre given)
+ * post, pre: bf16 [hidden] or NULL.  gate: NULL (ST_GATE_NONE), [rows / rows_per,
+ * hidden] each row shared by rows_per rows (ST_GATE_COLUMNS), [rows]
+ * (ST_GATE_TOKENS) or [rows, hidden] (ST_GATE_FULL), of `gate_dtype`.  fp32 inside.
+ * rstd_post, rstd_pre (fp32 [rows]) are kept for the backward, or NULL.
+ *
+ * The backward takes dh and dnormed (either may be NULL: no gradient) and writes
+ * what is asked for (not NULL): dy, dresidual; dpost and dpre fp32 [hidden]; dgate
+ * fp32 [rows / rows_per, hidden] or [rows], or of the gate's type for ST_GATE_FULL.
+ * Sums over rows are joined in a fixed order in `workspace`, which dpost, dpre and
+ * the gate of ST_GATE_COLUMNS need (query with rows_per = rows for other gates).
+ */
+#define ST_GATE_NONE 0
+#define ST_GATE_COLUMNS 1
+#define ST_GATE_TOKENS 2
+#define ST_GATE_FULL 3
+int st_residual_norms_fwd(const uint16_t* y, const uint16_t* residual, const uint16_t* post,
+                          const uint16_t* pre, const void* gate, int32_t gate_mode,
+                          int32_t gate_dtype, int64_t rows_per, int64_t rows, int64_t hidden,
+                          float scale, float eps, uint16_t* h, uint16_t* normed,
+                          float* rstd_post, float* rstd_pre, st_stream_t stream);
+int64_t st_residual_norms_workspace_bytes(int64_t rows, int64_t hidden, int64_t rows_per);
+int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual, const uint16_t* post,
+                          const uint16_t* pre, const void* gate, int32_t gate_mode,
+                          int32_t gate_dtype, int64_t rows_per, int64_t rows, int64_t hidden,
+                          float scale, float eps, const float* rstd_post,
+                          const float* rstd_pre, const uint16_t* dh, const uint16_t* dnormed,
+                          uint16_t* dy, uint16_t* dresidual, void* dgate, float* dpost,
+                          float* dpre, void* workspace, int64_t workspace_bytes,
+                          st_stream_t stream);
+
+/* -------------------------------------------------------------- embedding */
+/*
+ * out[t] = bf16(scale * table[ids[t]]) for n tokens (no counterpart on the device in
+ * the reference); table [vocab, hidden] bf16 or fp32 (`dtype`), ids int64 or, with
+ * ids32, int32.  A token outside [0, vocab) gives NaN.
+ * The backward writes grad [vocab, hidden] (bf16 or fp32, 16-byte aligned): scale
+ * times the fp32 sum of dout [n, hidden] (bf16) over each token's positions in
+ * rising order; zeros for tokens that do not occur.  With `accumulate` (fp32 only)
+ * the sums are added and other rows left as they are.  Tokens equal to padding_idx
+ * or outside the table take no part.
+ */
+int st_embedding_fwd(const void* table, int32_t dtype, const void* ids, int32_t ids32, int64_t n,
+                     int64_t vocab, int64_t hidden, float scale, uint16_t* out,
+                     st_stream_t stream);
+int64_t st_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t hidden);
+int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t ids32, int64_t n, int64_t vocab,
+                     int64_t hidden, float scale, int64_t padding_idx, void* grad,
+                     int32_t grad_dtype, int32_t accumulate, void* workspace,
+                     int64_t workspace_bytes, st_stream_t stream);
+
+/* ---------------------------------------------------------------- balance */
+/*
+ * Balance loss of a router (no counterpart in the reference): logits bf16 or fp32
+ * [groups * per_group, experts], picks [groups * per_group, top_k], valid (bytes, 0:
+ * the token takes no part; NULL: all valid).  p = softmax of a token's logits, or with
+ * `sigmoid` its sigmoids over their sum (+ 1e-20); for a group of n valid tokens with
+ * c_e picks of expert e (picks outside [0, experts) are not counted)
+ *   L_g = experts * sum_e c_e / (top_k n) * mean(p_e)
+ * and `loss` is the mean over the groups with a valid token (0 without any).  counts
+ * [groups, experts] and tokens [groups + 1] (valid tokens a group; then the number of
+ * groups that have some) are results too and what the backward needs; dloss is one
+ * fp32 on the device.  experts <= 512, top_k <= 64, groups < 65536, per_group < 2^25.
+ */
+int64_t st_balance_workspace_bytes(int64_t groups, int64_t per_group, int32_t experts);
+int st_balance_fwd(const void* logits, int32_t dtype, const int32_t* picks, const uint8_t* valid,
+                   int64_t groups, int64_t per_group, int32_t experts, int32_t top_k,
+                   int32_t sigmoid, float* loss, int64_t* counts, int32_t* tokens,
+                   void* workspace, int64_t workspace_bytes, st_stream_t stream);
+int st_balance_bwd(const void* logits, int32_t dtype, const uint8_t* valid, int64_t groups,
+                   int64_t per_group, int32_t experts, int32_t top_k, int32_t sigmoid,
+                   const int64_t* counts, const int32_t* tokens, const float* dloss,
+                   void* dlogits, st_stream_t stream);
+
 /* ---------------------------------------------------------------- updates */
 /*
  * Orthogonalised updates (no counterpart in the reference): for every matrix U of

@@ -23,6 +23,7 @@ ST_OK, ST_EINVAL, ST_EUNSUPPORTED, ST_EDEVICE, ST_EWORKSPACE = range(5)
 ST_FLAG_HI_NIBBLE_FIRST = 1
 ST_FLAG_GROUP64 = 2
 ST_DTYPE_BF16, ST_DTYPE_F32 = 0, 1
+ST_GATE_NONE, ST_GATE_COLUMNS, ST_GATE_TOKENS, ST_GATE_FULL = range(4)
 ST_Q4_FWD, ST_Q4_DGRAD, ST_Q4_DGRAD_SWIGLU = range(3)
 
 _P = ctypes.c_void_p
@@ -119,6 +120,19 @@ _SIGNATURES = {
                                      _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "st_token_logprobs_bwd": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _F, _F, _I64,
                                      _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P]),
+    "st_residual_norms_fwd": (_I32, [_P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _F, _F, _P,
+                                     _P, _P, _P, _P]),
+    "st_residual_norms_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "st_residual_norms_bwd": (_I32, [_P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _F, _F, _P,
+                                     _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "st_embedding_fwd": (_I32, [_P, _I32, _P, _I32, _I64, _I64, _I64, _F, _P, _P]),
+    "st_embedding_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "st_embedding_bwd": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _F, _I64, _P, _I32, _I32, _P, _I64,
+                                _P]),
+    "st_balance_workspace_bytes": (_I64, [_I64, _I64, _I32]),
+    "st_balance_fwd": (_I32, [_P, _I32, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I64,
+                              _P]),
+    "st_balance_bwd": (_I32, [_P, _I32, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),
     "st_orthogonalize_workspace_bytes": (_I64, [_I32, _P]),
     "st_orthogonalize": (_I32, [_I32, _P, _I32, _I32, _D, _D, _D, _D, _P, _I64, _P]),
     "st_cross_entropy_rows": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _F, _P, _P]),

@@ -1,0 +1,290 @@
+// Balance loss of a router and its per-expert counts, and the gradient of its logits.
+//
+//   p = softmax(l)  or  sigma(l) / (sum sigma(l) + 1e-20)
+//   a group of tokens (all of them, or a row's) with n valid ones:
+//     c_e picks of expert e,  P_e = mean of p_e,  L_g = E sum_e c_e / (k n) P_e
+//   L = mean of L_g over the groups with a valid token (1 when balanced)
+//   dp_e = a_e = dL E c_e / (k n^2 groups);  dl_e = p_e (a_e - sum a p)  or
+//          (a_e - sum a p) / (sum sigma + 1e-20) sigma_e (1 - sigma_e)
+//
+// A wave holds a token's logits (up to 512 experts, 8 a lane), so each is read once
+// forward and once backward; picks are counted in LDS (whole numbers: their order
+// does not matter), probabilities summed in fp32 in registers over a workgroup's
+// tokens and joined over the workgroups in their order.
+#include "common.h"
+
+namespace {
+
+constexpr int NTH = 256, WAVES = NTH / 64;
+constexpr int MAXE = 512, PER = MAXE / 64;
+constexpr float TINY = 1e-20f;
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+struct Args {
+  const void* logits;
+  const int32_t* picks;
+  const uint8_t* valid;
+  int64_t groups, per_group;  // tokens of a group
+  int32_t E, k, sigmoid;
+  int64_t chunk, chunks;  // tokens of a workgroup, workgroups of a group
+  float* probs;           // [groups][chunks][E]
+  int32_t* counted;       // [groups][chunks][E + 1], the last: valid tokens
+  float* terms;           // [groups]
+  float* loss;
+  int64_t* counts;  // [groups][E]
+  int32_t* tokens;  // [groups] valid tokens, and behind them the groups that have some
+  const float* dloss;
+  void* dlogits;
+};
+
+// The scores e of a token and the reciprocal of their sum: p = e * inv; lane + 64 i
+// is the expert.
+template <bool BF>
+__device__ __forceinline__ float scores(const Args& a, int64_t t, int lane, float (&v)[PER]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 64 * i;
+    v[i] = -INFINITY;
+    if (e < a.E)
+      v[i] = BF ? st::bf16_to_f32(((const uint16_t*)a.logits)[t * a.E + e])
+                : ((const float*)a.logits)[t * a.E + e];
+    mx = fmaxf(mx, v[i]);
+  }
+  float sum = 0.0f;
+  if (a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      v[i] = lane + 64 * i < a.E ? 1.0f / (1.0f + expf(-v[i])) : 0.0f;
+      sum += v[i];
+    }
+    return 1.0f / (wave_sum(sum) + TINY);
+  }
+  mx = wave_max(mx);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    v[i] = lane + 64 * i < a.E ? expf(v[i] - mx) : 0.0f;
+    sum += v[i];
+  }
+  return 1.0f / wave_sum(sum);
+}
+
+template <bool BF>
+__global__ __launch_bounds__(NTH) void balance_sums(Args a) {
+  __shared__ float sums[WAVES][MAXE];
+  __shared__ int32_t count[MAXE + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t g = blockIdx.y, c = blockIdx.x;
+  for (int i = threadIdx.x; i <= MAXE; i += NTH) count[i] = 0;
+  __syncthreads();
+  float p[PER] = {};
+  int n = 0;
+  const int64_t z = min((c + 1) * a.chunk, a.per_group);
+  for (int64_t i = c * a.chunk + wave; i < z; i += WAVES) {
+    const int64_t t = g * a.per_group + i;
+    if (a.valid && !a.valid[t]) continue;  // the same for the whole wave
+    float v[PER];
+    const float inv = scores<BF>(a, t, lane, v);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) p[j] += v[j] * inv;
+    if (lane < a.k) {
+      const int e = a.picks[t * a.k + lane];
+      if (e >= 0 && e < a.E) atomicAdd(&count[e], 1);
+    }
+    ++n;
+  }
+  if (lane == 0) atomicAdd(&count[MAXE], n);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) sums[wave][lane + 64 * j] = p[j];
+  __syncthreads();
+  float* to = a.probs + (g * a.chunks + c) * a.E;
+  int32_t* nt = a.counted + (g * a.chunks + c) * (a.E + 1);
+  for (int e = threadIdx.x; e < a.E; e += NTH) {
+    float s = sums[0][e];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) s += sums[w][e];
+    to[e] = s;
+    nt[e] = count[e];
+  }
+  if (threadIdx.x == 0) nt[a.E] = count[MAXE];
+}
+
+// A group's chunks joined; with one group also the loss itself.
+__global__ __launch_bounds__(MAXE) void balance_join(Args a) {
+  __shared__ float red[MAXE / 64];
+  const int e = threadIdx.x;
+  const int64_t g = blockIdx.x;
+  int64_t n = 0, picks = 0;
+  float p = 0.0f;
+  for (int64_t c = 0; c < a.chunks; ++c) {
+    const int32_t* nt = a.counted + (g * a.chunks + c) * (a.E + 1);
+    n += nt[a.E];
+    if (e < a.E) {
+      picks += nt[e];
+      p += a.probs[(g * a.chunks + c) * a.E + e];
+    }
+  }
+  if (e < a.E) a.counts[g * a.E + e] = picks;
+  const float many = (float)(n > 0 ? n : 1);
+  float s = wave_sum((float)picks * (float)a.E / ((float)a.k * many) * (p / many));
+  if ((e & 63) == 0) red[e >> 6] = s;
+  __syncthreads();
+  if (e == 0) {
+    s = red[0];
+    for (int w = 1; w < MAXE / 64; ++w) s += red[w];
+    a.tokens[g] = (int32_t)n;
+    if (a.groups == 1) {
+      *a.loss = s;
+      a.tokens[1] = n > 0;
+    } else {
+      a.terms[g] = s;
+    }
+  }
+}
+
+__global__ __launch_bounds__(64) void balance_mean(Args a) {
+  float s = 0.0f;
+  int some = 0;
+  for (int64_t g = threadIdx.x; g < a.groups; g += 64) {
+    s += a.terms[g];
+    some += a.tokens[g] > 0;
+  }
+  s = wave_sum(s);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) some += __shfl_xor(some, d);
+  if (threadIdx.x == 0) {
+    *a.loss = s / (float)(some > 0 ? some : 1);
+    a.tokens[a.groups] = some;
+  }
+}
+
+template <bool BF>
+__global__ __launch_bounds__(NTH) void balance_bwd(Args a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t g = blockIdx.y, z = min((int64_t)(blockIdx.x + 1) * a.chunk, a.per_group);
+  const float n = (float)a.tokens[g];
+  const float each = *a.dloss * (float)a.E / ((float)a.k * n * n * (float)a.tokens[a.groups]);
+  float w[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int e = lane + 64 * j;
+    w[j] = e < a.E ? each * (float)a.counts[g * a.E + e] : 0.0f;
+  }
+  for (int64_t i = blockIdx.x * a.chunk + wave; i < z; i += WAVES) {
+    const int64_t t = g * a.per_group + i;
+    float v[PER], d[PER];
+    if (a.valid && !a.valid[t]) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) d[j] = 0.0f;
+    } else {
+      const float inv = scores<BF>(a, t, lane, v);
+      float dot = 0.0f;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) dot += w[j] * (v[j] * inv);
+      dot = wave_sum(dot);
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        d[j] = v[j] * inv * (w[j] - dot) * (a.sigmoid ? 1.0f - v[j] : 1.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int e = lane + 64 * j;
+      if (e >= a.E) continue;
+      if (BF)
+        ((uint16_t*)a.dlogits)[t * a.E + e] = st::f32_to_bf16(d[j]);
+      else
+        ((float*)a.dlogits)[t * a.E + e] = d[j];
+    }
+  }
+}
+
+// Tokens of a workgroup: about 512 workgroups in all, at least one token a wave.
+void plan(Args& a) {
+  const int64_t want = st::cdiv(512, a.groups);
+  a.chunk = st::cdiv(st::cdiv(a.per_group, want), WAVES) * WAVES;
+  a.chunks = st::cdiv(a.per_group, a.chunk);
+}
+
+int check_args(const Args& a, int32_t dtype, const char* what) {
+  ST_CHECK_ARG(dtype == ST_DTYPE_BF16 || dtype == ST_DTYPE_F32, "dtype codes are bf16 and fp32");
+  ST_CHECK_ARG(a.groups >= 1 && a.per_group >= 1, "%s: groups %lld of %lld tokens", what,
+               (long long)a.groups, (long long)a.per_group);
+  ST_CHECK_ARG(a.E >= 1 && a.E <= MAXE && a.k >= 1 && a.k <= 64, "%s: experts 1..512, picks 1..64",
+               what);
+  if (a.groups >= 65536 || a.per_group >= (int64_t)1 << 25)
+    return st::fail(ST_EUNSUPPORTED, "%s: 65536 groups or 2^25 tokens a group and more", what);
+  return ST_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t st_balance_workspace_bytes(int64_t groups, int64_t per_group, int32_t experts) {
+  Args a = {};
+  a.groups = groups, a.per_group = per_group, a.E = experts, a.k = 1;
+  if (check_args(a, ST_DTYPE_F32, "st_balance") != ST_OK) return 0;
+  plan(a);
+  return (groups * a.chunks * (2 * (int64_t)experts + 1) + groups) * 4;
+}
+
+extern "C" int st_balance_fwd(const void* logits, int32_t dtype, const int32_t* picks,
+                              const uint8_t* valid, int64_t groups, int64_t per_group,
+                              int32_t experts, int32_t top_k, int32_t sigmoid, float* loss,
+                              int64_t* counts, int32_t* tokens, void* workspace,
+                              int64_t workspace_bytes, st_stream_t stream) {
+  Args a = {};
+  a.logits = logits, a.picks = picks, a.valid = valid, a.groups = groups, a.per_group = per_group;
+  a.E = experts, a.k = top_k, a.sigmoid = sigmoid, a.loss = loss, a.counts = counts;
+  a.tokens = tokens;
+  const int rc = check_args(a, dtype, "st_balance_fwd");
+  if (rc != ST_OK) return rc;
+  ST_CHECK_ARG(logits && picks && loss && counts && tokens, "st_balance_fwd: NULL");
+  const int64_t need = st_balance_workspace_bytes(groups, per_group, experts);
+  if (!workspace || workspace_bytes < need)
+    return st::fail(ST_EWORKSPACE, "st_balance_fwd needs %lld workspace bytes", (long long)need);
+  ST_CHECK_ARG(((uintptr_t)workspace & 3) == 0, "workspace must be 4-byte aligned");
+  plan(a);
+  a.probs = (float*)workspace;
+  a.counted = (int32_t*)(a.probs + groups * a.chunks * experts);
+  a.terms = (float*)(a.counted + groups * a.chunks * (experts + 1));
+  const hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)a.chunks, (unsigned)groups);
+  if (dtype == ST_DTYPE_BF16)
+    balance_sums<true><<<grid, NTH, 0, s>>>(a);
+  else
+    balance_sums<false><<<grid, NTH, 0, s>>>(a);
+  balance_join<<<(unsigned)groups, MAXE, 0, s>>>(a);
+  if (groups > 1) balance_mean<<<1, 64, 0, s>>>(a);
+  return st::check_launch("st_balance_fwd");
+}
+
+extern "C" int st_balance_bwd(const void* logits, int32_t dtype, const uint8_t* valid,
+                              int64_t groups, int64_t per_group, int32_t experts, int32_t top_k,
+                              int32_t sigmoid, const int64_t* counts, const int32_t* tokens,
+                              const float* dloss, void* dlogits, st_stream_t stream) {
+  Args a = {};
+  a.logits = logits, a.valid = valid, a.groups = groups, a.per_group = per_group;
+  a.E = experts, a.k = top_k, a.sigmoid = sigmoid, a.counts = (int64_t*)counts;
+  a.tokens = (int32_t*)tokens, a.dloss = dloss, a.dlogits = dlogits;
+  const int rc = check_args(a, dtype, "st_balance_bwd");
+  if (rc != ST_OK) return rc;
+  ST_CHECK_ARG(logits && counts && tokens && dloss && dlogits, "st_balance_bwd: NULL");
+  // about 2048 workgroups, two tokens a wave at least: its weights are read per wave
+  a.chunk = st::cdiv(st::cdiv(per_group, st::cdiv(2048, groups)), 2 * WAVES) * 2 * WAVES;
+  a.chunks = st::cdiv(per_group, a.chunk);
+  const dim3 grid((unsigned)a.chunks, (unsigned)groups);
+  if (dtype == ST_DTYPE_BF16)
+    balance_bwd<true><<<grid, NTH, 0, (hipStream_t)stream>>>(a);
+  else
+    balance_bwd<false><<<grid, NTH, 0, (hipStream_t)stream>>>(a);
+  return st::check_launch("st_balance_bwd");
+}

@@ -1,0 +1,530 @@
+// Token embedding: scaled lookup, and the table's gradient by sorted tokens.
+//
+//   out[t] = scale table[id_t];   dtable[v] = scale sum_{t: id_t = v} dout[t]
+//
+// Both are bound by HBM.  The gradient's sums must not depend on the order in which
+// workgroups arrive, so no float is added atomically: (token, position) pairs are
+// sorted by token (least significant digit first, nine bits a pass, stable, so each
+// token's positions rise), and chunks of the sorted list are summed in that order,
+// each row of dout read once.  A token whose positions reach over a chunk's end
+// leaves partial sums, which a last kernel joins from chunk to chunk.  A dense
+// gradient is cleared by the launch that sorts: up to 16384 tokens are sorted by one
+// workgroup in LDS while the others clear.
+#include <cmath>
+
+#include "common.h"
+
+namespace {
+
+constexpr int NTH = 256;
+constexpr int BITS = 9, BINS = 1 << BITS;
+constexpr int64_t SMALL = 16384;  // tokens one workgroup sorts (16 a thread)
+constexpr int TILE = 2048;        // keys of a workgroup beyond that
+
+__device__ __forceinline__ int64_t id_at(const void* ids, int ids32, int64_t i) {
+  return ids32 ? (int64_t)((const int32_t*)ids)[i] : ((const int64_t*)ids)[i];
+}
+// The sort key: tokens outside the table and the padding token come last.
+__device__ __forceinline__ uint32_t key_of(int64_t id, int64_t V, int64_t padding) {
+  return id < 0 || id >= V || id == padding ? (uint32_t)V : (uint32_t)id;
+}
+
+// ---------------------------------------------------------------- lookup
+template <int VEC, bool F32>
+__global__ __launch_bounds__(NTH) void lookup(const void* __restrict__ table,
+                                              const void* __restrict__ ids, int ids32, int64_t n,
+                                              int64_t V, int64_t H, float scale,
+                                              uint16_t* __restrict__ out) {
+  for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
+    const int64_t id = id_at(ids, ids32, t);
+    const bool in = id >= 0 && id < V;
+    for (int64_t i = threadIdx.x * VEC; i < H; i += (int64_t)blockDim.x * VEC) {
+      float f[VEC];
+      const int64_t at = (in ? id : 0) * H + i;
+      if constexpr (VEC == 8) {
+        if constexpr (F32) {
+          const float4 a = *(const float4*)((const float*)table + at);
+          const float4 b = *(const float4*)((const float*)table + at + 4);
+          f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+          f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+        } else {
+          const uint4 v = *(const uint4*)((const uint16_t*)table + at);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[2 * e] = __uint_as_float(w[e] << 16);
+            f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
+        }
+      } else {
+        f[0] = F32 ? ((const float*)table)[at] : st::bf16_to_f32(((const uint16_t*)table)[at]);
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = in ? f[e] * scale : NAN;
+      uint16_t* to = out + t * H + i;
+      if constexpr (VEC == 8)
+        *(uint4*)to = make_uint4(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
+                                 st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7]));
+      else
+        *to = st::f32_to_bf16(f[0]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- sort
+// Rank of each lane's key among its wave's keys of one digit, those of earlier
+// calls first (count[] starts at zero).  Lanes that are not `live` take no part.
+__device__ __forceinline__ uint32_t wave_rank(uint32_t digit, bool live, uint32_t* count) {
+  const int lane = threadIdx.x & 63;
+  unsigned long long same = __ballot(live);
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
+    const unsigned long long set = __ballot((digit >> b) & 1u);
+    same &= (digit >> b) & 1u ? set : ~set;
+  }
+  uint32_t base = 0;
+  const int first = __ffsll((long long)same) - 1;
+  if (live && lane == first) base = atomicAdd(&count[digit], (uint32_t)__popcll(same));
+  base = __shfl(base, live ? first : 0);
+  return base + (uint32_t)__popcll(same & ((1ull << lane) - 1));
+}
+
+// Exclusive sums of count[wave][digit] over digits, then waves, in place; 64 W
+// threads.
+template <int W>
+__device__ __forceinline__ void scan_counts(uint32_t (*count)[BINS], uint32_t* totals) {
+  constexpr int PER = BINS * W / (64 * W);  // counters a thread: 8 bins of one wave
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // thread order = digit-major: entry e = digit * W + w
+  uint32_t v[PER], sum = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int e = threadIdx.x * PER + k;
+    v[k] = count[e % W][e / W];
+    sum += v[k];
+  }
+  uint32_t inc = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t x = __shfl_up(inc, d);
+    if (lane >= d) inc += x;
+  }
+  if (lane == 63) totals[wave] = inc;
+  __syncthreads();
+  uint32_t base = inc - sum;
+  for (int w = 0; w < wave; ++w) base += totals[w];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int e = threadIdx.x * PER + k;
+    count[e % W][e / W] = base;
+    base += v[k];
+  }
+  __syncthreads();
+}
+
+// Up to 16384 tokens: workgroup 0 sorts, the others clear `words` 16-byte words.
+__global__ __launch_bounds__(1024) void sort_small(const void* __restrict__ ids, int ids32, int n,
+                                                   int64_t V, int64_t padding, int passes,
+                                                   uint32_t* __restrict__ tok,
+                                                   uint32_t* __restrict__ pos,
+                                                   uint4* __restrict__ clear, int64_t words) {
+  if (blockIdx.x) {
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < words;
+         i += (int64_t)(gridDim.x - 1) * 1024)
+      clear[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  __shared__ uint32_t count[16][BINS];
+  __shared__ uint32_t totals[16];
+  __shared__ uint32_t keys[SMALL];
+  __shared__ uint16_t where[SMALL];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int steps = (n + 1023) / 1024, first = wave * steps * 64 + lane;
+  uint32_t key[16], rank[16];
+  uint16_t at[16];
+#pragma unroll
+  for (int s = 0; s < 16; ++s) {
+    const int i = first + s * 64;
+    const bool live = s < steps && i < n;
+    key[s] = live ? key_of(id_at(ids, ids32, i), V, padding) : 0;
+    at[s] = (uint16_t)i;
+  }
+  for (int p = 0; p < passes; ++p) {
+    for (int i = threadIdx.x; i < 16 * BINS; i += 1024) (&count[0][0])[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 16; ++s)
+      if (s < steps) rank[s] = wave_rank((key[s] >> (BITS * p)) & (BINS - 1), first + s * 64 < n,
+                                         count[wave]);
+    __syncthreads();
+    scan_counts<16>(count, totals);
+#pragma unroll
+    for (int s = 0; s < 16; ++s)
+      if (s < steps && first + s * 64 < n) {
+        const uint32_t to = count[wave][(key[s] >> (BITS * p)) & (BINS - 1)] + rank[s];
+        keys[to] = key[s];
+        where[to] = at[s];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 16; ++s)
+      if (s < steps && first + s * 64 < n) {
+        key[s] = keys[first + s * 64];
+        at[s] = where[first + s * 64];
+      }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int s = 0; s < 16; ++s)
+    if (s < steps && first + s * 64 < n) {
+      tok[first + s * 64] = key[s];
+      pos[first + s * 64] = at[s];
+    }
+}
+
+// More tokens: per pass the tiles' digit counts [digit][tile], their exclusive sums,
+// and the move.  The first pass reads the ids themselves.
+__global__ __launch_bounds__(NTH) void tile_counts(const void* __restrict__ ids, int ids32,
+                                                   const uint32_t* __restrict__ tok, int64_t n,
+                                                   int64_t V, int64_t padding, int shift,
+                                                   int64_t tiles, uint32_t* __restrict__ counts) {
+  __shared__ uint32_t hist[BINS];
+  for (int i = threadIdx.x; i < BINS; i += NTH) hist[i] = 0;
+  __syncthreads();
+  for (int s = 0; s < TILE / NTH; ++s) {
+    const int64_t i = (int64_t)blockIdx.x * TILE + s * NTH + threadIdx.x;
+    if (i < n) {
+      const uint32_t key = tok ? tok[i] : key_of(id_at(ids, ids32, i), V, padding);
+      atomicAdd(&hist[(key >> shift) & (BINS - 1)], 1u);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += NTH) counts[i * tiles + blockIdx.x] = hist[i];
+}
+
+__global__ __launch_bounds__(1024) void tile_scan(uint32_t* __restrict__ counts, int64_t many) {
+  __shared__ uint32_t totals[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t per = (many + 1023) / 1024, a = threadIdx.x * per, z = min(a + per, many);
+  uint32_t sum = 0;
+  for (int64_t i = a; i < z; ++i) sum += counts[i];
+  uint32_t inc = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t x = __shfl_up(inc, d);
+    if (lane >= d) inc += x;
+  }
+  if (lane == 63) totals[wave] = inc;
+  __syncthreads();
+  uint32_t base = inc - sum;
+  for (int w = 0; w < wave; ++w) base += totals[w];
+  for (int64_t i = a; i < z; ++i) {
+    const uint32_t v = counts[i];
+    counts[i] = base;
+    base += v;
+  }
+}
+
+__global__ __launch_bounds__(NTH) void tile_move(const void* __restrict__ ids, int ids32,
+                                                 const uint32_t* __restrict__ tok,
+                                                 const uint32_t* __restrict__ pos, int64_t n,
+                                                 int64_t V, int64_t padding, int shift,
+                                                 int64_t tiles,
+                                                 const uint32_t* __restrict__ counts,
+                                                 uint32_t* __restrict__ tok_out,
+                                                 uint32_t* __restrict__ pos_out) {
+  constexpr int W = NTH / 64, STEPS = TILE / NTH;
+  __shared__ uint32_t count[W][BINS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < W * BINS; i += NTH) (&count[0][0])[i] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * TILE + wave * (TILE / W) + lane;
+  uint32_t key[STEPS], at[STEPS], rank[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int64_t i = first + s * 64;
+    const bool live = i < n;
+    key[s] = !live ? 0 : tok ? tok[i] : key_of(id_at(ids, ids32, i), V, padding);
+    at[s] = !live ? 0 : tok ? pos[i] : (uint32_t)i;
+    rank[s] = wave_rank((key[s] >> shift) & (BINS - 1), live, count[wave]);
+  }
+  __syncthreads();
+  // the tile's place of each digit, then the waves' before this one
+  for (int d = threadIdx.x; d < BINS; d += NTH) {
+    uint32_t base = counts[d * tiles + blockIdx.x];
+    for (int w = 0; w < W; ++w) {
+      const uint32_t v = count[w][d];
+      count[w][d] = base;
+      base += v;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+    if (first + s * 64 < n) {
+      const uint32_t to = count[wave][(key[s] >> shift) & (BINS - 1)] + rank[s];
+      tok_out[to] = key[s];
+      pos_out[to] = at[s];
+    }
+}
+
+__global__ __launch_bounds__(NTH) void clear_words(uint4* __restrict__ p, int64_t words) {
+  for (int64_t i = (int64_t)blockIdx.x * NTH + threadIdx.x; i < words; i += (int64_t)gridDim.x * NTH)
+    p[i] = make_uint4(0, 0, 0, 0);
+}
+// what 16-byte words leave of a gradient
+__global__ __launch_bounds__(64) void clear_tail(uint16_t* __restrict__ p, int halves) {
+  if ((int)threadIdx.x < halves) p[threadIdx.x] = 0;
+}
+
+// ---------------------------------------------------------------- sums
+struct Sums {
+  const uint16_t* dout;
+  const uint32_t *tok, *pos;
+  int64_t n, V, H;
+  int64_t chunk;  // sorted entries of a workgroup
+  float scale;
+  int32_t grad_f32, accumulate;
+  void* grad;
+  float* partial;  // [chunks][2][H]: of the run from the chunk before, of the run into the next
+};
+
+template <int VEC>
+__device__ __forceinline__ void add_row(const uint16_t* p, float (&acc)[VEC]) {
+  if constexpr (VEC == 8) {
+    const uint4 v = *(const uint4*)p;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[2 * e] += __uint_as_float(w[e] << 16);
+      acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+    }
+  } else {
+    acc[0] += st::bf16_to_f32(p[0]);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_f(float* p, const float (&f)[VEC]) {
+  if constexpr (VEC == 8) {
+    *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
+    *(float4*)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    p[0] = f[0];
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void write_row(const Sums& a, uint32_t token, int64_t i,
+                                          const float (&acc)[VEC]) {
+  const int64_t at = (int64_t)token * a.H + i;
+  float f[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] = a.scale * acc[e];
+  if (a.grad_f32) {
+    float* p = (float*)a.grad + at;
+    if (a.accumulate) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] += p[e];
+    }
+    store_f<VEC>(p, f);
+  } else {
+    uint16_t* p = (uint16_t*)a.grad + at;
+    if constexpr (VEC == 8)
+      *(uint4*)p = make_uint4(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
+                              st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7]));
+    else
+      *p = st::f32_to_bf16(f[0]);
+  }
+}
+
+// A chunk of the sorted list: sums of its runs of one token.
+template <int VEC>
+__global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
+  const int64_t c = blockIdx.x, e0 = c * a.chunk, e1 = min(e0 + a.chunk, a.n);
+  const int64_t i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (i >= a.H || a.tok[e0] >= a.V) return;  // no barriers below
+  bool from = e0 > 0 && a.tok[e0 - 1] == a.tok[e0];  // the run began in an earlier chunk
+  float acc[VEC] = {};
+  for (int64_t e = e0; e < e1; ++e) {
+    const uint32_t token = a.tok[e];
+    if (token >= a.V) return;  // only such ones follow
+    add_row<VEC>(a.dout + (int64_t)a.pos[e] * a.H + i, acc);
+    const bool end = e + 1 == a.n || a.tok[e + 1] != token;
+    if (!end && e + 1 < e1) continue;
+    if (from)
+      store_f<VEC>(a.partial + c * 2 * a.H + i, acc);
+    else if (!end)
+      store_f<VEC>(a.partial + (c * 2 + 1) * a.H + i, acc);
+    else
+      write_row<VEC>(a, token, i, acc);
+    from = false;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+  }
+}
+
+// The run that begins in chunk c and goes on behind it.
+template <int VEC>
+__global__ __launch_bounds__(NTH) void join_runs(Sums a) {
+  const int64_t c = blockIdx.x, next = (c + 1) * a.chunk;  // next < n by the grid
+  const uint32_t token = a.tok[next];
+  const int64_t i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (i >= a.H || token >= a.V || a.tok[next - 1] != token) return;
+  const int64_t e0 = c * a.chunk;
+  if (a.tok[e0] == token && e0 > 0 && a.tok[e0 - 1] == token) return;  // began earlier
+  float acc[VEC];
+  const float* p = a.partial + (c * 2 + 1) * a.H + i;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = p[k];
+  for (int64_t d = c + 1; d * a.chunk < a.n && a.tok[d * a.chunk] == token; ++d) {
+    p = a.partial + d * 2 * a.H + i;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] += p[k];
+  }
+  write_row<VEC>(a, token, i, acc);
+}
+
+// ---------------------------------------------------------------- host
+int64_t chunk_of(int64_t n) { return n <= 32768 ? 16 : 32; }
+int passes_of(int64_t V) {  // of keys 0..V
+  int bits = 1;
+  while (V >> bits) ++bits;
+  return (bits + BITS - 1) / BITS;
+}
+int64_t align16(int64_t b) { return (b + 15) & ~(int64_t)15; }
+
+struct Layout {
+  int64_t tok[2], pos[2], counts, partial, bytes;
+};
+Layout layout(int64_t n, int64_t H) {
+  Layout l = {};
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t a = at;
+    at += align16(bytes);
+    return a;
+  };
+  const int two = n > SMALL ? 2 : 1;
+  for (int k = 0; k < two; ++k) l.tok[k] = take(4 * n), l.pos[k] = take(4 * n);
+  if (n > SMALL) l.counts = take(4 * BINS * st::cdiv(n, TILE));
+  l.partial = take(st::cdiv(n, chunk_of(n)) * 2 * H * 4);
+  l.bytes = at;
+  return l;
+}
+
+int check_sizes(const char* what, int64_t n, int64_t V, int64_t H) {
+  ST_CHECK_ARG(n >= 0 && V >= 1 && H >= 1, "%s: %lld tokens, table %lld x %lld", what, (long long)n,
+               (long long)V, (long long)H);
+  if (n >= (int64_t)1 << 31 || V >= (int64_t)1 << 31 || H >= (int64_t)1 << 24)
+    return st::fail(ST_EUNSUPPORTED, "%s: 2^31 tokens or rows, or 2^24 columns, and more", what);
+  return ST_OK;
+}
+
+// Threads of a workgroup over the columns of a row, VEC at a time.
+unsigned threads_of(int64_t H, int VEC) {
+  const int64_t t = st::cdiv(st::cdiv(H, VEC), 64) * 64;
+  return (unsigned)(t < NTH ? t : NTH);
+}
+
+}  // namespace
+
+extern "C" int st_embedding_fwd(const void* table, int32_t dtype, const void* ids, int32_t ids32,
+                                int64_t n, int64_t vocab, int64_t hidden, float scale,
+                                uint16_t* out, st_stream_t stream) {
+  const int rc = check_sizes("st_embedding_fwd", n, vocab, hidden);
+  if (rc != ST_OK) return rc;
+  ST_CHECK_ARG(dtype == ST_DTYPE_BF16 || dtype == ST_DTYPE_F32, "dtype codes are bf16 and fp32");
+  if (n == 0) return ST_OK;
+  ST_CHECK_ARG(table && ids && out, "st_embedding_fwd: NULL");
+  const bool vec = hidden % 8 == 0 && (((uintptr_t)table | (uintptr_t)out) & 15) == 0;
+  const unsigned grid = (unsigned)(n < (1 << 20) ? n : 1 << 20), th = threads_of(hidden, vec ? 8 : 1);
+  const hipStream_t s = (hipStream_t)stream;
+  auto run = [&](auto kernel) {
+    kernel<<<grid, th, 0, s>>>(table, ids, ids32, n, vocab, hidden, scale, out);
+  };
+  if (vec)
+    dtype == ST_DTYPE_F32 ? run(lookup<8, true>) : run(lookup<8, false>);
+  else
+    dtype == ST_DTYPE_F32 ? run(lookup<1, true>) : run(lookup<1, false>);
+  return st::check_launch("st_embedding_fwd");
+}
+
+extern "C" int64_t st_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t hidden) {
+  if (n < 1 || check_sizes("st_embedding_bwd", n, vocab, hidden) != ST_OK) return 0;
+  return layout(n, hidden).bytes;
+}
+
+extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t ids32, int64_t n,
+                                int64_t vocab, int64_t hidden, float scale, int64_t padding_idx,
+                                void* grad, int32_t grad_dtype, int32_t accumulate, void* workspace,
+                                int64_t workspace_bytes, st_stream_t stream) {
+  const int rc = check_sizes("st_embedding_bwd", n, vocab, hidden);
+  if (rc != ST_OK) return rc;
+  ST_CHECK_ARG(grad_dtype == ST_DTYPE_BF16 || grad_dtype == ST_DTYPE_F32,
+               "dtype codes are bf16 and fp32");
+  ST_CHECK_ARG(!accumulate || grad_dtype == ST_DTYPE_F32,
+               "st_embedding_bwd adds to fp32 gradients only");
+  ST_CHECK_ARG(grad && ((uintptr_t)grad & 15) == 0, "st_embedding_bwd: NULL or misaligned gradient");
+  const hipStream_t s = (hipStream_t)stream;
+  const int64_t bytes = vocab * hidden * (grad_dtype == ST_DTYPE_F32 ? 4 : 2);
+  const int64_t words = accumulate ? 0 : bytes / 16;
+  const int tail = accumulate ? 0 : (int)(bytes % 16 / 2);
+  if (n > 0) {
+    ST_CHECK_ARG(dout && ids, "st_embedding_bwd: NULL");
+    const int64_t need = layout(n, hidden).bytes;
+    if (!workspace || workspace_bytes < need)
+      return st::fail(ST_EWORKSPACE, "st_embedding_bwd needs %lld workspace bytes", (long long)need);
+    ST_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
+  }
+  const int64_t blocks = st::cdiv(words, 4 * 1024);  // four words a thread at least
+  const unsigned fill = (unsigned)(blocks < 2048 ? blocks : 2048);
+  if (tail)
+    clear_tail<<<1, 64, 0, s>>>((uint16_t*)((char*)grad + bytes - 2 * tail), tail);
+  if (n == 0) {
+    if (words) clear_words<<<fill * 4, NTH, 0, s>>>((uint4*)grad, words);
+    return st::check_launch("st_embedding_bwd");
+  }
+  const Layout l = layout(n, hidden);
+  char* w = (char*)workspace;
+  const int passes = passes_of(vocab);
+  int last = 0;
+  if (n <= SMALL) {
+    sort_small<<<1 + fill, 1024, 0, s>>>(ids, ids32, (int)n, vocab, padding_idx, passes,
+                                         (uint32_t*)(w + l.tok[0]), (uint32_t*)(w + l.pos[0]),
+                                         (uint4*)grad, words);
+  } else {
+    if (words) clear_words<<<fill * 4, NTH, 0, s>>>((uint4*)grad, words);
+    const int64_t tiles = st::cdiv(n, TILE);
+    uint32_t* counts = (uint32_t*)(w + l.counts);
+    for (int p = 0; p < passes; ++p) {
+      const uint32_t* tok = p ? (const uint32_t*)(w + l.tok[last]) : nullptr;
+      const uint32_t* pos = p ? (const uint32_t*)(w + l.pos[last]) : nullptr;
+      const int to = p & 1;
+      tile_counts<<<(unsigned)tiles, NTH, 0, s>>>(ids, ids32, tok, n, vocab, padding_idx, BITS * p,
+                                                  tiles, counts);
+      tile_scan<<<1, 1024, 0, s>>>(counts, BINS * tiles);
+      tile_move<<<(unsigned)tiles, NTH, 0, s>>>(ids, ids32, tok, pos, n, vocab, padding_idx, BITS * p,
+                                                tiles, counts, (uint32_t*)(w + l.tok[to]),
+                                                (uint32_t*)(w + l.pos[to]));
+      last = to;
+    }
+  }
+  Sums a = {};
+  a.dout = dout, a.tok = (const uint32_t*)(w + l.tok[last]), a.pos = (const uint32_t*)(w + l.pos[last]);
+  a.n = n, a.V = vocab, a.H = hidden, a.chunk = chunk_of(n), a.scale = scale;
+  a.grad_f32 = grad_dtype == ST_DTYPE_F32, a.accumulate = accumulate, a.grad = grad;
+  a.partial = (float*)(w + l.partial);
+  const bool vec = hidden % 8 == 0 && ((uintptr_t)dout & 15) == 0;
+  const unsigned th = threads_of(hidden, vec ? 8 : 1);
+  const int64_t chunks = st::cdiv(n, a.chunk), slices = st::cdiv(hidden, (int64_t)th * (vec ? 8 : 1));
+  if (chunks * slices * th >= (int64_t)1 << 32 || slices >= 65536)
+    return st::fail(ST_EUNSUPPORTED, "st_embedding_bwd: more threads than a launch takes");
+  const dim3 grid((unsigned)chunks, (unsigned)slices), more((unsigned)chunks - 1, (unsigned)slices);
+  if (vec) {
+    sum_runs<8><<<grid, th, 0, s>>>(a);
+    if (chunks > 1) join_runs<8><<<more, th, 0, s>>>(a);
+  } else {
+    sum_runs<1><<<grid, th, 0, s>>>(a);
+    if (chunks > 1) join_runs<1><<<more, th, 0, s>>>(a);
+  }
+  return st::check_launch("st_embedding_bwd");
+}

@@ -199,8 +199,18 @@ def window_layer_major(model, session, items, *, normalization, token_chunk, obj
     return losses
 
 
+def _tensors(projection):
+    """``(parameter, gradient, m, v)`` of what a projection, or a trained embedding,
+    holds."""
+    p = projection
+    if hasattr(p, "A"):
+        return ((p.A, p.grad_A, p.m_A, p.v_A), (p.B, p.grad_B, p.m_B, p.v_B))
+    return ((p.weight, p.grad, p.m, p.v),)
+
+
 class AdamW:
-    """Bias-corrected fp32 AdamW over LoRA projections (optimizer.py:227-342)."""
+    """Bias-corrected fp32 AdamW over LoRA projections (optimizer.py:227-342) and a
+    trained embedding."""
 
     def __init__(self, lr=1e-4, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
         self.lr, self.beta1, self.beta2, self.eps = lr, beta1, beta2, eps
@@ -209,10 +219,9 @@ class AdamW:
 
     def zero_grad(self, projections):
         for p in projections.values():
-            p.grad_A.zero_()
-            p.grad_B.zero_()
-            p.A.grad = None
-            p.B.grad = None
+            for param, grad, _, _ in _tensors(p):
+                grad.zero_()
+                param.grad = None
 
     def step(self, projections):
         n = self.step_count + 1
@@ -220,7 +229,7 @@ class AdamW:
         bc2_sqrt = math.sqrt(1.0 - self.beta2 ** n)
         with torch.no_grad():
             for p in projections.values():
-                for param, grad, m, v in ((p.A, p.grad_A, p.m_A, p.v_A), (p.B, p.grad_B, p.m_B, p.v_B)):
+                for param, grad, m, v in _tensors(p):
                     if self.weight_decay != 0.0:
                         param.mul_(1.0 - self.lr * self.weight_decay)
                     m.lerp_(grad, 1.0 - self.beta1)

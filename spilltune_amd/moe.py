@@ -26,13 +26,13 @@ benchmark configuration and is optional.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
 from .codecs import GROUP, codebook, encode
-from .ops import _launch, lora_gemm
+from .ops import _launch, _no_tangents, _once, _scratch, lora_gemm
 
 _BF16 = torch.bfloat16
 _F32 = torch.float32
@@ -147,6 +147,87 @@ def make_expert_lora(name, experts, in_features, out_features, *, rank, alpha, d
         B.normal_(0.0, b_std, generator=generator)
     return ExpertLoRA(name, rank, alpha, experts, in_features, out_features, segments,
                       A.to(device), B.to(device))
+
+
+# ----------------------------------------------------------------- balance
+class BalanceLoss(NamedTuple):
+    """What :func:`balance_loss` gives."""
+    loss: torch.Tensor    # fp32, a scalar; 1 when every expert is picked alike
+    counts: torch.Tensor  # int64 [groups, experts], picks of each expert
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, indices, valid, groups, sigmoid):
+        E, k = logits.shape[-1], indices.shape[-1]
+        per, dev = logits.numel() // E // groups, logits.device
+        loss = torch.empty((), dtype=_F32, device=dev)
+        counts = torch.empty((groups, E), dtype=torch.int64, device=dev)
+        tokens = torch.empty(groups + 1, dtype=_I32, device=dev)
+        dtype = _lib.ST_DTYPE_F32 if logits.dtype == _F32 else _lib.ST_DTYPE_BF16
+        with _lib.on_device(dev):
+            nbytes = _lib.query("st_balance_workspace_bytes", groups, per, E)
+            ws = _scratch(dev, nbytes)
+            _lib.call("st_balance_fwd", logits.data_ptr(), dtype, indices.data_ptr(),
+                      _lib.ptr(valid), groups, per, E, k, sigmoid, loss.data_ptr(),
+                      counts.data_ptr(), tokens.data_ptr(), _lib.ptr(ws), nbytes, _stream(dev))
+        ctx.save_for_backward(logits, valid, counts, tokens)
+        ctx.meta = (groups, per, k, sigmoid, dtype)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    def backward(ctx, dloss, _):
+        _once()
+        logits, valid, counts, tokens = ctx.saved_tensors
+        groups, per, k, sigmoid, dtype = ctx.meta
+        dev = logits.device
+        dloss = dloss.contiguous()
+        dlogits = torch.empty_like(logits)
+        with _lib.on_device(dev):
+            _lib.call("st_balance_bwd", logits.data_ptr(), dtype, _lib.ptr(valid), groups, per,
+                      logits.shape[-1], k, sigmoid, counts.data_ptr(), tokens.data_ptr(),
+                      dloss.data_ptr(), dlogits.data_ptr(), _stream(dev))
+        return dlogits, None, None, None, None
+
+
+def balance_loss(logits, indices, *, score="softmax", valid=None, per_row=False):
+    """Balance loss and per-expert counts of a router as :class:`BalanceLoss`, from
+    its ``logits`` [..., E] (bf16 or fp32) and the experts it picked, ``indices``
+    [..., k] (int32 or int64; an index outside [0, E) is not counted).
+
+    For ``n`` valid tokens with ``c_e`` picks of expert ``e`` it is ``E * sum_e (c_e / (k
+    n)) * mean(p_e)`` with ``p`` the softmax of a token's logits or, with
+    ``score="sigmoid"``, its sigmoids over their sum; differentiable in ``logits``
+    through ``p``.  ``valid`` (bool [...]) leaves padded tokens out, whatever their
+    logits are.  ``per_row``: each row of [B, S, E] is balanced by itself, the loss is
+    the mean over the rows with a valid token, and ``counts`` are the rows'.  Without
+    any valid token it is 0."""
+    if logits.dtype not in (_BF16, _F32) or logits.dim() < 2:
+        raise ValueError("unsupported_capability: balance_loss expects bf16 or fp32 logits [..., E]")
+    shape, E = logits.shape[:-1], logits.shape[-1]
+    if indices.dtype not in (_I32, torch.int64) or indices.dim() != logits.dim() \
+            or indices.shape[:-1] != shape:
+        raise ValueError(f"unsupported_capability: indices must be int32 or int64 {(*shape, 'k')}")
+    if not 1 <= E <= 512 or not 1 <= indices.shape[-1] <= 64:
+        raise ValueError("unsupported_capability: balance_loss takes 1 to 512 experts, 1 to 64 picks")
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError("unsupported_capability: score is softmax or sigmoid")
+    if valid is not None and (valid.dtype != torch.bool or valid.shape != shape):
+        raise ValueError(f"unsupported_capability: valid must be bool {tuple(shape)}")
+    if per_row and logits.dim() != 3:
+        raise ValueError("unsupported_capability: per_row takes logits [B, S, E]")
+    if not logits.numel():
+        raise ValueError("unsupported_capability: balance_loss needs at least one token")
+    _no_tangents(logits)
+    if not logits.is_cuda:
+        raise ValueError("unsupported_capability: balance_loss runs on the GPU")
+    if any(t is not None and t.device != logits.device for t in (indices, valid)):
+        raise ValueError("unsupported_capability: logits, indices and valid on one device")
+    groups = shape[0] if per_row else 1
+    return BalanceLoss(*_BalanceLoss.apply(
+        logits.contiguous(), indices.to(_I32).contiguous(),
+        None if valid is None else valid.contiguous(), groups, int(score == "sigmoid")))
 
 
 # ----------------------------------------------------------------- the function

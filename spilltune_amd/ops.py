@@ -670,6 +670,220 @@ def rms_norm_residual(x: torch.Tensor, weight: torch.Tensor, eps: float):
     return _RMSNormResidual.apply(x.contiguous(), weight.detach().contiguous(), eps)
 
 
+# ----------------------------------------------------------------- norms around a part
+def _residual_norms(y, residual, post, pre, gate, mode, rows_per, scale, eps, keep):
+    """(h, normed, rstd_post, rstd_pre), None where there is none."""
+    H, dev = y.shape[-1], y.device
+    rows = y.numel() // H
+    h = torch.empty_like(y)
+    normed = None if pre is None else torch.empty_like(y)
+    if not rows:
+        return h, normed, None, None
+    r1 = torch.empty(rows, dtype=_F32, device=dev) if keep and post is not None else None
+    r2 = torch.empty(rows, dtype=_F32, device=dev) if keep and pre is not None else None
+    with _lib.on_device(dev):
+        _lib.call("st_residual_norms_fwd", y.data_ptr(), residual.data_ptr(), _lib.ptr(post),
+                  _lib.ptr(pre), _lib.ptr(gate), mode, int(gate is not None and gate.dtype == _F32),
+                  rows_per, rows, H, scale, eps, h.data_ptr(), _lib.ptr(normed), _lib.ptr(r1),
+                  _lib.ptr(r2), _lib.stream_handle(dev))
+    return h, normed, r1, r2
+
+
+class _ResidualNorms(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, residual, post, pre, gate, mode, rows_per, scale, eps):
+        h, normed, r1, r2 = _residual_norms(y, residual, post, pre, gate, mode, rows_per, scale, eps,
+                                            True)
+        ctx.save_for_backward(y, residual, post, pre, gate, r1, r2)
+        ctx.meta = (mode, rows_per, scale, eps)
+        ctx.set_materialize_grads(False)
+        return h if normed is None else (h, normed)
+
+    @staticmethod
+    def backward(ctx, dh, dn=None):
+        _once()
+        if dh is None and dn is None:
+            return (None,) * 9
+        y, residual, post, pre, gate, r1, r2 = ctx.saved_tensors
+        mode, rows_per, scale, eps = ctx.meta
+        H, dev = y.shape[-1], y.device
+        rows = y.numel() // H
+        dh, dn = (None if g is None else _operand(g) for g in (dh, dn))
+        need = ctx.needs_input_grad
+        dy, dres = (torch.empty_like(y) if n else None for n in need[:2])
+        dpost = torch.empty(H, dtype=_F32, device=dev) if need[2] else None
+        dpre = torch.empty(H, dtype=_F32, device=dev) if need[3] and dn is not None else None
+        dgate = None
+        if need[4]:
+            dgate = torch.empty_like(gate, dtype=gate.dtype if mode == _lib.ST_GATE_FULL else _F32)
+        if not rows:
+            return dy, dres, *(None if g is None else g.zero_().to(p.dtype)
+                               for g, p in ((dpost, post), (dpre, pre), (dgate, gate))), *(None,) * 4
+        with _lib.on_device(dev):
+            nbytes = 0
+            if dpost is not None or dpre is not None or (dgate is not None
+                                                         and mode == _lib.ST_GATE_COLUMNS):
+                nbytes = _lib.query("st_residual_norms_workspace_bytes", rows, H,
+                                    rows_per if mode == _lib.ST_GATE_COLUMNS else rows)
+            ws = _scratch(dev, nbytes)
+            _lib.call("st_residual_norms_bwd", y.data_ptr(), residual.data_ptr(), _lib.ptr(post),
+                      _lib.ptr(pre), _lib.ptr(gate), mode,
+                      int(gate is not None and gate.dtype == _F32), rows_per, rows, H, scale, eps,
+                      _lib.ptr(r1), _lib.ptr(r2), _lib.ptr(dh), _lib.ptr(dn), _lib.ptr(dy),
+                      _lib.ptr(dres), _lib.ptr(dgate), _lib.ptr(dpost), _lib.ptr(dpre),
+                      _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+        return (dy, dres, *(None if g is None else g.to(p.dtype)
+                            for g, p in ((dpost, post), (dpre, pre), (dgate, gate))),
+                None, None, None, None)
+
+
+def _gate_kind(gate, shape):
+    """(kind, rows that share a row of it) of a gate for rows of ``shape``."""
+    got, H = tuple(gate.shape), shape[-1]
+    rows = math.prod(shape[:-1])
+    if got == shape:
+        return _lib.ST_GATE_FULL, 1
+    if got == (H,):
+        return _lib.ST_GATE_COLUMNS, max(1, rows)
+    if got == shape[:-1] + (1,):
+        return _lib.ST_GATE_TOKENS, 1
+    if len(shape) == 3 and got == (shape[0], 1, H):
+        return _lib.ST_GATE_COLUMNS, max(1, shape[1])
+    raise ValueError(f"unsupported_capability: a gate of {got} for {shape}: one value a channel [H], a "
+                     "row's channels [B, 1, H], a token [..., 1] or an entry")
+
+
+def residual_norms(y, residual, post=None, pre=None, *, gate=None, scale=1.0, eps=1e-6):
+    """What stands between two parts of a decoder block, in one pass: the norm after
+    a part's output ``y``, its gate and scale, the residual add, and the norm before
+    the next part (all bf16 [..., H], H at most 16384)::
+
+        z = rms(y) * post      (y itself without post)
+        h = residual + scale * gate * z
+        normed = rms(h) * pre
+
+    Returns ``h``, or ``(h, normed)`` with ``pre``.  ``rms(x)`` is ``x / sqrt(mean(x^2) +
+    eps)``; ``post`` and ``pre`` bf16 [H].  ``gate`` (bf16 or fp32): one value a
+    channel [H], the channels of each row of a batch [B, 1, H], one a token
+    [..., 1], or one an entry [..., H].
+
+    fp32 inside with each result rounded once (``normed`` comes from the unrounded
+    ``h``), unlike :func:`rms_norm`, which rounds where the reference's tensors do.
+    Differentiable in all five tensors; a shared weight's gradient is summed in fp32
+    in a fixed order."""
+    if y.dtype != _BF16 or residual.dtype != _BF16 or y.dim() < 1 or y.shape != residual.shape:
+        raise ValueError("unsupported_capability: residual_norms expects y and residual in bf16, of one "
+                         "shape [..., H]")
+    shape = tuple(y.shape)
+    H = shape[-1]
+    if not 1 <= H <= 16384:
+        raise ValueError(f"unsupported_capability: residual_norms takes hidden sizes of 1 to 16384, "
+                         f"not {H}")
+    for w, name in ((post, "post"), (pre, "pre")):
+        if w is not None and (w.dtype != _BF16 or tuple(w.shape) != (H,)):
+            raise ValueError(f"unsupported_capability: {name} must be bf16 [{H}]")
+    mode, rows_per = _lib.ST_GATE_NONE, 1
+    if gate is not None:
+        if gate.dtype not in (_BF16, _F32):
+            raise ValueError("unsupported_capability: a gate is bf16 or fp32")
+        mode, rows_per = _gate_kind(gate, shape)
+    scale, eps = float(scale), float(eps)
+    if not math.isfinite(scale) or not math.isfinite(eps) or eps < 0:
+        raise ValueError("unsupported_capability: scale must be finite, eps not negative")
+    given = (y, residual, post, pre, gate)
+    _no_tangents(*given)
+    if not y.is_cuda:
+        raise ValueError("unsupported_capability: residual_norms runs on the GPU")
+    if any(t is not None and t.device != y.device for t in given):
+        raise ValueError("unsupported_capability: all tensors on one device")
+    args = (*(None if t is None else _operand(t) for t in given), mode, rows_per, scale, eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+        return _ResidualNorms.apply(*args)
+    h, normed, _, _ = _residual_norms(*args, False)
+    return h if normed is None else (h, normed)
+
+
+# ----------------------------------------------------------------- embedding
+def _lookup(table, ids, scale):
+    V, H = table.shape
+    out = torch.empty((*ids.shape, H), dtype=_BF16, device=table.device)
+    with _lib.on_device(table.device):
+        _lib.call("st_embedding_fwd", table.data_ptr(),
+                  _lib.ST_DTYPE_F32 if table.dtype == _F32 else _lib.ST_DTYPE_BF16, ids.data_ptr(),
+                  int(ids.dtype == torch.int32), ids.numel(), V, H, scale, out.data_ptr(),
+                  _lib.stream_handle(table.device))
+    return out
+
+
+def _embedding_grad(grad, ids, dout, scale, padding_idx, accumulate):
+    """Writes (or adds) the gradient of a table into ``grad`` [V, H]."""
+    V, H = grad.shape
+    dev = grad.device
+    with _lib.on_device(dev):
+        nbytes = _lib.query("st_embedding_bwd_workspace_bytes", ids.numel(), V, H)
+        ws = _scratch(dev, nbytes)
+        _lib.call("st_embedding_bwd", dout.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int32),
+                  ids.numel(), V, H, scale, -1 if padding_idx is None else padding_idx,
+                  grad.data_ptr(), _lib.ST_DTYPE_F32 if grad.dtype == _F32 else _lib.ST_DTYPE_BF16,
+                  int(accumulate), _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.meta = (table.shape, table.dtype, scale, padding_idx)
+        return _lookup(table, ids, scale)
+
+    @staticmethod
+    def backward(ctx, dout):
+        _once()
+        (ids,) = ctx.saved_tensors
+        shape, dtype, scale, padding_idx = ctx.meta
+        grad = torch.empty(shape, dtype=dtype, device=dout.device)
+        _embedding_grad(grad, ids, _operand(dout), scale, padding_idx, False)
+        return grad, None, None, None
+
+
+def _embedding_args(table, ids, scale, padding_idx):
+    """``(ids on the table's device, scale)``, checked."""
+    if table.dim() != 2 or table.dtype not in (_BF16, _F32) or not all(table.shape):
+        raise ValueError("unsupported_capability: embedding takes a bf16 or fp32 table [V, H]")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError("unsupported_capability: ids must be int64 or int32")
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("unsupported_capability: scale must be finite")
+    if padding_idx is not None and (isinstance(padding_idx, bool) or not isinstance(padding_idx, int)
+                                    or not 0 <= padding_idx < table.shape[0]):
+        raise ValueError("unsupported_capability: padding_idx must be a row of the table")
+    if not table.is_cuda:
+        raise ValueError("unsupported_capability: embedding runs on the GPU")
+    if ids.device.type == "cpu":
+        if ids.numel() and not (0 <= int(ids.min()) and int(ids.max()) < table.shape[0]):
+            raise ValueError("unsupported_capability: ids must be rows of the table")
+        ids = ids.to(table.device)
+    if ids.device != table.device:
+        raise ValueError("unsupported_capability: ids and table on one device")
+    return ids.contiguous(), scale
+
+
+def embedding(table, ids, *, scale=1.0, padding_idx=None):
+    """``bf16(scale * table[ids])`` for a table [V, H] in bf16 or fp32 on the device
+    and ids (int64 or int32) of any shape: [..., H].
+
+    Differentiable in ``table``: its gradient (dense, of the table's type) is the
+    fp32 sum over each token's positions in rising order, the same bits every time;
+    positions of ``padding_idx`` pass none on.  An id outside the table is refused
+    when it comes from the host; on the device it gives NaN and no gradient."""
+    ids, scale = _embedding_args(table, ids, scale, padding_idx)
+    _no_tangents(table)
+    table = _operand(table)
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _Embedding.apply(table, ids, scale, padding_idx)
+    return _lookup(table, ids, scale)
+
+
 # ----------------------------------------------------------------- terminal
 def linear_bf16(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """``y = bf16(x w^T)`` on the MFMA GEMM (fp32 accumulation)."""
@@ -1263,6 +1477,6 @@ def attention_scale(head_dim: int) -> float:
 __all__ = ["Q4Weight", "concat_rows", "lora_fusable", "q4_lora_linear", "rms_norm", "rope_qkv", "rope_heads",
            "causal_attention", "swiglu", "swiglu_pair", "lora_gemm", "attention_scale",
            "mla_rope", "mla_attention",
-           "rms_norm_residual",
+           "rms_norm_residual", "residual_norms", "embedding",
            "linear_bf16", "linear_bf16_dgrad", "supervised_chunk_intervals",
            "chunked_causal_loss", "TokenLogProbs", "token_logprobs"]
