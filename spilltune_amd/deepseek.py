@@ -30,7 +30,7 @@ import math
 import torch
 
 from . import moe, ops, packed
-from .dense import CausalMask, key_lengths
+from .dense import CausalMask, key_lengths, valid_tokens
 
 ATTENTION_TARGETS_Q_LORA = ("self_attn.q_a_proj", "self_attn.q_b_proj",
                             "self_attn.kv_a_proj_with_mqa", "self_attn.kv_b_proj",
@@ -190,11 +190,13 @@ def deepseek_block(hidden_states, position_embeddings, attention_mask, *, parame
         return out.view(B, S, Hd)
     shared = {k: v for k, v in (("gate", lora_shared_gate), ("up", lora_shared_up),
                                 ("down", lora_shared_down)) if v is not None}
+    balance = c.get("balance")  # optional, an ExpertBalance
     routed_shared = moe.deepseek_moe_feed_forward(
-        xn2, w, num_experts=c["experts"], top_k=c["top_k"], groups=c["groups"],
+        xn2.view(B, S, Hd), w, num_experts=c["experts"], top_k=c["top_k"], groups=c["groups"],
         group_k=c["group_k"], normalize=c["normalize"], scale=c["router_scale"],
-        lora_shared=shared or None)
-    return (h1 + routed_shared).view(B, S, Hd)
+        lora_shared=shared or None, balance=balance,
+        valid=valid_tokens(attention_mask) if balance is not None else None)
+    return (h1 + routed_shared.view(B * S, Hd)).view(B, S, Hd)
 
 
 def make_deepseek_block(index: int, weights: dict, *, codec: str, parameters: dict, rank: int,

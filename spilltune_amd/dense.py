@@ -19,7 +19,9 @@ no reference to slot memory.  Differences in *how*, not *what*:
   kernel, exactly as adding ``finfo(bf16).min`` does (exp underflows to 0);
 * packed rows (no counterpart in the reference) come as a
   :class:`~spilltune_amd.packed.SpanMask` and as
-  :class:`~spilltune_amd.packed.Positions` in the place of (cos, sin).
+  :class:`~spilltune_amd.packed.Positions` in the place of (cos, sin);
+* norms on both sides of a part, its gate and a residual scale (no counterpart
+  either) go through :func:`~spilltune_amd.ops.residual_norms`.
 """
 from __future__ import annotations
 
@@ -53,6 +55,17 @@ def key_lengths(valid: torch.Tensor, device, what: str = "unsupported_capability
     return valid.sum(1).to(device=device, dtype=torch.int32)
 
 
+def valid_tokens(mask) -> torch.Tensor | None:
+    """The tokens of a batch that are not padding (bool [batch, length]; None: all),
+    from its attention mask: those within a row's valid prefix, or with a run of keys
+    to see."""
+    if isinstance(mask, packed.SpanMask):
+        return mask.key_end > mask.key_start
+    if mask is None or mask.lengths is None:
+        return None
+    return torch.arange(mask.length, device=mask.lengths.device) < mask.lengths[:, None]
+
+
 def positions_and_masks(valid: torch.Tensor, *, head_dim: int, theta: float, device,
                         dtype=torch.bfloat16, rotary=None):
     """Rotary tables (bf16 cos/sin [B,S,D]) and the causal mask marker
@@ -83,11 +96,21 @@ def _weight(weights, name):
 def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv_heads, head_dim,
                 eps, lora_q=None, lora_k=None, lora_v=None, lora_o=None, lora_gate=None,
                 lora_up=None, lora_down=None, qk_norm=False, feed_forward=None, moe=None,
-                lora_experts_gate_up=None, lora_experts_down=None, **weights):
-    """``moe`` (``num_experts``, ``top_k``, ``norm_topk_prob``) makes the
+                lora_experts_gate_up=None, lora_experts_down=None, post_norms=False,
+                residual_scale=1.0, **weights):
+    """``moe`` (``num_experts``, ``top_k``, ``norm_topk_prob``; optionally ``balance``,
+    a :class:`~spilltune_amd.moe.ExpertBalance`) makes the
     feed-forward the Qwen3-MoE block of qwen3_moe.py:95-113 over the slot's
     ``mlp.experts.*`` stacks, with the optional per-expert LoRA objects
-    ``lora_experts_gate_up`` / ``lora_experts_down``."""
+    ``lora_experts_gate_up`` / ``lora_experts_down``.
+
+    ``post_norms`` (no counterpart in the reference): attention and feed-forward are
+    normalised on both sides -- ``input_layernorm`` and ``post_attention_layernorm``
+    around the one, ``pre_feedforward_layernorm`` and ``post_feedforward_layernorm``
+    around the other.  ``residual_scale`` multiplies what a part adds to the residual,
+    and so do the per-channel gates ``self_attn.output_gate`` and ``mlp.output_gate``
+    ([hidden]) where the weights hold them.  Without any of these the block is the
+    reference's."""
     if attention_mask is not None and not isinstance(attention_mask, (CausalMask, packed.SpanMask)):
         raise ValueError("unsupported_capability: only the causal mask marker and span masks are "
                          "supported")
@@ -95,8 +118,11 @@ def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv
         from . import moe as moe_ops
 
         def feed_forward(x, w):
+            valid = valid_tokens(attention_mask) if moe.get("balance") is not None else None
             return moe_ops.moe_feed_forward(x, w, lora_gate_up=lora_experts_gate_up,
-                                            lora_down=lora_experts_down, **moe)
+                                            lora_down=lora_experts_down, valid=valid, **moe)
+    gates = weights.get("self_attn.output_gate"), weights.get("mlp.output_gate")
+    around = post_norms or residual_scale != 1.0 or any(g is not None for g in gates)
     B, S, Hd = hidden_states.shape
     by_position = isinstance(position_embeddings, packed.Positions)
     if by_position and (position_embeddings.rotary.head_dim != head_dim
@@ -152,9 +178,29 @@ def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv
         kv_len = attention_mask.lengths if attention_mask is not None else None
         attended = ops.causal_attention(q, k, v, ops.attention_scale(head_dim), kv_len)
     attended = attended.reshape(B * S, heads * head_dim)
-    h1 = ops.q4_lora_linear(attended, _weight(weights, "self_attn.o_proj"), [lora_o], residual=residual)
+    wo = _weight(weights, "self_attn.o_proj")
+    if around:
+        # norm, gate, scale and add of the part's output and the norm before the next
+        # in one kernel each way, in the place of the o and down epilogues' adds
+        after, before = ("post_attention_layernorm", "pre_feedforward_layernorm") if post_norms \
+            else (None, "post_attention_layernorm")
+        y = ops.q4_lora_linear(attended, wo, [lora_o])
+        h1, xn2 = ops.residual_norms(y, residual, weights[after + ".weight"] if after else None,
+                                     weights[before + ".weight"], gate=gates[0],
+                                     scale=residual_scale, eps=eps)
+    else:
+        h1 = ops.q4_lora_linear(attended, wo, [lora_o], residual=residual)
+        h1, xn2 = ops.rms_norm_residual(h1, weights["post_attention_layernorm.weight"], eps)
 
-    h1, xn2 = ops.rms_norm_residual(h1, weights["post_attention_layernorm.weight"], eps)
+    def joined(out):  # the block's output from its feed-forward's
+        if not around:
+            return out.view(B, S, Hd)
+        post = weights["post_feedforward_layernorm.weight"] if post_norms else None
+        return ops.residual_norms(out, h1, post, gate=gates[1], scale=residual_scale,
+                                  eps=eps).view(B, S, Hd)
+
+    if feed_forward is not None and around:
+        return joined(feed_forward(xn2.view(B, S, Hd), weights).reshape(B * S, Hd))
     if feed_forward is not None:  # e.g. the MoE block (dense.py:152)
         return (h1 + feed_forward(xn2.view(B, S, Hd), weights).reshape(B * S, Hd)).view(B, S, Hd)
     wg, wu = _weight(weights, "mlp.gate_proj"), _weight(weights, "mlp.up_proj")
@@ -162,16 +208,17 @@ def dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv
     loras_gu = [lora_gate, lora_up]
     inter = wg.out_features
     wd = _weight(weights, "mlp.down_proj")
+    add = None if around else h1
     if gu is not None and ops.lora_fusable(loras_gu, partial=True):
         # down reads silu(gate) * up of the fused gate|up output; its input-
         # gradient GEMM applies the SwiGLU VJP in the epilogue
         out = ops.q4_lora_linear(ops.q4_lora_linear(xn2, gu, loras_gu, partial=True), wd,
-                                 [lora_down], residual=h1, swiglu=True)
+                                 [lora_down], residual=add, swiglu=True)
     else:
         act = ops.swiglu_pair(ops.q4_lora_linear(xn2, wg, [lora_gate]),
                               ops.q4_lora_linear(xn2, wu, [lora_up]))
-        out = ops.q4_lora_linear(act, wd, [lora_down], residual=h1)
-    return out.view(B, S, Hd)
+        out = ops.q4_lora_linear(act, wd, [lora_down], residual=add)
+    return joined(out)
 
 
 def lora_kwargs(adapters: dict) -> dict:

@@ -22,6 +22,8 @@ I/O around it).
   :mod:`spilltune_amd.packed`) in all of the above, an ``objective`` on token log
   probabilities in the place of the cross-entropy, and :func:`score`, the log
   probabilities of given rows; these have no counterpart in the reference.
+* A :class:`~spilltune_amd.embedding.TokenEmbedding` in the place of the host table:
+  looked up on the device, scaled, trained with the adapters (no counterpart either).
 * :class:`DenseModel` -- the adapter surface the engine uses
   (adapters/protocol.py:23-34) for a Llama-family model whose decoder
   matrices are stored 4-bit.
@@ -35,6 +37,7 @@ import torch.nn.functional as F
 
 from . import ops, packed, slots
 from .dense import positions_and_masks
+from .embedding import TokenEmbedding
 from .recompute import (_borrow_weights, _call_functional_block, block_adapter_backward,
                         streaming_block)
 
@@ -60,6 +63,28 @@ def forward(model, session, hidden, positions, masks, *, accumulate=False):
                                  session.reloader(block), block.adapters, block.index,
                                  accumulate_adapter_grads=accumulate)
     return hidden
+
+
+def _trainables(model) -> dict:
+    """What an optimizer steps: the projections, and ``"embedding"`` where the model's
+    table is trained."""
+    result = flatten(model)
+    if isinstance(model.embedding, TokenEmbedding):
+        result["embedding"] = model.embedding
+    return result
+
+
+def _embed(model, input_ids):
+    """Rows of the model's table: a trained one's on the device, or the host's."""
+    if isinstance(model.embedding, TokenEmbedding):
+        return model.embedding(input_ids)
+    return F.embedding(input_ids.cpu(), model.embedding).to(model.device)
+
+
+def _embedding_grad(model, input_ids, gradient, accumulate):
+    """Takes the embedded rows' gradient into a trained table's."""
+    if isinstance(model.embedding, TokenEmbedding):
+        model.embedding.add_grad(input_ids, gradient, accumulate)
 
 
 def _row_inputs(model, input_ids, documents):
@@ -109,11 +134,10 @@ def microbatch(model, session, input_ids, labels, *, normalization, token_chunk,
     ``documents``: packed rows (labels across a document's start are dropped);
     ``objective``: a function of :class:`LabelLogProbs` (which tells it ``item``)
     to a scalar, in the place of the cross-entropy."""
-    device = model.device
     positions, masks = _row_inputs(model, input_ids, documents)
     if documents is not None:
         labels = packed.document_labels(labels, documents)
-    embedded = F.embedding(input_ids.cpu(), model.embedding).to(device).detach().requires_grad_(True)
+    embedded = _embed(model, input_ids).detach().requires_grad_(True)
     hidden = forward(model, session, embedded, positions, masks, accumulate=accumulate)
     terminal_input = hidden.detach().requires_grad_(True)
     normalized = model.terminal_norm(terminal_input)
@@ -123,6 +147,7 @@ def microbatch(model, session, input_ids, labels, *, normalization, token_chunk,
     if not torch.isfinite(loss) or not torch.isfinite(gradient).all():
         raise FloatingPointError("non-finite causal loss/gradient")
     hidden.backward(gradient)
+    _embedding_grad(model, input_ids, embedded.grad, accumulate)
     return float(loss.detach()), embedded.grad.detach().clone()
 
 
@@ -135,7 +160,7 @@ def score(model, session, input_ids, *, documents=None, top=0, temperature=1.0):
     with torch.no_grad():
         positions, masks = _row_inputs(model, input_ids, documents)
         tokens = input_ids if documents is None else packed.document_labels(input_ids, documents)
-        embedded = F.embedding(input_ids.cpu(), model.embedding).to(model.device)
+        embedded = _embed(model, input_ids)
         normalized = model.terminal_norm(forward(model, session, embedded, positions, masks))
         return ops.token_logprobs(normalized[:, :-1], model.head, tokens[:, 1:].to(torch.int64),
                                   top=top, temperature=temperature)
@@ -159,7 +184,6 @@ def window_layer_major(model, session, items, *, normalization, token_chunk, obj
     same order as the microbatch-major loop, so the gradients and losses are
     the same bits.  ``objective`` as for :func:`microbatch`; ``names`` its ``item`` of
     each microbatch (default 0, 1, ...).  Returns the per-microbatch losses."""
-    device = model.device
     names = range(len(items)) if names is None else names
     if len(names) != len(items):
         raise ValueError(f"unsupported_capability: {len(names)} names for {len(items)} microbatches")
@@ -168,8 +192,8 @@ def window_layer_major(model, session, items, *, normalization, token_chunk, obj
         positions, masks = _row_inputs(model, ids, *documents or [None])
         if documents and documents[0] is not None:
             labels = packed.document_labels(labels, documents[0])
-        embedded = F.embedding(ids.cpu(), model.embedding).to(device)
-        mbs.append({"pos": positions, "masks": masks, "h": [embedded], "labels": labels})
+        mbs.append({"ids": ids, "pos": positions, "masks": masks, "h": [_embed(model, ids)],
+                    "labels": labels})
     for block in model.blocks:
         with _borrow_weights(session.reloader(block), "forward") as weights, torch.no_grad():
             for mb in mbs:
@@ -196,6 +220,8 @@ def window_layer_major(model, session, items, *, normalization, token_chunk, obj
                                                  mb["masks"][block.kind], weights, block.kwargs)
                 # the first microbatch replaces (zero + add), later ones accumulate
                 mb["g"] = block_adapter_backward(out, hidden, ordered, mb["g"], k > 0, block.index)
+    for k, mb in enumerate(mbs):
+        _embedding_grad(model, mb["ids"], mb["g"], k > 0)
     return losses
 
 
@@ -248,7 +274,7 @@ def train(model, session, rows, *, steps, accumulation=1, lr=1e-4, weight_decay=
     place of the cross-entropy, see :func:`microbatch`.  ``optimizer`` (an
     :class:`AdamW` or :class:`~spilltune_amd.muon.Muon`, with its own rates) in the
     place of the AdamW of ``lr`` and ``weight_decay``."""
-    projections = flatten(model)
+    projections = _trainables(model)
     if optimizer is None:
         optimizer = AdamW(lr=lr, weight_decay=weight_decay)
     cursor, losses = 0, []
@@ -286,14 +312,24 @@ class DenseModel:
 
     def __init__(self, *, embedding, norm, head, layers=None, heads, kv_heads, head_dim, eps,
                  theta, rank, alpha, targets, device, codec="nf4-g128", generator=None,
-                 blocks=None, qk_norm=False, rotary=None):
-        """``layers``: per-layer weight dicts, encoded here; or ``blocks``:
+                 blocks=None, qk_norm=False, rotary=None, post_norms=False, residual_scale=1.0):
+        """``embedding``: a host table, or a :class:`~spilltune_amd.embedding.TokenEmbedding`
+        that is trained.  ``layers``: per-layer weight dicts, encoded here; or ``blocks``:
         prebuilt BlockPlans (e.g. ``slots.make_archive_block``).  ``rotary``: the
         model's :class:`~spilltune_amd.packed.Rotary`, of plain and of packed rows
         (default: whole heads, ``theta``, no scaling; plain rows then by bf16
-        tables)."""
+        tables).  ``post_norms`` and ``residual_scale`` of ``layers``: see
+        :func:`~spilltune_amd.dense.dense_block`."""
         self.device = torch.device(device)
-        self.embedding = embedding.to(torch.bfloat16).contiguous()      # stays on the host
+        if isinstance(embedding, TokenEmbedding):
+            if embedding.weight.device.type != self.device.type or (
+                    self.device.index is not None
+                    and embedding.weight.device.index != self.device.index):
+                raise ValueError("unsupported_capability: a trained embedding lives on the model's "
+                                 "device")
+            self.embedding = embedding
+        else:
+            self.embedding = embedding.to(torch.bfloat16).contiguous()      # stays on the host
         self.norm = norm.to(torch.bfloat16).to(self.device)
         self.head = head.to(torch.bfloat16).to(self.device)
         self.eps, self.theta, self.head_dim = eps, theta, head_dim
@@ -305,7 +341,8 @@ class DenseModel:
             slots.make_dense_block(i, w, codec=codec, heads=heads, kv_heads=kv_heads,
                                    head_dim=head_dim, eps=eps, rank=rank, alpha=alpha,
                                    targets=targets, device=self.device, generator=generator,
-                                   qk_norm=qk_norm)
+                                   qk_norm=qk_norm, post_norms=post_norms,
+                                   residual_scale=residual_scale)
             for i, w in enumerate(layers)]
 
     def positions_and_masks(self, valid):

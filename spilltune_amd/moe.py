@@ -25,6 +25,7 @@ benchmark configuration and is optional.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import NamedTuple, Optional
 
@@ -230,6 +231,60 @@ def balance_loss(logits, indices, *, score="softmax", valid=None, per_row=False)
         None if valid is None else valid.contiguous(), groups, int(score == "sigmoid")))
 
 
+class ExpertBalance:
+    """The balance term of an MoE layer (or of several that share the object): each
+    pass that is differentiated adds ``coefficient`` times :func:`balance_loss` of its
+    router to the loss whose gradient flows, and is counted here -- ``loss`` the sum of
+    the passes' losses (without the coefficient), ``counts`` (int64 [E]) of their picks,
+    both on the device, ``passes`` how many.  The routers are frozen: the term teaches
+    the adapters before them.
+
+    Every microbatch adds its own term, so a window of ``n`` of them that is to add one
+    average takes the coefficient over ``n``.  ``per_row`` balances each row by itself.
+    The term is in the gradients; the losses that the engine returns are without it."""
+
+    def __init__(self, coefficient: float, *, per_row: bool = False):
+        self.coefficient, self.per_row = float(coefficient), bool(per_row)
+        if not math.isfinite(self.coefficient):
+            raise ValueError("unsupported_capability: coefficient must be finite")
+        self.reset()
+
+    def reset(self):
+        self.loss, self.counts, self.passes = None, None, 0
+
+    def record(self, loss, counts):
+        loss, counts = loss.detach().clone(), counts.sum(0)
+        self.loss = loss if self.loss is None else self.loss + loss
+        self.counts = counts if self.counts is None else self.counts + counts
+        self.passes += 1
+
+
+class _WithTerm(torch.autograd.Function):
+    """``out``, whose backward also passes ``coefficient`` on to ``loss``: the gradient of
+    the sum of what ``out`` leads to and ``coefficient * loss``."""
+
+    @staticmethod
+    def forward(ctx, out, loss, coefficient):
+        ctx.coefficient = coefficient
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, dout):
+        return dout, torch.full((), ctx.coefficient, dtype=_F32, device=dout.device), None
+
+
+def _balanced(out, logits, indices, score, balance, valid, shape):
+    """``out`` with the balance term of its router attached, where a pass is
+    differentiated."""
+    if balance is None or not (torch.is_grad_enabled() and logits.requires_grad):
+        return out
+    lead = shape[:-1] if len(shape) > 1 else (1,)
+    loss, counts = balance_loss(logits.view(*lead, -1), indices.view(*lead, -1), score=score,
+                                valid=valid, per_row=balance.per_row)
+    balance.record(loss, counts)
+    return _WithTerm.apply(out, loss, balance.coefficient)
+
+
 # ----------------------------------------------------------------- the function
 def _stream(dev):
     return _lib.stream_handle(dev)
@@ -344,16 +399,18 @@ class _MoEFeedForward(torch.autograd.Function):
         ctx.meta = (gate_up, down, cfg, has_lora, has_gu, has_d)
         ctx.save_for_backward(flat, router, logits, weights, indices, offsets, row_token,
                               pick_row, gu, h, v, T_gu, T_d, A_gu, B_gu, A_d, B_d)
-        ctx.mark_non_differentiable(logits, weights, indices)
+        ctx.mark_non_differentiable(weights, indices)
+        ctx.set_materialize_grads(False)
         return out, logits, weights, indices
 
     @staticmethod
-    def backward(ctx, dout, _dlogits, _dweights, _dindices):
+    def backward(ctx, dout, given, _dweights, _dindices):
+        # `given`: the gradient of the logits from a loss on them (the balance loss)
         gate_up, down, cfg, has_lora, has_gu, has_d = ctx.meta
         top_k, norm, gu_rank, gu_scale, d_rank, d_scale, sig, groups, group_k, rscale = cfg
         (flat, router, logits, weights, indices, offsets, row_token, pick_row, gu, h, v,
          T_gu, T_d, A_gu, B_gu, A_d, B_d) = ctx.saved_tensors
-        dout = dout.contiguous()
+        dout = torch.zeros_like(flat) if dout is None else dout.contiguous()
         T, H = flat.shape
         E, I = gate_up.experts, down.in_features
         R = T * top_k
@@ -416,6 +473,8 @@ class _MoEFeedForward(torch.autograd.Function):
             dlogits = torch.empty((T, E), dtype=_F32, device=dev)
             _lib.call("st_moe_route_sigmoid_bwd", _lib.ptr(logits), _lib.ptr(indices),
                       _lib.ptr(dw), T, E, top_k, int(norm), float(rscale), _lib.ptr(dlogits), st)
+            if given is not None:
+                dlogits.add_(given)
             drouter = torch.empty((T, H), dtype=_F32, device=dev)
             if router.dtype == _BF16:
                 lora_gemm(T, H, E, dlogits, E, 1, router, H, 1, 1.0, drouter)
@@ -432,6 +491,8 @@ class _MoEFeedForward(torch.autograd.Function):
         dlogits = torch.empty((T, E), dtype=_BF16, device=dev)
         _lib.call("st_moe_route_softmax_bwd", _lib.ptr(logits), _lib.ptr(indices), _lib.ptr(dw),
                   T, E, top_k, int(norm), _lib.ptr(dlogits), st)
+        if given is not None:
+            dlogits.add_(given)
         Ec = E
         if E % 8:  # the GEMM contracts 16-byte chunks: zero-pad the expert dimension
             Ec = E + (-E) % 8
@@ -450,7 +511,7 @@ class _MoEFeedForward(torch.autograd.Function):
 
 
 def moe_feed_forward(hidden, weights, *, num_experts, top_k, norm_topk_prob, lora_gate_up=None,
-                     lora_down=None, return_routing=False):
+                     lora_down=None, return_routing=False, balance=None, valid=None):
     """``moe_feed_forward`` of qwen3_moe.py:95-113 on 4-bit experts.
 
     ``weights``: ``mlp.gate.weight`` (bf16 ``[E, H]`` router),
@@ -458,7 +519,9 @@ def moe_feed_forward(hidden, weights, *, num_experts, top_k, norm_topk_prob, lor
     (:class:`Q4Experts`, ``[E, 2I, H]`` and ``[E, H, I]``).  Optional
     ``lora_gate_up`` (:class:`ExpertLoRA`, 2 segments) and ``lora_down``
     (1 segment), either or both, adapt every expert.  With ``return_routing`` also returns the
-    ``(weights, indices)`` the router picked."""
+    ``(weights, indices)`` the router picked.  ``balance`` (:class:`ExpertBalance`) adds
+    its term to the loss that is differentiated, over the tokens marked in ``valid``
+    (bool, ``hidden``'s shape without the last; default all)."""
     router = weights["mlp.gate.weight"]
     gate_up = weights["mlp.experts.gate_up_proj"]
     down = weights["mlp.experts.down_proj"]
@@ -475,9 +538,9 @@ def moe_feed_forward(hidden, weights, *, num_experts, top_k, norm_topk_prob, lor
         raise ValueError("expert shapes do not match the router")
     cfg, lora = _lora_cfg(top_k, norm_topk_prob, lora_gate_up, lora_down,
                           (False, 0, 0, 1.0))
-    out, _, w, idx = _MoEFeedForward.apply(flat.contiguous(), router.detach().contiguous(), None,
-                                           gate_up, down, cfg, *lora)
-    out = out.reshape(shape)
+    out, logits, w, idx = _MoEFeedForward.apply(flat.contiguous(), router.detach().contiguous(),
+                                                None, gate_up, down, cfg, *lora)
+    out = _balanced(out, logits, idx, "softmax", balance, valid, shape).reshape(shape)
     return (out, w, idx) if return_routing else out
 
 
@@ -500,7 +563,7 @@ def _lora_cfg(top_k, normalize, lora_gate_up, lora_down, router_cfg):
 
 def deepseek_moe_feed_forward(hidden, weights, *, num_experts, top_k, groups, group_k,
                               normalize, scale, lora_gate_up=None, lora_down=None,
-                              lora_shared=None, return_routing=False):
+                              lora_shared=None, return_routing=False, balance=None, valid=None):
     """The MoE part of ``deepseek_block`` (adapters/deepseek.py:115-126,
     158-174) on 4-bit experts: ``route`` (fp32 sigmoid scores, selection by
     score + ``e_score_correction_bias`` among the ``group_k`` best of
@@ -518,7 +581,8 @@ def deepseek_moe_feed_forward(hidden, weights, *, num_experts, top_k, groups, gr
     ``mlp.shared_experts.{gate,up,down}_proj.weight`` (:class:`~spilltune_amd.ops.Q4Weight`).
     ``lora_shared`` optionally maps ``"gate"``, ``"up"``, ``"down"`` to LoRA
     projections of the shared expert; ``lora_gate_up``/``lora_down`` adapt
-    every routed expert (this build's extension, as for Qwen3)."""
+    every routed expert (this build's extension, as for Qwen3).  ``balance`` and
+    ``valid`` as for :func:`moe_feed_forward`, on the sigmoid scores."""
     from . import ops
     router = weights["mlp.gate.weight"]
     bias = weights["mlp.gate.e_score_correction_bias"]
@@ -540,9 +604,10 @@ def deepseek_moe_feed_forward(hidden, weights, *, num_experts, top_k, groups, gr
     cfg, lora = _lora_cfg(top_k, normalize, lora_gate_up, lora_down,
                           (True, int(groups), int(group_k), float(scale)))
     flat = flat.contiguous()
-    out, _, w, idx = _MoEFeedForward.apply(flat, router.detach().contiguous(),
-                                           bias.detach().float().contiguous(), gate_up, down,
-                                           cfg, *lora)
+    out, logits, w, idx = _MoEFeedForward.apply(flat, router.detach().contiguous(),
+                                                bias.detach().float().contiguous(), gate_up, down,
+                                                cfg, *lora)
+    out = _balanced(out, logits, idx, "sigmoid", balance, valid, shape)
     prefix = "mlp.shared_experts."
     if prefix + "gate_proj.weight" in weights:
         ls = lora_shared or {}

@@ -434,9 +434,16 @@ class ResidentSession:
         self.views.clear()
 
 
+def _around(post_norms, residual_scale) -> dict:
+    """dense_block's keywords for norms on both sides of a part and scaled residuals."""
+    return {**({"post_norms": True} if post_norms else {}),
+            **({"residual_scale": float(residual_scale)} if residual_scale != 1.0 else {})}
+
+
 def make_archive_block(reader, index: int, *, heads: int, kv_heads: int, head_dim: int,
                        eps: float, rank: int, alpha: float, targets, device, functional=None,
-                       generator=None, prefix: str | None = None, qk_norm: bool = False) -> BlockPlan:
+                       generator=None, prefix: str | None = None, qk_norm: bool = False,
+                       post_norms: bool = False, residual_scale: float = 1.0) -> BlockPlan:
     """A BlockPlan for layer ``index`` of an ``archive.ArchiveReader``: storage
     specs from the archive manifest, raw entries as meta tensors (layout only);
     pass ``reader.image_loader(prefix)`` to the session to fill its image."""
@@ -452,6 +459,7 @@ def make_archive_block(reader, index: int, *, heads: int, kv_heads: int, head_di
               **lora_kwargs(adapters)}
     if qk_norm:
         kwargs["qk_norm"] = True
+    kwargs.update(_around(post_norms, residual_scale))
     return BlockPlan(index, "full_attention", functional or dense_block, kwargs, host, adapters,
                      specs)
 
@@ -459,7 +467,8 @@ def make_archive_block(reader, index: int, *, heads: int, kv_heads: int, head_di
 def make_dense_block(index: int, weights: dict, *, codec: str, heads: int, kv_heads: int,
                      head_dim: int, eps: float, rank: int, alpha: float, targets, device,
                      functional=None, generator=None, qk_norm: bool = False, moe=None,
-                     expert_lora_rank: int = 0, expert_lora_alpha: float = 16.0) -> BlockPlan:
+                     expert_lora_rank: int = 0, expert_lora_alpha: float = 16.0,
+                     post_norms: bool = False, residual_scale: float = 1.0) -> BlockPlan:
     """Encode one dense decoder layer (``weights``: name -> CPU fp32/bf16 tensor,
     HF names without the ``model.layers.{i}.`` prefix) into a BlockPlan whose
     host weights are the flattened 4-bit records (codecs.flatten layout of the
@@ -470,7 +479,8 @@ def make_dense_block(index: int, weights: dict, *, codec: str, heads: int, kv_he
     ``mlp.experts.down_proj [E, H, I]`` stacks 4-bit in the same image, so the
     whole decoder layer, every expert included, moves through the slot as in
     qwen3_moe.py:146-152; the router ``mlp.gate.weight`` stays bf16.
-    ``expert_lora_rank`` > 0 adds per-expert LoRA on gate|up and down."""
+    ``expert_lora_rank`` > 0 adds per-expert LoRA on gate|up and down.
+    ``post_norms`` and ``residual_scale``: see ``dense.dense_block``."""
     from .dense import dense_block, lora_kwargs
     from .lora import create_lora_for_block
     host, specs = {}, {}
@@ -503,6 +513,7 @@ def make_dense_block(index: int, weights: dict, *, codec: str, heads: int, kv_he
         kwargs["qk_norm"] = True
     if moe is not None:
         kwargs["moe"] = dict(moe)
+    kwargs.update(_around(post_norms, residual_scale))
     return BlockPlan(index, "full_attention", functional or dense_block, kwargs, host, adapters,
                      specs)
 
