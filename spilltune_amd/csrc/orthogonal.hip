@@ -27,8 +27,9 @@
 namespace {
 
 typedef double d4 __attribute__((ext_vector_type(4)));
+typedef double d2 __attribute__((ext_vector_type(2)));
 constexpr int NTH = 256;
-constexpr int MAXE = 60;        // entries of a launch's table (kernel arguments: 4 KB)
+constexpr int MAXE = 54;        // entries of a launch's table (kernel arguments: 4 KB)
 constexpr int64_t MAXR = 1024;  // short side
 
 // A batch of equal matrices, back to back.
@@ -36,28 +37,27 @@ struct Entry {
   const void* x;
   void* out;
   int64_t part, poly;      // its first matrix's place in the two scratch areas (doubles)
-  int32_t K, r, chunks;    // long and short side, chunks of the long side in gram
-  int32_t tall;            // the short side is the contiguous one
-  uint32_t tile0;          // its first workgroup in the present launch
-  int32_t vec;             // rows may be read four elements at a time
+  int32_t K, r;            // long and short side
+  int32_t CH, chunks;      // long elements of a workgroup in gram, and its workgroups
+  int32_t AL;              // long elements of a workgroup in apply
+  int16_t tall;            // the short side is the contiguous one
+  int16_t vec;             // rows may be read four elements at a time
 };
 struct Table {
   Entry e[MAXE];
+  uint32_t tile0[64];  // the entries' first workgroups in the present launch, then ~0
   int32_t n, steps;
-  int32_t CH, AL;  // long elements of a workgroup in gram and apply
   double a, b, c, eps;
 };
 
-__device__ __forceinline__ const Entry& find(const Table& t, uint32_t b) {
-  int lo = 0, hi = t.n - 1;  // the last entry with tile0 <= b
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.e[mid].tile0 <= b)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return t.e[lo];
+// The last entry with tile0 <= b and its place among the entry's workgroups: one
+// load for all entries (a search would be six dependent ones, 1 us of each
+// workgroup's time).
+__device__ __forceinline__ const Entry& find(const Table& t, uint32_t b, uint32_t& w) {
+  const uint32_t mine = t.tile0[threadIdx.x & 63];
+  const int i = __popcll(__ballot(mine <= b)) - 1;
+  w = b - __builtin_amdgcn_readlane(mine, i);
+  return t.e[i];
 }
 
 template <bool BF>
@@ -110,44 +110,100 @@ __device__ __forceinline__ void store_upto4(void* p, int64_t i, int n, bool vec,
 
 // ---------------------------------------------------------------- G = U U'
 // One workgroup: a chunk of the long side and one block pair (I <= J) of 16 T short
-// rows each.  A wave takes 32 long elements at a time, of which lane group q holds
-// eight: in a wide matrix 8q..8q+7 (128 contiguous bytes a row), in a tall one
-// 4s + q, s = 0..7 (whole contiguous rows).  Which element is which k does not
-// matter to a sum over all of them, as long as both operands agree.
-template <bool BF, int T>
+// rows each, of which the tiles on and above the diagonal are formed.  A wave takes 32
+// long elements at a time, of which lane group q holds eight: in a wide matrix
+// 8q..8q+7 (128 contiguous bytes a row), in a tall one 4s + q, s = 0..7 (whole
+// contiguous rows).  Which element is which k does not matter to a sum over all of
+// them, as long as both operands agree.
+//
+// FULL: all 32 are inside and may be read four at a time.  Then there is no branch
+// around a load (rows past the short side read the last one and are cleared), which
+// would make the wave wait for it at the branch's end; the elements that follow are
+// under way while the present ones are multiplied.
+template <bool BF, int T, bool TALL, bool FULL>
 __device__ __forceinline__ void gram_rows(const Entry& e, const void* x, int row0, int64_t k0,
                                           int64_t kend, int lane, float (&u)[T][8]) {
   const int m = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int t = 0; t < T; ++t) {
-    const int i = row0 + 16 * t + m;
-    if (i >= e.r) {
-#pragma unroll
-      for (int s = 0; s < 8; ++s) u[t][s] = 0.0f;
-    } else if (e.tall) {
+    const int i = row0 + 16 * t + m, at = i < e.r ? i : e.r - 1;
+    if constexpr (TALL) {
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
         const int64_t k = k0 + 4 * s + q;
-        u[t][s] = k < kend ? load1<BF>(x, k * e.r + i) : 0.0f;
+        u[t][s] = FULL || k < kend ? load1<BF>(x, k * e.r + at) : 0.0f;
       }
     } else {
       const int64_t k = k0 + 8 * q;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int64_t left = kend - k - 4 * h;
-        load_upto4<BF>(x, (int64_t)i * e.K + k + 4 * h, (int)(left < 4 ? left : 4), e.vec,
-                       u[t] + 4 * h);
+        if constexpr (FULL) {
+          load4<BF>(x, (int64_t)at * e.K + k + 4 * h, u[t] + 4 * h);
+        } else {
+          const int64_t left = kend - k - 4 * h;
+          load_upto4<BF>(x, (int64_t)at * e.K + k + 4 * h, (int)(left < 4 ? left : 4), e.vec,
+                         u[t] + 4 * h);
+        }
       }
     }
+  }
+}
+template <int T>
+__device__ __forceinline__ void clear_rows(const Entry& e, int row0, int lane, float (&u)[T][8]) {
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int s = 0; s < 8; ++s) u[t][s] = row0 + 16 * t + (lane & 15) < e.r ? u[t][s] : 0.0f;
+}
+
+// acc[i][j] += rows rowa + 16 i times rows rowb + 16 j over k0, k0 + step, .. < k1;
+// SAME: the two are one, and the tiles below the diagonal stay out.
+template <bool BF, int T, bool TALL, bool SAME>
+__device__ __forceinline__ void gram_walk(const Entry& e, const void* x, int rowa, int rowb,
+                                          int64_t k0, int64_t k1, int step, int lane,
+                                          d4 (&acc)[T][T]) {
+  auto multiply = [&](float (&a)[T][8], float (&b)[T][8]) {
+    clear_rows<T>(e, rowa, lane, a);
+    if constexpr (!SAME) clear_rows<T>(e, rowb, lane, b);
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = SAME ? i : 0; j < T; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(
+              (double)a[i][s], (double)(SAME ? a : b)[j][s], acc[i][j], 0, 0, 0);
+  };
+  float a[T][8], b[T][8], na[T][8], nb[T][8];
+  if (e.vec || TALL) {
+    if (k0 + 32 <= k1) {
+      gram_rows<BF, T, TALL, true>(e, x, rowa, k0, k1, lane, na);
+      if constexpr (!SAME) gram_rows<BF, T, TALL, true>(e, x, rowb, k0, k1, lane, nb);
+    }
+    for (; k0 + 32 <= k1; k0 += step) {
+      const int64_t next = k0 + step + 32 <= k1 ? k0 + step : k0;
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int s = 0; s < 8; ++s) a[i][s] = na[i][s], b[i][s] = SAME ? 0.0f : nb[i][s];
+      gram_rows<BF, T, TALL, true>(e, x, rowa, next, k1, lane, na);
+      if constexpr (!SAME) gram_rows<BF, T, TALL, true>(e, x, rowb, next, k1, lane, nb);
+      multiply(a, b);
+    }
+  }
+  for (; k0 < k1; k0 += step) {
+    gram_rows<BF, T, TALL, false>(e, x, rowa, k0, k1, lane, a);
+    if constexpr (!SAME) gram_rows<BF, T, TALL, false>(e, x, rowb, k0, k1, lane, b);
+    multiply(a, b);
   }
 }
 
 template <int T, bool BF>
 __global__ __launch_bounds__(NTH) void gram(Table tab, double* __restrict__ part) {
-  __shared__ double sum[T * T * 256];
-  const Entry& e = find(tab, blockIdx.x);
+  __shared__ double sum[T < 4 ? T * T * 256 : 1];
+  uint32_t w;
+  const Entry& e = find(tab, blockIdx.x, w);
   const int nb = T < 4 ? 1 : (e.r + 63) / 64, pairs = nb * (nb + 1) / 2;
-  const uint32_t w = blockIdx.x - e.tile0;
   const int pair = (int)(w % pairs);
   const uint32_t mc = w / pairs;  // matrix * chunks + chunk
   const int64_t mat = mc / e.chunks, chunk = mc % e.chunks;
@@ -155,152 +211,229 @@ __global__ __launch_bounds__(NTH) void gram(Table tab, double* __restrict__ part
   while (J >= nb - I) J -= nb - I, ++I;
   J += I;
   const void* x = (const char*)e.x + mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t k1 = (chunk + 1) * tab.CH < e.K ? (chunk + 1) * tab.CH : e.K;
-  const bool diag = I == J;
-  d4 acc[T][T] = {};
-  for (int64_t k0 = chunk * tab.CH + 32 * wave; k0 < k1; k0 += 128) {
-    float a[T][8], b[T][8];
-    gram_rows<BF, T>(e, x, I * 16 * T, k0, k1, lane, a);
-    if (T == 4 && !diag) {
-      gram_rows<BF, T>(e, x, J * 16 * T, k0, k1, lane, b);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t k0 = chunk * e.CH, k1 = k0 + e.CH < e.K ? k0 + e.CH : e.K;
+  double* to = part + e.part + ((int64_t)mc * pairs + pair) * (T * T * 256);
+  if constexpr (T == 4) {
+    // Each wave a quarter of the block, two tiles by two, over the whole chunk: 32
+    // registers of sums leave room for more waves, and for the elements under way.
+    const int wi = wave >> 1, wj = wave & 1;
+    if (I == J && wi > wj) return;
+    d4 acc[2][2] = {};
+    const int ra = I * 64 + 32 * wi, rb = J * 64 + 32 * wj;
+    if (e.tall)
+      gram_walk<BF, 2, true, false>(e, x, ra, rb, k0, k1, 32, lane, acc);
+    else
+      gram_walk<BF, 2, false, false>(e, x, ra, rb, k0, k1, 32, lane, acc);
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < T; ++i)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int j = 0; j < T; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[i][s], (double)b[j][s],
-                                                             acc[i][j], 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
+        for (int v = 0; v < 4; ++v)
+          to[((2 * wi + i) * 4 + 2 * wj + j) * 256 + v * 64 + lane] = acc[i][j][v];
+  } else {
+    d4 acc[T][T] = {};
+    if (e.tall)
+      gram_walk<BF, T, true, true>(e, x, 0, 0, k0 + 32 * wave, k1, 128, lane, acc);
+    else
+      gram_walk<BF, T, false, true>(e, x, 0, 0, k0 + 32 * wave, k1, 128, lane, acc);
+    // the waves' sums in their order, so that the result does not depend on the time
+    for (int o = 0; o < NTH / 64; ++o) {
+      if (wave == o) {
 #pragma unroll
         for (int i = 0; i < T; ++i)
 #pragma unroll
           for (int j = i; j < T; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[i][s], (double)a[j][s],
-                                                             acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const int at = (i * T + j) * 256 + v * 64 + lane;
+              sum[at] = o ? sum[at] + acc[i][j][v] : acc[i][j][v];
+            }
+      }
+      __syncthreads();
     }
+    for (int i = threadIdx.x; i < T * T * 256; i += NTH)
+      if (i / 256 / T <= i / 256 % T) to[i] = sum[i];
   }
-  // the waves' sums in their order, so that the result does not depend on the time
-  for (int o = 0; o < NTH / 64; ++o) {
-    if (wave == o) {
-#pragma unroll
-      for (int i = 0; i < T; ++i)
-#pragma unroll
-        for (int j = 0; j < T; ++j)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int at = (i * T + j) * 256 + v * 64 + lane;
-            sum[at] = o ? sum[at] + acc[i][j][v] : acc[i][j][v];
-          }
-    }
-    __syncthreads();
-  }
-  double* to = part + e.part + ((int64_t)mc * pairs + pair) * (T * T * 256);
-  for (int i = threadIdx.x; i < T * T * 256; i += NTH) to[i] = sum[i];
 }
 
-// Element (row, col) of G from the chunks' partial sums; tiles below a diagonal
-// block's diagonal were not formed.
-template <int T>
-__device__ __forceinline__ double gram_at(const double* part, int chunks, int nb, int row, int col) {
-  int bi = row / (16 * T), bj = col / (16 * T);
-  if (bi > bj || (bi == bj && row / 16 > col / 16)) {
+// Element (row, col) of U U' from sums over blocks of 64 short rows; what lies below
+// the diagonal was not formed, or is not the upper half's to the bit.
+__device__ __forceinline__ double gram_at(const double* part, int nb, int row, int col) {
+  if (row > col) {
     const int s = row;
     row = col, col = s;
-    bi = row / (16 * T), bj = col / (16 * T);
   }
-  const int pair = bi * nb - bi * (bi - 1) / 2 + bj - bi, pairs = nb * (nb + 1) / 2;
-  const int i = row / 16 % T, j = col / 16 % T, m = row % 16;
-  const double* p = part + (int64_t)pair * (T * T * 256) + (i * T + j) * 256 + m / 4 * 64 +
-                    m % 4 * 16 + col % 16;
-  double s = 0.0;
-  for (int c = 0; c < chunks; ++c) s += p[(int64_t)c * pairs * (T * T * 256)];
-  return s;
+  const int bi = row / 64, bj = col / 64;
+  const int pair = bi * nb - bi * (bi - 1) / 2 + bj - bi;
+  const int tile = row / 16 % 4 * 4 + col / 16 % 4, m = row % 16;
+  return part[(int64_t)pair * 4096 + tile * 256 + m / 4 * 64 + m % 4 * 16 + col % 16];
+}
+
+// ---------------------------------------------------------------- P, r <= 16
+// One wave holds everything in registers: register v of lane (m, q) is element
+// [4v + q][m], which is what a product wants of either operand, so a product of two
+// symmetric matrices is four instructions on the registers they lie in.  Two sums
+// each, as an instruction waits 75 ns for the sum before it.
+__device__ __forceinline__ d4 product16(d4 a, d4 b) {
+  d4 x = {0.0, 0.0, 0.0, 0.0}, y = x;
+  x = __builtin_amdgcn_mfma_f64_16x16x4f64(a[0], b[0], x, 0, 0, 0);
+  y = __builtin_amdgcn_mfma_f64_16x16x4f64(a[1], b[1], y, 0, 0, 0);
+  x = __builtin_amdgcn_mfma_f64_16x16x4f64(a[2], b[2], x, 0, 0, 0);
+  y = __builtin_amdgcn_mfma_f64_16x16x4f64(a[3], b[3], y, 0, 0, 0);
+  return x + y;
+}
+// The upper half in both places; `turn` is 16 x 17 doubles of this wave's own.
+__device__ __forceinline__ d4 mirrored(d4 g, double* turn, int m, int q) {
+#pragma unroll
+  for (int v = 0; v < 4; ++v) turn[(4 * v + q) * 17 + m] = g[v];
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const double t = turn[m * 17 + 4 * v + q];
+    if (4 * v + q > m) g[v] = t;
+  }
+  __builtin_amdgcn_wave_barrier();
+  return g;
+}
+// P of the sums `g` (register v of lane (m, q): [4v + q][m], zero from r on).
+__device__ __forceinline__ d4 steps16(const Table& tab, d4 g, double* turn, int m, int q) {
+  double trace = 0.0;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) trace += 4 * v + q == m ? g[v] : 0.0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) trace += __shfl_xor(trace, o);
+  const double inv = 1.0 / (sqrt(trace) + tab.eps);
+  d4 one, P;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) one[v] = 4 * v + q == m ? 1.0 : 0.0;
+  d4 G = mirrored(g * inv * inv, turn, m, q);
+  P = one * inv;
+  for (int s = 0; s < tab.steps; ++s) {
+    const d4 Q = product16(G, G) * tab.c + G * tab.b + one * tab.a;
+    P = product16(Q, P);
+    if (s + 1 < tab.steps) G = mirrored(product16(product16(Q, G), Q), turn, m, q);
+  }
+  return P;
+}
+
+__global__ __launch_bounds__(64) void poly16(Table tab, const double* __restrict__ part,
+                                             double* __restrict__ poly) {
+  __shared__ double turn[16 * 17];
+  uint32_t mat;
+  const Entry& e = find(tab, blockIdx.x, mat);
+  const int lane = threadIdx.x, m = lane & 15, q = lane >> 4;
+  const double* p = part + e.part + (int64_t)mat * e.chunks * 256 + lane;
+  d4 g = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+  for (int c = 0; c < e.chunks; ++c)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) g[v] += p[c * 256 + v * 64];
+  const d4 P = steps16(tab, g, turn, m, q);
+#pragma unroll
+  for (int v = 0; v < 4; ++v) poly[e.poly + (int64_t)mat * 256 + v * 64 + lane] = P[v];
 }
 
 // ---------------------------------------------------------------- P, r <= 64
-// One workgroup of T waves a matrix, everything in LDS; wave w forms tile row w.
+// One workgroup of four waves a matrix, everything in LDS; T tiles of 16 rows, tile
+// (w, j) the work of wave (w T + j) % 4.
 template <int T>
-__device__ __forceinline__ void small_product(const double* A, const double* B, int w, int lane,
-                                              d4 (&acc)[T]) {
+__device__ __forceinline__ d4 product_tile(const double* A, const double* B, int w, int j, int lane) {
   constexpr int R = 16 * T;
   const int m = lane & 15, q = lane >> 4;
+  d4 x = {0.0, 0.0, 0.0, 0.0}, y = x;
 #pragma unroll
-  for (int j = 0; j < T; ++j) acc[j] = d4{0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-  for (int k = 0; k < R; k += 4) {
-    const double a = A[(k + q) * R + 16 * w + m];  // A symmetric
-#pragma unroll
-    for (int j = 0; j < T; ++j)
-      acc[j] = __builtin_amdgcn_mfma_f64_16x16x4f64(a, B[(k + q) * R + 16 * j + m], acc[j], 0, 0, 0);
+  for (int k = 0; k < R; k += 8) {
+    x = __builtin_amdgcn_mfma_f64_16x16x4f64(A[(k + q) * R + 16 * w + m],  // A symmetric
+                                             B[(k + q) * R + 16 * j + m], x, 0, 0, 0);
+    y = __builtin_amdgcn_mfma_f64_16x16x4f64(A[(k + 4 + q) * R + 16 * w + m],
+                                             B[(k + 4 + q) * R + 16 * j + m], y, 0, 0, 0);
   }
-}
-template <int T>
-__device__ __forceinline__ void small_store(double* D, int w, int lane, const d4 (&acc)[T]) {
-  constexpr int R = 16 * T;
-#pragma unroll
-  for (int j = 0; j < T; ++j)
-#pragma unroll
-    for (int v = 0; v < 4; ++v)
-      D[(16 * w + 4 * v + (lane >> 4)) * R + 16 * j + (lane & 15)] = acc[j][v];
+  return x + y;
 }
 
 template <int T>
-__global__ __launch_bounds__(64 * T) void poly_small(Table tab, const double* __restrict__ part,
-                                                     double* __restrict__ poly) {
-  constexpr int R = 16 * T, N = R * R;
+__global__ __launch_bounds__(NTH) void poly_small(Table tab, const double* __restrict__ part,
+                                                  double* __restrict__ poly) {
+  constexpr int R = 16 * T, N = R * R, OWN = T * T / 4;  // tiles of a wave
   __shared__ double G[N], Q[N], P[N];
-  const Entry& e = find(tab, blockIdx.x);
-  const int64_t mat = blockIdx.x - e.tile0;
-  const double* mine = part + e.part + mat * e.chunks * (T * T * 256);
-  for (int i = threadIdx.x; i < N; i += 64 * T)
-    G[i] = gram_at<T>(mine, e.chunks, 1, i / R, i % R);
+  uint32_t mat;
+  const Entry& e = find(tab, blockIdx.x, mat);
+  const double* mine = part + e.part + (int64_t)mat * e.chunks * N;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
+  // the tiles on and above the diagonal, as the waves of gram left them
+  for (int i = threadIdx.x; i < N; i += NTH) {
+    const int row = i / 256 / T * 16 + (i & 255) / 64 * 4 + (i & 63) / 16;
+    const int col = i / 256 % T * 16 + (i & 15);
+    if (row > col) continue;
+    double s = 0.0;
+#pragma unroll 4
+    for (int c = 0; c < e.chunks; ++c) s += mine[(int64_t)c * N + i];
+    G[row * R + col] = G[col * R + row] = s;
+  }
   __syncthreads();
   double trace = 0.0;
   for (int i = 0; i < e.r; ++i) trace += G[i * R + i];
   __syncthreads();
   const double inv = 1.0 / (sqrt(trace) + tab.eps);
-  for (int i = threadIdx.x; i < N; i += 64 * T) {
+  for (int i = threadIdx.x; i < N; i += NTH) {
     G[i] = G[i] * inv * inv;
     P[i] = i / R == i % R ? inv : 0.0;
   }
   __syncthreads();
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int s = 0; s < tab.steps; ++s) {
-    d4 x[T], h[T];
-    small_product<T>(G, G, w, lane, x);
+    const bool more = s + 1 < tab.steps;
+    d4 x[OWN], h[OWN];
 #pragma unroll
-    for (int j = 0; j < T; ++j)
+    for (int o = 0; o < OWN; ++o) {
+      const int t = o * 4 + wave, w = t / T, j = t % T;
+      x[o] = product_tile<T>(G, G, w, j, lane);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const int row = 16 * w + 4 * v + (lane >> 4), col = 16 * j + (lane & 15);
-        Q[row * R + col] =
-            tab.c * x[j][v] + tab.b * G[row * R + col] + (row == col ? tab.a : 0.0);
+        const int at = (16 * w + 4 * v + q) * R + 16 * j + m;
+        Q[at] = tab.c * x[o][v] + tab.b * G[at] + (16 * w + 4 * v + q == 16 * j + m ? tab.a : 0.0);
       }
+    }
     __syncthreads();
-    small_product<T>(Q, P, w, lane, x);
-    if (s + 1 < tab.steps) small_product<T>(Q, G, w, lane, h);
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int t = o * 4 + wave;
+      x[o] = product_tile<T>(Q, P, t / T, t % T, lane);
+      if (more) h[o] = product_tile<T>(Q, G, t / T, t % T, lane);
+    }
     __syncthreads();
-    small_store<T>(P, w, lane, x);
-    if (s + 1 < tab.steps) {
-      small_store<T>(G, w, lane, h);  // Q G
-      __syncthreads();
-      small_product<T>(G, Q, w, lane, x);
-      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < T; ++j)
+    for (int o = 0; o < OWN; ++o) {
+      const int t = o * 4 + wave;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int row = 16 * w + 4 * v + (lane >> 4), col = 16 * j + (lane & 15);
-          if (row <= col) G[row * R + col] = G[col * R + row] = x[j][v];
-        }
+      for (int v = 0; v < 4; ++v) {
+        const int at = (16 * (t / T) + 4 * v + q) * R + 16 * (t % T) + m;
+        P[at] = x[o][v];
+        if (more) G[at] = h[o][v];  // Q G
+      }
+    }
+    __syncthreads();
+    if (!more) break;
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int t = o * 4 + wave;
+      if (t / T <= t % T) x[o] = product_tile<T>(G, Q, t / T, t % T, lane);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int t = o * 4 + wave;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int row = 16 * (t / T) + 4 * v + q, col = 16 * (t % T) + m;
+        if (row <= col) G[row * R + col] = G[col * R + row] = x[o][v];
+      }
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < N; i += 64 * T) poly[e.poly + mat * N + i] = P[i];
+  for (int i = threadIdx.x; i < N; i += NTH) poly[e.poly + (int64_t)mat * N + i] = P[i];
 }
 
 // ---------------------------------------------------------------- P, larger r
@@ -308,32 +441,44 @@ __global__ __launch_bounds__(64 * T) void poly_small(Table tab, const double* __
 // scratch: G, Q, P (two, in turn) and H = Q G, one behind the other.
 enum { SLOT_G, SLOT_Q, SLOT_P0, SLOT_P1, SLOT_H, SLOTS };
 
-__global__ __launch_bounds__(NTH) void poly_sum(Table tab, const double* __restrict__ part,
-                                                double* __restrict__ poly) {
-  const Entry& e = find(tab, blockIdx.x);
-  const int nb = (e.r + 63) / 64, R = 64 * nb;
-  const uint32_t w = blockIdx.x - e.tile0, per = (uint32_t)R * R / 1024;
-  const int64_t mat = w / per;
-  const double* mine = part + e.part + mat * e.chunks * (nb * (nb + 1) / 2) * 4096;
-  double* to = poly + e.poly + mat * SLOTS * R * R + (int64_t)SLOT_H * R * R;
-  for (int i = threadIdx.x; i < 1024; i += NTH) {
-    const int at = (int)(w % per) * 1024 + i;
-    to[at] = gram_at<4>(mine, e.chunks, nb, at / R, at % R);
+// The chunks' sums joined into the first chunk's place.
+__global__ __launch_bounds__(NTH) void poly_sum(Table tab, double* __restrict__ part) {
+  uint32_t w;
+  const Entry& e = find(tab, blockIdx.x, w);
+  const int nb = (e.r + 63) / 64, pairs = nb * (nb + 1) / 2;
+  const uint32_t per = pairs * 4096 / (2 * NTH);
+  double2* p = (double2*)(part + e.part + (int64_t)(w / per) * e.chunks * pairs * 4096) +
+               (w % per) * NTH + threadIdx.x;
+  double2 s = make_double2(0.0, 0.0);
+#pragma unroll 4
+  for (int c = 0; c < e.chunks; ++c) {
+    const double2 x = p[(int64_t)c * pairs * 2048];
+    s.x += x.x, s.y += x.y;
   }
+  *p = s;
 }
 
-__global__ __launch_bounds__(NTH) void poly_norm(Table tab, double* __restrict__ poly) {
-  const Entry& e = find(tab, blockIdx.x);
-  const int R = (e.r + 63) / 64 * 64;
-  const uint32_t w = blockIdx.x - e.tile0, per = (uint32_t)R * R / 1024;
+// G = U U' / (|U|_F + eps)^2 and P = I / (|U|_F + eps), from the joined sums.
+__global__ __launch_bounds__(NTH) void poly_norm(Table tab, const double* __restrict__ part,
+                                                 double* __restrict__ poly) {
+  __shared__ double red[NTH / 64];
+  uint32_t w;
+  const Entry& e = find(tab, blockIdx.x, w);
+  const int nb = (e.r + 63) / 64, R = 64 * nb;
+  const uint32_t per = (uint32_t)R * R / 1024;
+  const double* mine = part + e.part + (int64_t)(w / per) * e.chunks * (nb * (nb + 1) / 2) * 4096;
   double* base = poly + e.poly + (int64_t)(w / per) * SLOTS * R * R;
-  const double* raw = base + (int64_t)SLOT_H * R * R;
   double trace = 0.0;
-  for (int i = 0; i < e.r; ++i) trace += raw[(int64_t)i * R + i];
+  for (int i = threadIdx.x; i < e.r; i += NTH) trace += gram_at(mine, nb, i, i);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) trace += __shfl_xor(trace, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = trace;
+  __syncthreads();
+  trace = red[0] + red[1] + red[2] + red[3];
   const double inv = 1.0 / (sqrt(trace) + tab.eps);
   for (int i = threadIdx.x; i < 1024; i += NTH) {
     const int at = (int)(w % per) * 1024 + i;
-    base[at] = raw[at] * inv * inv;  // SLOT_G
+    base[at] = gram_at(mine, nb, at / R, at % R) * inv * inv;  // SLOT_G
     base[(int64_t)SLOT_P0 * R * R + at] = at / R == at % R ? inv : 0.0;
   }
 }
@@ -342,10 +487,11 @@ __global__ __launch_bounds__(NTH) void poly_norm(Table tab, double* __restrict__
 // mode 2: G = H Q, its upper half in both places.
 __global__ __launch_bounds__(NTH) void poly_step(Table tab, int mode, int turn,
                                                  double* __restrict__ poly) {
-  __shared__ double As[64 * 32], Bs[64 * 32];
-  const Entry& e = find(tab, blockIdx.x);
+  __shared__ double As[128 * 32], Bs[128 * 32];
+  uint32_t w;
+  const Entry& e = find(tab, blockIdx.x, w);
   const int R = (e.r + 63) / 64 * 64;
-  const uint32_t w = blockIdx.x - e.tile0, per = (uint32_t)R * R / 1024;
+  const uint32_t per = (uint32_t)R * R / 1024;
   double* base = poly + e.poly + (int64_t)(w / per) * SLOTS * R * R;
   const int i0 = (int)(w % per) / (R / 32) * 32, j0 = (int)(w % per) % (R / 32) * 32;
   const int64_t RR = (int64_t)R * R;
@@ -357,20 +503,39 @@ __global__ __launch_bounds__(NTH) void poly_step(Table tab, int mode, int turn,
   double* D = base + (mode == 0 ? SLOT_Q : h ? SLOT_H : mode == 1 ? into : SLOT_G) * RR;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m = lane & 15, q = lane >> 4, wi = 16 * (wave >> 1), wj = 16 * (wave & 1);
-  d4 acc = {0.0, 0.0, 0.0, 0.0};
-  for (int k0 = 0; k0 < R; k0 += 64) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 32; i += NTH) {
-      const int64_t row = (int64_t)(k0 + i / 32) * R;
-      As[i] = A[row + i0 + i % 32];  // A symmetric
-      Bs[i] = B[row + j0 + i % 32];
+  d4 acc = {0.0, 0.0, 0.0, 0.0}, odd = acc;
+  const int lr = threadIdx.x / 16, lc = threadIdx.x % 16 * 2;
+  const d2* pa = (const d2*)(A + (int64_t)lr * R + i0 + lc);  // A symmetric
+  const d2* pb = (const d2*)(B + (int64_t)lr * R + j0 + lc);
+  const int64_t by = 8 * (int64_t)R;  // 16 rows
+  d2* wa = (d2*)(As + lr * 32 + lc);
+  d2* wb = (d2*)(Bs + lr * 32 + lc);
+  for (int k0 = 0; k0 < R; k0 += 128) {
+    // 128 rows of either operand under way at once: what a launch takes is one round
+    // trip to memory (with 64 rows and the next 64 behind them 9 us, so 6)
+    d2 ta[8], tb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t at = k0 + 16 * i < R ? k0 / 16 + i : 0;
+      ta[i] = pa[at * by], tb[i] = pb[at * by];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 64; k += 4)
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(As[(k + q) * 32 + wi + m], Bs[(k + q) * 32 + wj + m],
-                                                 acc, 0, 0, 0);
+    for (int i = 0; i < 8; ++i) wa[256 * i] = ta[i], wb[256 * i] = tb[i];
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 128; h += 64) {
+      if (k0 + h >= R) break;
+#pragma unroll
+      for (int k = h; k < h + 64; k += 8) {
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(As[(k + q) * 32 + wi + m],
+                                                   Bs[(k + q) * 32 + wj + m], acc, 0, 0, 0);
+        odd = __builtin_amdgcn_mfma_f64_16x16x4f64(As[(k + 4 + q) * 32 + wi + m],
+                                                   Bs[(k + 4 + q) * 32 + wj + m], odd, 0, 0, 0);
+      }
+    }
   }
+  acc += odd;
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     const int row = i0 + wi + 4 * v + q, col = j0 + wj + m;
@@ -384,90 +549,211 @@ __global__ __launch_bounds__(NTH) void poly_step(Table tab, int mode, int turn,
 }
 
 // ---------------------------------------------------------------- out = P U
-// One workgroup: tab.AL long elements and one block of 16 T short rows; a wave
-// takes 64 long elements at a time.  Wide: lane (m, q) reads four long elements
+// A wave takes 64 long elements at a time.  Wide: lane (m, q) reads four long elements
 // 4m.. of short row 4t + q, which is B[k = 4t + q][j = m] of four products, and
 // stores four long elements of rows 4v + q.  Tall: it reads the short elements
 // 4q.. of long row m, so that step t's k is 4q + t, and with P's rows taken in the
 // order 4 (m % 4) + m / 4 it holds the short elements 4q.. of that row again.
+// u[n]: wide, of row 4n + q; tall, of the n-th 16 long rows.  FULL as in gram.
+template <bool BF, bool TALL, bool FULL>
+__device__ __forceinline__ void apply_rows(const Entry& e, const void* x, int row0, int64_t k0,
+                                           int64_t l1, int m, int q, float (&u)[4][4]) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    if constexpr (TALL) {
+      const int64_t k = k0 + 16 * n + m;
+      const int i = row0 + 4 * q;
+      if constexpr (FULL)
+        load4<BF>(x, k * e.r + (i < e.r ? i : 0), u[n]);
+      else
+        load_upto4<BF>(x, k * e.r + i, k < l1 ? e.r - i : 0, e.vec, u[n]);
+    } else {
+      const int i = row0 + 4 * n + q;
+      const int64_t k = k0 + 4 * m, left = i < e.r ? l1 - k : 0;
+      if constexpr (FULL)
+        load4<BF>(x, (int64_t)(i < e.r ? i : 0) * e.K + k, u[n]);
+      else
+        load_upto4<BF>(x, (int64_t)i * e.K + k, (int)(left < 4 ? left : 4), e.vec, u[n]);
+    }
+  }
+}
+// acc[i][c] += of one tile of 16 short elements from row0 on: Ps is P's block, its
+// rows k0.. taken, N tiles of its columns from col0 on.
+template <int N, bool TALL>
+__device__ __forceinline__ void apply_tile(const Entry& e, const double* Ps, int ld, int row0,
+                                           int k0, int col0, int m, int q, const float (&u)[4][4],
+                                           d4 (&acc)[N][4]) {
+  const int prow = TALL ? 4 * (m & 3) + (m >> 2) : m;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int k = TALL ? 4 * q + t : 4 * t + q;
+    double b[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) b[c] = row0 + k < e.r ? (double)(TALL ? u[c][t] : u[t][c]) : 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const double a = Ps[(k0 + k) * ld + col0 + 16 * i + prow];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        acc[i][c] = __builtin_amdgcn_mfma_f64_16x16x4f64(a, b[c], acc[i][c], 0, 0, 0);
+    }
+  }
+}
+template <int N, bool BF, bool TALL>
+__device__ __forceinline__ void apply_store(const Entry& e, void* out, int row0, int64_t k0,
+                                            int64_t l1, int m, int q, const d4 (&acc)[N][4]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float f[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) f[n] = (float)(TALL ? acc[i][s][n] : acc[i][n][s]);
+      if constexpr (TALL) {
+        const int64_t k = k0 + 16 * s + m;
+        const int row = row0 + 16 * i + 4 * q;
+        store_upto4<BF>(out, k * e.r + row, k < l1 ? e.r - row : 0, e.vec, f);
+      } else {
+        const int row = row0 + 16 * i + 4 * s + q;
+        const int64_t k = k0 + 4 * m, left = row < e.r ? l1 - k : 0;
+        store_upto4<BF>(out, (int64_t)row * e.K + k, (int)(left < 4 ? left : 4), e.vec, f);
+      }
+    }
+}
+
+// Short sides of one block, 16 T: a workgroup takes e.AL long elements, a wave every
+// fourth 64 of them, its next ones on their way while the present ones are multiplied.
+template <int T, bool BF, bool TALL>
+__device__ __forceinline__ void apply_walk(const Entry& e, const void* x, void* out,
+                                           const double* P, double* Ps, int64_t k0, int64_t l1,
+                                           int m, int q) {
+  constexpr int R = 16 * T;
+  float u[T][4][4], next[T][4][4];
+  const bool fast = e.vec && k0 + 64 <= l1;
+  if (fast) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) apply_rows<BF, TALL, true>(e, x, 16 * t, k0, l1, m, q, next[t]);
+  }
+  for (int i = threadIdx.x; i < R * R; i += NTH) Ps[i] = P[i];
+  __syncthreads();
+  if (fast) {
+    for (; k0 + 64 <= l1; k0 += 256) {
+      const int64_t kn = k0 + 256 + 64 <= l1 ? k0 + 256 : k0;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) u[t][a][b] = next[t][a][b];
+        apply_rows<BF, TALL, true>(e, x, 16 * t, kn, l1, m, q, next[t]);
+      }
+      d4 acc[T][4] = {};
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        apply_tile<T, TALL>(e, Ps, R, 16 * t, 16 * t, 0, m, q, u[t], acc);
+      apply_store<T, BF, TALL>(e, out, 0, k0, l1, m, q, acc);
+    }
+  }
+  for (; k0 < l1; k0 += 256) {
+    d4 acc[T][4] = {};
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      apply_rows<BF, TALL, false>(e, x, 16 * t, k0, l1, m, q, u[t]);
+      apply_tile<T, TALL>(e, Ps, R, 16 * t, 16 * t, 0, m, q, u[t], acc);
+    }
+    apply_store<T, BF, TALL>(e, out, 0, k0, l1, m, q, acc);
+  }
+}
+
 template <int T, bool BF>
-__global__ __launch_bounds__(NTH) void apply(Table tab, int last, const double* __restrict__ poly) {
-  constexpr int R16 = 16 * T;
-  __shared__ double Ps[R16 * R16];
-  const Entry& e = find(tab, blockIdx.x);
-  const int nb = T < 4 ? 1 : (e.r + 63) / 64, R = R16 * nb;
-  const uint32_t w = blockIdx.x - e.tile0, tiles = (uint32_t)((e.K + tab.AL - 1) / tab.AL);
+__global__ __launch_bounds__(NTH) void apply(Table tab, const double* __restrict__ poly) {
+  constexpr int R = 16 * T;
+  __shared__ double Ps[R * R];
+  uint32_t w;
+  const Entry& e = find(tab, blockIdx.x, w);
+  const uint32_t tiles = (uint32_t)((e.K + e.AL - 1) / e.AL);
+  const int64_t mat = w / tiles, l0 = (int64_t)(w % tiles) * e.AL;
+  const int64_t l1 = l0 + e.AL < e.K ? l0 + e.AL : e.K;
+  const int64_t off = mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
+  const void* x = (const char*)e.x + off;
+  void* out = (char*)e.out + off;
+  const double* P = poly + e.poly + mat * R * R;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (e.tall)
+    apply_walk<T, BF, true>(e, x, out, P, Ps, l0 + 64 * wave, l1, lane & 15, lane >> 4);
+  else
+    apply_walk<T, BF, false>(e, x, out, P, Ps, l0 + 64 * wave, l1, lane & 15, lane >> 4);
+}
+
+// Short sides of blocks of 64: a workgroup takes e.AL long elements of one block, 128
+// at a time, a wave half of the block's rows and 64 of them.  P's blocks stay in LDS
+// where there are at most two.
+template <bool BF, bool TALL>
+__device__ __forceinline__ void apply64_walk(const Entry& e, const void* x, void* out,
+                                             const double* P, double* Pall, int nb, int I,
+                                             int64_t l0, int64_t l1, int wave, int m, int q) {
+  const int R = 64 * nb, wi = wave & 1, wl = wave >> 1;
+  for (int64_t step = l0; step < l1; step += 128) {
+    const int64_t k0 = step + 64 * wl;  // a wave past the end loads nothing and stores nothing
+    const bool fast = e.vec && k0 + 64 <= l1;
+    d4 acc[2][4] = {};
+    float u[4][4], next[4][4];
+    if (fast) apply_rows<BF, TALL, true>(e, x, 0, k0, l1, m, q, next);
+    for (int kb = 0; kb < nb; ++kb) {
+      double* Ps = Pall + (nb <= 2 ? kb : 0) * 4096;
+      if (nb > 2 || step == l0) {
+        __syncthreads();
+        for (int i = 2 * threadIdx.x; i < 4096; i += 2 * NTH)
+          *(d2*)(Ps + i) = *(const d2*)(P + (int64_t)(kb * 64 + i / 64) * R + I * 64 + i % 64);
+        __syncthreads();
+      }
+      if (fast) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          const int row = kb * 64 + 16 * kt;
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) u[a][b] = next[a][b];
+          apply_rows<BF, TALL, true>(e, x, row + 16, k0, l1, m, q, next);
+          apply_tile<2, TALL>(e, Ps, 64, row, 16 * kt, 32 * wi, m, q, u, acc);
+        }
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          const int row = kb * 64 + 16 * kt;
+          apply_rows<BF, TALL, false>(e, x, row, k0, l1, m, q, u);
+          apply_tile<2, TALL>(e, Ps, 64, row, 16 * kt, 32 * wi, m, q, u, acc);
+        }
+      }
+    }
+    apply_store<2, BF, TALL>(e, out, I * 64 + 32 * wi, k0, l1, m, q, acc);
+  }
+}
+
+template <bool BF>
+__global__ __launch_bounds__(NTH) void apply64(Table tab, int last, const double* __restrict__ poly) {
+  __shared__ double Pall[2 * 4096];
+  uint32_t w;
+  const Entry& e = find(tab, blockIdx.x, w);
+  const int nb = (e.r + 63) / 64, R = 64 * nb;
+  const uint32_t tiles = (uint32_t)((e.K + e.AL - 1) / e.AL);
   const int I = (int)(w % nb);
   const uint32_t mt = w / nb;
-  const int64_t mat = mt / tiles, l0 = (int64_t)(mt % tiles) * tab.AL;
-  const int64_t l1 = l0 + tab.AL < e.K ? l0 + tab.AL : e.K;
+  const int64_t mat = mt / tiles, l0 = (int64_t)(mt % tiles) * e.AL;
+  const int64_t l1 = l0 + e.AL < e.K ? l0 + e.AL : e.K;
   const int64_t off = mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
   const void* x = (const char*)e.x + off;
   void* out = (char*)e.out + off;
   const double* P = poly + e.poly;
   P += nb == 1 ? mat * R * R : (mat * SLOTS + (last ? SLOT_P1 : SLOT_P0)) * R * R;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
-  const int prow = e.tall ? 4 * (m & 3) + (m >> 2) : m;
-  for (int64_t step = l0; step < l1; step += 4 * 64) {
-    const int64_t k0 = step + 64 * wave;  // a wave past the end loads nothing and stores nothing
-    d4 acc[T][4] = {};
-    for (int kb = 0; kb < nb; ++kb) {
-      if (nb > 1 || step == l0) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < R16 * R16; i += NTH)
-          Ps[i] = P[(int64_t)(kb * R16 + i / R16) * R + I * R16 + i % R16];
-        __syncthreads();
-      }
-      float u[T][4][4];  // wide: [kt][t][c], tall: [kt][c][t]
-#pragma unroll
-      for (int kt = 0; kt < T; ++kt)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (e.tall) {
-            const int64_t k = k0 + 16 * t + m;
-            const int i = kb * R16 + 16 * kt + 4 * q, left = k < l1 ? e.r - i : 0;
-            load_upto4<BF>(x, k * e.r + i, left, e.vec, u[kt][t]);
-          } else {
-            const int i = kb * R16 + 16 * kt + 4 * t + q;
-            const int64_t k = k0 + 4 * m, left = i < e.r ? l1 - k : 0;
-            load_upto4<BF>(x, (int64_t)i * e.K + k, (int)(left < 4 ? left : 4), e.vec, u[kt][t]);
-          }
-        }
-#pragma unroll
-      for (int kt = 0; kt < T; ++kt)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int k = 16 * kt + (e.tall ? 4 * q + t : 4 * t + q);
-          double b[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) b[c] = (double)(e.tall ? u[kt][c][t] : u[kt][t][c]);
-#pragma unroll
-          for (int i = 0; i < T; ++i) {
-            const double a = Ps[k * R16 + 16 * i + prow];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              acc[i][c] = __builtin_amdgcn_mfma_f64_16x16x4f64(a, b[c], acc[i][c], 0, 0, 0);
-          }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < T; ++i)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        float f[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) f[n] = (float)(e.tall ? acc[i][s][n] : acc[i][n][s]);
-        if (e.tall) {
-          const int64_t k = k0 + 16 * s + m;
-          const int row = I * R16 + 16 * i + 4 * q;
-          store_upto4<BF>(out, k * e.r + row, k < l1 ? e.r - row : 0, e.vec, f);
-        } else {
-          const int row = I * R16 + 16 * i + 4 * s + q;
-          const int64_t k = k0 + 4 * m, left = row < e.r ? l1 - k : 0;
-          store_upto4<BF>(out, (int64_t)row * e.K + k, (int)(left < 4 ? left : 4), e.vec, f);
-        }
-      }
-  }
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (e.tall)
+    apply64_walk<BF, true>(e, x, out, P, Pall, nb, I, l0, l1, wave, lane & 15, lane >> 4);
+  else
+    apply64_walk<BF, false>(e, x, out, P, Pall, nb, I, l0, l1, wave, lane & 15, lane >> 4);
 }
 
 // ---------------------------------------------------------------- host
@@ -501,17 +787,22 @@ int make_plan(const st_matrix_batch* in, int32_t n, int32_t at, int32_t dtype, P
     const uintptr_t mask = dtype == ST_DTYPE_BF16 ? 7 : 15;
     e.vec = (e.tall ? r : K) % 4 == 0 && (((uintptr_t)b.x | (uintptr_t)b.out) & mask) == 0;
     p.count[t.n++] = b.count;
-    total += b.count * K;
+    const int64_t nb = p.T < 4 ? 1 : st::cdiv(r, 64);
+    total += b.count * K * (nb * (nb + 1) / 2);
   }
-  // Long elements of a workgroup: about 2048 workgroups where there is that much
-  // work, never less than one round of its four waves.
-  const int64_t ch = st::cdiv(total, 2048);
-  t.CH = (int32_t)(st::cdiv(ch < 256 ? 256 : ch > 4096 ? 4096 : ch, 128) * 128);
-  t.AL = (int32_t)(st::cdiv(ch < 256 ? 256 : ch > 2048 ? 2048 : ch, 256) * 256);
+  // Long elements of a workgroup: about 1024 workgroups where there is that much
+  // work (all of them run at once then), never less than two rounds of its waves.
+  int64_t ch = st::cdiv(total, 1024);  // total: over the block pairs of gram
+  if (ch < 256) ch = 256;
+  if (ch > 4096) ch = 4096;
+  auto share = [&](int64_t K, int64_t unit) {  // of equal pieces of at most about ch
+    return st::cdiv(st::cdiv(K, st::cdiv(K, ch)), unit) * unit;
+  };
   for (int i = 0; i < t.n; ++i) {
     Entry& e = t.e[i];
     const int64_t nb = (e.r + 16 * p.T - 1) / (16 * p.T);
-    e.chunks = (int32_t)st::cdiv(e.K, t.CH);
+    e.CH = (int32_t)share(e.K, 128), e.AL = (int32_t)share(e.K, p.T == 4 ? 128 : 256);
+    e.chunks = (int32_t)st::cdiv(e.K, e.CH);
     e.part = p.part, e.poly = p.poly;
     p.part += p.count[i] * e.chunks * (nb * (nb + 1) / 2) * p.T * p.T * 256;
     const int64_t R = 16 * p.T * nb;
@@ -524,8 +815,9 @@ int make_plan(const st_matrix_batch* in, int32_t n, int32_t at, int32_t dtype, P
 template <typename F>
 int64_t number(Plan& p, F per_matrix) {
   int64_t at = 0;
+  for (int i = 0; i < 64; ++i) p.tab.tile0[i] = ~0u;
   for (int i = 0; i < p.tab.n; ++i) {
-    p.tab.e[i].tile0 = (uint32_t)at;
+    p.tab.tile0[i] = (uint32_t)at;
     at += p.count[i] * per_matrix(p.tab.e[i]);
     if (at * NTH >= (int64_t)1 << 32) return -1;
   }
@@ -536,35 +828,38 @@ template <int T, bool BF>
 int launch(Plan& p, double* part, double* poly, hipStream_t stream) {
   auto blocks = [](const Entry& e) { return T < 4 ? (int64_t)1 : ((int64_t)e.r + 63) / 64; };
   const bool large = T == 4 && p.tab.e[0].r > 64;
-  auto tiles = [&](const Entry& e) { return blocks(e) * blocks(e) * 4; };
-  const int64_t ng = number(p, [&](const Entry& e) {
-    return e.chunks * blocks(e) * (blocks(e) + 1) / 2;
-  });
-  const int64_t np = ng < 0 ? -1 : number(p, [&](const Entry& e) { return large ? tiles(e) : 1; });
-  const int64_t na = np < 0 ? -1 : number(p, [&](const Entry& e) {
-    return st::cdiv(e.K, p.tab.AL) * blocks(e);
-  });
-  if (na < 0)
+  auto in_gram = [&](const Entry& e) { return e.chunks * blocks(e) * (blocks(e) + 1) / 2; };
+  auto in_sum = [&](const Entry& e) { return blocks(e) * (blocks(e) + 1) / 2 * 8; };
+  auto in_poly = [&](const Entry& e) { return large ? blocks(e) * blocks(e) * 4 : (int64_t)1; };
+  auto in_apply = [&](const Entry& e) { return st::cdiv(e.K, e.AL) * blocks(e); };
+  if (number(p, in_gram) < 0 || number(p, in_sum) < 0 || number(p, in_poly) < 0 ||
+      number(p, in_apply) < 0)
     return st::fail(ST_EUNSUPPORTED, "too many matrices for a launch: call with fewer at a time");
-  number(p, [&](const Entry& e) { return e.chunks * blocks(e) * (blocks(e) + 1) / 2; });
-  gram<T, BF><<<dim3((unsigned)ng), NTH, 0, stream>>>(p.tab, part);
-  number(p, [&](const Entry& e) { return large ? tiles(e) : 1; });
+  gram<T, BF><<<(unsigned)number(p, in_gram), NTH, 0, stream>>>(p.tab, part);
   int turn = 0;
-  if (!large) {
-    poly_small<T><<<dim3((unsigned)np), 64 * T, 0, stream>>>(p.tab, part, poly);
-  } else {
-    poly_sum<<<dim3((unsigned)np), NTH, 0, stream>>>(p.tab, part, poly);
-    poly_norm<<<dim3((unsigned)np), NTH, 0, stream>>>(p.tab, poly);
+  if (large) {
+    poly_sum<<<(unsigned)number(p, in_sum), NTH, 0, stream>>>(p.tab, part);
+    const unsigned np = (unsigned)number(p, in_poly);
+    poly_norm<<<np, NTH, 0, stream>>>(p.tab, part, poly);
     for (int s = 0; s < p.tab.steps; ++s) {
       const bool more = s + 1 < p.tab.steps;
-      poly_step<<<dim3((unsigned)np), NTH, 0, stream>>>(p.tab, 0, turn, poly);
-      poly_step<<<dim3((unsigned)np, more ? 2 : 1), NTH, 0, stream>>>(p.tab, 1, turn, poly);
-      if (more) poly_step<<<dim3((unsigned)np), NTH, 0, stream>>>(p.tab, 2, turn, poly);
+      poly_step<<<np, NTH, 0, stream>>>(p.tab, 0, turn, poly);
+      poly_step<<<dim3(np, more ? 2 : 1), NTH, 0, stream>>>(p.tab, 1, turn, poly);
+      if (more) poly_step<<<np, NTH, 0, stream>>>(p.tab, 2, turn, poly);
       turn ^= 1;
     }
+  } else {
+    const unsigned np = (unsigned)number(p, in_poly);
+    if constexpr (T == 1)
+      poly16<<<np, 64, 0, stream>>>(p.tab, part, poly);
+    else
+      poly_small<T><<<np, NTH, 0, stream>>>(p.tab, part, poly);
   }
-  number(p, [&](const Entry& e) { return st::cdiv(e.K, p.tab.AL) * blocks(e); });
-  apply<T, BF><<<dim3((unsigned)na), NTH, 0, stream>>>(p.tab, turn, poly);
+  const unsigned na = (unsigned)number(p, in_apply);
+  if constexpr (T == 4)
+    apply64<BF><<<na, NTH, 0, stream>>>(p.tab, turn, poly);
+  else
+    apply<T, BF><<<na, NTH, 0, stream>>>(p.tab, poly);
   return st::check_launch("st_orthogonalize");
 }
 
