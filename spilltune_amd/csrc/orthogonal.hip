@@ -29,7 +29,7 @@ namespace {
 typedef double d4 __attribute__((ext_vector_type(4)));
 typedef double d2 __attribute__((ext_vector_type(2)));
 constexpr int NTH = 256;
-constexpr int MAXE = 54;        // entries of a launch's table (kernel arguments: 4 KB)
+constexpr int MAXE = 48;        // entries of a launch's table (kernel arguments: 4 KB)
 constexpr int64_t MAXR = 1024;  // short side
 
 // A batch of equal matrices, back to back.
@@ -43,18 +43,23 @@ struct Entry {
   int16_t tall;            // the short side is the contiguous one
   int16_t vec;             // rows may be read four elements at a time
 };
+enum { IN_GRAM, IN_SUM, IN_POLY, IN_APPLY, PHASES };
 struct Table {
   Entry e[MAXE];
-  uint32_t tile0[64];  // the entries' first workgroups in the present launch, then ~0
+  uint32_t tile0[PHASES][64];  // the entries' first workgroups in a phase, then ~0
   int32_t n, steps;
   double a, b, c, eps;
 };
+static_assert(sizeof(Table) <= 3840 && sizeof(Table) % 4 == 0, "kernel arguments");
+
+// Kernel arguments lie in the host's memory: gram, the first launch, copies the table
+// beside the sums, where the others find it in a third of the time.
 
 // The last entry with tile0 <= b and its place among the entry's workgroups: one
 // load for all entries (a search would be six dependent ones, 1 us of each
 // workgroup's time).
-__device__ __forceinline__ const Entry& find(const Table& t, uint32_t b, uint32_t& w) {
-  const uint32_t mine = t.tile0[threadIdx.x & 63];
+__device__ __forceinline__ const Entry& find(const Table& t, int phase, uint32_t b, uint32_t& w) {
+  const uint32_t mine = t.tile0[phase][threadIdx.x & 63];
   const int i = __popcll(__ballot(mine <= b)) - 1;
   w = b - __builtin_amdgcn_readlane(mine, i);
   return t.e[i];
@@ -199,10 +204,15 @@ __device__ __forceinline__ void gram_walk(const Entry& e, const void* x, int row
 }
 
 template <int T, bool BF>
-__global__ __launch_bounds__(NTH) void gram(Table tab, double* __restrict__ part) {
+__global__ __launch_bounds__(NTH) void gram(Table tab, double* __restrict__ part,
+                                            uint32_t* __restrict__ copy) {
   __shared__ double sum[T < 4 ? T * T * 256 : 1];
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += NTH)
+      copy[i] = ((const uint32_t*)&tab)[i];
+  }
   uint32_t w;
-  const Entry& e = find(tab, blockIdx.x, w);
+  const Entry& e = find(tab, IN_GRAM, blockIdx.x, w);
   const int nb = T < 4 ? 1 : (e.r + 63) / 64, pairs = nb * (nb + 1) / 2;
   const int pair = (int)(w % pairs);
   const uint32_t mc = w / pairs;  // matrix * chunks + chunk
@@ -319,11 +329,12 @@ __device__ __forceinline__ d4 steps16(const Table& tab, d4 g, double* turn, int 
   return P;
 }
 
-__global__ __launch_bounds__(64) void poly16(Table tab, const double* __restrict__ part,
+__global__ __launch_bounds__(64) void poly16(const Table* __restrict__ table, const double* __restrict__ part,
                                              double* __restrict__ poly) {
   __shared__ double turn[16 * 17];
+  const Table& tab = *table;
   uint32_t mat;
-  const Entry& e = find(tab, blockIdx.x, mat);
+  const Entry& e = find(tab, IN_POLY, blockIdx.x, mat);
   const int lane = threadIdx.x, m = lane & 15, q = lane >> 4;
   const double* p = part + e.part + (int64_t)mat * e.chunks * 256 + lane;
   d4 g = {0.0, 0.0, 0.0, 0.0};
@@ -355,12 +366,13 @@ __device__ __forceinline__ d4 product_tile(const double* A, const double* B, int
 }
 
 template <int T>
-__global__ __launch_bounds__(NTH) void poly_small(Table tab, const double* __restrict__ part,
+__global__ __launch_bounds__(NTH) void poly_small(const Table* __restrict__ table, const double* __restrict__ part,
                                                   double* __restrict__ poly) {
   constexpr int R = 16 * T, N = R * R, OWN = T * T / 4;  // tiles of a wave
   __shared__ double G[N], Q[N], P[N];
+  const Table& tab = *table;
   uint32_t mat;
-  const Entry& e = find(tab, blockIdx.x, mat);
+  const Entry& e = find(tab, IN_POLY, blockIdx.x, mat);
   const double* mine = part + e.part + (int64_t)mat * e.chunks * N;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
   // the tiles on and above the diagonal, as the waves of gram left them
@@ -442,9 +454,10 @@ __global__ __launch_bounds__(NTH) void poly_small(Table tab, const double* __res
 enum { SLOT_G, SLOT_Q, SLOT_P0, SLOT_P1, SLOT_H, SLOTS };
 
 // The chunks' sums joined into the first chunk's place.
-__global__ __launch_bounds__(NTH) void poly_sum(Table tab, double* __restrict__ part) {
+__global__ __launch_bounds__(NTH) void poly_sum(const Table* __restrict__ table, double* __restrict__ part) {
+  const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, blockIdx.x, w);
+  const Entry& e = find(tab, IN_SUM, blockIdx.x, w);
   const int nb = (e.r + 63) / 64, pairs = nb * (nb + 1) / 2;
   const uint32_t per = pairs * 4096 / (2 * NTH);
   double2* p = (double2*)(part + e.part + (int64_t)(w / per) * e.chunks * pairs * 4096) +
@@ -459,11 +472,12 @@ __global__ __launch_bounds__(NTH) void poly_sum(Table tab, double* __restrict__ 
 }
 
 // G = U U' / (|U|_F + eps)^2 and P = I / (|U|_F + eps), from the joined sums.
-__global__ __launch_bounds__(NTH) void poly_norm(Table tab, const double* __restrict__ part,
+__global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table, const double* __restrict__ part,
                                                  double* __restrict__ poly) {
   __shared__ double red[NTH / 64];
+  const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, blockIdx.x, w);
+  const Entry& e = find(tab, IN_POLY, blockIdx.x, w);
   const int nb = (e.r + 63) / 64, R = 64 * nb;
   const uint32_t per = (uint32_t)R * R / 1024;
   const double* mine = part + e.part + (int64_t)(w / per) * e.chunks * (nb * (nb + 1) / 2) * 4096;
@@ -485,11 +499,12 @@ __global__ __launch_bounds__(NTH) void poly_norm(Table tab, const double* __rest
 
 // mode 0: Q = aI + bG + cGG;  mode 1: P' = Q P and (blockIdx.y = 1) H = Q G;
 // mode 2: G = H Q, its upper half in both places.
-__global__ __launch_bounds__(NTH) void poly_step(Table tab, int mode, int turn,
+__global__ __launch_bounds__(NTH) void poly_step(const Table* __restrict__ table, int mode, int turn,
                                                  double* __restrict__ poly) {
   __shared__ double As[128 * 32], Bs[128 * 32];
+  const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, blockIdx.x, w);
+  const Entry& e = find(tab, IN_POLY, blockIdx.x, w);
   const int R = (e.r + 63) / 64 * 64;
   const uint32_t per = (uint32_t)R * R / 1024;
   double* base = poly + e.poly + (int64_t)(w / per) * SLOTS * R * R;
@@ -666,11 +681,12 @@ __device__ __forceinline__ void apply_walk(const Entry& e, const void* x, void* 
 }
 
 template <int T, bool BF>
-__global__ __launch_bounds__(NTH) void apply(Table tab, const double* __restrict__ poly) {
+__global__ __launch_bounds__(NTH) void apply(const Table* __restrict__ table, const double* __restrict__ poly) {
   constexpr int R = 16 * T;
   __shared__ double Ps[R * R];
+  const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, blockIdx.x, w);
+  const Entry& e = find(tab, IN_APPLY, blockIdx.x, w);
   const uint32_t tiles = (uint32_t)((e.K + e.AL - 1) / e.AL);
   const int64_t mat = w / tiles, l0 = (int64_t)(w % tiles) * e.AL;
   const int64_t l1 = l0 + e.AL < e.K ? l0 + e.AL : e.K;
@@ -733,10 +749,11 @@ __device__ __forceinline__ void apply64_walk(const Entry& e, const void* x, void
 }
 
 template <bool BF>
-__global__ __launch_bounds__(NTH) void apply64(Table tab, int last, const double* __restrict__ poly) {
+__global__ __launch_bounds__(NTH) void apply64(const Table* __restrict__ table, int last, const double* __restrict__ poly) {
   __shared__ double Pall[2 * 4096];
+  const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, blockIdx.x, w);
+  const Entry& e = find(tab, IN_APPLY, blockIdx.x, w);
   const int nb = (e.r + 63) / 64, R = 64 * nb;
   const uint32_t tiles = (uint32_t)((e.K + e.AL - 1) / e.AL);
   const int I = (int)(w % nb);
@@ -811,55 +828,63 @@ int make_plan(const st_matrix_batch* in, int32_t n, int32_t at, int32_t dtype, P
   return taken;
 }
 
-// Numbers the workgroups of a launch; their count, or -1 beyond a launch's limit.
+// Numbers the workgroups of a phase; their count, or -1 beyond a launch's limit.
 template <typename F>
-int64_t number(Plan& p, F per_matrix) {
+int64_t number(Plan& p, int phase, F per_matrix) {
   int64_t at = 0;
-  for (int i = 0; i < 64; ++i) p.tab.tile0[i] = ~0u;
+  for (int i = 0; i < 64; ++i) p.tab.tile0[phase][i] = ~0u;
   for (int i = 0; i < p.tab.n; ++i) {
-    p.tab.tile0[i] = (uint32_t)at;
+    p.tab.tile0[phase][i] = (uint32_t)at;
     at += p.count[i] * per_matrix(p.tab.e[i]);
     if (at * NTH >= (int64_t)1 << 32) return -1;
   }
   return at;
 }
 
+constexpr int64_t TABLE_BYTES = (sizeof(Table) + 15) / 16 * 16;
+
 template <int T, bool BF>
-int launch(Plan& p, double* part, double* poly, hipStream_t stream) {
+int launch(Plan& p, char* workspace, hipStream_t stream) {
   auto blocks = [](const Entry& e) { return T < 4 ? (int64_t)1 : ((int64_t)e.r + 63) / 64; };
   const bool large = T == 4 && p.tab.e[0].r > 64;
-  auto in_gram = [&](const Entry& e) { return e.chunks * blocks(e) * (blocks(e) + 1) / 2; };
-  auto in_sum = [&](const Entry& e) { return blocks(e) * (blocks(e) + 1) / 2 * 8; };
-  auto in_poly = [&](const Entry& e) { return large ? blocks(e) * blocks(e) * 4 : (int64_t)1; };
-  auto in_apply = [&](const Entry& e) { return st::cdiv(e.K, e.AL) * blocks(e); };
-  if (number(p, in_gram) < 0 || number(p, in_sum) < 0 || number(p, in_poly) < 0 ||
-      number(p, in_apply) < 0)
+  const int64_t ng = number(p, IN_GRAM, [&](const Entry& e) {
+    return e.chunks * blocks(e) * (blocks(e) + 1) / 2;
+  });
+  const int64_t ns = number(p, IN_SUM, [&](const Entry& e) {
+    return blocks(e) * (blocks(e) + 1) / 2 * 8;
+  });
+  const int64_t np = number(p, IN_POLY, [&](const Entry& e) {
+    return large ? blocks(e) * blocks(e) * 4 : (int64_t)1;
+  });
+  const int64_t na = number(p, IN_APPLY, [&](const Entry& e) {
+    return st::cdiv(e.K, e.AL) * blocks(e);
+  });
+  if (ng < 0 || ns < 0 || np < 0 || na < 0)
     return st::fail(ST_EUNSUPPORTED, "too many matrices for a launch: call with fewer at a time");
-  gram<T, BF><<<(unsigned)number(p, in_gram), NTH, 0, stream>>>(p.tab, part);
+  const Table* tab = (const Table*)workspace;
+  double* part = (double*)(workspace + TABLE_BYTES);
+  double* poly = part + p.part;
+  gram<T, BF><<<(unsigned)ng, NTH, 0, stream>>>(p.tab, part, (uint32_t*)workspace);
   int turn = 0;
   if (large) {
-    poly_sum<<<(unsigned)number(p, in_sum), NTH, 0, stream>>>(p.tab, part);
-    const unsigned np = (unsigned)number(p, in_poly);
-    poly_norm<<<np, NTH, 0, stream>>>(p.tab, part, poly);
+    poly_sum<<<(unsigned)ns, NTH, 0, stream>>>(tab, part);
+    poly_norm<<<(unsigned)np, NTH, 0, stream>>>(tab, part, poly);
     for (int s = 0; s < p.tab.steps; ++s) {
       const bool more = s + 1 < p.tab.steps;
-      poly_step<<<np, NTH, 0, stream>>>(p.tab, 0, turn, poly);
-      poly_step<<<dim3(np, more ? 2 : 1), NTH, 0, stream>>>(p.tab, 1, turn, poly);
-      if (more) poly_step<<<np, NTH, 0, stream>>>(p.tab, 2, turn, poly);
+      poly_step<<<(unsigned)np, NTH, 0, stream>>>(tab, 0, turn, poly);
+      poly_step<<<dim3((unsigned)np, more ? 2 : 1), NTH, 0, stream>>>(tab, 1, turn, poly);
+      if (more) poly_step<<<(unsigned)np, NTH, 0, stream>>>(tab, 2, turn, poly);
       turn ^= 1;
     }
+  } else if constexpr (T == 1) {
+    poly16<<<(unsigned)np, 64, 0, stream>>>(tab, part, poly);
   } else {
-    const unsigned np = (unsigned)number(p, in_poly);
-    if constexpr (T == 1)
-      poly16<<<np, 64, 0, stream>>>(p.tab, part, poly);
-    else
-      poly_small<T><<<np, NTH, 0, stream>>>(p.tab, part, poly);
+    poly_small<T><<<(unsigned)np, NTH, 0, stream>>>(tab, part, poly);
   }
-  const unsigned na = (unsigned)number(p, in_apply);
   if constexpr (T == 4)
-    apply64<BF><<<na, NTH, 0, stream>>>(p.tab, turn, poly);
+    apply64<BF><<<(unsigned)na, NTH, 0, stream>>>(tab, turn, poly);
   else
-    apply<T, BF><<<na, NTH, 0, stream>>>(p.tab, poly);
+    apply<T, BF><<<(unsigned)na, NTH, 0, stream>>>(tab, poly);
   return st::check_launch("st_orthogonalize");
 }
 
@@ -889,7 +914,7 @@ extern "C" int64_t st_orthogonalize_workspace_bytes(int32_t n, const st_matrix_b
     at += make_plan(table, n, at, ST_DTYPE_F32, p);
     if (p.part + p.poly > most) most = p.part + p.poly;
   }
-  return most * 8;
+  return most ? most * 8 + TABLE_BYTES : 0;
 }
 
 extern "C" int st_orthogonalize(int32_t n, const st_matrix_batch* table, int32_t dtype,
@@ -920,13 +945,12 @@ extern "C" int st_orthogonalize(int32_t n, const st_matrix_batch* table, int32_t
     at += make_plan(table, n, at, dtype, p);
     if (!p.tab.n) continue;
     p.tab.steps = steps, p.tab.a = a, p.tab.b = b, p.tab.c = c, p.tab.eps = eps;
-    double* part = (double*)workspace;
-    double* poly = part + p.part;
+    char* ws = (char*)workspace;
     const hipStream_t s = (hipStream_t)stream;
     const bool bf = dtype == ST_DTYPE_BF16;
-    const int r = p.T == 1 ? (bf ? launch<1, true>(p, part, poly, s) : launch<1, false>(p, part, poly, s))
-                : p.T == 2 ? (bf ? launch<2, true>(p, part, poly, s) : launch<2, false>(p, part, poly, s))
-                           : (bf ? launch<4, true>(p, part, poly, s) : launch<4, false>(p, part, poly, s));
+    const int r = p.T == 1   ? (bf ? launch<1, true>(p, ws, s) : launch<1, false>(p, ws, s))
+                  : p.T == 2 ? (bf ? launch<2, true>(p, ws, s) : launch<2, false>(p, ws, s))
+                             : (bf ? launch<4, true>(p, ws, s) : launch<4, false>(p, ws, s));
     if (r != ST_OK) return r;
   }
   return ST_OK;
