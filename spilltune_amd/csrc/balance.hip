@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int NTH = 256, WAVES = NTH / 64;
+constexpr int NTH = 256, WAVES = NTH / 64, JOIN = 1024;
 constexpr int MAXE = 512, PER = MAXE / 64;
 constexpr float TINY = 1e-20f;
 
@@ -119,35 +119,63 @@ __global__ __launch_bounds__(NTH) void balance_sums(Args a) {
   if (threadIdx.x == 0) nt[a.E] = count[MAXE];
 }
 
-// A group's chunks joined; with one group also the loss itself.
-__global__ __launch_bounds__(MAXE) void balance_join(Args a) {
-  __shared__ float red[MAXE / 64];
-  const int e = threadIdx.x;
+// Sums of the chunks of a group, one wave each 64 experts at a time: wave w takes the
+// chunks w, w + WAVES, .., whose loads do not wait for one another; the waves' sums are
+// added in their order.
+__global__ __launch_bounds__(JOIN) void balance_join(Args a) {
+  constexpr int W = JOIN / 64;
+  __shared__ float probs[W][64];
+  __shared__ int32_t count[W][64], total[W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t g = blockIdx.x;
-  int64_t n = 0, picks = 0;
-  float p = 0.0f;
-  for (int64_t c = 0; c < a.chunks; ++c) {
-    const int32_t* nt = a.counted + (g * a.chunks + c) * (a.E + 1);
-    n += nt[a.E];
+  const int32_t* counted = a.counted + g * a.chunks * (a.E + 1);
+  const float* sums = a.probs + g * a.chunks * a.E;
+  int n = 0;  // fewer than 2^25 tokens a group
+  for (int64_t c = threadIdx.x; c < a.chunks; c += JOIN) n += counted[c * (a.E + 1) + a.E];
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) n += __shfl_xor(n, d);
+  if (lane == 0) total[wave] = n;
+  __syncthreads();
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) n += total[w];
+  const float many = (float)(n > 0 ? n : 1);
+  float loss = 0.0f;
+  for (int e0 = 0; e0 < a.E; e0 += 64) {
+    const int e = e0 + lane;
+    float p = 0.0f;
+    int32_t picks = 0;
     if (e < a.E) {
-      picks += nt[e];
-      p += a.probs[(g * a.chunks + c) * a.E + e];
+#pragma unroll 8
+      for (int64_t c = wave; c < a.chunks; c += W) {
+        p += sums[c * a.E + e];
+        picks += counted[c * (a.E + 1) + e];
+      }
+    }
+    __syncthreads();
+    probs[wave][lane] = p;
+    count[wave][lane] = picks;
+    __syncthreads();
+    if (wave == 0) {
+      int64_t all = 0;
+      p = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) p += probs[w][lane], all += count[w][lane];
+      if (e < a.E) {
+        a.counts[g * a.E + e] = all;
+        loss += (float)all * (float)a.E / ((float)a.k * many) * (p / many);
+      }
     }
   }
-  if (e < a.E) a.counts[g * a.E + e] = picks;
-  const float many = (float)(n > 0 ? n : 1);
-  float s = wave_sum((float)picks * (float)a.E / ((float)a.k * many) * (p / many));
-  if ((e & 63) == 0) red[e >> 6] = s;
-  __syncthreads();
-  if (e == 0) {
-    s = red[0];
-    for (int w = 1; w < MAXE / 64; ++w) s += red[w];
-    a.tokens[g] = (int32_t)n;
+  if (wave) return;
+  loss = wave_sum(loss);
+  if (lane == 0) {
+    a.tokens[g] = n;
     if (a.groups == 1) {
-      *a.loss = s;
+      *a.loss = loss;
       a.tokens[1] = n > 0;
     } else {
-      a.terms[g] = s;
+      a.terms[g] = loss;
     }
   }
 }
@@ -208,10 +236,10 @@ __global__ __launch_bounds__(NTH) void balance_bwd(Args a) {
   }
 }
 
-// Tokens of a workgroup: about 512 workgroups in all, at least one token a wave.
+// Tokens of a workgroup: about 512 workgroups in all, at least four tokens a wave.
 void plan(Args& a) {
   const int64_t want = st::cdiv(512, a.groups);
-  a.chunk = st::cdiv(st::cdiv(a.per_group, want), WAVES) * WAVES;
+  a.chunk = st::cdiv(st::cdiv(a.per_group, want), 4 * WAVES) * 4 * WAVES;
   a.chunks = st::cdiv(a.per_group, a.chunk);
 }
 
@@ -262,7 +290,7 @@ extern "C" int st_balance_fwd(const void* logits, int32_t dtype, const int32_t* 
     balance_sums<true><<<grid, NTH, 0, s>>>(a);
   else
     balance_sums<false><<<grid, NTH, 0, s>>>(a);
-  balance_join<<<(unsigned)groups, MAXE, 0, s>>>(a);
+  balance_join<<<(unsigned)groups, JOIN, 0, s>>>(a);
   if (groups > 1) balance_mean<<<1, 64, 0, s>>>(a);
   return st::check_launch("st_balance_fwd");
 }
