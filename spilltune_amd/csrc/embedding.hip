@@ -19,6 +19,9 @@ namespace {
 constexpr int NTH = 256;
 constexpr int BITS = 9, BINS = 1 << BITS;
 constexpr int64_t SMALL = 16384;  // tokens one workgroup sorts (16 a thread)
+// 16-byte words up to which the launch that sorts in LDS also clears, one workgroup a
+// CU beside it: 64 MB in the sort's time, 2.1 GB in 364 us instead of 310 and 25
+constexpr int64_t CLEAR_APART = (64 << 20) / 16;
 constexpr int TILE = 2048;        // keys of a workgroup beyond that
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int ids32, int64_t i) {
@@ -69,6 +72,18 @@ __global__ __launch_bounds__(NTH) void lookup(const void* __restrict__ table,
         *to = st::f32_to_bf16(f[0]);
     }
   }
+}
+
+// ---------------------------------------------------------------- clear
+// Workgroup `b` of `many` clears its share: one 16-byte word a thread and as many
+// workgroups as that takes (2.1 GB: 310 us, where loops of any kind took 350 to 420).
+template <int NT>
+__device__ __forceinline__ void clear_share(uint4* p, int64_t words, int64_t b, int64_t many) {
+  for (int64_t i = b * NT + threadIdx.x; i < words; i += many * NT) p[i] = make_uint4(0, 0, 0, 0);
+}
+unsigned clear_blocks(int64_t words) {
+  const int64_t b = st::cdiv(words, NTH);
+  return (unsigned)(b < (1 << 23) ? b : 1 << 23);
 }
 
 // ---------------------------------------------------------------- sort
@@ -128,12 +143,7 @@ __global__ __launch_bounds__(1024) void sort_small(const void* __restrict__ ids,
                                                    uint32_t* __restrict__ tok,
                                                    uint32_t* __restrict__ pos,
                                                    uint4* __restrict__ clear, int64_t words) {
-  if (blockIdx.x) {
-    for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < words;
-         i += (int64_t)(gridDim.x - 1) * 1024)
-      clear[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
+  if (blockIdx.x) return clear_share<1024>(clear, words, blockIdx.x - 1, gridDim.x - 1);
   __shared__ uint32_t count[16][BINS];
   __shared__ uint32_t totals[16];
   __shared__ uint32_t keys[SMALL];
@@ -183,14 +193,19 @@ __global__ __launch_bounds__(1024) void sort_small(const void* __restrict__ ids,
 }
 
 // More tokens: per pass the tiles' digit counts [digit][tile], their exclusive sums,
-// and the move.  The first pass reads the ids themselves.
+// and the move.  The first pass reads the ids themselves, and its workgroups behind
+// the tiles' clear the gradient.
 __global__ __launch_bounds__(NTH) void tile_counts(const void* __restrict__ ids, int ids32,
                                                    const uint32_t* __restrict__ tok, int64_t n,
                                                    int64_t V, int64_t padding, int shift,
-                                                   int64_t tiles, uint32_t* __restrict__ counts) {
+                                                   int64_t tiles, uint32_t* __restrict__ counts,
+                                                   uint4* __restrict__ clear, int64_t words) {
   __shared__ uint32_t hist[BINS];
+  if (blockIdx.x >= tiles)
+    return clear_share<NTH>(clear, words, blockIdx.x - tiles, gridDim.x - tiles);
   for (int i = threadIdx.x; i < BINS; i += NTH) hist[i] = 0;
   __syncthreads();
+#pragma unroll
   for (int s = 0; s < TILE / NTH; ++s) {
     const int64_t i = (int64_t)blockIdx.x * TILE + s * NTH + threadIdx.x;
     if (i < n) {
@@ -202,29 +217,48 @@ __global__ __launch_bounds__(NTH) void tile_counts(const void* __restrict__ ids,
   for (int i = threadIdx.x; i < BINS; i += NTH) counts[i * tiles + blockIdx.x] = hist[i];
 }
 
+// Exclusive sums of all counts in place, 8192 at a time.
 __global__ __launch_bounds__(1024) void tile_scan(uint32_t* __restrict__ counts, int64_t many) {
   __shared__ uint32_t totals[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t per = (many + 1023) / 1024, a = threadIdx.x * per, z = min(a + per, many);
-  uint32_t sum = 0;
-  for (int64_t i = a; i < z; ++i) sum += counts[i];
-  uint32_t inc = sum;
+  uint32_t carry = 0;
+  for (int64_t i0 = 0; i0 < many; i0 += 8192) {
+    const int64_t at = i0 + threadIdx.x * 8;
+    uint32_t v[8], sum = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t x = __shfl_up(inc, d);
-    if (lane >= d) inc += x;
-  }
-  if (lane == 63) totals[wave] = inc;
-  __syncthreads();
-  uint32_t base = inc - sum;
-  for (int w = 0; w < wave; ++w) base += totals[w];
-  for (int64_t i = a; i < z; ++i) {
-    const uint32_t v = counts[i];
-    counts[i] = base;
-    base += v;
+    for (int k = 0; k < 8; ++k) {
+      v[k] = at + k < many ? counts[at + k] : 0;
+      sum += v[k];
+    }
+    uint32_t inc = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t x = __shfl_up(inc, d);
+      if (lane >= d) inc += x;
+    }
+    if (lane == 63) totals[wave] = inc;
+    __syncthreads();
+    uint32_t base = carry + inc - sum;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const uint32_t t = totals[w];
+      if (w < wave) base += t;
+      carry += t;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (at + k < many) counts[at + k] = base;
+      base += v[k];
+    }
+    __syncthreads();
   }
 }
 
+// SUMMED: counts are exclusive sums already.  Otherwise each workgroup forms its own
+// from the counts themselves (up to MOVE_TILES tiles: 2 us in the place of a launch of
+// one workgroup, 7 us).
+constexpr int64_t MOVE_TILES = 64;
+template <bool SUMMED>
 __global__ __launch_bounds__(NTH) void tile_move(const void* __restrict__ ids, int ids32,
                                                  const uint32_t* __restrict__ tok,
                                                  const uint32_t* __restrict__ pos, int64_t n,
@@ -233,29 +267,67 @@ __global__ __launch_bounds__(NTH) void tile_move(const void* __restrict__ ids, i
                                                  const uint32_t* __restrict__ counts,
                                                  uint32_t* __restrict__ tok_out,
                                                  uint32_t* __restrict__ pos_out) {
-  constexpr int W = NTH / 64, STEPS = TILE / NTH;
+  constexpr int W = NTH / 64, STEPS = TILE / NTH, OWN = BINS / NTH;
   __shared__ uint32_t count[W][BINS];
+  __shared__ uint32_t totals[W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int i = threadIdx.x; i < W * BINS; i += NTH) (&count[0][0])[i] = 0;
-  __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * TILE + wave * (TILE / W) + lane;
   uint32_t key[STEPS], at[STEPS], rank[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
     const int64_t i = first + s * 64;
-    const bool live = i < n;
-    key[s] = !live ? 0 : tok ? tok[i] : key_of(id_at(ids, ids32, i), V, padding);
-    at[s] = !live ? 0 : tok ? pos[i] : (uint32_t)i;
-    rank[s] = wave_rank((key[s] >> shift) & (BINS - 1), live, count[wave]);
+    key[s] = i >= n ? 0 : tok ? tok[i] : key_of(id_at(ids, ids32, i), V, padding);
+    at[s] = i >= n ? 0 : tok ? pos[i] : (uint32_t)i;
+  }
+  // the tile's place of the digits OWN threadIdx.x ..
+  uint32_t place[OWN];
+  if constexpr (SUMMED) {
+#pragma unroll
+    for (int o = 0; o < OWN; ++o)
+      place[o] = counts[(threadIdx.x * OWN + o) * tiles + blockIdx.x];
+  } else {
+    uint32_t sum = 0, all[OWN];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const uint32_t* p = counts + (threadIdx.x * OWN + o) * tiles;
+      uint32_t before = 0;
+      all[o] = 0;
+#pragma unroll 8
+      for (int t = 0; t < (int)tiles; ++t) {
+        const uint32_t c = p[t];
+        all[o] += c;
+        before += t < (int)blockIdx.x ? c : 0;
+      }
+      place[o] = before;
+      sum += all[o];
+    }
+    uint32_t inc = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t x = __shfl_up(inc, d);
+      if (lane >= d) inc += x;
+    }
+    if (lane == 63) totals[wave] = inc;
+    __syncthreads();
+    uint32_t base = inc - sum;
+    for (int w = 0; w < wave; ++w) base += totals[w];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) place[o] += base, base += all[o];
   }
   __syncthreads();
-  // the tile's place of each digit, then the waves' before this one
-  for (int d = threadIdx.x; d < BINS; d += NTH) {
-    uint32_t base = counts[d * tiles + blockIdx.x];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+    rank[s] = wave_rank((key[s] >> shift) & (BINS - 1), first + s * 64 < n, count[wave]);
+  __syncthreads();
+  // then the waves' before this one
+#pragma unroll
+  for (int o = 0; o < OWN; ++o) {
+    const int d = threadIdx.x * OWN + o;
     for (int w = 0; w < W; ++w) {
       const uint32_t v = count[w][d];
-      count[w][d] = base;
-      base += v;
+      count[w][d] = place[o];
+      place[o] += v;
     }
   }
   __syncthreads();
@@ -269,8 +341,7 @@ __global__ __launch_bounds__(NTH) void tile_move(const void* __restrict__ ids, i
 }
 
 __global__ __launch_bounds__(NTH) void clear_words(uint4* __restrict__ p, int64_t words) {
-  for (int64_t i = (int64_t)blockIdx.x * NTH + threadIdx.x; i < words; i += (int64_t)gridDim.x * NTH)
-    p[i] = make_uint4(0, 0, 0, 0);
+  clear_share<NTH>(p, words, blockIdx.x, gridDim.x);
 }
 // what 16-byte words leave of a gradient
 __global__ __launch_bounds__(64) void clear_tail(uint16_t* __restrict__ p, int halves) {
@@ -290,24 +361,10 @@ struct Sums {
 };
 
 template <int VEC>
-__device__ __forceinline__ void add_row(const uint16_t* p, float (&acc)[VEC]) {
-  if constexpr (VEC == 8) {
-    const uint4 v = *(const uint4*)p;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[2 * e] += __uint_as_float(w[e] << 16);
-      acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
-    }
-  } else {
-    acc[0] += st::bf16_to_f32(p[0]);
-  }
-}
-template <int VEC>
 __device__ __forceinline__ void store_f(float* p, const float (&f)[VEC]) {
-  if constexpr (VEC == 8) {
+  if constexpr (VEC >= 4) {
     *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
-    *(float4*)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    if constexpr (VEC == 8) *(float4*)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
   } else {
     p[0] = f[0];
   }
@@ -331,60 +388,137 @@ __device__ __forceinline__ void write_row(const Sums& a, uint32_t token, int64_t
     if constexpr (VEC == 8)
       *(uint4*)p = make_uint4(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
                               st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7]));
+    else if constexpr (VEC == 4)
+      *(uint2*)p = make_uint2(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]));
     else
       *p = st::f32_to_bf16(f[0]);
   }
 }
 
-// A chunk of the sorted list: sums of its runs of one token.
+// A chunk of the sorted list: sums of its runs of one token.  Each wave has the
+// chunk's tokens and positions in its lanes (lane l: entry e0 - 1 + l, so the
+// neighbours' too), and eight rows are read at once.
+constexpr int AHEAD = 8;
 template <int VEC>
-__global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
-  const int64_t c = blockIdx.x, e0 = c * a.chunk, e1 = min(e0 + a.chunk, a.n);
-  const int64_t i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  if (i >= a.H || a.tok[e0] >= a.V) return;  // no barriers below
-  bool from = e0 > 0 && a.tok[e0 - 1] == a.tok[e0];  // the run began in an earlier chunk
-  float acc[VEC] = {};
-  for (int64_t e = e0; e < e1; ++e) {
-    const uint32_t token = a.tok[e];
-    if (token >= a.V) return;  // only such ones follow
-    add_row<VEC>(a.dout + (int64_t)a.pos[e] * a.H + i, acc);
-    const bool end = e + 1 == a.n || a.tok[e + 1] != token;
-    if (!end && e + 1 < e1) continue;
-    if (from)
-      store_f<VEC>(a.partial + c * 2 * a.H + i, acc);
-    else if (!end)
-      store_f<VEC>(a.partial + (c * 2 + 1) * a.H + i, acc);
-    else
-      write_row<VEC>(a, token, i, acc);
-    from = false;
+struct Raw {
+  uint4 v;
+};
+template <>
+struct Raw<4> {
+  uint2 v;
+};
+template <>
+struct Raw<1> {
+  uint16_t v;
+};
+template <int VEC>
+__device__ __forceinline__ void read_row(const uint16_t* p, Raw<VEC>& r) {
+  if constexpr (VEC == 8)
+    r.v = *(const uint4*)p;
+  else if constexpr (VEC == 4)
+    r.v = *(const uint2*)p;
+  else
+    r.v = *p;
+}
+template <int VEC>
+__device__ __forceinline__ void add_row(const Raw<VEC>& r, float (&acc)[VEC]) {
+  if constexpr (VEC == 4) {
+    acc[0] += __uint_as_float(r.v.x << 16), acc[1] += __uint_as_float(r.v.x & 0xffff0000u);
+    acc[2] += __uint_as_float(r.v.y << 16), acc[3] += __uint_as_float(r.v.y & 0xffff0000u);
+  } else if constexpr (VEC == 8) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+    for (int e = 0; e < 4; ++e) {
+      acc[2 * e] += __uint_as_float(w[e] << 16);
+      acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+    }
+  } else {
+    acc[0] += st::bf16_to_f32(r.v);
   }
 }
 
-// The run that begins in chunk c and goes on behind it.
+template <int VEC>
+__global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t c = blockIdx.x, e0 = c * a.chunk;
+  const int many = (int)(e0 + a.chunk < a.n ? a.chunk : a.n - e0);
+  const int64_t mine = e0 - 1 + lane;
+  const bool here = mine >= 0 && mine < a.n && lane <= many + 1;
+  // before the first and after the last stands a token of no one's
+  const uint32_t tok = here ? a.tok[mine] : ~0u, pos = here ? a.pos[mine] : 0;
+  const uint32_t V = (uint32_t)a.V;
+  // entries from the first one that takes no part on are behind the end
+  const int count = __popcll(__ballot(here && lane >= 1 && lane <= many && tok < V));
+  const int64_t i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (!count || i >= a.H) return;  // no barriers below
+  auto token = [&](int e) { return __builtin_amdgcn_readlane(tok, e + 1); };  // -1..many
+  auto row = [&](int e) {
+    return a.dout + (int64_t)__builtin_amdgcn_readlane(pos, e + 1) * a.H + i;
+  };
+  bool from = token(-1) == token(0);  // the run began in an earlier chunk
+  float acc[VEC] = {};
+  for (int e0 = 0; e0 < count; e0 += AHEAD) {
+    Raw<VEC> now[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) read_row<VEC>(row(e0 + k < count ? e0 + k : e0), now[k]);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int e = e0 + k;
+      if (e >= count) break;
+      add_row<VEC>(now[k], acc);
+      const bool end = token(e + 1) != token(e);
+      if (!end && e + 1 < many) continue;
+      if (from)
+        store_f<VEC>(a.partial + c * 2 * a.H + i, acc);
+      else if (!end)
+        store_f<VEC>(a.partial + (c * 2 + 1) * a.H + i, acc);
+      else
+        write_row<VEC>(a, token(e), i, acc);
+      from = false;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+    }
+  }
+}
+
+// The run that begins in chunk c and goes on behind it: the partial sums of the
+// chunks whose first token it is, 64 chunks' tokens looked up at once.
 template <int VEC>
 __global__ __launch_bounds__(NTH) void join_runs(Sums a) {
-  const int64_t c = blockIdx.x, next = (c + 1) * a.chunk;  // next < n by the grid
-  const uint32_t token = a.tok[next];
+  const int lane = threadIdx.x & 63;
+  const int64_t c = blockIdx.x, e0 = c * a.chunk, next = e0 + a.chunk;  // next < n by the grid
+  const uint32_t token = a.tok[next], last = a.tok[next - 1], first = a.tok[e0];
+  const uint32_t before = e0 > 0 ? a.tok[e0 - 1] : ~0u;
   const int64_t i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  if (i >= a.H || token >= a.V || a.tok[next - 1] != token) return;
-  const int64_t e0 = c * a.chunk;
-  if (a.tok[e0] == token && e0 > 0 && a.tok[e0 - 1] == token) return;  // began earlier
-  float acc[VEC];
+  // (lanes past the columns stay: the others ask for their chunks)
+  if (token >= a.V || last != token) return;
+  if (first == token && before == token) return;  // began earlier
+  const bool in = i < a.H;
+  float acc[VEC] = {};
   const float* p = a.partial + (c * 2 + 1) * a.H + i;
+  if (in) {
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] = p[k];
-  for (int64_t d = c + 1; d * a.chunk < a.n && a.tok[d * a.chunk] == token; ++d) {
-    p = a.partial + d * 2 * a.H + i;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += p[k];
+    for (int k = 0; k < VEC; ++k) acc[k] = p[k];
   }
-  write_row<VEC>(a, token, i, acc);
+  for (int64_t d0 = c + 1;; d0 += 64) {
+    const int64_t e = (d0 + lane) * a.chunk;
+    const unsigned long long same = __ballot(e < a.n && a.tok[e < a.n ? e : 0] == token);
+    const int run = ~same ? __ffsll((long long)~same) - 1 : 64;
+    if (in) {
+      p = a.partial + d0 * 2 * a.H + i;
+#pragma unroll 8
+      for (int d = 0; d < run; ++d) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += p[d * 2 * a.H + k];
+      }
+    }
+    if (run < 64) break;
+  }
+  if (in) write_row<VEC>(a, token, i, acc);
 }
 
 // ---------------------------------------------------------------- host
-int64_t chunk_of(int64_t n) { return n <= 32768 ? 16 : 32; }
+int64_t chunk_of(int64_t n) { return n <= 16384 ? 8 : n <= 65536 ? 16 : 32; }
 int passes_of(int64_t V) {  // of keys 0..V
   int bits = 1;
   while (V >> bits) ++bits;
@@ -475,12 +609,11 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
       return st::fail(ST_EWORKSPACE, "st_embedding_bwd needs %lld workspace bytes", (long long)need);
     ST_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
   }
-  const int64_t blocks = st::cdiv(words, 4 * 1024);  // four words a thread at least
-  const unsigned fill = (unsigned)(blocks < 2048 ? blocks : 2048);
+  const unsigned fill = clear_blocks(words);
   if (tail)
     clear_tail<<<1, 64, 0, s>>>((uint16_t*)((char*)grad + bytes - 2 * tail), tail);
   if (n == 0) {
-    if (words) clear_words<<<fill * 4, NTH, 0, s>>>((uint4*)grad, words);
+    if (words) clear_words<<<fill, NTH, 0, s>>>((uint4*)grad, words);
     return st::check_launch("st_embedding_bwd");
   }
   const Layout l = layout(n, hidden);
@@ -488,23 +621,31 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
   const int passes = passes_of(vocab);
   int last = 0;
   if (n <= SMALL) {
-    sort_small<<<1 + fill, 1024, 0, s>>>(ids, ids32, (int)n, vocab, padding_idx, passes,
-                                         (uint32_t*)(w + l.tok[0]), (uint32_t*)(w + l.pos[0]),
-                                         (uint4*)grad, words);
+    const bool apart = words > CLEAR_APART;
+    if (apart) clear_words<<<fill, NTH, 0, s>>>((uint4*)grad, words);
+    sort_small<<<1 + (apart ? 0 : (fill + 3) / 4), 1024, 0, s>>>(
+        ids, ids32, (int)n, vocab, padding_idx, passes, (uint32_t*)(w + l.tok[0]),
+        (uint32_t*)(w + l.pos[0]), (uint4*)grad, apart ? 0 : words);
   } else {
-    if (words) clear_words<<<fill * 4, NTH, 0, s>>>((uint4*)grad, words);
     const int64_t tiles = st::cdiv(n, TILE);
     uint32_t* counts = (uint32_t*)(w + l.counts);
     for (int p = 0; p < passes; ++p) {
       const uint32_t* tok = p ? (const uint32_t*)(w + l.tok[last]) : nullptr;
       const uint32_t* pos = p ? (const uint32_t*)(w + l.pos[last]) : nullptr;
       const int to = p & 1;
-      tile_counts<<<(unsigned)tiles, NTH, 0, s>>>(ids, ids32, tok, n, vocab, padding_idx, BITS * p,
-                                                  tiles, counts);
-      tile_scan<<<1, 1024, 0, s>>>(counts, BINS * tiles);
-      tile_move<<<(unsigned)tiles, NTH, 0, s>>>(ids, ids32, tok, pos, n, vocab, padding_idx, BITS * p,
-                                                tiles, counts, (uint32_t*)(w + l.tok[to]),
-                                                (uint32_t*)(w + l.pos[to]));
+      tile_counts<<<(unsigned)(tiles + (p ? 0 : fill)), NTH, 0, s>>>(
+          ids, ids32, tok, n, vocab, padding_idx, BITS * p, tiles, counts, (uint4*)grad, words);
+      auto move = [&](auto kernel) {
+        kernel<<<(unsigned)tiles, NTH, 0, s>>>(ids, ids32, tok, pos, n, vocab, padding_idx, BITS * p,
+                                               tiles, counts, (uint32_t*)(w + l.tok[to]),
+                                               (uint32_t*)(w + l.pos[to]));
+      };
+      if (tiles <= MOVE_TILES) {
+        move(tile_move<false>);
+      } else {
+        tile_scan<<<1, 1024, 0, s>>>(counts, BINS * tiles);
+        move(tile_move<true>);
+      }
       last = to;
     }
   }
@@ -513,13 +654,17 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
   a.n = n, a.V = vocab, a.H = hidden, a.chunk = chunk_of(n), a.scale = scale;
   a.grad_f32 = grad_dtype == ST_DTYPE_F32, a.accumulate = accumulate, a.grad = grad;
   a.partial = (float*)(w + l.partial);
-  const bool vec = hidden % 8 == 0 && ((uintptr_t)dout & 15) == 0;
-  const unsigned th = threads_of(hidden, vec ? 8 : 1);
-  const int64_t chunks = st::cdiv(n, a.chunk), slices = st::cdiv(hidden, (int64_t)th * (vec ? 8 : 1));
+  // as many columns a lane as make 16 bytes of the gradient
+  const int vec = hidden % 8 == 0 && ((uintptr_t)dout & 15) == 0 ? (a.grad_f32 ? 4 : 8) : 1;
+  const unsigned th = threads_of(hidden, vec);
+  const int64_t chunks = st::cdiv(n, a.chunk), slices = st::cdiv(hidden, (int64_t)th * vec);
   if (chunks * slices * th >= (int64_t)1 << 32 || slices >= 65536)
     return st::fail(ST_EUNSUPPORTED, "st_embedding_bwd: more threads than a launch takes");
   const dim3 grid((unsigned)chunks, (unsigned)slices), more((unsigned)chunks - 1, (unsigned)slices);
-  if (vec) {
+  if (vec == 4) {
+    sum_runs<4><<<grid, th, 0, s>>>(a);
+    if (chunks > 1) join_runs<4><<<more, th, 0, s>>>(a);
+  } else if (vec == 8) {
     sum_runs<8><<<grid, th, 0, s>>>(a);
     if (chunks > 1) join_runs<8><<<more, th, 0, s>>>(a);
   } else {
