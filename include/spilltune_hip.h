@@ -651,10 +651,10 @@ int st_moe_lora_grads(int64_t rows, int32_t R, int64_t seg_len, int32_t nseg,
  * rstd_post, rstd_pre (fp32 [rows]) are kept for the backward, or NULL.
  *
  * The backward takes dh and dnormed (either may be NULL: no gradient) and writes
- * what is asked for (not NULL): dy, dresidual; dpost and dpre fp32 [hidden]; dgate
- * fp32 [rows / rows_per, hidden] or [rows], or of the gate's type for ST_GATE_FULL.
- * Sums over rows are joined in a fixed order in `workspace`, which dpost, dpre and
- * the gate of ST_GATE_COLUMNS need (query with rows_per = rows for other gates).
+ * what is asked for (not NULL): dy, dresidual; dpost and dpre bf16 [hidden]; dgate
+ * of the gate's shape and type.  Sums over rows are joined in a fixed order in
+ * `workspace`, which dpost, dpre and the gate of ST_GATE_COLUMNS need (query with
+ * rows_per = rows for other gates).
  */
 #define ST_GATE_NONE 0
 #define ST_GATE_COLUMNS 1
@@ -671,8 +671,8 @@ int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual, const uin
                           int32_t gate_dtype, int64_t rows_per, int64_t rows, int64_t hidden,
                           float scale, float eps, const float* rstd_post,
                           const float* rstd_pre, const uint16_t* dh, const uint16_t* dnormed,
-                          uint16_t* dy, uint16_t* dresidual, void* dgate, float* dpost,
-                          float* dpre, void* workspace, int64_t workspace_bytes,
+                          uint16_t* dy, uint16_t* dresidual, void* dgate, uint16_t* dpost,
+                          uint16_t* dpre, void* workspace, int64_t workspace_bytes,
                           st_stream_t stream);
 
 /* -------------------------------------------------------------- embedding */

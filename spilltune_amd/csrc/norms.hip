@@ -46,7 +46,7 @@ struct Args {
   // backward
   const uint16_t *dh, *dn;
   uint16_t *dy, *dres;
-  void* dgate;     // GATE_FULL: the gate's type; GATE_TOKENS: fp32 [rows]
+  void* dgate;     // of the gate's type
   float* partial;  // [runs][3][H]: dpost, dpre, dgate of the run's rows
   int64_t runs, per_run;
 };
@@ -70,19 +70,42 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return v;
 }
 
+// VEC bf16 as they lie.  Elements past the row (`in` false) read its first ones and are
+// cleared: a load under a branch would be waited for at the branch's end.
 template <int VEC>
-__device__ __forceinline__ void load_bf16(const uint16_t* p, int64_t i, bool in, float (&f)[VEC]) {
+struct Raw {
+  uint4 v;
+};
+template <>
+struct Raw<1> {
+  uint32_t v;
+};
+template <int VEC>
+__device__ __forceinline__ Raw<VEC> raw(const uint16_t* row, int64_t i, bool in) {
+  Raw<VEC> r;
+  if constexpr (VEC == 8)
+    r.v = *(const uint4*)(row + (in ? i : 0));
+  else
+    r.v = row[in ? i : 0];
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ void unpack(const Raw<VEC>& r, bool in, float (&f)[VEC]) {
   if constexpr (VEC == 8) {
-    const uint4 v = in ? *(const uint4*)(p + i) : make_uint4(0, 0, 0, 0);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t w[4] = {in ? r.v.x : 0, in ? r.v.y : 0, in ? r.v.z : 0, in ? r.v.w : 0};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       f[2 * e] = __uint_as_float(w[e] << 16);
       f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
     }
   } else {
-    f[0] = in ? st::bf16_to_f32(p[i]) : 0.0f;
+    f[0] = in ? __uint_as_float(r.v << 16) : 0.0f;
   }
+}
+template <int VEC>
+__device__ __forceinline__ void load_bf16(const uint16_t* row, int64_t i, bool in,
+                                          float (&f)[VEC]) {
+  unpack<VEC>(raw<VEC>(row, i, in), in, f);
 }
 template <int VEC>
 __device__ __forceinline__ void store_bf16(uint16_t* p, int64_t i, const float (&f)[VEC]) {
@@ -93,14 +116,16 @@ __device__ __forceinline__ void store_bf16(uint16_t* p, int64_t i, const float (
     p[i] = st::f32_to_bf16(f[0]);
 }
 template <int VEC>
-__device__ __forceinline__ void load_f32(const float* p, int64_t i, bool in, float (&f)[VEC]) {
+__device__ __forceinline__ void load_f32(const float* row, int64_t i, bool in, float (&f)[VEC]) {
+  const float* p = row + (in ? i : 0);
   if constexpr (VEC == 8) {
-    const float4 z = make_float4(0, 0, 0, 0);
-    const float4 a = in ? *(const float4*)(p + i) : z, b = in ? *(const float4*)(p + i + 4) : z;
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
   } else {
-    f[0] = in ? p[i] : 0.0f;
+    f[0] = *p;
   }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] = in ? f[e] : 0.0f;
 }
 template <int VEC>
 __device__ __forceinline__ void store_f32(float* p, int64_t i, const float (&f)[VEC]) {
@@ -128,11 +153,11 @@ __device__ __forceinline__ void gate_of(const Args& a, int64_t row, int64_t i, b
     for (int e = 0; e < VEC; ++e) f[e] = a.scale * g;
     return;
   }
-  const int64_t at = (a.gate_mode == GATE_FULL ? row : row / a.rows_per) * a.H + i;
+  const int64_t at = (a.gate_mode == GATE_FULL ? row : row / a.rows_per) * a.H;
   if (a.gate_f32)
-    load_f32<VEC>((const float*)a.gate, at, in, f);
+    load_f32<VEC>((const float*)a.gate + at, i, in, f);
   else
-    load_bf16<VEC>((const uint16_t*)a.gate, at, in, f);
+    load_bf16<VEC>((const uint16_t*)a.gate + at, i, in, f);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) f[e] *= a.scale;
 }
@@ -147,8 +172,8 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
-      load_bf16<VEC>(a.y, base + i, i < a.H, y[n]);
-      load_bf16<VEC>(a.res, base + i, i < a.H, h[n]);
+      load_bf16<VEC>(a.y + base, i, i < a.H, y[n]);
+      load_bf16<VEC>(a.res + base, i, i < a.H, h[n]);
     }
     float r1 = 1.0f;
     if (a.post) {
@@ -173,7 +198,7 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
         h[n][e] += g[e] * z;
         ss += h[n][e] * h[n][e];
       }
-      if (i < a.H) store_bf16<VEC>(a.h, base + i, h[n]);
+      if (i < a.H) store_bf16<VEC>(a.h + base, i, h[n]);
     }
     if (a.pre) {  // the same way for the whole launch
       const float r2 = 1.0f / sqrtf(block_sum<NT>(ss, red[1]) * over + a.eps);
@@ -185,7 +210,7 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
         load_bf16<VEC>(a.pre, i, i < a.H, w);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) w[e] *= h[n][e] * r2;
-        if (i < a.H) store_bf16<VEC>(a.normed, base + i, w);
+        if (i < a.H) store_bf16<VEC>(a.normed + base, i, w);
       }
     }
     if constexpr (NT > 64) __syncthreads();  // the sums' places are free again
@@ -193,9 +218,13 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
 }
 
 // SUMS: run blockIdx.x of `per_run` rows (all of one gate row), columns' sums kept.
-template <int VEC, int NT, int NV, bool SUMS>
+// GATE: there is one.  The next row is read while the present one is worked on (up to
+// 16 elements a thread: beyond, registers are short), and rows wait as the bf16 they
+// are: with them in fp32, fewer waves fit.
+template <int VEC, int NT, int NV, bool SUMS, bool GATE>
 __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
   __shared__ float red[3][NT / 64];
+  constexpr bool EARLY = SUMS && VEC * NV <= 16;
   const float over = 1.0f / (float)a.H;
   float dpost[NV][VEC] = {}, dpre[NV][VEC] = {}, dgate[NV][VEC] = {};
   int64_t row, end, by;
@@ -207,76 +236,106 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
   } else {
     row = blockIdx.x, end = a.rows, by = gridDim.x;
   }
-  for (; row < end; row += by) {
-    const int64_t base = row * a.H;
-    float y[NV][VEC], h[NV][VEC], d[NV][VEC], gn[NV][VEC];
+  // (a gradient that is not there: y in its place, cleared)
+  const bool has_dh = a.dh, has_dn = a.dn;
+  const uint16_t *dh = has_dh ? a.dh : a.y, *dn = has_dn ? a.dn : a.y;
+  Raw<VEC> ny[NV], nh[NV], nd[NV], nn[NV];
+  auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
-      const bool in = i < a.H;
-      load_bf16<VEC>(a.y, base + i, in, y[n]);
-      load_bf16<VEC>(a.res, base + i, in, h[n]);
-      load_bf16<VEC>(a.dh, base + i, in && a.dh, d[n]);
-      load_bf16<VEC>(a.dn, base + i, in && a.dn, gn[n]);
+      const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC, base = r * a.H;
+      ny[n] = raw<VEC>(a.y + base, i, i < a.H);
+      nh[n] = raw<VEC>(a.res + base, i, i < a.H);
+      nd[n] = raw<VEC>(dh + base, i, i < a.H);
+      nn[n] = raw<VEC>(dn + base, i, i < a.H);
     }
-    const float r1 = a.post ? a.r1[row] : 1.0f, r2 = a.dn ? a.r2[row] : 0.0f;
-    if (a.dn) {
-      float dot = 0.0f;
+  };
+  fetch(row);
+  for (; row < end; row += by) {
+    const int64_t base = row * a.H;
+    Raw<VEC> ry[NV], rh[NV], rd[NV], rn[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) ry[n] = ny[n], rh[n] = nh[n], rd[n] = nd[n], rn[n] = nn[n];
+    if (EARLY) fetch(row + by < end ? row + by : row);
+    const float r1 = a.post ? a.r1[row] : 1.0f, r2 = has_dn ? a.r2[row] : 0.0f;
+    float d[NV][VEC];
+    if (has_dn) {
+      float h[NV][VEC], gn[NV][VEC], dot = 0.0f;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
         const bool in = i < a.H;
-        float w[VEC], g[VEC], p[VEC];
+        float y[VEC], w[VEC], g[VEC], p[VEC];
+        unpack<VEC>(ry[n], in, y);
+        unpack<VEC>(rh[n], in, h[n]);
+        unpack<VEC>(rn[n], in, gn[n]);
         if (a.post) load_bf16<VEC>(a.post, i, in, w);
         load_bf16<VEC>(a.pre, i, in, p);
-        gate_of<VEC>(a, row, i, in, g);
+        if (GATE) gate_of<VEC>(a, row, i, in, g);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          h[n][e] += g[e] * (a.post ? y[n][e] * r1 * w[e] : y[n][e]);
-          if constexpr (SUMS) dpre[n][e] += gn[n][e] * h[n][e] * r2;
+          const float z = a.post ? y[e] * r1 * w[e] : y[e];
+          h[n][e] = __builtin_fmaf(GATE ? g[e] : a.scale, z, h[n][e]);
+          if constexpr (SUMS) dpre[n][e] = __builtin_fmaf(gn[n][e], h[n][e] * r2, dpre[n][e]);
           gn[n][e] *= p[e];
-          dot += gn[n][e] * h[n][e];
+          dot = __builtin_fmaf(gn[n][e], h[n][e], dot);
         }
       }
       const float c = block_sum<NT>(dot, red[0]) * over * r2 * r2;
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
+      for (int n = 0; n < NV; ++n) {
+        const bool in = ((int64_t)n * NT + threadIdx.x) * VEC < a.H;
+        unpack<VEC>(rd[n], in && has_dh, d[n]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d[n][e] += r2 * (gn[n][e] - h[n][e] * c);
+        for (int e = 0; e < VEC; ++e)
+          d[n][e] = __builtin_fmaf(r2, __builtin_fmaf(-c, h[n][e], gn[n][e]), d[n][e]);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        unpack<VEC>(rd[n], ((int64_t)n * NT + threadIdx.x) * VEC < a.H && has_dh, d[n]);
     }
     float dot = 0.0f, gdot = 0.0f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
       const bool in = i < a.H;
-      if (a.dres && in) store_bf16<VEC>(a.dres, base + i, d[n]);
-      float w[VEC], g[VEC], dz[VEC];
+      if (a.dres && in) store_bf16<VEC>(a.dres + base, i, d[n]);
+      float y[VEC], w[VEC], g[VEC], dz[VEC];
+      unpack<VEC>(ry[n], in, y);
       if (a.post) load_bf16<VEC>(a.post, i, in, w);
-      gate_of<VEC>(a, row, i, in, g);
+      if (GATE) gate_of<VEC>(a, row, i, in, g);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float yn = y[n][e] * r1, z = a.post ? yn * w[e] : yn;
-        dz[e] = a.scale * d[n][e] * z;
-        gdot += dz[e];
-        float q = g[e] * d[n][e];
+        const float yn = y[e] * r1;
+        if (GATE) {
+          dz[e] = a.scale * d[n][e] * (a.post ? yn * w[e] : yn);
+          gdot += dz[e];
+        }
+        float q = (GATE ? g[e] : a.scale) * d[n][e];
         if constexpr (SUMS) {
-          dgate[n][e] += dz[e];
-          dpost[n][e] += q * yn;
+          if (GATE) dgate[n][e] += dz[e];
+          dpost[n][e] = __builtin_fmaf(q, yn, dpost[n][e]);
         }
         if (a.post) q *= w[e];
-        dot += q * y[n][e];
+        dot = __builtin_fmaf(q, y[e], dot);
         d[n][e] = q;
       }
-      if (a.gate_mode == GATE_FULL && a.dgate && in) {
+      if (GATE && a.gate_mode == GATE_FULL && a.dgate && in) {
         if (a.gate_f32)
-          store_f32<VEC>((float*)a.dgate, base + i, dz);
+          store_f32<VEC>((float*)a.dgate + base, i, dz);
         else
-          store_bf16<VEC>((uint16_t*)a.dgate, base + i, dz);
+          store_bf16<VEC>((uint16_t*)a.dgate + base, i, dz);
       }
     }
-    if (a.gate_mode == GATE_TOKENS && a.dgate) {
+    if (GATE && a.gate_mode == GATE_TOKENS && a.dgate) {
       gdot = block_sum<NT>(gdot, red[1]);
-      if (threadIdx.x == 0) ((float*)a.dgate)[row] = gdot;
+      if (threadIdx.x == 0) {
+        if (a.gate_f32)
+          ((float*)a.dgate)[row] = gdot;
+        else
+          ((uint16_t*)a.dgate)[row] = st::f32_to_bf16(gdot);
+      }
     }
     if (a.dy) {
       float c = 0.0f;
@@ -284,13 +343,17 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
+        const bool in = i < a.H;
         if (a.post) {
+          float y[VEC];
+          unpack<VEC>(ry[n], in, y);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[n][e] = r1 * (d[n][e] - y[n][e] * c);
+          for (int e = 0; e < VEC; ++e) d[n][e] = r1 * __builtin_fmaf(-c, y[e], d[n][e]);
         }
-        if (i < a.H) store_bf16<VEC>(a.dy, base + i, d[n]);
+        if (in) store_bf16<VEC>(a.dy + base, i, d[n]);
       }
     }
+    if (!EARLY && row + by < end) fetch(row + by);
     if constexpr (NT > 64) __syncthreads();  // the sums' places are free again
   }
   if constexpr (SUMS) {
@@ -301,7 +364,7 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
       if (i >= a.H) continue;
       store_f32<VEC>(to, i, dpost[n]);
       store_f32<VEC>(to + a.H, i, dpre[n]);
-      store_f32<VEC>(to + 2 * a.H, i, dgate[n]);
+      if (GATE) store_f32<VEC>(to + 2 * a.H, i, dgate[n]);
     }
   }
 }
@@ -310,13 +373,13 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
 // runs each.  blockIdx.y: dpost, dpre, then dgate's rows.
 __global__ __launch_bounds__(1024) void norms_join(const float* __restrict__ partial, int64_t H,
                                                    int64_t runs, int64_t groups,
-                                                   float* __restrict__ dpost,
-                                                   float* __restrict__ dpre,
-                                                   float* __restrict__ dgate) {
+                                                   uint16_t* __restrict__ dpost,
+                                                   uint16_t* __restrict__ dpre,
+                                                   void* __restrict__ dgate, int gate_f32) {
   __shared__ float red[16][64];
   const int col = threadIdx.x & 63, part = threadIdx.x >> 6;
   const int64_t i = (int64_t)blockIdx.x * 64 + col, what = blockIdx.y;
-  float* out = what == 0 ? dpost : what == 1 ? dpre : dgate;
+  void* out = what == 0 ? dpost : what == 1 ? dpre : dgate;
   if (!out) return;
   const int64_t many = what < 2 ? runs : runs / groups, first = what < 2 ? 0 : (what - 2) * many;
   const int64_t share = (many + 15) / 16, a = part * share, z = min(a + share, many);
@@ -331,15 +394,21 @@ __global__ __launch_bounds__(1024) void norms_join(const float* __restrict__ par
   if (part == 0 && i < H) {
     s = red[0][col];
     for (int k = 1; k < 16; ++k) s += red[k][col];
-    out[(what < 2 ? 0 : what - 2) * H + i] = s;
+    const int64_t at = (what < 2 ? 0 : what - 2) * H + i;
+    if (what >= 2 && gate_f32)
+      ((float*)out)[at] = s;
+    else
+      ((uint16_t*)out)[at] = st::f32_to_bf16(s);
   }
 }
 
 // ---------------------------------------------------------------- host
-// Runs of rows in a backward that sums over rows: about 512, never across gate rows.
-void plan_runs(int64_t rows, int64_t rows_per, int64_t& runs, int64_t& per_run) {
+// Runs of rows in a backward that sums over rows, never across gate rows: as many as
+// workgroups run at once, so that none waits for a second turn (2103 rows of 7168: 421
+// runs of 5 rows 76 us, 234 of 9 rows 66).
+void plan_runs(int64_t rows, int64_t rows_per, int64_t H, int64_t& runs, int64_t& per_run) {
   const int64_t groups = rows / rows_per;
-  int64_t each = st::cdiv(512, groups);
+  int64_t each = st::cdiv(H > 4096 ? 256 : 512, groups);
   if (each > rows_per) each = rows_per;
   per_run = st::cdiv(rows_per, each);
   runs = groups * st::cdiv(rows_per, per_run);
@@ -350,22 +419,32 @@ void go(const Args& a, bool bwd, bool sums, hipStream_t s) {
   const unsigned grid = (unsigned)(a.rows < (1 << 20) ? a.rows : 1 << 20);
   if (!bwd)
     norms_fwd<VEC, NT, NV><<<grid, NT, 0, s>>>(a);
+  else if (sums && a.gate)
+    norms_bwd<VEC, NT, NV, true, true><<<(unsigned)a.runs, NT, 0, s>>>(a);
   else if (sums)
-    norms_bwd<VEC, NT, NV, true><<<(unsigned)a.runs, NT, 0, s>>>(a);
+    norms_bwd<VEC, NT, NV, true, false><<<(unsigned)a.runs, NT, 0, s>>>(a);
+  else if (a.gate)
+    norms_bwd<VEC, NT, NV, false, true><<<grid, NT, 0, s>>>(a);
   else
-    norms_bwd<VEC, NT, NV, false><<<grid, NT, 0, s>>>(a);
+    norms_bwd<VEC, NT, NV, false, false><<<grid, NT, 0, s>>>(a);
 }
 
-// A row in one wave where it fits (no barriers), in four to sixteen waves otherwise;
-// rows of whole 16-byte chunks eight elements a lane at a time, others one by one.
+// A row in one wave where it fits (no barriers), in two to sixteen waves otherwise;
+// rows of whole 16-byte chunks eight elements a lane at a time, others one by one.  The
+// forward and the sums over rows do better with sixteen elements a thread (fewer waves
+// at a barrier; 8192 rows of 4096 forward 47 us against 52), the plain backward with
+// eight (84 against 95).
 void dispatch(const Args& a, bool bwd, bool sums, hipStream_t s) {
   const int64_t H = a.H;
   if (H % 8 == 0) {
     if (H <= 512) go<8, 64, 1>(a, bwd, sums, s);
-    else if (H <= 1024) go<8, 64, 2>(a, bwd, sums, s);
+    else if (H <= 1024) go<8, 128, 1>(a, bwd, sums, s);
     else if (H <= 2048) go<8, 256, 1>(a, bwd, sums, s);
+    else if (H <= 4096 && bwd) go<8, 512, 1>(a, bwd, sums, s);
     else if (H <= 4096) go<8, 256, 2>(a, bwd, sums, s);
+    else if (H <= 8192 && bwd && !sums) go<8, 1024, 1>(a, bwd, sums, s);
     else if (H <= 8192) go<8, 512, 2>(a, bwd, sums, s);
+    else if (bwd && sums) go<8, 512, 4>(a, bwd, sums, s);
     else go<8, 1024, 2>(a, bwd, sums, s);
   } else {
     if (H <= 256) go<1, 64, 4>(a, bwd, sums, s);
@@ -426,7 +505,7 @@ extern "C" int st_residual_norms_fwd(const uint16_t* y, const uint16_t* residual
 extern "C" int64_t st_residual_norms_workspace_bytes(int64_t rows, int64_t hidden, int64_t rows_per) {
   if (rows < 1 || hidden < 1 || rows_per < 1 || rows % rows_per) return 0;
   int64_t runs, per_run;
-  plan_runs(rows, rows_per, runs, per_run);
+  plan_runs(rows, rows_per, hidden, runs, per_run);
   return runs * 3 * hidden * 4;
 }
 
@@ -436,7 +515,7 @@ extern "C" int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual
                                      int64_t rows, int64_t hidden, float scale, float eps,
                                      const float* rstd_post, const float* rstd_pre,
                                      const uint16_t* dh, const uint16_t* dnormed, uint16_t* dy,
-                                     uint16_t* dresidual, void* dgate, float* dpost, float* dpre,
+                                     uint16_t* dresidual, void* dgate, uint16_t* dpost, uint16_t* dpre,
                                      void* workspace, int64_t workspace_bytes,
                                      st_stream_t stream) {
   Args a = {};
@@ -455,7 +534,7 @@ extern "C" int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual
   if (sums) {
     // gate rows only bound the runs where their sums are asked for
     if (!columns) a.rows_per = gate_mode == GATE_COLUMNS ? rows_per : rows;
-    plan_runs(rows, a.rows_per, a.runs, a.per_run);
+    plan_runs(rows, a.rows_per, hidden, a.runs, a.per_run);
     const int64_t need = a.runs * 3 * hidden * 4;
     if (!workspace || workspace_bytes < need)
       return st::fail(ST_EWORKSPACE, "st_residual_norms_bwd needs %lld workspace bytes",
@@ -468,7 +547,7 @@ extern "C" int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual
     dispatch(a, true, true, (hipStream_t)stream);
     norms_join<<<dim3((unsigned)st::cdiv(hidden, 64), (unsigned)(columns ? groups + 2 : 2)), 1024, 0,
                  (hipStream_t)stream>>>(a.partial, hidden, a.runs, groups, dpost, dpre,
-                                        columns ? (float*)dgate : nullptr);
+                                        columns ? dgate : nullptr, a.gate_f32);
   } else {
     dispatch(a, true, false, (hipStream_t)stream);
   }

@@ -711,14 +711,12 @@ class _ResidualNorms(torch.autograd.Function):
         dh, dn = (None if g is None else _operand(g) for g in (dh, dn))
         need = ctx.needs_input_grad
         dy, dres = (torch.empty_like(y) if n else None for n in need[:2])
-        dpost = torch.empty(H, dtype=_F32, device=dev) if need[2] else None
-        dpre = torch.empty(H, dtype=_F32, device=dev) if need[3] and dn is not None else None
-        dgate = None
-        if need[4]:
-            dgate = torch.empty_like(gate, dtype=gate.dtype if mode == _lib.ST_GATE_FULL else _F32)
+        dpost = torch.empty_like(post) if need[2] else None
+        dpre = torch.empty_like(pre) if need[3] and dn is not None else None
+        dgate = torch.empty_like(gate) if need[4] else None
         if not rows:
-            return dy, dres, *(None if g is None else g.zero_().to(p.dtype)
-                               for g, p in ((dpost, post), (dpre, pre), (dgate, gate))), *(None,) * 4
+            return dy, dres, *(None if g is None else g.zero_() for g in (dpost, dpre, dgate)), \
+                *(None,) * 4
         with _lib.on_device(dev):
             nbytes = 0
             if dpost is not None or dpre is not None or (dgate is not None
@@ -732,9 +730,7 @@ class _ResidualNorms(torch.autograd.Function):
                       _lib.ptr(r1), _lib.ptr(r2), _lib.ptr(dh), _lib.ptr(dn), _lib.ptr(dy),
                       _lib.ptr(dres), _lib.ptr(dgate), _lib.ptr(dpost), _lib.ptr(dpre),
                       _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
-        return (dy, dres, *(None if g is None else g.to(p.dtype)
-                            for g, p in ((dpost, post), (dpre, pre), (dgate, gate))),
-                None, None, None, None)
+        return dy, dres, dpost, dpre, dgate, None, None, None, None
 
 
 def _gate_kind(gate, shape):
