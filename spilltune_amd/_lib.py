@@ -236,7 +236,8 @@ class RkProduct(ctypes.Structure):
 
 
 class MatrixBatch(ctypes.Structure):
-    """``st_matrix_batch`` (include/spilltune_hip.h): equal matrices back to back."""
+    """``st_matrix_batch`` (include/spilltune_hip.h): equal matrices back to back; five
+    64-bit words, which a caller with many may write as such."""
     _fields_ = [("x", ctypes.c_void_p), ("out", ctypes.c_void_p), ("count", ctypes.c_int64),
                 ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
 
@@ -253,4 +254,4 @@ def lut_array(values) -> ctypes.Array:
 
 
 def i64_array(values) -> ctypes.Array:
-    return (ctypes.c_int64 * max(1, len(values)))(*[int(v) for v in values])
+    return (ctypes.c_int64 * max(1, len(values)))(*map(int, values))

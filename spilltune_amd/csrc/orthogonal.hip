@@ -29,7 +29,7 @@ namespace {
 typedef double d4 __attribute__((ext_vector_type(4)));
 typedef double d2 __attribute__((ext_vector_type(2)));
 constexpr int NTH = 256;
-constexpr int MAXE = 48;        // entries of a launch's table (kernel arguments: 4 KB)
+constexpr int MAXE = 44;        // entries of a launch's table (kernel arguments: 4 KB)
 constexpr int64_t MAXR = 1024;  // short side
 
 // A batch of equal matrices, back to back.
@@ -43,7 +43,7 @@ struct Entry {
   int16_t tall;            // the short side is the contiguous one
   int16_t vec;             // rows may be read four elements at a time
 };
-enum { IN_GRAM, IN_SUM, IN_POLY, IN_APPLY, PHASES };
+enum { IN_GRAM, IN_SUM, IN_NORM, IN_POLY, IN_APPLY, PHASES };
 struct Table {
   Entry e[MAXE];
   uint32_t tile0[PHASES][64];  // the entries' first workgroups in a phase, then ~0
@@ -65,21 +65,26 @@ __device__ __forceinline__ const Entry& find(const Table& t, int phase, uint32_t
   return t.e[i];
 }
 
+// Pointers that were read from memory, said to be ones to device memory: otherwise
+// their loads are flat ones, which are counted as LDS reads too and waited for with them.
+#define GLOBAL(T) __attribute__((address_space(1))) T
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
 template <bool BF>
 __device__ __forceinline__ float load1(const void* p, int64_t i) {
   if constexpr (BF)
-    return st::bf16_to_f32(((const uint16_t*)p)[i]);
+    return st::bf16_to_f32(((const GLOBAL(uint16_t)*)p)[i]);
   else
-    return ((const float*)p)[i];
+    return ((const GLOBAL(float)*)p)[i];
 }
 template <bool BF>
 __device__ __forceinline__ void load4(const void* p, int64_t i, float* f) {
   if constexpr (BF) {
-    const uint2 w = *(const uint2*)((const uint16_t*)p + i);
+    const u32x2 w = *(const GLOBAL(u32x2)*)((const uint16_t*)p + i);
     f[0] = __uint_as_float(w.x << 16), f[1] = __uint_as_float(w.x & 0xffff0000u);
     f[2] = __uint_as_float(w.y << 16), f[3] = __uint_as_float(w.y & 0xffff0000u);
   } else {
-    const float4 w = *(const float4*)((const float*)p + i);
+    const f32x4 w = *(const GLOBAL(f32x4)*)((const float*)p + i);
     f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
   }
 }
@@ -97,19 +102,19 @@ template <bool BF>
 __device__ __forceinline__ void store_upto4(void* p, int64_t i, int n, bool vec, const float* f) {
   if (vec && n >= 4) {
     if constexpr (BF)
-      *(uint2*)((uint16_t*)p + i) =
-          make_uint2(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]));
+      *(GLOBAL(u32x2)*)((uint16_t*)p + i) =
+          u32x2{st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3])};
     else
-      *(float4*)((float*)p + i) = make_float4(f[0], f[1], f[2], f[3]);
+      *(GLOBAL(f32x4)*)((float*)p + i) = f32x4{f[0], f[1], f[2], f[3]};
     return;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (e < n) {
       if constexpr (BF)
-        ((uint16_t*)p)[i + e] = st::f32_to_bf16(f[e]);
+        ((GLOBAL(uint16_t)*)p)[i + e] = st::f32_to_bf16(f[e]);
       else
-        ((float*)p)[i + e] = f[e];
+        ((GLOBAL(float)*)p)[i + e] = f[e];
     }
 }
 
@@ -163,44 +168,64 @@ __device__ __forceinline__ void clear_rows(const Entry& e, int row0, int lane, f
 
 // acc[i][j] += rows rowa + 16 i times rows rowb + 16 j over k0, k0 + step, .. < k1;
 // SAME: the two are one, and the tiles below the diagonal stay out.
-template <bool BF, int T, bool TALL, bool SAME>
+template <bool BF, int TA, int TB, bool TALL, bool SAME>
 __device__ __forceinline__ void gram_walk(const Entry& e, const void* x, int rowa, int rowb,
                                           int64_t k0, int64_t k1, int step, int lane,
-                                          d4 (&acc)[T][T]) {
-  auto multiply = [&](float (&a)[T][8], float (&b)[T][8]) {
-    clear_rows<T>(e, rowa, lane, a);
-    if constexpr (!SAME) clear_rows<T>(e, rowb, lane, b);
+                                          d4 (&acc)[TA][TB]) {
+  auto multiply = [&](float (&a)[TA][8], float (&b)[TB][8]) {
+    clear_rows<TA>(e, rowa, lane, a);
+    if constexpr (!SAME) clear_rows<TB>(e, rowb, lane, b);
 #pragma unroll
     for (int s = 0; s < 8; ++s)
 #pragma unroll
-      for (int i = 0; i < T; ++i)
+      for (int i = 0; i < TA; ++i)
 #pragma unroll
-        for (int j = SAME ? i : 0; j < T; ++j)
+        for (int j = SAME ? i : 0; j < TB; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(
-              (double)a[i][s], (double)(SAME ? a : b)[j][s], acc[i][j], 0, 0, 0);
+              (double)a[i][s], SAME ? (double)a[j < TA ? j : 0][s] : (double)b[j][s], acc[i][j], 0, 0,
+              0);
   };
-  float a[T][8], b[T][8], na[T][8], nb[T][8];
+  float a[TA][8], b[TB][8], na[TA][8], nb[TB][8];
   if (e.vec || TALL) {
     if (k0 + 32 <= k1) {
-      gram_rows<BF, T, TALL, true>(e, x, rowa, k0, k1, lane, na);
-      if constexpr (!SAME) gram_rows<BF, T, TALL, true>(e, x, rowb, k0, k1, lane, nb);
+      gram_rows<BF, TA, TALL, true>(e, x, rowa, k0, k1, lane, na);
+      if constexpr (!SAME) gram_rows<BF, TB, TALL, true>(e, x, rowb, k0, k1, lane, nb);
     }
     for (; k0 + 32 <= k1; k0 += step) {
       const int64_t next = k0 + step + 32 <= k1 ? k0 + step : k0;
 #pragma unroll
-      for (int i = 0; i < T; ++i)
+      for (int s = 0; s < 8; ++s) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s) a[i][s] = na[i][s], b[i][s] = SAME ? 0.0f : nb[i][s];
-      gram_rows<BF, T, TALL, true>(e, x, rowa, next, k1, lane, na);
-      if constexpr (!SAME) gram_rows<BF, T, TALL, true>(e, x, rowb, next, k1, lane, nb);
+        for (int i = 0; i < TA; ++i) a[i][s] = na[i][s];
+#pragma unroll
+        for (int i = 0; i < TB; ++i) b[i][s] = SAME ? 0.0f : nb[i][s];
+      }
+      gram_rows<BF, TA, TALL, true>(e, x, rowa, next, k1, lane, na);
+      if constexpr (!SAME) gram_rows<BF, TB, TALL, true>(e, x, rowb, next, k1, lane, nb);
       multiply(a, b);
     }
   }
   for (; k0 < k1; k0 += step) {
-    gram_rows<BF, T, TALL, false>(e, x, rowa, k0, k1, lane, a);
-    if constexpr (!SAME) gram_rows<BF, T, TALL, false>(e, x, rowb, k0, k1, lane, b);
+    gram_rows<BF, TA, TALL, false>(e, x, rowa, k0, k1, lane, a);
+    if constexpr (!SAME) gram_rows<BF, TB, TALL, false>(e, x, rowb, k0, k1, lane, b);
     multiply(a, b);
   }
+}
+// One wave's tiles of a block of 4 x 4, from tile (ti, tj) on, over a chunk.
+template <bool BF, int TA, int TB, bool SAME>
+__device__ __forceinline__ void gram_tiles(const Entry& e, const void* x, int rowI, int rowJ, int ti,
+                                           int tj, int64_t k0, int64_t k1, int lane, double* to) {
+  d4 acc[TA][TB] = {};
+  if (e.tall)
+    gram_walk<BF, TA, TB, true, SAME>(e, x, rowI + 16 * ti, rowJ + 16 * tj, k0, k1, 32, lane, acc);
+  else
+    gram_walk<BF, TA, TB, false, SAME>(e, x, rowI + 16 * ti, rowJ + 16 * tj, k0, k1, 32, lane, acc);
+#pragma unroll
+  for (int i = 0; i < TA; ++i)
+#pragma unroll
+    for (int j = SAME ? i : 0; j < TB; ++j)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) to[((ti + i) * 4 + tj + j) * 256 + v * 64 + lane] = acc[i][j][v];
 }
 
 template <int T, bool BF>
@@ -227,28 +252,22 @@ __global__ __launch_bounds__(NTH) void gram(Table tab, double* __restrict__ part
   double* to = part + e.part + ((int64_t)mc * pairs + pair) * (T * T * 256);
   if constexpr (T == 4) {
     // Each wave a quarter of the block, two tiles by two, over the whole chunk: 32
-    // registers of sums leave room for more waves, and for the elements under way.
-    const int wi = wave >> 1, wj = wave & 1;
-    if (I == J && wi > wj) return;
-    d4 acc[2][2] = {};
-    const int ra = I * 64 + 32 * wi, rb = J * 64 + 32 * wj;
-    if (e.tall)
-      gram_walk<BF, 2, true, false>(e, x, ra, rb, k0, k1, 32, lane, acc);
+    // registers of sums leave room for more waves, and for the elements under way.  Of
+    // a block on the diagonal, two waves take its two ends (three tiles each) and two
+    // the rest, so that no SIMD has four tiles while another has none.
+    if (I != J)
+      gram_tiles<BF, 2, 2, false>(e, x, I * 64, J * 64, wave >> 1 << 1, (wave & 1) << 1, k0, k1, lane,
+                                  to);
+    else if (wave < 2)
+      gram_tiles<BF, 2, 2, true>(e, x, I * 64, I * 64, 2 * wave, 2 * wave, k0, k1, lane, to);
     else
-      gram_walk<BF, 2, false, false>(e, x, ra, rb, k0, k1, 32, lane, acc);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          to[((2 * wi + i) * 4 + 2 * wj + j) * 256 + v * 64 + lane] = acc[i][j][v];
+      gram_tiles<BF, 1, 2, false>(e, x, I * 64, I * 64, wave - 2, 2, k0, k1, lane, to);
   } else {
     d4 acc[T][T] = {};
     if (e.tall)
-      gram_walk<BF, T, true, true>(e, x, 0, 0, k0 + 32 * wave, k1, 128, lane, acc);
+      gram_walk<BF, T, T, true, true>(e, x, 0, 0, k0 + 32 * wave, k1, 128, lane, acc);
     else
-      gram_walk<BF, T, false, true>(e, x, 0, 0, k0 + 32 * wave, k1, 128, lane, acc);
+      gram_walk<BF, T, T, false, true>(e, x, 0, 0, k0 + 32 * wave, k1, 128, lane, acc);
     // the waves' sums in their order, so that the result does not depend on the time
     for (int o = 0; o < NTH / 64; ++o) {
       if (wave == o) {
@@ -347,7 +366,7 @@ __global__ __launch_bounds__(64) void poly16(const Table* __restrict__ table, co
   for (int v = 0; v < 4; ++v) poly[e.poly + (int64_t)mat * 256 + v * 64 + lane] = P[v];
 }
 
-// ---------------------------------------------------------------- P, r <= 64
+// ---------------------------------------------------------------- P, r <= 32
 // One workgroup of four waves a matrix, everything in LDS; T tiles of 16 rows, tile
 // (w, j) the work of wave (w T + j) % 4.
 template <int T>
@@ -448,9 +467,9 @@ __global__ __launch_bounds__(NTH) void poly_small(const Table* __restrict__ tabl
   for (int i = threadIdx.x; i < N; i += NTH) poly[e.poly + (int64_t)mat * N + i] = P[i];
 }
 
-// ---------------------------------------------------------------- P, larger r
-// The same in tiles of 32 x 32, a workgroup each, over matrices of R = 64 nb in
-// scratch: G, Q, P (two, in turn) and H = Q G, one behind the other.
+// ---------------------------------------------------------------- P, r > 32
+// Matrices of R = 64 nb in scratch, one behind the other: G, Q (or the other G), P (two,
+// in turn) and H = Q G.
 enum { SLOT_G, SLOT_Q, SLOT_P0, SLOT_P1, SLOT_H, SLOTS };
 
 // The chunks' sums joined into the first chunk's place.
@@ -477,7 +496,7 @@ __global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table
   __shared__ double red[NTH / 64];
   const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, IN_POLY, blockIdx.x, w);
+  const Entry& e = find(tab, IN_NORM, blockIdx.x, w);
   const int nb = (e.r + 63) / 64, R = 64 * nb;
   const uint32_t per = (uint32_t)R * R / 1024;
   const double* mine = part + e.part + (int64_t)(w / per) * e.chunks * (nb * (nb + 1) / 2) * 4096;
@@ -497,6 +516,86 @@ __global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table
   }
 }
 
+// Short sides of 64 and 128: a step is one launch.  A workgroup holds all of G in LDS
+// and forms 16 rows of the next G and P by themselves,
+//   H = aG + b GG + c GGG,  G' = aH + b HG + c HGG,  P' = aP + b PG + c PGG,
+// each product those rows times G.  That is six products of 16 rows in the place of
+// four of all, but nothing waits for another workgroup within a step: 25 us at 28
+// matrices of 128 (10 us of products, the rest G's way into LDS and the barriers) where
+// the three launches of the tiles below took 33.  (G' as one polynomial of G, whose
+// coefficients reach 37, lost two more digits.)
+// Wave j forms columns 16 j..; the rows that are multiplied next stand transposed in
+// LDS, rows of 17 doubles.  G' is written from its upper half to both places.
+template <int R>
+__global__ __launch_bounds__(4 * R) void poly_panel(const Table* __restrict__ table, int turn,
+                                                    int more, double* __restrict__ poly) {
+  __shared__ double G[R * R];
+  __shared__ double T[R * 17];
+  const Table& tab = *table;
+  uint32_t w;
+  const Entry& e = find(tab, IN_POLY, blockIdx.x, w);
+  const int I = (int)(w % (R / 16));
+  double* base = poly + e.poly + (int64_t)(w / (R / 16)) * SLOTS * R * R;
+  const double* Gold = base + (int64_t)(turn ? SLOT_Q : SLOT_G) * R * R;
+  double* Gnew = base + (int64_t)(turn ? SLOT_G : SLOT_Q) * R * R;
+  const double* Pold = base + (int64_t)(turn ? SLOT_P1 : SLOT_P0) * R * R;
+  double* Pnew = base + (int64_t)(turn ? SLOT_P0 : SLOT_P1) * R * R;
+  const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+  const int j = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  d2 in[R / 8];
+#pragma unroll
+  for (int i = 0; i < R / 8; ++i) in[i] = ((const d2*)Gold)[threadIdx.x + 4 * R * i];
+  for (int i = threadIdx.x; i < 16 * R; i += 4 * R)
+    T[i / 16 * 17 + i % 16] = Pold[(int64_t)(i / 16) * R + 16 * I + i % 16];  // P symmetric
+#pragma unroll
+  for (int i = 0; i < R / 8; ++i) ((d2*)G)[threadIdx.x + 4 * R * i] = in[i];
+  double p[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) p[v] = Pold[(int64_t)(16 * I + 4 * v + q) * R + 16 * j + m];
+  __syncthreads();
+  auto times = [&](const double* A, int ld) {  // the rows A[k][i] times G's columns 16 j..
+    d4 x = {0.0, 0.0, 0.0, 0.0}, y = x;
+#pragma unroll 8
+    for (int k = 0; k < R; k += 8) {
+      x = __builtin_amdgcn_mfma_f64_16x16x4f64(A[(k + q) * ld + m], G[(k + q) * R + 16 * j + m], x, 0,
+                                               0, 0);
+      y = __builtin_amdgcn_mfma_f64_16x16x4f64(A[(k + 4 + q) * ld + m],
+                                               G[(k + 4 + q) * R + 16 * j + m], y, 0, 0, 0);
+    }
+    return x + y;
+  };
+  auto next = [&](d4 x) {  // x times G
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 4; ++v) T[(16 * j + m) * 17 + 4 * v + q] = x[v];
+    __syncthreads();
+    return times(T, 17);
+  };
+  const double ca = tab.a, cb = tab.b, cc = tab.c;
+  const d4 z1 = times(T, 17);
+  d4 y = z1;
+  if (more) y = times(G + 16 * I, R);  // G symmetric
+  const d4 z2 = next(z1);
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    Pnew[(int64_t)(16 * I + 4 * v + q) * R + 16 * j + m] = ca * p[v] + cb * z1[v] + cc * z2[v];
+  if (!more) return;
+  d4 h;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) h[v] = ca * G[(16 * I + 4 * v + q) * R + 16 * j + m];
+  h += y * cb;
+  h += next(y) * cc;
+  y = next(h);
+  const d4 g = h * ca + y * cb + next(y) * cc;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const int row = 16 * I + 4 * v + q, col = 16 * j + m;
+    if (row <= col)
+      Gnew[(int64_t)row * R + col] = Gnew[(int64_t)col * R + row] = g[v];
+  }
+}
+
+// Short sides beyond 128, in tiles of 32 x 32 and three launches a step.
 // mode 0: Q = aI + bG + cGG;  mode 1: P' = Q P and (blockIdx.y = 1) H = Q G;
 // mode 2: G = H Q, its upper half in both places.
 __global__ __launch_bounds__(NTH) void poly_step(const Table* __restrict__ table, int mode, int turn,
@@ -710,6 +809,20 @@ __device__ __forceinline__ void apply64_walk(const Entry& e, const void* x, void
                                              const double* P, double* Pall, int nb, int I,
                                              int64_t l0, int64_t l1, int wave, int m, int q) {
   const int R = 64 * nb, wi = wave & 1, wl = wave >> 1;
+  auto fill = [&](double* Ps, int kb) {
+    d2 in[8];
+    const d2* from = (const d2*)(P + (int64_t)(kb * 64 + threadIdx.x / 32) * R + I * 64) +
+                     threadIdx.x % 32;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) in[i] = from[(int64_t)i * 4 * R];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ((d2*)Ps)[threadIdx.x + 256 * i] = in[i];
+  };
+  if (nb <= 2) {
+    fill(Pall, 0);
+    if (nb == 2) fill(Pall + 4096, 1);
+    __syncthreads();
+  }
   for (int64_t step = l0; step < l1; step += 128) {
     const int64_t k0 = step + 64 * wl;  // a wave past the end loads nothing and stores nothing
     const bool fast = e.vec && k0 + 64 <= l1;
@@ -718,10 +831,9 @@ __device__ __forceinline__ void apply64_walk(const Entry& e, const void* x, void
     if (fast) apply_rows<BF, TALL, true>(e, x, 0, k0, l1, m, q, next);
     for (int kb = 0; kb < nb; ++kb) {
       double* Ps = Pall + (nb <= 2 ? kb : 0) * 4096;
-      if (nb > 2 || step == l0) {
+      if (nb > 2) {
         __syncthreads();
-        for (int i = 2 * threadIdx.x; i < 4096; i += 2 * NTH)
-          *(d2*)(Ps + i) = *(const d2*)(P + (int64_t)(kb * 64 + i / 64) * R + I * 64 + i % 64);
+        fill(Ps, kb);
         __syncthreads();
       }
       if (fast) {
@@ -764,7 +876,7 @@ __global__ __launch_bounds__(NTH) void apply64(const Table* __restrict__ table, 
   const void* x = (const char*)e.x + off;
   void* out = (char*)e.out + off;
   const double* P = poly + e.poly;
-  P += nb == 1 ? mat * R * R : (mat * SLOTS + (last ? SLOT_P1 : SLOT_P0)) * R * R;
+  P += (mat * SLOTS + (last ? SLOT_P1 : SLOT_P0)) * R * R;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (e.tall)
@@ -781,49 +893,68 @@ struct Plan {  // one table's launches
   int64_t part = 0, poly = 0;  // doubles
 };
 
-int tiles_of(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
+// Equal pieces of at most about `most` of a long side, in whole units.
+int64_t piece(int64_t K, int64_t most, int64_t unit) {
+  return st::cdiv(st::cdiv(K, st::cdiv(K, most)), unit) * unit;
+}
+// Long elements of a workgroup: the length whose rounds of `slots` workgroups at a time
+// take least, each as long as its longest piece and `start` elements more.  (28 factors
+// of rank 128: 648 workgroups of 512 elements on 512 places wait for a second round and
+// take 134 us, 460 of 768 take 122.)
+template <typename F>
+int64_t pick(const Plan& p, int64_t unit, int64_t slots, int64_t start, F blocks) {
+  int64_t best = unit, least = INT64_MAX;
+  for (const int k : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24}) {
+    int64_t n = 0, longest = 0;
+    for (int i = 0; i < p.tab.n; ++i) {
+      const int64_t K = p.tab.e[i].K, l = piece(K, k * unit, unit);
+      n += p.count[i] * blocks(p.tab.e[i]) * st::cdiv(K, l);
+      longest = l > longest ? l : longest;
+    }
+    const int64_t cost = st::cdiv(n, slots) * (longest + start);
+    if (cost < least) least = cost, best = k * unit;
+    if (n <= slots) break;  // one round: longer ones only take longer
+  }
+  return best;
+}
 
-// The next table: entries from `at` on whose short sides take tiles of one size and
-// are either all within one block or all beyond it.  Returns the entries taken.
+// The next table: entries from `at` on whose short sides are of one class (up to 16, 32,
+// 64, 128, more).  Returns the entries taken.
 int make_plan(const st_matrix_batch* in, int32_t n, int32_t at, int32_t dtype, Plan& p) {
   p = Plan();
   Table& t = p.tab;
-  int64_t total = 0;
   int taken = 0;
-  bool large = false, first = true;
+  int kind = 0;
   t.n = 0;
   for (; at + taken < n && t.n < MAXE; ++taken) {
     const st_matrix_batch& b = in[at + taken];
     if (b.count == 0 || b.rows == 0 || b.cols == 0) continue;
     const int64_t r = b.rows < b.cols ? b.rows : b.cols, K = b.rows < b.cols ? b.cols : b.rows;
-    if (first) p.T = tiles_of(r), large = r > 64, first = false;
-    if (tiles_of(r) != p.T || (r > 64) != large) break;
+    const int mine = r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 3 : r <= 128 ? 4 : 5;
+    if (!kind) kind = mine, p.T = kind < 3 ? kind : 4;
+    if (mine != kind) break;
     Entry& e = t.e[t.n];
     e.x = b.x, e.out = b.out;
     e.K = (int32_t)K, e.r = (int32_t)r, e.tall = b.rows > b.cols;
     const uintptr_t mask = dtype == ST_DTYPE_BF16 ? 7 : 15;
     e.vec = (e.tall ? r : K) % 4 == 0 && (((uintptr_t)b.x | (uintptr_t)b.out) & mask) == 0;
     p.count[t.n++] = b.count;
-    const int64_t nb = p.T < 4 ? 1 : st::cdiv(r, 64);
-    total += b.count * K * (nb * (nb + 1) / 2);
   }
-  // Long elements of a workgroup: about 1024 workgroups where there is that much
-  // work (all of them run at once then), never less than two rounds of its waves.
-  int64_t ch = st::cdiv(total, 1024);  // total: over the block pairs of gram
-  if (ch < 256) ch = 256;
-  if (ch > 4096) ch = 4096;
-  auto share = [&](int64_t K, int64_t unit) {  // of equal pieces of at most about ch
-    return st::cdiv(st::cdiv(K, st::cdiv(K, ch)), unit) * unit;
-  };
+  auto nb = [&](const Entry& e) { return ((int64_t)e.r + 16 * p.T - 1) / (16 * p.T); };
+  auto pairs = [&](const Entry& e) { return nb(e) * (nb(e) + 1) / 2; };
+  // places: 256 CUs and as many workgroups each as the kernels' registers and LDS allow
+  const int64_t ch = p.T == 4 ? pick(p, 128, 768, 192, pairs)
+                              : pick(p, 128, p.T == 1 ? 2048 : 1280, 256, pairs);
+  const int64_t al = p.T == 4 ? pick(p, 128, 512, 64, nb)
+                              : pick(p, 256, p.T == 1 ? 1280 : 512, 256, nb);
   for (int i = 0; i < t.n; ++i) {
     Entry& e = t.e[i];
-    const int64_t nb = (e.r + 16 * p.T - 1) / (16 * p.T);
-    e.CH = (int32_t)share(e.K, 128), e.AL = (int32_t)share(e.K, p.T == 4 ? 128 : 256);
+    e.CH = (int32_t)piece(e.K, ch, 128), e.AL = (int32_t)piece(e.K, al, p.T == 4 ? 128 : 256);
     e.chunks = (int32_t)st::cdiv(e.K, e.CH);
     e.part = p.part, e.poly = p.poly;
-    p.part += p.count[i] * e.chunks * (nb * (nb + 1) / 2) * p.T * p.T * 256;
-    const int64_t R = 16 * p.T * nb;
-    p.poly += p.count[i] * R * R * (nb > 1 ? SLOTS : 1);
+    p.part += p.count[i] * e.chunks * pairs(e) * p.T * p.T * 256;
+    const int64_t R = 16 * p.T * nb(e);
+    p.poly += p.count[i] * R * R * (p.T == 4 ? SLOTS : 1);
   }
   return taken;
 }
@@ -846,40 +977,46 @@ constexpr int64_t TABLE_BYTES = (sizeof(Table) + 15) / 16 * 16;
 template <int T, bool BF>
 int launch(Plan& p, char* workspace, hipStream_t stream) {
   auto blocks = [](const Entry& e) { return T < 4 ? (int64_t)1 : ((int64_t)e.r + 63) / 64; };
-  const bool large = T == 4 && p.tab.e[0].r > 64;
+  const int nb = (int)blocks(p.tab.e[0]);  // 1, 2 or more for all entries
   const int64_t ng = number(p, IN_GRAM, [&](const Entry& e) {
     return e.chunks * blocks(e) * (blocks(e) + 1) / 2;
   });
   const int64_t ns = number(p, IN_SUM, [&](const Entry& e) {
     return blocks(e) * (blocks(e) + 1) / 2 * 8;
   });
+  const int64_t nn = number(p, IN_NORM, [&](const Entry& e) { return blocks(e) * blocks(e) * 4; });
   const int64_t np = number(p, IN_POLY, [&](const Entry& e) {
-    return large ? blocks(e) * blocks(e) * 4 : (int64_t)1;
+    return T < 4 ? (int64_t)1 : nb <= 2 ? (int64_t)4 * nb : blocks(e) * blocks(e) * 4;
   });
   const int64_t na = number(p, IN_APPLY, [&](const Entry& e) {
     return st::cdiv(e.K, e.AL) * blocks(e);
   });
-  if (ng < 0 || ns < 0 || np < 0 || na < 0)
+  if (ng < 0 || ns < 0 || nn < 0 || np < 0 || na < 0)
     return st::fail(ST_EUNSUPPORTED, "too many matrices for a launch: call with fewer at a time");
   const Table* tab = (const Table*)workspace;
   double* part = (double*)(workspace + TABLE_BYTES);
   double* poly = part + p.part;
   gram<T, BF><<<(unsigned)ng, NTH, 0, stream>>>(p.tab, part, (uint32_t*)workspace);
   int turn = 0;
-  if (large) {
-    poly_sum<<<(unsigned)ns, NTH, 0, stream>>>(tab, part);
-    poly_norm<<<(unsigned)np, NTH, 0, stream>>>(tab, part, poly);
-    for (int s = 0; s < p.tab.steps; ++s) {
-      const bool more = s + 1 < p.tab.steps;
-      poly_step<<<(unsigned)np, NTH, 0, stream>>>(tab, 0, turn, poly);
-      poly_step<<<dim3((unsigned)np, more ? 2 : 1), NTH, 0, stream>>>(tab, 1, turn, poly);
-      if (more) poly_step<<<(unsigned)np, NTH, 0, stream>>>(tab, 2, turn, poly);
-      turn ^= 1;
-    }
-  } else if constexpr (T == 1) {
+  if constexpr (T == 1) {
     poly16<<<(unsigned)np, 64, 0, stream>>>(tab, part, poly);
-  } else {
+  } else if constexpr (T == 2) {
     poly_small<T><<<(unsigned)np, NTH, 0, stream>>>(tab, part, poly);
+  } else {
+    poly_sum<<<(unsigned)ns, NTH, 0, stream>>>(tab, part);
+    poly_norm<<<(unsigned)nn, NTH, 0, stream>>>(tab, part, poly);
+    for (int s = 0; s < p.tab.steps; ++s, turn ^= 1) {
+      const int more = s + 1 < p.tab.steps;
+      if (nb == 1) {
+        poly_panel<64><<<(unsigned)np, 256, 0, stream>>>(tab, turn, more, poly);
+      } else if (nb == 2) {
+        poly_panel<128><<<(unsigned)np, 512, 0, stream>>>(tab, turn, more, poly);
+      } else {
+        poly_step<<<(unsigned)np, NTH, 0, stream>>>(tab, 0, turn, poly);
+        poly_step<<<dim3((unsigned)np, more ? 2 : 1), NTH, 0, stream>>>(tab, 1, turn, poly);
+        if (more) poly_step<<<(unsigned)np, NTH, 0, stream>>>(tab, 2, turn, poly);
+      }
+    }
   }
   if constexpr (T == 4)
     apply64<BF><<<(unsigned)na, NTH, 0, stream>>>(tab, turn, poly);

@@ -47,19 +47,16 @@ def orthogonalize(matrices, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     a, b, c = (float(v) for v in coefficients)
     if isinstance(steps, bool) or not isinstance(steps, int):
         raise ValueError("unsupported_capability: steps must be an integer")
-    table = (_lib.MatrixBatch * len(given))()
-    keep, out = [], []
-    for entry, x in zip(table, given):
-        x = x.contiguous()
-        y = torch.empty_like(x)
-        rows, cols = x.shape[-2:]
-        entry.x, entry.out = x.data_ptr(), y.data_ptr()
-        entry.rows, entry.cols = rows, cols
-        entry.count = x.numel() // (rows * cols) if rows and cols else 0
-        keep.append(x)
-        out.append(y)
     if device.type != "cuda":
         raise ValueError("unsupported_capability: orthogonalize runs on the GPU")
+    given = [x.contiguous() for x in given]
+    out = [torch.empty_like(x) for x in given]
+    numbers = []  # st_matrix_batch: five 64-bit words each
+    for x, y in zip(given, out):
+        rows, cols = x.shape[-2:]
+        numbers += (x.data_ptr(), y.data_ptr(), x.numel() // (rows * cols) if rows and cols else 0,
+                    rows, cols)
+    table = _lib.i64_array(numbers)
     with _lib.on_device(device):
         nbytes = _lib.query("st_orthogonalize_workspace_bytes", len(given), table)
         ws = _scratch(device, nbytes)
