@@ -449,34 +449,85 @@ __global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
   const uint32_t V = (uint32_t)a.V;
   // entries from the first one that takes no part on are behind the end
   const int count = __popcll(__ballot(here && lane >= 1 && lane <= many && tok < V));
-  const int64_t i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  if (!count || i >= a.H) return;  // no barriers below
+  if (!count) return;  // the same for the whole wave
+  // lanes past the columns stay, since the others read their tokens: they add the row's
+  // first columns and write nothing
+  const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  const bool in = col < a.H;
+  const int64_t i = in ? col : 0;
   auto token = [&](int e) { return __builtin_amdgcn_readlane(tok, e + 1); };  // -1..many
   auto row = [&](int e) {
     return a.dout + (int64_t)__builtin_amdgcn_readlane(pos, e + 1) * a.H + i;
   };
   bool from = token(-1) == token(0);  // the run began in an earlier chunk
   float acc[VEC] = {};
-  for (int e0 = 0; e0 < count; e0 += AHEAD) {
+  for (int b = 0; b < count; b += AHEAD) {
     Raw<VEC> now[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) read_row<VEC>(row(e0 + k < count ? e0 + k : e0), now[k]);
+    for (int k = 0; k < AHEAD; ++k) read_row<VEC>(row(b + k < count ? b + k : b), now[k]);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int e = e0 + k;
+      const int e = b + k;
       if (e >= count) break;
       add_row<VEC>(now[k], acc);
       const bool end = token(e + 1) != token(e);
       if (!end && e + 1 < many) continue;
-      if (from)
-        store_f<VEC>(a.partial + c * 2 * a.H + i, acc);
-      else if (!end)
-        store_f<VEC>(a.partial + (c * 2 + 1) * a.H + i, acc);
-      else
-        write_row<VEC>(a, token(e), i, acc);
+      const uint32_t whose = token(e);
+      if (in) {
+        if (from)
+          store_f<VEC>(a.partial + c * 2 * a.H + i, acc);
+        else if (!end)
+          store_f<VEC>(a.partial + (c * 2 + 1) * a.H + i, acc);
+        else
+          write_row<VEC>(a, whose, i, acc);
+      }
       from = false;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+    }
+  }
+}
+
+// The same for few tokens, without partial sums and the launch that joins them: a
+// workgroup sums the runs that begin in its chunk to their ends, wherever these are
+// (at most WHOLE entries, 64 rounds of loads).
+constexpr int64_t WHOLE = 512;
+template <int VEC>
+__global__ __launch_bounds__(NTH) void sum_whole(Sums a) {
+  const int lane = threadIdx.x & 63;
+  const int n = (int)a.n, e0 = (int)(blockIdx.x * a.chunk), stop = e0 + (int)a.chunk;
+  const uint32_t V = (uint32_t)a.V;
+  // lanes past the columns stay, as in sum_runs: every lane holds a token
+  const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  const bool in = col < a.H;
+  const int64_t i = in ? col : 0;
+  bool open = false;  // within a run of this workgroup's
+  float acc[VEC] = {};
+  for (int w = e0;; w += 56) {  // lane l: entry w - 1 + l, up to the one behind w + 56
+    const int mine = w - 1 + lane;
+    const bool here = mine >= 0 && mine < n;
+    const uint32_t tok = here ? a.tok[mine] : ~0u, pos = here ? a.pos[mine] : 0;
+    for (int b = 0; b < 56; b += AHEAD) {
+      Raw<VEC> now[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        read_row<VEC>(a.dout + (int64_t)__builtin_amdgcn_readlane(pos, b + k + 1) * a.H + i, now[k]);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int e = w + b + k;
+        const uint32_t token = __builtin_amdgcn_readlane(tok, b + k + 1);
+        if (!open) {
+          if (e >= stop || token >= V) return;  // (~0 behind the last entry)
+          if (__builtin_amdgcn_readlane(tok, b + k) == token) continue;  // begun before e0
+          open = true;
+        }
+        add_row<VEC>(now[k], acc);
+        if (__builtin_amdgcn_readlane(tok, b + k + 2) == token) continue;
+        if (in) write_row<VEC>(a, token, i, acc);
+        open = false;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+      }
     }
   }
 }
@@ -661,15 +712,19 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
   if (chunks * slices * th >= (int64_t)1 << 32 || slices >= 65536)
     return st::fail(ST_EUNSUPPORTED, "st_embedding_bwd: more threads than a launch takes");
   const dim3 grid((unsigned)chunks, (unsigned)slices), more((unsigned)chunks - 1, (unsigned)slices);
-  if (vec == 4) {
-    sum_runs<4><<<grid, th, 0, s>>>(a);
-    if (chunks > 1) join_runs<4><<<more, th, 0, s>>>(a);
-  } else if (vec == 8) {
-    sum_runs<8><<<grid, th, 0, s>>>(a);
-    if (chunks > 1) join_runs<8><<<more, th, 0, s>>>(a);
-  } else {
-    sum_runs<1><<<grid, th, 0, s>>>(a);
-    if (chunks > 1) join_runs<1><<<more, th, 0, s>>>(a);
-  }
+  auto sums = [&](auto whole, auto runs, auto join) {
+    if (n <= WHOLE) {
+      whole<<<grid, th, 0, s>>>(a);
+    } else {
+      runs<<<grid, th, 0, s>>>(a);
+      if (chunks > 1) join<<<more, th, 0, s>>>(a);
+    }
+  };
+  if (vec == 4)
+    sums(sum_whole<4>, sum_runs<4>, join_runs<4>);
+  else if (vec == 8)
+    sums(sum_whole<8>, sum_runs<8>, join_runs<8>);
+  else
+    sums(sum_whole<1>, sum_runs<1>, join_runs<1>);
   return st::check_launch("st_embedding_bwd");
 }

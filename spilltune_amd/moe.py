@@ -164,14 +164,15 @@ class _BalanceLoss(torch.autograd.Function):
         per, dev = logits.numel() // E // groups, logits.device
         loss = torch.empty((), dtype=_F32, device=dev)
         counts = torch.empty((groups, E), dtype=torch.int64, device=dev)
-        tokens = torch.empty(groups + 1, dtype=_I32, device=dev)
         dtype = _lib.ST_DTYPE_F32 if logits.dtype == _F32 else _lib.ST_DTYPE_BF16
         with _lib.on_device(dev):
             nbytes = _lib.query("st_balance_workspace_bytes", groups, per, E)
-            ws = _scratch(dev, nbytes)
+            # the groups' valid tokens, which the backward reads, and the call's scratch
+            tokens = torch.empty(4 * (groups + 1) + nbytes, dtype=torch.uint8, device=dev)
             _lib.call("st_balance_fwd", logits.data_ptr(), dtype, indices.data_ptr(),
                       _lib.ptr(valid), groups, per, E, k, sigmoid, loss.data_ptr(),
-                      counts.data_ptr(), tokens.data_ptr(), _lib.ptr(ws), nbytes, _stream(dev))
+                      counts.data_ptr(), tokens.data_ptr(), tokens.data_ptr() + 4 * (groups + 1),
+                      nbytes, _stream(dev))
         ctx.save_for_backward(logits, valid, counts, tokens)
         ctx.meta = (groups, per, k, sigmoid, dtype)
         ctx.mark_non_differentiable(counts)

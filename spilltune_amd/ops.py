@@ -672,29 +672,29 @@ def rms_norm_residual(x: torch.Tensor, weight: torch.Tensor, eps: float):
 
 # ----------------------------------------------------------------- norms around a part
 def _residual_norms(y, residual, post, pre, gate, mode, rows_per, scale, eps, keep):
-    """(h, normed, rstd_post, rstd_pre), None where there is none."""
+    """(h, normed or None, both norms' statistics [2, rows] for a backward or None)."""
     H, dev = y.shape[-1], y.device
     rows = y.numel() // H
     h = torch.empty_like(y)
     normed = None if pre is None else torch.empty_like(y)
     if not rows:
-        return h, normed, None, None
-    r1 = torch.empty(rows, dtype=_F32, device=dev) if keep and post is not None else None
-    r2 = torch.empty(rows, dtype=_F32, device=dev) if keep and pre is not None else None
+        return h, normed, None
+    stats = torch.empty((2, rows), dtype=_F32, device=dev) if keep else None
+    r1, r2 = (None, None) if stats is None else (stats.data_ptr(), stats.data_ptr() + 4 * rows)
     with _lib.on_device(dev):
         _lib.call("st_residual_norms_fwd", y.data_ptr(), residual.data_ptr(), _lib.ptr(post),
                   _lib.ptr(pre), _lib.ptr(gate), mode, int(gate is not None and gate.dtype == _F32),
-                  rows_per, rows, H, scale, eps, h.data_ptr(), _lib.ptr(normed), _lib.ptr(r1),
-                  _lib.ptr(r2), _lib.stream_handle(dev))
-    return h, normed, r1, r2
+                  rows_per, rows, H, scale, eps, h.data_ptr(), _lib.ptr(normed), r1, r2,
+                  _lib.stream_handle(dev))
+    return h, normed, stats
 
 
 class _ResidualNorms(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, residual, post, pre, gate, mode, rows_per, scale, eps):
-        h, normed, r1, r2 = _residual_norms(y, residual, post, pre, gate, mode, rows_per, scale, eps,
-                                            True)
-        ctx.save_for_backward(y, residual, post, pre, gate, r1, r2)
+        h, normed, stats = _residual_norms(y, residual, post, pre, gate, mode, rows_per, scale, eps,
+                                           True)
+        ctx.save_for_backward(y, residual, post, pre, gate, stats)
         ctx.meta = (mode, rows_per, scale, eps)
         ctx.set_materialize_grads(False)
         return h if normed is None else (h, normed)
@@ -704,7 +704,7 @@ class _ResidualNorms(torch.autograd.Function):
         _once()
         if dh is None and dn is None:
             return (None,) * 9
-        y, residual, post, pre, gate, r1, r2 = ctx.saved_tensors
+        y, residual, post, pre, gate, stats = ctx.saved_tensors
         mode, rows_per, scale, eps = ctx.meta
         H, dev = y.shape[-1], y.device
         rows = y.numel() // H
@@ -727,7 +727,8 @@ class _ResidualNorms(torch.autograd.Function):
             _lib.call("st_residual_norms_bwd", y.data_ptr(), residual.data_ptr(), _lib.ptr(post),
                       _lib.ptr(pre), _lib.ptr(gate), mode,
                       int(gate is not None and gate.dtype == _F32), rows_per, rows, H, scale, eps,
-                      _lib.ptr(r1), _lib.ptr(r2), _lib.ptr(dh), _lib.ptr(dn), _lib.ptr(dy),
+                      stats.data_ptr(), stats.data_ptr() + 4 * rows, _lib.ptr(dh), _lib.ptr(dn),
+                      _lib.ptr(dy),
                       _lib.ptr(dres), _lib.ptr(dgate), _lib.ptr(dpost), _lib.ptr(dpre),
                       _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
         return dy, dres, dpost, dpre, dgate, None, None, None, None
@@ -795,7 +796,7 @@ def residual_norms(y, residual, post=None, pre=None, *, gate=None, scale=1.0, ep
     args = (*(None if t is None else _operand(t) for t in given), mode, rows_per, scale, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
         return _ResidualNorms.apply(*args)
-    h, normed, _, _ = _residual_norms(*args, False)
+    h, normed, _ = _residual_norms(*args, False)
     return h if normed is None else (h, normed)
 
 
