@@ -311,3 +311,36 @@ def test_embedding_on_the_models_device():
         engine.DenseModel(embedding=e, norm=torch.zeros(16), head=torch.zeros(8, 16), blocks=[],
                           heads=2, kv_heads=1, head_dim=8, eps=1e-6, theta=1e4, rank=1, alpha=1.0,
                           targets=(), device="cpu")
+
+
+def test_balance_through_a_deepseek_block():
+    """The block hands its router's term on: other input gradients, the same output, and
+    the padded tokens' picks left out."""
+    from spilltune_amd import deepseek
+    from tests import test_gpu_mla as TM
+    dev = torch.device("cuda:0")
+    c = TM._params(heads=4, nope=128, rope=64, vdim=128, kv_rank=128, q_rank=None, interleave=False,
+                   moe=True, rope_cfg=TM.DEFAULT)
+    g = torch.Generator().manual_seed(31)
+    w = TM._layer_weights(g, c, 256, 128, 256, 16)
+    valid = torch.arange(40) < torch.tensor([[40], [23]])
+    hidden, dy = (torch.randn(2, 40, 256, generator=g).to(BF) for _ in range(2))
+    dy[~valid] = 0
+    res = []
+    for coefficient in (None, 5.0):
+        balance = None if coefficient is None else moe.ExpertBalance(coefficient)
+        block = deepseek.make_deepseek_block(0, w, codec="nf4-g128", parameters=dict(c, balance=balance),
+                                             rank=4, alpha=8.0, device=dev,
+                                             generator=torch.Generator().manual_seed(1))
+        rot, mask = deepseek.positions_and_masks(valid, rope=c["rope_cfg"], rope_dim=c["rope"],
+                                                 device=dev)
+        session = slots.ResidentSession([block], dev)
+        x = hidden.to(dev).requires_grad_(True)
+        with session.run():
+            out = streaming_block(x, rot, mask, block.functional, block.kwargs,
+                                  session.reloader(block), block.adapters, 0)
+            out.backward(dy.to(dev))
+        session.close()
+        res.append((out.detach(), x.grad))
+    assert torch.equal(res[0][0], res[1][0]) and not torch.equal(res[0][1], res[1][1])
+    assert balance.passes == 1 and int(balance.counts.sum()) == int(valid.sum()) * c["top_k"]

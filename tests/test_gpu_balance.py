@@ -184,6 +184,28 @@ def test_layouts_streams_and_graphs():
         assert torch.equal(loss, eager[0]) and torch.equal(counts, eager[1]) and torch.equal(g, eager[2])
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 logits: the last row's gradient as by itself (each row its own)."""
+    B, S, E = 3, 1400000, 512
+    x = torch.zeros(B, S, E, dtype=BF, device="cuda")
+    i = torch.zeros(B, S, 1, dtype=torch.int32, device="cuda")
+    x[-1, -2000:] = torch.randn(2000, E, device="cuda", generator=torch.Generator("cuda").manual_seed(1)
+                                ).to(BF)
+    i[-1, -2000:, 0] = torch.arange(2000, device="cuda", dtype=torch.int32) % E
+    valid = torch.zeros(B, S, dtype=torch.bool, device="cuda")
+    valid[-1, -2000:] = True
+    x.requires_grad_(True)
+    loss, counts = moe.balance_loss(x, i, valid=valid, per_row=True)
+    (g,) = torch.autograd.grad(loss, [x])
+    assert int(counts[-1].sum()) == 2000 and int(counts[:2].sum()) == 0
+    few = x.detach()[-1:, -2000:].clone()
+    want, _, _ = check(few, i[-1:, -2000:], dloss=1.0)
+    assert abs(float(loss.detach()) - float(want.detach())) < 1e-4
+    check_few = few.clone().requires_grad_(True)
+    (fg,) = torch.autograd.grad(moe.balance_loss(check_few, i[-1:, -2000:]).loss, [check_few])
+    assert torch.equal(g[-1, -2000:], fg[0]) and (g[0, :9] == 0).all() and (g[-1, :9] == 0).all()
+
+
 def test_refused_derivatives():
     x, i = make(1, 4, 8, 2, F32)
     leaf = x.requires_grad_(True)

@@ -125,6 +125,15 @@ def test_layouts():
     check(muon.orthogonalize(b), b)
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in one batch: the last matrices as by themselves."""
+    u = torch.zeros(2100, 16, 65536, device="cuda")
+    u[-2:] = make((2, 16, 65536), 4)
+    out = muon.orthogonalize(u)
+    check(out[-2:], u[-2:])
+    assert (out[:2] == 0).all() and (out[1024:1026] == 0).all()
+
+
 def test_streams_and_graphs():
     us = [make((16, 4096), 1), make((4096, 16), 2), make((100, 333), 3)]
     ref = muon.orthogonalize(us)

@@ -261,3 +261,21 @@ def test_refused_derivatives():
         dual = forward_ad.make_dual(t["y"].detach(), up[0])
         with pytest.raises(NotImplementedError):
             ops.residual_norms(dual, t["residual"])
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 entries: the last rows as by themselves."""
+    rows, H = 131100, 16384
+    y = torch.zeros(rows, H, dtype=BF, device="cuda")
+    res = torch.zeros_like(y)
+    g = torch.Generator("cuda").manual_seed(1)
+    y[-3:], res[-3:] = (torch.randn(3, H, generator=g, device="cuda").to(BF) for _ in range(2))
+    w = torch.ones(H, dtype=BF, device="cuda")
+    y.requires_grad_(True)
+    h, n = ops.residual_norms(y, res, w, w)
+    (dy,) = torch.autograd.grad([h, n], [y], [h.detach(), n.detach()])
+    few = y.detach()[-3:].clone().requires_grad_(True)
+    fh, fn = ops.residual_norms(few, res[-3:], w, w)
+    (fd,) = torch.autograd.grad([fh, fn], [few], [fh.detach(), fn.detach()])
+    assert torch.equal(h[-3:], fh) and torch.equal(n[-3:], fn) and torch.equal(dy[-3:], fd)
+    assert (h[:5] == 0).all() and (dy[:5] == 0).all() and (h[65536:65541] == 0).all()
