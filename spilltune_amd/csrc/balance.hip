@@ -7,8 +7,9 @@
 //   dp_e = a_e = dL E c_e / (k n^2 groups);  dl_e = p_e (a_e - sum a p)  or
 //          (a_e - sum a p) / (sum sigma + 1e-20) sigma_e (1 - sigma_e)
 //
-// A wave holds a token's logits (up to 512 experts, 8 a lane), so each is read once
-// forward and once backward; picks are counted in LDS (whole numbers: their order
+// A wave holds a token's logits (up to 512 experts, PER = 1, 2, 4 or 8 a lane), so each
+// is read once forward and once backward, the next token's while the present one's are
+// worked on (16384 tokens of 256 experts: 17 MB in 12.5 us forward, 12.2 us backward); picks are counted in LDS (whole numbers: their order
 // does not matter), probabilities summed in fp32 in registers over a workgroup's
 // tokens and joined over the workgroups in their order.
 #include "common.h"
@@ -16,7 +17,7 @@
 namespace {
 
 constexpr int NTH = 256, WAVES = NTH / 64, JOIN = 1024;
-constexpr int MAXE = 512, PER = MAXE / 64;
+constexpr int MAXE = 512;
 constexpr float TINY = 1e-20f;
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -47,20 +48,20 @@ struct Args {
   void* dlogits;
 };
 
-// The scores e of a token and the reciprocal of their sum: p = e * inv; lane + 64 i
-// is the expert.
-template <bool BF>
-__device__ __forceinline__ float scores(const Args& a, int64_t t, int lane, float (&v)[PER]) {
-  float mx = -INFINITY;
+// A token's logits; lane + 64 i is the expert.  Lanes past the experts read the first
+// ones (a load under a branch would be waited for at its end).
+template <bool BF, int PER>
+__device__ __forceinline__ void fetch(const Args& a, int64_t t, int lane, float (&v)[PER]) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = lane + 64 * i;
-    v[i] = -INFINITY;
-    if (e < a.E)
-      v[i] = BF ? st::bf16_to_f32(((const uint16_t*)a.logits)[t * a.E + e])
-                : ((const float*)a.logits)[t * a.E + e];
-    mx = fmaxf(mx, v[i]);
+    const int64_t at = t * a.E + (lane + 64 * i < a.E ? lane + 64 * i : 0);
+    v[i] = BF ? st::bf16_to_f32(((const uint16_t*)a.logits)[at]) : ((const float*)a.logits)[at];
   }
+}
+// The scores e of a token in the place of its logits, and the reciprocal of their sum:
+// p = e * inv.
+template <int PER>
+__device__ __forceinline__ float scores(const Args& a, int lane, float (&v)[PER]) {
   float sum = 0.0f;
   if (a.sigmoid) {
 #pragma unroll
@@ -70,6 +71,9 @@ __device__ __forceinline__ float scores(const Args& a, int64_t t, int lane, floa
     }
     return 1.0f / (wave_sum(sum) + TINY);
   }
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mx = fmaxf(mx, v[i]);
   mx = wave_max(mx);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -79,31 +83,44 @@ __device__ __forceinline__ float scores(const Args& a, int64_t t, int lane, floa
   return 1.0f / wave_sum(sum);
 }
 
-template <bool BF>
+template <bool BF, int PER>
 __global__ __launch_bounds__(NTH) void balance_sums(Args a) {
-  __shared__ float sums[WAVES][MAXE];
-  __shared__ int32_t count[MAXE + 1];
+  __shared__ float sums[WAVES][64 * PER];
+  __shared__ int32_t count[64 * PER + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t g = blockIdx.y, c = blockIdx.x;
-  for (int i = threadIdx.x; i <= MAXE; i += NTH) count[i] = 0;
+  for (int i = threadIdx.x; i <= 64 * PER; i += NTH) count[i] = 0;
   __syncthreads();
-  float p[PER] = {};
+  float p[PER] = {}, next[PER];
   int n = 0;
-  const int64_t z = min((c + 1) * a.chunk, a.per_group);
-  for (int64_t i = c * a.chunk + wave; i < z; i += WAVES) {
-    const int64_t t = g * a.per_group + i;
-    if (a.valid && !a.valid[t]) continue;  // the same for the whole wave
+  const int64_t z = min((c + 1) * a.chunk, a.per_group), t0 = g * a.per_group;
+  int64_t i = c * a.chunk + wave;
+  const int64_t last = a.per_group - 1;
+  // what the next token needs, also where there is none (the last one's then)
+  auto ahead = [&](int64_t k, bool& valid, int& pick) {
+    const int64_t t = t0 + (k < z ? k : last);
+    fetch<BF, PER>(a, t, lane, next);
+    valid = !a.valid || a.valid[t];
+    pick = a.picks[t * a.k + (lane < a.k ? lane : 0)];
+  };
+  bool valid;
+  int pick;
+  ahead(i, valid, pick);
+  for (; i < z; i += WAVES) {
     float v[PER];
-    const float inv = scores<BF>(a, t, lane, v);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = next[j];
+    const bool live = valid;
+    const int e = pick;
+    ahead(i + WAVES, valid, pick);
+    if (!live) continue;  // the same for the whole wave
+    const float inv = scores<PER>(a, lane, v);
 #pragma unroll
     for (int j = 0; j < PER; ++j) p[j] += v[j] * inv;
-    if (lane < a.k) {
-      const int e = a.picks[t * a.k + lane];
-      if (e >= 0 && e < a.E) atomicAdd(&count[e], 1);
-    }
+    if (lane < a.k && e >= 0 && e < a.E) atomicAdd(&count[e], 1);
     ++n;
   }
-  if (lane == 0) atomicAdd(&count[MAXE], n);
+  if (lane == 0) atomicAdd(&count[64 * PER], n);
 #pragma unroll
   for (int j = 0; j < PER; ++j) sums[wave][lane + 64 * j] = p[j];
   __syncthreads();
@@ -116,7 +133,7 @@ __global__ __launch_bounds__(NTH) void balance_sums(Args a) {
     to[e] = s;
     nt[e] = count[e];
   }
-  if (threadIdx.x == 0) nt[a.E] = count[MAXE];
+  if (threadIdx.x == 0) nt[a.E] = count[64 * PER];
 }
 
 // Sums of the chunks of a group, one wave each 64 experts at a time: wave w takes the
@@ -196,10 +213,20 @@ __global__ __launch_bounds__(64) void balance_mean(Args a) {
   }
 }
 
-template <bool BF>
+template <bool BF, int PER>
 __global__ __launch_bounds__(NTH) void balance_bwd(Args a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t g = blockIdx.y, z = min((int64_t)(blockIdx.x + 1) * a.chunk, a.per_group);
+  const int64_t t0 = g * a.per_group, last = a.per_group - 1;
+  int64_t i = blockIdx.x * a.chunk + wave;
+  float next[PER];
+  auto ahead = [&](int64_t k, bool& valid) {
+    const int64_t t = t0 + (k < z ? k : last);
+    fetch<BF, PER>(a, t, lane, next);
+    valid = !a.valid || a.valid[t];
+  };
+  bool valid;
+  ahead(i, valid);
   const float n = (float)a.tokens[g];
   const float each = *a.dloss * (float)a.E / ((float)a.k * n * n * (float)a.tokens[a.groups]);
   float w[PER];
@@ -208,14 +235,15 @@ __global__ __launch_bounds__(NTH) void balance_bwd(Args a) {
     const int e = lane + 64 * j;
     w[j] = e < a.E ? each * (float)a.counts[g * a.E + e] : 0.0f;
   }
-  for (int64_t i = blockIdx.x * a.chunk + wave; i < z; i += WAVES) {
-    const int64_t t = g * a.per_group + i;
+  for (; i < z; i += WAVES) {
+    const int64_t t = t0 + i;
     float v[PER], d[PER];
-    if (a.valid && !a.valid[t]) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) d[j] = 0.0f;
-    } else {
-      const float inv = scores<BF>(a, t, lane, v);
+    for (int j = 0; j < PER; ++j) v[j] = next[j], d[j] = 0.0f;
+    const bool live = valid;
+    ahead(i + WAVES, valid);
+    if (live) {  // the same for the whole wave
+      const float inv = scores<PER>(a, lane, v);
       float dot = 0.0f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) dot += w[j] * (v[j] * inv);
@@ -286,10 +314,20 @@ extern "C" int st_balance_fwd(const void* logits, int32_t dtype, const int32_t* 
   a.terms = (float*)(a.counted + groups * a.chunks * (experts + 1));
   const hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)a.chunks, (unsigned)groups);
-  if (dtype == ST_DTYPE_BF16)
-    balance_sums<true><<<grid, NTH, 0, s>>>(a);
+  auto run = [&](auto bf, auto f32) {
+    if (dtype == ST_DTYPE_BF16)
+      bf<<<grid, NTH, 0, s>>>(a);
+    else
+      f32<<<grid, NTH, 0, s>>>(a);
+  };
+  if (experts <= 64)
+    run(balance_sums<true, 1>, balance_sums<false, 1>);
+  else if (experts <= 128)
+    run(balance_sums<true, 2>, balance_sums<false, 2>);
+  else if (experts <= 256)
+    run(balance_sums<true, 4>, balance_sums<false, 4>);
   else
-    balance_sums<false><<<grid, NTH, 0, s>>>(a);
+    run(balance_sums<true, 8>, balance_sums<false, 8>);
   balance_join<<<(unsigned)groups, JOIN, 0, s>>>(a);
   if (groups > 1) balance_mean<<<1, 64, 0, s>>>(a);
   return st::check_launch("st_balance_fwd");
@@ -310,9 +348,19 @@ extern "C" int st_balance_bwd(const void* logits, int32_t dtype, const uint8_t* 
   a.chunk = st::cdiv(st::cdiv(per_group, st::cdiv(2048, groups)), 2 * WAVES) * 2 * WAVES;
   a.chunks = st::cdiv(per_group, a.chunk);
   const dim3 grid((unsigned)a.chunks, (unsigned)groups);
-  if (dtype == ST_DTYPE_BF16)
-    balance_bwd<true><<<grid, NTH, 0, (hipStream_t)stream>>>(a);
+  auto run = [&](auto bf, auto f32) {
+    if (dtype == ST_DTYPE_BF16)
+      bf<<<grid, NTH, 0, (hipStream_t)stream>>>(a);
+    else
+      f32<<<grid, NTH, 0, (hipStream_t)stream>>>(a);
+  };
+  if (experts <= 64)
+    run(balance_bwd<true, 1>, balance_bwd<false, 1>);
+  else if (experts <= 128)
+    run(balance_bwd<true, 2>, balance_bwd<false, 2>);
+  else if (experts <= 256)
+    run(balance_bwd<true, 4>, balance_bwd<false, 4>);
   else
-    balance_bwd<false><<<grid, NTH, 0, (hipStream_t)stream>>>(a);
+    run(balance_bwd<true, 8>, balance_bwd<false, 8>);
   return st::check_launch("st_balance_bwd");
 }
