@@ -641,7 +641,7 @@ int st_moe_lora_grads(int64_t rows, int32_t R, int64_t seg_len, int32_t nseg,
  * Norms after and before a part of a block with its gate and residual scale (no
  * counterpart in the reference); y, residual, h, normed and their gradients bf16
  * [rows, hidden], contiguous, hidden at most 16384, every tensor on a 16-byte
- * boundary (a gate of ST_GATE_TOKENS on its element's):
+ * boundary (a gate of ST_GATE_TOKENS on its element's), no result over an operand:
  *   z = post ? y * rsqrt(mean(y^2) + eps) * post : y
  *   h = residual + scale * gate * z
  *   normed = h * rsqrt(mean(h^2) + eps) * pre     (of the unrounded h; pre given)

@@ -9,9 +9,10 @@
 //
 // A wave holds a token's logits (up to 512 experts, PER = 1, 2, 4 or 8 a lane), so each
 // is read once forward and once backward, the next token's while the present one's are
-// worked on (16384 tokens of 256 experts: 17 MB in 12.5 us forward, 12.2 us backward); picks are counted in LDS (whole numbers: their order
-// does not matter), probabilities summed in fp32 in registers over a workgroup's
-// tokens and joined over the workgroups in their order.
+// worked on (16384 tokens of 256 experts: 17 MB in 12.5 us forward, 12.2 us backward);
+// picks are counted in LDS (whole numbers: their order does not matter), probabilities
+// summed in fp32 in registers over a workgroup's tokens and joined over the workgroups
+// in their order.
 #include "common.h"
 
 namespace {

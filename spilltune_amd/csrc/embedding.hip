@@ -32,8 +32,38 @@ __device__ __forceinline__ uint32_t key_of(int64_t id, int64_t V, int64_t paddin
   return id < 0 || id >= V || id == padding ? (uint32_t)V : (uint32_t)id;
 }
 
+// A row that is no multiple of VEC columns (RAG) starts on any element; its last VEC are
+// moved back to end with it: the first `skip` of them are another thread's too, worked
+// out alike and stored twice, or added to the gradient by that one alone.  (8192 tokens,
+// 32000 rows of 1001 columns: sums 9.1 us, of 1000 columns 8.9.)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+template <typename V, typename ANY, bool RAG>
+__device__ __forceinline__ V load(const void* p) {
+  if constexpr (RAG)
+    return *(const ANY*)p;
+  else
+    return *(const V*)p;
+}
+template <typename V, typename ANY, bool RAG>
+__device__ __forceinline__ void store(void* p, V v) {
+  if constexpr (RAG)
+    *(ANY*)p = v;
+  else
+    *(V*)p = v;
+}
+template <bool RAG>
+__device__ __forceinline__ void store_bf16x8(uint16_t* p, const float (&f)[8]) {
+  store<u32x4, u32x4_any, RAG>(p, u32x4{st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
+                                        st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7])});
+}
+
 // ---------------------------------------------------------------- lookup
-template <int VEC, bool F32>
+template <int VEC, bool F32, bool RAG>
 __global__ __launch_bounds__(NTH) void lookup(const void* __restrict__ table,
                                               const void* __restrict__ ids, int ids32, int64_t n,
                                               int64_t V, int64_t H, float scale,
@@ -41,18 +71,18 @@ __global__ __launch_bounds__(NTH) void lookup(const void* __restrict__ table,
   for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
     const int64_t id = id_at(ids, ids32, t);
     const bool in = id >= 0 && id < V;
-    for (int64_t i = threadIdx.x * VEC; i < H; i += (int64_t)blockDim.x * VEC) {
+    for (int64_t col = threadIdx.x * VEC; col < H; col += (int64_t)blockDim.x * VEC) {
+      const int64_t i = RAG && col + VEC > H ? H - VEC : col;
       float f[VEC];
       const int64_t at = (in ? id : 0) * H + i;
       if constexpr (VEC == 8) {
         if constexpr (F32) {
-          const float4 a = *(const float4*)((const float*)table + at);
-          const float4 b = *(const float4*)((const float*)table + at + 4);
-          f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-          f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+          const float* p = (const float*)table + at;
+          const f32x4 a = load<f32x4, f32x4_any, RAG>(p), b = load<f32x4, f32x4_any, RAG>(p + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
         } else {
-          const uint4 v = *(const uint4*)((const uint16_t*)table + at);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          const u32x4 w = load<u32x4, u32x4_any, RAG>((const uint16_t*)table + at);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             f[2 * e] = __uint_as_float(w[e] << 16);
@@ -66,8 +96,7 @@ __global__ __launch_bounds__(NTH) void lookup(const void* __restrict__ table,
       for (int e = 0; e < VEC; ++e) f[e] = in ? f[e] * scale : NAN;
       uint16_t* to = out + t * H + i;
       if constexpr (VEC == 8)
-        *(uint4*)to = make_uint4(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
-                                 st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7]));
+        store_bf16x8<RAG>(to, f);
       else
         *to = st::f32_to_bf16(f[0]);
     }
@@ -360,17 +389,18 @@ struct Sums {
   float* partial;  // [chunks][2][H]: of the run from the chunk before, of the run into the next
 };
 
-template <int VEC>
+template <int VEC, bool RAG>
 __device__ __forceinline__ void store_f(float* p, const float (&f)[VEC]) {
-  if constexpr (VEC >= 4) {
-    *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
-    if constexpr (VEC == 8) *(float4*)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
+  if constexpr (VEC == 1) {
     p[0] = f[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4)
+      store<f32x4, f32x4_any, RAG>(p + e, f32x4{f[e], f[e + 1], f[e + 2], f[e + 3]});
   }
 }
-template <int VEC>
-__device__ __forceinline__ void write_row(const Sums& a, uint32_t token, int64_t i,
+template <int VEC, bool RAG>
+__device__ __forceinline__ void write_row(const Sums& a, uint32_t token, int64_t i, int skip,
                                           const float (&acc)[VEC]) {
   const int64_t at = (int64_t)token * a.H + i;
   float f[VEC];
@@ -378,18 +408,24 @@ __device__ __forceinline__ void write_row(const Sums& a, uint32_t token, int64_t
   for (int e = 0; e < VEC; ++e) f[e] = a.scale * acc[e];
   if (a.grad_f32) {
     float* p = (float*)a.grad + at;
+    if (RAG && a.accumulate && skip) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (e >= skip) p[e] += f[e];
+      return;
+    }
     if (a.accumulate) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] += p[e];
     }
-    store_f<VEC>(p, f);
+    store_f<VEC, RAG>(p, f);
   } else {
     uint16_t* p = (uint16_t*)a.grad + at;
     if constexpr (VEC == 8)
-      *(uint4*)p = make_uint4(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
-                              st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7]));
+      store_bf16x8<RAG>(p, f);
     else if constexpr (VEC == 4)
-      *(uint2*)p = make_uint2(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]));
+      store<u32x2, u32x2_any, RAG>(
+          p, u32x2{st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3])});
     else
       *p = st::f32_to_bf16(f[0]);
   }
@@ -401,43 +437,39 @@ __device__ __forceinline__ void write_row(const Sums& a, uint32_t token, int64_t
 constexpr int AHEAD = 8;
 template <int VEC>
 struct Raw {
-  uint4 v;
+  u32x4 v;
 };
 template <>
 struct Raw<4> {
-  uint2 v;
+  u32x2 v;
 };
 template <>
 struct Raw<1> {
   uint16_t v;
 };
-template <int VEC>
+template <int VEC, bool RAG>
 __device__ __forceinline__ void read_row(const uint16_t* p, Raw<VEC>& r) {
   if constexpr (VEC == 8)
-    r.v = *(const uint4*)p;
+    r.v = load<u32x4, u32x4_any, RAG>(p);
   else if constexpr (VEC == 4)
-    r.v = *(const uint2*)p;
+    r.v = load<u32x2, u32x2_any, RAG>(p);
   else
     r.v = *p;
 }
 template <int VEC>
 __device__ __forceinline__ void add_row(const Raw<VEC>& r, float (&acc)[VEC]) {
-  if constexpr (VEC == 4) {
-    acc[0] += __uint_as_float(r.v.x << 16), acc[1] += __uint_as_float(r.v.x & 0xffff0000u);
-    acc[2] += __uint_as_float(r.v.y << 16), acc[3] += __uint_as_float(r.v.y & 0xffff0000u);
-  } else if constexpr (VEC == 8) {
-    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+  if constexpr (VEC > 1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[2 * e] += __uint_as_float(w[e] << 16);
-      acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+    for (int e = 0; e < VEC / 2; ++e) {
+      acc[2 * e] += __uint_as_float(r.v[e] << 16);
+      acc[2 * e + 1] += __uint_as_float(r.v[e] & 0xffff0000u);
     }
   } else {
     acc[0] += st::bf16_to_f32(r.v);
   }
 }
 
-template <int VEC>
+template <int VEC, bool RAG>
 __global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
   const int lane = threadIdx.x & 63;
   const int64_t c = blockIdx.x, e0 = c * a.chunk;
@@ -454,7 +486,8 @@ __global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
   // first columns and write nothing
   const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   const bool in = col < a.H;
-  const int64_t i = in ? col : 0;
+  const int64_t i = !in ? 0 : RAG && col + VEC > a.H ? a.H - VEC : col;
+  const int skip = RAG && in ? (int)(col - i) : 0;
   auto token = [&](int e) { return __builtin_amdgcn_readlane(tok, e + 1); };  // -1..many
   auto row = [&](int e) {
     return a.dout + (int64_t)__builtin_amdgcn_readlane(pos, e + 1) * a.H + i;
@@ -464,7 +497,7 @@ __global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
   for (int b = 0; b < count; b += AHEAD) {
     Raw<VEC> now[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) read_row<VEC>(row(b + k < count ? b + k : b), now[k]);
+    for (int k = 0; k < AHEAD; ++k) read_row<VEC, RAG>(row(b + k < count ? b + k : b), now[k]);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       const int e = b + k;
@@ -475,11 +508,11 @@ __global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
       const uint32_t whose = token(e);
       if (in) {
         if (from)
-          store_f<VEC>(a.partial + c * 2 * a.H + i, acc);
+          store_f<VEC, RAG>(a.partial + c * 2 * a.H + i, acc);
         else if (!end)
-          store_f<VEC>(a.partial + (c * 2 + 1) * a.H + i, acc);
+          store_f<VEC, RAG>(a.partial + (c * 2 + 1) * a.H + i, acc);
         else
-          write_row<VEC>(a, whose, i, acc);
+          write_row<VEC, RAG>(a, whose, i, skip, acc);
       }
       from = false;
 #pragma unroll
@@ -492,7 +525,7 @@ __global__ __launch_bounds__(NTH) void sum_runs(Sums a) {
 // workgroup sums the runs that begin in its chunk to their ends, wherever these are
 // (at most WHOLE entries, 64 rounds of loads).
 constexpr int64_t WHOLE = 512;
-template <int VEC>
+template <int VEC, bool RAG>
 __global__ __launch_bounds__(NTH) void sum_whole(Sums a) {
   const int lane = threadIdx.x & 63;
   const int n = (int)a.n, e0 = (int)(blockIdx.x * a.chunk), stop = e0 + (int)a.chunk;
@@ -500,7 +533,8 @@ __global__ __launch_bounds__(NTH) void sum_whole(Sums a) {
   // lanes past the columns stay, as in sum_runs: every lane holds a token
   const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   const bool in = col < a.H;
-  const int64_t i = in ? col : 0;
+  const int64_t i = !in ? 0 : RAG && col + VEC > a.H ? a.H - VEC : col;
+  const int skip = RAG && in ? (int)(col - i) : 0;
   bool open = false;  // within a run of this workgroup's
   float acc[VEC] = {};
   for (int w = e0;; w += 56) {  // lane l: entry w - 1 + l, up to the one behind w + 56
@@ -511,7 +545,8 @@ __global__ __launch_bounds__(NTH) void sum_whole(Sums a) {
       Raw<VEC> now[AHEAD];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
-        read_row<VEC>(a.dout + (int64_t)__builtin_amdgcn_readlane(pos, b + k + 1) * a.H + i, now[k]);
+        read_row<VEC, RAG>(a.dout + (int64_t)__builtin_amdgcn_readlane(pos, b + k + 1) * a.H + i,
+                           now[k]);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int e = w + b + k;
@@ -523,7 +558,7 @@ __global__ __launch_bounds__(NTH) void sum_whole(Sums a) {
         }
         add_row<VEC>(now[k], acc);
         if (__builtin_amdgcn_readlane(tok, b + k + 2) == token) continue;
-        if (in) write_row<VEC>(a, token, i, acc);
+        if (in) write_row<VEC, RAG>(a, token, i, skip, acc);
         open = false;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
@@ -534,17 +569,19 @@ __global__ __launch_bounds__(NTH) void sum_whole(Sums a) {
 
 // The run that begins in chunk c and goes on behind it: the partial sums of the
 // chunks whose first token it is, 64 chunks' tokens looked up at once.
-template <int VEC>
+template <int VEC, bool RAG>
 __global__ __launch_bounds__(NTH) void join_runs(Sums a) {
   const int lane = threadIdx.x & 63;
   const int64_t c = blockIdx.x, e0 = c * a.chunk, next = e0 + a.chunk;  // next < n by the grid
   const uint32_t token = a.tok[next], last = a.tok[next - 1], first = a.tok[e0];
   const uint32_t before = e0 > 0 ? a.tok[e0 - 1] : ~0u;
-  const int64_t i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  const bool in = col < a.H;
+  const int64_t i = !in ? 0 : RAG && col + VEC > a.H ? a.H - VEC : col;
+  const int skip = RAG && in ? (int)(col - i) : 0;
   // (lanes past the columns stay: the others ask for their chunks)
   if (token >= a.V || last != token) return;
   if (first == token && before == token) return;  // began earlier
-  const bool in = i < a.H;
   float acc[VEC] = {};
   const float* p = a.partial + (c * 2 + 1) * a.H + i;
   if (in) {
@@ -565,7 +602,7 @@ __global__ __launch_bounds__(NTH) void join_runs(Sums a) {
     }
     if (run < 64) break;
   }
-  if (in) write_row<VEC>(a, token, i, acc);
+  if (in) write_row<VEC, RAG>(a, token, i, skip, acc);
 }
 
 // ---------------------------------------------------------------- host
@@ -620,16 +657,20 @@ extern "C" int st_embedding_fwd(const void* table, int32_t dtype, const void* id
   ST_CHECK_ARG(dtype == ST_DTYPE_BF16 || dtype == ST_DTYPE_F32, "dtype codes are bf16 and fp32");
   if (n == 0) return ST_OK;
   ST_CHECK_ARG(table && ids && out, "st_embedding_fwd: NULL");
-  const bool vec = hidden % 8 == 0 && (((uintptr_t)table | (uintptr_t)out) & 15) == 0;
-  const unsigned grid = (unsigned)(n < (1 << 20) ? n : 1 << 20), th = threads_of(hidden, vec ? 8 : 1);
+  const bool whole = hidden % 8 == 0 && (((uintptr_t)table | (uintptr_t)out) & 15) == 0;
+  const unsigned grid = (unsigned)(n < (1 << 20) ? n : 1 << 20);
+  const unsigned th = threads_of(hidden, hidden < 8 ? 1 : 8);
   const hipStream_t s = (hipStream_t)stream;
   auto run = [&](auto kernel) {
     kernel<<<grid, th, 0, s>>>(table, ids, ids32, n, vocab, hidden, scale, out);
   };
-  if (vec)
-    dtype == ST_DTYPE_F32 ? run(lookup<8, true>) : run(lookup<8, false>);
+  const bool f32 = dtype == ST_DTYPE_F32;
+  if (hidden < 8)
+    f32 ? run(lookup<1, true, false>) : run(lookup<1, false, false>);
+  else if (whole)
+    f32 ? run(lookup<8, true, false>) : run(lookup<8, false, false>);
   else
-    dtype == ST_DTYPE_F32 ? run(lookup<1, true>) : run(lookup<1, false>);
+    f32 ? run(lookup<8, true, true>) : run(lookup<8, false, true>);
   return st::check_launch("st_embedding_fwd");
 }
 
@@ -706,7 +747,8 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
   a.grad_f32 = grad_dtype == ST_DTYPE_F32, a.accumulate = accumulate, a.grad = grad;
   a.partial = (float*)(w + l.partial);
   // as many columns a lane as make 16 bytes of the gradient
-  const int vec = hidden % 8 == 0 && ((uintptr_t)dout & 15) == 0 ? (a.grad_f32 ? 4 : 8) : 1;
+  const bool even = hidden % 8 == 0 && ((uintptr_t)dout & 15) == 0;
+  const int vec = hidden < 8 ? 1 : a.grad_f32 ? 4 : 8;
   const unsigned th = threads_of(hidden, vec);
   const int64_t chunks = st::cdiv(n, a.chunk), slices = st::cdiv(hidden, (int64_t)th * vec);
   if (chunks * slices * th >= (int64_t)1 << 32 || slices >= 65536)
@@ -720,11 +762,15 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
       if (chunks > 1) join<<<more, th, 0, s>>>(a);
     }
   };
-  if (vec == 4)
-    sums(sum_whole<4>, sum_runs<4>, join_runs<4>);
-  else if (vec == 8)
-    sums(sum_whole<8>, sum_runs<8>, join_runs<8>);
+  if (vec == 1)
+    sums(sum_whole<1, false>, sum_runs<1, false>, join_runs<1, false>);
+  else if (vec == 4 && even)
+    sums(sum_whole<4, false>, sum_runs<4, false>, join_runs<4, false>);
+  else if (vec == 4)
+    sums(sum_whole<4, true>, sum_runs<4, true>, join_runs<4, true>);
+  else if (even)
+    sums(sum_whole<8, false>, sum_runs<8, false>, join_runs<8, false>);
   else
-    sums(sum_whole<1>, sum_runs<1>, join_runs<1>);
+    sums(sum_whole<8, true>, sum_runs<8, true>, join_runs<8, true>);
   return st::check_launch("st_embedding_bwd");
 }

@@ -70,76 +70,115 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return v;
 }
 
-// VEC bf16 as they lie.  Elements past the row (`in` false) read its first ones and are
-// cleared: a load under a branch would be waited for at the branch's end.
+// A thread's n-th chunk of a row.  Where the row is no multiple of a chunk (RAG), the last
+// chunk is moved back to end with it: its first `skip` elements are the chunk's before,
+// worked out and stored by both alike, and counted in no sum here.  Elements past the row
+// (`in` false) read its first ones and are cleared: a load under a branch would be waited
+// for at the branch's end.  (4096 rows of 4097: 45 us forward, 82 backward; one element a
+// load took 640 and 1245.)
+struct Place {
+  int64_t i;
+  bool in;
+  int skip;
+};
+template <int VEC, int NT, bool RAG>
+__device__ __forceinline__ Place place(int n, int64_t H) {
+  Place c;
+  const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
+  c.in = i < H;
+  c.i = !c.in ? 0 : RAG && i + VEC > H ? H - VEC : i;
+  c.skip = RAG && c.in ? (int)(i - c.i) : 0;
+  return c;
+}
+// Ragged rows start on any element.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+// VEC bf16 as they lie.
 template <int VEC>
 struct Raw {
-  uint4 v;
+  u32x4 v;
 };
 template <>
 struct Raw<1> {
   uint32_t v;
 };
-template <int VEC>
-__device__ __forceinline__ Raw<VEC> raw(const uint16_t* row, int64_t i, bool in) {
+template <int VEC, bool RAG>
+__device__ __forceinline__ Raw<VEC> raw(const uint16_t* row, const Place& c) {
   Raw<VEC> r;
-  if constexpr (VEC == 8)
-    r.v = *(const uint4*)(row + (in ? i : 0));
+  if constexpr (VEC == 1)
+    r.v = row[c.i];
+  else if constexpr (RAG)
+    r.v = *(const u32x4_any*)(row + c.i);
   else
-    r.v = row[in ? i : 0];
+    r.v = *(const u32x4*)(row + c.i);
   return r;
 }
 template <int VEC>
 __device__ __forceinline__ void unpack(const Raw<VEC>& r, bool in, float (&f)[VEC]) {
   if constexpr (VEC == 8) {
-    const uint32_t w[4] = {in ? r.v.x : 0, in ? r.v.y : 0, in ? r.v.z : 0, in ? r.v.w : 0};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      f[2 * e] = __uint_as_float(w[e] << 16);
-      f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      const uint32_t w = in ? r.v[e] : 0;
+      f[2 * e] = __uint_as_float(w << 16);
+      f[2 * e + 1] = __uint_as_float(w & 0xffff0000u);
     }
   } else {
     f[0] = in ? __uint_as_float(r.v << 16) : 0.0f;
   }
 }
-template <int VEC>
-__device__ __forceinline__ void load_bf16(const uint16_t* row, int64_t i, bool in,
-                                          float (&f)[VEC]) {
-  unpack<VEC>(raw<VEC>(row, i, in), in, f);
+template <int VEC, bool RAG>
+__device__ __forceinline__ void load_bf16(const uint16_t* row, const Place& c, float (&f)[VEC]) {
+  unpack<VEC>(raw<VEC, RAG>(row, c), c.in, f);
 }
-template <int VEC>
-__device__ __forceinline__ void store_bf16(uint16_t* p, int64_t i, const float (&f)[VEC]) {
-  if constexpr (VEC == 8)
-    *(uint4*)(p + i) = make_uint4(st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
-                                  st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7]));
-  else
-    p[i] = st::f32_to_bf16(f[0]);
-}
-template <int VEC>
-__device__ __forceinline__ void load_f32(const float* row, int64_t i, bool in, float (&f)[VEC]) {
-  const float* p = row + (in ? i : 0);
+template <int VEC, bool RAG>
+__device__ __forceinline__ void store_bf16(uint16_t* row, const Place& c, const float (&f)[VEC]) {
   if constexpr (VEC == 8) {
-    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    const u32x4 w = {st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3]),
+                     st::pack_bf16x2(f[4], f[5]), st::pack_bf16x2(f[6], f[7])};
+    if constexpr (RAG)
+      *(u32x4_any*)(row + c.i) = w;
+    else
+      *(u32x4*)(row + c.i) = w;
+  } else {
+    row[c.i] = st::f32_to_bf16(f[0]);
+  }
+}
+template <int VEC, bool RAG>
+__device__ __forceinline__ void load_f32(const float* row, const Place& c, float (&f)[VEC]) {
+  const float* p = row + c.i;
+  if constexpr (VEC == 8) {
+    f32x4 a, b;
+    if constexpr (RAG)
+      a = *(const f32x4_any*)p, b = *(const f32x4_any*)(p + 4);
+    else
+      a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
   } else {
     f[0] = *p;
   }
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) f[e] = in ? f[e] : 0.0f;
+  for (int e = 0; e < VEC; ++e) f[e] = c.in ? f[e] : 0.0f;
 }
-template <int VEC>
-__device__ __forceinline__ void store_f32(float* p, int64_t i, const float (&f)[VEC]) {
+template <int VEC, bool RAG>
+__device__ __forceinline__ void store_f32(float* row, const Place& c, const float (&f)[VEC]) {
+  float* p = row + c.i;
   if constexpr (VEC == 8) {
-    *(float4*)(p + i) = make_float4(f[0], f[1], f[2], f[3]);
-    *(float4*)(p + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    const f32x4 a = {f[0], f[1], f[2], f[3]}, b = {f[4], f[5], f[6], f[7]};
+    if constexpr (RAG)
+      *(f32x4_any*)p = a, *(f32x4_any*)(p + 4) = b;
+    else
+      *(f32x4*)p = a, *(f32x4*)(p + 4) = b;
   } else {
-    p[i] = f[0];
+    p[0] = f[0];
   }
 }
 
 // scale * gate of one chunk
-template <int VEC>
-__device__ __forceinline__ void gate_of(const Args& a, int64_t row, int64_t i, bool in,
+template <int VEC, bool RAG>
+__device__ __forceinline__ void gate_of(const Args& a, int64_t row, const Place& c,
                                         float (&f)[VEC]) {
   if (a.gate_mode == GATE_NONE) {
 #pragma unroll
@@ -155,14 +194,14 @@ __device__ __forceinline__ void gate_of(const Args& a, int64_t row, int64_t i, b
   }
   const int64_t at = (a.gate_mode == GATE_FULL ? row : row / a.rows_per) * a.H;
   if (a.gate_f32)
-    load_f32<VEC>((const float*)a.gate + at, i, in, f);
+    load_f32<VEC, RAG>((const float*)a.gate + at, c, f);
   else
-    load_bf16<VEC>((const uint16_t*)a.gate + at, i, in, f);
+    load_bf16<VEC, RAG>((const uint16_t*)a.gate + at, c, f);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) f[e] *= a.scale;
 }
 
-template <int VEC, int NT, int NV>
+template <int VEC, int NT, int NV, bool RAG>
 __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
   __shared__ float red[2][NT / 64];
   const float over = 1.0f / (float)a.H;
@@ -171,46 +210,48 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
     float y[NV][VEC], h[NV][VEC];
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
-      load_bf16<VEC>(a.y + base, i, i < a.H, y[n]);
-      load_bf16<VEC>(a.res + base, i, i < a.H, h[n]);
+      const Place c = place<VEC, NT, RAG>(n, a.H);
+      load_bf16<VEC, RAG>(a.y + base, c, y[n]);
+      load_bf16<VEC, RAG>(a.res + base, c, h[n]);
     }
     float r1 = 1.0f;
     if (a.post) {
       float ss = 0.0f;
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
+      for (int n = 0; n < NV; ++n) {
+        const Place c = place<VEC, NT, RAG>(n, a.H);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) ss += y[n][e] * y[n][e];
+        for (int e = 0; e < VEC; ++e) ss += e < c.skip ? 0.0f : y[n][e] * y[n][e];
+      }
       r1 = 1.0f / sqrtf(block_sum<NT>(ss, red[0]) * over + a.eps);
       if (a.r1 && threadIdx.x == 0) a.r1[row] = r1;
     }
     float ss = 0.0f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
+      const Place c = place<VEC, NT, RAG>(n, a.H);
       float w[VEC], g[VEC];
-      if (a.post) load_bf16<VEC>(a.post, i, i < a.H, w);
-      gate_of<VEC>(a, row, i, i < a.H, g);
+      if (a.post) load_bf16<VEC, RAG>(a.post, c, w);
+      gate_of<VEC, RAG>(a, row, c, g);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float z = a.post ? y[n][e] * r1 * w[e] : y[n][e];
         h[n][e] += g[e] * z;
-        ss += h[n][e] * h[n][e];
+        ss += e < c.skip ? 0.0f : h[n][e] * h[n][e];
       }
-      if (i < a.H) store_bf16<VEC>(a.h + base, i, h[n]);
+      if (c.in) store_bf16<VEC, RAG>(a.h + base, c, h[n]);
     }
     if (a.pre) {  // the same way for the whole launch
       const float r2 = 1.0f / sqrtf(block_sum<NT>(ss, red[1]) * over + a.eps);
       if (a.r2 && threadIdx.x == 0) a.r2[row] = r2;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
+        const Place c = place<VEC, NT, RAG>(n, a.H);
         float w[VEC];
-        load_bf16<VEC>(a.pre, i, i < a.H, w);
+        load_bf16<VEC, RAG>(a.pre, c, w);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) w[e] *= h[n][e] * r2;
-        if (i < a.H) store_bf16<VEC>(a.normed + base, i, w);
+        if (c.in) store_bf16<VEC, RAG>(a.normed + base, c, w);
       }
     }
     if constexpr (NT > 64) __syncthreads();  // the sums' places are free again
@@ -218,15 +259,38 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
 }
 
 // SUMS: run blockIdx.x of `per_run` rows (all of one gate row), columns' sums kept.
-// GATE: there is one.  The next row is read while the present one is worked on (up to
-// 16 elements a thread: beyond, registers are short), and rows wait as the bf16 they
-// are: with them in fp32, fewer waves fit.
-template <int VEC, int NT, int NV, bool SUMS, bool GATE>
+// GATE: there is one.  Rows wait in registers as the bf16 they are (in fp32, fewer waves
+// fit), with SUMS the next one on its way while the present one is worked on.
+// Beyond 8192 columns (WIDE) a thread has no registers for that: it reads its chunks
+// again where it needs them, out of the caches, and two of the columns' sums lie in LDS
+// (2048 x 16384 with learnt norms and gate: 170 us, with all of it in registers 470).
+template <int VEC, int NT, int NV, bool SUMS, bool GATE, bool RAG>
 __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
   __shared__ float red[3][NT / 64];
-  constexpr bool EARLY = SUMS && VEC * NV <= 16;
+  constexpr bool WIDE = NT * NV * VEC > 8192, LDS = SUMS && WIDE, EARLY = SUMS && !WIDE;
+  __shared__ f32x4 kept[LDS ? 2 * NV * VEC / 4 * NT : 1];  // dpost and dpre, a thread's own
   const float over = 1.0f / (float)a.H;
   float dpost[NV][VEC] = {}, dpre[NV][VEC] = {}, dgate[NV][VEC] = {};
+  auto add = [&](int which, int n, float (&sum)[VEC], const float (&x)[VEC],
+                 const float (&y)[VEC]) {
+    if constexpr (LDS) {
+#pragma unroll
+      for (int q = 0; q < VEC / 4; ++q) {
+        f32x4& k = kept[((which * NV + n) * (VEC / 4) + q) * NT + threadIdx.x];
+        f32x4 v = k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(x[4 * q + e], y[4 * q + e], v[e]);
+        k = v;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] = __builtin_fmaf(x[e], y[e], sum[e]);
+    }
+  };
+  if constexpr (LDS) {
+#pragma unroll
+    for (int k = 0; k < 2 * NV * VEC / 4; ++k) kept[k * NT + threadIdx.x] = f32x4{};
+  }
   int64_t row, end, by;
   if constexpr (SUMS) {
     const int64_t in_group = a.runs / (a.rows / a.rows_per);  // runs of a gate row
@@ -241,13 +305,15 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
   const uint16_t *dh = has_dh ? a.dh : a.y, *dn = has_dn ? a.dn : a.y;
   Raw<VEC> ny[NV], nh[NV], nd[NV], nn[NV];
   auto fetch = [&](int64_t r) {
+    if (WIDE) return;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC, base = r * a.H;
-      ny[n] = raw<VEC>(a.y + base, i, i < a.H);
-      nh[n] = raw<VEC>(a.res + base, i, i < a.H);
-      nd[n] = raw<VEC>(dh + base, i, i < a.H);
-      nn[n] = raw<VEC>(dn + base, i, i < a.H);
+      const Place c = place<VEC, NT, RAG>(n, a.H);
+      const int64_t base = r * a.H;
+      ny[n] = raw<VEC, RAG>(a.y + base, c);
+      nh[n] = raw<VEC, RAG>(a.res + base, c);
+      nd[n] = raw<VEC, RAG>(dh + base, c);
+      nn[n] = raw<VEC, RAG>(dn + base, c);
     }
   };
   fetch(row);
@@ -257,35 +323,43 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) ry[n] = ny[n], rh[n] = nh[n], rd[n] = nd[n], rn[n] = nn[n];
     if (EARLY) fetch(row + by < end ? row + by : row);
+    auto chunk = [&](const Raw<VEC>(&r)[NV], const uint16_t* p, int n) {
+      if constexpr (WIDE)
+        return raw<VEC, RAG>(p + base, place<VEC, NT, RAG>(n, a.H));
+      else
+        return r[n];
+    };
     const float r1 = a.post ? a.r1[row] : 1.0f, r2 = has_dn ? a.r2[row] : 0.0f;
     float d[NV][VEC];
     if (has_dn) {
       float h[NV][VEC], gn[NV][VEC], dot = 0.0f;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
-        const bool in = i < a.H;
-        float y[VEC], w[VEC], g[VEC], p[VEC];
-        unpack<VEC>(ry[n], in, y);
-        unpack<VEC>(rh[n], in, h[n]);
-        unpack<VEC>(rn[n], in, gn[n]);
-        if (a.post) load_bf16<VEC>(a.post, i, in, w);
-        load_bf16<VEC>(a.pre, i, in, p);
-        if (GATE) gate_of<VEC>(a, row, i, in, g);
+        const Place c = place<VEC, NT, RAG>(n, a.H);
+        float y[VEC], w[VEC], g[VEC], p[VEC], hr[VEC];
+        unpack<VEC>(chunk(ry, a.y, n), c.in, y);
+        unpack<VEC>(chunk(rh, a.res, n), c.in, h[n]);
+        unpack<VEC>(chunk(rn, dn, n), c.in, gn[n]);
+        if (a.post) load_bf16<VEC, RAG>(a.post, c, w);
+        load_bf16<VEC, RAG>(a.pre, c, p);
+        if (GATE) gate_of<VEC, RAG>(a, row, c, g);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float z = a.post ? y[e] * r1 * w[e] : y[e];
           h[n][e] = __builtin_fmaf(GATE ? g[e] : a.scale, z, h[n][e]);
-          if constexpr (SUMS) dpre[n][e] = __builtin_fmaf(gn[n][e], h[n][e] * r2, dpre[n][e]);
+          hr[e] = h[n][e] * r2;
+        }
+        if constexpr (SUMS) add(1, n, dpre[n], gn[n], hr);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
           gn[n][e] *= p[e];
-          dot = __builtin_fmaf(gn[n][e], h[n][e], dot);
+          dot = e < c.skip ? dot : __builtin_fmaf(gn[n][e], h[n][e], dot);
         }
       }
       const float c = block_sum<NT>(dot, red[0]) * over * r2 * r2;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        const bool in = ((int64_t)n * NT + threadIdx.x) * VEC < a.H;
-        unpack<VEC>(rd[n], in && has_dh, d[n]);
+        unpack<VEC>(chunk(rd, dh, n), place<VEC, NT, RAG>(n, a.H).in && has_dh, d[n]);
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
           d[n][e] = __builtin_fmaf(r2, __builtin_fmaf(-c, h[n][e], gn[n][e]), d[n][e]);
@@ -293,39 +367,38 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
     } else {
 #pragma unroll
       for (int n = 0; n < NV; ++n)
-        unpack<VEC>(rd[n], ((int64_t)n * NT + threadIdx.x) * VEC < a.H && has_dh, d[n]);
+        unpack<VEC>(chunk(rd, dh, n), place<VEC, NT, RAG>(n, a.H).in && has_dh, d[n]);
     }
     float dot = 0.0f, gdot = 0.0f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
-      const bool in = i < a.H;
-      if (a.dres && in) store_bf16<VEC>(a.dres + base, i, d[n]);
-      float y[VEC], w[VEC], g[VEC], dz[VEC];
-      unpack<VEC>(ry[n], in, y);
-      if (a.post) load_bf16<VEC>(a.post, i, in, w);
-      if (GATE) gate_of<VEC>(a, row, i, in, g);
+      const Place c = place<VEC, NT, RAG>(n, a.H);
+      if (a.dres && c.in) store_bf16<VEC, RAG>(a.dres + base, c, d[n]);
+      float y[VEC], yn[VEC], w[VEC], g[VEC], dz[VEC];
+      unpack<VEC>(chunk(ry, a.y, n), c.in, y);
+      if (a.post) load_bf16<VEC, RAG>(a.post, c, w);
+      if (GATE) gate_of<VEC, RAG>(a, row, c, g);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float yn = y[e] * r1;
+        yn[e] = y[e] * r1;
         if (GATE) {
-          dz[e] = a.scale * d[n][e] * (a.post ? yn * w[e] : yn);
-          gdot += dz[e];
+          dz[e] = a.scale * d[n][e] * (a.post ? yn[e] * w[e] : yn[e]);
+          gdot += e < c.skip ? 0.0f : dz[e];
+          if constexpr (SUMS) dgate[n][e] += dz[e];
         }
-        float q = (GATE ? g[e] : a.scale) * d[n][e];
-        if constexpr (SUMS) {
-          if (GATE) dgate[n][e] += dz[e];
-          dpost[n][e] = __builtin_fmaf(q, yn, dpost[n][e]);
-        }
-        if (a.post) q *= w[e];
-        dot = __builtin_fmaf(q, y[e], dot);
-        d[n][e] = q;
+        d[n][e] *= GATE ? g[e] : a.scale;
       }
-      if (GATE && a.gate_mode == GATE_FULL && a.dgate && in) {
+      if constexpr (SUMS) add(0, n, dpost[n], d[n], yn);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (a.post) d[n][e] *= w[e];
+        dot = e < c.skip ? dot : __builtin_fmaf(d[n][e], y[e], dot);
+      }
+      if (GATE && a.gate_mode == GATE_FULL && a.dgate && c.in) {
         if (a.gate_f32)
-          store_f32<VEC>((float*)a.dgate + base, i, dz);
+          store_f32<VEC, RAG>((float*)a.dgate + base, c, dz);
         else
-          store_bf16<VEC>((uint16_t*)a.dgate + base, i, dz);
+          store_bf16<VEC, RAG>((uint16_t*)a.dgate + base, c, dz);
       }
     }
     if (GATE && a.gate_mode == GATE_TOKENS && a.dgate) {
@@ -342,15 +415,14 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
       if (a.post) c = block_sum<NT>(dot, red[2]) * over * r1 * r1;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
-        const bool in = i < a.H;
+        const Place at = place<VEC, NT, RAG>(n, a.H);
         if (a.post) {
           float y[VEC];
-          unpack<VEC>(ry[n], in, y);
+          unpack<VEC>(chunk(ry, a.y, n), at.in, y);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) d[n][e] = r1 * __builtin_fmaf(-c, y[e], d[n][e]);
         }
-        if (in) store_bf16<VEC>(a.dy + base, i, d[n]);
+        if (at.in) store_bf16<VEC, RAG>(a.dy + base, at, d[n]);
       }
     }
     if (!EARLY && row + by < end) fetch(row + by);
@@ -360,11 +432,18 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
     float* to = a.partial + (int64_t)blockIdx.x * 3 * a.H;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int64_t i = ((int64_t)n * NT + threadIdx.x) * VEC;
-      if (i >= a.H) continue;
-      store_f32<VEC>(to, i, dpost[n]);
-      store_f32<VEC>(to + a.H, i, dpre[n]);
-      if (GATE) store_f32<VEC>(to + 2 * a.H, i, dgate[n]);
+      const Place c = place<VEC, NT, RAG>(n, a.H);
+      if (!c.in) continue;
+      if constexpr (LDS) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          dpost[n][e] = kept[(n * (VEC / 4) + e / 4) * NT + threadIdx.x][e % 4];
+          dpre[n][e] = kept[((NV + n) * (VEC / 4) + e / 4) * NT + threadIdx.x][e % 4];
+        }
+      }
+      store_f32<VEC, RAG>(to, c, dpost[n]);
+      store_f32<VEC, RAG>(to + a.H, c, dpre[n]);
+      if (GATE) store_f32<VEC, RAG>(to + 2 * a.H, c, dgate[n]);
     }
   }
 }
@@ -404,54 +483,56 @@ __global__ __launch_bounds__(1024) void norms_join(const float* __restrict__ par
 
 // ---------------------------------------------------------------- host
 // Runs of rows in a backward that sums over rows, never across gate rows: as many as
-// workgroups run at once, so that none waits for a second turn (2103 rows of 7168: 421
-// runs of 5 rows 76 us, 234 of 9 rows 66).
+// workgroups run at once, so that none waits for a second turn and no CU idles (2103 rows
+// of 7168: 421 runs of 5 rows 76 us, 234 of 9 rows 66; 30000 rows of 512: 512 runs 140,
+// 3072 42; of 1001: 512 runs 210, 1536 113).  A CU holds 12 of the kernel's waves up to
+// 2048 columns, two workgroups of eight to 4096, one beyond.  Runs of at least two rows
+// where there are as many: each costs as much as a row again in partial sums.
 void plan_runs(int64_t rows, int64_t rows_per, int64_t H, int64_t& runs, int64_t& per_run) {
   const int64_t groups = rows / rows_per;
-  int64_t each = st::cdiv(H > 4096 ? 256 : 512, groups);
-  if (each > rows_per) each = rows_per;
+  const int64_t at_once = H > 4096 ? 256 : H > 2048 ? 512 : 256 * 12 / st::cdiv(H, 512);
+  int64_t each = st::cdiv(at_once, groups);
+  if (each > rows_per / 2) each = rows_per > 1 ? rows_per / 2 : 1;
   per_run = st::cdiv(rows_per, each);
   runs = groups * st::cdiv(rows_per, per_run);
 }
 
-template <int VEC, int NT, int NV>
+template <int VEC, int NT, int NV, bool RAG>
 void go(const Args& a, bool bwd, bool sums, hipStream_t s) {
   const unsigned grid = (unsigned)(a.rows < (1 << 20) ? a.rows : 1 << 20);
   if (!bwd)
-    norms_fwd<VEC, NT, NV><<<grid, NT, 0, s>>>(a);
+    norms_fwd<VEC, NT, NV, RAG><<<grid, NT, 0, s>>>(a);
   else if (sums && a.gate)
-    norms_bwd<VEC, NT, NV, true, true><<<(unsigned)a.runs, NT, 0, s>>>(a);
+    norms_bwd<VEC, NT, NV, true, true, RAG><<<(unsigned)a.runs, NT, 0, s>>>(a);
   else if (sums)
-    norms_bwd<VEC, NT, NV, true, false><<<(unsigned)a.runs, NT, 0, s>>>(a);
+    norms_bwd<VEC, NT, NV, true, false, RAG><<<(unsigned)a.runs, NT, 0, s>>>(a);
   else if (a.gate)
-    norms_bwd<VEC, NT, NV, false, true><<<grid, NT, 0, s>>>(a);
+    norms_bwd<VEC, NT, NV, false, true, RAG><<<grid, NT, 0, s>>>(a);
   else
-    norms_bwd<VEC, NT, NV, false, false><<<grid, NT, 0, s>>>(a);
+    norms_bwd<VEC, NT, NV, false, false, RAG><<<grid, NT, 0, s>>>(a);
 }
 
-// A row in one wave where it fits (no barriers), in two to sixteen waves otherwise;
-// rows of whole 16-byte chunks eight elements a lane at a time, others one by one.  The
-// forward and the sums over rows do better with sixteen elements a thread (fewer waves
-// at a barrier; 8192 rows of 4096 forward 47 us against 52), the plain backward with
-// eight (84 against 95).
-void dispatch(const Args& a, bool bwd, bool sums, hipStream_t s) {
+// A row in one wave where it fits (no barriers), in two to sixteen waves otherwise, in
+// chunks of eight elements.  The forward and the sums over rows do better with sixteen
+// elements a thread (fewer waves at a barrier; 8192 rows of 4096 forward 47 us against
+// 52), the plain backward with eight (84 against 95).
+template <bool RAG>
+void by_size(const Args& a, bool bwd, bool sums, hipStream_t s) {
   const int64_t H = a.H;
-  if (H % 8 == 0) {
-    if (H <= 512) go<8, 64, 1>(a, bwd, sums, s);
-    else if (H <= 1024) go<8, 128, 1>(a, bwd, sums, s);
-    else if (H <= 2048) go<8, 256, 1>(a, bwd, sums, s);
-    else if (H <= 4096 && bwd) go<8, 512, 1>(a, bwd, sums, s);
-    else if (H <= 4096) go<8, 256, 2>(a, bwd, sums, s);
-    else if (H <= 8192 && bwd && !sums) go<8, 1024, 1>(a, bwd, sums, s);
-    else if (H <= 8192) go<8, 512, 2>(a, bwd, sums, s);
-    else if (bwd && sums) go<8, 512, 4>(a, bwd, sums, s);
-    else go<8, 1024, 2>(a, bwd, sums, s);
-  } else {
-    if (H <= 256) go<1, 64, 4>(a, bwd, sums, s);
-    else if (H <= 1024) go<1, 256, 4>(a, bwd, sums, s);
-    else if (H <= 4096) go<1, 512, 8>(a, bwd, sums, s);
-    else go<1, 1024, 16>(a, bwd, sums, s);
-  }
+  if (H <= 512) go<8, 64, 1, RAG>(a, bwd, sums, s);
+  else if (H <= 1024) go<8, 128, 1, RAG>(a, bwd, sums, s);
+  else if (H <= 2048) go<8, 256, 1, RAG>(a, bwd, sums, s);
+  else if (H <= 4096 && bwd) go<8, 512, 1, RAG>(a, bwd, sums, s);
+  else if (H <= 4096) go<8, 256, 2, RAG>(a, bwd, sums, s);
+  else if (H <= 8192 && bwd && !sums) go<8, 1024, 1, RAG>(a, bwd, sums, s);
+  else if (H <= 8192) go<8, 512, 2, RAG>(a, bwd, sums, s);
+  else if (bwd && a.gate) go<8, 512, 4, RAG>(a, bwd, sums, s);
+  else go<8, 1024, 2, RAG>(a, bwd, sums, s);
+}
+void dispatch(const Args& a, bool bwd, bool sums, hipStream_t s) {
+  if (a.H < 8) go<1, 64, 1, false>(a, bwd, sums, s);
+  else if (a.H % 8 == 0) by_size<false>(a, bwd, sums, s);
+  else by_size<true>(a, bwd, sums, s);
 }
 
 int check_args(const Args& a, const char* what) {

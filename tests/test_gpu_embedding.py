@@ -200,6 +200,25 @@ def test_token_embedding_adds_and_replaces(n):
     assert (e.grad == 0).all()
 
 
+@pytest.mark.parametrize("n", [300, 20000])
+@pytest.mark.parametrize("H", [4, 9, 12, 15, 33, 1001, 1027])
+def test_columns_that_end_inside_a_chunk(H, n):
+    """Rows of no whole chunks: looked up, summed and added to a gradient once each."""
+    for dtype in (F32, BF):
+        table, ids, dout = make(n, 50, H, dtype, seed=H)
+        t = table.clone().requires_grad_(True)
+        out = ops.embedding(t, ids, scale=1.7)
+        want = table[ids].double() * 1.7
+        assert ((out.double() - want).abs() <= (2**-8 + 2**-22) * want.abs()).all()
+        (grad,) = torch.autograd.grad(out, [t], dout)
+        check_grad(grad, ids, dout, 1.7)
+    e = TokenEmbedding(table, device="cuda", scale=1.7)
+    before = torch.randn_like(e.grad)
+    e.grad.copy_(before)
+    e.add_grad(ids, dout)
+    check_grad(e.grad, ids, dout, 1.7, before=before)
+
+
 def test_adamw_updates_a_table():
     table, ids, dout = make(50, 60, 16, seed=10)
     e = TokenEmbedding(table, device="cuda")

@@ -122,6 +122,12 @@ def test_forms(H, post, pre, gate, gate_dtype):
     check(*inputs((3, 7, H), post, pre, gate, gate_dtype, seed=H), scale=1.7)
 
 
+@pytest.mark.parametrize("gate", [None, "channel", "row", "full"])
+@pytest.mark.parametrize("H", [9, 1001, 8193, 12296, 16383])
+def test_ragged_and_wide_rows(H, gate):
+    check(*inputs((2, 9, H), gate=gate, gate_dtype=F32, seed=H), scale=0.7)
+
+
 @pytest.mark.parametrize("shape,gate", [((1, 1, 4096), "channel"), ((700, 64), "channel"),
                                         ((5000, 3, 16), "row"), ((2, 1500, 136), "row"),
                                         ((3, 1, 40), "row"), ((4096,), None), ((4, 128), "token"),
