@@ -698,10 +698,11 @@ int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t ids32, int64
 /* ---------------------------------------------------------------- balance */
 /*
  * Balance loss of a router (no counterpart in the reference): logits bf16 or fp32
- * [groups * per_group, experts], picks [groups * per_group, top_k], valid (bytes, 0:
- * the token takes no part; NULL: all valid).  p = softmax of a token's logits, or with
- * `sigmoid` its sigmoids over their sum (+ 1e-20); for a group of n valid tokens with
- * c_e picks of expert e (picks outside [0, experts) are not counted)
+ * [groups * per_group, experts], picks [groups * per_group, top_k] (int32 or, with
+ * picks64, int64), valid (bytes, 0: the token takes no part; NULL: all valid).  p =
+ * softmax of a token's logits, or with `sigmoid` its sigmoids over their sum (+ 1e-20);
+ * for a group of n valid tokens with c_e picks of expert e (picks outside [0, experts)
+ * are not counted)
  *   L_g = experts * sum_e c_e / (top_k n) * mean(p_e)
  * and `loss` is the mean over the groups with a valid token (0 without any).  counts
  * [groups, experts] and tokens [groups + 1] (valid tokens a group; then the number of
@@ -709,9 +710,9 @@ int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t ids32, int64
  * fp32 on the device.  experts <= 512, top_k <= 64, groups < 65536, per_group < 2^25.
  */
 int64_t st_balance_workspace_bytes(int64_t groups, int64_t per_group, int32_t experts);
-int st_balance_fwd(const void* logits, int32_t dtype, const int32_t* picks, const uint8_t* valid,
-                   int64_t groups, int64_t per_group, int32_t experts, int32_t top_k,
-                   int32_t sigmoid, float* loss, int64_t* counts, int32_t* tokens,
+int st_balance_fwd(const void* logits, int32_t dtype, const void* picks, int32_t picks64,
+                   const uint8_t* valid, int64_t groups, int64_t per_group, int32_t experts,
+                   int32_t top_k, int32_t sigmoid, float* loss, int64_t* counts, int32_t* tokens,
                    void* workspace, int64_t workspace_bytes, st_stream_t stream);
 int st_balance_bwd(const void* logits, int32_t dtype, const uint8_t* valid, int64_t groups,
                    int64_t per_group, int32_t experts, int32_t top_k, int32_t sigmoid,

@@ -130,8 +130,8 @@ _SIGNATURES = {
     "st_embedding_bwd": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _F, _I64, _P, _I32, _I32, _P, _I64,
                                 _P]),
     "st_balance_workspace_bytes": (_I64, [_I64, _I64, _I32]),
-    "st_balance_fwd": (_I32, [_P, _I32, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I64,
-                              _P]),
+    "st_balance_fwd": (_I32, [_P, _I32, _P, _I32, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P,
+                              _I64, _P]),
     "st_balance_bwd": (_I32, [_P, _I32, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),
     "st_orthogonalize_workspace_bytes": (_I64, [_I32, _P]),
     "st_orthogonalize": (_I32, [_I32, _P, _I32, _I32, _D, _D, _D, _D, _P, _I64, _P]),

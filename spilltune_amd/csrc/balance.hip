@@ -34,7 +34,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 struct Args {
   const void* logits;
-  const int32_t* picks;
+  const int32_t* picks;  // words of 32 bits, `wide` of them a pick
+  int32_t wide;
   const uint8_t* valid;
   int64_t groups, per_group;  // tokens of a group
   int32_t E, k, sigmoid;
@@ -98,22 +99,23 @@ __global__ __launch_bounds__(NTH) void balance_sums(Args a) {
   int64_t i = c * a.chunk + wave;
   const int64_t last = a.per_group - 1;
   // what the next token needs, also where there is none (the last one's then)
-  auto ahead = [&](int64_t k, bool& valid, int& pick) {
+  auto ahead = [&](int64_t k, bool& valid, int& pick, int& high) {
     const int64_t t = t0 + (k < z ? k : last);
     fetch<BF, PER>(a, t, lane, next);
     valid = !a.valid || a.valid[t];
-    pick = a.picks[t * a.k + (lane < a.k ? lane : 0)];
+    const int32_t* p = a.picks + (t * a.k + (lane < a.k ? lane : 0)) * a.wide;
+    pick = p[0], high = a.wide == 2 ? p[a.wide - 1] : 0;
   };
   bool valid;
-  int pick;
-  ahead(i, valid, pick);
+  int pick, high;
+  ahead(i, valid, pick, high);
   for (; i < z; i += WAVES) {
     float v[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) v[j] = next[j];
     const bool live = valid;
-    const int e = pick;
-    ahead(i + WAVES, valid, pick);
+    const int e = high ? -1 : pick;
+    ahead(i + WAVES, valid, pick, high);
     if (!live) continue;  // the same for the whole wave
     const float inv = scores<PER>(a, lane, v);
 #pragma unroll
@@ -293,13 +295,14 @@ extern "C" int64_t st_balance_workspace_bytes(int64_t groups, int64_t per_group,
   return (groups * a.chunks * (2 * (int64_t)experts + 1) + groups) * 4;
 }
 
-extern "C" int st_balance_fwd(const void* logits, int32_t dtype, const int32_t* picks,
-                              const uint8_t* valid, int64_t groups, int64_t per_group,
-                              int32_t experts, int32_t top_k, int32_t sigmoid, float* loss,
+extern "C" int st_balance_fwd(const void* logits, int32_t dtype, const void* picks,
+                              int32_t picks64, const uint8_t* valid, int64_t groups,
+                              int64_t per_group, int32_t experts, int32_t top_k, int32_t sigmoid, float* loss,
                               int64_t* counts, int32_t* tokens, void* workspace,
                               int64_t workspace_bytes, st_stream_t stream) {
   Args a = {};
-  a.logits = logits, a.picks = picks, a.valid = valid, a.groups = groups, a.per_group = per_group;
+  a.logits = logits, a.picks = (const int32_t*)picks, a.wide = picks64 ? 2 : 1, a.valid = valid;
+  a.groups = groups, a.per_group = per_group;
   a.E = experts, a.k = top_k, a.sigmoid = sigmoid, a.loss = loss, a.counts = counts;
   a.tokens = tokens;
   const int rc = check_args(a, dtype, "st_balance_fwd");

@@ -170,9 +170,9 @@ class _BalanceLoss(torch.autograd.Function):
             # the groups' valid tokens, which the backward reads, and the call's scratch
             tokens = torch.empty(4 * (groups + 1) + nbytes, dtype=torch.uint8, device=dev)
             _lib.call("st_balance_fwd", logits.data_ptr(), dtype, indices.data_ptr(),
-                      _lib.ptr(valid), groups, per, E, k, sigmoid, loss.data_ptr(),
-                      counts.data_ptr(), tokens.data_ptr(), tokens.data_ptr() + 4 * (groups + 1),
-                      nbytes, _stream(dev))
+                      int(indices.dtype == torch.int64), _lib.ptr(valid), groups, per, E, k, sigmoid,
+                      loss.data_ptr(), counts.data_ptr(), tokens.data_ptr(),
+                      tokens.data_ptr() + 4 * (groups + 1), nbytes, _stream(dev))
         ctx.save_for_backward(logits, valid, counts, tokens)
         ctx.meta = (groups, per, k, sigmoid, dtype)
         ctx.mark_non_differentiable(counts)
@@ -228,7 +228,7 @@ def balance_loss(logits, indices, *, score="softmax", valid=None, per_row=False)
         raise ValueError("unsupported_capability: logits, indices and valid on one device")
     groups = shape[0] if per_row else 1
     return BalanceLoss(*_BalanceLoss.apply(
-        logits.contiguous(), indices.to(_I32).contiguous(),
+        logits.contiguous(), indices.contiguous(),
         None if valid is None else valid.contiguous(), groups, int(score == "sigmoid")))
 
 
@@ -237,8 +237,8 @@ class ExpertBalance:
     pass that is differentiated adds ``coefficient`` times :func:`balance_loss` of its
     router to the loss whose gradient flows, and is counted here -- ``loss`` the sum of
     the passes' losses (without the coefficient), ``counts`` (int64 [E]) of their picks,
-    both on the device, ``passes`` how many.  The routers are frozen: the term teaches
-    the adapters before them.
+    both on the device, ``passes`` how many (of a captured pass, what its last replay
+    left, once).  The routers are frozen: the term teaches the adapters before them.
 
     Every microbatch adds its own term, so a window of ``n`` of them that is to add one
     average takes the coefficient over ``n``.  ``per_row`` balances each row by itself.

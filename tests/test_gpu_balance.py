@@ -113,7 +113,7 @@ def test_nothing_valid():
     for per_row in (False, True):
         loss, counts, g = check(x, i, valid=torch.zeros(2, 6, dtype=torch.bool, device="cuda"),
                                 per_row=per_row)
-        assert float(loss) == 0.0 and int(counts.sum()) == 0 and (g == 0).all()
+        assert float(loss.detach()) == 0.0 and int(counts.sum()) == 0 and (g == 0).all()
 
 
 def test_picks_outside_and_twice():
@@ -121,7 +121,10 @@ def test_picks_outside_and_twice():
     i[0, :7, 0], i[1, 3, 2], i[1, 4, 1] = -1, 32, -(1 << 31)
     i[0, 10] = 3  # one expert four times
     check(x, i)
-    check(x, i.long(), per_row=True)
+    wide = i.long()
+    wide[1, 5:9, 0] += 1 << 32  # whose lower halves are experts
+    wide[0, 11, 1] = -(1 << 63)
+    check(x, wide, per_row=True)
 
 
 def test_sure_routers():
