@@ -8,7 +8,8 @@
 // number of steps; in between stand r x r matrices alone.
 //
 // Everything between the loads and the stores is in 64 bits, on the matrix cores
-// (v_mfma_f64_16x16x4: 46 TFLOP/s measured, dependent ones 75 ns apart).  In 32 bits
+// (v_mfma_f64_16x16x4: 77 TFLOP/s measured and dependent ones 27 ns apart with the sums
+// in vector registers, 26 and 81 in the accumulation ones).  In 32 bits
 // G loses the squares of singular values below 2^-12 of the largest, and the steps
 // then multiply what was lost by a^2 each.  64 bits bound the steps too: an error of
 // 2^-53 grows by a^2 a step, so |a|^(2 steps) may reach 1e13 (12 steps at a = 3.4445).
@@ -21,6 +22,7 @@
 // leaves between G and its transpose grows by a^2 a step as well: without this, 7 steps
 // are off by 5e-12 and 12 by 6e-7 of the largest entry, with it by 3e-15.)
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 
@@ -39,14 +41,24 @@ struct Entry {
   int64_t part, poly;      // its first matrix's place in the two scratch areas (doubles)
   int32_t K, r;            // long and short side
   int32_t CH, chunks;      // long elements of a workgroup in gram, and its workgroups
-  int32_t AL;              // long elements of a workgroup in apply
+  int32_t AL;              // long elements of a workgroup in apply (all three: r <= 32)
   int16_t tall;            // the short side is the contiguous one
   int16_t vec;             // rows may be read four elements at a time
 };
 enum { IN_GRAM, IN_SUM, IN_NORM, IN_POLY, IN_APPLY, PHASES };
+// Equal shares of all units of a phase, one behind the other, for `wgs` workgroups: the
+// first `rem` take q + 1 units, the others q.
+struct Shares {
+  uint32_t wgs, q, rem;
+  __host__ __device__ uint32_t begin(uint32_t b) const { return b * q + (b < rem ? b : rem); }
+  __host__ __device__ uint32_t owner(uint32_t u) const {
+    return u < rem * (q + 1) ? u / (q + 1) : rem + (u - rem * (q + 1)) / q;
+  }
+};
 struct Table {
   Entry e[MAXE];
-  uint32_t tile0[PHASES][64];  // the entries' first workgroups in a phase, then ~0
+  uint32_t tile0[PHASES][64];  // the entries' first workgroups (units) in a phase, then ~0
+  Shares gram, apply;          // r > 32
   int32_t n, steps;
   double a, b, c, eps;
 };
@@ -64,6 +76,41 @@ __device__ __forceinline__ const Entry& find(const Table& t, int phase, uint32_t
   w = b - __builtin_amdgcn_readlane(mine, i);
   return t.e[i];
 }
+// The workgroup's number among all, counted XCD by XCD: neighbours, which read the same
+// matrix, share an L2.
+__device__ __forceinline__ uint32_t neighbours() {
+  const uint32_t x = blockIdx.x % 8, each = gridDim.x / 8, rem = gridDim.x % 8;
+  return x * each + min(x, rem) + blockIdx.x / 8;
+}
+// The long side of short sides beyond 32 goes in units of this many elements, of which a
+// workgroup takes an equal share; it may end inside one matrix and begin inside another.
+constexpr int UNIT = 128;
+__host__ __device__ inline uint32_t units_of(const Entry& e, int unit) {
+  return (uint32_t)(e.K + unit - 1) / unit;
+}
+// In gram the pairs of a block with itself come first, whose ten tiles of sixteen make
+// a unit of 192 elements cost as much (28 factors of rank 128: with units of 128 for both
+// 78 us, so 69).
+constexpr int SELF = 192;
+struct Pairs {
+  uint32_t nb, self, other, each;  // blocks, units of either kind of pair, of a matrix
+  __host__ __device__ explicit Pairs(const Entry& e)
+      : nb((uint32_t)(e.r + 63) / 64), self(units_of(e, SELF)), other(units_of(e, UNIT)),
+        each(nb * self + nb * (nb - 1) / 2 * other) {}
+  __host__ __device__ uint32_t many() const { return nb * (nb + 1) / 2; }
+  // pair p's first unit in its matrix
+  __host__ __device__ uint32_t begin(uint32_t p) const {
+    return p < nb ? p * self : nb * self + (p - nb) * other;
+  }
+  // pair p's blocks
+  __device__ void blocks(uint32_t p, int& I, int& J) const {
+    I = J = (int)p;
+    if (p < nb) return;
+    I = 0, J = (int)(p - nb);  // (0,1..nb-1), (1,2..nb-1), ...
+    while (J >= (int)nb - 1 - I) J -= (int)nb - 1 - I, ++I;
+    J += I + 1;
+  }
+};
 
 // Pointers that were read from memory, said to be ones to device memory: otherwise
 // their loads are flat ones, which are counted as LDS reads too and waited for with them.
@@ -99,13 +146,17 @@ __device__ __forceinline__ void load_upto4(const void* p, int64_t i, int n, bool
   for (int e = 0; e < 4; ++e) f[e] = e < n ? load1<BF>(p, i + e) : 0.0f;
 }
 template <bool BF>
+__device__ __forceinline__ void store4(void* p, int64_t i, const float* f) {
+  if constexpr (BF)
+    *(GLOBAL(u32x2)*)((uint16_t*)p + i) =
+        u32x2{st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3])};
+  else
+    *(GLOBAL(f32x4)*)((float*)p + i) = f32x4{f[0], f[1], f[2], f[3]};
+}
+template <bool BF>
 __device__ __forceinline__ void store_upto4(void* p, int64_t i, int n, bool vec, const float* f) {
   if (vec && n >= 4) {
-    if constexpr (BF)
-      *(GLOBAL(u32x2)*)((uint16_t*)p + i) =
-          u32x2{st::pack_bf16x2(f[0], f[1]), st::pack_bf16x2(f[2], f[3])};
-    else
-      *(GLOBAL(f32x4)*)((float*)p + i) = f32x4{f[0], f[1], f[2], f[3]};
+    store4<BF>(p, i, f);
     return;
   }
 #pragma unroll
@@ -127,9 +178,9 @@ __device__ __forceinline__ void store_upto4(void* p, int64_t i, int n, bool vec,
 // them, as long as both operands agree.
 //
 // FULL: all 32 are inside and may be read four at a time.  Then there is no branch
-// around a load (rows past the short side read the last one and are cleared), which
-// would make the wave wait for it at the branch's end; the elements that follow are
-// under way while the present ones are multiplied.
+// around a load, which would make the wave wait for it at the branch's end; the elements
+// that follow are under way while the present ones are multiplied.  Rows past the short
+// side read the last one; their sums are cleared.
 template <bool BF, int T, bool TALL, bool FULL>
 __device__ __forceinline__ void gram_rows(const Entry& e, const void* x, int row0, int64_t k0,
                                           int64_t kend, int lane, float (&u)[T][8]) {
@@ -158,14 +209,6 @@ __device__ __forceinline__ void gram_rows(const Entry& e, const void* x, int row
     }
   }
 }
-template <int T>
-__device__ __forceinline__ void clear_rows(const Entry& e, int row0, int lane, float (&u)[T][8]) {
-#pragma unroll
-  for (int t = 0; t < T; ++t)
-#pragma unroll
-    for (int s = 0; s < 8; ++s) u[t][s] = row0 + 16 * t + (lane & 15) < e.r ? u[t][s] : 0.0f;
-}
-
 // acc[i][j] += rows rowa + 16 i times rows rowb + 16 j over k0, k0 + step, .. < k1;
 // SAME: the two are one, and the tiles below the diagonal stay out.
 template <bool BF, int TA, int TB, bool TALL, bool SAME>
@@ -173,8 +216,6 @@ __device__ __forceinline__ void gram_walk(const Entry& e, const void* x, int row
                                           int64_t k0, int64_t k1, int step, int lane,
                                           d4 (&acc)[TA][TB]) {
   auto multiply = [&](float (&a)[TA][8], float (&b)[TB][8]) {
-    clear_rows<TA>(e, rowa, lane, a);
-    if constexpr (!SAME) clear_rows<TB>(e, rowb, lane, b);
 #pragma unroll
     for (int s = 0; s < 8; ++s)
 #pragma unroll
@@ -182,8 +223,7 @@ __device__ __forceinline__ void gram_walk(const Entry& e, const void* x, int row
 #pragma unroll
         for (int j = SAME ? i : 0; j < TB; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(
-              (double)a[i][s], SAME ? (double)a[j < TA ? j : 0][s] : (double)b[j][s], acc[i][j], 0, 0,
-              0);
+              (double)a[i][s], (double)(SAME ? a[j < TA ? j : 0][s] : b[j][s]), acc[i][j], 0, 0, 0);
   };
   float a[TA][8], b[TB][8], na[TA][8], nb[TB][8];
   if (e.vec || TALL) {
@@ -211,21 +251,30 @@ __device__ __forceinline__ void gram_walk(const Entry& e, const void* x, int row
     multiply(a, b);
   }
 }
+// A sum of the Gram matrix, or 0 past the short side.
+__device__ __forceinline__ double inside(const Entry& e, double sum, int row, int col) {
+  return row < e.r && col < e.r ? sum : 0.0;
+}
 // One wave's tiles of a block of 4 x 4, from tile (ti, tj) on, over a chunk.
 template <bool BF, int TA, int TB, bool SAME>
 __device__ __forceinline__ void gram_tiles(const Entry& e, const void* x, int rowI, int rowJ, int ti,
                                            int tj, int64_t k0, int64_t k1, int lane, double* to) {
   d4 acc[TA][TB] = {};
-  if (e.tall)
-    gram_walk<BF, TA, TB, true, SAME>(e, x, rowI + 16 * ti, rowJ + 16 * tj, k0, k1, 32, lane, acc);
-  else
-    gram_walk<BF, TA, TB, false, SAME>(e, x, rowI + 16 * ti, rowJ + 16 * tj, k0, k1, 32, lane, acc);
+  rowI += 16 * ti, rowJ += 16 * tj;
+  if (rowI < e.r && rowJ < e.r) {  // (zeros past the short side are read, too)
+    if (e.tall)
+      gram_walk<BF, TA, TB, true, SAME>(e, x, rowI, rowJ, k0, k1, 32, lane, acc);
+    else
+      gram_walk<BF, TA, TB, false, SAME>(e, x, rowI, rowJ, k0, k1, 32, lane, acc);
+  }
 #pragma unroll
   for (int i = 0; i < TA; ++i)
 #pragma unroll
     for (int j = SAME ? i : 0; j < TB; ++j)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) to[((ti + i) * 4 + tj + j) * 256 + v * 64 + lane] = acc[i][j][v];
+      for (int v = 0; v < 4; ++v)
+        to[((ti + i) * 4 + tj + j) * 256 + v * 64 + lane] =
+            inside(e, acc[i][j][v], rowI + 16 * i + 4 * v + (lane >> 4), rowJ + 16 * j + (lane & 15));
 }
 
 template <int T, bool BF>
@@ -236,33 +285,50 @@ __global__ __launch_bounds__(NTH) void gram(Table tab, double* __restrict__ part
     for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += NTH)
       copy[i] = ((const uint32_t*)&tab)[i];
   }
-  uint32_t w;
-  const Entry& e = find(tab, IN_GRAM, blockIdx.x, w);
-  const int nb = T < 4 ? 1 : (e.r + 63) / 64, pairs = nb * (nb + 1) / 2;
-  const int pair = (int)(w % pairs);
-  const uint32_t mc = w / pairs;  // matrix * chunks + chunk
-  const int64_t mat = mc / e.chunks, chunk = mc % e.chunks;
-  int I = 0, J = pair;  // pairs row by row: (0,0..nb-1), (1,1..nb-1), ...
-  while (J >= nb - I) J -= nb - I, ++I;
-  J += I;
-  const void* x = (const char*)e.x + mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t k0 = chunk * e.CH, k1 = k0 + e.CH < e.K ? k0 + e.CH : e.K;
-  double* to = part + e.part + ((int64_t)mc * pairs + pair) * (T * T * 256);
+  uint32_t w;
   if constexpr (T == 4) {
-    // Each wave a quarter of the block, two tiles by two, over the whole chunk: 32
-    // registers of sums leave room for more waves, and for the elements under way.  Of
-    // a block on the diagonal, two waves take its two ends (three tiles each) and two
-    // the rest, so that no SIMD has four tiles while another has none.
-    if (I != J)
-      gram_tiles<BF, 2, 2, false>(e, x, I * 64, J * 64, wave >> 1 << 1, (wave & 1) << 1, k0, k1, lane,
-                                  to);
-    else if (wave < 2)
-      gram_tiles<BF, 2, 2, true>(e, x, I * 64, I * 64, 2 * wave, 2 * wave, k0, k1, lane, to);
-    else
-      gram_tiles<BF, 1, 2, false>(e, x, I * 64, I * 64, wave - 2, 2, k0, k1, lane, to);
+    // a unit is 128 long elements of a block pair; the sums of a workgroup's units of
+    // one pair go to the place numbered by both
+    const uint32_t b = neighbours(), end = tab.gram.begin(b + 1);
+    for (uint32_t u = tab.gram.begin(b); u < end;) {
+      const Entry& e = find(tab, IN_GRAM, u, w);
+      const Pairs pairs(e);
+      const uint32_t mat = w / pairs.each, in = w % pairs.each, selves = pairs.nb * pairs.self;
+      const uint32_t pair = in < selves ? in / pairs.self : pairs.nb + (in - selves) / pairs.other;
+      const uint32_t first = in - pairs.begin(pair);
+      const uint32_t many = min((pair < pairs.nb ? pairs.self : pairs.other) - first, end - u);
+      const int unit = pair < pairs.nb ? SELF : UNIT;
+      u += many;
+      int I, J;
+      pairs.blocks(pair, I, J);
+      const void* x = (const char*)e.x + mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
+      const int64_t k0 = (int64_t)first * unit, k1 = min(k0 + (int64_t)many * unit, (int64_t)e.K);
+      double* to = part + e.part + ((int64_t)mat * pairs.many() + pair + b) * 4096;
+      // what a lane reads is worked out here, each time: kept over the loop, the three
+      // forms' addresses below would take the third wave's registers
+      int mine = lane;
+      asm volatile("" : "+v"(mine));
+      // Each wave a quarter of the block, two tiles by two: 32 registers of sums leave
+      // room for more waves, and for the elements under way.  Of a block with itself,
+      // two waves take its two ends (three tiles each) and two the rest, other waves in
+      // every other block.
+      const int as = wave ^ (pair & 1 ? 2 : 0);
+      if (I != J)
+        gram_tiles<BF, 2, 2, false>(e, x, I * 64, J * 64, wave >> 1 << 1, (wave & 1) << 1, k0, k1,
+                                    mine, to);
+      else if (as < 2)
+        gram_tiles<BF, 2, 2, true>(e, x, I * 64, I * 64, 2 * as, 2 * as, k0, k1, mine, to);
+      else
+        gram_tiles<BF, 1, 2, false>(e, x, I * 64, I * 64, as - 2, 2, k0, k1, mine, to);
+    }
   } else {
+    const Entry& e = find(tab, IN_GRAM, blockIdx.x, w);
+    const int64_t mat = w / e.chunks, chunk = w % e.chunks;
+    const void* x = (const char*)e.x + mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
+    const int64_t k0 = chunk * e.CH, k1 = k0 + e.CH < e.K ? k0 + e.CH : e.K;
+    double* to = part + e.part + (int64_t)w * (T * T * 256);
     d4 acc[T][T] = {};
     if (e.tall)
       gram_walk<BF, T, T, true, true>(e, x, 0, 0, k0 + 32 * wave, k1, 128, lane, acc);
@@ -283,8 +349,11 @@ __global__ __launch_bounds__(NTH) void gram(Table tab, double* __restrict__ part
       }
       __syncthreads();
     }
-    for (int i = threadIdx.x; i < T * T * 256; i += NTH)
-      if (i / 256 / T <= i / 256 % T) to[i] = sum[i];
+    for (int i = threadIdx.x; i < T * T * 256; i += NTH) {
+      const int row = i / 256 / T, col = i / 256 % T;
+      if (row <= col)
+        to[i] = inside(e, sum[i], 16 * row + i % 256 / 16, 16 * col + i % 16);
+    }
   }
 }
 
@@ -305,7 +374,7 @@ __device__ __forceinline__ double gram_at(const double* part, int nb, int row, i
 // One wave holds everything in registers: register v of lane (m, q) is element
 // [4v + q][m], which is what a product wants of either operand, so a product of two
 // symmetric matrices is four instructions on the registers they lie in.  Two sums
-// each, as an instruction waits 75 ns for the sum before it.
+// each, as an instruction waits 27 ns for the sum before it.
 __device__ __forceinline__ d4 product16(d4 a, d4 b) {
   d4 x = {0.0, 0.0, 0.0, 0.0}, y = x;
   x = __builtin_amdgcn_mfma_f64_16x16x4f64(a[0], b[0], x, 0, 0, 0);
@@ -348,7 +417,8 @@ __device__ __forceinline__ d4 steps16(const Table& tab, d4 g, double* turn, int 
   return P;
 }
 
-__global__ __launch_bounds__(64) void poly16(const Table* __restrict__ table, const double* __restrict__ part,
+__global__ __launch_bounds__(64) void poly16(const Table* __restrict__ table,
+                                             const double* __restrict__ part,
                                              double* __restrict__ poly) {
   __shared__ double turn[16 * 17];
   const Table& tab = *table;
@@ -385,7 +455,8 @@ __device__ __forceinline__ d4 product_tile(const double* A, const double* B, int
 }
 
 template <int T>
-__global__ __launch_bounds__(NTH) void poly_small(const Table* __restrict__ table, const double* __restrict__ part,
+__global__ __launch_bounds__(NTH) void poly_small(const Table* __restrict__ table,
+                                                  const double* __restrict__ part,
                                                   double* __restrict__ poly) {
   constexpr int R = 16 * T, N = R * R, OWN = T * T / 4;  // tiles of a wave
   __shared__ double G[N], Q[N], P[N];
@@ -472,26 +543,38 @@ __global__ __launch_bounds__(NTH) void poly_small(const Table* __restrict__ tabl
 // in turn) and H = Q G.
 enum { SLOT_G, SLOT_Q, SLOT_P0, SLOT_P1, SLOT_H, SLOTS };
 
-// The chunks' sums joined into the first chunk's place.
-__global__ __launch_bounds__(NTH) void poly_sum(const Table* __restrict__ table, double* __restrict__ part) {
+// The workgroups' sums of a block pair joined, in their order, in the place of H.
+__global__ __launch_bounds__(NTH) void poly_sum(const Table* __restrict__ table,
+                                                const double* __restrict__ part,
+                                                double* __restrict__ poly) {
   const Table& tab = *table;
-  uint32_t w;
+  uint32_t w, at;
   const Entry& e = find(tab, IN_SUM, blockIdx.x, w);
-  const int nb = (e.r + 63) / 64, pairs = nb * (nb + 1) / 2;
-  const uint32_t per = pairs * 4096 / (2 * NTH);
-  double2* p = (double2*)(part + e.part + (int64_t)(w / per) * e.chunks * pairs * 4096) +
-               (w % per) * NTH + threadIdx.x;
+  const Pairs pairs(e);
+  const uint32_t combo = w / 8, piece = w % 8, mat = combo / pairs.many();
+  const uint32_t pair = combo % pairs.many(), R = 64 * pairs.nb;
+  int I, J;
+  pairs.blocks(pair, I, J);
+  const uint32_t u0 = tab.tile0[IN_GRAM][&e - tab.e] + mat * pairs.each + pairs.begin(pair);
+  const uint32_t b0 = tab.gram.owner(u0);
+  const uint32_t many =
+      tab.gram.owner(u0 + (pair < pairs.nb ? pairs.self : pairs.other) - 1) - b0 + 1;
+  at = piece * NTH + threadIdx.x;
+  const double2* p = (const double2*)(part + e.part + ((int64_t)combo + b0) * 4096) + at;
   double2 s = make_double2(0.0, 0.0);
 #pragma unroll 4
-  for (int c = 0; c < e.chunks; ++c) {
-    const double2 x = p[(int64_t)c * pairs * 2048];
+  for (uint32_t c = 0; c < many; ++c) {
+    const double2 x = p[(int64_t)c * 2048];
     s.x += x.x, s.y += x.y;
   }
-  *p = s;
+  // (gram_at counts the pairs row by row)
+  const int64_t place = I * pairs.nb - I * (I - 1) / 2 + J - I;
+  double* to = poly + e.poly + ((int64_t)mat * SLOTS + SLOT_H) * R * R;
+  ((double2*)(to + place * 4096))[at] = s;
 }
 
 // G = U U' / (|U|_F + eps)^2 and P = I / (|U|_F + eps), from the joined sums.
-__global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table, const double* __restrict__ part,
+__global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table,
                                                  double* __restrict__ poly) {
   __shared__ double red[NTH / 64];
   const Table& tab = *table;
@@ -499,8 +582,8 @@ __global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table
   const Entry& e = find(tab, IN_NORM, blockIdx.x, w);
   const int nb = (e.r + 63) / 64, R = 64 * nb;
   const uint32_t per = (uint32_t)R * R / 1024;
-  const double* mine = part + e.part + (int64_t)(w / per) * e.chunks * (nb * (nb + 1) / 2) * 4096;
   double* base = poly + e.poly + (int64_t)(w / per) * SLOTS * R * R;
+  const double* mine = base + (int64_t)SLOT_H * R * R;
   double trace = 0.0;
   for (int i = threadIdx.x; i < e.r; i += NTH) trace += gram_at(mine, nb, i, i);
 #pragma unroll
@@ -520,10 +603,11 @@ __global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table
 // and forms 16 rows of the next G and P by themselves,
 //   H = aG + b GG + c GGG,  G' = aH + b HG + c HGG,  P' = aP + b PG + c PGG,
 // each product those rows times G.  That is six products of 16 rows in the place of
-// four of all, but nothing waits for another workgroup within a step: 25 us at 28
-// matrices of 128 (10 us of products, the rest G's way into LDS and the barriers) where
-// the three launches of the tiles below took 33.  (G' as one polynomial of G, whose
-// coefficients reach 37, lost two more digits.)
+// four of all, but nothing waits for another workgroup within a step: 21 us at 28
+// matrices of 128 (10 us of products, the rest G's way into LDS and the barriers; 25
+// with a matrix's workgroups on all XCDs) where the three launches of the tiles below
+// took 33.  (G' as one polynomial of G, whose coefficients reach 37, lost two more
+// digits.)
 // Wave j forms columns 16 j..; the rows that are multiplied next stand transposed in
 // LDS, rows of 17 doubles.  G' is written from its upper half to both places.
 template <int R>
@@ -533,7 +617,7 @@ __global__ __launch_bounds__(4 * R) void poly_panel(const Table* __restrict__ ta
   __shared__ double T[R * 17];
   const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, IN_POLY, blockIdx.x, w);
+  const Entry& e = find(tab, IN_POLY, neighbours(), w);
   const int I = (int)(w % (R / 16));
   double* base = poly + e.poly + (int64_t)(w / (R / 16)) * SLOTS * R * R;
   const double* Gold = base + (int64_t)(turn ? SLOT_Q : SLOT_G) * R * R;
@@ -691,19 +775,19 @@ __device__ __forceinline__ void apply_rows(const Entry& e, const void* x, int ro
     }
   }
 }
-// acc[i][c] += of one tile of 16 short elements from row0 on: Ps is P's block, its
-// rows k0.. taken, N tiles of its columns from col0 on.
+// acc[i][c] += of one tile of 16 short elements: Ps is P's block, its rows k0.. taken, N
+// tiles of its columns from col0 on.  Past the short side P is zero off its diagonal, and
+// U's place holds others of its elements.
 template <int N, bool TALL>
-__device__ __forceinline__ void apply_tile(const Entry& e, const double* Ps, int ld, int row0,
-                                           int k0, int col0, int m, int q, const float (&u)[4][4],
-                                           d4 (&acc)[N][4]) {
+__device__ __forceinline__ void apply_tile(const double* Ps, int ld, int k0, int col0, int m, int q,
+                                           const float (&u)[4][4], d4 (&acc)[N][4]) {
   const int prow = TALL ? 4 * (m & 3) + (m >> 2) : m;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const int k = TALL ? 4 * q + t : 4 * t + q;
     double b[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) b[c] = row0 + k < e.r ? (double)(TALL ? u[c][t] : u[t][c]) : 0.0;
+    for (int c = 0; c < 4; ++c) b[c] = (double)(TALL ? u[c][t] : u[t][c]);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const double a = Ps[(k0 + k) * ld + col0 + 16 * i + prow];
@@ -713,7 +797,7 @@ __device__ __forceinline__ void apply_tile(const Entry& e, const double* Ps, int
     }
   }
 }
-template <int N, bool BF, bool TALL>
+template <int N, bool BF, bool TALL, bool FULL>
 __device__ __forceinline__ void apply_store(const Entry& e, void* out, int row0, int64_t k0,
                                             int64_t l1, int m, int q, const d4 (&acc)[N][4]) {
 #pragma unroll
@@ -726,14 +810,23 @@ __device__ __forceinline__ void apply_store(const Entry& e, void* out, int row0,
       if constexpr (TALL) {
         const int64_t k = k0 + 16 * s + m;
         const int row = row0 + 16 * i + 4 * q;
-        store_upto4<BF>(out, k * e.r + row, k < l1 ? e.r - row : 0, e.vec, f);
+        if constexpr (!FULL)
+          store_upto4<BF>(out, k * e.r + row, k < l1 ? e.r - row : 0, e.vec, f);
+        else if (row < e.r)
+          store4<BF>(out, k * e.r + row, f);
       } else {
         const int row = row0 + 16 * i + 4 * s + q;
         const int64_t k = k0 + 4 * m, left = row < e.r ? l1 - k : 0;
-        store_upto4<BF>(out, (int64_t)row * e.K + k, (int)(left < 4 ? left : 4), e.vec, f);
+        if constexpr (!FULL)
+          store_upto4<BF>(out, (int64_t)row * e.K + k, (int)(left < 4 ? left : 4), e.vec, f);
+        else if (row < e.r)
+          store4<BF>(out, (int64_t)row * e.K + k, f);
       }
     }
 }
+
+// (Entries are copied: read where they are used, behind a store, they would be vector
+// loads, and waiting for those waits for the tiles under way.)
 
 // Short sides of one block, 16 T: a workgroup takes e.AL long elements, a wave every
 // fourth 64 of them, its next ones on their way while the present ones are multiplied.
@@ -764,8 +857,8 @@ __device__ __forceinline__ void apply_walk(const Entry& e, const void* x, void* 
       d4 acc[T][4] = {};
 #pragma unroll
       for (int t = 0; t < T; ++t)
-        apply_tile<T, TALL>(e, Ps, R, 16 * t, 16 * t, 0, m, q, u[t], acc);
-      apply_store<T, BF, TALL>(e, out, 0, k0, l1, m, q, acc);
+        apply_tile<T, TALL>(Ps, R, 16 * t, 0, m, q, u[t], acc);
+      apply_store<T, BF, TALL, true>(e, out, 0, k0, l1, m, q, acc);
     }
   }
   for (; k0 < l1; k0 += 256) {
@@ -773,19 +866,20 @@ __device__ __forceinline__ void apply_walk(const Entry& e, const void* x, void* 
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       apply_rows<BF, TALL, false>(e, x, 16 * t, k0, l1, m, q, u[t]);
-      apply_tile<T, TALL>(e, Ps, R, 16 * t, 16 * t, 0, m, q, u[t], acc);
+      apply_tile<T, TALL>(Ps, R, 16 * t, 0, m, q, u[t], acc);
     }
-    apply_store<T, BF, TALL>(e, out, 0, k0, l1, m, q, acc);
+    apply_store<T, BF, TALL, false>(e, out, 0, k0, l1, m, q, acc);
   }
 }
 
 template <int T, bool BF>
-__global__ __launch_bounds__(NTH) void apply(const Table* __restrict__ table, const double* __restrict__ poly) {
+__global__ __launch_bounds__(NTH) void apply(const Table* __restrict__ table,
+                                             const double* __restrict__ poly) {
   constexpr int R = 16 * T;
   __shared__ double Ps[R * R];
   const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, IN_APPLY, blockIdx.x, w);
+  const Entry e = find(tab, IN_APPLY, blockIdx.x, w);
   const uint32_t tiles = (uint32_t)((e.K + e.AL - 1) / e.AL);
   const int64_t mat = w / tiles, l0 = (int64_t)(w % tiles) * e.AL;
   const int64_t l1 = l0 + e.AL < e.K ? l0 + e.AL : e.K;
@@ -801,14 +895,16 @@ __global__ __launch_bounds__(NTH) void apply(const Table* __restrict__ table, co
     apply_walk<T, BF, false>(e, x, out, P, Ps, l0 + 64 * wave, l1, lane & 15, lane >> 4);
 }
 
-// Short sides of blocks of 64: a workgroup takes e.AL long elements of one block, 128
-// at a time, a wave half of the block's rows and 64 of them.  P's blocks stay in LDS
-// where there are at most two.
+// Short sides of blocks of 64: a workgroup takes its share of units of 128 long elements
+// of one block, a unit at a time, a wave half of the block's rows and 64 of them.  P's
+// blocks stay in LDS where there are at most two.  The tile of U that follows, be it of
+// the next unit, is on its way while the present one is multiplied.
 template <bool BF, bool TALL>
 __device__ __forceinline__ void apply64_walk(const Entry& e, const void* x, void* out,
                                              const double* P, double* Pall, int nb, int I,
                                              int64_t l0, int64_t l1, int wave, int m, int q) {
-  const int R = 64 * nb, wi = wave & 1, wl = wave >> 1;
+  const int R = 64 * nb, wi = wave & 1, wl = wave >> 1, rows = I * 64 + 32 * wi;
+  const bool idle = rows >= e.r;  // (of the last block; the others wait for it below)
   auto fill = [&](double* Ps, int kb) {
     d2 in[8];
     const d2* from = (const d2*)(P + (int64_t)(kb * 64 + threadIdx.x / 32) * R + I * 64) +
@@ -818,17 +914,22 @@ __device__ __forceinline__ void apply64_walk(const Entry& e, const void* x, void
 #pragma unroll
     for (int i = 0; i < 8; ++i) ((d2*)Ps)[threadIdx.x + 256 * i] = in[i];
   };
+  int64_t k0 = l0 + 64 * wl;  // a wave past the end loads nothing and stores nothing
+  const bool fast = e.vec && k0 + 64 <= l1;
+  float next[4][4];
+  if (fast) apply_rows<BF, TALL, true>(e, x, 0, k0, l1, m, q, next);
+  __syncthreads();  // P's places are free again
   if (nb <= 2) {
     fill(Pall, 0);
     if (nb == 2) fill(Pall + 4096, 1);
     __syncthreads();
   }
-  for (int64_t step = l0; step < l1; step += 128) {
-    const int64_t k0 = step + 64 * wl;  // a wave past the end loads nothing and stores nothing
-    const bool fast = e.vec && k0 + 64 <= l1;
+  // one unit; the two kinds of loads in loops of their own: where they meet, the wave
+  // waits for the loads under way (28 factors of rank 128: 124 us, so 103)
+  auto unit = [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    const int64_t kn = k0 + UNIT + 64 <= l1 ? k0 + UNIT : k0;
     d4 acc[2][4] = {};
-    float u[4][4], next[4][4];
-    if (fast) apply_rows<BF, TALL, true>(e, x, 0, k0, l1, m, q, next);
     for (int kb = 0; kb < nb; ++kb) {
       double* Ps = Pall + (nb <= 2 ? kb : 0) * 4096;
       if (nb > 2) {
@@ -836,53 +937,59 @@ __device__ __forceinline__ void apply64_walk(const Entry& e, const void* x, void
         fill(Ps, kb);
         __syncthreads();
       }
-      if (fast) {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          const int row = kb * 64 + 16 * kt;
+      if (idle) continue;
+      const int stop = min(e.r, kb * 64 + 64);
+#pragma unroll 1
+      for (int row = kb * 64; row < stop; row += 16) {
+        float u[4][4];
+        if constexpr (FULL) {
+          const bool end = row + 16 >= e.r;
 #pragma unroll
           for (int a = 0; a < 4; ++a)
 #pragma unroll
             for (int b = 0; b < 4; ++b) u[a][b] = next[a][b];
-          apply_rows<BF, TALL, true>(e, x, row + 16, k0, l1, m, q, next);
-          apply_tile<2, TALL>(e, Ps, 64, row, 16 * kt, 32 * wi, m, q, u, acc);
-        }
-      } else {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          const int row = kb * 64 + 16 * kt;
+          apply_rows<BF, TALL, true>(e, x, end ? 0 : row + 16, end ? kn : k0, l1, m, q, next);
+        } else {
           apply_rows<BF, TALL, false>(e, x, row, k0, l1, m, q, u);
-          apply_tile<2, TALL>(e, Ps, 64, row, 16 * kt, 32 * wi, m, q, u, acc);
         }
+        apply_tile<2, TALL>(Ps, 64, row % 64, 32 * wi, m, q, u, acc);
       }
     }
-    apply_store<2, BF, TALL>(e, out, I * 64 + 32 * wi, k0, l1, m, q, acc);
-  }
+    if (!idle) apply_store<2, BF, TALL, FULL>(e, out, rows, k0, l1, m, q, acc);
+    k0 += UNIT;
+  };
+  int64_t step = l0;
+  if (fast)
+    for (; step < l1 && k0 + 64 <= l1; step += UNIT) unit(std::true_type());
+  for (; step < l1; step += UNIT) unit(std::false_type());
 }
 
 template <bool BF>
-__global__ __launch_bounds__(NTH) void apply64(const Table* __restrict__ table, int last, const double* __restrict__ poly) {
+__global__ __launch_bounds__(NTH) void apply64(const Table* __restrict__ table, int last,
+                                               const double* __restrict__ poly) {
   __shared__ double Pall[2 * 4096];
   const Table& tab = *table;
-  uint32_t w;
-  const Entry& e = find(tab, IN_APPLY, blockIdx.x, w);
-  const int nb = (e.r + 63) / 64, R = 64 * nb;
-  const uint32_t tiles = (uint32_t)((e.K + e.AL - 1) / e.AL);
-  const int I = (int)(w % nb);
-  const uint32_t mt = w / nb;
-  const int64_t mat = mt / tiles, l0 = (int64_t)(mt % tiles) * e.AL;
-  const int64_t l1 = l0 + e.AL < e.K ? l0 + e.AL : e.K;
-  const int64_t off = mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
-  const void* x = (const char*)e.x + off;
-  void* out = (char*)e.out + off;
-  const double* P = poly + e.poly;
-  P += (mat * SLOTS + (last ? SLOT_P1 : SLOT_P0)) * R * R;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (e.tall)
-    apply64_walk<BF, true>(e, x, out, P, Pall, nb, I, l0, l1, wave, lane & 15, lane >> 4);
-  else
-    apply64_walk<BF, false>(e, x, out, P, Pall, nb, I, l0, l1, wave, lane & 15, lane >> 4);
+  const uint32_t b = neighbours(), end = tab.apply.begin(b + 1);
+  for (uint32_t at = tab.apply.begin(b); at < end;) {
+    uint32_t w;
+    const Entry e = find(tab, IN_APPLY, at, w);
+    const uint32_t units = units_of(e, UNIT), mb = w / units, first = w % units;
+    const uint32_t many = min(units - first, end - at);
+    at += many;
+    const int nb = (e.r + 63) / 64, R = 64 * nb, I = (int)(mb % nb);
+    const int64_t mat = mb / nb, l0 = (int64_t)first * UNIT;
+    const int64_t l1 = min(l0 + (int64_t)many * UNIT, (int64_t)e.K);
+    const int64_t off = mat * e.r * (int64_t)e.K * (BF ? 2 : 4);
+    const void* x = (const char*)e.x + off;
+    void* out = (char*)e.out + off;
+    const double* P = poly + e.poly + (mat * SLOTS + (last ? SLOT_P1 : SLOT_P0)) * R * R;
+    if (e.tall)
+      apply64_walk<BF, true>(e, x, out, P, Pall, nb, I, l0, l1, wave, lane & 15, lane >> 4);
+    else
+      apply64_walk<BF, false>(e, x, out, P, Pall, nb, I, l0, l1, wave, lane & 15, lane >> 4);
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -897,18 +1004,16 @@ struct Plan {  // one table's launches
 int64_t piece(int64_t K, int64_t most, int64_t unit) {
   return st::cdiv(st::cdiv(K, st::cdiv(K, most)), unit) * unit;
 }
-// Long elements of a workgroup: the length whose rounds of `slots` workgroups at a time
-// take least, each as long as its longest piece and `start` elements more.  (28 factors
-// of rank 128: 648 workgroups of 512 elements on 512 places wait for a second round and
-// take 134 us, 460 of 768 take 122.)
-template <typename F>
-int64_t pick(const Plan& p, int64_t unit, int64_t slots, int64_t start, F blocks) {
+// Long elements of a workgroup at short sides up to 32: the length whose rounds of
+// `slots` workgroups at a time take least, each as long as its longest piece and `start`
+// elements more.
+int64_t pick(const Plan& p, int64_t unit, int64_t slots, int64_t start) {
   int64_t best = unit, least = INT64_MAX;
   for (const int k : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24}) {
     int64_t n = 0, longest = 0;
     for (int i = 0; i < p.tab.n; ++i) {
       const int64_t K = p.tab.e[i].K, l = piece(K, k * unit, unit);
-      n += p.count[i] * blocks(p.tab.e[i]) * st::cdiv(K, l);
+      n += p.count[i] * st::cdiv(K, l);
       longest = l > longest ? l : longest;
     }
     const int64_t cost = st::cdiv(n, slots) * (longest + start);
@@ -916,6 +1021,13 @@ int64_t pick(const Plan& p, int64_t unit, int64_t slots, int64_t start, F blocks
     if (n <= slots) break;  // one round: longer ones only take longer
   }
   return best;
+}
+
+// Workgroups of gram and apply64 at short sides beyond 32: two a CU run at once.
+constexpr int64_t GRAM_WGS = 512, APPLY_WGS = 512;
+Shares shares(int64_t units, int64_t wgs) {
+  if (wgs > units) wgs = units;
+  return {(uint32_t)wgs, (uint32_t)(units / wgs), (uint32_t)(units % wgs)};
 }
 
 // The next table: entries from `at` on whose short sides are of one class (up to 16, 32,
@@ -940,22 +1052,27 @@ int make_plan(const st_matrix_batch* in, int32_t n, int32_t at, int32_t dtype, P
     e.vec = (e.tall ? r : K) % 4 == 0 && (((uintptr_t)b.x | (uintptr_t)b.out) & mask) == 0;
     p.count[t.n++] = b.count;
   }
-  auto nb = [&](const Entry& e) { return ((int64_t)e.r + 16 * p.T - 1) / (16 * p.T); };
-  auto pairs = [&](const Entry& e) { return nb(e) * (nb(e) + 1) / 2; };
   // places: 256 CUs and as many workgroups each as the kernels' registers and LDS allow
-  const int64_t ch = p.T == 4 ? pick(p, 128, 768, 192, pairs)
-                              : pick(p, 128, p.T == 1 ? 2048 : 1280, 256, pairs);
-  const int64_t al = p.T == 4 ? pick(p, 128, 512, 64, nb)
-                              : pick(p, 256, p.T == 1 ? 1280 : 512, 256, nb);
+  const int64_t ch = p.T == 4 ? 0 : pick(p, 128, p.T == 1 ? 2048 : 1280, 256);
+  const int64_t al = p.T == 4 ? 0 : pick(p, 256, p.T == 1 ? 1280 : 512, 256);
+  int64_t combos = 0;  // block pairs of matrices
   for (int i = 0; i < t.n; ++i) {
     Entry& e = t.e[i];
-    e.CH = (int32_t)piece(e.K, ch, 128), e.AL = (int32_t)piece(e.K, al, p.T == 4 ? 128 : 256);
-    e.chunks = (int32_t)st::cdiv(e.K, e.CH);
-    e.part = p.part, e.poly = p.poly;
-    p.part += p.count[i] * e.chunks * pairs(e) * p.T * p.T * 256;
-    const int64_t R = 16 * p.T * nb(e);
-    p.poly += p.count[i] * R * R * (p.T == 4 ? SLOTS : 1);
+    e.poly = p.poly;
+    if (p.T == 4) {
+      const int64_t nb = st::cdiv(e.r, 64);
+      e.part = 4096 * combos;
+      combos += p.count[i] * nb * (nb + 1) / 2;
+      p.poly += p.count[i] * SLOTS * 4096 * nb * nb;
+    } else {
+      e.CH = (int32_t)piece(e.K, ch, 128), e.AL = (int32_t)piece(e.K, al, 256);
+      e.chunks = (int32_t)st::cdiv(e.K, e.CH);
+      e.part = p.part;
+      p.part += p.count[i] * e.chunks * p.T * p.T * 256;
+      p.poly += p.count[i] * p.T * p.T * 256;
+    }
   }
+  if (p.T == 4 && t.n) p.part = 4096 * (combos + GRAM_WGS);
   return taken;
 }
 
@@ -976,10 +1093,10 @@ constexpr int64_t TABLE_BYTES = (sizeof(Table) + 15) / 16 * 16;
 
 template <int T, bool BF>
 int launch(Plan& p, char* workspace, hipStream_t stream) {
-  auto blocks = [](const Entry& e) { return T < 4 ? (int64_t)1 : ((int64_t)e.r + 63) / 64; };
+  auto blocks = [](const Entry& e) { return ((int64_t)e.r + 63) / 64; };
   const int nb = (int)blocks(p.tab.e[0]);  // 1, 2 or more for all entries
-  const int64_t ng = number(p, IN_GRAM, [&](const Entry& e) {
-    return e.chunks * blocks(e) * (blocks(e) + 1) / 2;
+  int64_t ng = number(p, IN_GRAM, [&](const Entry& e) {
+    return T < 4 ? (int64_t)e.chunks : (int64_t)Pairs(e).each;
   });
   const int64_t ns = number(p, IN_SUM, [&](const Entry& e) {
     return blocks(e) * (blocks(e) + 1) / 2 * 8;
@@ -988,11 +1105,15 @@ int launch(Plan& p, char* workspace, hipStream_t stream) {
   const int64_t np = number(p, IN_POLY, [&](const Entry& e) {
     return T < 4 ? (int64_t)1 : nb <= 2 ? (int64_t)4 * nb : blocks(e) * blocks(e) * 4;
   });
-  const int64_t na = number(p, IN_APPLY, [&](const Entry& e) {
-    return st::cdiv(e.K, e.AL) * blocks(e);
+  int64_t na = number(p, IN_APPLY, [&](const Entry& e) {
+    return T < 4 ? st::cdiv(e.K, e.AL) : st::cdiv(e.K, UNIT) * blocks(e);
   });
   if (ng < 0 || ns < 0 || nn < 0 || np < 0 || na < 0)
     return st::fail(ST_EUNSUPPORTED, "too many matrices for a launch: call with fewer at a time");
+  if (T == 4) {
+    p.tab.gram = shares(ng, GRAM_WGS), ng = p.tab.gram.wgs;
+    p.tab.apply = shares(na, APPLY_WGS), na = p.tab.apply.wgs;
+  }
   const Table* tab = (const Table*)workspace;
   double* part = (double*)(workspace + TABLE_BYTES);
   double* poly = part + p.part;
@@ -1003,8 +1124,8 @@ int launch(Plan& p, char* workspace, hipStream_t stream) {
   } else if constexpr (T == 2) {
     poly_small<T><<<(unsigned)np, NTH, 0, stream>>>(tab, part, poly);
   } else {
-    poly_sum<<<(unsigned)ns, NTH, 0, stream>>>(tab, part);
-    poly_norm<<<(unsigned)nn, NTH, 0, stream>>>(tab, part, poly);
+    poly_sum<<<(unsigned)ns, NTH, 0, stream>>>(tab, part, poly);
+    poly_norm<<<(unsigned)nn, NTH, 0, stream>>>(tab, poly);
     for (int s = 0; s < p.tab.steps; ++s, turn ^= 1) {
       const int more = s + 1 < p.tab.steps;
       if (nb == 1) {
