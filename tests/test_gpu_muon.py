@@ -92,6 +92,28 @@ def test_many_matrices_of_many_shapes_in_one_call():
     assert all(torch.equal(a, b) for a, b in zip(muon.orthogonalize(us), out))
 
 
+@pytest.mark.parametrize("shapes", [
+    [(70, 40, 300), (5, 700, 64), (64, 33), (2, 48, 4097)],       # short sides of one block
+    [(3, 128, 5000), (90, 200, 72), (100, 131), (5000, 96), (7, 127, 1001)],  # of two
+    [(2, 200, 3000), (3000, 150), (5, 129, 260), (193, 194)],     # of more
+    [(700, 64, 65), (4, 64, 2000)]])                              # more units than workgroups
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shares_that_end_inside_matrices(shapes, dtype):
+    us = [make(s, i, dtype) for i, s in enumerate(shapes)]
+    for u, o in zip(us, muon.orthogonalize(us)):
+        check(o, u)
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 300), (3, 300, 72), (3, 100, 1000), (3, 150, 400)])
+def test_one_matrix_that_is_not_finite_among_others(shape):
+    """Also in the last row of a short side that ends inside a tile."""
+    u = make(shape, 4)
+    u[1, -1, -1] = math.inf
+    out = muon.orthogonalize(u)
+    assert torch.isnan(out[1]).all()
+    check(out[::2], u[::2])
+
+
 def test_small_singular_values_keep_their_digits():
     """Directions 1e-5 of the largest: their squares are below 32 bits' resolution."""
     g = torch.Generator().manual_seed(1)
