@@ -17,8 +17,8 @@
 // result rounded once; normed comes from the unrounded h.
 //
 // Sums over rows (dpost, dpre, and dgate where a gate is shared by rows): a
-// workgroup walks a run of rows with the columns' sums in registers, and a second
-// kernel joins the runs in their order.
+// workgroup walks a run of rows with the columns' sums in registers or LDS, and a
+// second kernel joins the runs in their order.
 #include <cmath>
 
 #include "common.h"
@@ -260,20 +260,28 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
 
 // SUMS: run blockIdx.x of `per_run` rows (all of one gate row), columns' sums kept.
 // GATE: there is one.  Rows wait in registers as the bf16 they are (in fp32, fewer waves
-// fit), with SUMS the next one on its way while the present one is worked on.
-// Beyond 8192 columns (WIDE) a thread has no registers for that: it reads its chunks
-// again where it needs them, out of the caches, and two of the columns' sums lie in LDS
-// (2048 x 16384 with learnt norms and gate: 170 us, with all of it in registers 470).
+// fit).  The columns' sums of rows over more than one wave lie in LDS, each read and
+// written by its own thread alone: in registers they left a CU 8 to 12 waves in the place
+// of 16 (8192 x 4096 with learnt norms and gate 140 us, so 99; 2103 x 7168 66, 54).  Rows
+// of one wave keep them, and the next row is under way (30000 x 512: 42, in LDS 55).
+// Beyond 8192 columns (WIDE) a thread has no registers for its row either: it reads its
+// chunks again where it needs them, out of the caches (2048 x 16384: 170 us, with all of
+// it in registers 470).
 template <int VEC, int NT, int NV, bool SUMS, bool GATE, bool RAG>
-__global__ __launch_bounds__(NT) void norms_bwd(Args a) {
+__global__ __launch_bounds__(NT, SUMS && NT > 64 && NV == 1 ? 4 : 1) void norms_bwd(Args a) {
   __shared__ float red[3][NT / 64];
-  constexpr bool WIDE = NT * NV * VEC > 8192, LDS = SUMS && WIDE, EARLY = SUMS && !WIDE;
-  __shared__ f32x4 kept[LDS ? 2 * NV * VEC / 4 * NT : 1];  // dpost and dpre, a thread's own
+  constexpr bool WIDE = NT * NV * VEC > 8192, LDS = SUMS && NT > 64, EARLY = SUMS && !LDS;
+  // dpost, dpre and, where there is room, dgate
+  constexpr int KEPT = !LDS ? 0 : GATE && !WIDE ? 3 : 2;
+  __shared__ f32x4 kept[LDS ? KEPT * NV * VEC / 4 * NT : 1];
   const float over = 1.0f / (float)a.H;
   float dpost[NV][VEC] = {}, dpre[NV][VEC] = {}, dgate[NV][VEC] = {};
+  float one[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) one[e] = 1.0f;
   auto add = [&](int which, int n, float (&sum)[VEC], const float (&x)[VEC],
                  const float (&y)[VEC]) {
-    if constexpr (LDS) {
+    if (which < KEPT) {
 #pragma unroll
       for (int q = 0; q < VEC / 4; ++q) {
         f32x4& k = kept[((which * NV + n) * (VEC / 4) + q) * NT + threadIdx.x];
@@ -289,7 +297,7 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
   };
   if constexpr (LDS) {
 #pragma unroll
-    for (int k = 0; k < 2 * NV * VEC / 4; ++k) kept[k * NT + threadIdx.x] = f32x4{};
+    for (int k = 0; k < KEPT * NV * VEC / 4; ++k) kept[k * NT + threadIdx.x] = f32x4{};
   }
   int64_t row, end, by;
   if constexpr (SUMS) {
@@ -384,10 +392,10 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
         if (GATE) {
           dz[e] = a.scale * d[n][e] * (a.post ? yn[e] * w[e] : yn[e]);
           gdot += e < c.skip ? 0.0f : dz[e];
-          if constexpr (SUMS) dgate[n][e] += dz[e];
         }
         d[n][e] *= GATE ? g[e] : a.scale;
       }
+      if constexpr (SUMS && GATE) add(2, n, dgate[n], dz, one);
       if constexpr (SUMS) add(0, n, dpost[n], d[n], yn);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -439,6 +447,8 @@ __global__ __launch_bounds__(NT) void norms_bwd(Args a) {
         for (int e = 0; e < VEC; ++e) {
           dpost[n][e] = kept[(n * (VEC / 4) + e / 4) * NT + threadIdx.x][e % 4];
           dpre[n][e] = kept[((NV + n) * (VEC / 4) + e / 4) * NT + threadIdx.x][e % 4];
+          if (KEPT == 3)
+            dgate[n][e] = kept[((2 * NV + n) * (VEC / 4) + e / 4) * NT + threadIdx.x][e % 4];
         }
       }
       store_f32<VEC, RAG>(to, c, dpost[n]);
@@ -483,14 +493,16 @@ __global__ __launch_bounds__(1024) void norms_join(const float* __restrict__ par
 
 // ---------------------------------------------------------------- host
 // Runs of rows in a backward that sums over rows, never across gate rows: as many as
-// workgroups run at once, so that none waits for a second turn and no CU idles (2103 rows
-// of 7168: 421 runs of 5 rows 76 us, 234 of 9 rows 66; 30000 rows of 512: 512 runs 140,
-// 3072 42; of 1001: 512 runs 210, 1536 113).  A CU holds 12 of the kernel's waves up to
-// 2048 columns, two workgroups of eight to 4096, one beyond.  Runs of at least two rows
-// where there are as many: each costs as much as a row again in partial sums.
+// workgroups run at once, so that none waits for a second turn and no CU idles (30000
+// rows of 512: 512 runs 140 us, 3072 42).  A CU holds 12 waves that keep their sums in
+// registers, or 16, or one workgroup beyond 4096 columns.  Runs of at least two rows where
+// there are as many: each costs as much as a row again in partial sums.
 void plan_runs(int64_t rows, int64_t rows_per, int64_t H, int64_t& runs, int64_t& per_run) {
   const int64_t groups = rows / rows_per;
-  const int64_t at_once = H > 4096 ? 256 : H > 2048 ? 512 : 256 * 12 / st::cdiv(H, 512);
+  const int64_t at_once = H > 4096  ? 256
+                          : H > 2048 ? 512
+                          : H > 512  ? 256 * 16 / st::cdiv(H, 512)
+                                     : 256 * 12;
   int64_t each = st::cdiv(at_once, groups);
   if (each > rows_per / 2) each = rows_per > 1 ? rows_per / 2 : 1;
   per_run = st::cdiv(rows_per, each);
@@ -524,7 +536,7 @@ void by_size(const Args& a, bool bwd, bool sums, hipStream_t s) {
   else if (H <= 2048) go<8, 256, 1, RAG>(a, bwd, sums, s);
   else if (H <= 4096 && bwd) go<8, 512, 1, RAG>(a, bwd, sums, s);
   else if (H <= 4096) go<8, 256, 2, RAG>(a, bwd, sums, s);
-  else if (H <= 8192 && bwd && !sums) go<8, 1024, 1, RAG>(a, bwd, sums, s);
+  else if (H <= 8192 && bwd) go<8, 1024, 1, RAG>(a, bwd, sums, s);
   else if (H <= 8192) go<8, 512, 2, RAG>(a, bwd, sums, s);
   else if (bwd && a.gate) go<8, 512, 4, RAG>(a, bwd, sums, s);
   else go<8, 1024, 2, RAG>(a, bwd, sums, s);
