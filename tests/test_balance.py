@@ -22,8 +22,8 @@ def test_arguments(args, kw, match):
 
 
 def _fwd(logits=4096, dtype=1, groups=1, per=4, E=8, k=2, ws=4096, nbytes=1 << 40):
-    _lib.call("st_balance_fwd", logits, dtype, 4096, None, groups, per, E, k, 0, 4096, 4096, 4096, ws,
-              nbytes, None)
+    _lib.call("st_balance_fwd", logits, dtype, 4096, 0, None, groups, per, E, k, 0, 4096, 4096, 4096,
+              ws, nbytes, None)
 
 
 @pytest.mark.parametrize("kw,match", [
