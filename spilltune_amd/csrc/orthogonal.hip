@@ -41,6 +41,7 @@ struct Entry {
   int64_t part, poly;      // its first matrix's place in the two scratch areas (doubles)
   int32_t K, r;            // long and short side
   int32_t CH, chunks;      // long elements of a workgroup in gram, and its workgroups
+                           // (of matrices done whole CH is their number)
   int32_t AL;              // long elements of a workgroup in apply (all three: r <= 32)
   int16_t tall;            // the short side is the contiguous one
   int16_t vec;             // rows may be read four elements at a time
@@ -992,10 +993,150 @@ __global__ __launch_bounds__(NTH) void apply64(const Table* __restrict__ table, 
   }
 }
 
+// ---------------------------------------------------------------- all of it, r <= 16
+// Matrices with long sides up to WHOLE: a workgroup of eight waves holds one in its
+// registers, or two, four or eight shorter ones, so it is read once and nothing goes
+// through memory in between (a call on 128 experts' factors at rank 16: 49 us, with the
+// three launches of longer ones 55; on 14 factors of rank 4 37 and 47).
+// Registers hold U as the last product wants it; for the Gram matrix each wave turns 64
+// long elements at a time over in LDS.  One wave a matrix does the steps; two workgroups a
+// CU cover for one another.
+constexpr int WAVES = 8, BLOCKS = 4, WHOLE = 64 * WAVES * BLOCKS;
+constexpr int LD = 68;  // floats of a row that is turned over
+static_assert(LD * sizeof(float) >= 17 * sizeof(double), "a tile is the room of steps16, too");
+// waves that hold a matrix
+__host__ __device__ inline int waves_of(const Entry& e) {
+  int w = WAVES;
+  while (w > 1 && e.K <= 32 * w * BLOCKS) w /= 2;
+  return w;
+}
+
+// 64 long elements from k0 on, as apply_rows; what lies behind the end is cleared where it
+// is first used, so that nothing waits for all loads.
+template <bool BF, bool TALL>
+__device__ __forceinline__ void whole_rows(const Entry& e, const void* x, int k0, int m, int q,
+                                           float (&u)[4][4]) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int k = TALL ? k0 + 16 * n + m : k0 + 4 * m, i = TALL ? 4 * q : 4 * n + q;
+    const uint32_t at = TALL ? k * e.r + i : i * e.K + k;  // below 16 WHOLE
+    load4<BF>(x, k < e.K && i < e.r ? at : 0, u[n]);
+  }
+}
+template <bool TALL>
+__device__ __forceinline__ void whole_clear(const Entry& e, int k0, int m, float (&u)[4][4]) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const bool in = (TALL ? k0 + 16 * n + m : k0 + 4 * m) < e.K;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) u[n][c] = in ? u[n][c] : 0.0f;
+  }
+}
+
+// `wave` of the `waves` that hold the matrix; `sum` and `tile` are its own, the sums of the
+// others behind the first one's.  `live`: there is one.
+template <bool BF, bool TALL>
+__device__ __forceinline__ void whole_walk(const Table& tab, const Entry& e, const void* x,
+                                           void* out, double* sum, float* tile, int wave, int waves,
+                                           bool live, int lane) {
+  const int m = lane & 15, q = lane >> 4;
+  float u[BLOCKS][4][4];
+  if (e.vec) {
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j)
+      whole_rows<BF, TALL>(e, x, 64 * (wave + waves * j), m, q, u[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j)
+      apply_rows<BF, TALL, false>(e, x, 0, 64 * (wave + waves * j), e.K, m, q, u[j]);
+  }
+  d4 g = {0.0, 0.0, 0.0, 0.0}, odd = g;
+#pragma unroll
+  for (int j = 0; j < BLOCKS; ++j) {
+    const int k0 = 64 * (wave + waves * j);
+    if (k0 >= e.K) break;
+    if (e.vec) whole_clear<TALL>(e, k0, m, u[j]);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if constexpr (TALL) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tile[(4 * q + c) * LD + 16 * n + m] = u[j][n][c];
+      } else {
+        *(f32x4*)(tile + (4 * n + q) * LD + 4 * m) =
+            f32x4{u[j][n][0], u[j][n][1], u[j][n][2], u[j][n][3]};
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    // lane (m, q) takes row m's elements 16q..: which is which k does not matter
+    f32x4 a[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) a[n] = *(const f32x4*)(tile + m * LD + 16 * q + 4 * n);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; c += 2) {
+        const double v = a[n][c], w = a[n][c + 1];
+        g = __builtin_amdgcn_mfma_f64_16x16x4f64(v, v, g, 0, 0, 0);
+        odd = __builtin_amdgcn_mfma_f64_16x16x4f64(w, w, odd, 0, 0, 0);
+      }
+  }
+  g += odd;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) sum[v * 64 + lane] = g[v];
+  __syncthreads();
+  double* Ps = sum - wave * 256;  // the first wave's, which it has read by then
+  if (wave == 0) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      double s = sum[v * 64 + lane];
+      for (int w = 1; w < waves; ++w) s += sum[w * 256 + v * 64 + lane];
+      g[v] = inside(e, s, 4 * v + q, m);
+    }
+    const d4 P = steps16(tab, g, (double*)tile, m, q);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) Ps[v * 64 + lane] = P[v];
+  }
+  __syncthreads();
+  if (!live) return;
+#pragma unroll
+  for (int j = 0; j < BLOCKS; ++j) {
+    const int64_t k0 = 64 * (wave + waves * j);
+    if (k0 >= e.K) break;
+    d4 acc[1][4] = {};
+    apply_tile<1, TALL>(Ps, 16, 0, 0, m, q, u[j], acc);
+    if (e.vec && k0 + 64 <= e.K)
+      apply_store<1, BF, TALL, true>(e, out, 0, k0, e.K, m, q, acc);
+    else
+      apply_store<1, BF, TALL, false>(e, out, 0, k0, e.K, m, q, acc);
+  }
+}
+
+template <bool BF>
+__global__ __launch_bounds__(64 * WAVES, 4) void whole(Table tab) {
+  __shared__ double sums[WAVES][256];
+  __shared__ f32x4 tiles[WAVES][4 * LD];
+  uint32_t w;
+  const Entry e = find(tab, IN_POLY, blockIdx.x, w);
+  const int at = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = waves_of(e);
+  // (a workgroup's last matrices may not be there: their waves work on the last one)
+  const uint32_t mat = w * (WAVES / waves) + at / waves, last = (uint32_t)e.CH - 1;
+  const int64_t off = (int64_t)min(mat, last) * e.r * (int64_t)e.K * (BF ? 2 : 4);
+  const void* x = (const char*)e.x + off;
+  void* out = (char*)e.out + off;
+  if (e.tall)
+    whole_walk<BF, true>(tab, e, x, out, sums[at], (float*)tiles[at], at % waves, waves, mat <= last,
+                         threadIdx.x & 63);
+  else
+    whole_walk<BF, false>(tab, e, x, out, sums[at], (float*)tiles[at], at % waves, waves,
+                          mat <= last, threadIdx.x & 63);
+}
+
 // ---------------------------------------------------------------- host
 struct Plan {  // one table's launches
   Table tab;
   int T = 1;
+  bool whole = false;
   int64_t count[MAXE];
   int64_t part = 0, poly = 0;  // doubles
 };
@@ -1052,6 +1193,15 @@ int make_plan(const st_matrix_batch* in, int32_t n, int32_t at, int32_t dtype, P
     e.vec = (e.tall ? r : K) % 4 == 0 && (((uintptr_t)b.x | (uintptr_t)b.out) & mask) == 0;
     p.count[t.n++] = b.count;
   }
+  int64_t all = 0;
+  p.whole = p.T == 1;
+  for (int i = 0; i < t.n; ++i) {
+    p.whole = p.whole && t.e[i].K <= WHOLE;
+    all += p.count[i];
+  }
+  if (all * 64 * WAVES >= (int64_t)1 << 32) p.whole = false;  // more than a launch takes
+  for (int i = 0; p.whole && i < t.n; ++i) t.e[i].CH = (int32_t)p.count[i];
+  if (p.whole) return taken;
   // places: 256 CUs and as many workgroups each as the kernels' registers and LDS allow
   const int64_t ch = p.T == 4 ? 0 : pick(p, 128, p.T == 1 ? 2048 : 1280, 256);
   const int64_t al = p.T == 4 ? 0 : pick(p, 256, p.T == 1 ? 1280 : 512, 256);
@@ -1090,6 +1240,14 @@ int64_t number(Plan& p, int phase, F per_matrix) {
 }
 
 constexpr int64_t TABLE_BYTES = (sizeof(Table) + 15) / 16 * 16;
+
+template <bool BF>
+int launch_whole(Plan& p, hipStream_t stream) {
+  for (int i = 0; i < p.tab.n; ++i) p.count[i] = st::cdiv(p.count[i], WAVES / waves_of(p.tab.e[i]));
+  const int64_t n = number(p, IN_POLY, [](const Entry&) { return (int64_t)1; });
+  whole<BF><<<(unsigned)n, 64 * WAVES, 0, stream>>>(p.tab);
+  return st::check_launch("st_orthogonalize");
+}
 
 template <int T, bool BF>
 int launch(Plan& p, char* workspace, hipStream_t stream) {
@@ -1206,7 +1364,8 @@ extern "C" int st_orthogonalize(int32_t n, const st_matrix_batch* table, int32_t
     char* ws = (char*)workspace;
     const hipStream_t s = (hipStream_t)stream;
     const bool bf = dtype == ST_DTYPE_BF16;
-    const int r = p.T == 1   ? (bf ? launch<1, true>(p, ws, s) : launch<1, false>(p, ws, s))
+    const int r = p.whole    ? (bf ? launch_whole<true>(p, s) : launch_whole<false>(p, s))
+                  : p.T == 1 ? (bf ? launch<1, true>(p, ws, s) : launch<1, false>(p, ws, s))
                   : p.T == 2 ? (bf ? launch<2, true>(p, ws, s) : launch<2, false>(p, ws, s))
                              : (bf ? launch<4, true>(p, ws, s) : launch<4, false>(p, ws, s));
     if (r != ST_OK) return r;

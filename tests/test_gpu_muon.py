@@ -104,7 +104,19 @@ def test_shares_that_end_inside_matrices(shapes, dtype):
         check(o, u)
 
 
-@pytest.mark.parametrize("shape", [(3, 40, 300), (3, 300, 72), (3, 100, 1000), (3, 150, 400)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("r", [1, 3, 12, 16])
+def test_matrices_held_whole(r, dtype):
+    """Long sides that eight, four, two and one wave hold, one more, and odd counts of them;
+    with a longer one in the call, none is."""
+    us = [make((3 + K % 7, *((r, K) if K % 3 else (K, r))), K, dtype)
+          for K in (16, 64, 65, 255, 256, 257, 511, 512, 516, 1023, 1024, 1025, 2044, 2047, 2048)]
+    for group in (us, us + [make((r, 2049), 1, dtype)]):
+        for u, o in zip(group, muon.orthogonalize(group)):
+            check(o, u)
+
+
+@pytest.mark.parametrize("shape", [(3, 7, 600), (3, 300, 12), (3, 40, 300), (3, 300, 72), (3, 100, 1000), (3, 150, 400)])
 def test_one_matrix_that_is_not_finite_among_others(shape):
     """Also in the last row of a short side that ends inside a tile."""
     u = make(shape, 4)

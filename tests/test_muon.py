@@ -36,7 +36,8 @@ def _call(shape=(4, 8), count=1, dtype=1, steps=5, abc=(3.4445, -4.775, 2.0315),
     ({"dtype": 2}, "dtype"), ({"steps": 0}, "steps"), ({"steps": 13}, "steps"),
     ({"steps": 65, "abc": (1.0, 0.0, 0.0)}, "steps"), ({"abc": (math.nan, 0.0, 0.0)}, "finite"),
     ({"eps": -1.0}, "eps"), ({"x": None}, "NULL"), ({"x": 4097}, "misaligned"),
-    ({"nbytes": 16}, "workspace"), ({"ws": None}, "workspace"),
+    ({"shape": (4, 4096), "nbytes": 16}, "workspace"), ({"shape": (4, 4096), "ws": None}, "workspace"),
+    ({"shape": (33, 40), "ws": None}, "workspace"),
     # 2^23 matrices of 32 chunks each: more workgroups than a launch numbers
     ({"shape": (1, 1 << 20), "count": (1 << 24) - 1, "nbytes": 1 << 60}, "too many"),
 ])
