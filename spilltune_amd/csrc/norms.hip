@@ -494,7 +494,7 @@ __global__ __launch_bounds__(1024) void norms_join(const float* __restrict__ par
 // ---------------------------------------------------------------- host
 // Runs of rows in a backward that sums over rows, never across gate rows: as many as
 // workgroups run at once, so that none waits for a second turn and no CU idles (30000
-// rows of 512: 512 runs 140 us, 3072 42).  A CU holds 12 waves that keep their sums in
+// rows of 512: two runs a CU 140 us, twelve 42).  A CU holds 12 waves that keep their sums in
 // registers, or 16, or one workgroup beyond 4096 columns.  Runs of at least two rows where
 // there are as many: each costs as much as a row again in partial sums.
 void plan_runs(int64_t rows, int64_t rows_per, int64_t H, int64_t& runs, int64_t& per_run) {

@@ -682,19 +682,22 @@ __global__ __launch_bounds__(4 * R) void poly_panel(const Table* __restrict__ ta
 
 // Short sides beyond 128, in tiles of 32 x 32 and three launches a step.
 // mode 0: Q = aI + bG + cGG;  mode 1: P' = Q P and (blockIdx.y = 1) H = Q G;
-// mode 2: G = H Q, its upper half in both places.
+// mode 2: G = H Q.  All are polynomials of one symmetric matrix, so symmetric: the tiles on
+// and above the diagonal are formed and written to both places, turned over in LDS (4
+// matrices of 1024: @@ us for a mode 0, every tile formed 210).
 __global__ __launch_bounds__(NTH) void poly_step(const Table* __restrict__ table, int mode, int turn,
                                                  double* __restrict__ poly) {
   __shared__ double As[128 * 32], Bs[128 * 32];
   const Table& tab = *table;
   uint32_t w;
-  const Entry& e = find(tab, IN_POLY, blockIdx.x, w);
+  const Entry& e = find(tab, IN_POLY, neighbours(), w);
   const int R = (e.r + 63) / 64 * 64;
-  const uint32_t per = (uint32_t)R * R / 1024;
+  const int nt = R / 32, per = nt * (nt + 1) / 2;
   double* base = poly + e.poly + (int64_t)(w / per) * SLOTS * R * R;
-  const int i0 = (int)(w % per) / (R / 32) * 32, j0 = (int)(w % per) % (R / 32) * 32;
+  int i0 = 0, j0 = (int)(w % per);  // (0,0..nt-1), (1,1..nt-1), ...
+  while (j0 >= nt - i0) j0 -= nt - i0, ++i0;
+  j0 = 32 * (j0 + i0), i0 *= 32;
   const int64_t RR = (int64_t)R * R;
-  if (mode == 2 && i0 > j0) return;
   const int from = turn ? SLOT_P1 : SLOT_P0, into = turn ? SLOT_P0 : SLOT_P1;
   const bool h = mode == 1 && blockIdx.y == 1;
   const double* A = base + (mode == 0 ? SLOT_G : mode == 1 ? SLOT_Q : SLOT_H) * RR;
@@ -735,15 +738,22 @@ __global__ __launch_bounds__(NTH) void poly_step(const Table* __restrict__ table
     }
   }
   acc += odd;
+  __syncthreads();
+  double* tile = As;  // rows of 33
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
-    const int row = i0 + wi + 4 * v + q, col = j0 + wj + m;
-    const int64_t at = (int64_t)row * R + col;
-    if (mode == 2) {
-      if (row <= col) D[at] = D[(int64_t)col * R + row] = acc[v];
-    } else {
-      D[at] = mode == 0 ? tab.c * acc[v] + tab.b * A[at] + (row == col ? tab.a : 0.0) : acc[v];
-    }
+    const int row = wi + 4 * v + q, col = wj + m;
+    const int64_t at = (int64_t)(i0 + row) * R + j0 + col;
+    tile[row * 33 + col] =
+        mode ? acc[v] : tab.c * acc[v] + tab.b * A[at] + (i0 + row == j0 + col ? tab.a : 0.0);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = threadIdx.x; i < 1024; i += NTH) {
+    const int row = i / 32, col = i % 32;
+    const double up = tile[row * 33 + col], low = tile[col * 33 + row];
+    D[(int64_t)(i0 + row) * R + j0 + col] = i0 == j0 && row > col ? low : up;
+    if (i0 != j0) D[(int64_t)(j0 + row) * R + i0 + col] = low;
   }
 }
 
@@ -1261,7 +1271,7 @@ int launch(Plan& p, char* workspace, hipStream_t stream) {
   });
   const int64_t nn = number(p, IN_NORM, [&](const Entry& e) { return blocks(e) * blocks(e) * 4; });
   const int64_t np = number(p, IN_POLY, [&](const Entry& e) {
-    return T < 4 ? (int64_t)1 : nb <= 2 ? (int64_t)4 * nb : blocks(e) * blocks(e) * 4;
+    return T < 4 ? (int64_t)1 : nb <= 2 ? (int64_t)4 * nb : blocks(e) * (2 * blocks(e) + 1);
   });
   int64_t na = number(p, IN_APPLY, [&](const Entry& e) {
     return T < 4 ? st::cdiv(e.K, e.AL) : st::cdiv(e.K, UNIT) * blocks(e);
