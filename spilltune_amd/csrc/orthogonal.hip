@@ -683,8 +683,9 @@ __global__ __launch_bounds__(4 * R) void poly_panel(const Table* __restrict__ ta
 // Short sides beyond 128, in tiles of 32 x 32 and three launches a step.
 // mode 0: Q = aI + bG + cGG;  mode 1: P' = Q P and (blockIdx.y = 1) H = Q G;
 // mode 2: G = H Q.  All are polynomials of one symmetric matrix, so symmetric: the tiles on
-// and above the diagonal are formed and written to both places, turned over in LDS (4
-// matrices of 1024: @@ us for a mode 0, every tile formed 210).
+// and above the diagonal are formed and written to both places, turned over in LDS, a
+// matrix's workgroups on one XCD (a launch of mode 0 at 4 matrices of 1024: 135 us, every
+// tile formed 216; at 16 of 256 16 and 22).
 __global__ __launch_bounds__(NTH) void poly_step(const Table* __restrict__ table, int mode, int turn,
                                                  double* __restrict__ poly) {
   __shared__ double As[128 * 32], Bs[128 * 32];
