@@ -66,13 +66,13 @@ def orthogonalize(matrices, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 
 
 def _factors(proj):
-    """``(parameter, gradient, momentum)`` of an adapter's two factors, each as a
-    view of its matrices: [matrices, rows, columns] of per-expert ones, whose fused
-    gate and up are matrices of their own."""
+    """``(parameter, gradient, momentum)`` of an adapter's two factors; of per-expert
+    ones a view of the matrices, [matrices, rows, columns], whose fused gate and up are
+    matrices of their own.  (For use without gradients.)"""
     n = getattr(proj, "segments", 1)
     for t in ((proj.A, proj.grad_A, proj.m_A), (proj.B, proj.grad_B, proj.m_B)):
         if t[0].dim() == 2:
-            yield tuple(x.detach() for x in t)
+            yield t
         else:
             shape = (t[0].shape[0] * n, t[0].shape[1] // n, t[0].shape[2])
             yield tuple(x.detach().view(shape) for x in t)
@@ -118,9 +118,9 @@ class Muon:
             if self.table is None:
                 raise ValueError(f"unsupported_capability: no optimizer for {sorted(tables)}")
             self.table.step(tables)
-        factors = [f for k, p in projections.items() if k not in tables for f in _factors(p)]
-        if factors:
-            with torch.no_grad():
+        with torch.no_grad():
+            factors = [f for k, p in projections.items() if k not in tables for f in _factors(p)]
+            if factors:
                 params, grads, moments = (list(t) for t in zip(*factors))
                 torch._foreach_lerp_(moments, grads, 1.0 - self.momentum)
                 updates = torch._foreach_lerp(grads, moments, self.momentum) if self.nesterov \
