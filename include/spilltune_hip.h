@@ -684,7 +684,9 @@ int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual, const uin
  * times the fp32 sum of dout [n, hidden] (bf16) over each token's positions in
  * rising order; zeros for tokens that do not occur.  With `accumulate` (fp32 only)
  * the sums are added and other rows left as they are.  Tokens equal to padding_idx
- * or outside the table take no part.
+ * or outside the table take no part.  A launch takes fewer than 2^32 threads: n / 32
+ * times those of a row (one for 4 columns of an fp32 gradient, 8 of a bf16 one; whole
+ * waves, beyond 256 whole workgroups), or the call is refused before any work.
  */
 int st_embedding_fwd(const void* table, int32_t dtype, const void* ids, int32_t ids32, int64_t n,
                      int64_t vocab, int64_t hidden, float scale, uint16_t* out,

@@ -690,6 +690,12 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
   ST_CHECK_ARG(!accumulate || grad_dtype == ST_DTYPE_F32,
                "st_embedding_bwd adds to fp32 gradients only");
   ST_CHECK_ARG(grad && ((uintptr_t)grad & 15) == 0, "st_embedding_bwd: NULL or misaligned gradient");
+  // as many columns a lane as make 16 bytes of the gradient
+  const int vec = hidden < 8 ? 1 : grad_dtype == ST_DTYPE_F32 ? 4 : 8;
+  const unsigned th = threads_of(hidden, vec);
+  const int64_t chunks = st::cdiv(n, chunk_of(n)), slices = st::cdiv(hidden, (int64_t)th * vec);
+  if (chunks * slices * th >= (int64_t)1 << 32)
+    return st::fail(ST_EUNSUPPORTED, "st_embedding_bwd: more threads than a launch takes");
   const hipStream_t s = (hipStream_t)stream;
   const int64_t bytes = vocab * hidden * (grad_dtype == ST_DTYPE_F32 ? 4 : 2);
   const int64_t words = accumulate ? 0 : bytes / 16;
@@ -746,13 +752,7 @@ extern "C" int st_embedding_bwd(const uint16_t* dout, const void* ids, int32_t i
   a.n = n, a.V = vocab, a.H = hidden, a.chunk = chunk_of(n), a.scale = scale;
   a.grad_f32 = grad_dtype == ST_DTYPE_F32, a.accumulate = accumulate, a.grad = grad;
   a.partial = (float*)(w + l.partial);
-  // as many columns a lane as make 16 bytes of the gradient
   const bool even = hidden % 8 == 0 && ((uintptr_t)dout & 15) == 0;
-  const int vec = hidden < 8 ? 1 : a.grad_f32 ? 4 : 8;
-  const unsigned th = threads_of(hidden, vec);
-  const int64_t chunks = st::cdiv(n, a.chunk), slices = st::cdiv(hidden, (int64_t)th * vec);
-  if (chunks * slices * th >= (int64_t)1 << 32 || slices >= 65536)
-    return st::fail(ST_EUNSUPPORTED, "st_embedding_bwd: more threads than a launch takes");
   const dim3 grid((unsigned)chunks, (unsigned)slices), more((unsigned)chunks - 1, (unsigned)slices);
   auto sums = [&](auto whole, auto runs, auto join) {
     if (n <= WHOLE) {
