@@ -25,6 +25,7 @@ benchmark configuration and is optional.
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass, field
 from typing import NamedTuple, Optional
@@ -232,13 +233,18 @@ def balance_loss(logits, indices, *, score="softmax", valid=None, per_row=False)
         None if valid is None else valid.contiguous(), groups, int(score == "sigmoid")))
 
 
+def _capturing(t) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class ExpertBalance:
     """The balance term of an MoE layer (or of several that share the object): each
     pass that is differentiated adds ``coefficient`` times :func:`balance_loss` of its
     router to the loss whose gradient flows, and is counted here -- ``loss`` the sum of
     the passes' losses (without the coefficient), ``counts`` (int64 [E]) of their picks,
-    both on the device, ``passes`` how many (of a captured pass, what its last replay
-    left, once).  The routers are frozen: the term teaches the adapters before them.
+    both on the device (None without a pass), ``passes`` how many.  A captured pass
+    counts once, from its first replay on, with what its last one left; :meth:`reset`
+    forgets it too.  The routers are frozen: the term teaches the adapters before them.
 
     Every microbatch adds its own term, so a window of ``n`` of them that is to add one
     average takes the coefficient over ``n``.  ``per_row`` balances each row by itself.
@@ -251,13 +257,33 @@ class ExpertBalance:
         self.reset()
 
     def reset(self):
-        self.loss, self.counts, self.passes = None, None, 0
+        self._sums, self._captured, self.passes = None, [], 0
 
     def record(self, loss, counts):
-        loss, counts = loss.detach().clone(), counts.sum(0)
-        self.loss = loss if self.loss is None else self.loss + loss
-        self.counts = counts if self.counts is None else self.counts + counts
+        loss, counts = loss.detach(), counts.detach()
+        if _capturing(loss):
+            # the graph's own tensors, which every replay writes anew: kept alive here, and
+            # added when they are asked for (an addition in the graph would read whatever
+            # follows the eager sums in their memory)
+            self._captured.append((loss, counts))
+        else:
+            now = loss.clone(), counts.sum(0)
+            self._sums = now if self._sums is None else tuple(a + b for a, b in zip(self._sums, now))
         self.passes += 1
+
+    def _sum(self, which):
+        parts = [] if self._sums is None else [self._sums[which]]
+        for loss, counts in self._captured:
+            parts.append(counts.sum(0) if which else loss.clone())
+        return functools.reduce(torch.add, parts) if parts else None
+
+    @property
+    def loss(self):
+        return self._sum(0)
+
+    @property
+    def counts(self):
+        return self._sum(1)
 
 
 class _WithTerm(torch.autograd.Function):
