@@ -288,16 +288,20 @@ class ExpertBalance:
 
 class _WithTerm(torch.autograd.Function):
     """``out``, whose backward also passes ``coefficient`` on to ``loss``: the gradient of
-    the sum of what ``out`` leads to and ``coefficient * loss``."""
+    the sum of what ``out`` leads to and ``coefficient * loss``.  ``record``: what the
+    first backward is to call."""
 
     @staticmethod
-    def forward(ctx, out, loss, coefficient):
-        ctx.coefficient = coefficient
+    def forward(ctx, out, loss, coefficient, record):
+        ctx.coefficient, ctx.record = coefficient, record
         return out.view_as(out)
 
     @staticmethod
     def backward(ctx, dout):
-        return dout, torch.full((), ctx.coefficient, dtype=_F32, device=dout.device), None
+        if ctx.record is not None:
+            ctx.record()
+            ctx.record = None
+        return dout, torch.full((), ctx.coefficient, dtype=_F32, device=dout.device), None, None
 
 
 def _balanced(out, logits, indices, score, balance, valid, shape):
@@ -308,8 +312,14 @@ def _balanced(out, logits, indices, score, balance, valid, shape):
     lead = shape[:-1] if len(shape) > 1 else (1,)
     loss, counts = balance_loss(logits.view(*lead, -1), indices.view(*lead, -1), score=score,
                                 valid=valid, per_row=balance.per_row)
-    balance.record(loss, counts)
-    return _WithTerm.apply(out, loss, balance.coefficient)
+    record = functools.partial(balance.record, loss.detach(), counts)
+    # A forward within a backward is one that is formed again: of a pass that ran without
+    # gradients its own backward follows, which counts it; of one that ran with them, and
+    # was counted then (torch's checkpoint without reentrance), only saved tensors are taken.
+    again = torch._C._current_graph_task_id() != -1
+    if not again:
+        record()
+    return _WithTerm.apply(out, loss, balance.coefficient, record if again else None)
 
 
 # ----------------------------------------------------------------- the function

@@ -1,5 +1,7 @@
 """What an ExpertBalance keeps of the passes (the loss itself: test_gpu_balance.py)."""
+import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from spilltune_amd import moe
 
@@ -45,3 +47,67 @@ def test_captured_passes_count_with_their_last_replay(monkeypatch):
         assert abs(float(balance.loss) - total) < 1e-6
     balance.reset()
     assert balance.loss is None and balance.passes == 0
+
+
+def _plain_balance_loss(logits, indices, *, score, valid, per_row):
+    """The loss of one group in plain torch, on the host."""
+    E = logits.shape[-1]
+    counts = torch.bincount(indices.reshape(-1).long(), minlength=E)
+    p = logits.float().softmax(-1).reshape(-1, E).mean(0)
+    return moe.BalanceLoss(E * (counts / counts.sum() * p).sum(), counts[None])
+
+
+def _engine(f, x):
+    """A block formed again in its backward, as the engine does."""
+    class Again(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            ctx.save_for_backward(x)
+            with torch.no_grad():
+                return f(x)
+
+        @staticmethod
+        def backward(ctx, dy):
+            x = ctx.saved_tensors[0].detach().requires_grad_(True)
+            with torch.enable_grad():
+                y = f(x)
+            return torch.autograd.grad(y, [x], dy)[0]
+    return Again.apply(x)
+
+
+@pytest.mark.parametrize("how", [
+    lambda f, x: f(x), lambda f, x: checkpoint(f, x, use_reentrant=False),
+    lambda f, x: checkpoint(f, x, use_reentrant=True), _engine],
+    ids=["plain", "checkpoint", "reentrant", "engine"])
+def test_a_pass_counts_once_however_it_is_formed(monkeypatch, how):
+    monkeypatch.setattr(moe, "balance_loss", _plain_balance_loss)
+    g = torch.Generator().manual_seed(4)
+    w, x = torch.randn(6, 8, generator=g), torch.randn(2, 5, 6, generator=g).requires_grad_(True)
+    balance = moe.ExpertBalance(0.5)
+
+    def layer(x):
+        logits = x.reshape(-1, 6) @ w
+        out = moe._balanced(torch.tanh(x.reshape(-1, 6)), logits, logits.topk(2)[1], "softmax", balance,
+                            None, x.shape)
+        return out.reshape(x.shape).sin()
+    up = torch.randn(x.shape, generator=g)
+    how(layer, x).backward(up)  # (torch's reentrant checkpoint takes no autograd.grad)
+    assert balance.passes == 1 and int(balance.counts.sum()) == 20
+    logits = x.reshape(-1, 6) @ w
+    loss, _ = _plain_balance_loss(logits, logits.topk(2)[1], score="softmax", valid=None, per_row=False)
+    (want,) = torch.autograd.grad((torch.tanh(x).sin() * up).sum() + 0.5 * loss, [x])
+    assert torch.allclose(x.grad, want, rtol=1e-5, atol=1e-6)  # sums of eight fp32 terms up to 4
+    assert abs(float(balance.loss) - float(loss.detach())) < 1e-5
+    with torch.no_grad():
+        layer(x)
+    assert balance.passes == 1
+
+
+def test_a_pass_is_there_after_its_forward(monkeypatch):
+    monkeypatch.setattr(moe, "balance_loss", _plain_balance_loss)
+    balance, x = moe.ExpertBalance(0.5), torch.rand(5, 8).requires_grad_(True)
+    out = moe._balanced(x * 2, x * 3, x.topk(2)[1], "softmax", balance, None, x.shape)
+    assert balance.passes == 1 and int(balance.counts.sum()) == 10
+    for _ in range(2):
+        out.sum().backward(retain_graph=True)
+    assert balance.passes == 1

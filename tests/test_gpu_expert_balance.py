@@ -1,6 +1,7 @@
 """An ExpertBalance through an MoE layer: captured and replayed."""
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from spilltune_amd import moe
 
@@ -75,3 +76,21 @@ def test_sums_of_replayed_passes(sigmoid, per_row):
         del noise
     balance.reset()
     assert balance.loss is None and balance.counts is None and balance.passes == 0
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_passes_count_once(reentrant):
+    """A layer that torch's checkpoint forms again: the plain pass's sums and gradients."""
+    dev = torch.device("cuda:0")
+    layer = _layer(False, dev)
+    g = torch.Generator("cuda").manual_seed(5)
+    x, up = (torch.randn(B, S, H, device=dev, generator=g).to(BF) for _ in range(2))
+    got = []
+    for again in (False, True):
+        balance, leaf = moe.ExpertBalance(2.0), x.clone().requires_grad_(True)
+        f = lambda t: layer(t, balance, None)  # noqa: B023,E731
+        out = checkpoint(f, leaf, use_reentrant=reentrant) if again else f(leaf)
+        out.backward(up)
+        got.append((leaf.grad, balance.loss, balance.counts, balance.passes))
+    assert got[0][3] == got[1][3] == 1
+    assert all(torch.equal(a, b) for a, b in zip(got[0][:3], got[1][:3]))
