@@ -252,6 +252,11 @@ __device__ __forceinline__ void gram_walk(const Entry& e, const void* x, int row
     multiply(a, b);
   }
 }
+// 1 / (|U|_F + eps), or 0 of a zero matrix without eps, which stays zero.
+__device__ __forceinline__ double over(double trace, double eps) {
+  const double norm = sqrt(trace) + eps;
+  return norm == 0.0 ? 0.0 : 1.0 / norm;
+}
 // A sum of the Gram matrix, or 0 past the short side.
 __device__ __forceinline__ double inside(const Entry& e, double sum, int row, int col) {
   return row < e.r && col < e.r ? sum : 0.0;
@@ -404,7 +409,7 @@ __device__ __forceinline__ d4 steps16(const Table& tab, d4 g, double* turn, int 
   for (int v = 0; v < 4; ++v) trace += 4 * v + q == m ? g[v] : 0.0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) trace += __shfl_xor(trace, o);
-  const double inv = 1.0 / (sqrt(trace) + tab.eps);
+  const double inv = over(trace, tab.eps);
   d4 one, P;
 #pragma unroll
   for (int v = 0; v < 4; ++v) one[v] = 4 * v + q == m ? 1.0 : 0.0;
@@ -480,7 +485,7 @@ __global__ __launch_bounds__(NTH) void poly_small(const Table* __restrict__ tabl
   double trace = 0.0;
   for (int i = 0; i < e.r; ++i) trace += G[i * R + i];
   __syncthreads();
-  const double inv = 1.0 / (sqrt(trace) + tab.eps);
+  const double inv = over(trace, tab.eps);
   for (int i = threadIdx.x; i < N; i += NTH) {
     G[i] = G[i] * inv * inv;
     P[i] = i / R == i % R ? inv : 0.0;
@@ -592,7 +597,7 @@ __global__ __launch_bounds__(NTH) void poly_norm(const Table* __restrict__ table
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = trace;
   __syncthreads();
   trace = red[0] + red[1] + red[2] + red[3];
-  const double inv = 1.0 / (sqrt(trace) + tab.eps);
+  const double inv = over(trace, tab.eps);
   for (int i = threadIdx.x; i < 1024; i += NTH) {
     const int at = (int)(w % per) * 1024 + i;
     base[at] = gram_at(mine, nb, at / R, at % R) * inv * inv;  // SLOT_G
