@@ -729,7 +729,8 @@ int st_balance_bwd(const void* logits, int32_t dtype, const uint8_t* valid, int6
  * 1024), written to `out` in the same layout.  x and out bf16 or fp32 (`dtype`),
  * all sums in 64 bits; out may not overlap any x.  |a|^(2 steps) <= 1e13, which
  * bounds the growth of what 64 bits round.  A matrix with a value that is not
- * finite gives NaN throughout.  `table` is a host array read during the call.
+ * finite gives NaN throughout.  `table` is a host array read during the call.  What
+ * is refused is refused before any work; the query gives -1 for sizes that are.
  */
 typedef struct st_matrix_batch {
   const void* x;

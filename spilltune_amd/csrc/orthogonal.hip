@@ -1242,15 +1242,33 @@ int make_plan(const st_matrix_batch* in, int32_t n, int32_t at, int32_t dtype, P
   return taken;
 }
 
-// Numbers the workgroups of a phase; their count, or -1 beyond a launch's limit.
-template <typename F>
-int64_t number(Plan& p, int phase, F per_matrix) {
+// Workgroups (units) of a matrix in a phase.
+int64_t each_of(const Plan& p, int phase, const Entry& e) {
+  const int64_t nb = st::cdiv(e.r, 64);
+  switch (phase) {
+    case IN_GRAM: return p.T < 4 ? (int64_t)e.chunks : (int64_t)Pairs(e).each;
+    case IN_SUM: return p.T < 4 ? 0 : nb * (nb + 1) / 2 * 8;
+    case IN_NORM: return p.T < 4 ? 0 : nb * nb * 4;
+    case IN_POLY: return p.T < 4 ? 1 : nb <= 2 ? 4 * nb : nb * (2 * nb + 1);
+    default: return p.T < 4 ? st::cdiv(e.K, e.AL) : st::cdiv(e.K, UNIT) * nb;
+  }
+}
+// Every phase's workgroups fit a launch.
+bool fits(const Plan& p) {
+  for (int phase = 0; phase < PHASES; ++phase) {
+    int64_t all = 0;
+    for (int i = 0; i < p.tab.n; ++i) all += p.count[i] * each_of(p, phase, p.tab.e[i]);
+    if (all * NTH >= (int64_t)1 << 32) return false;
+  }
+  return true;
+}
+// Numbers the workgroups of a phase; their count.
+int64_t number(Plan& p, int phase) {
   int64_t at = 0;
   for (int i = 0; i < 64; ++i) p.tab.tile0[phase][i] = ~0u;
   for (int i = 0; i < p.tab.n; ++i) {
     p.tab.tile0[phase][i] = (uint32_t)at;
-    at += p.count[i] * per_matrix(p.tab.e[i]);
-    if (at * NTH >= (int64_t)1 << 32) return -1;
+    at += p.count[i] * each_of(p, phase, p.tab.e[i]);
   }
   return at;
 }
@@ -1260,30 +1278,16 @@ constexpr int64_t TABLE_BYTES = (sizeof(Table) + 15) / 16 * 16;
 template <bool BF>
 int launch_whole(Plan& p, hipStream_t stream) {
   for (int i = 0; i < p.tab.n; ++i) p.count[i] = st::cdiv(p.count[i], WAVES / waves_of(p.tab.e[i]));
-  const int64_t n = number(p, IN_POLY, [](const Entry&) { return (int64_t)1; });
+  const int64_t n = number(p, IN_POLY);
   whole<BF><<<(unsigned)n, 64 * WAVES, 0, stream>>>(p.tab);
   return st::check_launch("st_orthogonalize");
 }
 
 template <int T, bool BF>
 int launch(Plan& p, char* workspace, hipStream_t stream) {
-  auto blocks = [](const Entry& e) { return ((int64_t)e.r + 63) / 64; };
-  const int nb = (int)blocks(p.tab.e[0]);  // 1, 2 or more for all entries
-  int64_t ng = number(p, IN_GRAM, [&](const Entry& e) {
-    return T < 4 ? (int64_t)e.chunks : (int64_t)Pairs(e).each;
-  });
-  const int64_t ns = number(p, IN_SUM, [&](const Entry& e) {
-    return blocks(e) * (blocks(e) + 1) / 2 * 8;
-  });
-  const int64_t nn = number(p, IN_NORM, [&](const Entry& e) { return blocks(e) * blocks(e) * 4; });
-  const int64_t np = number(p, IN_POLY, [&](const Entry& e) {
-    return T < 4 ? (int64_t)1 : nb <= 2 ? (int64_t)4 * nb : blocks(e) * (2 * blocks(e) + 1);
-  });
-  int64_t na = number(p, IN_APPLY, [&](const Entry& e) {
-    return T < 4 ? st::cdiv(e.K, e.AL) : st::cdiv(e.K, UNIT) * blocks(e);
-  });
-  if (ng < 0 || ns < 0 || nn < 0 || np < 0 || na < 0)
-    return st::fail(ST_EUNSUPPORTED, "too many matrices for a launch: call with fewer at a time");
+  const int nb = (p.tab.e[0].r + 63) / 64;  // 1, 2 or more for all entries
+  int64_t ng = number(p, IN_GRAM), na = number(p, IN_APPLY);
+  const int64_t np = number(p, IN_POLY), ns = number(p, IN_SUM), nn = number(p, IN_NORM);
   if (T == 4) {
     p.tab.gram = shares(ng, GRAM_WGS), ng = p.tab.gram.wgs;
     p.tab.apply = shares(na, APPLY_WGS), na = p.tab.apply.wgs;
@@ -1335,24 +1339,34 @@ int check_table(int32_t n, const st_matrix_batch* table) {
   }
   return ST_OK;
 }
-
-}  // namespace
-
-extern "C" int64_t st_orthogonalize_workspace_bytes(int32_t n, const st_matrix_batch* table) {
-  if (check_table(n, table) != ST_OK) return 0;
+// The sizes of all tables, checked before the first launch, and their workspace.
+int survey(int32_t n, const st_matrix_batch* table, int64_t& bytes) {
+  const int rc = check_table(n, table);
+  if (rc != ST_OK) return rc;
   int64_t most = 0;
   Plan p;
   for (int32_t at = 0; at < n;) {
     at += make_plan(table, n, at, ST_DTYPE_F32, p);
+    if (p.tab.n && !p.whole && !fits(p))
+      return st::fail(ST_EUNSUPPORTED, "too many matrices for a launch: call with fewer at a time");
     if (p.part + p.poly > most) most = p.part + p.poly;
   }
-  return most ? most * 8 + TABLE_BYTES : 0;
+  bytes = most ? most * 8 + TABLE_BYTES : 0;
+  return ST_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t st_orthogonalize_workspace_bytes(int32_t n, const st_matrix_batch* table) {
+  int64_t bytes = 0;
+  return survey(n, table, bytes) == ST_OK ? bytes : -1;
 }
 
 extern "C" int st_orthogonalize(int32_t n, const st_matrix_batch* table, int32_t dtype,
                                 int32_t steps, double a, double b, double c, double eps,
                                 void* workspace, int64_t workspace_bytes, st_stream_t stream) {
-  const int rc = check_table(n, table);
+  int64_t need = 0;
+  const int rc = survey(n, table, need);
   if (rc != ST_OK) return rc;
   ST_CHECK_ARG(dtype == ST_DTYPE_BF16 || dtype == ST_DTYPE_F32, "dtype codes are bf16 and fp32");
   ST_CHECK_ARG(std::isfinite(a) && std::isfinite(b) && std::isfinite(c) && std::isfinite(eps) &&
@@ -1368,7 +1382,6 @@ extern "C" int st_orthogonalize(int32_t n, const st_matrix_batch* table, int32_t
     ST_CHECK_ARG(m.x && m.out, "matrices %d: NULL", i);
     ST_CHECK_ARG((((uintptr_t)m.x | (uintptr_t)m.out) & mask) == 0, "matrices %d: misaligned", i);
   }
-  const int64_t need = st_orthogonalize_workspace_bytes(n, table);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return st::fail(ST_EWORKSPACE, "st_orthogonalize needs %lld workspace bytes", (long long)need);
   ST_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");

@@ -25,3 +25,18 @@ def test_zero_matrix_without_eps(shape, dtype):
     u[2].view(-1)[-1] = float("nan")
     out = muon.orthogonalize(u, eps=0.0)
     assert (out[1] == 0).all() and out[2].isnan().all() and not out[0].isnan().any()
+
+
+def test_more_matrices_than_another_rank_could_have():
+    """2^21 and a few matrices of rank 17: bounded by the launches they take, whose
+    workgroups are one a matrix (matrices of rank 33 take eight)."""
+    n = (1 << 21) + 5
+    u = torch.zeros(n, 17, 18, device="cuda")
+    for at in (0, 1 << 20, n - 3):
+        u[at:at + 3] = make((3, 17, 18), at % 100)
+    out = muon.orthogonalize(u)
+    for at in (0, 1 << 20, n - 3):
+        check(out[at:at + 3], u[at:at + 3])
+    assert (out[3:1 << 20] == 0).all() and (out[(1 << 20) + 3:n - 3] == 0).all()
+    del u, out
+    torch.cuda.empty_cache()
