@@ -34,6 +34,25 @@ def orthogonalize(matrices, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     given = [matrices] if single else list(matrices)
     if not given:
         return []
+    out = _run(_prepare(given, steps, coefficients, eps), given)
+    return out[0] if single else out
+
+
+def _rule(steps, coefficients, eps=1e-7):
+    """``(steps, a, b, c, eps)``, checked."""
+    a, b, c = (float(v) for v in coefficients)
+    if isinstance(steps, bool) or not isinstance(steps, int):
+        raise ValueError("unsupported_capability: steps must be an integer")
+    if not (math.isfinite(a) and math.isfinite(b) and math.isfinite(c) and 0.0 <= eps < math.inf):
+        raise ValueError("unsupported_capability: coefficients must be finite, eps not negative")
+    if not 1 <= steps <= 64 or 2.0 * steps * math.log10(max(abs(a), 1.0)) > 13.0:
+        raise ValueError("unsupported_capability: steps must be 1 to 64 with |a|^(2 steps) at most "
+                         f"1e13, got {steps}")
+    return steps, a, b, c, float(eps)
+
+
+def _prepare(given, steps, coefficients, eps):
+    """Everything of a call that depends on sizes alone, checked."""
     if not all(isinstance(x, torch.Tensor) for x in given):
         raise ValueError("unsupported_capability: orthogonalize takes tensors")
     dtype, device = given[0].dtype, given[0].device
@@ -44,25 +63,32 @@ def orthogonalize(matrices, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     if torch.is_grad_enabled() and any(x.requires_grad for x in given):
         raise ValueError("unsupported_capability: orthogonalize has no derivative")
     _no_tangents(*given)
-    a, b, c = (float(v) for v in coefficients)
-    if isinstance(steps, bool) or not isinstance(steps, int):
-        raise ValueError("unsupported_capability: steps must be an integer")
+    rule = _rule(steps, coefficients, eps)
+    numbers = []  # st_matrix_batch: five 64-bit words each, addresses first
+    for x in given:
+        rows, cols = x.shape[-2:]
+        numbers += (0, 0, x.numel() // (rows * cols) if rows and cols else 0, rows, cols)
+    table = _lib.i64_array(numbers)
+    nbytes = _lib.query("st_orthogonalize_workspace_bytes", len(given), table)
+    if nbytes < 0:
+        _lib.check(_lib.ST_EUNSUPPORTED, "st_orthogonalize")
     if device.type != "cuda":
         raise ValueError("unsupported_capability: orthogonalize runs on the GPU")
+    return table, nbytes, rule, dtype, device
+
+
+def _run(plan, given):
+    """The call on tensors of the sizes, type and device that ``plan`` was made for."""
+    table, nbytes, rule, dtype, device = plan
     given = [x.contiguous() for x in given]
     out = [torch.empty_like(x) for x in given]
-    numbers = []  # st_matrix_batch: five 64-bit words each
-    for x, y in zip(given, out):
-        rows, cols = x.shape[-2:]
-        numbers += (x.data_ptr(), y.data_ptr(), x.numel() // (rows * cols) if rows and cols else 0,
-                    rows, cols)
-    table = _lib.i64_array(numbers)
+    for i, (x, y) in enumerate(zip(given, out)):
+        table[5 * i], table[5 * i + 1] = x.data_ptr(), y.data_ptr()
     with _lib.on_device(device):
-        nbytes = _lib.query("st_orthogonalize_workspace_bytes", len(given), table)
         ws = _scratch(device, nbytes)
-        _lib.call("st_orthogonalize", len(given), table, _DTYPES[dtype], steps, a, b, c, float(eps),
-                  _lib.ptr(ws), nbytes, _lib.stream_handle(device))
-    return out[0] if single else out
+        _lib.call("st_orthogonalize", len(given), table, _DTYPES[dtype], *rule, _lib.ptr(ws), nbytes,
+                  _lib.stream_handle(device))
+    return out
 
 
 def _factors(proj):
@@ -97,6 +123,7 @@ class Muon:
         if not (math.isfinite(lr) and 0.0 <= momentum < 1.0 and weight_decay >= 0.0):
             raise ValueError("unsupported_capability: lr must be finite, momentum in [0, 1), "
                              "weight_decay not negative")
+        _rule(steps, coefficients)
         self.lr, self.momentum, self.nesterov = lr, momentum, nesterov
         self.weight_decay, self.steps, self.coefficients = weight_decay, steps, tuple(coefficients)
         self.match_rms, self.table = match_rms, table
@@ -114,22 +141,24 @@ class Muon:
 
     def step(self, projections):
         tables = {k: p for k, p in projections.items() if not hasattr(p, "A")}
-        if tables:
-            if self.table is None:
-                raise ValueError(f"unsupported_capability: no optimizer for {sorted(tables)}")
-            self.table.step(tables)
+        if tables and self.table is None:
+            raise ValueError(f"unsupported_capability: no optimizer for {sorted(tables)}")
         with torch.no_grad():
             factors = [f for k, p in projections.items() if k not in tables for f in _factors(p)]
             if factors:
                 params, grads, moments = (list(t) for t in zip(*factors))
+                # what the update refuses, it refuses before a momentum has moved
+                plan = _prepare(moments, self.steps, self.coefficients, 1e-7)
                 torch._foreach_lerp_(moments, grads, 1.0 - self.momentum)
                 updates = torch._foreach_lerp(grads, moments, self.momentum) if self.nesterov \
                     else moments
-                updates = orthogonalize(updates, steps=self.steps, coefficients=self.coefficients)
+                updates = _run(plan, updates)
                 torch._foreach_mul_(updates, [-self.lr * self._scale(u.shape) for u in updates])
                 if self.weight_decay:
                     torch._foreach_mul_(params, 1.0 - self.lr * self.weight_decay)
                 torch._foreach_add_(params, updates)
+        if tables:
+            self.table.step(tables)
         self.step_count += 1
 
 
