@@ -18,7 +18,8 @@ class TokenEmbedding:
     """``weight`` (fp32 [V, H], a copy on ``device``), its gradient buffer ``grad`` and
     the AdamW moments ``m`` and ``v``.  ``scale`` multiplies the rows that are looked
     up, as some models scale theirs by the root of the hidden size; tokens equal to
-    ``padding_idx`` are looked up and not trained.  A head that was tied to the table
+    ``padding_idx`` are looked up and not trained, nor does a weight decay reach their
+    row.  A head that was tied to the table
     is a tensor of its own and stays frozen."""
 
     name = "embedding"

@@ -257,7 +257,11 @@ class AdamW:
             for p in projections.values():
                 for param, grad, m, v in _tensors(p):
                     if self.weight_decay != 0.0:
+                        row = getattr(p, "padding_idx", None)  # of a table: not trained
+                        kept = None if row is None else param[row].clone()
                         param.mul_(1.0 - self.lr * self.weight_decay)
+                        if kept is not None:
+                            param[row] = kept
                     m.lerp_(grad, 1.0 - self.beta1)
                     v.mul_(self.beta2).addcmul_(grad, grad, value=1.0 - self.beta2)
                     denom = (v.sqrt() / bc2_sqrt).add_(self.eps)
