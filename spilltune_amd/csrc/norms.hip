@@ -625,7 +625,8 @@ extern "C" int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual
   if (rows == 0) return ST_OK;
   const bool columns = dgate && gate_mode == GATE_COLUMNS, sums = dpost || dpre || columns;
   if (sums) {
-    // gate rows only bound the runs where their sums are asked for
+    // no run crosses a gate row, so that the kernel finds one gate row a run where their
+    // sums are asked for (with a frozen gate the same runs)
     if (!columns) a.rows_per = gate_mode == GATE_COLUMNS ? rows_per : rows;
     plan_runs(rows, a.rows_per, hidden, a.runs, a.per_run);
     const int64_t need = a.runs * 3 * hidden * 4;
@@ -634,8 +635,10 @@ extern "C" int st_residual_norms_bwd(const uint16_t* y, const uint16_t* residual
                       (long long)need);
     ST_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
     const int64_t groups = rows / a.rows_per;
-    if (a.runs >= (int64_t)1 << 22 || groups + 2 >= 65536)
+    if (columns && groups + 2 >= 65536)
       return st::fail(ST_EUNSUPPORTED, "st_residual_norms_bwd: 65534 gate rows and more");
+    if (a.runs >= (int64_t)1 << 22)
+      return st::fail(ST_EUNSUPPORTED, "st_residual_norms_bwd: 2^22 frozen gate rows and more");
     a.partial = (float*)workspace;
     dispatch(a, true, true, (hipStream_t)stream);
     norms_join<<<dim3((unsigned)st::cdiv(hidden, 64), (unsigned)(columns ? groups + 2 : 2)), 1024, 0,
