@@ -8,6 +8,7 @@ whose optimizer is AdamW, finetune/optimizer.py:227-342).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -68,7 +69,7 @@ def _prepare(given, steps, coefficients, eps):
     for x in given:
         rows, cols = x.shape[-2:]
         numbers += (0, 0, x.numel() // (rows * cols) if rows and cols else 0, rows, cols)
-    table = _lib.i64_array(numbers)
+    table = (ctypes.c_int64 * len(numbers))(*numbers)
     nbytes = _lib.query("st_orthogonalize_workspace_bytes", len(given), table)
     if nbytes < 0:
         _lib.check(_lib.ST_EUNSUPPORTED, "st_orthogonalize")
@@ -82,8 +83,10 @@ def _run(plan, given):
     table, nbytes, rule, dtype, device = plan
     given = [x.contiguous() for x in given]
     out = [torch.empty_like(x) for x in given]
-    for i, (x, y) in enumerate(zip(given, out)):
-        table[5 * i], table[5 * i + 1] = x.data_ptr(), y.data_ptr()
+    at = 0
+    for x, y in zip(given, out):
+        table[at:at + 2] = x.data_ptr(), y.data_ptr()
+        at += 5
     with _lib.on_device(device):
         ws = _scratch(device, nbytes)
         _lib.call("st_orthogonalize", len(given), table, _DTYPES[dtype], *rule, _lib.ptr(ws), nbytes,
