@@ -9,10 +9,12 @@
 //
 // A wave holds a token's logits (up to 512 experts, PER = 1, 2, 4 or 8 a lane), so each
 // is read once forward and once backward, the next token's while the present one's are
-// worked on (16384 tokens of 256 experts: 17 MB in 12.5 us forward, 12.2 us backward);
-// picks are counted in LDS (whole numbers: their order does not matter), probabilities
-// summed in fp32 in registers over a workgroup's tokens and joined over the workgroups
-// in their order.
+// worked on; picks are counted in LDS (whole numbers: their order does not matter),
+// probabilities summed in fp32 in registers over a workgroup's tokens and joined over the
+// workgroups in their order.  16384 tokens of 256 experts (17 MB): the sums 13 us, the join
+// 8 in four rows and 19 as one group (one workgroup a group), the mean over rows 1.5,
+// backward 12.  The sums' waves have one token ahead and are eight a CU: 2 MB in flight in
+// all, which a round trip to memory of about 1.5 us makes the 1.3 TB/s measured.
 #include "common.h"
 
 namespace {

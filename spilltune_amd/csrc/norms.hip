@@ -74,7 +74,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // chunk is moved back to end with it: its first `skip` elements are the chunk's before,
 // worked out and stored by both alike, and counted in no sum here.  Elements past the row
 // (`in` false) read its first ones and are cleared: a load under a branch would be waited
-// for at the branch's end.  (4096 rows of 4097: 45 us forward, 82 backward; one element a
+// for at the branch's end.  (4096 rows of 4097: 47 us forward, 87 backward; one element a
 // load took 640 and 1245.)
 struct Place {
   int64_t i;
@@ -262,11 +262,11 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
 // GATE: there is one.  Rows wait in registers as the bf16 they are (in fp32, fewer waves
 // fit).  The columns' sums of rows over more than one wave lie in LDS, each read and
 // written by its own thread alone: in registers they left a CU 8 to 12 waves in the place
-// of 16 (8192 x 4096 with learnt norms and gate 140 us, so 99; 2103 x 7168 66, 54).  Rows
-// of one wave keep them, and the next row is under way (30000 x 512: 42, in LDS 55).
+// of 16 (8192 x 4096 with learnt norms and gate 140 us, so 105; 2103 x 7168 takes 59).  Rows
+// of one wave keep them, and the next row is under way (30000 x 512: 39, in LDS 55).
 // Beyond 8192 columns (WIDE) a thread has no registers for its row either: it reads its
-// chunks again where it needs them, out of the caches (2048 x 16384: 170 us, with all of
-// it in registers 470).
+// chunks again where it needs them, out of the caches (2048 x 16384: a training pass 165
+// us, with all of it in registers 470).
 template <int VEC, int NT, int NV, bool SUMS, bool GATE, bool RAG>
 __global__ __launch_bounds__(NT, SUMS && NT > 64 && NV == 1 ? 4 : 1) void norms_bwd(Args a) {
   __shared__ float red[3][NT / 64];
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(1024) void norms_join(const float* __restrict__ par
 // ---------------------------------------------------------------- host
 // Runs of rows in a backward that sums over rows, never across gate rows: as many as
 // workgroups run at once, so that none waits for a second turn and no CU idles (30000
-// rows of 512: two runs a CU 140 us, twelve 42).  A CU holds 12 waves that keep their sums in
+// rows of 512: two runs a CU 140 us, twelve 39).  A CU holds 12 waves that keep their sums in
 // registers, or 16, or one workgroup beyond 4096 columns.  Runs of at least two rows where
 // there are as many: each costs as much as a row again in partial sums.
 void plan_runs(int64_t rows, int64_t rows_per, int64_t H, int64_t& runs, int64_t& per_run) {
@@ -525,9 +525,10 @@ void go(const Args& a, bool bwd, bool sums, hipStream_t s) {
 }
 
 // A row in one wave where it fits (no barriers), in two to sixteen waves otherwise, in
-// chunks of eight elements.  The forward and the sums over rows do better with sixteen
-// elements a thread (fewer waves at a barrier; 8192 rows of 4096 forward 47 us against
-// 52), the plain backward with eight (84 against 95).
+// chunks of eight elements.  From 2049 columns on the forward does better with sixteen
+// elements a thread (fewer waves at a barrier; 8192 rows of 4096 47 us against 52), the
+// backward with eight (84 against 95).  Rows of fewer than 512 columns leave lanes idle:
+// 100000 of 64 take 45 us forward and 59 backward, of 128 46 and 60.
 template <bool RAG>
 void by_size(const Args& a, bool bwd, bool sums, hipStream_t s) {
   const int64_t H = a.H;

@@ -529,6 +529,7 @@ class _MoEFeedForward(torch.autograd.Function):
         _lib.call("st_moe_route_softmax_bwd", _lib.ptr(logits), _lib.ptr(indices), _lib.ptr(dw),
                   T, E, top_k, int(norm), _lib.ptr(dlogits), st)
         if given is not None:
+            # bf16 logits have bf16 gradients: the sum of two is rounded as autograd's is
             dlogits.add_(given)
         Ec = E
         if E % 8:  # the GEMM contracts 16-byte chunks: zero-pad the expert dimension
