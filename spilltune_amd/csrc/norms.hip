@@ -236,7 +236,7 @@ __global__ __launch_bounds__(NT) void norms_fwd(Args a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float z = a.post ? y[n][e] * r1 * w[e] : y[n][e];
-        h[n][e] += g[e] * z;
+        h[n][e] = __builtin_fmaf(g[e], z, h[n][e]);  // as the backward forms it again
         ss += e < c.skip ? 0.0f : h[n][e] * h[n][e];
       }
       if (c.in) store_bf16<VEC, RAG>(a.h + base, c, h[n]);
