@@ -234,7 +234,10 @@ def balance_loss(logits, indices, *, score="softmax", valid=None, per_row=False)
 
 
 def _capturing(t) -> bool:
-    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+    if not t.is_cuda:
+        return False
+    with _lib.on_device(t.device):
+        return torch.cuda.is_current_stream_capturing()
 
 
 class ExpertBalance:

@@ -42,6 +42,7 @@ def orthogonalize(matrices, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 def _rule(steps, coefficients, eps=1e-7):
     """``(steps, a, b, c, eps)``, checked."""
     a, b, c = (float(v) for v in coefficients)
+    eps = float(eps)
     if isinstance(steps, bool) or not isinstance(steps, int):
         raise ValueError("unsupported_capability: steps must be an integer")
     if not (math.isfinite(a) and math.isfinite(b) and math.isfinite(c) and 0.0 <= eps < math.inf):
@@ -49,7 +50,7 @@ def _rule(steps, coefficients, eps=1e-7):
     if not 1 <= steps <= 64 or 2.0 * steps * math.log10(max(abs(a), 1.0)) > 13.0:
         raise ValueError("unsupported_capability: steps must be 1 to 64 with |a|^(2 steps) at most "
                          f"1e13, got {steps}")
-    return steps, a, b, c, float(eps)
+    return steps, a, b, c, eps
 
 
 def _prepare(given, steps, coefficients, eps):
@@ -126,9 +127,9 @@ class Muon:
         if not (math.isfinite(lr) and 0.0 <= momentum < 1.0 and weight_decay >= 0.0):
             raise ValueError("unsupported_capability: lr must be finite, momentum in [0, 1), "
                              "weight_decay not negative")
-        _rule(steps, coefficients)
         self.lr, self.momentum, self.nesterov = lr, momentum, nesterov
         self.weight_decay, self.steps, self.coefficients = weight_decay, steps, tuple(coefficients)
+        _rule(self.steps, self.coefficients)
         self.match_rms, self.table = match_rms, table
         self.step_count = 0
 

@@ -50,6 +50,7 @@ def test_many_small_matrices_are_taken(sizes):
 def test_the_optimizer_refuses_its_rule_at_once(kw, match):
     with pytest.raises(ValueError, match=match):
         muon.Muon(**kw)
+    assert muon.Muon(coefficients=iter((1, 0.5, 0))).coefficients == (1, 0.5, 0)
 
 
 def _projection(rank, inner, outer):
